@@ -214,6 +214,103 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
                  int Bt, int T, int D, int N, int K, void *stream);
 
 /*
+ * Losses of a language model's head, without keeping the logits.
+ *
+ * x (rows, dim) with row stride ldx, w (vocab, dim) with row stride ldw, both
+ * of one storage type; z = x w^T never exists as a whole: the forward reduces
+ * it tile by tile to one log-sum-exp a row, the backward recomputes it in
+ * pieces of the vocabulary.
+ *
+ * Cross entropy, target (rows) int64:
+ *     loss[m] = log sum_v exp z[m,v] - z[m, target[m]]
+ * Distillation from a teacher's top k, index (rows, k) int64 and its logits
+ * (rows, k) float32, over the entries with index >= 0:
+ *     p = softmax(logits / temperature),  q = softmax(z / temperature)
+ *     loss[m] = temperature^2 sum_j p_j (log p_j - log q[index_j])
+ * An index may occur twice in a row (its probabilities add up).
+ *
+ * A row whose target is ignore_index, or that has no entry with index >= 0
+ * (or only logits of -inf), is left out: loss 0, gradient 0, whatever x holds
+ * there, and it does not count in the mean. An index >= vocab, or a target
+ * outside [0, vocab) that is not ignore_index, makes the row's loss NaN and,
+ * in the backward, its gradients (nothing is read out of bounds).
+ *
+ * reduction: MMS_REDUCE_NONE (loss, dloss: rows floats), MMS_REDUCE_MEAN (over
+ * the rows that count; NaN if there is none) or MMS_REDUCE_SUM (one float).
+ * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, lse, picked, prob, count
+ * are float32, sums are float32. fp32 products run on the tensor cores as
+ * three bf16 parts a factor, with every partial product above 2^-24.
+ *
+ * The forward writes what the backward needs: lse2 (rows), the log-sum-exp of
+ * z / temperature in units of log 2; picked (rows, k; k = 1 for the cross
+ * entropy), z / temperature at the indices in the same units; prob (rows, k)
+ * = p; count (1) = the rows that count. dx (rows, dim) and dw (vocab, dim)
+ * are contiguous; either may be NULL and is then not computed.
+ *
+ * x, w, dx, dw need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.
+ * The workspace (256-byte aligned) has mms_head_workspace_size() bytes.
+ * No counterpart in the reference, which computes the logits and calls
+ * PyTorch's cross entropy (mamba_metal/model.py:293-297).
+ */
+#define MMS_F32 0
+#define MMS_BF16 1
+#define MMS_REDUCE_NONE 0
+#define MMS_REDUCE_MEAN 1
+#define MMS_REDUCE_SUM 2
+#define MMS_HEAD_MAX_K 1024
+size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long long ldx,
+                               long long ldw, int backward);
+int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *target, int64_t ignore_index, int reduction, float *loss,
+                      float *lse2, float *picked, float *count, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
+                      void *stream);
+int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *target, int64_t ignore_index, int reduction,
+                      const float *dloss, const float *lse2, const float *picked,
+                      const float *count, void *dx, void *dw, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
+                      void *stream);
+int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *index, const float *logits, int k, float temperature,
+                      int reduction, float *loss, float *lse2, float *picked, float *prob,
+                      float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
+                      int dim, int dtype, void *stream);
+int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *index, int k, float temperature, int reduction,
+                      const float *dloss, const float *lse2, const float *picked,
+                      const float *prob, const float *count, void *dx, void *dw, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
+                      void *stream);
+
+/*
+ * Residual sum after a block and norm before the next one, one kernel each way:
+ *     a = y * silu(gate)                  (gate NULL: a = y)
+ *     b = post * a / rms(a)               (post NULL: b = a)
+ *     h = x + scale * b                   (scale NULL: h = x + b)
+ *     u = weight * h / rms(h)             rms(v) = sqrt(mean(v^2) + eps)
+ * x, y, h, u (rows, dim) contiguous, gate (rows, dim) with row stride ldg >=
+ * dim, weight, post, scale (dim), all of storage type dtype; u comes from h
+ * before its rounding. The forward also writes stat (rows, 2) float32: 1/rms(a)
+ * (0 without post) and 1/rms(h). The backward gives the gradients of every
+ * input from dh and du; dgate (rows, dim) is contiguous; dweight, dpost,
+ * dscale are sums over the rows in a fixed order, through a workspace of
+ * mms_norm_workspace_size() bytes (256-byte aligned). dy may be dx's pointer
+ * where gate, post and scale are NULL (their values are the same).
+ * Arrays need their element's alignment.
+ * No counterpart in the reference (PyTorch ops there, mamba_metal/model.py:85-95).
+ */
+size_t mms_norm_workspace_size(int rows, int dim);
+int mms_norm_fwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
+                 const void *post, const void *scale, float eps, void *h, void *u, float *stat,
+                 int rows, int dim, int dtype, void *stream);
+int mms_norm_bwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
+                 const void *post, const void *scale, const float *stat, const void *dh,
+                 const void *du, void *dx, void *dy, void *dgate, void *dweight, void *dpost,
+                 void *dscale, void *workspace, size_t workspace_bytes, int rows, int dim,
+                 int dtype, void *stream);
+
+/*
  * Device-side status of the kernels launched so far, for failure detection.
  * The backward's TMA staging waits on completion barriers with a bounded
  * poll; a wait that runs out records a flag instead of hanging the GPU (the

@@ -9,6 +9,7 @@
 
 #include <atomic>
 
+#include "mms_head.h"
 #include "mms_kernels.h"
 #include "mms_scan.h"
 
@@ -88,6 +89,67 @@ bool proj_ok(float dt_min, float dt_max)
            dt_max > dt_min;
 }
 
+// Sizes, types and pointers of the head's losses; the workspace's size comes last.
+int check_head(const void *x, long long ldx, const void *w, long long ldw, int rows, int vocab,
+               int dim, int k, float tau, int dtype, int reduction)
+{
+    if (rows < 1 || vocab < 1 || dim < 1 || rows > (1 << 24) || k < 1 || k > MMS_HEAD_MAX_K ||
+        ldx < dim || ldw < dim || (dtype != MMS_F32 && dtype != MMS_BF16) ||
+        reduction < MMS_REDUCE_NONE || reduction > MMS_REDUCE_SUM || !(tau > 0.f) || tau > 3.0e38f ||
+        !x || !w)
+        return MMS_ERR_INVALID_ARG;
+    return aligned(x, 16) && aligned(w, 16) ? MMS_OK : MMS_ERR_MISALIGNED;
+}
+
+mms::HeadArgs head_args(const void *x, long long ldx, const void *w, long long ldw,
+                        const int64_t *index, int k, int reduction, void *workspace, int rows,
+                        int vocab, int dim, int dtype)
+{
+    mms::HeadArgs a{};
+    a.x = x; a.w = w; a.ldx = ldx; a.ldw = ldw;
+    a.rows = rows; a.vocab = vocab; a.dim = dim; a.bf16 = dtype == MMS_BF16;
+    a.index = index; a.k = k; a.tau = 1.f; a.reduction = reduction; a.workspace = workspace;
+    return a;
+}
+
+int head_fwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
+{
+    if (!a.index || !a.loss || !a.lse2 || !a.picked || !a.count) return MMS_ERR_INVALID_ARG;
+    if (!aligned(a.index, 8) || !aligned(a.logits, 4) || !aligned(a.loss, 4) ||
+        !aligned(a.lse2, 4) || !aligned(a.picked, 4) || !aligned(a.prob, 4) || !aligned(a.count, 4))
+        return MMS_ERR_MISALIGNED;
+    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
+                                                                    a.ldx, a.ldw, false))
+        return MMS_ERR_WORKSPACE;
+    if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
+    return status_of(mms::launch_head_fwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int head_bwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
+{
+    if (!a.index || !a.dloss || !a.c_lse2 || !a.c_picked || !a.c_count) return MMS_ERR_INVALID_ARG;
+    if (!aligned(a.index, 8) || !aligned(a.dloss, 4) || !aligned(a.c_lse2, 4) ||
+        !aligned(a.c_picked, 4) || !aligned(a.c_prob, 4) || !aligned(a.c_count, 4) ||
+        !aligned(a.dx, 16) || !aligned(a.dw, 16))
+        return MMS_ERR_MISALIGNED;
+    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
+                                                                    a.ldx, a.ldw, true))
+        return MMS_ERR_WORKSPACE;
+    if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
+    return status_of(mms::launch_head_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int check_norm(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
+               const void *post, const void *scale, int rows, int dim, int dtype)
+{
+    if (rows < 1 || dim < 1 || (gate && ldg < dim) || (dtype != MMS_F32 && dtype != MMS_BF16) ||
+        !x || !y || !weight)
+        return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    return aligned(x, e) && aligned(y, e) && aligned(gate, e) && aligned(weight, e) &&
+           aligned(post, e) && aligned(scale, e) ? MMS_OK : MMS_ERR_MISALIGNED;
+}
+
 std::atomic<uint32_t> g_wait_limit{0};
 std::atomic<int> g_skip_item{-1};
 
@@ -112,7 +174,7 @@ const char *mms_status_string(int status)
     case MMS_OK: return "ok";
     case MMS_ERR_INVALID_ARG: return "invalid argument (size out of range or NULL pointer)";
     case MMS_ERR_UNSUPPORTED_N: return "unsupported d_state: N must be a multiple of 4 in [4, 64]";
-    case MMS_ERR_WORKSPACE: return "workspace missing or smaller than mms_bwd_workspace_size()";
+    case MMS_ERR_WORKSPACE: return "workspace missing or smaller than the entry point's size function says";
     case MMS_ERR_MISALIGNED: return "misaligned pointer (B, C, Aneg, ckpt, dB, dC, dAneg need 16 bytes)";
     case MMS_ERR_CUDA: return "CUDA call failed (mms_last_cuda_error() names the CUDA error)";
     case MMS_ERR_TIMEOUT: return "a kernel timed out waiting for its staged copies (results invalid)";
@@ -250,6 +312,122 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg, const
     mms::BwdArgs a{fp(x), fp(dt), aneg, B, C, fp(dy), ckpt, fp(dx), fp(ddt), daneg, dB, dC,
                    workspace, Bt, T, D, N, K, mms::Proj{0, 0.f, 0.f, 0.f}, 1};
     return status_of(mms::launch_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long long ldx,
+                               long long ldw, int backward)
+{
+    if (rows < 1 || vocab < 1 || dim < 1 || rows > (1 << 24) || ldx < dim || ldw < dim ||
+        (dtype != MMS_F32 && dtype != MMS_BF16))
+        return 0;
+    return mms::head_workspace_bytes(rows, vocab, dim, dtype == MMS_BF16, ldx, ldw, backward != 0);
+}
+
+int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *target, int64_t ignore_index, int reduction, float *loss,
+                      float *lse2, float *picked, float *count, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
+{
+    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, 1, 1.f, dtype, reduction);
+    if (rc) return rc;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
+    a.ignore_index = ignore_index;
+    a.loss = loss; a.lse2 = lse2; a.picked = picked; a.count = count;
+    return head_fwd(a, workspace_bytes, stream);
+}
+
+int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *target, int64_t ignore_index, int reduction,
+                      const float *dloss, const float *lse2, const float *picked,
+                      const float *count, void *dx, void *dw, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
+{
+    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, 1, 1.f, dtype, reduction);
+    if (rc) return rc;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
+    a.ignore_index = ignore_index;
+    a.dloss = dloss; a.c_lse2 = lse2; a.c_picked = picked; a.c_count = count;
+    a.dx = dx; a.dw = dw;
+    return head_bwd(a, workspace_bytes, stream);
+}
+
+int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *index, const float *logits, int k, float temperature,
+                      int reduction, float *loss, float *lse2, float *picked, float *prob,
+                      float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
+                      int dim, int dtype, void *stream)
+{
+    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, k, temperature, dtype, reduction);
+    if (rc) return rc;
+    if (!logits || !prob) return MMS_ERR_INVALID_ARG;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
+    a.kd = true; a.tau = temperature; a.logits = logits;
+    a.loss = loss; a.lse2 = lse2; a.picked = picked; a.prob = prob; a.count = count;
+    return head_fwd(a, workspace_bytes, stream);
+}
+
+int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *index, int k, float temperature, int reduction,
+                      const float *dloss, const float *lse2, const float *picked,
+                      const float *prob, const float *count, void *dx, void *dw, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
+{
+    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, k, temperature, dtype, reduction);
+    if (rc) return rc;
+    if (!prob) return MMS_ERR_INVALID_ARG;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
+    a.kd = true; a.tau = temperature;
+    a.dloss = dloss; a.c_lse2 = lse2; a.c_picked = picked; a.c_prob = prob; a.c_count = count;
+    a.dx = dx; a.dw = dw;
+    return head_bwd(a, workspace_bytes, stream);
+}
+
+size_t mms_norm_workspace_size(int rows, int dim)
+{
+    return rows < 1 || dim < 1 ? 0 : mms::norm_workspace_bytes(rows, dim);
+}
+
+int mms_norm_fwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
+                 const void *post, const void *scale, float eps, void *h, void *u, float *stat,
+                 int rows, int dim, int dtype, void *stream)
+{
+    const int rc = check_norm(x, y, gate, ldg, weight, post, scale, rows, dim, dtype);
+    if (rc) return rc;
+    if (!h || !u || !stat || !(eps >= 0.f)) return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    if (!aligned(h, e) || !aligned(u, e) || !aligned(stat, 4)) return MMS_ERR_MISALIGNED;
+    mms::NormArgs a{};
+    a.x = x; a.y = y; a.gate = gate; a.ldg = ldg; a.weight = weight; a.post = post; a.scale = scale;
+    a.eps = eps; a.h = h; a.u = u; a.stat = stat;
+    a.rows = rows; a.dim = dim; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_norm_fwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int mms_norm_bwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
+                 const void *post, const void *scale, const float *stat, const void *dh,
+                 const void *du, void *dx, void *dy, void *dgate, void *dweight, void *dpost,
+                 void *dscale, void *workspace, size_t workspace_bytes, int rows, int dim,
+                 int dtype, void *stream)
+{
+    const int rc = check_norm(x, y, gate, ldg, weight, post, scale, rows, dim, dtype);
+    if (rc) return rc;
+    if (!stat || !dh || !du || !dx || !dy || !dweight || (gate && !dgate) || (post && !dpost) ||
+        (scale && !dscale) || (dx == dy && (gate || post || scale)))
+        return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    if (!aligned(stat, 4) || !aligned(dh, e) || !aligned(du, e) || !aligned(dx, e) ||
+        !aligned(dy, e) || !aligned(dgate, e) || !aligned(dweight, e) || !aligned(dpost, e) ||
+        !aligned(dscale, e))
+        return MMS_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < mms::norm_workspace_bytes(rows, dim)) return MMS_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return MMS_ERR_MISALIGNED;
+    mms::NormArgs a{};
+    a.x = x; a.y = y; a.gate = gate; a.ldg = ldg; a.weight = weight; a.post = post; a.scale = scale;
+    a.c_stat = stat; a.dh = dh; a.du = du; a.dx = dx; a.dy = dy; a.dgate = dgate;
+    a.dweight = dweight; a.dpost = post ? dpost : nullptr; a.dscale = scale ? dscale : nullptr;
+    a.workspace = workspace;
+    a.rows = rows; a.dim = dim; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_norm_bwd(a, static_cast<cudaStream_t>(stream)));
 }
 
 int mms_device_status(void)

@@ -28,6 +28,9 @@ MMS_ERR_UNSUPPORTED_BF16 = 8
 # Every symbol include/mms_scan.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+_Z = ctypes.c_size_t
+_F = ctypes.c_float
 SIGNATURES = {
     "mms_abi_version": ([], _I),
     "mms_status_string": ([_I], ctypes.c_char_p),
@@ -47,6 +50,15 @@ SIGNATURES = {
                      + [_P], _I),
     "mms_fwd_bf16": ([_P] * 7 + [_I] * 5 + [_P], _I),
     "mms_bwd_bf16": ([_P] * 13 + [ctypes.c_size_t] + [_I] * 5 + [_P], _I),
+    "mms_head_workspace_size": ([_I] * 4 + [_L] * 2 + [_I], _Z),
+    "mms_linear_ce_fwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 5 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_linear_ce_bwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 7 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_linear_kd_fwd": ([_P, _L, _P, _L, _P, _P, _I, _F, _I] + [_P] * 6 + [_Z] + [_I] * 4
+                          + [_P], _I),
+    "mms_linear_kd_bwd": ([_P, _L, _P, _L, _P, _I, _F, _I] + [_P] * 8 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_norm_workspace_size": ([_I] * 2, _Z),
+    "mms_norm_fwd": ([_P] * 3 + [_L] + [_P] * 3 + [_F] + [_P] * 3 + [_I] * 3 + [_P], _I),
+    "mms_norm_bwd": ([_P] * 3 + [_L] + [_P] * 13 + [_Z] + [_I] * 3 + [_P], _I),
     "mms_debug_set_wait": ([ctypes.c_uint, _I], _I),
     "mms_probe_pipe": ([_I] * 3 + [_P] * 4, _I),
     "mms_probe_ops_per_cta": ([_I] * 2, ctypes.c_longlong),
@@ -234,6 +246,120 @@ def gate_bwd(dout, y, z, d_skip):
                           _ptr(dz), _ptr(dd), _ptr(ws), nb, bt, t_len, d, _stream(y.device))
     _check(rc, "mms_gate_bwd")
     return dy, dz, dd
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _dtype(t) -> int:
+    return 1 if t.dtype == torch.bfloat16 else 0
+
+
+def _head_workspace(x, w, backward: bool):
+    nb = int(load().mms_head_workspace_size(x.shape[0], w.shape[0], x.shape[1], _dtype(x),
+                                            x.stride(0), w.stride(0), int(backward)))
+    return torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
+
+
+def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
+    """(loss, lse2, picked, count) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides."""
+    m, d = x.shape
+    red = REDUCTIONS[reduction]
+    loss = torch.empty((m,) if red == 0 else (), device=x.device)
+    lse2, picked, count = (torch.empty(n, device=x.device) for n in (m, m, 1))
+    ws = _head_workspace(x, w, False)
+    rc = load().mms_linear_ce_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
+                                  ignore_index, red, _ptr(loss), _ptr(lse2), _ptr(picked),
+                                  _ptr(count), _ptr(ws), ws.numel(), m, w.shape[0], d, _dtype(x),
+                                  _stream(x.device))
+    _check(rc, "mms_linear_ce_fwd")
+    return loss, lse2, picked, count
+
+
+def _head_grads(x, w, need_x: bool, need_w: bool):
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+    dw = torch.empty(w.shape, device=w.device, dtype=w.dtype) if need_w else None
+    return dx, dw, 0 if dx is None else _ptr(dx), 0 if dw is None else _ptr(dw)
+
+
+def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, lse2, picked, count,
+                  need_x: bool = True, need_w: bool = True):
+    """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
+    dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
+    ws = _head_workspace(x, w, True)
+    rc = load().mms_linear_ce_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
+                                  ignore_index, REDUCTIONS[reduction], _ptr(dloss), _ptr(lse2),
+                                  _ptr(picked), _ptr(count), pdx, pdw, _ptr(ws), ws.numel(),
+                                  x.shape[0], w.shape[0], x.shape[1], _dtype(x), _stream(x.device))
+    _check(rc, "mms_linear_ce_bwd")
+    return dx, dw
+
+
+def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
+    """(loss, lse2, picked, prob, count) of mms_linear_kd_fwd."""
+    m, d = x.shape
+    k = index.shape[1]
+    red = REDUCTIONS[reduction]
+    loss = torch.empty((m,) if red == 0 else (), device=x.device)
+    lse2, count = torch.empty(m, device=x.device), torch.empty(1, device=x.device)
+    picked, prob = torch.empty(m, k, device=x.device), torch.empty(m, k, device=x.device)
+    ws = _head_workspace(x, w, False)
+    rc = load().mms_linear_kd_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
+                                  _ptr(logits), k, temperature, red, _ptr(loss), _ptr(lse2),
+                                  _ptr(picked), _ptr(prob), _ptr(count), _ptr(ws), ws.numel(), m,
+                                  w.shape[0], d, _dtype(x), _stream(x.device))
+    _check(rc, "mms_linear_kd_fwd")
+    return loss, lse2, picked, prob, count
+
+
+def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, lse2, picked, prob, count,
+                  need_x: bool = True, need_w: bool = True):
+    """(dx, dw) of mms_linear_kd_bwd; None for one that is not needed."""
+    dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
+    ws = _head_workspace(x, w, True)
+    rc = load().mms_linear_kd_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
+                                  index.shape[1], temperature, REDUCTIONS[reduction], _ptr(dloss),
+                                  _ptr(lse2), _ptr(picked), _ptr(prob), _ptr(count), pdx, pdw,
+                                  _ptr(ws), ws.numel(), x.shape[0], w.shape[0], x.shape[1],
+                                  _dtype(x), _stream(x.device))
+    _check(rc, "mms_linear_kd_bwd")
+    return dx, dw
+
+
+def _opt(t) -> int:
+    return 0 if t is None else _ptr(t)
+
+
+def norm_fwd(x, y, gate, weight, post, scale, eps: float):
+    """(h, u, stat) of mms_norm_fwd; x, y (M, D) contiguous, gate (M, D) with a row stride."""
+    m, d = x.shape
+    h, u = torch.empty_like(x), torch.empty_like(x)
+    stat = torch.empty(m, 2, device=x.device)
+    rc = load().mms_norm_fwd(_ptr(x), _ptr(y), _opt(gate), d if gate is None else gate.stride(0),
+                             _ptr(weight), _opt(post), _opt(scale), eps, _ptr(h), _ptr(u),
+                             _ptr(stat), m, d, _dtype(x), _stream(x.device))
+    _check(rc, "mms_norm_fwd")
+    return h, u, stat
+
+
+def norm_bwd(x, y, gate, weight, post, scale, stat, dh, du):
+    """(dx, dy, dgate, dweight, dpost, dscale) of mms_norm_bwd; None beside an input that is None."""
+    m, d = x.shape
+    dx = torch.empty_like(x)
+    # without gate, post and scale the gradients of x and y are the same values
+    dy = dx if gate is None and post is None and scale is None else torch.empty_like(x)
+    dgate = None if gate is None else torch.empty_like(x)
+    dweight = torch.empty_like(weight)
+    dpost, dscale = (None if t is None else torch.empty_like(t) for t in (post, scale))
+    lib = load()
+    nb = int(lib.mms_norm_workspace_size(m, d))
+    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
+    rc = lib.mms_norm_bwd(_ptr(x), _ptr(y), _opt(gate), d if gate is None else gate.stride(0),
+                          _ptr(weight), _opt(post), _opt(scale), _ptr(stat), _ptr(dh), _ptr(du),
+                          _ptr(dx), _ptr(dy), _opt(dgate), _ptr(dweight), _opt(dpost), _opt(dscale),
+                          _ptr(ws), nb, m, d, _dtype(x), _stream(x.device))
+    _check(rc, "mms_norm_bwd")
+    return dx, dy, dgate, dweight, dpost, dscale
 
 
 def pipe_rate(kind: str, device=None, iters: int = 4096, ctas_per_sm: int = 4) -> float:

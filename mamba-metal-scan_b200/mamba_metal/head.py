@@ -1,0 +1,222 @@
+"""Losses of a language model's head without its logits, on NVIDIA B200 (sm_100a).
+
+    linear_cross_entropy(x, weight, target)       softmax cross entropy of x W^T
+    linear_distillation(x, weight, index, logits) KL divergence from a teacher's top k
+
+x (..., D) are the model's last hidden states, weight (V, D) is the head. The
+(rows, V) logits never exist as a whole: the forward keeps one log-sum-exp a
+row, the backward computes the logits again in pieces of the vocabulary (see
+csrc/mms_head.cu). The reference model computes them and calls PyTorch's cross
+entropy (mamba_metal/model.py:293-297).
+
+Dispatch as in `mamba_metal.scan`: 'auto' runs the CUDA kernels on CUDA
+tensors and PyTorch ops elsewhere, 'cuda' / 'metal' force the kernels, 'torch'
+forces PyTorch ops. The kernels take float32 or bfloat16 (x and weight alike)
+and give a float32 loss; gradients have x's and weight's type.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from mamba_metal import _native
+from mamba_metal.scan import _IMPLS
+
+MAX_K = 1024          # entries a row of linear_distillation's teacher lists (MMS_HEAD_MAX_K)
+
+
+def _reduce(rows, counts, reduction: str):
+    if reduction == "none":
+        return rows
+    return rows.sum() / counts.sum() if reduction == "mean" else rows.sum()
+
+
+def linear_cross_entropy_ref(x, weight, target, ignore_index: int = -100, reduction: str = "mean"):
+    """linear_cross_entropy in PyTorch ops, with the logits (any device and float type)."""
+    logits = F.linear(x, weight).float() if x.dtype in (torch.bfloat16, torch.float16) \
+        else F.linear(x, weight)
+    loss = F.cross_entropy(logits.reshape(-1, weight.shape[0]), target.reshape(-1).long(),
+                           ignore_index=ignore_index, reduction=reduction)
+    return loss.reshape(target.shape) if reduction == "none" else loss
+
+
+def linear_distillation_ref(x, weight, teacher_index, teacher_logits, temperature: float = 1.0,
+                            reduction: str = "mean"):
+    """linear_distillation in PyTorch ops, with the logits (any device and float type)."""
+    logits = F.linear(x, weight)
+    if x.dtype in (torch.bfloat16, torch.float16):
+        logits = logits.float()
+    index = teacher_index.long()
+    valid = index >= 0
+    t = (teacher_logits.to(logits.dtype) / temperature).masked_fill(~valid, float("-inf"))
+    some = ~(t == float("-inf")).all(-1)
+    # a row without entries gets a finite stand-in, then probability 0 everywhere
+    log_p = torch.log_softmax(t.masked_fill(~some[..., None], 0.0), -1)
+    p = torch.where(some[..., None] & valid, log_p.exp(), torch.zeros_like(log_p))
+    log_q = torch.log_softmax(logits / temperature, -1).gather(-1, index.clamp(min=0))
+    terms = torch.where(p == 0, torch.zeros_like(p), p * (log_p - log_q))
+    rows = torch.where(some, temperature ** 2 * terms.sum(-1), torch.zeros_like(terms[..., 0]))
+    return _reduce(rows, some, reduction)
+
+
+# ------------------------------------------------------------------- the kernels
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """(rows, D) with unit column stride, a row stride >= D and a 16-byte aligned base: a view
+    of t where its layout allows, else a copy."""
+    d = t.shape[-1]
+    t = t.reshape(-1, d)
+    if t.shape[0] == 1 or d == 1 or t.stride(1) != 1 or t.stride(0) < d:
+        t = t.contiguous()
+        if t.stride() != (d, 1):                # sizes of one: strides are free, the kernels' are not
+            t = t.as_strided(t.shape, (d, 1))
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _check_head(what, x, weight, others, reduction):
+    tensors = (x, weight, *others)
+    if not all(t.is_cuda for t in tensors) or len({t.device for t in tensors}) != 1:
+        raise RuntimeError(f"{what} runs the CUDA kernels and needs every input on the same CUDA "
+                           "device; saw " + ", ".join(str(t.device) for t in tensors))
+    if x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
+        raise RuntimeError(f"{what} takes float32 or bfloat16, x and weight alike; got {x.dtype}, "
+                           f"{weight.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+        raise ValueError(f"bad shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    if others[0].is_floating_point() or others[0].dtype == torch.bool:
+        raise RuntimeError(f"{what} takes integer indices; got {others[0].dtype}")
+
+
+def _check_reduction(reduction):
+    if reduction not in _native.REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}; want 'mean', 'sum' or 'none'")
+
+
+def _no_rows(x, shape, reduction):
+    """The loss of no rows (0 / 0 for a mean), part of x's graph."""
+    if reduction == "none":
+        return x.float().sum(-1).reshape(shape)
+    s = x.float().sum()
+    return s / 0.0 if reduction == "mean" else s
+
+
+class LinearCrossEntropyCUDA(torch.autograd.Function):
+    """linear_cross_entropy on x (M, D), weight (V, D), target (M), forward and backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction):
+        with torch.cuda.device(x.device):
+            loss, lse2, picked, count = _native.linear_ce_fwd(x, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(x, weight, target, lse2, picked, count)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, weight, target, lse2, picked, count = ctx.saved_tensors
+        with torch.cuda.device(x.device):
+            dx, dw = _native.linear_ce_bwd(x, weight, target, ctx.ignore_index, ctx.reduction,
+                                           dloss.float().contiguous(), lse2, picked, count,
+                                           *ctx.needs_input_grad[:2])
+        return dx, dw, None, None, None
+
+
+class LinearDistillationCUDA(torch.autograd.Function):
+    """linear_distillation on x (M, D), weight (V, D), index and logits (M, k)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, index, logits, temperature, reduction):
+        with torch.cuda.device(x.device):
+            loss, lse2, picked, prob, count = _native.linear_kd_fwd(x, weight, index, logits,
+                                                                    temperature, reduction)
+        ctx.save_for_backward(x, weight, index, lse2, picked, prob, count)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, weight, index, lse2, picked, prob, count = ctx.saved_tensors
+        with torch.cuda.device(x.device):
+            dx, dw = _native.linear_kd_bwd(x, weight, index, ctx.temperature, ctx.reduction,
+                                           dloss.float().contiguous(), lse2, picked, prob, count,
+                                           *ctx.needs_input_grad[:2])
+        return dx, dw, None, None, None, None
+
+
+def _dispatch(impl: str, x) -> bool:
+    """Whether the kernels run."""
+    if impl not in _IMPLS:
+        raise ValueError(f"unknown scan_impl {impl!r}; want 'auto', 'cuda', 'metal' or 'torch'")
+    if impl in ("cuda", "metal") and not x.is_cuda:
+        raise RuntimeError(f"scan_impl={impl!r} needs CUDA tensors; got device {x.device.type!r}")
+    return impl != "torch" and x.is_cuda
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         ignore_index: int = -100, reduction: str = "mean", impl: str = "auto"):
+    """Softmax cross entropy of the logits x W^T, without keeping them.
+
+    x (..., D), weight (V, D), target (...) integers. Rows whose target is
+    ignore_index have loss and gradient 0, whatever x holds there, and do not
+    count in the mean (which is NaN if no row counts). A target outside
+    [0, V) that is not ignore_index gives a NaN loss and NaN gradients.
+    reduction 'mean', 'sum' or 'none' (target's shape); the loss is float32.
+    Differentiable once, with respect to x and weight.
+    """
+    _check_reduction(reduction)
+    if not _dispatch(impl, x):
+        return linear_cross_entropy_ref(x, weight, target, ignore_index, reduction)
+    _check_head("linear_cross_entropy", x, weight, (target,), reduction)
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target {tuple(target.shape)} does not match x {tuple(x.shape)}")
+    if target.numel() == 0:
+        return _no_rows(x, target.shape, reduction)
+    loss = LinearCrossEntropyCUDA.apply(_rows(x), _rows(weight), target.reshape(-1).long().contiguous(),
+                                        int(ignore_index), reduction)
+    return loss.reshape(target.shape) if reduction == "none" else loss
+
+
+def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor,
+                        teacher_logits: torch.Tensor, temperature: float = 1.0,
+                        reduction: str = "mean", impl: str = "auto"):
+    """KL divergence from a teacher's top k logits to softmax(x W^T / temperature).
+
+        p = softmax(teacher_logits / temperature) over the entries with index >= 0
+        loss = temperature^2 sum_j p_j (log p_j - log q[teacher_index_j])
+
+    with q over the whole vocabulary, without keeping the student's logits.
+    teacher_index (..., k) integers, teacher_logits (..., k) floats (used as
+    float32; not differentiated), k <= 1024. Entries with a negative index
+    are empty, whatever their logit; rows without an entry (or with only
+    logits of -inf) have loss and gradient 0 and do not count in the mean. An
+    index may occur twice; one >= V gives a NaN loss and NaN gradients.
+    Differentiable once, with respect to x and weight.
+    """
+    _check_reduction(reduction)
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite; got {temperature}")
+    if teacher_index.dim() < 1 or teacher_logits.shape != teacher_index.shape \
+            or teacher_index.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"bad shapes: x {tuple(x.shape)}, teacher_index {tuple(teacher_index.shape)}, "
+                         f"teacher_logits {tuple(teacher_logits.shape)}")
+    k = teacher_index.shape[-1]
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"linear_distillation takes 1 to {MAX_K} entries a row; got {k}")
+    if not _dispatch(impl, x):
+        return linear_distillation_ref(x, weight, teacher_index, teacher_logits.detach(),
+                                       temperature, reduction)
+    _check_head("linear_distillation", x, weight, (teacher_index, teacher_logits), reduction)
+    if not teacher_logits.is_floating_point():
+        raise RuntimeError(f"teacher_logits must be floating point; got {teacher_logits.dtype}")
+    lead = x.shape[:-1]
+    if teacher_index.numel() == 0:
+        return _no_rows(x, lead, reduction)
+    loss = LinearDistillationCUDA.apply(_rows(x), _rows(weight),
+                                        teacher_index.reshape(-1, k).long().contiguous(),
+                                        teacher_logits.detach().reshape(-1, k).float().contiguous(),
+                                        temperature, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss

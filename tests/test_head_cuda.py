@@ -1,0 +1,358 @@
+"""The head's losses on the GPU (mms_linear_ce_*, mms_linear_kd_*) against float64.
+
+Every case is compared element by element with the definition in float64 on the CPU, within
+bounds that _head_ref.py derives from the number of roundings. A second, norm-wise check is as
+sharp as independent roundings make it: bf16 gradients take two roundings (dz, the result), each
+at most 2^-8 relative, so 2^-7 of the norm holds when no sum cancels below its largest term;
+float32 gradients 2e-5 (sums of up to 4096 terms at 2^-24 each, all in one direction, are 2.4e-4;
+independent ones 4e-6).
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from _head_ref import check, check_norm, solve, sparse, u
+from mamba_metal import (_native, linear_cross_entropy, linear_cross_entropy_ref,
+                         linear_distillation, linear_distillation_ref, residual_rms_norm)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def head_inputs(rows, vocab, dim, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    w = torch.randn(vocab, dim, generator=gen) * (2.0 / math.sqrt(dim))
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    x = torch.randn(rows, dim, generator=gen) + 3 * torch.rand(rows, 1, generator=gen) * w[target]
+    return x.to(dtype), w.to(dtype), target, gen
+
+
+def leaves(x, w):
+    return x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+
+
+def compare(x, w, parts, tau, reduction, dloss, loss, grads):
+    want = solve(x, w, *parts, tau, reduction, dloss)
+    check("loss", loss, want["loss"], want["e_loss"])
+    tol = 2.0 ** -7 if x.dtype == BF16 else 2e-5
+    for name, got in zip(("dx", "dw"), grads):
+        assert got.dtype == x.dtype
+        check(name, got, want[name], want["e_" + name])
+        check_norm(name, got, want[name], tol)
+    return want
+
+
+def run_ce(x, w, target, reduction, dloss, ignore=-100):
+    xd, wd = leaves(x, w)
+    loss = linear_cross_entropy(xd, wd, target.to(DEV), ignore_index=ignore, reduction=reduction)
+    return loss, torch.autograd.grad(loss, [xd, wd], dloss.to(DEV).reshape(loss.shape))
+
+
+SIZES = [(1, 1, 1), (1, 5, 8), (3, 256, 64), (2, 257, 65), (130, 255, 63), (127, 513, 640),
+         (128, 32, 200), (129, 1000, 72), (256, 512, 128), (257, 777, 1000), (600, 4100, 136),
+         (64, 9001, 8)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,dim", SIZES)
+def test_cross_entropy_at_odd_sizes(rows, vocab, dim, dtype):
+    x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=rows + vocab + dim)
+    reduction = ("none", "mean", "sum")[(rows + dim) % 3]
+    dloss = torch.randn(rows, generator=gen) if reduction == "none" else torch.tensor(0.7)
+    loss, grads = run_ce(x, w, target, reduction, dloss)
+    compare(x, w, sparse(1, target=target, ignore=-100), 1.0, reduction, dloss, loss, grads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,dim,k,tau", [(1, 1, 1, 1, 1.0), (1, 70, 24, 1, 2.0), (5, 300, 65, 7, 0.5),
+                                                  (130, 1000, 72, 33, 2.0), (257, 513, 640, 64, 4.0),
+                                                  (40, 2000, 128, 1024, 1.0)])
+def test_distillation_at_odd_sizes(rows, vocab, dim, k, tau, dtype):
+    x, w, _, gen = head_inputs(rows, vocab, dim, dtype, seed=rows + vocab + dim)
+    index = torch.randint(0, vocab, (rows, k), generator=gen)          # with repeats
+    logits = 3 * torch.randn(rows, k, generator=gen)
+    reduction = ("mean", "none", "sum")[rows % 3]
+    dloss = torch.randn(rows, generator=gen) if reduction == "none" else torch.tensor(-1.3)
+    xd, wd = leaves(x, w)
+    loss = linear_distillation(xd, wd, index.to(DEV), logits.to(DEV), temperature=tau, reduction=reduction)
+    grads = torch.autograd.grad(loss, [xd, wd], dloss.to(DEV).reshape(loss.shape))
+    parts = sparse(k, index=index, logits=logits, tau=tau)
+    compare(x, w, parts, tau, reduction, dloss, loss, grads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_pieces_of_the_vocabulary(dtype, monkeypatch):
+    """More than one piece: rows * 4096 entries of dz exceed the bound on a piece."""
+    rows, vocab, dim = (12000, 30000, 16) if dtype == F32 else (36000, 9000, 16)
+    x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=3)
+    target[::3] = -100
+    loss, grads = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    # float64 on the GPU, in row blocks: the CPU would take minutes
+    xd, wd, t = x.to(DEV).double(), w.to(DEV).double(), target.to(DEV)
+    keep = t >= 0
+    n = keep.sum()
+    total, dx, dw = 0.0, torch.empty_like(xd), torch.zeros_like(wd)
+    for a in range(0, rows, 4000):
+        s = slice(a, a + 4000)
+        z = xd[s] @ wd.t()
+        lse = torch.logsumexp(z, 1)
+        at = t[s].clamp(min=0)[:, None]
+        total += float(((lse - z.gather(1, at)[:, 0]) * keep[s]).sum())
+        d = torch.exp(z - lse[:, None]).scatter_add(1, at, torch.full_like(at, -1, dtype=z.dtype))
+        d = d * (keep[s] / n)[:, None]
+        dx[s] = d @ wd
+        dw += d.t() @ (xd[s] * keep[s][:, None])
+    assert abs(float(loss.detach()) - total / float(n)) <= 2e-6 * abs(total / float(n))
+    tol = 2.0 ** -7 if dtype == BF16 else 2e-5
+    check_norm("dx", grads[0], dx.cpu(), tol)
+    check_norm("dw", grads[1], dw.cpu(), tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_left_out_rows_may_hold_anything(dtype):
+    """Ignored rows with NaN and infinities: loss and gradient 0 there, none of it elsewhere."""
+    x, w, target, gen = head_inputs(150, 400, 72, dtype, seed=5)
+    target[::4] = 7777
+    x[0], x[4], x[8, 3] = float("nan"), float("inf"), float("-inf")
+    dloss = torch.randn(150, generator=gen)
+    loss, grads = run_ce(x, w, target, "none", dloss, ignore=7777)
+    parts = sparse(1, target=target, ignore=7777)
+    compare(x, w, parts, 1.0, "none", dloss, loss, grads)
+    assert (loss[::4] == 0).all() and (grads[0][::4] == 0).all()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_every_row_left_out(reduction):
+    x, w, target, _ = head_inputs(9, 50, 24, F32)
+    target[:] = -100
+    loss, grads = run_ce(x, w, target, reduction, torch.ones(9) if reduction == "none" else torch.tensor(1.0))
+    if reduction == "mean":
+        assert torch.isnan(loss)                                       # 0 / 0, as PyTorch's
+    else:
+        assert (loss == 0).all()
+    assert all((gr == 0).all() for gr in grads)
+
+
+def test_empty_places_of_a_teacher_list():
+    """Negative indices, logits of -inf, NaN in empty places, rows with nothing left."""
+    rows, vocab, dim, k = 40, 333, 72, 6
+    x, w, _, gen = head_inputs(rows, vocab, dim, F32, seed=8)
+    index = torch.randint(0, vocab, (rows, k), generator=gen)
+    logits = 2 * torch.randn(rows, k, generator=gen)
+    index[::3, 1::2] = -1
+    logits[::3, 1] = float("nan")                                      # in an empty place
+    logits[1::3, 2] = float("-inf")
+    logits[2, :] = torch.finfo(torch.float32).min                      # the type's lowest: all alike
+    index[5] = -1                                                      # nothing left
+    logits[7] = float("-inf")                                          # nothing left either
+    x[5] = float("nan")
+    xd, wd = leaves(x, w)
+    loss = linear_distillation(xd, wd, index.to(DEV), logits.to(DEV), temperature=2.0)
+    grads = torch.autograd.grad(loss, [xd, wd])
+    parts = sparse(k, index=index, logits=torch.where(index < 0, 0.0, logits), tau=2.0)
+    assert not parts[3][5] and not parts[3][7] and parts[3].sum() == rows - 2
+    compare(x, w, parts, 2.0, "mean", torch.tensor(1.0), loss, grads)
+
+
+def test_indices_outside_the_vocabulary_are_loud_and_stay_in_bounds():
+    x, w, target, gen = head_inputs(10, 60, 24, F32)
+    target[3], target[6] = 60, -5
+    loss, grads = run_ce(x, w, target, "none", torch.ones(10))
+    bad = torch.zeros(10, dtype=torch.bool)
+    bad[3] = bad[6] = True
+    assert torch.equal(torch.isnan(loss.cpu()), bad)
+    assert torch.equal(torch.isnan(grads[0].cpu()).all(1), bad) and torch.isnan(grads[1]).all()
+    index, logits = torch.randint(0, 60, (10, 4), generator=gen), torch.zeros(10, 4)
+    index[2, 1] = 1 << 40
+    loss = linear_distillation(x.to(DEV), w.to(DEV), index.to(DEV), logits.to(DEV), reduction="none")
+    assert torch.isnan(loss[2]) and torch.isfinite(loss[torch.arange(10) != 2]).all()
+
+
+def test_infinite_and_nan_logits_reach_the_loss():
+    """A row that counts and holds inf or NaN has a NaN loss, as PyTorch's."""
+    x, w, target, _ = head_inputs(6, 300, 24, F32)
+    x[1, 0], x[2, 5] = float("inf"), float("nan")
+    loss = linear_cross_entropy(x.to(DEV), w.to(DEV), target.to(DEV), reduction="none").cpu()
+    assert torch.equal(torch.isnan(loss), torch.tensor([False, True, True, False, False, False]))
+
+
+def test_large_logits_do_not_overflow():
+    """Logits of +-3e4: the running maximum keeps every exponential in range."""
+    x, w, target, _ = head_inputs(33, 700, 64, F32, seed=2)
+    x = x * 4000
+    dloss = torch.ones(33)
+    loss, grads = run_ce(x, w, target, "none", dloss)
+    assert torch.isfinite(loss).all() and all(torch.isfinite(gr).all() for gr in grads)
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, 1) - z.gather(1, target[:, None])[:, 0]
+    # each logit to (dim + 16) 2^-23 of its products' magnitudes
+    bound = 2 * (64 + 16) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).amax(1) + 1e-6 * z.abs().amax(1)
+    assert ((loss.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strided_and_unaligned_inputs(dtype):
+    """Rows of a wider tensor, a base off 16 bytes, a transposed weight, leading dimensions."""
+    x, w, target, _ = head_inputs(90, 301, 40, dtype, seed=4)
+    want = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    wide = torch.full((90, 131), float("nan"), dtype=dtype, device=DEV)
+    views = [wide[:, 8:48], wide[:, 3:43]]
+    t = target.to(DEV)
+    for v in views:
+        wide.fill_(float("nan"))
+        v.copy_(x.to(DEV))
+        xs = v.detach().requires_grad_(True)
+        ws = w.to(DEV).t().contiguous().t().requires_grad_(True)
+        loss = linear_cross_entropy(xs, ws, t)
+        gr = torch.autograd.grad(loss, [xs, ws])
+        assert torch.equal(loss, want[0]) and all(torch.equal(a, b) for a, b in zip(gr, want[1]))
+    xs = x.to(DEV).reshape(3, 30, 40).requires_grad_(True)
+    loss = linear_cross_entropy(xs, w.to(DEV), t.reshape(3, 30).int(), reduction="none")
+    assert loss.shape == (3, 30)
+    assert torch.autograd.grad(loss.mean(), xs)[0].shape == (3, 30, 40)
+
+
+def test_one_gradient_alone_and_none():
+    x, w, target, _ = head_inputs(70, 301, 40, F32, seed=4)
+    _, (dx, dw) = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    t = target.to(DEV)
+    xd, wd = leaves(x, w)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(xd, w.to(DEV), t), xd)[0], dx)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x.to(DEV), wd, t), wd)[0], dw)
+    with torch.no_grad():
+        assert not linear_cross_entropy(xd, wd, t).requires_grad
+    # a weight used twice: both uses' gradients add up
+    loss = linear_cross_entropy(xd, wd, t) + linear_cross_entropy(xd, wd, t)
+    assert torch.allclose(torch.autograd.grad(loss, wd)[0], 2 * dw, rtol=1e-6, atol=0)
+
+
+def test_results_do_not_change_from_call_to_call():
+    x, w, target, _ = head_inputs(300, 5000, 256, BF16, seed=4)
+    a = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    b = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    assert torch.equal(a[0], b[0]) and all(torch.equal(p, q) for p, q in zip(a[1], b[1]))
+
+
+def test_gradient_against_differences():
+    """Central differences of the kernel's own loss along a direction v: off by at most
+    h^2 / 6 of the third derivative (third cumulants of a variable within a range R are below
+    0.0963 R^3, R the spread of the row's logits along v) and the losses' error over h."""
+    x, w, target, gen = head_inputs(64, 500, 96, F32, seed=6)
+    v = torch.randn(64, 96, generator=gen)
+    dv = torch.randn(500, 96, generator=gen) * 0.1
+    h = 2.0 ** -6
+    xd, wd, t = x.to(DEV), w.to(DEV), target.to(DEV)
+    _, (dx, dw) = run_ce(x, w, target, "sum", torch.tensor(1.0))
+    for step_x, step_w, slope in ((v, None, (dx.cpu().double() * v).sum()),
+                                  (None, dv, (dw.cpu().double() * dv).sum())):
+        vals = []
+        for s in (h, -h):
+            a = xd if step_x is None else xd + s * step_x.to(DEV)
+            b = wd if step_w is None else wd + s * step_w.to(DEV)
+            vals.append(float(linear_cross_entropy(a, b, t, reduction="none").double().sum()))
+        zv = (v.double() @ w.double().t()) if step_w is None else (x.double() @ dv.double().t())
+        spread = zv.amax(1) - zv.amin(1)
+        ez = 112 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).amax(1)
+        bound = float((h * h / 6 * 0.0963 * spread ** 3).sum() + (2 * ez + 2e-6).sum() / h)
+        assert abs((vals[0] - vals[1]) / (2 * h) - float(slope)) <= bound
+
+
+def test_another_stream_and_a_captured_graph():
+    x, w, target, _ = head_inputs(260, 900, 128, BF16, seed=1)
+    want_loss, want = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    xd, wd = leaves(x, w)
+    t = target.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            loss = linear_cross_entropy(xd, wd, t)
+            grads = torch.autograd.grad(loss, [xd, wd])
+        side.synchronize()
+        assert torch.equal(loss, want_loss) and all(torch.equal(a, b) for a, b in zip(grads, want))
+    del loss, grads
+    xd, wd = leaves(x, w)               # leaves that no eager graph has met
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = linear_cross_entropy(xd, wd, t)
+            grads = torch.autograd.grad(loss, [xd, wd])
+        graphs.append((graph, loss.detach(), grads))
+        del loss
+    with torch.no_grad():
+        xd.copy_(2 * xd)
+    for graph, _, _ in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        xd.copy_(xd / 2)
+    for graph, loss, grads in graphs:
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want_loss) and all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_the_refs_agree_with_the_kernels():
+    x, w, target, gen = head_inputs(50, 400, 64, F32, seed=9)
+    index, logits = torch.randint(-1, 400, (50, 5), generator=gen), torch.randn(50, 5, generator=gen)
+    a = linear_cross_entropy(x.to(DEV), w.to(DEV), target.to(DEV), impl="cuda")
+    assert abs(float(a) - float(linear_cross_entropy_ref(x.double(), w.double(), target))) <= 1e-5
+    b = linear_distillation(x.to(DEV), w.to(DEV), index.to(DEV), logits.to(DEV), 2.0, impl="metal")
+    assert abs(float(b) - float(linear_distillation_ref(x.double(), w.double(), index, logits.double(), 2.0))) <= 1e-5
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_head_and_both_losses_together(dtype):
+    """The end of a training step: residual norm, then cross entropy and distillation on its
+    output, gradients of both through the norm to the block's output and the head."""
+    rows, vocab, dim, k = 140, 700, 96, 8
+    x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=12)
+    y = (0.5 * torch.randn(rows, dim, generator=gen)).to(dtype)
+    nw = (1 + 0.1 * torch.randn(dim, generator=gen)).to(dtype)
+    index, logits = torch.randint(0, vocab, (rows, k), generator=gen), torch.randn(rows, k, generator=gen)
+    target[3] = -100
+
+    def step(x, y, nw, w, target, index, logits, impl):
+        lv = [t.detach().requires_grad_(True) for t in (x, y, nw, w)]
+        _, hidden = residual_rms_norm(lv[0], lv[1], lv[2], impl=impl)
+        loss = linear_cross_entropy(hidden, lv[3], target, impl=impl) \
+            + 0.5 * linear_distillation(hidden, lv[3], index, logits, 2.0, impl=impl)
+        return loss, torch.autograd.grad(loss, lv)
+
+    got = step(*(t.to(DEV) for t in (x, y, nw, w, target, index, logits)), "cuda")
+    want = step(*(t.double() for t in (x, y, nw, w)), target, index, logits.double(), "torch")
+    # bf16: the norm's output, each loss' dz, each loss' gradient, their sum and the norm's
+    # gradient are rounded: six roundings of 2^-8; float32 as above
+    tol = 6 * u(dtype) if dtype == BF16 else 2e-5
+    assert abs(float(got[0]) - float(want[0])) <= tol * float(want[0])
+    for name, a, b in zip(("dx", "dy", "dnorm", "dw"), got[1], want[1]):
+        check_norm(name, a, b, tol)
+
+
+def test_gpu_refusals():
+    x, w, target, _ = head_inputs(4, 20, 8, F32)
+    xd, wd, t = x.to(DEV), w.to(DEV), target.to(DEV)
+    with pytest.raises(RuntimeError, match="same CUDA"):
+        linear_cross_entropy(xd, w, t)
+    with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+        linear_cross_entropy(xd.half(), wd.half(), t)
+    with pytest.raises(RuntimeError, match="alike"):
+        linear_cross_entropy(xd, wd.bfloat16(), t)
+    with pytest.raises(RuntimeError, match="integer"):
+        linear_cross_entropy(xd, wd, t.float())
+    with pytest.raises(ValueError, match="target"):
+        linear_cross_entropy(xd, wd, t[:3])
+    with pytest.raises(ValueError, match="shapes"):
+        linear_cross_entropy(xd, wd[:, :5], t)
+    assert linear_cross_entropy(xd[:0], wd, t[:0], reduction="none").shape == (0,)
+    assert torch.isnan(linear_cross_entropy(xd[:0], wd, t[:0]))
+    loss = linear_cross_entropy(xd.requires_grad_(True), wd, t)
+    (dx,) = torch.autograd.grad(loss, xd, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    assert _native.device_status() == _native.MMS_OK
