@@ -434,9 +434,10 @@ int mms_device_status(void)
 {
     const cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return status_of(e);
-    const int t = mms::w8_take_timeout(), f = mms::fwd_take_timeout(), c = mms::cp_take_timeout();
-    if (t < 0 || f < 0 || c < 0) return status_of(cudaGetLastError());
-    return t || f || c ? MMS_ERR_TIMEOUT : MMS_OK;
+    const int t = mms::w8_take_timeout(), f = mms::fwd_take_timeout(), c = mms::cp_take_timeout(),
+              m = mms::mm_take_timeout();
+    if (t < 0 || f < 0 || c < 0 || m < 0) return status_of(cudaGetLastError());
+    return t || f || c || m ? MMS_ERR_TIMEOUT : MMS_OK;
 }
 
 const char *mms_last_cuda_error(void) { return cudaGetErrorString(g_last_cuda); }

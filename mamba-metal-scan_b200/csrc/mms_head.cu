@@ -15,7 +15,7 @@
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
 //
-// Forward:   products (MM_LSE) -> one (max, sum) per row and 256 columns;
+// Forward:   products (MM_LSE) -> one (max, sum) per row and 128 columns;
 //            pick_kernel: the dot products at the indices; lse_kernel joins
 //            the parts; a loss kernel; for mean / sum one block adds rows up.
 // Backward:  rows_kernel: r; stage_kernel: x with the left-out rows as zeros
@@ -43,7 +43,7 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 long long padded(int dim) { return (dim + 7) / 8 * 8; }     // rows of 16-byte multiples
 
-// Pieces of the vocabulary (each a multiple of MM_LSE_TILE rows of w but the
+// Pieces of the vocabulary (each a multiple of MM_COLS rows of w but the
 // last): as few equal ones as keep `bytes_per_row` (per vocabulary entry)
 // times the piece below PIECE_BYTES, at least 4096 entries each so that a
 // piece's products stay long.
@@ -51,7 +51,7 @@ int piece_size(int vocab, size_t bytes_per_row)
 {
     const long long most = std::max<long long>(4096, (long long)(PIECE_BYTES / bytes_per_row));
     const int pieces = ceil_div(vocab, most);
-    const long long v = ceil_div(ceil_div(vocab, pieces), MM_LSE_TILE) * (long long)MM_LSE_TILE;
+    const long long v = ceil_div(ceil_div(vocab, pieces), MM_COLS) * (long long)MM_COLS;
     return (int)std::min<long long>(v, vocab);
 }
 

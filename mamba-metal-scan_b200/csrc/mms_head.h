@@ -24,7 +24,8 @@ struct Factor {
 //   MM_GRAD   g[m, n] = rs[m] 2^(c s - lse2[m]) (0 where rs[m] is 0), as bf16 planes
 //   MM_OUT    out[m, n] = s (+ acc[m, n]), float32 or bf16
 enum MmKind { MM_LSE, MM_GRAD, MM_OUT };
-constexpr int MM_LSE_TILE = 256;
+constexpr int MM_LSE_TILE = 128;
+constexpr int MM_COLS = 256;            // columns of a tile
 
 struct MmArgs {
     Factor a, b;
@@ -41,7 +42,13 @@ struct MmArgs {
     bool out_bf16;              // MM_OUT
 };
 
+// Factors: 16-byte aligned, ld and plane multiples of 8. `g`: 16-byte aligned,
+// ldg and gplane multiples of 8, its rows are written up to the next multiple
+// of 8 columns. `out` 16-byte aligned.
 cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream);
+// 1 if a wait of the products timed out since the last call (and clears it),
+// 0 if not, -1 if the flag could not be read.
+int mm_take_timeout();
 
 // The two losses share everything but their sparse part: row m has the
 // entries index[m, 0..k), and for the distillation their probabilities.

@@ -356,3 +356,20 @@ def test_gpu_refusals():
     with pytest.raises(RuntimeError):
         dx.sum().backward()
     assert _native.device_status() == _native.MMS_OK
+
+
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable():
+    """The products' TMA waits, made to run out by withholding one step's copies."""
+    x, w, target, _ = head_inputs(300, 1000, 1024, BF16, seed=1)
+    want_loss, want = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    lib = _native.load()
+    assert lib.mms_debug_set_wait(1 << 10, 3) == _native.MMS_OK
+    try:
+        run_ce(x, w, target, "mean", torch.tensor(1.0))
+        status = _native.device_status()
+    finally:
+        lib.mms_debug_set_wait(0, -1)
+    assert status == _native.MMS_ERR_TIMEOUT
+    loss, grads = run_ce(x, w, target, "mean", torch.tensor(1.0))
+    assert _native.device_status() == _native.MMS_OK
+    assert torch.equal(loss, want_loss) and all(torch.equal(a, b) for a, b in zip(grads, want))
