@@ -15,7 +15,7 @@
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
 //
-// Forward:   products (MM_LSE) -> one (max, sum) per row and 128 columns;
+// Forward:   products (MM_LSE) -> one (max, sum) per row and half tile;
 //            pick_kernel: the dot products at the indices; lse_kernel joins
 //            the parts; a loss kernel; for mean / sum one block adds rows up.
 // Backward:  rows_kernel: r; stage_kernel: x with the left-out rows as zeros
@@ -69,11 +69,13 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, bool bf16, long long ldx, lon
     l.stage_w = !bf16 || ldw % 8;
     const size_t row = (size_t)padded(dim) * 2 * l.planes;
     l.piece = piece_size(vocab, std::max<size_t>(l.stage_w ? row : 1,
-                                                 (size_t)rows * sizeof(float2) / MM_LSE_TILE + 1));
+                                                 (size_t)rows * sizeof(float2) / 64 + 1));
+    const int last = vocab - (vocab - 1) / l.piece * l.piece;
     size_t o = 0;
     l.xs = o; o += l.stage_x ? up256(row * rows) : 0;
     l.ws = o; o += l.stage_w ? up256(row * l.piece) : 0;
-    l.part = o; o += up256((size_t)(ceil_div(l.piece, MM_LSE_TILE) + 1) * rows * sizeof(float2));
+    l.part = o; o += up256((size_t)(std::max(mm_lse_parts(rows, l.piece, dim, l.planes),
+                                            mm_lse_parts(rows, last, dim, l.planes)) + 1) * rows * sizeof(float2));
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
     l.total = o;
     return l;
@@ -83,7 +85,7 @@ struct BwdLayout {
     bool stage_w;
     int planes, piece;
     long long ldg;
-    size_t xs, ws, g, dxacc, rs, total;
+    size_t xs, ws, g, dxacc, rs, split, split_bytes, total;
 };
 
 BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
@@ -100,6 +102,10 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
     l.g = o; o += up256((size_t)rows * l.ldg * 2 * l.planes);
     l.dxacc = o; o += l.piece < vocab ? up256((size_t)rows * dim * sizeof(float)) : 0;
     l.rs = o; o += up256((size_t)rows * sizeof(float));
+    // partial sums; the last, smaller piece splits as far as this room goes
+    l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.planes),
+                             mm_split_bytes(l.piece, dim, rows, l.planes));
+    l.split = o; o += up256(l.split_bytes);
     l.total = o;
     return l;
 }
@@ -396,7 +402,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         cudaError_t e = launch_mm(MM_LSE, mm, stream);
         if (e != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
-            part, ceil_div(nv, MM_LSE_TILE), v0 == 0, last, a.rows, a.lse2,
+            part, mm_lse_parts(a.rows, nv, a.dim, l.planes), v0 == 0, last, a.rows, a.lse2,
             a.kd ? nullptr : a.index, a.ignore_index, a.picked, rowloss);
     }
     if (a.kd)
@@ -436,6 +442,8 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
                                                             l.planes);
         MmArgs out{};
         out.planes = l.planes;
+        out.split = fl(a.workspace, l.split);
+        out.split_bytes = l.split_bytes;
         if (a.dx) {
             out.a = Factor{g, l.ldg, gplane, false};
             out.b = mm.b;

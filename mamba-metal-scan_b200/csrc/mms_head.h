@@ -19,13 +19,13 @@ struct Factor {
 };
 
 // The three products of the losses, s[m, n] = sum_k a(m, k) b(n, k):
-//   MM_LSE    each row's log-sum-exp over tiles of MM_LSE_TILE columns:
-//             part[tile * m + row] = (max, sum of 2^(c s - max)), in units of log 2
+//   MM_LSE    each row's log-sum-exp over parts of the columns:
+//             part[i * m + row] = (max, sum of 2^(c s - max)), in units of log 2,
+//             i < mm_lse_parts()
 //   MM_GRAD   g[m, n] = rs[m] 2^(c s - lse2[m]) (0 where rs[m] is 0), as bf16 planes
 //   MM_OUT    out[m, n] = s (+ acc[m, n]), float32 or bf16
 enum MmKind { MM_LSE, MM_GRAD, MM_OUT };
-constexpr int MM_LSE_TILE = 128;
-constexpr int MM_COLS = 256;            // columns of a tile
+constexpr int MM_COLS = 256;            // columns of the widest tile
 
 struct MmArgs {
     Factor a, b;
@@ -38,9 +38,14 @@ struct MmArgs {
     long long ldg, gplane;      // MM_GRAD
     const float *acc;           // MM_OUT: added, (m, n) with row stride ldo; may be null
     void *out;                  // MM_OUT
-    long long ldo;              // MM_OUT
+    long long ldo;              // MM_OUT (= n where split may be used)
     bool out_bf16;              // MM_OUT
+    float *split;               // MM_OUT: room for partial sums over parts of k,
+    size_t split_bytes;         //         mm_split_bytes() or less
 };
+
+int mm_lse_parts(int m, int n, int k, int planes);
+size_t mm_split_bytes(int m, int n, int k, int planes);
 
 // Factors: 16-byte aligned, ld and plane multiples of 8. `g`: 16-byte aligned,
 // ldg and gplane multiples of 8, its rows are written up to the next multiple
