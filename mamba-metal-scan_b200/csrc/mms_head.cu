@@ -15,17 +15,33 @@
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
 //
-// Forward:   products (MM_LSE) -> one (max, sum) per row and half tile;
-//            pick_kernel: the dot products at the indices; lse_kernel joins
-//            the parts; a loss kernel; for mean / sum one block adds rows up.
-// Backward:  rows_kernel: r; stage_kernel: x with the left-out rows as zeros
-//            (so that nothing in them, NaN included, reaches dw); per piece:
-//            product MM_GRAD, sparse_kernel sets dz at the indices (from
-//            picked, in fp32, as r (expm1(log q) + 1 - p): no cancellation
-//            when a target's probability is near 1), then MM_OUT twice.
+// Forward:   pick_kernel: the dot products at the indices; products (MM_LSE)
+//            -> one (max, sum) per row and half tile, joined by lse_kernel;
+//            a loss kernel; one block adds the rows up.
+// Backward:  rows_kernel: r; x staged with the left-out rows as zeros (so that
+//            nothing in them, NaN included, reaches dw); per piece: product
+//            MM_GRAD, sparse_kernel sets dz at the indices (from picked, in
+//            fp32, as expm1(log q) + 1 - p: no cancellation when a target's
+//            probability is near 1), then MM_OUT twice.
 //
-// fp32 factors are split into three bf16 planes (8 bits of mantissa each):
-// the products of planes i + j <= 2 leave out terms below 2^-24.
+// bf16: dz is stored as r (q - p) in bf16, one plane. Its rounding (2^-8 a
+// value at most) averages out over a sum of many; with up to FEW_ROWS rows one
+// value can dominate a whole gradient, so a second plane holds the rest there
+// (one more pass of two products that such sizes do not feel).
+//
+// float32: factors are split into two fp16 planes, 22 bits, after a scaling by
+// a power of two that brings the largest element into [2^14, 2^15); the
+// product of the second planes (below 2^-22 of a term) is left out. Elements
+// below 2^-29 of the largest lose bits to fp16's range: 2^-39 of the largest is
+// the absolute bound. Three passes of the tensor cores; three bf16 planes would
+// keep float32's range but need six. The scalings follow the output's rows
+// where they can, so that rows do not disturb one another:
+//   z  = x w^T    x scaled row by row, w as a whole
+//   dz = 2^14 (q - p) without r, in [-2^14, 2^14]
+//   dx = r dz w   r in the epilogue
+//   dw = dz^T (r x)   r x scaled as a whole
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 #include "mms_common.cuh"
@@ -37,7 +53,9 @@ namespace mms {
 namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
-constexpr size_t PIECE_BYTES = (size_t)256 << 20;   // bound on one staged or dz piece
+constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // bound on one staged or dz piece
+constexpr int FEW_ROWS = 256;
+constexpr float DZ_UNIT = 16384.f;                  // float32: the scale of dz's planes
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -55,91 +73,217 @@ int piece_size(int vocab, size_t bytes_per_row)
     return (int)std::min<long long>(v, vocab);
 }
 
-struct FwdLayout {
+// Both directions: planes of x and w, and whether they are staged.
+struct Layout {
     bool stage_x, stage_w;
-    int planes, piece;
-    size_t xs, ws, part, rowloss, total;
+    int planes, piece, last;        // vocabulary entries of a piece, of the last one
+    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and maxima)
+    size_t total;
 };
+
+struct FwdLayout : Layout {
+    size_t part, rowloss;
+};
+
+struct BwdLayout : Layout {
+    int gplanes;
+    long long ldg;
+    size_t xr, g, dxacc, rs, split, split_bytes;
+};
+
+size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
+{
+    const size_t row = (size_t)padded(dim) * 2 * l.planes;
+    l.piece = piece_size(vocab, std::max<size_t>(l.stage_w ? row : 1, per_entry));
+    l.last = vocab - (vocab - 1) / l.piece * l.piece;
+    size_t o = 0;
+    l.muls = o; o += 256;
+    l.row_mul = o; o += l.planes > 1 ? up256((size_t)rows * sizeof(float)) : 0;
+    l.xs = o; o += l.stage_x ? up256(row * rows) : 0;
+    l.ws = o; o += l.stage_w ? up256(row * l.piece) : 0;
+    return o;
+}
 
 FwdLayout fwd_layout(int rows, int vocab, int dim, bool bf16, long long ldx, long long ldw)
 {
     FwdLayout l;
-    l.planes = bf16 ? 1 : 3;
+    l.planes = bf16 ? 1 : 2;
     l.stage_x = !bf16 || ldx % 8;
     l.stage_w = !bf16 || ldw % 8;
-    const size_t row = (size_t)padded(dim) * 2 * l.planes;
-    l.piece = piece_size(vocab, std::max<size_t>(l.stage_w ? row : 1,
-                                                 (size_t)rows * sizeof(float2) / 64 + 1));
-    const int last = vocab - (vocab - 1) / l.piece * l.piece;
-    size_t o = 0;
-    l.xs = o; o += l.stage_x ? up256(row * rows) : 0;
-    l.ws = o; o += l.stage_w ? up256(row * l.piece) : 0;
-    l.part = o; o += up256((size_t)(std::max(mm_lse_parts(rows, l.piece, dim, l.planes),
-                                            mm_lse_parts(rows, last, dim, l.planes)) + 1) * rows * sizeof(float2));
+    size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * sizeof(float2) / 32 + 1);
+    const int parts = std::max(mm_lse_parts(rows, l.piece, dim, l.planes, l.planes),
+                               mm_lse_parts(rows, l.last, dim, l.planes, l.planes));
+    l.part = o; o += up256((size_t)(parts + 1) * rows * sizeof(float2));
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
     l.total = o;
     return l;
 }
 
-struct BwdLayout {
-    bool stage_w;
-    int planes, piece;
-    long long ldg;
-    size_t xs, ws, g, dxacc, rs, split, split_bytes, total;
-};
-
 BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
 {
     BwdLayout l;
-    l.planes = bf16 ? 1 : 3;
+    l.planes = bf16 ? 1 : 2;
+    l.gplanes = bf16 && rows > FEW_ROWS ? 1 : 2;
+    l.stage_x = true;
     l.stage_w = !bf16 || ldw % 8;
-    const size_t row = (size_t)padded(dim) * 2 * l.planes;
-    l.piece = piece_size(vocab, std::max<size_t>(l.stage_w ? row : 1, (size_t)rows * 2 * l.planes));
+    size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * 2 * l.gplanes);
     l.ldg = (l.piece + 7) / 8 * 8;
-    size_t o = 0;
-    l.xs = o; o += up256(row * rows);
-    l.ws = o; o += l.stage_w ? up256(row * l.piece) : 0;
-    l.g = o; o += up256((size_t)rows * l.ldg * 2 * l.planes);
+    l.xr = o; o += l.planes > 1 ? up256((size_t)padded(dim) * 2 * l.planes * rows) : 0;
+    l.g = o; o += up256((size_t)rows * l.ldg * 2 * l.gplanes);
     l.dxacc = o; o += l.piece < vocab ? up256((size_t)rows * dim * sizeof(float)) : 0;
     l.rs = o; o += up256((size_t)rows * sizeof(float));
     // partial sums; the last, smaller piece splits as far as this room goes
-    l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.planes),
-                             mm_split_bytes(l.piece, dim, rows, l.planes));
+    l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.gplanes, l.planes),
+                             mm_split_bytes(l.piece, dim, rows, l.gplanes, l.planes));
     l.split = o; o += up256(l.split_bytes);
     l.total = o;
     return l;
 }
 
-// out[p, r, 0..cols) = the bf16 planes of src[r, 0..cols); rows with rs = 0
-// (if given) as zeros. Row stride ld of out, planes apart by `plane`.
+// ------------------------------------------------------------------- staging
+
+// Powers of two: 2^e as two factors (e may be beyond float32's exponents).
+struct Pow2 {
+    float a, b;
+    __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+};
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+// The exponent that brings `top` into [2^14, 2^15); 0 for 0.
+__device__ __forceinline__ int exponent_for(float top) {
+    return top == 0.f ? 0 : 14 - max((int)(__float_as_uint(top) >> 23) - 127, -126);
+}
+__device__ __forceinline__ Pow2 scale_by(int e) { return Pow2{pow2(e / 2), pow2(e - e / 2)}; }
+__device__ __forceinline__ float finite_abs(float v) {
+    v = fabsf(v);
+    return v <= 3.4028234e38f ? v : 0.f;
+}
+
+// 8 elements of a row from column c on; 0 beyond `cols`.
 template <typename T>
-__global__ void __launch_bounds__(256)
-stage_kernel(const T *__restrict__ src, long long lds, const float *__restrict__ rs,
-             __nv_bfloat16 *__restrict__ out, long long ld, long long plane, int rows, int cols,
-             int planes)
-{
-    const long long total = (long long)rows * cols;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
-         i += (long long)gridDim.x * 256) {
-        const long long r = i / cols;
-        const int c = (int)(i - r * cols);
-        float v = to_f(src[r * lds + c]);
-        if (rs && rs[r] == 0.f) v = 0.f;
-        for (int p = 0; p < planes; ++p) {
-            const __nv_bfloat16 q = __float2bfloat16_rn(v);
-            out[p * plane + r * ld + c] = q;
-            v -= to_f(q);
-        }
+__device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, float (&v)[8]) {
+    if (c + 8 <= cols && reinterpret_cast<uintptr_t>(p + c) % 16 == 0) {
+        uint4 q[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = __ldg(reinterpret_cast<const uint4 *>(p + c) + i);
+        const T *e = reinterpret_cast<const T *>(q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(p[c + i]) : 0.f;
     }
 }
 
-template <typename T>
-void stage(const void *src, long long lds, const float *rs, __nv_bfloat16 *out, long long ld,
-           long long plane, int rows, int cols, int planes, cudaStream_t stream)
+// How a staged matrix is scaled: not at all (bf16), each row to its own
+// maximum, or all of it to the maximum that `top` holds.
+enum StageKind { ST_COPY, ST_ROWS, ST_WHOLE };
+
+struct StageArgs {
+    const void *src;
+    long long lds;
+    uint16_t *out;
+    long long ld, plane;
+    int rows, cols;
+    const float *rs;            // ST_COPY, ST_ROWS: rows with 0 there become 0; ST_WHOLE: factors of the rows
+    float *mul;                 // ST_ROWS: 2^-e of each row; ST_WHOLE: of all
+    unsigned *top;              // ST_WHOLE: the maximum's bits; ST_ROWS: the maximum of |rs| row maximum goes here
+};
+
+// LP lanes a row, 8 columns a lane and step.
+template <typename T, int KIND, int LP>
+__global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
 {
-    const long long blocks = ((long long)rows * cols + 255) / 256;
-    stage_kernel<T><<<(int)std::min<long long>(blocks, 148 * 16), 256, 0, stream>>>(
-        static_cast<const T *>(src), lds, rs, out, ld, plane, rows, cols, planes);
+    const int lane = threadIdx.x % LP;
+    float top = 0.f;
+    constexpr int RW = 32 / LP;                             // rows a warp has at once
+    for (int r0 = (blockIdx.x * 8 + threadIdx.x / 32) * RW; r0 < a.rows; r0 += gridDim.x * 8 * RW) {
+        const int r = r0 + threadIdx.x % 32 / LP;           // lanes beyond the rows stay for the shuffles
+        const bool in = r < a.rows;
+        const T *src = static_cast<const T *>(a.src) + (size_t)r * a.lds;
+        uint16_t *out = a.out + (size_t)r * a.ld;
+        const float rs = !in ? 0.f : a.rs ? a.rs[r] : 1.f;
+        const int cols = rs == 0.f ? 0 : a.cols;            // nothing of a left-out row is read
+        Pow2 by{1.f, 1.f};
+        if (KIND == ST_ROWS) {
+            float m = 0.f;
+            for (int c = lane * 8; c < cols; c += LP * 8) {
+                float v[8];
+                load8(src, c, cols, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
+            }
+#pragma unroll
+            for (int o = LP / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o, LP));
+            const int e = exponent_for(m);
+            by = scale_by(e);
+            if (in && lane == 0) a.mul[r] = pow2(-e);
+            top = fmaxf(top, finite_abs(rs * m));
+        }
+        if (KIND == ST_WHOLE) {
+            const int e = exponent_for(__uint_as_float(*a.top));
+            by = scale_by(e);
+            if (r == 0 && lane == 0) *a.mul = pow2(-e);
+        }
+        for (int c = lane * 8; in && c < a.cols; c += LP * 8) {
+            float v[8];
+            load8(src, c, cols, v);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint16_t h[2], l[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x = v[2 * i + j];
+                    if (KIND == ST_COPY) {
+                        h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+                    } else {
+                        x = by(KIND == ST_WHOLE ? rs * x : x);
+                        const __half q = __float2half_rn(x);
+                        h[j] = __half_as_ushort(q);
+                        l[j] = __half_as_ushort(__float2half_rn(x - __half2float(q)));
+                    }
+                }
+                hi[i] = h[0] | (uint32_t)h[1] << 16;
+                if (KIND != ST_COPY) lo[i] = l[0] | (uint32_t)l[1] << 16;
+            }
+            *reinterpret_cast<uint4 *>(out + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (KIND != ST_COPY)
+                *reinterpret_cast<uint4 *>(out + a.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+    if (KIND == ST_ROWS && a.top) {                         // non-negative floats compare as their bits
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));
+    }
+}
+
+// The largest finite magnitude of a float32 matrix, as bits (top starts at 0).
+__global__ void __launch_bounds__(256)
+top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, unsigned *top)
+{
+    float m = 0.f;
+    for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
+#pragma unroll 2
+        for (int c = threadIdx.x % 32 * 8; c < cols; c += 256) {
+            float v[8];
+            load8(src + (size_t)r * lds, c, cols, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
+        }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    if (threadIdx.x % 32 == 0 && m > 0.f) atomicMax(top, __float_as_uint(m));
+}
+
+int grid_of(long long rows, int per_block) { return (int)std::min<long long>((rows + per_block - 1) / per_block, 148 * 16); }
+
+template <typename T, int KIND>
+void stage(const StageArgs &a, cudaStream_t s)
+{
+    if (a.cols <= 64) stage_kernel<T, KIND, 8><<<grid_of(a.rows, 32), 256, 0, s>>>(a);
+    else if (a.cols <= 128) stage_kernel<T, KIND, 16><<<grid_of(a.rows, 16), 256, 0, s>>>(a);
+    else stage_kernel<T, KIND, 32><<<grid_of(a.rows, 8), 256, 0, s>>>(a);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -171,7 +315,14 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
         s = __int_as_float(0x7fc00000);
     } else {
         const T *xr = x + e / k * ldx, *wr = w + v * ldw;
-        for (int i = lane; i < dim; i += 32) s = fmaf(to_f(xr[i]), to_f(wr[i]), s);
+#pragma unroll 2
+        for (int i = lane * 8; i < dim; i += 256) {
+            float p[8], q[8];
+            load8(xr, i, dim, p);
+            load8(wr, i, dim, q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf(p[j], q[j], s);
+        }
         s = warp_sum(s) * c;
     }
     if (lane == 0) picked[e] = s;
@@ -309,12 +460,13 @@ __global__ void rows_kernel(const float *__restrict__ dloss, const float *__rest
     rs[m] = r;
 }
 
-// dz at the sparse entries that lie in this piece of the vocabulary.
+// dz at the sparse entries that lie in this piece of the vocabulary; `unit` in
+// place of r if it is not 0.
 __global__ void __launch_bounds__(256)
 sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
               const float *__restrict__ picked, const float *__restrict__ lse2,
-              const float *__restrict__ rs, int k, long long n, int v0, int v1,
-              __nv_bfloat16 *__restrict__ g, long long ldg, long long gplane, int planes)
+              const float *__restrict__ rs, float unit, int k, long long n, int v0, int v1,
+              uint16_t *__restrict__ g, long long ldg, long long gplane, int planes)
 {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= n) return;
@@ -329,35 +481,59 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
         for (int j = 0; j < k; ++j)
             if (index[m * k + j] == v) p += prob[m * k + j];
     }
-    float d = r * (expm1f(LN2 * (picked[e] - lse2[m])) + (1.f - p));
+    float d = (unit != 0.f ? unit : r) * (expm1f(LN2 * (picked[e] - lse2[m])) + (1.f - p));
     for (int q = 0; q < planes; ++q) {
-        const __nv_bfloat16 t = __float2bfloat16_rn(d);
-        g[q * gplane + m * ldg + (v - v0)] = t;
-        d -= to_f(t);
+        uint16_t *o = g + q * gplane + m * ldg + (v - v0);
+        if (unit != 0.f) {
+            const __half t = __float2half_rn(d);
+            *o = __half_as_ushort(t);
+            d -= __half2float(t);
+        } else {
+            const __nv_bfloat16 t = __float2bfloat16_rn(d);
+            *o = __bfloat16_as_ushort(t);
+            d -= to_f(t);
+        }
     }
 }
 
-__nv_bfloat16 *bf(void *base, size_t off) {
-    return reinterpret_cast<__nv_bfloat16 *>(static_cast<char *>(base) + off);
-}
+uint16_t *u16(void *base, size_t off) { return reinterpret_cast<uint16_t *>(static_cast<char *>(base) + off); }
 float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast<char *>(base) + off); }
 
-void stage_any(bool bf16, const void *src, long long lds, const float *rs, __nv_bfloat16 *out,
-               long long ld, long long plane, int rows, int cols, int planes, cudaStream_t stream)
+// muls: w's scale, r x's scale, and the bits of the two maxima they come from.
+cudaError_t top_of_w(const HeadArgs &a, const Layout &l, cudaStream_t s)
 {
-    if (bf16) stage<__nv_bfloat16>(src, lds, rs, out, ld, plane, rows, cols, planes, stream);
-    else stage<float>(src, lds, rs, out, ld, plane, rows, cols, planes, stream);
+    unsigned *top = reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 2);
+    const cudaError_t e = cudaMemsetAsync(top, 0, 2 * sizeof(unsigned), s);
+    if (e == cudaSuccess)
+        top_kernel<<<grid_of(a.vocab, 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw, a.vocab, a.dim, top);
+    return e;
 }
 
 // Rows [v0, v0 + n) of w as a factor: staged, or w itself.
-Factor w_factor(const HeadArgs &a, bool staged, __nv_bfloat16 *ws, int piece, int planes, int v0,
-                int n, bool t, cudaStream_t stream)
+Factor w_factor(const HeadArgs &a, const Layout &l, int v0, int n, cudaStream_t s)
 {
-    if (!staged) return Factor{static_cast<const __nv_bfloat16 *>(a.w) + (size_t)v0 * a.ldw, a.ldw, 0, t};
-    const long long ld = padded(a.dim), plane = ld * piece;
-    const char *src = static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4);
-    stage_any(a.bf16, src, a.ldw, nullptr, ws, ld, plane, n, a.dim, planes, stream);
-    return Factor{ws, ld, plane, t};
+    if (!l.stage_w) return Factor{static_cast<const uint16_t *>(a.w) + (size_t)v0 * a.ldw, a.ldw, 0, 1, false};
+    const long long ld = padded(a.dim);
+    float *muls = fl(a.workspace, l.muls);
+    StageArgs st{static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4), a.ldw,
+                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, muls,
+                 reinterpret_cast<unsigned *>(muls + 2)};
+    if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
+    else stage<float, ST_WHOLE>(st, s);
+    return Factor{st.out, ld, st.plane, l.planes, false};
+}
+
+// x as a factor of z: staged (rows with rs = 0 as zeros), or x itself.
+Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, cudaStream_t s)
+{
+    if (!l.stage_x) return Factor{static_cast<const uint16_t *>(a.x), a.ldx, 0, 1, false};
+    const long long ld = padded(a.dim);
+    StageArgs st{a.x, a.ldx, u16(a.workspace, l.xs), ld, ld * a.rows, a.rows, a.dim, rs,
+                 fl(a.workspace, l.row_mul),
+                 rs ? reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3) : nullptr};
+    if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
+    else stage<float, ST_ROWS>(st, s);
+    return Factor{st.out, ld, st.plane, l.planes, false};
 }
 
 }  // namespace
@@ -385,25 +561,25 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         pick_kernel<float><<<pick_grid, 256, 0, stream>>>(
             static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index,
             a.kd, a.ignore_index, a.k, c, a.picked, n, a.vocab, a.dim);
-    Factor x{static_cast<const __nv_bfloat16 *>(a.x), a.ldx, 0, false};
-    if (l.stage_x) {
-        x = Factor{bf(a.workspace, l.xs), padded(a.dim), padded(a.dim) * a.rows, false};
-        stage_any(a.bf16, a.x, a.ldx, nullptr, bf(a.workspace, l.xs), x.ld, x.plane, a.rows, a.dim,
-                  l.planes, stream);
-    }
+    cudaError_t e;
+    if (l.planes > 1 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
+    const Factor x = x_factor(a, l, nullptr, stream);
     for (int v0 = 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
-        const bool last = v0 + nv == a.vocab;
         MmArgs mm{};
         mm.a = x;
-        mm.b = w_factor(a, l.stage_w, bf(a.workspace, l.ws), l.piece, l.planes, v0, nv, false, stream);
-        mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.planes = l.planes; mm.c = c;
+        mm.b = w_factor(a, l, v0, nv, stream);
+        mm.fp16 = !a.bf16;
+        mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
+        if (l.planes > 1) {
+            mm.row_mul = fl(a.workspace, l.row_mul);
+            mm.mul = fl(a.workspace, l.muls);
+        }
         mm.part = part + a.rows;                        // part 0: the pieces before
-        cudaError_t e = launch_mm(MM_LSE, mm, stream);
-        if (e != cudaSuccess) return e;
+        if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
-            part, mm_lse_parts(a.rows, nv, a.dim, l.planes), v0 == 0, last, a.rows, a.lse2,
-            a.kd ? nullptr : a.index, a.ignore_index, a.picked, rowloss);
+            part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
+            a.lse2, a.kd ? nullptr : a.index, a.ignore_index, a.picked, rowloss);
     }
     if (a.kd)
         kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau, a.lse2,
@@ -422,42 +598,63 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     rows_kernel<<<ceil_div(a.rows, 256), 256, 0, stream>>>(a.dloss, a.c_count, a.index, prob,
                                                            a.c_picked, a.k, a.ignore_index,
                                                            a.reduction, a.tau, rs, a.rows);
-    const long long ldx = padded(a.dim), n = (long long)a.rows * a.k;
-    __nv_bfloat16 *xs = bf(a.workspace, l.xs), *g = bf(a.workspace, l.g);
-    stage_any(a.bf16, a.x, a.ldx, rs, xs, ldx, ldx * a.rows, a.rows, a.dim, l.planes, stream);
-    const long long gplane = (long long)a.rows * l.ldg;
+    cudaError_t e;
+    const bool f32 = l.planes > 1;
+    float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
+    if (f32 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
+    const Factor x = x_factor(a, l, rs, stream);
+    Factor xr = x;                                      // the factor of dw: x, or r x
+    if (f32) {
+        StageArgs st{a.x, a.ldx, u16(a.workspace, l.xr), x.ld, x.plane, a.rows, a.dim, rs, muls + 1,
+                     reinterpret_cast<unsigned *>(muls + 3)};
+        stage<float, ST_WHOLE>(st, stream);
+        xr.p = st.out;
+    }
+    xr.t = true;
+    const long long n = (long long)a.rows * a.k, gplane = (long long)a.rows * l.ldg;
+    const float unit = f32 ? DZ_UNIT : 0.f;
+    uint16_t *g = u16(a.workspace, l.g);
     for (int v0 = 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
         const bool first = v0 == 0, last = v0 + nv == a.vocab;
         MmArgs mm{};
-        mm.planes = l.planes;
-        mm.a = Factor{xs, ldx, ldx * a.rows, false};
-        mm.b = w_factor(a, l.stage_w, bf(a.workspace, l.ws), l.piece, l.planes, v0, nv, false, stream);
+        mm.a = x;
+        mm.b = w_factor(a, l, v0, nv, stream);
+        mm.fp16 = f32;
         mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
-        mm.lse2 = a.c_lse2; mm.rs = rs; mm.g = g; mm.ldg = l.ldg; mm.gplane = gplane;
-        cudaError_t e = launch_mm(MM_GRAD, mm, stream);
-        if (e != cudaSuccess) return e;
-        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_picked, a.c_lse2, rs,
-                                                            a.k, n, v0, v0 + nv, g, l.ldg, gplane,
-                                                            l.planes);
+        if (f32) {
+            mm.row_mul = row_mul;
+            mm.mul = muls;
+        }
+        mm.lse2 = a.c_lse2; mm.rs = rs; mm.g_unit = unit;
+        mm.g = g; mm.ldg = l.ldg; mm.gplane = gplane; mm.gplanes = l.gplanes;
+        if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) return e;
+        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_picked, a.c_lse2, rs, unit,
+                                                            a.k, n, v0, v0 + nv, g, l.ldg, gplane, l.gplanes);
         MmArgs out{};
-        out.planes = l.planes;
+        out.fp16 = f32;
+        out.c = f32 ? 1.f / DZ_UNIT : 1.f;
+        out.n = a.dim;
         out.split = fl(a.workspace, l.split);
         out.split_bytes = l.split_bytes;
+        out.a = Factor{g, l.ldg, gplane, l.gplanes, false};
         if (a.dx) {
-            out.a = Factor{g, l.ldg, gplane, false};
             out.b = mm.b;
             out.b.t = true;
-            out.m = a.rows; out.n = a.dim; out.k = nv; out.ldo = a.dim;
+            out.m = a.rows; out.k = nv;
+            out.row_mul = f32 ? rs : nullptr;
+            out.mul = f32 ? muls : nullptr;
             out.acc = first ? nullptr : acc;
             out.out = last ? a.dx : acc;
             out.out_bf16 = last && a.bf16;
             if ((e = launch_mm(MM_OUT, out, stream)) != cudaSuccess) return e;
         }
         if (a.dw) {
-            out.a = Factor{g, l.ldg, gplane, true};
-            out.b = Factor{xs, ldx, ldx * a.rows, true};
-            out.m = nv; out.n = a.dim; out.k = a.rows; out.ldo = a.dim;
+            out.a.t = true;
+            out.b = xr;
+            out.m = nv; out.k = a.rows;
+            out.row_mul = nullptr;
+            out.mul = f32 ? muls + 1 : nullptr;
             out.acc = nullptr;
             out.out = static_cast<char *>(a.dw) + (size_t)v0 * a.dim * (a.bf16 ? 2 : 4);
             out.out_bf16 = a.bf16;

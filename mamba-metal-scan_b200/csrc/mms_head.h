@@ -1,52 +1,56 @@
 // Internal interface of the head's losses (mms_head.cu) and their matrix
-// products (mms_head_mm.cu).
+// products (mms_head_mm.cu), and of the residual norm (mms_norm.cu).
 #pragma once
 
-#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
 
 namespace mms {
 
-// A factor of a product: 1 bf16 matrix, or 3 (planes apart by `plane`
-// elements) whose sum is the fp32 matrix. Element (r, k), with k the summed
-// index, is at p[r * ld + k], or at p[k * ld + r] if `t`.
+// A factor of a product: `planes` matrices of 16-bit floats, apart by `plane`
+// elements, whose sum is the factor. Element (r, k), with k the summed index,
+// is at p[r * ld + k], or at p[k * ld + r] if `t`.
 struct Factor {
-    const __nv_bfloat16 *p;
+    const uint16_t *p;
     long long ld, plane;
+    int planes;
     bool t;
 };
 
-// The three products of the losses, s[m, n] = sum_k a(m, k) b(n, k):
+// The three products of the losses, s[m, n] = f sum_k a(m, k) b(n, k) with
+// f = c * (row_mul ? row_mul[m] : 1) * (mul ? *mul : 1):
 //   MM_LSE    each row's log-sum-exp over parts of the columns:
-//             part[i * m + row] = (max, sum of 2^(c s - max)), in units of log 2,
+//             part[i * m + row] = (max, sum of 2^(s - max)), in units of log 2,
 //             i < mm_lse_parts()
-//   MM_GRAD   g[m, n] = rs[m] 2^(c s - lse2[m]) (0 where rs[m] is 0), as bf16 planes
+//   MM_GRAD   g[m, n] = r 2^(s - lse2[m]) as planes of 16-bit floats; 0 where
+//             rs[m] is 0; r = rs[m], or the constant g_unit if that is not 0
 //   MM_OUT    out[m, n] = s (+ acc[m, n]), float32 or bf16
 enum MmKind { MM_LSE, MM_GRAD, MM_OUT };
 constexpr int MM_COLS = 256;            // columns of the widest tile
 
 struct MmArgs {
     Factor a, b;
+    bool fp16;                  // the planes are fp16, else bf16
     int m, n, k;
-    int planes;                 // 1 or 3, of both factors (and of g)
-    float c;                    // MM_LSE, MM_GRAD
+    float c;
+    const float *row_mul, *mul;
     float2 *part;               // MM_LSE
     const float *lse2, *rs;     // MM_GRAD
-    __nv_bfloat16 *g;           // MM_GRAD
+    float g_unit;               // MM_GRAD
+    uint16_t *g;                // MM_GRAD
     long long ldg, gplane;      // MM_GRAD
-    const float *acc;           // MM_OUT: added, (m, n) with row stride ldo; may be null
-    void *out;                  // MM_OUT
-    long long ldo;              // MM_OUT (= n where split may be used)
+    int gplanes;                // MM_GRAD
+    const float *acc;           // MM_OUT: added, laid out as out; may be null
+    void *out;                  // MM_OUT, row stride n
     bool out_bf16;              // MM_OUT
-    float *split;               // MM_OUT: room for partial sums over parts of k,
+    float *split;               // MM_OUT: room for partial sums,
     size_t split_bytes;         //         mm_split_bytes() or less
 };
 
-int mm_lse_parts(int m, int n, int k, int planes);
-size_t mm_split_bytes(int m, int n, int k, int planes);
-
+// Planes: 1 x 1, 2 x 1 or 2 x 2; the product of the second planes is left out.
+int mm_lse_parts(int m, int n, int k, int planes_a, int planes_b);
+size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b);
 // Factors: 16-byte aligned, ld and plane multiples of 8. `g`: 16-byte aligned,
 // ldg and gplane multiples of 8, its rows are written up to the next multiple
 // of 8 columns. `out` 16-byte aligned.

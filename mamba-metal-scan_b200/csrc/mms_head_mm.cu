@@ -18,8 +18,8 @@
 // so the concurrent tiles share one side's panels in L2 and the long side is
 // read from HBM once.
 //
-// float32 factors are three bf16 planes each; a product then runs over the
-// six pairs of planes with i + j <= 2, smallest terms first.
+// float32 factors are two fp16 planes each (see mms_head.cu); a product then
+// runs over the pairs of planes but the two second ones, smallest terms first.
 //
 // The tensor core adds each 16 summed elements to its fp32 sum with truncation,
 // not rounding, so a long sum drifts towards zero by about n 2^-25 of itself
@@ -28,9 +28,18 @@
 // goes to its own tensor memory buffer and the epilogue warps add the parts up
 // in registers, rounding to nearest (`PARTS`).
 //
+// The epilogue turns a warp's 32 rows x 32 columns through shared memory, so
+// that its stores (and the reads of `acc`) cover whole sectors of a row.
+//
+// Tiles that do not fill a last round of the 74 pairs are split along the
+// summed dimension; their partial sums go to a workspace that a second kernel
+// adds up in order.
+//
 // Every wait is bounded. A wait that runs out sets a flag for
 // mms_device_status; all roles leave, the leader waits (bounded) for the
 // copies in flight, and the pair leaves together.
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 #include "mms_common.cuh"
@@ -48,45 +57,50 @@ constexpr int TM = 256, BK = 64, STAGES = 6, THREADS = 384;
 constexpr int HALF = 16384;                                  // bytes of one CTA's a (or b) per stage
 constexpr int GROUP = 16;
 constexpr int PART = 256;                                    // summed elements (of each pair of planes) per part
-constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * HALF + 256;
+constexpr int TURN = 32 * 33;                                // floats of a warp's tile to turn
+constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * HALF + 8 * TURN * 4;
 
 __device__ unsigned int g_mm_timeout;
 
 struct Tiles {
     int mt, nt, bn;         // tiles of rows and columns, columns per tile (a multiple of 64)
-    int splits, kb;         // work items per tile, steps of BK summed elements of each
-    int steps;              // steps of the whole sum
+    int whole, splits;      // tiles done by one item each; items of every other tile
+    int items;
+    int steps, kb;          // steps of BK summed elements, and of them in an item of a split tile
     int part;               // steps per part of a sum
 };
 
-// Columns per tile and splits of the sum: the cheapest by a model of the clocks
-// of a pair. A step of 64 summed elements is the larger of the multiplies
-// (2 clocks a column, at full rate) and the copies of 16 KB + 64 bytes a
-// column into each CTA; an item ends with an epilogue that nothing overlaps
-// on the last one; the waves are those of 74 pairs. Splits pay a write and a
-// read of their partial sums and one more launch.
-Tiles plan(MmKind kind, int m, int n, int k, int planes, size_t split_bytes)
+int passes_of(int planes_a, int planes_b) { return planes_a + planes_b - 1; }
+
+// Columns per tile and splits of the tiles beyond whole rounds: the cheapest
+// by a model of a pair's clocks. A step of 64 summed elements is the larger of
+// the multiplies (2 clocks a column, at full rate) and the copies of 16 KB +
+// 64 bytes a column into each CTA; an item ends with an epilogue that nothing
+// overlaps on the last one. Splits pay a write and a read of their partial
+// sums and one more launch.
+Tiles plan(MmKind kind, int m, int n, int k, int passes, size_t split_bytes)
 {
+    constexpr int PAIRS = N_SM / 2;
     Tiles best{};
     double least = 0;
-    const int passes = planes == 3 ? 6 : 1;
-    const int steps = (k + BK - 1) / BK;
     for (int bn = 256; bn >= 64; bn -= 64) {
         Tiles q;
         q.mt = (m + TM - 1) / TM;
         q.nt = (n + bn - 1) / bn;
         q.bn = bn;
-        q.steps = steps;
-        const long long tiles = (long long)q.mt * q.nt;
+        q.steps = (k + BK - 1) / BK;
+        const int tiles = q.mt * q.nt, rest = tiles % PAIRS;
         const double step = std::max(2.0 * bn, 234 + 0.92 * bn) * passes;
-        for (int s = 1; s <= (kind == MM_OUT ? 74 : 1); ++s) {
-            if (s > 1 && (tiles * s > 74 * 8 || steps < 4 * s || (size_t)s * m * n * 4 > split_bytes)) break;
-            q.kb = (steps + s - 1) / s;
-            q.splits = (steps + q.kb - 1) / q.kb;
+        const double whole = (double)(tiles / PAIRS) * (q.steps * step + 300);
+        for (int s = 1; s <= (kind == MM_OUT && rest ? PAIRS : 1); ++s) {
+            q.kb = (q.steps + s - 1) / s;
+            if (s > 1 && (q.kb < 4 || rest * s > 4 * PAIRS || (size_t)rest * s * TM * bn * 4 > split_bytes)) break;
+            q.splits = (q.steps + q.kb - 1) / q.kb;
             if (q.splits != s) continue;
-            const double waves = (double)((tiles * s + N_SM / 2 - 1) / (N_SM / 2));
-            double cost = waves * (q.kb * step + 300) + 1500 + 10 * bn;
-            if (s > 1) cost += 5000 + (2.0 * s + 1) * m * n * 4 / 3000;
+            q.whole = s > 1 ? tiles - rest : tiles;
+            q.items = q.whole + (tiles - q.whole) * s;
+            double cost = whole + (rest * s + PAIRS - 1) / PAIRS * (q.kb * step + 300) + 1500 + 10 * bn;
+            if (s > 1) cost += 5000 + 2.0 * rest * s * TM * bn * 4 / 3000;
             if (!best.mt || cost < 0.97 * least) {
                 best = q;
                 least = cost;
@@ -94,6 +108,22 @@ Tiles plan(MmKind kind, int m, int n, int k, int planes, size_t split_bytes)
         }
     }
     return best;
+}
+
+// Item t: its tile, and its steps of the sum; `split` its number among the
+// items of split tiles, or -1.
+__device__ __forceinline__ void item_of(const Tiles &q, int t, int &tile, int &split, int &begin, int &end) {
+    if (t < q.whole) {
+        tile = t;
+        split = -1;
+        begin = 0;
+        end = q.steps;
+    } else {
+        split = t - q.whole;
+        tile = q.whole + split / q.splits;
+        begin = split % q.splits * q.kb;
+        end = min(q.steps, begin + q.kb);
+    }
 }
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t limit) {
@@ -113,60 +143,50 @@ __device__ __forceinline__ void tile_of(const Tiles &q, int t, int &mi, int &ni)
     ni = rows_fast ? s : f;
 }
 
-// The pair of planes of pass c (of 6): a's in the low half, smallest products first.
+// The planes of pass c of (planes_a, planes_b): the last pass is (0, 0), before
+// it (0, 1) if b has two, and first (1, 0).
 __device__ __forceinline__ void planes_of(int passes, int c, int &pa, int &pb) {
-    if (passes == 1) {
-        pa = pb = 0;
-        return;
-    }
-    // (1,1) (0,2) (2,0) (0,1) (1,0) (0,0)
-    const int ta = 0x010201, tb = 0x001021;      // digit c
-    pa = ta >> (4 * c) & 15;
-    pb = tb >> (4 * c) & 15;
+    pa = passes > 1 && c == 0;
+    pb = passes > 2 && c == 1;
 }
 
-__device__ __forceinline__ void store_planes(const MmArgs &a, int m, int n, const float (&v)[32]) {
-    float t[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t[i] = v[i];
-    for (int p = 0; p < a.planes; ++p) {
-        __nv_bfloat16 *g = a.g + p * a.gplane + (size_t)m * a.ldg + n;
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            if (n + i >= a.n) break;             // ldg is a multiple of 8: whole pieces fit the row
-            __nv_bfloat16 q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                q[j] = __float2bfloat16_rn(t[i + j]);
-                t[i + j] -= to_f(q[j]);
-            }
-            *reinterpret_cast<uint4 *>(g + i) = *reinterpret_cast<const uint4 *>(q);
-        }
-    }
+__device__ __forceinline__ uint16_t half_bits(bool fp16, float v) {
+    return fp16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+__device__ __forceinline__ float half_value(bool fp16, uint16_t b) {
+    return fp16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
 }
 
-// What follows the product on 32 columns of one row.
+// What follows the product on 32 columns of one row per lane.
 template <int KIND>
 struct Epilogue {
+    float f;                    // the product's factor
     float mx, s;                // MM_LSE: running maximum and sum
     float lse2, rs;             // MM_GRAD
     __device__ __forceinline__ void begin(const MmArgs &a, int m) {
+        const bool in = m < a.m;
+        f = a.c;
+        if (a.row_mul) f *= in ? a.row_mul[m] : 0.f;
+        if (a.mul) f *= *a.mul;
         if (KIND == MM_LSE) {
             mx = -INFINITY;
             s = 0.f;
         }
         if (KIND == MM_GRAD) {
-            lse2 = m < a.m ? a.lse2[m] : 0.f;
-            rs = m < a.m ? a.rs[m] : 0.f;
+            lse2 = in ? a.lse2[m] : 0.f;
+            rs = in ? a.rs[m] : 0.f;
+            if (rs != 0.f && a.g_unit != 0.f) rs = a.g_unit;
         }
     }
-    __device__ __forceinline__ void chunk(const MmArgs &a, int split, int m, int n, float (&v)[32]) {
-        if (n >= a.n) return;
+    // m0: the row of lane 0; rows and columns beyond the product are left out.
+    __device__ __forceinline__ void chunk(const MmArgs &a, const Tiles &q, int split, int m0, int n, int tile_col,
+                                          float (&v)[32], float *turn) {
         if (KIND == MM_LSE) {
+            if (n >= a.n) return;
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                v[i] = n + i < a.n ? v[i] * a.c : -INFINITY;
+                v[i] = n + i < a.n ? v[i] * f : -INFINITY;
                 top = fmaxf(top, v[i]);
             }
             const float now = fmaxf(mx, top), ref = now == -INFINITY ? 0.f : now;
@@ -175,51 +195,105 @@ struct Epilogue {
             for (int i = 0; i < 32; ++i) t += ex2(v[i] - ref);
             mx = now;
             s = t;
-        } else if (KIND == MM_GRAD) {
-            if (m >= a.m) return;
+            return;
+        }
+        if (n >= a.n || m0 >= a.m) return;                     // the whole warp
+        const int lane = threadIdx.x % 32;
+        __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = rs == 0.f ? 0.f : rs * ex2(v[i] * a.c - lse2);
-            store_planes(a, m, n, v);
-        } else {
-            if (m >= a.m) return;
-            const size_t o = ((size_t)split * a.m + m) * a.ldo + n;
-            const int left = min(32, a.n - n);
-            if (a.acc) {
+        for (int i = 0; i < 32; ++i)
+            turn[lane * 33 + i] = KIND == MM_GRAD ? rs == 0.f ? 0.f : rs * ex2(v[i] * f - lse2) : v[i] * f;
+        __syncwarp();
+        const int rows = min(32, a.m - m0), cols = min(32, a.n - n);
+        if (KIND == MM_GRAD) {
+            const int g8 = lane % 4 * 8;                       // 8 columns, 8 rows at a time
+            if (g8 >= cols) return;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i < left) v[i] += a.acc[o + i];
-            }
-            if (a.out_bf16) {
-                __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + o;
-                if (left == 32 && a.ldo % 8 == 0) {
+            for (int r = lane / 4; r < 32; r += 8) {
+                if (r >= rows) break;
+                uint16_t *g = a.g + (size_t)(m0 + r) * a.ldg + n + g8;
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        __nv_bfloat16 q[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) q[j] = __float2bfloat16_rn(v[i + j]);
-                        *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(q);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (i < left) p[i] = __float2bfloat16_rn(v[i]);
+                for (int j = 0; j < 4; ++j) {
+                    const float x = turn[r * 33 + g8 + 2 * j], y = turn[r * 33 + g8 + 2 * j + 1];
+                    const uint16_t p = half_bits(a.fp16, x), o = half_bits(a.fp16, y);
+                    hi[j] = p | (uint32_t)o << 16;
+                    if (a.gplanes > 1)
+                        lo[j] = half_bits(a.fp16, x - half_value(a.fp16, p)) |
+                                (uint32_t)half_bits(a.fp16, y - half_value(a.fp16, o)) << 16;
                 }
-            } else {
-                float *p = static_cast<float *>(a.out) + o;
-                if (left == 32 && a.ldo % 4 == 0) {
+                *reinterpret_cast<uint4 *>(g) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (a.gplanes > 1)
+                    *reinterpret_cast<uint4 *>(g + a.gplane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            return;
+        }
+        if (split >= 0) {                                      // 4 rows of 32 columns at a time
+            float *p = a.split + (size_t)split * TM * q.bn + tile_col;
+            const int c = lane % 8 * 4, tile_row = m0 % TM;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) st4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-                } else {
+            for (int r = lane / 8; r < 32; r += 4) {
+                const float *t = turn + r * 33 + c;
+                st4(p + (size_t)(tile_row + r) * q.bn + c, make_float4(t[0], t[1], t[2], t[3]));
+            }
+            return;
+        }
+        const size_t o = (size_t)m0 * a.n + n;
+        const float *acc = a.acc ? a.acc + o : nullptr;
+        if (a.out_bf16) {
+            __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + o;
+            if (cols == 32 && a.n % 8 == 0) {
+                const int c = lane % 4 * 8;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (i < left) p[i] = v[i];
+                for (int r = lane / 4; r < 32; r += 8) {
+                    if (r >= rows) break;
+                    const size_t e = (size_t)r * a.n + c;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float x = turn[r * 33 + c + 2 * j], y = turn[r * 33 + c + 2 * j + 1];
+                        if (acc) {
+                            x += acc[e + 2 * j];
+                            y += acc[e + 2 * j + 1];
+                        }
+                        w[j] = half_bits(false, x) | (uint32_t)half_bits(false, y) << 16;
+                    }
+                    *reinterpret_cast<uint4 *>(p + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else if (lane < cols) {
+#pragma unroll 4
+                for (int r = 0; r < rows; ++r) {
+                    const size_t e = (size_t)r * a.n + lane;
+                    p[e] = __float2bfloat16_rn(turn[r * 33 + lane] + (acc ? acc[e] : 0.f));
+                }
+            }
+        } else {
+            float *p = static_cast<float *>(a.out) + o;
+            if (cols == 32 && a.n % 4 == 0) {
+                const int c = lane % 8 * 4;
+#pragma unroll
+                for (int r = lane / 8; r < 32; r += 4) {
+                    if (r >= rows) break;
+                    const size_t e = (size_t)r * a.n + c;
+                    const float *t = turn + r * 33 + c;
+                    float4 w = make_float4(t[0], t[1], t[2], t[3]);
+                    if (acc) {
+                        const float4 q4 = *reinterpret_cast<const float4 *>(acc + e);
+                        w = make_float4(w.x + q4.x, w.y + q4.y, w.z + q4.z, w.w + q4.w);
+                    }
+                    st4(p + e, w);
+                }
+            } else if (lane < cols) {
+#pragma unroll 4
+                for (int r = 0; r < rows; ++r) {
+                    const size_t e = (size_t)r * a.n + lane;
+                    p[e] = turn[r * 33 + lane] + (acc ? acc[e] : 0.f);
                 }
             }
         }
     }
     __device__ __forceinline__ void end(const MmArgs &a, int m, int i) {
-        if (KIND == MM_LSE && m < a.m)
-            a.part[(size_t)i * a.m + m] = make_float2(mx, s);
+        if (KIND == MM_LSE && m < a.m) a.part[(size_t)i * a.m + m] = make_float2(mx, s);
     }
 };
 
@@ -257,8 +331,8 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     cluster_sync();
     umma_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2, items = q.mt * q.nt * q.splits;
-    const int passes = a.planes == 3 ? 6 : 1;
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    const int passes = a.a.planes + a.b.planes - 1;
     const int bhalf = q.bn / 2;
     const int bblocks = BT ? (bhalf + 63) / 64 : 0;
 
@@ -268,10 +342,10 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t b_bytes = BT ? bblocks * 8192u : bhalf * 128u;
         int it = 0;
         bool ok = true;
-        for (int t = pair; ok && t < items; t += pairs) {
-            int mi, ni;
-            tile_of(q, t / q.splits, mi, ni);
-            const int k_begin = t % q.splits * q.kb, k_end = min(q.steps, k_begin + q.kb);
+        for (int t = pair; ok && t < q.items; t += pairs) {
+            int tile, split, k_begin, k_end, mi, ni;
+            item_of(q, t, tile, split, k_begin, k_end);
+            tile_of(q, tile, mi, ni);
             const int m0 = mi * TM + rank * 128, n0 = ni * q.bn + rank * bhalf;
             for (int k_first = k_begin; ok && k_first < k_end; k_first += q.part)
             for (int c = 0; ok && c < passes; ++c) {
@@ -306,11 +380,12 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         if (!ok) failed = 1;
     } else if (warp == 9 && lane == 0 && rank == 0) {
-        const uint32_t idesc = umma_idesc(q.bn, AT, BT);
+        const uint32_t idesc = umma_idesc(q.bn, a.fp16, AT, BT);
         int it = 0, use = 0;
         bool ok = true;
-        for (int t = pair; ok && t < items; t += pairs) {
-        const int k_begin = t % q.splits * q.kb, k_end = min(q.steps, k_begin + q.kb);
+        for (int t = pair; ok && t < q.items; t += pairs) {
+        int tile, split, k_begin, k_end;
+        item_of(q, t, tile, split, k_begin, k_end);
         for (int k_first = k_begin; k_first < k_end; k_first += q.part, ++use) {
             const int buf = use & 1;
             if (!wait_bar(tempty + 8 * buf, ((use >> 1) & 1) ^ 1, limit)) {
@@ -349,13 +424,14 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int quad = warp % 4, side = warp / 4;
         const uint32_t lane_base = tmem + ((uint32_t)quad << 21);
         const int cols = q.bn / 2, c0 = side * cols;
+        float *turn = reinterpret_cast<float *>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * 2 * HALF) + warp * TURN;
         int use = 0;
         bool ok = true;
-        for (int t = pair; ok && t < items; t += pairs) {
-            int mi, ni;
-            tile_of(q, t / q.splits, mi, ni);
-            const int split = t % q.splits, k_begin = split * q.kb, k_end = min(q.steps, k_begin + q.kb);
-            const int m = mi * TM + rank * 128 + quad * 32 + lane;
+        for (int t = pair; ok && t < q.items; t += pairs) {
+            int tile, split, k_begin, k_end, mi, ni;
+            item_of(q, t, tile, split, k_begin, k_end);
+            tile_of(q, tile, mi, ni);
+            const int m0 = mi * TM + rank * 128 + quad * 32, m = m0 + lane;
             Epilogue<KIND> ep;
             ep.begin(a, m);
             float2 sum[PARTS ? 4 : 1][16];
@@ -387,7 +463,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(leader_addr(tempty + 8 * buf));
                     }
-                    if (!PARTS && 32 * c < cols) ep.chunk(a, split, m, ni * q.bn + c0 + 32 * c, v);
+                    if (!PARTS && 32 * c < cols) ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c, v, turn);
                 }
             }
             if (!ok) break;
@@ -395,7 +471,8 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     if (32 * c < cols)
-                        ep.chunk(a, split, m, ni * q.bn + c0 + 32 * c, reinterpret_cast<float (&)[32]>(sum[c]));
+                        ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c,
+                                 reinterpret_cast<float (&)[32]>(sum[c]), turn);
             }
             ep.end(a, m, ni * 2 + side);
         }
@@ -414,13 +491,12 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (warp == 9) tmem_free_pair(tmem);
 }
 
-bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor &f, int planes, int rows, int k,
-            int box_rows)
+bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor &f, int rows, int k, int box_rows)
 {
-    const cuuint64_t dim[3] = {(cuuint64_t)(f.t ? rows : k), (cuuint64_t)(f.t ? k : rows), (cuuint64_t)planes};
-    const cuuint64_t stride[2] = {(cuuint64_t)f.ld * 2, (cuuint64_t)(planes == 1 ? f.ld : f.plane) * 2};
+    const cuuint64_t dim[3] = {(cuuint64_t)(f.t ? rows : k), (cuuint64_t)(f.t ? k : rows), (cuuint64_t)f.planes};
+    const cuuint64_t stride[2] = {(cuuint64_t)f.ld * 2, (cuuint64_t)(f.planes == 1 ? f.ld : f.plane) * 2};
     const cuuint32_t box[3] = {64, (cuuint32_t)(f.t ? BK : box_rows), 1}, one[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16 *>(f.p), dim, stride, box, one,
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<uint16_t *>(f.p), dim, stride, box, one,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -428,72 +504,70 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
 template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
-    q.part = PARTS ? PART / BK : q.kb;
+    q.part = PARTS ? PART / BK : q.steps;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
-    if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.planes, a.m, a.k, 128) ||
-        !encode(fn, &mb, a.b, a.planes, a.n, a.k, q.bn / 2))
+    if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
         return cudaErrorInvalidValue;
     constexpr auto kernel = mm_kernel<KIND, AT, BT, PARTS>;
     const cudaError_t e = smem_opt_in<kernel>(SMEM);
     if (e != cudaSuccess) return e;
-    const int pairs = std::min(N_SM / 2, q.mt * q.nt * q.splits);
+    const int pairs = std::min(N_SM / 2, q.items);
     kernel<<<2 * pairs, THREADS, SMEM, stream>>>(ma, mb, a, q, tma_wait_limit(), tma_skip_item());
     return cudaGetLastError();
 }
 
-// out = acc + the splits' partial sums, in order.
+// out = acc + the partial sums of the split tiles, in order; a CTA per 8 rows of a tile.
 template <typename T>
-__global__ void __launch_bounds__(256)
-split_sum_kernel(const float *__restrict__ part, int splits, const float *__restrict__ acc, T *__restrict__ out,
-                 long long n)
+__global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Tiles q)
 {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        float s = acc ? acc[i] : 0.f;
-        for (int k = 0; k < splits; ++k) s += part[k * n + i];
-        out[i] = from_f<T>(s);
+    int mi, ni;
+    tile_of(q, q.whole + blockIdx.y, mi, ni);
+    const float *p = a.split + (size_t)blockIdx.y * q.splits * TM * q.bn;
+    for (int i = threadIdx.x; i < 8 * q.bn; i += 256) {
+        const int r = blockIdx.x * 8 + i / q.bn, c = i % q.bn, m = mi * TM + r, n = ni * q.bn + c;
+        if (m >= a.m || n >= a.n) continue;
+        const size_t o = (size_t)m * a.n + n;
+        float s = a.acc ? a.acc[o] : 0.f;
+#pragma unroll 4
+        for (int k = 0; k < q.splits; ++k) s += p[((size_t)k * TM + r) * q.bn + c];
+        static_cast<T *>(a.out)[o] = from_f<T>(s);
     }
 }
 
 }  // namespace
 
-int mm_lse_parts(int m, int n, int k, int planes) { return 2 * plan(MM_LSE, m, n, k, planes, 0).nt; }
-
-size_t mm_split_bytes(int m, int n, int k, int planes)
+int mm_lse_parts(int m, int n, int k, int planes_a, int planes_b)
 {
-    const Tiles q = plan(MM_OUT, m, n, k, planes, ~(size_t)0);
-    return q.splits > 1 ? (size_t)q.splits * m * n * 4 : 0;
+    return 2 * plan(MM_LSE, m, n, k, passes_of(planes_a, planes_b), 0).nt;
+}
+
+size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b)
+{
+    const Tiles q = plan(MM_OUT, m, n, k, passes_of(planes_a, planes_b), ~(size_t)0);
+    return (size_t)(q.items - q.whole) * TM * q.bn * 4;
 }
 
 cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
-    const Tiles q = plan(kind, a.m, a.n, a.k, a.planes, a.split_bytes);
+    const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
-    const bool parts = q.kb * BK > PART && (kind == MM_LSE || a.planes == 3);
+    const bool parts = (q.whole ? q.steps : q.kb) * BK > PART && (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);
     if (kind == MM_GRAD)
         return parts ? launch<MM_GRAD, false, false, true>(a, q, stream)
                      : launch<MM_GRAD, false, false, false>(a, q, stream);
-    MmArgs o = a;
-    if (q.splits > 1) {
-        o.out = a.split;
-        o.out_bf16 = false;
-        o.acc = nullptr;
-        o.ldo = a.n;
-    }
-    const cudaError_t e = a.a.t ? parts ? launch<MM_OUT, true, true, true>(o, q, stream)
-                                        : launch<MM_OUT, true, true, false>(o, q, stream)
-                                : parts ? launch<MM_OUT, false, true, true>(o, q, stream)
-                                        : launch<MM_OUT, false, true, false>(o, q, stream);
-    if (e != cudaSuccess || q.splits == 1) return e;
-    const long long n = (long long)a.m * a.n;           // out is contiguous (ldo == n)
-    const int grid = (int)std::min<long long>((n + 255) / 256, N_SM * 16);
-    if (a.out_bf16)
-        split_sum_kernel<<<grid, 256, 0, stream>>>(a.split, q.splits, a.acc, static_cast<__nv_bfloat16 *>(a.out), n);
-    else
-        split_sum_kernel<<<grid, 256, 0, stream>>>(a.split, q.splits, a.acc, static_cast<float *>(a.out), n);
+    const cudaError_t e = a.a.t ? parts ? launch<MM_OUT, true, true, true>(a, q, stream)
+                                        : launch<MM_OUT, true, true, false>(a, q, stream)
+                                : parts ? launch<MM_OUT, false, true, true>(a, q, stream)
+                                        : launch<MM_OUT, false, true, false>(a, q, stream);
+    const int rest = q.mt * q.nt - q.whole;
+    if (e != cudaSuccess || !rest) return e;
+    const dim3 grid(TM / 8, rest);
+    if (a.out_bf16) split_sum_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a, q);
+    else split_sum_kernel<float><<<grid, 256, 0, stream>>>(a, q);
     return cudaGetLastError();
 }
 

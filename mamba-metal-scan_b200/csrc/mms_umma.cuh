@@ -38,10 +38,10 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead, uint
            (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// Instruction descriptor: bf16 x bf16 -> fp32, M = 256 over the pair, N = n;
-// at / bt: the factor's rows (not the summed dimension) are contiguous.
-__device__ __forceinline__ uint32_t umma_idesc(int n, bool at, bool bt) {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (at ? 1u << 15 : 0u) | (bt ? 1u << 16 : 0u) |
+// Instruction descriptor: fp16 x fp16 or bf16 x bf16 -> fp32, M = 256 over the
+// pair, N = n; at / bt: the factor's rows (not the summed dimension) are contiguous.
+__device__ __forceinline__ uint32_t umma_idesc(int n, bool fp16, bool at, bool bt) {
+    return 1u << 4 | (fp16 ? 0u : 1u << 7 | 1u << 10) | (at ? 1u << 15 : 0u) | (bt ? 1u << 16 : 0u) |
            (uint32_t)(n >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
 }
 

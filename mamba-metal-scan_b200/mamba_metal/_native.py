@@ -6,6 +6,7 @@ load, every CUDA scan call raises RuntimeError naming the problem.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -246,6 +247,14 @@ def gate_bwd(dout, y, z, d_skip):
                           _ptr(dz), _ptr(dd), _ptr(ws), nb, bt, t_len, d, _stream(y.device))
     _check(rc, "mms_gate_bwd")
     return dy, dz, dd
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """torch.cuda.device(device), or a context that costs nothing where it is current already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}

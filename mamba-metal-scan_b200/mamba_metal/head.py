@@ -66,7 +66,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """(rows, D) with unit column stride, a row stride >= D and a 16-byte aligned base: a view
     of t where its layout allows, else a copy."""
     d = t.shape[-1]
-    t = t.reshape(-1, d)
+    if t.dim() != 2:
+        t = t.reshape(-1, d)
     if t.shape[0] == 1 or d == 1 or t.stride(1) != 1 or t.stride(0) < d:
         t = t.contiguous()
         if t.stride() != (d, 1):                # sizes of one: strides are free, the kernels' are not
@@ -76,7 +77,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _check_head(what, x, weight, others, reduction):
     tensors = (x, weight, *others)
-    if not all(t.is_cuda for t in tensors) or len({t.device for t in tensors}) != 1:
+    if not x.is_cuda or any(t.device != x.device for t in tensors):
         raise RuntimeError(f"{what} runs the CUDA kernels and needs every input on the same CUDA "
                            "device; saw " + ", ".join(str(t.device) for t in tensors))
     if x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
@@ -84,13 +85,18 @@ def _check_head(what, x, weight, others, reduction):
                            f"{weight.dtype}")
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError(f"bad shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    if others[0].is_floating_point() or others[0].dtype == torch.bool:
+    if others[0].dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
         raise RuntimeError(f"{what} takes integer indices; got {others[0].dtype}")
 
 
 def _check_reduction(reduction):
     if reduction not in _native.REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r}; want 'mean', 'sum' or 'none'")
+
+
+def _flat(t, *shape):
+    """t.reshape(shape), without a view where the shape is that already."""
+    return t if t.dim() == len(shape) else t.reshape(shape)
 
 
 def _no_rows(x, shape, reduction):
@@ -106,7 +112,7 @@ class LinearCrossEntropyCUDA(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             loss, lse2, picked, count = _native.linear_ce_fwd(x, weight, target, ignore_index, reduction)
         ctx.save_for_backward(x, weight, target, lse2, picked, count)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
@@ -116,7 +122,7 @@ class LinearCrossEntropyCUDA(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss):
         x, weight, target, lse2, picked, count = ctx.saved_tensors
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             dx, dw = _native.linear_ce_bwd(x, weight, target, ctx.ignore_index, ctx.reduction,
                                            dloss.float().contiguous(), lse2, picked, count,
                                            *ctx.needs_input_grad[:2])
@@ -128,7 +134,7 @@ class LinearDistillationCUDA(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, index, logits, temperature, reduction):
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             loss, lse2, picked, prob, count = _native.linear_kd_fwd(x, weight, index, logits,
                                                                     temperature, reduction)
         ctx.save_for_backward(x, weight, index, lse2, picked, prob, count)
@@ -139,7 +145,7 @@ class LinearDistillationCUDA(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss):
         x, weight, index, lse2, picked, prob, count = ctx.saved_tensors
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             dx, dw = _native.linear_kd_bwd(x, weight, index, ctx.temperature, ctx.reduction,
                                            dloss.float().contiguous(), lse2, picked, prob, count,
                                            *ctx.needs_input_grad[:2])
@@ -174,9 +180,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise ValueError(f"target {tuple(target.shape)} does not match x {tuple(x.shape)}")
     if target.numel() == 0:
         return _no_rows(x, target.shape, reduction)
-    loss = LinearCrossEntropyCUDA.apply(_rows(x), _rows(weight), target.reshape(-1).long().contiguous(),
-                                        int(ignore_index), reduction)
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    x2, w2 = _rows(x), _rows(weight)
+    t = _flat(target, -1).long().contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = LinearCrossEntropyCUDA.apply(x2, w2, t, int(ignore_index), reduction)
+    else:
+        with _native.on_device(x.device):
+            loss = _native.linear_ce_fwd(x2, w2, t, int(ignore_index), reduction)[0]
+    return _flat(loss, *target.shape) if reduction == "none" else loss
 
 
 def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor,
@@ -215,8 +226,12 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: to
     lead = x.shape[:-1]
     if teacher_index.numel() == 0:
         return _no_rows(x, lead, reduction)
-    loss = LinearDistillationCUDA.apply(_rows(x), _rows(weight),
-                                        teacher_index.reshape(-1, k).long().contiguous(),
-                                        teacher_logits.detach().reshape(-1, k).float().contiguous(),
-                                        temperature, reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+    x2, w2 = _rows(x), _rows(weight)
+    index = _flat(teacher_index, -1, k).long().contiguous()
+    logits = _flat(teacher_logits.detach(), -1, k).float().contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = LinearDistillationCUDA.apply(x2, w2, index, logits, temperature, reduction)
+    else:
+        with _native.on_device(x.device):
+            loss = _native.linear_kd_fwd(x2, w2, index, logits, temperature, reduction)[0]
+    return _flat(loss, *lead) if reduction == "none" else loss

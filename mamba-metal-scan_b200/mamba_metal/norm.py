@@ -42,7 +42,7 @@ class ResidualRMSNormCUDA(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, weight, post, gate, scale, eps):
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             h, u, stat = _native.norm_fwd(x, y, gate, weight, post, scale, eps)
         ctx.save_for_backward(x, y, weight, post, gate, scale, stat)
         return h, u
@@ -51,7 +51,7 @@ class ResidualRMSNormCUDA(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, du):
         x, y, weight, post, gate, scale, stat = ctx.saved_tensors
-        with torch.cuda.device(x.device):
+        with _native.on_device(x.device):
             dx, dy, dgate, dweight, dpost, dscale = _native.norm_bwd(
                 x, y, gate, weight, post, scale, stat, dh.contiguous(), du.contiguous())
         return dx, dy, dweight, dpost, dgate, dscale, None
@@ -59,7 +59,8 @@ class ResidualRMSNormCUDA(torch.autograd.Function):
 
 def _strided_rows(t: torch.Tensor) -> torch.Tensor:
     """(rows, D) with unit column stride and one row stride >= D: a view where t's layout allows."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     if t.shape[0] == 1 or t.shape[1] == 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
         if t.stride() != (t.shape[1], 1):
@@ -80,29 +81,38 @@ def residual_rms_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
     """
     if impl not in _IMPLS:
         raise ValueError(f"unknown scan_impl {impl!r}; want 'auto', 'cuda', 'metal' or 'torch'")
-    if not float(eps) >= 0.0:
+    eps = float(eps)
+    if not eps >= 0.0:
         raise ValueError(f"eps must not be negative; got {eps}")
     rows = [t for t in (x, y, gate) if t is not None]
     vectors = [t for t in (weight, post_weight, scale) if t is not None]
-    if x.dim() < 1 or any(t.shape != x.shape for t in rows) \
-            or any(t.shape != x.shape[-1:] for t in vectors):
+    shape = x.shape
+    if x.dim() < 1 or any(t.shape != shape for t in rows) or any(t.shape != shape[-1:] for t in vectors):
         raise ValueError("bad shapes: x, y, gate " + ", ".join(str(tuple(t.shape)) for t in rows)
                          + "; weight, post_weight, scale "
                          + ", ".join(str(tuple(t.shape)) for t in vectors))
     if impl == "torch" or (impl == "auto" and not x.is_cuda):
         return residual_rms_norm_ref(x, y, weight, post_weight, gate, scale, eps)
-    if not x.is_cuda or len({t.device for t in rows + vectors}) != 1:
+    tensors = rows + vectors
+    device, dtype = x.device, x.dtype
+    if not x.is_cuda or any(t.device != device for t in tensors):
         raise RuntimeError(f"scan_impl={impl!r} needs every tensor on the same CUDA device; saw "
-                           + ", ".join(str(t.device) for t in rows + vectors))
-    if x.dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != x.dtype for t in rows + vectors):
+                           + ", ".join(str(t.device) for t in tensors))
+    if dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != dtype for t in tensors):
         raise RuntimeError("residual_rms_norm takes float32 or bfloat16, all tensors alike; got "
-                           + ", ".join(str(t.dtype) for t in rows + vectors))
+                           + ", ".join(str(t.dtype) for t in tensors))
     if x.numel() == 0:
         return residual_rms_norm_ref(x, y, weight, post_weight, gate, scale, eps)
-    d = x.shape[-1]
-    h, u = ResidualRMSNormCUDA.apply(
-        x.reshape(-1, d).contiguous(), y.reshape(-1, d).contiguous(), weight.contiguous(),
-        None if post_weight is None else post_weight.contiguous(),
-        None if gate is None else _strided_rows(gate), None if scale is None else scale.contiguous(),
-        float(eps))
-    return h.reshape(x.shape), u.reshape(x.shape)
+    d = shape[-1]
+    flat = x.dim() == 2                     # no views, so no autograd nodes, where none are needed
+    args = (x.contiguous() if flat else x.reshape(-1, d).contiguous(),
+            y.contiguous() if flat else y.reshape(-1, d).contiguous(), weight.contiguous(),
+            None if post_weight is None else post_weight.contiguous(),
+            None if gate is None else _strided_rows(gate), None if scale is None else scale.contiguous())
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        h, u = ResidualRMSNormCUDA.apply(*args, eps)
+    else:
+        x, y, weight, post_weight, gate, scale = args
+        with _native.on_device(device):
+            h, u, _ = _native.norm_fwd(x, y, gate, weight, post_weight, scale, eps)
+    return (h, u) if flat else (h.view(shape), u.view(shape))

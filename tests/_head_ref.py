@@ -3,8 +3,11 @@
 u(t) is the unit roundoff (half of torch.finfo(t).eps). With g(n) = (n + 16) * 2^-23 the
 kernels' sums of n products err by at most g(n) times the sum of the products' magnitudes:
 every step of an accumulation, rounded or truncated to 24 bits, loses at most 2^-23 of a
-partial sum that those magnitudes bound, and the 16 covers the three bf16 parts of a float32
-factor (left-out terms below 2^-23 a product) and the scaling by log2(e) / temperature.
+partial sum that those magnitudes bound, and the 16 covers the two fp16 parts of a float32
+factor (each factor to 2^-22, the left-out product of the second parts 2^-22: 3 * 2^-22 =
+6 * 2^-23) and the scaling by log2(e) / temperature. The fp16 parts follow a scaling of the
+largest element to at least 2^14 and end at fp16's last step of 2^-24: half of it is 2^-39 of
+the largest element, the absolute term FOOT (for dz, whose scale is 2^14 times 1: 2^-39 of r).
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import math
 import torch
 
 U32 = 2.0 ** -24
+FOOT = 2.0 ** -39
 
 
 def u(dtype) -> float:
@@ -49,6 +53,8 @@ def solve(x, w, index, p, own, counts, tau, reduction, dloss):
     vocab = w.shape[0]
     z = x @ w.t() / tau
     ez = (g(dim) * (x.abs() @ w.abs().t()) / tau).amax(1)            # a bound on any logit of the row
+    if dtype == torch.float32:
+        ez = ez + FOOT * (w.abs().max() * x.abs().sum(1) + x.abs().amax(1) * w.abs().sum(1).max()) / tau
     lse = torch.logsumexp(z, 1)
     log_q = z.gather(1, index) - lse[:, None]
     row = torch.where(counts, tau ** 2 * (own - (p * log_q).sum(1)), 0.0)
@@ -70,13 +76,18 @@ def solve(x, w, index, p, own, counts, tau, reduction, dloss):
     mass = p.sum(1, keepdim=True)
     dz = (q * mass).scatter_add(1, index, -p) * r[:, None]
     # dz: q to within the errors of z and lse; p to 32 roundings; then stored with dtype's
-    # roundoff (float32: three parts, 2^-24)
+    # roundoff (float32: two parts, 2^-22)
     ed = r.abs()[:, None] * (q * (2 * (ez + e_lse)[:, None] + 16 * U32)
                              + torch.zeros_like(q).scatter_add(1, index, (64 + p.shape[1]) * U32 * (p + log_q.abs().clamp(max=1))))
     ed = ed + dz.abs() * (u(dtype) if dtype != torch.float32 else 4 * U32)
+    if dtype == torch.float32:
+        ed = ed + 2 * FOOT * r.abs()[:, None]
     dx, dw = dz @ w, dz.t() @ x
     e_dx = ed @ w.abs() + g(vocab) * (dz.abs() @ w.abs())
     e_dw = ed.t() @ x.abs() + g(rows) * (dz.t().abs() @ x.abs())
+    if dtype == torch.float32:
+        e_dx = e_dx + FOOT * w.abs().max() * dz.abs().sum(1, keepdim=True)
+        e_dw = e_dw + FOOT * (r[:, None] * x).abs().max() * (dz / torch.where(r == 0, 1.0, r)[:, None]).abs().sum(0)[:, None]
     tiny = 1e-36                                                     # float32's range at its foot
     e_dx = e_dx * (1 + u(dtype)) + u(dtype) * dx.abs() + tiny
     e_dw = e_dw * (1 + u(dtype)) + u(dtype) * dw.abs() + tiny
