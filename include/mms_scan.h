@@ -238,12 +238,13 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * reduction: MMS_REDUCE_NONE (loss, dloss: rows floats), MMS_REDUCE_MEAN (over
  * the rows that count; NaN if there is none) or MMS_REDUCE_SUM (one float).
  * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, lse, picked, prob, count
- * are float32, sums are float32. fp32 products run on the tensor cores as
- * three bf16 parts a factor, with every partial product above 2^-24.
+ * are float32, sums are float32. float32 products run on the tensor cores as
+ * two scaled fp16 parts a factor (22 bits; see csrc/mms_head.cu).
  *
- * The forward writes what the backward needs: lse2 (rows), the log-sum-exp of
- * z / temperature in units of log 2; picked (rows, k; k = 1 for the cross
- * entropy), z / temperature at the indices in the same units; prob (rows, k)
+ * The forward writes what the backward needs: lse2 (rows, 2), the log-sum-exp
+ * of z / temperature in units of log 2 as its largest term and the rest;
+ * logq2 (rows, k; k = 1 for the cross entropy), log2 of q at the indices;
+ * prob (rows, k)
  * = p; count (1) = the rows that count. dx (rows, dim) and dw (vocab, dim)
  * are contiguous; either may be NULL and is then not computed.
  *
@@ -262,23 +263,23 @@ size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long lon
                                long long ldw, int backward);
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction, float *loss,
-                      float *lse2, float *picked, float *count, void *workspace,
+                      float *lse2, float *logq2, float *count, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
                       void *stream);
 int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction,
-                      const float *dloss, const float *lse2, const float *picked,
+                      const float *dloss, const float *lse2, const float *logq2,
                       const float *count, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
                       void *stream);
 int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, const float *logits, int k, float temperature,
-                      int reduction, float *loss, float *lse2, float *picked, float *prob,
+                      int reduction, float *loss, float *lse2, float *logq2, float *prob,
                       float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
                       int dim, int dtype, void *stream);
 int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, int k, float temperature, int reduction,
-                      const float *dloss, const float *lse2, const float *picked,
+                      const float *dloss, const float *lse2, const float *logq2,
                       const float *prob, const float *count, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
                       void *stream);

@@ -114,9 +114,9 @@ mms::HeadArgs head_args(const void *x, long long ldx, const void *w, long long l
 
 int head_fwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
 {
-    if (!a.index || !a.loss || !a.lse2 || !a.picked || !a.count) return MMS_ERR_INVALID_ARG;
+    if (!a.index || !a.loss || !a.lse2 || !a.logq2 || !a.count) return MMS_ERR_INVALID_ARG;
     if (!aligned(a.index, 8) || !aligned(a.logits, 4) || !aligned(a.loss, 4) ||
-        !aligned(a.lse2, 4) || !aligned(a.picked, 4) || !aligned(a.prob, 4) || !aligned(a.count, 4))
+        !aligned(a.lse2, 8) || !aligned(a.logq2, 4) || !aligned(a.prob, 4) || !aligned(a.count, 4))
         return MMS_ERR_MISALIGNED;
     if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
                                                                     a.ldx, a.ldw, false))
@@ -127,9 +127,9 @@ int head_fwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
 
 int head_bwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
 {
-    if (!a.index || !a.dloss || !a.c_lse2 || !a.c_picked || !a.c_count) return MMS_ERR_INVALID_ARG;
-    if (!aligned(a.index, 8) || !aligned(a.dloss, 4) || !aligned(a.c_lse2, 4) ||
-        !aligned(a.c_picked, 4) || !aligned(a.c_prob, 4) || !aligned(a.c_count, 4) ||
+    if (!a.index || !a.dloss || !a.c_lse2 || !a.c_logq2 || !a.c_count) return MMS_ERR_INVALID_ARG;
+    if (!aligned(a.index, 8) || !aligned(a.dloss, 4) || !aligned(a.c_lse2, 8) ||
+        !aligned(a.c_logq2, 4) || !aligned(a.c_prob, 4) || !aligned(a.c_count, 4) ||
         !aligned(a.dx, 16) || !aligned(a.dw, 16))
         return MMS_ERR_MISALIGNED;
     if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
@@ -325,20 +325,20 @@ size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long lon
 
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction, float *loss,
-                      float *lse2, float *picked, float *count, void *workspace,
+                      float *lse2, float *logq2, float *count, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
 {
     const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, 1, 1.f, dtype, reduction);
     if (rc) return rc;
     mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
     a.ignore_index = ignore_index;
-    a.loss = loss; a.lse2 = lse2; a.picked = picked; a.count = count;
+    a.loss = loss; a.lse2 = lse2; a.logq2 = logq2; a.count = count;
     return head_fwd(a, workspace_bytes, stream);
 }
 
 int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction,
-                      const float *dloss, const float *lse2, const float *picked,
+                      const float *dloss, const float *lse2, const float *logq2,
                       const float *count, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
 {
@@ -346,14 +346,14 @@ int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw
     if (rc) return rc;
     mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
     a.ignore_index = ignore_index;
-    a.dloss = dloss; a.c_lse2 = lse2; a.c_picked = picked; a.c_count = count;
+    a.dloss = dloss; a.c_lse2 = lse2; a.c_logq2 = logq2; a.c_count = count;
     a.dx = dx; a.dw = dw;
     return head_bwd(a, workspace_bytes, stream);
 }
 
 int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, const float *logits, int k, float temperature,
-                      int reduction, float *loss, float *lse2, float *picked, float *prob,
+                      int reduction, float *loss, float *lse2, float *logq2, float *prob,
                       float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
                       int dim, int dtype, void *stream)
 {
@@ -362,13 +362,13 @@ int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw
     if (!logits || !prob) return MMS_ERR_INVALID_ARG;
     mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
     a.kd = true; a.tau = temperature; a.logits = logits;
-    a.loss = loss; a.lse2 = lse2; a.picked = picked; a.prob = prob; a.count = count;
+    a.loss = loss; a.lse2 = lse2; a.logq2 = logq2; a.prob = prob; a.count = count;
     return head_fwd(a, workspace_bytes, stream);
 }
 
 int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, int k, float temperature, int reduction,
-                      const float *dloss, const float *lse2, const float *picked,
+                      const float *dloss, const float *lse2, const float *logq2,
                       const float *prob, const float *count, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
 {
@@ -377,7 +377,7 @@ int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw
     if (!prob) return MMS_ERR_INVALID_ARG;
     mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
     a.kd = true; a.tau = temperature;
-    a.dloss = dloss; a.c_lse2 = lse2; a.c_picked = picked; a.c_prob = prob; a.c_count = count;
+    a.dloss = dloss; a.c_lse2 = lse2; a.c_logq2 = logq2; a.c_prob = prob; a.c_count = count;
     a.dx = dx; a.dw = dw;
     return head_bwd(a, workspace_bytes, stream);
 }

@@ -3,31 +3,39 @@
 //
 // With z = x w^T (rows x vocab) and c = log2(e) / tau (tau = 1 for the cross
 // entropy), in units of log 2:
-//     lse2[m]   = log2 sum_v 2^(c z[m, v])
-//     picked[m, j] = c z[m, index[m, j]]
-//     CE  loss  = ln2 (lse2 - picked)
-//     KD  loss  = tau^2 sum_j p_j (log p_j - ln2 (picked_j - lse2))
+//     lse2[m]   = (top, log2 sum_v 2^(c z[m, v] - top)),  top = max_v c z[m, v]
+//     logq2[m, j] = c z[m, index[m, j]] - lse2, the log-probability there
+//     CE  loss  = -ln2 logq2
+//     KD  loss  = tau^2 sum_j p_j (log p_j - ln2 logq2_j)
 // and for an upstream factor r[m] (dloss, times 1 / count for a mean, times
 // tau for the distillation; 0 for a row that is left out):
 //     dz[m, v]  = r (2^(c z - lse2) - sum of p_j with index_j = v)
 //     dx = dz w,   dw = dz^T x
+// The two halves of lse2 stay apart: their sum would round at the magnitude of
+// the logits, where the difference to a likely entry's logit is exact.
 // z is computed once forward (2 rows vocab dim flops) and again backward, in
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
 //
-// Forward:   pick_kernel: the dot products at the indices; products (MM_LSE)
-//            -> one (max, sum) per row and half tile, joined by lse_kernel;
-//            a loss kernel; one block adds the rows up.
+// Forward:   products (MM_LSE) -> one (max, sum) per row and half tile, joined
+//            by lse_kernel. The cross entropy's target logit is the product's
+//            own value, so that it cancels against lse2 where the target has
+//            nearly all the probability; the distillation's are dot products
+//            of their own (pick_kernel). Then a loss kernel; one block adds the
+//            rows up. Up to FEW_FWD rows (few_kernel) w is read once, as it
+//            is, by the CUDA cores: nothing is staged.
 // Backward:  rows_kernel: r; x staged with the left-out rows as zeros (so that
 //            nothing in them, NaN included, reaches dw); per piece: product
-//            MM_GRAD, sparse_kernel sets dz at the indices (from picked, in
+//            MM_GRAD, sparse_kernel sets dz at the indices (from logq2, in
 //            fp32, as expm1(log q) + 1 - p: no cancellation when a target's
 //            probability is near 1), then MM_OUT twice.
 //
-// bf16: dz is stored as r (q - p) in bf16, one plane. Its rounding (2^-8 a
-// value at most) averages out over a sum of many; with up to FEW_ROWS rows one
-// value can dominate a whole gradient, so a second plane holds the rest there
-// (one more pass of two products that such sizes do not feel).
+// bf16: dz is stored in bf16, one plane: without r where it is the same for
+// all rows (mean, sum: q - p is often close to -1, which bf16 holds better
+// than -1 / rows), as r (q - p) where it is not. The rounding (2^-8 a value at
+// most) averages out over a sum of many; with up to FEW_ROWS rows one value
+// can dominate a whole gradient, so a second plane holds the rest there (one
+// more pass of two products that such sizes do not feel).
 //
 // float32: factors are split into two fp16 planes, 22 bits, after a scaling by
 // a power of two that brings the largest element into [2^14, 2^15); the
@@ -55,6 +63,8 @@ namespace {
 constexpr float LN2 = 0.6931471805599453f;
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // bound on one staged or dz piece
 constexpr int FEW_ROWS = 256;
+constexpr int FEW_FWD = 8;
+constexpr int FEW_BLOCKS = 148 * 4;
 constexpr float DZ_UNIT = 16384.f;                  // float32: the scale of dz's planes
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -82,6 +92,7 @@ struct Layout {
 };
 
 struct FwdLayout : Layout {
+    bool few;
     size_t part, rowloss;
 };
 
@@ -107,12 +118,13 @@ size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
 FwdLayout fwd_layout(int rows, int vocab, int dim, bool bf16, long long ldx, long long ldw)
 {
     FwdLayout l;
-    l.planes = bf16 ? 1 : 2;
-    l.stage_x = !bf16 || ldx % 8;
-    l.stage_w = !bf16 || ldw % 8;
+    l.few = rows <= FEW_FWD;
+    l.planes = bf16 || l.few ? 1 : 2;
+    l.stage_x = !l.few && (!bf16 || ldx % 8);
+    l.stage_w = !l.few && (!bf16 || ldw % 8);
     size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * sizeof(float2) / 32 + 1);
-    const int parts = std::max(mm_lse_parts(rows, l.piece, dim, l.planes, l.planes),
-                               mm_lse_parts(rows, l.last, dim, l.planes, l.planes));
+    const int parts = l.few ? FEW_BLOCKS : std::max(mm_lse_parts(rows, l.piece, dim, l.planes, l.planes),
+                                                    mm_lse_parts(rows, l.last, dim, l.planes, l.planes));
     l.part = o; o += up256((size_t)(parts + 1) * rows * sizeof(float2));
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
     l.total = o;
@@ -235,6 +247,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
                 for (int j = 0; j < 2; ++j) {
                     float x = v[2 * i + j];
                     if (KIND == ST_COPY) {
+                        if (rs != rs) x = rs;               // a bad index: dw shows it
                         h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
                     } else {
                         x = by(KIND == ST_WHOLE ? rs * x : x);
@@ -297,21 +310,20 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// picked[m, j] = c * (x[m] . w[index[m, j]]), a warp each; NaN for an index
-// outside the vocabulary, 0 for an entry that is left out.
+// The distillation's logq2[m, j] = c * (x[m] . w[index[m, j]]), a warp each;
+// NaN for an index outside the vocabulary, 0 for an entry that is left out.
 template <typename T>
 __global__ void __launch_bounds__(256)
 pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw,
-            const int64_t *__restrict__ index, bool kd, int64_t ignore, int k, float c,
-            float *__restrict__ picked, long long n, int vocab, int dim)
+            const int64_t *__restrict__ index, int k, float c, float *__restrict__ logq2, long long n, int vocab, int dim)
 {
     const long long e = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (e >= n) return;
     const int64_t v = index[e];
     float s = 0.f;
-    if (kd ? v < 0 : v == ignore) {
-    } else if (v < 0 || v >= vocab) {
+    if (v < 0) {
+    } else if (v >= vocab) {
         s = __int_as_float(0x7fc00000);
     } else {
         const T *xr = x + e / k * ldx, *wr = w + v * ldw;
@@ -325,7 +337,7 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
         }
         s = warp_sum(s) * c;
     }
-    if (lane == 0) picked[e] = s;
+    if (lane == 0) logq2[e] = s;
 }
 
 // (max, sum) pairs join to the pair of both; a NaN in either sum stays.
@@ -335,18 +347,95 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
 }
 
+// The log-sum-exp of up to FEW_FWD rows over a share of w's rows per CTA: a
+// warp takes 4 rows of w at a time, its lanes 8 columns each, against R rows
+// of x (L1 holds them). Bound by reading w once.
+template <typename T, int R>
+__global__ void __launch_bounds__(256)
+few_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, float c, int rows,
+           int vocab, int dim, const int64_t *__restrict__ target, float *__restrict__ logq2,
+           float2 *__restrict__ part)
+{
+    __shared__ float2 sh[8][R];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    float2 run[R];
+    long long at[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        run[r] = make_float2(-INFINITY, 0.f);
+        at[r] = target && r < rows ? target[r] : -1;
+    }
+    for (int v = (blockIdx.x * 8 + warp) * 4; v < vocab; v += gridDim.x * 32) {
+        float s[R][4] = {};
+        const T *wr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wr[i] = w + (size_t)min(v + i, vocab - 1) * ldw;
+        for (int k = lane * 8; k < dim; k += 256) {
+            float q[4][8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load8(wr[i], k, dim, q[i]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float p[8];
+                load8(x + (size_t)min(r, rows - 1) * ldx, k, dim, p);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s[r][i] = fmaf(p[j], q[i][j], s[r][i]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float m = run[r].x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[r][i] = v + i < vocab ? warp_sum(s[r][i]) : -INFINITY;
+                if (v + i == at[r] && lane == 0) logq2[r] = s[r][i] * c;
+                m = fmaxf(m, s[r][i] * c);
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            float t = run[r].y * ex2(run[r].x - ref);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t += ex2(fmaf(s[r][i], c, -ref));
+            run[r] = make_float2(m, t);
+        }
+    }
+    if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r) sh[warp][r] = run[r];
+    __syncthreads();
+    if (threadIdx.x < rows) {
+        float2 t = sh[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t = join(t, sh[i][threadIdx.x]);
+        part[(size_t)blockIdx.x * rows + threadIdx.x] = t;
+    }
+}
+
+template <typename T>
+void launch_few(const HeadArgs &a, float c, float2 *part, int blocks, cudaStream_t s)
+{
+    const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
+    const int64_t *t = a.kd ? nullptr : a.index;
+    if (a.rows == 1) few_kernel<T, 1><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
+    else if (a.rows == 2) few_kernel<T, 2><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
+    else if (a.rows <= 4) few_kernel<T, 4><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
+    else few_kernel<T, 8><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
+}
+
 // One row a lane, 32 threads a row over the tiles. Parts 1..ntiles, and part
 // 0 (the pieces before) unless `first`. Writes part 0, or in the last piece
-// lse2 and the cross entropy's row loss.
+// lse2 and, from the target's logit in logq2, the cross entropy's row loss.
 __global__ void __launch_bounds__(1024)
-lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float *__restrict__ lse2,
-           const int64_t *__restrict__ target, int64_t ignore, const float *__restrict__ picked,
+lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__restrict__ lse2,
+           const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
            float *__restrict__ loss)
 {
     __shared__ float2 sh[32][33];
     const int m = blockIdx.x * 32 + threadIdx.x;
     float2 v = make_float2(-INFINITY, 0.f);
     if (m < rows)
+#pragma unroll 4
         for (int t = threadIdx.y + (first ? 1 : 0); t <= ntiles; t += 32)
             v = join(v, part[(size_t)t * rows + m]);
     sh[threadIdx.y][threadIdx.x] = v;
@@ -362,22 +451,28 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float *__r
         part[r] = v;
         return;
     }
-    const float l = v.x + log2f(v.y);
-    lse2[r] = l;
-    if (target) loss[r] = target[r] == ignore ? 0.f : LN2 * (l - picked[r]);
+    v.y = log2f(v.y);
+    lse2[r] = v;
+    if (!target) return;
+    const int64_t t = target[r];
+    float l = 0.f;
+    if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : (logq2[r] - v.x) - v.y;
+    logq2[r] = l;
+    loss[r] = -LN2 * l;
 }
 
 // Distillation's row loss, a warp a row: the teacher's softmax over its
 // entries, kept as prob, against the student's log-probabilities.
 __global__ void __launch_bounds__(256)
 kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, float tau,
-          const float *__restrict__ lse2, const float *__restrict__ picked,
+          const float2 *__restrict__ lse2, float *__restrict__ logq2,
           float *__restrict__ prob, float *__restrict__ loss, int rows)
 {
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (m >= rows) return;
     const size_t o = (size_t)m * k;
-    const float inv = 1.f / tau, l2 = lse2[m];
+    const float inv = 1.f / tau;
+    const float2 l2 = lse2[m];
     float top = -INFINITY;
     for (int j = lane; j < k; j += 32)
         if (index[o + j] >= 0) top = fmaxf(top, logits[o + j]);
@@ -392,10 +487,12 @@ kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, i
     float acc = 0.f;
     for (int j = lane; j < k; j += 32) {
         float p = 0.f;
+        const float lq = (logq2[o + j] - l2.x) - l2.y;
+        logq2[o + j] = lq;
         if (some && index[o + j] >= 0) {
             const float t = (logits[o + j] - top) * inv;
             p = expf(t) * over;
-            if (p != 0.f) acc += p * ((t - log_sum) - LN2 * (picked[o + j] - l2));
+            if (p != 0.f) acc += p * ((t - log_sum) - LN2 * lq);
         }
         prob[o + j] = p;
     }
@@ -441,20 +538,22 @@ total_kernel(const float *__restrict__ rowloss, const int64_t *__restrict__ inde
 }
 
 // rs[m]: the upstream factor of row m's dz; NaN where an index that counts
-// lies outside the vocabulary (picked is NaN there).
+// lies outside the vocabulary (logq2 is NaN there). *whole: the factor of all
+// rows that count, where it is the same.
 __global__ void rows_kernel(const float *__restrict__ dloss, const float *__restrict__ count,
                             const int64_t *__restrict__ index, const float *__restrict__ prob,
-                            const float *__restrict__ picked, int k, int64_t ignore, int reduction,
-                            float tau, float *__restrict__ rs, int rows)
+                            const float *__restrict__ logq2, int k, int64_t ignore, int reduction,
+                            float tau, float *__restrict__ rs, float *whole, int rows)
 {
     const int m = blockIdx.x * blockDim.x + threadIdx.x;
     if (m >= rows) return;
     float r = dloss[reduction == MMS_REDUCE_NONE ? m : 0] * tau;
     if (reduction == MMS_REDUCE_MEAN) r /= *count;
+    if (m == 0 && whole) *whole = r;
     if (!row_counts(index, prob, k, ignore, m)) r = 0.f;
     if (r != 0.f)
         for (int j = 0; j < k; ++j) {
-            const float z = picked[(size_t)m * k + j];
+            const float z = logq2[(size_t)m * k + j];
             if (z != z && !(prob && prob[(size_t)m * k + j] == 0.f)) r = z;
         }
     rs[m] = r;
@@ -464,9 +563,8 @@ __global__ void rows_kernel(const float *__restrict__ dloss, const float *__rest
 // place of r if it is not 0.
 __global__ void __launch_bounds__(256)
 sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
-              const float *__restrict__ picked, const float *__restrict__ lse2,
-              const float *__restrict__ rs, float unit, int k, long long n, int v0, int v1,
-              uint16_t *__restrict__ g, long long ldg, long long gplane, int planes)
+              const float *__restrict__ logq2, const float *__restrict__ rs, float unit, int k, long long n, int v0, int v1,
+              uint16_t *__restrict__ g, long long ldg, long long gplane, int planes, bool fp16)
 {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= n) return;
@@ -475,16 +573,22 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
     const long long m = e / k;
     const float r = rs[m];
     if (r == 0.f) return;                               // dz is 0 there already
-    float p = 1.f;
-    if (prob) {                                         // an index may occur twice
+    uint16_t *o = g + m * ldg + (v - v0);
+    float p = 1.f, d = expm1f(LN2 * logq2[e]);
+    if (prob) {                                         // an index may occur twice: the first one writes
         p = 0.f;
-        for (int j = 0; j < k; ++j)
-            if (index[m * k + j] == v) p += prob[m * k + j];
+        for (int j = 0; j < k; ++j) {
+            const long long f = m * k + j;
+            if (index[f] != v) continue;
+            if (f < e) return;
+            p += prob[f];
+        }
+        // float32: q as the product's own value, which is what the row's other entries add up to 1 with
+        if (fp16) d = (__half2float(__ushort_as_half(o[0])) + __half2float(__ushort_as_half(o[gplane]))) / unit - 1.f;
     }
-    float d = (unit != 0.f ? unit : r) * (expm1f(LN2 * (picked[e] - lse2[m])) + (1.f - p));
-    for (int q = 0; q < planes; ++q) {
-        uint16_t *o = g + q * gplane + m * ldg + (v - v0);
-        if (unit != 0.f) {
+    d = (unit != 0.f ? unit : r) * (d + (1.f - p));
+    for (int q = 0; q < planes; ++q, o += gplane) {
+        if (fp16) {
             const __half t = __float2half_rn(d);
             *o = __half_as_ushort(t);
             d -= __half2float(t);
@@ -551,20 +655,30 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     const float c = MMS_LOG2E / a.tau;
     float2 *part = reinterpret_cast<float2 *>(fl(a.workspace, l.part));
     float *rowloss = a.reduction == MMS_REDUCE_NONE ? a.loss : fl(a.workspace, l.rowloss);
-    const long long n = (long long)a.rows * a.k;
-    const int pick_grid = ceil_div(n, 8);
-    if (a.bf16)
-        pick_kernel<__nv_bfloat16><<<pick_grid, 256, 0, stream>>>(
-            static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w),
-            a.ldw, a.index, a.kd, a.ignore_index, a.k, c, a.picked, n, a.vocab, a.dim);
-    else
-        pick_kernel<float><<<pick_grid, 256, 0, stream>>>(
-            static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index,
-            a.kd, a.ignore_index, a.k, c, a.picked, n, a.vocab, a.dim);
+    if (a.kd) {
+        const long long n = (long long)a.rows * a.k;
+        if (a.bf16)
+            pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
+                static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w), a.ldw,
+                a.index, a.k, c, a.logq2, n, a.vocab, a.dim);
+        else
+            pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
+                static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index, a.k, c,
+                a.logq2, n, a.vocab, a.dim);
+    }
     cudaError_t e;
-    if (l.planes > 1 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
-    const Factor x = x_factor(a, l, nullptr, stream);
-    for (int v0 = 0; v0 < a.vocab; v0 += l.piece) {
+    const int64_t *target = a.kd ? nullptr : a.index;
+    if (l.few) {
+        const int blocks = std::min(ceil_div(a.vocab, 32), FEW_BLOCKS);
+        if (a.bf16) launch_few<__nv_bfloat16>(a, c, part + a.rows, blocks, stream);
+        else launch_few<float>(a, c, part + a.rows, blocks, stream);
+        lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows,
+                                                  reinterpret_cast<float2 *>(a.lse2), target,
+                                                  a.ignore_index, a.vocab, a.logq2, rowloss);
+    }
+    if (!l.few && l.planes > 1 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
+    const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, stream);
+    for (int v0 = l.few ? a.vocab : 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
         MmArgs mm{};
         mm.a = x;
@@ -576,14 +690,18 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
             mm.mul = fl(a.workspace, l.muls);
         }
         mm.part = part + a.rows;                        // part 0: the pieces before
+        mm.target = target;
+        mm.target_first = v0;
+        mm.logit_at = a.logq2;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
             part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
-            a.lse2, a.kd ? nullptr : a.index, a.ignore_index, a.picked, rowloss);
+            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rowloss);
     }
     if (a.kd)
-        kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau, a.lse2,
-                                                          a.picked, a.prob, rowloss, a.rows);
+        kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau,
+                                                          reinterpret_cast<const float2 *>(a.lse2),
+                                                          a.logq2, a.prob, rowloss, a.rows);
     total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, a.kd ? a.prob : nullptr, a.k,
                                          a.ignore_index, a.rows, a.reduction, a.loss, a.count);
     return cudaGetLastError();
@@ -594,10 +712,13 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     const BwdLayout l = bwd_layout(a.rows, a.vocab, a.dim, a.bf16, a.ldw);
     const float c = MMS_LOG2E / a.tau;
     const float *prob = a.kd ? a.c_prob : nullptr;
+    // bf16, all rows alike: dz without r, which comes in with the products' factors
+    const bool uniform = a.bf16 && a.reduction != MMS_REDUCE_NONE;
     float *rs = fl(a.workspace, l.rs), *acc = fl(a.workspace, l.dxacc);
     rows_kernel<<<ceil_div(a.rows, 256), 256, 0, stream>>>(a.dloss, a.c_count, a.index, prob,
-                                                           a.c_picked, a.k, a.ignore_index,
-                                                           a.reduction, a.tau, rs, a.rows);
+                                                           a.c_logq2, a.k, a.ignore_index,
+                                                           a.reduction, a.tau, rs,
+                                                           uniform ? fl(a.workspace, l.muls) + 1 : nullptr, a.rows);
     cudaError_t e;
     const bool f32 = l.planes > 1;
     float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
@@ -612,7 +733,7 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     }
     xr.t = true;
     const long long n = (long long)a.rows * a.k, gplane = (long long)a.rows * l.ldg;
-    const float unit = f32 ? DZ_UNIT : 0.f;
+    const float unit = f32 ? DZ_UNIT : uniform ? 1.f : 0.f;
     uint16_t *g = u16(a.workspace, l.g);
     for (int v0 = 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
@@ -626,11 +747,11 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             mm.row_mul = row_mul;
             mm.mul = muls;
         }
-        mm.lse2 = a.c_lse2; mm.rs = rs; mm.g_unit = unit;
+        mm.lse2 = reinterpret_cast<const float2 *>(a.c_lse2); mm.rs = rs; mm.g_unit = unit;
         mm.g = g; mm.ldg = l.ldg; mm.gplane = gplane; mm.gplanes = l.gplanes;
         if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) return e;
-        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_picked, a.c_lse2, rs, unit,
-                                                            a.k, n, v0, v0 + nv, g, l.ldg, gplane, l.gplanes);
+        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_logq2, rs, unit, a.k, n, v0,
+                                                            v0 + nv, g, l.ldg, gplane, l.gplanes, f32);
         MmArgs out{};
         out.fp16 = f32;
         out.c = f32 ? 1.f / DZ_UNIT : 1.f;
@@ -642,7 +763,7 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             out.b = mm.b;
             out.b.t = true;
             out.m = a.rows; out.k = nv;
-            out.row_mul = f32 ? rs : nullptr;
+            out.row_mul = f32 || uniform ? rs : nullptr;
             out.mul = f32 ? muls : nullptr;
             out.acc = first ? nullptr : acc;
             out.out = last ? a.dx : acc;
@@ -654,7 +775,7 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             out.b = xr;
             out.m = nv; out.k = a.rows;
             out.row_mul = nullptr;
-            out.mul = f32 ? muls + 1 : nullptr;
+            out.mul = f32 || uniform ? muls + 1 : nullptr;
             out.acc = nullptr;
             out.out = static_cast<char *>(a.dw) + (size_t)v0 * a.dim * (a.bf16 ? 2 : 4);
             out.out_bf16 = a.bf16;

@@ -23,7 +23,7 @@ struct Factor {
 //   MM_LSE    each row's log-sum-exp over parts of the columns:
 //             part[i * m + row] = (max, sum of 2^(s - max)), in units of log 2,
 //             i < mm_lse_parts()
-//   MM_GRAD   g[m, n] = r 2^(s - lse2[m]) as planes of 16-bit floats; 0 where
+//   MM_GRAD   g[m, n] = r 2^(s - lse2[m].x - lse2[m].y) as planes of 16-bit floats; 0 where
 //             rs[m] is 0; r = rs[m], or the constant g_unit if that is not 0
 //   MM_OUT    out[m, n] = s (+ acc[m, n]), float32 or bf16
 enum MmKind { MM_LSE, MM_GRAD, MM_OUT };
@@ -36,7 +36,11 @@ struct MmArgs {
     float c;
     const float *row_mul, *mul;
     float2 *part;               // MM_LSE
-    const float *lse2, *rs;     // MM_GRAD
+    const int64_t *target;      // MM_LSE: where target[m] - target_first is a column,
+    long long target_first;     //         logit_at[m] = s there; may be null
+    float *logit_at;
+    const float2 *lse2;         // MM_GRAD: (top, log2 of the sum of 2^(s - top))
+    const float *rs;            // MM_GRAD
     float g_unit;               // MM_GRAD
     uint16_t *g;                // MM_GRAD
     long long ldg, gplane;      // MM_GRAD
@@ -73,8 +77,8 @@ struct HeadArgs {
     bool kd;
     float tau;
     int reduction;
-    float *loss, *lse2, *picked, *prob, *count;     // forward outputs
-    const float *dloss, *c_lse2, *c_picked, *c_prob, *c_count;   // backward inputs
+    float *loss, *lse2, *logq2, *prob, *count;     // forward outputs
+    const float *dloss, *c_lse2, *c_logq2, *c_prob, *c_count;   // backward inputs
     void *dx, *dw;
     void *workspace;
 };

@@ -26,7 +26,9 @@
 // over n additions (measured: 1.1e-5 at 8192 elements). Where the result
 // stays float32 the sum is therefore cut into parts of PART elements: each
 // goes to its own tensor memory buffer and the epilogue warps add the parts up
-// in registers, rounding to nearest (`PARTS`).
+// in registers, rounding to nearest (`PARTS`). Parts of 512 cost nothing
+// beside the multiplies; of 256, 25 % of the log-sum-exp at 8192 x 131072 x
+// 2048 (4.15 ms against 3.31); of 128, 80 %.
 //
 // The epilogue turns a warp's 32 rows x 32 columns through shared memory, so
 // that its stores (and the reads of `acc`) cover whole sectors of a row.
@@ -56,14 +58,15 @@ namespace {
 constexpr int TM = 256, BK = 64, STAGES = 6, THREADS = 384;
 constexpr int HALF = 16384;                                  // bytes of one CTA's a (or b) per stage
 constexpr int GROUP = 16;
-constexpr int PART = 256;                                    // summed elements (of each pair of planes) per part
+constexpr int PART = 512;                                    // summed elements (of each pair of planes) per part
 constexpr int TURN = 32 * 33;                                // floats of a warp's tile to turn
 constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * HALF + 8 * TURN * 4;
 
 __device__ unsigned int g_mm_timeout;
 
 struct Tiles {
-    int mt, nt, bn;         // tiles of rows and columns, columns per tile (a multiple of 64)
+    int mt, nt, bn;         // tiles of rows and columns, columns per tile (a multiple of 32)
+    int half;               // of them, columns of the first four epilogue warps (at most 128)
     int whole, splits;      // tiles done by one item each; items of every other tile
     int items;
     int steps, kb;          // steps of BK summed elements, and of them in an item of a split tile
@@ -83,11 +86,12 @@ Tiles plan(MmKind kind, int m, int n, int k, int passes, size_t split_bytes)
     constexpr int PAIRS = N_SM / 2;
     Tiles best{};
     double least = 0;
-    for (int bn = 256; bn >= 64; bn -= 64) {
+    for (int bn = 256; bn >= 64; bn -= 32) {
         Tiles q;
         q.mt = (m + TM - 1) / TM;
         q.nt = (n + bn - 1) / bn;
         q.bn = bn;
+        q.half = bn > 128 ? 128 : (bn / 2 + 31) / 32 * 32;
         q.steps = (k + BK - 1) / BK;
         const int tiles = q.mt * q.nt, rest = tiles % PAIRS;
         const double step = std::max(2.0 * bn, 234 + 0.92 * bn) * passes;
@@ -162,7 +166,9 @@ template <int KIND>
 struct Epilogue {
     float f;                    // the product's factor
     float mx, s;                // MM_LSE: running maximum and sum
-    float lse2, rs;             // MM_GRAD
+    int at;                     // MM_LSE: the target's column, or -1
+    float2 lse2;                // MM_GRAD
+    float rs;
     __device__ __forceinline__ void begin(const MmArgs &a, int m) {
         const bool in = m < a.m;
         f = a.c;
@@ -171,9 +177,14 @@ struct Epilogue {
         if (KIND == MM_LSE) {
             mx = -INFINITY;
             s = 0.f;
+            at = -1;
+            if (a.target && in) {
+                const long long t = a.target[m] - a.target_first;
+                if (t >= 0 && t < a.n) at = (int)t;
+            }
         }
         if (KIND == MM_GRAD) {
-            lse2 = in ? a.lse2[m] : 0.f;
+            lse2 = in ? a.lse2[m] : make_float2(0.f, 0.f);
             rs = in ? a.rs[m] : 0.f;
             if (rs != 0.f && a.g_unit != 0.f) rs = a.g_unit;
         }
@@ -186,13 +197,20 @@ struct Epilogue {
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                v[i] = n + i < a.n ? v[i] * f : -INFINITY;
+                if (n + i >= a.n) v[i] = -INFINITY;
                 top = fmaxf(top, v[i]);
+            }
+            top *= f;                                          // f > 0
+            if ((unsigned)(at - n) < 32u) {
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) z = at - n == i ? v[i] : z;
+                a.logit_at[m0 + threadIdx.x % 32] = z * f;
             }
             const float now = fmaxf(mx, top), ref = now == -INFINITY ? 0.f : now;
             float t = s * ex2(mx - ref);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) t += ex2(v[i] - ref);
+            for (int i = 0; i < 32; ++i) t += ex2(fmaf(v[i], f, -ref));
             mx = now;
             s = t;
             return;
@@ -202,7 +220,8 @@ struct Epilogue {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-            turn[lane * 33 + i] = KIND == MM_GRAD ? rs == 0.f ? 0.f : rs * ex2(v[i] * f - lse2) : v[i] * f;
+            turn[lane * 33 + i] = KIND != MM_GRAD ? v[i] * f
+                                  : rs == 0.f ? 0.f : rs * ex2(fmaf(v[i], f, -lse2.x) - lse2.y);
         __syncwarp();
         const int rows = min(32, a.m - m0), cols = min(32, a.n - n);
         if (KIND == MM_GRAD) {
@@ -423,7 +442,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
         const int quad = warp % 4, side = warp / 4;
         const uint32_t lane_base = tmem + ((uint32_t)quad << 21);
-        const int cols = q.bn / 2, c0 = side * cols;
+        const int c0 = side * q.half, cols = side ? q.bn - q.half : q.half;
         float *turn = reinterpret_cast<float *>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * 2 * HALF) + warp * TURN;
         int use = 0;
         bool ok = true;
@@ -504,7 +523,8 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
 template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
-    q.part = PARTS ? PART / BK : q.steps;
+    // a few rows' dz meets a log-sum-exp that float32 cores summed: parts of one step there
+    q.part = !PARTS ? q.steps : KIND == MM_GRAD && a.m <= 8 ? 1 : PART / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -552,7 +572,8 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
-    const bool parts = (q.whole ? q.steps : q.kb) * BK > PART && (kind == MM_LSE || a.b.planes > 1);
+    const bool parts = ((q.whole ? q.steps : q.kb) * BK > PART || (kind == MM_GRAD && a.m <= 8)) &&
+                       (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);

@@ -271,18 +271,18 @@ def _head_workspace(x, w, backward: bool):
 
 
 def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
-    """(loss, lse2, picked, count) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides."""
+    """(loss, lse2, logq2, count) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides."""
     m, d = x.shape
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    lse2, picked, count = (torch.empty(n, device=x.device) for n in (m, m, 1))
+    lse2, logq2, count = (torch.empty(n, device=x.device) for n in ((m, 2), m, 1))
     ws = _head_workspace(x, w, False)
     rc = load().mms_linear_ce_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
-                                  ignore_index, red, _ptr(loss), _ptr(lse2), _ptr(picked),
+                                  ignore_index, red, _ptr(loss), _ptr(lse2), _ptr(logq2),
                                   _ptr(count), _ptr(ws), ws.numel(), m, w.shape[0], d, _dtype(x),
                                   _stream(x.device))
     _check(rc, "mms_linear_ce_fwd")
-    return loss, lse2, picked, count
+    return loss, lse2, logq2, count
 
 
 def _head_grads(x, w, need_x: bool, need_w: bool):
@@ -291,44 +291,44 @@ def _head_grads(x, w, need_x: bool, need_w: bool):
     return dx, dw, 0 if dx is None else _ptr(dx), 0 if dw is None else _ptr(dw)
 
 
-def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, lse2, picked, count,
+def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, lse2, logq2, count,
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
     ws = _head_workspace(x, w, True)
     rc = load().mms_linear_ce_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
                                   ignore_index, REDUCTIONS[reduction], _ptr(dloss), _ptr(lse2),
-                                  _ptr(picked), _ptr(count), pdx, pdw, _ptr(ws), ws.numel(),
+                                  _ptr(logq2), _ptr(count), pdx, pdw, _ptr(ws), ws.numel(),
                                   x.shape[0], w.shape[0], x.shape[1], _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_ce_bwd")
     return dx, dw
 
 
 def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
-    """(loss, lse2, picked, prob, count) of mms_linear_kd_fwd."""
+    """(loss, lse2, logq2, prob, count) of mms_linear_kd_fwd."""
     m, d = x.shape
     k = index.shape[1]
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    lse2, count = torch.empty(m, device=x.device), torch.empty(1, device=x.device)
-    picked, prob = torch.empty(m, k, device=x.device), torch.empty(m, k, device=x.device)
+    lse2, count = torch.empty(m, 2, device=x.device), torch.empty(1, device=x.device)
+    logq2, prob = torch.empty(m, k, device=x.device), torch.empty(m, k, device=x.device)
     ws = _head_workspace(x, w, False)
     rc = load().mms_linear_kd_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
                                   _ptr(logits), k, temperature, red, _ptr(loss), _ptr(lse2),
-                                  _ptr(picked), _ptr(prob), _ptr(count), _ptr(ws), ws.numel(), m,
+                                  _ptr(logq2), _ptr(prob), _ptr(count), _ptr(ws), ws.numel(), m,
                                   w.shape[0], d, _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_kd_fwd")
-    return loss, lse2, picked, prob, count
+    return loss, lse2, logq2, prob, count
 
 
-def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, lse2, picked, prob, count,
+def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, lse2, logq2, prob, count,
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_kd_bwd; None for one that is not needed."""
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
     ws = _head_workspace(x, w, True)
     rc = load().mms_linear_kd_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
                                   index.shape[1], temperature, REDUCTIONS[reduction], _ptr(dloss),
-                                  _ptr(lse2), _ptr(picked), _ptr(prob), _ptr(count), pdx, pdw,
+                                  _ptr(lse2), _ptr(logq2), _ptr(prob), _ptr(count), pdx, pdw,
                                   _ptr(ws), ws.numel(), x.shape[0], w.shape[0], x.shape[1],
                                   _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_kd_bwd")
