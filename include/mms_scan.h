@@ -249,7 +249,8 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * are contiguous; either may be NULL and is then not computed.
  *
  * x, w, dx, dw need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.
- * The workspace (256-byte aligned) has mms_head_workspace_size() bytes.
+ * The workspace (256-byte aligned) has mms_head_workspace_size() bytes, with
+ * k = 0 for the cross entropy; the two directions' sizes differ.
  * No counterpart in the reference, which computes the logits and calls
  * PyTorch's cross entropy (mamba_metal/model.py:293-297).
  */
@@ -259,7 +260,7 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
 #define MMS_REDUCE_MEAN 1
 #define MMS_REDUCE_SUM 2
 #define MMS_HEAD_MAX_K 1024
-size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long long ldx,
+size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, long long ldx,
                                long long ldw, int backward);
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction, float *loss,

@@ -118,8 +118,8 @@ int head_fwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
     if (!aligned(a.index, 8) || !aligned(a.logits, 4) || !aligned(a.loss, 4) ||
         !aligned(a.lse2, 8) || !aligned(a.logq2, 4) || !aligned(a.prob, 4) || !aligned(a.count, 4))
         return MMS_ERR_MISALIGNED;
-    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
-                                                                    a.ldx, a.ldw, false))
+    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.kd ? a.k : 0,
+                                                                    a.bf16, a.ldx, a.ldw, false))
         return MMS_ERR_WORKSPACE;
     if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
     return status_of(mms::launch_head_fwd(a, static_cast<cudaStream_t>(stream)));
@@ -132,8 +132,8 @@ int head_bwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
         !aligned(a.c_logq2, 4) || !aligned(a.c_prob, 4) || !aligned(a.c_count, 4) ||
         !aligned(a.dx, 16) || !aligned(a.dw, 16))
         return MMS_ERR_MISALIGNED;
-    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.bf16,
-                                                                    a.ldx, a.ldw, true))
+    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.kd ? a.k : 0,
+                                                                    a.bf16, a.ldx, a.ldw, true))
         return MMS_ERR_WORKSPACE;
     if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
     return status_of(mms::launch_head_bwd(a, static_cast<cudaStream_t>(stream)));
@@ -314,13 +314,13 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg, const
     return status_of(mms::launch_bwd(a, static_cast<cudaStream_t>(stream)));
 }
 
-size_t mms_head_workspace_size(int rows, int vocab, int dim, int dtype, long long ldx,
+size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, long long ldx,
                                long long ldw, int backward)
 {
-    if (rows < 1 || vocab < 1 || dim < 1 || rows > (1 << 24) || ldx < dim || ldw < dim ||
+    if (rows < 1 || vocab < 1 || dim < 1 || k < 0 || k > MMS_HEAD_MAX_K || rows > (1 << 24) || ldx < dim || ldw < dim ||
         (dtype != MMS_F32 && dtype != MMS_BF16))
         return 0;
-    return mms::head_workspace_bytes(rows, vocab, dim, dtype == MMS_BF16, ldx, ldw, backward != 0);
+    return mms::head_workspace_bytes(rows, vocab, dim, k, dtype == MMS_BF16, ldx, ldw, backward != 0);
 }
 
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,

@@ -18,12 +18,13 @@
 // workspace; the two products with dz follow piece by piece (6 more).
 //
 // Forward:   products (MM_LSE) -> one (max, sum) per row and half tile, joined
-//            by lse_kernel. The cross entropy's target logit is the product's
-//            own value, so that it cancels against lse2 where the target has
-//            nearly all the probability; the distillation's are dot products
-//            of their own (pick_kernel). Then a loss kernel; one block adds the
-//            rows up. Up to FEW_FWD rows (few_kernel) w is read once, as it
-//            is, by the CUDA cores: nothing is staged.
+//            by lse_kernel. The logits at the indices are the product's own
+//            values, so that its errors cancel against lse2's; the
+//            distillation's lists are sorted for that (order_kernel,
+//            before_kernel). Then a loss kernel; one block adds the rows up. Up to FEW_FWD rows (few_kernel) w is read once, as it
+//            is, by the CUDA cores: nothing is staged. The backward then takes
+//            dz from the same sums (few_grad_kernel), and so do pick_kernel's
+//            dot products for the distillation.
 // Backward:  rows_kernel: r; x staged with the left-out rows as zeros (so that
 //            nothing in them, NaN included, reaches dw); per piece: product
 //            MM_GRAD, sparse_kernel sets dz at the indices (from logq2, in
@@ -49,6 +50,8 @@
 //   dx = r dz w   r in the epilogue
 //   dw = dz^T (r x)   r x scaled as a whole
 #include <cuda_fp16.h>
+
+#include <limits.h>
 
 #include <algorithm>
 
@@ -93,10 +96,12 @@ struct Layout {
 
 struct FwdLayout : Layout {
     bool few;
+    size_t col, pos, before;        // the distillation's sorted lists
     size_t part, rowloss;
 };
 
 struct BwdLayout : Layout {
+    bool few;
     int gplanes;
     long long ldg;
     size_t xr, g, dxacc, rs, split, split_bytes;
@@ -115,7 +120,7 @@ size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
     return o;
 }
 
-FwdLayout fwd_layout(int rows, int vocab, int dim, bool bf16, long long ldx, long long ldw)
+FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw)
 {
     FwdLayout l;
     l.few = rows <= FEW_FWD;
@@ -127,6 +132,10 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, bool bf16, long long ldx, lon
                                                     mm_lse_parts(rows, l.last, dim, l.planes, l.planes));
     l.part = o; o += up256((size_t)(parts + 1) * rows * sizeof(float2));
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
+    const size_t lists = l.few ? 0 : (size_t)rows * k, blocks = lists ? (size_t)(vocab - 1) / LIST_BLOCK + 1 : 0;
+    l.col = o; o += up256(lists * sizeof(int));
+    l.pos = o; o += up256(lists * sizeof(uint16_t));
+    l.before = o; o += up256(blocks * rows * sizeof(uint16_t));
     l.total = o;
     return l;
 }
@@ -135,6 +144,7 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
 {
     BwdLayout l;
     l.planes = bf16 ? 1 : 2;
+    l.few = rows <= FEW_FWD;
     l.gplanes = bf16 && rows > FEW_ROWS ? 1 : 2;
     l.stage_x = true;
     l.stage_w = !bf16 || ldw % 8;
@@ -347,50 +357,80 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
 }
 
-// The log-sum-exp of up to FEW_FWD rows over a share of w's rows per CTA: a
-// warp takes 4 rows of w at a time, its lanes 8 columns each, against R rows
-// of x (L1 holds them). Bound by reading w once.
+// Up to FEW_FWD rows: a warp takes 4 rows of w at a time, its lanes 8 columns
+// each, against R rows of x (L1 holds them). Bound by reading w once. These
+// are the 4 R dot products, in every lane; pick_kernel adds in the same order.
 template <typename T, int R>
-__global__ void __launch_bounds__(256)
-few_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, float c, int rows,
-           int vocab, int dim, const int64_t *__restrict__ target, float *__restrict__ logq2,
-           float2 *__restrict__ part)
+__device__ __forceinline__ void few_dots(const T *__restrict__ x, long long ldx, const T *__restrict__ w,
+                                         long long ldw, int rows, int vocab, int dim, int v, float (&s)[R][4]) {
+    const T *wr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        wr[i] = w + (size_t)min(v + i, vocab - 1) * ldw;
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][i] = 0.f;
+    }
+    for (int k = threadIdx.x % 32 * 8; k < dim; k += 256) {
+        float q[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8(wr[i], k, dim, q[i]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float p[8];
+            load8(x + (size_t)min(r, rows - 1) * ldx, k, dim, p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[r][i] = fmaf(p[j], q[i][j], s[r][i]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[r][i] = warp_sum(s[r][i]);
+}
+
+struct FewArgs {
+    const void *x, *w;
+    long long ldx, ldw;
+    float c;
+    int rows, vocab, dim;
+    const int64_t *target;      // forward: the cross entropy's, whose logits go to `at`
+    float *at;
+    float2 *part;
+    const float2 *lse2;         // backward
+    const float *rs;
+    float unit;
+    uint16_t *g;
+    long long ldg, gplane;
+    int v0, n;                  // this piece
+    bool fp16;
+};
+
+// The log-sum-exp over a share of w's rows per CTA.
+template <typename T, int R>
+__global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 {
     __shared__ float2 sh[8][R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float c = a.c;
     float2 run[R];
     long long at[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         run[r] = make_float2(-INFINITY, 0.f);
-        at[r] = target && r < rows ? target[r] : -1;
+        at[r] = a.target && r < a.rows ? a.target[r] : -1;
     }
-    for (int v = (blockIdx.x * 8 + warp) * 4; v < vocab; v += gridDim.x * 32) {
-        float s[R][4] = {};
-        const T *wr[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wr[i] = w + (size_t)min(v + i, vocab - 1) * ldw;
-        for (int k = lane * 8; k < dim; k += 256) {
-            float q[4][8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) load8(wr[i], k, dim, q[i]);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float p[8];
-                load8(x + (size_t)min(r, rows - 1) * ldx, k, dim, p);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) s[r][i] = fmaf(p[j], q[i][j], s[r][i]);
-            }
-        }
+    for (int v = (blockIdx.x * 8 + warp) * 4; v < a.vocab; v += gridDim.x * 32) {
+        float s[R][4];
+        few_dots(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w), a.ldw, a.rows, a.vocab, a.dim, v, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float m = run[r].x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[r][i] = v + i < vocab ? warp_sum(s[r][i]) : -INFINITY;
-                if (v + i == at[r] && lane == 0) logq2[r] = s[r][i] * c;
+                if (v + i >= a.vocab) s[r][i] = -INFINITY;
+                if (v + i == at[r] && lane == 0) a.at[r] = s[r][i] * c;
                 m = fmaxf(m, s[r][i] * c);
             }
             const float ref = m == -INFINITY ? 0.f : m;
@@ -404,23 +444,119 @@ few_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long
 #pragma unroll
         for (int r = 0; r < R; ++r) sh[warp][r] = run[r];
     __syncthreads();
-    if (threadIdx.x < rows) {
+    if (threadIdx.x < a.rows) {
         float2 t = sh[0][threadIdx.x];
 #pragma unroll
         for (int i = 1; i < 8; ++i) t = join(t, sh[i][threadIdx.x]);
-        part[(size_t)blockIdx.x * rows + threadIdx.x] = t;
+        a.part[(size_t)blockIdx.x * a.rows + threadIdx.x] = t;
     }
 }
 
-template <typename T>
-void launch_few(const HeadArgs &a, float c, float2 *part, int blocks, cudaStream_t s)
+// dz of a piece of the vocabulary, two planes.
+template <typename T, int R>
+__global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
 {
-    const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
-    const int64_t *t = a.kd ? nullptr : a.index;
-    if (a.rows == 1) few_kernel<T, 1><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
-    else if (a.rows == 2) few_kernel<T, 2><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
-    else if (a.rows <= 4) few_kernel<T, 4><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
-    else few_kernel<T, 8><<<blocks, 256, 0, s>>>(x, a.ldx, w, a.ldw, c, a.rows, a.vocab, a.dim, t, a.logq2, part);
+    const int lane = threadIdx.x % 32, row = lane / 4, i = lane % 4;
+    const bool in = row < a.rows;
+    const float2 l = in ? a.lse2[row] : make_float2(0.f, 0.f);
+    const float rs = in ? a.rs[row] : 0.f, by = rs != 0.f && a.unit != 0.f ? a.unit : rs;
+    for (int v = (blockIdx.x * 8 + threadIdx.x / 32) * 4; v < a.n; v += gridDim.x * 32) {
+        float s[R][4];
+        few_dots(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w) + (size_t)a.v0 * a.ldw, a.ldw,
+                 a.rows, a.n, a.dim, v, s);
+        float z = 0.f;                                      // lane 4 r + i takes s[r][i]
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z = r == row && j == i ? s[r][j] : z;
+        if (!in || v + i >= a.n) continue;
+        float d = by == 0.f ? 0.f : by * ex2(fmaf(z, a.c, -l.x) - l.y);
+        uint16_t *o = a.g + (size_t)row * a.ldg + v + i;
+        for (int q = 0; q < 2; ++q, o += a.gplane) {
+            if (a.fp16) {
+                const __half t = __float2half_rn(d);
+                *o = __half_as_ushort(t);
+                d -= __half2float(t);
+            } else {
+                const __nv_bfloat16 t = __float2bfloat16_rn(d);
+                *o = __bfloat16_as_ushort(t);
+                d -= to_f(t);
+            }
+        }
+    }
+}
+
+template <typename T, int R>
+void launch_few_rows(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
+{
+    if (backward) few_grad_kernel<T, R><<<blocks, 256, 0, s>>>(a);
+    else few_kernel<T, R><<<blocks, 256, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_few(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
+{
+    if (a.rows == 1) launch_few_rows<T, 1>(a, blocks, backward, s);
+    else if (a.rows == 2) launch_few_rows<T, 2>(a, blocks, backward, s);
+    else if (a.rows <= 4) launch_few_rows<T, 4>(a, blocks, backward, s);
+    else launch_few_rows<T, 8>(a, blocks, backward, s);
+}
+
+FewArgs few_args(const HeadArgs &a, float c)
+{
+    FewArgs f{};
+    f.x = a.x; f.w = a.w; f.ldx = a.ldx; f.ldw = a.ldw; f.c = c;
+    f.rows = a.rows; f.vocab = a.vocab; f.dim = a.dim; f.fp16 = !a.bf16;
+    return f;
+}
+
+// The distillation's lists in ascending order, a warp a row: an entry's place
+// is the number of entries before it. Indices outside the vocabulary go last.
+__global__ void __launch_bounds__(256)
+order_kernel(const int64_t *__restrict__ index, int k, int rows, int vocab, int *__restrict__ col,
+             uint16_t *__restrict__ pos, float *__restrict__ logq2)
+{
+    extern __shared__ int sh_index[];
+    const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (m >= rows) return;
+    int *v = sh_index + threadIdx.x / 32 * k;
+    for (int j = lane; j < k; j += 32) {
+        const int64_t t = index[(size_t)m * k + j];
+        v[j] = t < 0 || t >= vocab ? INT_MAX : (int)t;
+        // no product will come for these
+        if (v[j] == INT_MAX) logq2[(size_t)m * k + j] = t < 0 ? 0.f : __int_as_float(0x7fc00000);
+    }
+    __syncwarp();
+    for (int j = lane; j < k; j += 32) {
+        const int t = v[j];
+        int place = 0;
+#pragma unroll 8
+        for (int i = 0; i < k; ++i) place += v[i] < t || (v[i] == t && i < j);
+        col[(size_t)m * k + place] = t;
+        pos[(size_t)m * k + place] = (uint16_t)j;
+    }
+}
+
+// before[b * rows + m]: entries of row m below column LIST_BLOCK * b. A thread
+// a row (32 a CTA, so that the stores are whole sectors) and 1/8 of the blocks.
+__global__ void __launch_bounds__(256)
+before_kernel(const int *__restrict__ col, int k, int rows, int blocks, uint16_t *__restrict__ before)
+{
+    const int m = blockIdx.x * 32 + threadIdx.x % 32;
+    if (m >= rows) return;
+    const int each = (blocks + 7) / 8, b0 = threadIdx.x / 32 * each, b1 = min(blocks, b0 + each);
+    const int *c = col + (size_t)m * k;
+    int lo = 0, hi = k;                                     // the first entry not below b0's column
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (c[mid] < (long long)b0 * LIST_BLOCK) lo = mid + 1;
+        else hi = mid;
+    }
+    int at = lo < k ? c[lo] : INT_MAX;
+    for (int b = b0; b < b1; ++b) {
+        while (at < (long long)b * LIST_BLOCK) at = ++lo < k ? c[lo] : INT_MAX;
+        before[(size_t)b * rows + m] = (uint16_t)lo;
+    }
 }
 
 // One row a lane, 32 threads a row over the tiles. Parts 1..ntiles, and part
@@ -583,8 +719,6 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
             if (f < e) return;
             p += prob[f];
         }
-        // float32: q as the product's own value, which is what the row's other entries add up to 1 with
-        if (fp16) d = (__half2float(__ushort_as_half(o[0])) + __half2float(__ushort_as_half(o[gplane]))) / unit - 1.f;
     }
     d = (unit != 0.f ? unit : r) * (d + (1.f - p));
     for (int q = 0; q < planes; ++q, o += gplane) {
@@ -642,21 +776,24 @@ Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, cudaStream_
 
 }  // namespace
 
-size_t head_workspace_bytes(int rows, int vocab, int dim, bool bf16, long long ldx, long long ldw,
+size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw,
                             bool backward)
 {
     return backward ? bwd_layout(rows, vocab, dim, bf16, ldw).total
-                    : fwd_layout(rows, vocab, dim, bf16, ldx, ldw).total;
+                    : fwd_layout(rows, vocab, dim, k, bf16, ldx, ldw).total;
 }
 
 cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
 {
-    const FwdLayout l = fwd_layout(a.rows, a.vocab, a.dim, a.bf16, a.ldx, a.ldw);
+    const FwdLayout l = fwd_layout(a.rows, a.vocab, a.dim, a.kd ? a.k : 0, a.bf16, a.ldx, a.ldw);
     const float c = MMS_LOG2E / a.tau;
     float2 *part = reinterpret_cast<float2 *>(fl(a.workspace, l.part));
     float *rowloss = a.reduction == MMS_REDUCE_NONE ? a.loss : fl(a.workspace, l.rowloss);
-    if (a.kd) {
-        const long long n = (long long)a.rows * a.k;
+    cudaError_t e;
+    const int64_t *target = a.kd ? nullptr : a.index;
+    Lists lists{};
+    if (a.kd && l.few) {
+        const int n = a.rows * a.k;
         if (a.bf16)
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w), a.ldw,
@@ -665,13 +802,21 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index, a.k, c,
                 a.logq2, n, a.vocab, a.dim);
+    } else if (a.kd) {
+        int *col = reinterpret_cast<int *>(fl(a.workspace, l.col));
+        uint16_t *pos = u16(a.workspace, l.pos), *before = u16(a.workspace, l.before);
+        order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, a.vocab, col,
+                                                                                pos, a.logq2);
+        before_kernel<<<ceil_div(a.rows, 32), 256, 0, stream>>>(col, a.k, a.rows, (a.vocab - 1) / LIST_BLOCK + 1,
+                                                               before);
+        lists = Lists{col, pos, before, a.k, a.rows};
     }
-    cudaError_t e;
-    const int64_t *target = a.kd ? nullptr : a.index;
     if (l.few) {
         const int blocks = std::min(ceil_div(a.vocab, 32), FEW_BLOCKS);
-        if (a.bf16) launch_few<__nv_bfloat16>(a, c, part + a.rows, blocks, stream);
-        else launch_few<float>(a, c, part + a.rows, blocks, stream);
+        FewArgs f = few_args(a, c);
+        f.target = target; f.at = a.logq2; f.part = part + a.rows;
+        if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, false, stream);
+        else launch_few<float>(f, blocks, false, stream);
         lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows,
                                                   reinterpret_cast<float2 *>(a.lse2), target,
                                                   a.ignore_index, a.vocab, a.logq2, rowloss);
@@ -691,8 +836,9 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         }
         mm.part = part + a.rows;                        // part 0: the pieces before
         mm.target = target;
-        mm.target_first = v0;
-        mm.logit_at = a.logq2;
+        mm.lists = lists;
+        mm.first_col = v0;
+        mm.at = a.logq2;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
             part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
@@ -749,7 +895,16 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         }
         mm.lse2 = reinterpret_cast<const float2 *>(a.c_lse2); mm.rs = rs; mm.g_unit = unit;
         mm.g = g; mm.ldg = l.ldg; mm.gplane = gplane; mm.gplanes = l.gplanes;
-        if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) return e;
+        if (l.few) {
+            FewArgs f = few_args(a, c);
+            f.lse2 = mm.lse2; f.rs = rs; f.unit = unit; f.g = g; f.ldg = l.ldg; f.gplane = gplane;
+            f.v0 = v0; f.n = nv;
+            const int blocks = std::min(ceil_div(nv, 32), FEW_BLOCKS);
+            if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, true, stream);
+            else launch_few<float>(f, blocks, true, stream);
+        } else if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) {
+            return e;
+        }
         sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_logq2, rs, unit, a.k, n, v0,
                                                             v0 + nv, g, l.ldg, gplane, l.gplanes, f32);
         MmArgs out{};

@@ -29,6 +29,16 @@ struct Factor {
 enum MmKind { MM_LSE, MM_GRAD, MM_OUT };
 constexpr int MM_COLS = 256;            // columns of the widest tile
 
+// Columns of each row in ascending order: col[m * k + i] (INT_MAX: none), the
+// place pos[m * k + i] each had before, and before[b * rows + m], how many of
+// them lie below column LIST_BLOCK * b.
+constexpr int LIST_BLOCK = 128;
+struct Lists {
+    const int *col;
+    const uint16_t *pos, *before;
+    int k, rows;
+};
+
 struct MmArgs {
     Factor a, b;
     bool fp16;                  // the planes are fp16, else bf16
@@ -36,9 +46,12 @@ struct MmArgs {
     float c;
     const float *row_mul, *mul;
     float2 *part;               // MM_LSE
-    const int64_t *target;      // MM_LSE: where target[m] - target_first is a column,
-    long long target_first;     //         logit_at[m] = s there; may be null
-    float *logit_at;
+    // MM_LSE: the products at given columns. One a row: where target[m] - first_col
+    // is a column, at[m] = s. Or `lists` of them (see Lists): at[m * k + pos] = s.
+    const int64_t *target;
+    Lists lists;                // lists.col may be null
+    float *at;
+    int first_col;              // of column 0
     const float2 *lse2;         // MM_GRAD: (top, log2 of the sum of 2^(s - top))
     const float *rs;            // MM_GRAD
     float g_unit;               // MM_GRAD
@@ -83,7 +96,8 @@ struct HeadArgs {
     void *workspace;
 };
 
-size_t head_workspace_bytes(int rows, int vocab, int dim, bool bf16, long long ldx, long long ldw,
+// k: entries of the distillation's lists, 0 for the cross entropy
+size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw,
                             bool backward);
 cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream);
 cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream);

@@ -42,6 +42,8 @@
 // copies in flight, and the pair leaves together.
 #include <cuda_fp16.h>
 
+#include <limits.h>
+
 #include <algorithm>
 
 #include "mms_common.cuh"
@@ -161,15 +163,34 @@ __device__ __forceinline__ float half_value(bool fp16, uint16_t b) {
     return fp16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
 }
 
+// v[i] without an indexed register file: halves of the candidates by each bit of i.
+__device__ __forceinline__ float pick32(const float (&v)[32], int i) {
+    float t[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = i & 16 ? v[j + 16] : v[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = i & 8 ? t[j + 8] : t[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = i & 4 ? t[j + 4] : t[j];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) t[j] = i & 2 ? t[j + 2] : t[j];
+    return i & 1 ? t[1] : t[0];
+}
+
 // What follows the product on 32 columns of one row per lane.
 template <int KIND>
 struct Epilogue {
     float f;                    // the product's factor
     float mx, s;                // MM_LSE: running maximum and sum
-    int at;                     // MM_LSE: the target's column, or -1
+    int at, nth;                // MM_LSE: the next column whose product is asked for, its number in the list
     float2 lse2;                // MM_GRAD
     float rs;
-    __device__ __forceinline__ void begin(const MmArgs &a, int m) {
+    __device__ __forceinline__ void next(const MmArgs &a, int m) {
+        const int c = nth < a.lists.k ? a.lists.col[(size_t)m * a.lists.k + nth] : INT_MAX;
+        at = c == INT_MAX ? c : c - a.first_col;
+    }
+    // m: this lane's row, n: the first column that this warp will see
+    __device__ __forceinline__ void begin(const MmArgs &a, int m, int n) {
         const bool in = m < a.m;
         f = a.c;
         if (a.row_mul) f *= in ? a.row_mul[m] : 0.f;
@@ -177,10 +198,15 @@ struct Epilogue {
         if (KIND == MM_LSE) {
             mx = -INFINITY;
             s = 0.f;
-            at = -1;
+            at = INT_MAX;
+            nth = 0;
             if (a.target && in) {
-                const long long t = a.target[m] - a.target_first;
+                const long long t = a.target[m] - a.first_col;
                 if (t >= 0 && t < a.n) at = (int)t;
+            }
+            if (a.lists.col && in && n < a.n) {
+                nth = a.lists.before[(size_t)((a.first_col + n) / LIST_BLOCK) * a.lists.rows + m];
+                next(a, m);
             }
         }
         if (KIND == MM_GRAD) {
@@ -201,11 +227,18 @@ struct Epilogue {
                 top = fmaxf(top, v[i]);
             }
             top *= f;                                          // f > 0
-            if ((unsigned)(at - n) < 32u) {
-                float z = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) z = at - n == i ? v[i] : z;
-                a.logit_at[m0 + threadIdx.x % 32] = z * f;
+            while (at < n + 32) {
+                const int m = m0 + threadIdx.x % 32;
+                if (at >= n) {
+                    const size_t to = a.target ? m : (size_t)m * a.lists.k + a.lists.pos[(size_t)m * a.lists.k + nth];
+                    a.at[to] = pick32(v, at - n) * f;
+                }
+                if (a.target) {
+                    at = INT_MAX;
+                } else {
+                    ++nth;
+                    next(a, m);
+                }
             }
             const float now = fmaxf(mx, top), ref = now == -INFINITY ? 0.f : now;
             float t = s * ex2(mx - ref);
@@ -452,7 +485,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             tile_of(q, tile, mi, ni);
             const int m0 = mi * TM + rank * 128 + quad * 32, m = m0 + lane;
             Epilogue<KIND> ep;
-            ep.begin(a, m);
+            ep.begin(a, m, ni * q.bn + c0);
             float2 sum[PARTS ? 4 : 1][16];
             for (int k_first = k_begin; k_first < k_end; k_first += q.part, ++use) {
                 const int buf = use & 1;
@@ -486,12 +519,23 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
             }
             if (!ok) break;
-            if (PARTS) {
+            if (PARTS && KIND == MM_LSE) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     if (32 * c < cols)
                         ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c,
                                  reinterpret_cast<float (&)[32]>(sum[c]), turn);
+            } else if (PARTS) {
+                // one copy of the code, the sums moving up: unrolled it spills registers
+#pragma unroll 1
+                for (int c = 0; 32 * c < cols; ++c) {
+                    ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c,
+                             reinterpret_cast<float (&)[32]>(sum[0]), turn);
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[j][i] = sum[PARTS ? j + 1 : 0][i];
+                }
             }
             ep.end(a, m, ni * 2 + side);
         }
@@ -523,8 +567,7 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
 template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
-    // a few rows' dz meets a log-sum-exp that float32 cores summed: parts of one step there
-    q.part = !PARTS ? q.steps : KIND == MM_GRAD && a.m <= 8 ? 1 : PART / BK;
+    q.part = PARTS ? PART / BK : q.steps;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -572,8 +615,7 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
-    const bool parts = ((q.whole ? q.steps : q.kb) * BK > PART || (kind == MM_GRAD && a.m <= 8)) &&
-                       (kind == MM_LSE || a.b.planes > 1);
+    const bool parts = (q.whole ? q.steps : q.kb) * BK > PART && (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);

@@ -51,7 +51,7 @@ SIGNATURES = {
                      + [_P], _I),
     "mms_fwd_bf16": ([_P] * 7 + [_I] * 5 + [_P], _I),
     "mms_bwd_bf16": ([_P] * 13 + [ctypes.c_size_t] + [_I] * 5 + [_P], _I),
-    "mms_head_workspace_size": ([_I] * 4 + [_L] * 2 + [_I], _Z),
+    "mms_head_workspace_size": ([_I] * 5 + [_L] * 2 + [_I], _Z),
     "mms_linear_ce_fwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 5 + [_Z] + [_I] * 4 + [_P], _I),
     "mms_linear_ce_bwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 7 + [_Z] + [_I] * 4 + [_P], _I),
     "mms_linear_kd_fwd": ([_P, _L, _P, _L, _P, _P, _I, _F, _I] + [_P] * 6 + [_Z] + [_I] * 4
@@ -264,8 +264,8 @@ def _dtype(t) -> int:
     return 1 if t.dtype == torch.bfloat16 else 0
 
 
-def _head_workspace(x, w, backward: bool):
-    nb = int(load().mms_head_workspace_size(x.shape[0], w.shape[0], x.shape[1], _dtype(x),
+def _head_workspace(x, w, k: int, backward: bool):
+    nb = int(load().mms_head_workspace_size(x.shape[0], w.shape[0], x.shape[1], k, _dtype(x),
                                             x.stride(0), w.stride(0), int(backward)))
     return torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
 
@@ -276,7 +276,7 @@ def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
     lse2, logq2, count = (torch.empty(n, device=x.device) for n in ((m, 2), m, 1))
-    ws = _head_workspace(x, w, False)
+    ws = _head_workspace(x, w, 0, False)
     rc = load().mms_linear_ce_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
                                   ignore_index, red, _ptr(loss), _ptr(lse2), _ptr(logq2),
                                   _ptr(count), _ptr(ws), ws.numel(), m, w.shape[0], d, _dtype(x),
@@ -295,7 +295,7 @@ def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, lse2, 
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    ws = _head_workspace(x, w, True)
+    ws = _head_workspace(x, w, 0, True)
     rc = load().mms_linear_ce_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
                                   ignore_index, REDUCTIONS[reduction], _ptr(dloss), _ptr(lse2),
                                   _ptr(logq2), _ptr(count), pdx, pdw, _ptr(ws), ws.numel(),
@@ -312,7 +312,7 @@ def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
     lse2, count = torch.empty(m, 2, device=x.device), torch.empty(1, device=x.device)
     logq2, prob = torch.empty(m, k, device=x.device), torch.empty(m, k, device=x.device)
-    ws = _head_workspace(x, w, False)
+    ws = _head_workspace(x, w, k, False)
     rc = load().mms_linear_kd_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
                                   _ptr(logits), k, temperature, red, _ptr(loss), _ptr(lse2),
                                   _ptr(logq2), _ptr(prob), _ptr(count), _ptr(ws), ws.numel(), m,
@@ -325,7 +325,7 @@ def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, lse2, 
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_kd_bwd; None for one that is not needed."""
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    ws = _head_workspace(x, w, True)
+    ws = _head_workspace(x, w, index.shape[1], True)
     rc = load().mms_linear_kd_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
                                   index.shape[1], temperature, REDUCTIONS[reduction], _ptr(dloss),
                                   _ptr(lse2), _ptr(logq2), _ptr(prob), _ptr(count), pdx, pdw,

@@ -129,10 +129,10 @@ def test_c_entries_check_before_any_launch():
     assert ce_fwd(red=3) == bad and ce_fwd(red=-1) == bad and ce_fwd(m=(1 << 24) + 1) == bad
     assert ce_fwd(x=None) == bad and ce_fwd(t=None) == bad and ce_fwd(out=None) == bad
     assert ce_fwd(x=_p(0x10008)) == mis and ce_fwd(t=_p(0x10004)) == mis
-    need = lib.mms_head_workspace_size(4, 8, 16, 0, 16, 16, 0)
+    need = lib.mms_head_workspace_size(4, 8, 16, 0, 0, 16, 16, 0)
     assert need > 0 and ce_fwd(nb=need - 1) == ws_err and ce_fwd(ws=None) == ws_err
     assert ce_fwd(ws=_p(0x20010)) == mis
-    assert lib.mms_head_workspace_size(0, 8, 16, 0, 16, 16, 0) == 0
+    assert lib.mms_head_workspace_size(0, 8, 16, 0, 0, 16, 16, 0) == 0
 
     def kd_fwd(k=2, tau=1.0, logits=ok, nb=0):
         return lib.mms_linear_kd_fwd(ok, 16, ok, 16, ok, logits, k, tau, 1, ok, ok, ok, ok, ok,
