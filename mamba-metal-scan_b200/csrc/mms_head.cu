@@ -11,8 +11,9 @@
 // tau for the distillation; 0 for a row that is left out):
 //     dz[m, v]  = r (2^(c z - lse2) - sum of p_j with index_j = v)
 //     dx = dz w,   dw = dz^T x
-// The two halves of lse2 stay apart: their sum would round at the magnitude of
-// the logits, where the difference to a likely entry's logit is exact.
+// The two halves of lse2 stay apart, and the logits at the indices keep their
+// rounding errors (`rest`): sums would round at the magnitude of the logits,
+// where the difference of a likely entry's logit to lse2 is small and exact.
 // z is computed once forward (2 rows vocab dim flops) and again backward, in
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
@@ -97,7 +98,7 @@ struct Layout {
 struct FwdLayout : Layout {
     bool few;
     size_t col, pos, before;        // the distillation's sorted lists
-    size_t part, rowloss;
+    size_t part, rowloss, rest;
 };
 
 struct BwdLayout : Layout {
@@ -132,6 +133,7 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long l
                                                     mm_lse_parts(rows, l.last, dim, l.planes, l.planes));
     l.part = o; o += up256((size_t)(parts + 1) * rows * sizeof(float2));
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
+    l.rest = o; o += up256((size_t)rows * std::max(k, 1) * sizeof(float));
     const size_t lists = l.few ? 0 : (size_t)rows * k, blocks = lists ? (size_t)(vocab - 1) / LIST_BLOCK + 1 : 0;
     l.col = o; o += up256(lists * sizeof(int));
     l.pos = o; o += up256(lists * sizeof(uint16_t));
@@ -325,7 +327,8 @@ __device__ __forceinline__ float warp_max(float v) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw,
-            const int64_t *__restrict__ index, int k, float c, float *__restrict__ logq2, long long n, int vocab, int dim)
+            const int64_t *__restrict__ index, int k, float c, float *__restrict__ logq2,
+            float *__restrict__ rest, long long n, int vocab, int dim)
 {
     const long long e = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
@@ -345,9 +348,12 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
 #pragma unroll
             for (int j = 0; j < 8; ++j) s = fmaf(p[j], q[j], s);
         }
-        s = warp_sum(s) * c;
+        s = warp_sum(s);
     }
-    if (lane == 0) logq2[e] = s;
+    if (lane) return;
+    const float p = s * c;
+    logq2[e] = p;
+    rest[e] = rounding_of(s, c, p);
 }
 
 // (max, sum) pairs join to the pair of both; a NaN in either sum stays.
@@ -396,7 +402,7 @@ struct FewArgs {
     float c;
     int rows, vocab, dim;
     const int64_t *target;      // forward: the cross entropy's, whose logits go to `at`
-    float *at;
+    float *at, *rest;
     float2 *part;
     const float2 *lse2;         // backward
     const float *rs;
@@ -430,7 +436,10 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (v + i >= a.vocab) s[r][i] = -INFINITY;
-                if (v + i == at[r] && lane == 0) a.at[r] = s[r][i] * c;
+                if (v + i == at[r] && lane == 0) {
+                    a.at[r] = s[r][i] * c;
+                    a.rest[r] = rounding_of(s[r][i], c, s[r][i] * c);
+                }
                 m = fmaxf(m, s[r][i] * c);
             }
             const float ref = m == -INFINITY ? 0.f : m;
@@ -514,7 +523,7 @@ FewArgs few_args(const HeadArgs &a, float c)
 // is the number of entries before it. Indices outside the vocabulary go last.
 __global__ void __launch_bounds__(256)
 order_kernel(const int64_t *__restrict__ index, int k, int rows, int vocab, int *__restrict__ col,
-             uint16_t *__restrict__ pos, float *__restrict__ logq2)
+             uint16_t *__restrict__ pos, float *__restrict__ logq2, float *__restrict__ rest)
 {
     extern __shared__ int sh_index[];
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -524,7 +533,10 @@ order_kernel(const int64_t *__restrict__ index, int k, int rows, int vocab, int 
         const int64_t t = index[(size_t)m * k + j];
         v[j] = t < 0 || t >= vocab ? INT_MAX : (int)t;
         // no product will come for these
-        if (v[j] == INT_MAX) logq2[(size_t)m * k + j] = t < 0 ? 0.f : __int_as_float(0x7fc00000);
+        if (v[j] == INT_MAX) {
+            logq2[(size_t)m * k + j] = t < 0 ? 0.f : __int_as_float(0x7fc00000);
+            rest[(size_t)m * k + j] = 0.f;
+        }
     }
     __syncwarp();
     for (int j = lane; j < k; j += 32) {
@@ -565,7 +577,7 @@ before_kernel(const int *__restrict__ col, int k, int rows, int blocks, uint16_t
 __global__ void __launch_bounds__(1024)
 lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__restrict__ lse2,
            const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
-           float *__restrict__ loss)
+           const float *__restrict__ rest, float *__restrict__ loss)
 {
     __shared__ float2 sh[32][33];
     const int m = blockIdx.x * 32 + threadIdx.x;
@@ -592,7 +604,7 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
     if (!target) return;
     const int64_t t = target[r];
     float l = 0.f;
-    if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : (logq2[r] - v.x) - v.y;
+    if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - v.y;
     logq2[r] = l;
     loss[r] = -LN2 * l;
 }
@@ -602,7 +614,7 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
 __global__ void __launch_bounds__(256)
 kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, float tau,
           const float2 *__restrict__ lse2, float *__restrict__ logq2,
-          float *__restrict__ prob, float *__restrict__ loss, int rows)
+          const float *__restrict__ rest, float *__restrict__ prob, float *__restrict__ loss, int rows)
 {
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (m >= rows) return;
@@ -623,7 +635,7 @@ kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, i
     float acc = 0.f;
     for (int j = lane; j < k; j += 32) {
         float p = 0.f;
-        const float lq = (logq2[o + j] - l2.x) - l2.y;
+        const float lq = ((logq2[o + j] - l2.x) + rest[o + j]) - l2.y;
         logq2[o + j] = lq;
         if (some && index[o + j] >= 0) {
             const float t = (logits[o + j] - top) * inv;
@@ -789,6 +801,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     const float c = MMS_LOG2E / a.tau;
     float2 *part = reinterpret_cast<float2 *>(fl(a.workspace, l.part));
     float *rowloss = a.reduction == MMS_REDUCE_NONE ? a.loss : fl(a.workspace, l.rowloss);
+    float *rest = fl(a.workspace, l.rest);
     cudaError_t e;
     const int64_t *target = a.kd ? nullptr : a.index;
     Lists lists{};
@@ -797,16 +810,16 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         if (a.bf16)
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w), a.ldw,
-                a.index, a.k, c, a.logq2, n, a.vocab, a.dim);
+                a.index, a.k, c, a.logq2, rest, n, a.vocab, a.dim);
         else
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index, a.k, c,
-                a.logq2, n, a.vocab, a.dim);
+                a.logq2, rest, n, a.vocab, a.dim);
     } else if (a.kd) {
         int *col = reinterpret_cast<int *>(fl(a.workspace, l.col));
         uint16_t *pos = u16(a.workspace, l.pos), *before = u16(a.workspace, l.before);
         order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, a.vocab, col,
-                                                                                pos, a.logq2);
+                                                                                pos, a.logq2, rest);
         before_kernel<<<ceil_div(a.rows, 32), 256, 0, stream>>>(col, a.k, a.rows, (a.vocab - 1) / LIST_BLOCK + 1,
                                                                before);
         lists = Lists{col, pos, before, a.k, a.rows};
@@ -814,12 +827,12 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     if (l.few) {
         const int blocks = std::min(ceil_div(a.vocab, 32), FEW_BLOCKS);
         FewArgs f = few_args(a, c);
-        f.target = target; f.at = a.logq2; f.part = part + a.rows;
+        f.target = target; f.at = a.logq2; f.rest = rest; f.part = part + a.rows;
         if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, false, stream);
         else launch_few<float>(f, blocks, false, stream);
         lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows,
                                                   reinterpret_cast<float2 *>(a.lse2), target,
-                                                  a.ignore_index, a.vocab, a.logq2, rowloss);
+                                                  a.ignore_index, a.vocab, a.logq2, rest, rowloss);
     }
     if (!l.few && l.planes > 1 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
     const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, stream);
@@ -839,15 +852,16 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.lists = lists;
         mm.first_col = v0;
         mm.at = a.logq2;
+        mm.rest = rest;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
             part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
-            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rowloss);
+            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rest, rowloss);
     }
     if (a.kd)
         kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau,
                                                           reinterpret_cast<const float2 *>(a.lse2),
-                                                          a.logq2, a.prob, rowloss, a.rows);
+                                                          a.logq2, rest, a.prob, rowloss, a.rows);
     total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, a.kd ? a.prob : nullptr, a.k,
                                          a.ignore_index, a.rows, a.reduction, a.loss, a.count);
     return cudaGetLastError();

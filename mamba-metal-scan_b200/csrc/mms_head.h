@@ -39,6 +39,12 @@ struct Lists {
     int k, rows;
 };
 
+// What a * b lost by rounding to p; 0 where p is not finite.
+__device__ __forceinline__ float rounding_of(float a, float b, float p) {
+    const float r = fmaf(a, b, -p);
+    return r == r ? r : 0.f;
+}
+
 struct MmArgs {
     Factor a, b;
     bool fp16;                  // the planes are fp16, else bf16
@@ -47,10 +53,11 @@ struct MmArgs {
     const float *row_mul, *mul;
     float2 *part;               // MM_LSE
     // MM_LSE: the products at given columns. One a row: where target[m] - first_col
-    // is a column, at[m] = s. Or `lists` of them (see Lists): at[m * k + pos] = s.
+    // is a column, at[m] + rest[m] = s, rest the rounding of at. Or `lists` of them
+    // (see Lists) at m * k + pos.
     const int64_t *target;
     Lists lists;                // lists.col may be null
-    float *at;
+    float *at, *rest;
     int first_col;              // of column 0
     const float2 *lse2;         // MM_GRAD: (top, log2 of the sum of 2^(s - top))
     const float *rs;            // MM_GRAD

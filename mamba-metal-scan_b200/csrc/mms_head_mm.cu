@@ -231,7 +231,9 @@ struct Epilogue {
                 const int m = m0 + threadIdx.x % 32;
                 if (at >= n) {
                     const size_t to = a.target ? m : (size_t)m * a.lists.k + a.lists.pos[(size_t)m * a.lists.k + nth];
-                    a.at[to] = pick32(v, at - n) * f;
+                    const float z = pick32(v, at - n), p = z * f;
+                    a.at[to] = p;
+                    a.rest[to] = rounding_of(z, f, p);
                 }
                 if (a.target) {
                     at = INT_MAX;
@@ -567,7 +569,8 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
 template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
-    q.part = PARTS ? PART / BK : q.steps;
+    // one round of tiles is short anyway: finer parts
+    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? 2 : PART / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -615,7 +618,8 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
-    const bool parts = (q.whole ? q.steps : q.kb) * BK > PART && (kind == MM_LSE || a.b.planes > 1);
+    const int steps = q.whole ? q.steps : q.kb;
+    const bool parts = (steps * BK > PART || (steps > 2 && q.items <= N_SM / 2)) && (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);

@@ -42,7 +42,11 @@ def compare(x, w, parts, tau, reduction, dloss, loss, grads):
     for name, got in zip(("dx", "dw"), grads):
         assert got.dtype == x.dtype
         check(name, got, want[name], want["e_" + name])
-        check_norm(name, got, want[name], tol)
+        # one entry in the vocabulary: q = p = 1 and the gradient is 0 by arithmetic, so a norm
+        # has no scale there (0 / 0); the kernels' log2 of a float32 sum near 1 is exact to 2^-24
+        # of 1, which the element-wise bound holds in absolute terms
+        if w.shape[0] > 1:
+            check_norm(name, got, want[name], tol)
     return want
 
 
