@@ -16,13 +16,16 @@
 // 16-byte aligned), and the one or two sums a row needs are block reductions.
 // A thread owns the same columns in every row, so the backward's sums over
 // rows stay in its registers; the CTAs' partial sums meet in the workspace in
-// a fixed order. Rows too long for that (above 512 x 16 elements) are read
+// a fixed order. The backward's five reads a row come a row ahead, by
+// cp.async into shared memory where each thread finds its own pieces again (no
+// barrier), and its arithmetic is on packed pairs. Rows too long for that (above 512 x 16 elements) are read
 // again for each sum.
 #include <algorithm>
 
 #include "mms_common.cuh"
 #include "mms_head.h"
 #include "mms_kernels.h"
+#include "mms_stage.cuh"
 
 namespace mms {
 
@@ -69,6 +72,20 @@ struct Cols {
             } else {
                 o[v] = c < dim ? to_f(p[c]) : 0.f;
             }
+        }
+    }
+    // the same pieces by cp.async to `dst` (one piece of 16 bytes a thread and v), and from there
+    __device__ static __forceinline__ void fetch(uint4 *dst, const T *__restrict__ p, int dim) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) cp16(dst + v * blockDim.x + threadIdx.x, p + (at(v) < dim ? at(v) : 0), at(v) < dim);
+    }
+    __device__ static __forceinline__ void take(const uint4 *src, float (&o)[E]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const uint4 q = src[v * blockDim.x + threadIdx.x];
+            const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+            for (int j = 0; j < VW; ++j) o[v * VW + j] = to_f(e[j]);
         }
     }
     __device__ static __forceinline__ void store(T *__restrict__ p, int dim, const float (&o)[E]) {
@@ -145,86 +162,166 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_fwd_kernel(const NormArgs a)
     }
 }
 
+template <int P>
+__device__ __forceinline__ float (&flat(float2 (&v)[P]))[2 * P] {
+    return reinterpret_cast<float (&)[2 * P]>(v);
+}
+
+// The backward's reads of a row, in the order of their places in shared memory.
+enum { IN_DU, IN_X, IN_Y, IN_DH, IN_GATE };
+// Rows in shared memory, this one and the next, where ROW_THREADS leave room for
+// them (5 x 512 x 16 bytes a row and piece); 0: loads at the top of the row.
+template <typename T, int E, bool VEC>
+constexpr int fetch_rows() {
+    return !VEC || E * sizeof(T) > 32 ? 0 : 2;
+}
+
+template <typename T, int E, bool VEC, int F>
+constexpr int fetch_bytes(int threads) {
+    return fetch_rows<T, E, VEC>() * (F & GATE ? 5 : 4) * threads * E * (int)sizeof(T);
+}
+
+template <typename T, int E, bool VEC, int F>
+struct RowReader {
+    using C = Cols<T, E, VEC>;
+    static constexpr int N = F & GATE ? 5 : 4, R = fetch_rows<T, E, VEC>();
+    const NormArgs &a;
+    uint4 *smem;                                // [R][N][NV * threads]
+    size_t r;
+    int slot;
+    __device__ __forceinline__ const T *src(int which, size_t row) const {
+        const size_t o = row * a.dim;
+        switch (which) {
+        case IN_DU: return static_cast<const T *>(a.du) + o;
+        case IN_X: return static_cast<const T *>(a.x) + o;
+        case IN_Y: return static_cast<const T *>(a.y) + o;
+        case IN_DH: return static_cast<const T *>(a.dh) + o;
+        default: return static_cast<const T *>(a.gate) + row * a.ldg;
+        }
+    }
+    __device__ __forceinline__ uint4 *place(int which, int s) const {
+        return smem + (size_t)(s * N + which) * C::NV * blockDim.x;
+    }
+    __device__ __forceinline__ void fetch(size_t row, int s) {
+        if constexpr (R > 0) {
+            if (row < (size_t)a.rows)
+#pragma unroll
+                for (int w = 0; w < N; ++w) C::fetch(place(w, s), src(w, row), a.dim);
+            cp_commit();                        // also without a row: the waits count groups
+        }
+    }
+    __device__ __forceinline__ void begin(size_t row) {
+        r = row;
+        slot = 0;
+        for (int i = 0; i < R - 1; ++i) fetch(r + (size_t)i * gridDim.x, i);
+    }
+    // This row is there; one more is on its way, into the place that the row before left.
+    __device__ __forceinline__ void ready() {
+        fetch(r + (size_t)(R - 1) * gridDim.x, slot == 0 ? R - 1 : slot - 1);
+        if constexpr (R > 0) cp_wait<R - 1>();
+    }
+    __device__ __forceinline__ void get(int which, float (&o)[E]) const {
+        if constexpr (R > 0) C::take(place(which, slot), o);
+        else C::load(src(which, r), a.dim, o);
+    }
+    __device__ __forceinline__ void next() {
+        r += gridDim.x;
+        slot = slot == R - 1 ? 0 : slot + 1;
+    }
+};
+
 // Sums over this CTA's rows go to part[(which * gridDim + block) * dim + column],
 // which = 0 dweight, 1 dscale, 2 dpost.
 template <typename T, int E, bool VEC, int F>
 __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
 {
     using C = Cols<T, E, VEC>;
+    extern __shared__ uint4 rows_smem[];
     __shared__ float sh[2][32];
     BlockSum sum{sh, 0};
     const float inv = 1.f / a.dim;
-    float sw[E], ss[E], sp[E];
+    constexpr int P = E / 2;                                 // packed pairs: half the instructions
+    float2 sw[P], ss[P], sp[P];
 #pragma unroll
-    for (int i = 0; i < E; ++i) sw[i] = ss[i] = sp[i] = 0.f;
-    for (size_t r = blockIdx.x; r < (size_t)a.rows; r += gridDim.x) {
-        const size_t o = r * a.dim;
-        float h[E], t[E], y[E], z[E], v[E], w[E], d[E];
-        C::load(static_cast<const T *>(a.du) + o, a.dim, t);
-        C::load(static_cast<const T *>(a.x) + o, a.dim, h);
-        C::load(static_cast<const T *>(a.y) + o, a.dim, y);
-        if (F & GATE) C::load(static_cast<const T *>(a.gate) + r * a.ldg, a.dim, z);
-        C::load(static_cast<const T *>(a.dh) + o, a.dim, d);
-        const float r1 = F & POST ? a.c_stat[2 * r] : 1.f, r2 = a.c_stat[2 * r + 1];
-        // v = a r1 (the normed a, or a itself), h
-        if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, w);
+    for (int i = 0; i < P; ++i) sw[i] = ss[i] = sp[i] = f2(0.f, 0.f);
+    RowReader<T, E, VEC, F> in{a, rows_smem, 0, 0};
+    for (in.begin(blockIdx.x); in.r < (size_t)a.rows; in.next()) {
+        in.ready();
+        const size_t o = in.r * a.dim;
+        float2 h[P], t[P], v[P], w[P], d[P];
+        const float r1 = F & POST ? a.c_stat[2 * in.r] : 1.f, r2 = a.c_stat[2 * in.r + 1];
+        const float2 r1p = f2(r1, r1), r2p = f2(r2, r2);
+        // v = a r1 (the normed a, or a itself), h = n
+        in.get(IN_Y, flat(v));
+        if (F & GATE) {
+            in.get(IN_GATE, flat(d));
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            v[i] = y[i];
-            if (F & GATE) v[i] *= z[i] * sigmoid_fast(z[i]);
-            if (F & POST) v[i] *= r1;
+            for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(d[i], f2(sigmoid_fast(d[i].x), sigmoid_fast(d[i].y))));
         }
-        float sc[E];
-        if (F & SCALE) C::load(static_cast<const T *>(a.scale), a.dim, sc);
+        in.get(IN_X, flat(h));
+        if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, flat(w));
+        if (F & SCALE) C::load(static_cast<const T *>(a.scale), a.dim, flat(d));
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            float b = v[i];
-            if (F & POST) b *= w[i];
-            if (F & SCALE) b *= sc[i];
-            h[i] = (h[i] + b) * r2;                          // n
+        for (int i = 0; i < P; ++i) {
+            if (F & POST) v[i] = mul2(v[i], r1p);
+            float2 b = v[i];
+            if (F & POST) b = mul2(b, w[i]);
+            h[i] = mul2(F & SCALE ? fma2(b, d[i], h[i]) : add2(h[i], b), r2p);
         }
-        float s = 0.f;
-        float ww[E];
-        C::load(static_cast<const T *>(a.weight), a.dim, ww);
+        in.get(IN_DU, flat(t));
+        float2 s = f2(0.f, 0.f);
+        C::load(static_cast<const T *>(a.weight), a.dim, flat(w));
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            sw[i] = fmaf(t[i], h[i], sw[i]);
-            t[i] *= ww[i];
-            s = fmaf(t[i], h[i], s);
+        for (int i = 0; i < P; ++i) {
+            sw[i] = fma2(t[i], h[i], sw[i]);
+            t[i] = mul2(t[i], w[i]);
+            s = fma2(t[i], h[i], s);
         }
-        const float mean = sum(s) * inv;
-        s = 0.f;
+        const float mean = sum(s.x + s.y) * inv;
+        const float2 meanp = f2(-mean, -mean);
+        in.get(IN_DH, flat(d));
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            d[i] = fmaf(r2, t[i] - h[i] * mean, d[i]);       // dh'
+        for (int i = 0; i < P; ++i) d[i] = fma2(r2p, fma2(h[i], meanp, t[i]), d[i]);        // dh'
+        C::store(static_cast<T *>(a.dx) + o, a.dim, flat(d));
+        if (F == 0) continue;                                // dy has dx's values
+        if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, flat(w));
+        if (F & SCALE) C::load(static_cast<const T *>(a.scale), a.dim, flat(h));
+        s = f2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
             t[i] = d[i];
             if (F & SCALE) {
-                ss[i] = fmaf(d[i], F & POST ? v[i] * w[i] : v[i], ss[i]);
-                t[i] *= sc[i];                               // db
+                ss[i] = fma2(d[i], F & POST ? mul2(v[i], w[i]) : v[i], ss[i]);
+                t[i] = mul2(t[i], h[i]);                     // db
             }
             if (F & POST) {
-                sp[i] = fmaf(t[i], v[i], sp[i]);
-                t[i] *= w[i];
-                s = fmaf(t[i], v[i], s);
+                sp[i] = fma2(t[i], v[i], sp[i]);
+                t[i] = mul2(t[i], w[i]);
+                s = fma2(t[i], v[i], s);
             }
         }
-        C::store(static_cast<T *>(a.dx) + o, a.dim, d);
-        if (F == 0) continue;                                // dy has dx's values
         if (F & POST) {
-            const float mean1 = sum(s) * inv;
+            const float mean1 = sum(s.x + s.y) * inv;
+            const float2 mean1p = f2(-mean1, -mean1);
 #pragma unroll
-            for (int i = 0; i < E; ++i) t[i] = r1 * (t[i] - v[i] * mean1);
+            for (int i = 0; i < P; ++i) t[i] = mul2(r1p, fma2(v[i], mean1p, t[i]));
         }
         if (F & GATE) {
+            in.get(IN_GATE, flat(w));
+            in.get(IN_Y, flat(v));
+            const float2 one = f2(1.f, 1.f);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float sig = sigmoid_fast(z[i]);
-                d[i] = t[i] * y[i] * (sig * (1.f + z[i] * (1.f - sig)));
-                t[i] *= z[i] * sig;
+            for (int i = 0; i < P; ++i) {
+                const float2 sig = f2(sigmoid_fast(w[i].x), sigmoid_fast(w[i].y));
+                const float2 zs = mul2(w[i], sig);
+                // silu' = sig (1 + z (1 - sig)) = sig + z sig - (z sig) sig
+                const float2 slope = fma2(zs, fma2(sig, f2(-1.f, -1.f), one), sig);
+                d[i] = mul2(mul2(t[i], v[i]), slope);
+                t[i] = mul2(t[i], zs);
             }
-            C::store(static_cast<T *>(a.dgate) + o, a.dim, d);
+            C::store(static_cast<T *>(a.dgate) + o, a.dim, flat(d));
         }
-        C::store(static_cast<T *>(a.dy) + o, a.dim, t);
+        C::store(static_cast<T *>(a.dy) + o, a.dim, flat(t));
     }
     const size_t plane = (size_t)gridDim.x * a.dim;
     float *part = static_cast<float *>(a.workspace) + (size_t)blockIdx.x * a.dim;
@@ -232,9 +329,9 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
     for (int i = 0; i < E; ++i) {
         const int c = C::at(i / C::VW) + i % C::VW;
         if (c >= a.dim) continue;
-        part[c] = sw[i];
-        if (F & SCALE) part[plane + c] = ss[i];
-        if (F & POST) part[2 * plane + c] = sp[i];
+        part[c] = flat(sw)[i];
+        if (F & SCALE) part[plane + c] = flat(ss)[i];
+        if (F & POST) part[2 * plane + c] = flat(sp)[i];
     }
 }
 
@@ -405,12 +502,12 @@ Shape shape_for(int dim, int vw)
 
 // CTAs of a kernel that fit the GPU at once (asked once per kernel and size).
 template <auto KERNEL>
-int resident(int threads)
+int resident(int threads, int smem)
 {
     static std::atomic<int> known[ROW_THREADS / 32 + 1];
     int n = known[threads / 32].load(std::memory_order_relaxed);
     if (!n) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) != cudaSuccess || n < 1) n = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem) != cudaSuccess || n < 1) n = 1;
         known[threads / 32].store(n, std::memory_order_relaxed);
     }
     return n * N_SM;
@@ -420,10 +517,13 @@ template <typename T, int E, bool VEC, int F>
 cudaError_t run(const NormArgs &a, int threads, bool backward, int *blocks, cudaStream_t stream)
 {
     if (backward) {
-        *blocks = std::min({a.rows, resident<norm_bwd_kernel<T, E, VEC, F>>(threads), MAX_ROW_BLOCKS});
-        norm_bwd_kernel<T, E, VEC, F><<<*blocks, threads, 0, stream>>>(a);
+        const int smem = fetch_bytes<T, E, VEC, F>(threads);
+        const cudaError_t e = smem_opt_in<norm_bwd_kernel<T, E, VEC, F>>(fetch_bytes<T, E, VEC, F>(ROW_THREADS));
+        if (e != cudaSuccess) return e;
+        *blocks = std::min({a.rows, resident<norm_bwd_kernel<T, E, VEC, F>>(threads, smem), MAX_ROW_BLOCKS});
+        norm_bwd_kernel<T, E, VEC, F><<<*blocks, threads, smem, stream>>>(a);
     } else {
-        const int grid = std::min(a.rows, resident<norm_fwd_kernel<T, E, VEC, F>>(threads));
+        const int grid = std::min(a.rows, resident<norm_fwd_kernel<T, E, VEC, F>>(threads, 0));
         norm_fwd_kernel<T, E, VEC, F><<<grid, threads, 0, stream>>>(a);
     }
     return cudaGetLastError();

@@ -4,7 +4,11 @@ API-compatible with the reference package's `mamba_metal.model`
 (Anamaya1729/mamba-metal-scan, mamba_metal/model.py): the same config fields,
 module names and parameter shapes (so state_dicts load either way), the same
 block arithmetic, and the same `scan_impl` switch. Only the scan itself is
-native; everything else is ordinary PyTorch.
+native by default; everything else is ordinary PyTorch. `fuse_norm` runs the
+residual sum after each block and the next norm as one kernel each way
+(`residual_rms_norm`), `fuse_loss` the head and its cross entropy without the
+logits (`linear_cross_entropy`); `TinyMamba.distill_loss` trains on a
+teacher's top k logits through the same head (`linear_distillation`).
 
 Block (reference model.py:161-256):
     x -> RMSNorm -> in_proj -> (x, z)
@@ -30,6 +34,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from mamba_metal.head import linear_cross_entropy, linear_distillation
+from mamba_metal.norm import residual_rms_norm
 from mamba_metal.scan import (SSM_CHUNK, gated_output, selective_scan, selective_scan_proj,
                               selective_scan_step, selective_scan_step_ref)
 
@@ -49,6 +55,8 @@ class MambaConfig:
     scan_impl: str = "auto"   # 'auto' | 'cuda' | 'metal' | 'torch'
     fuse_proj: bool = True    # CUDA scan computes dt and softplus(A) itself (selective_scan_proj)
     fuse_gate: bool = True    # (y + D_skip) * silu(z) as one CUDA kernel each way (gated_output)
+    fuse_norm: bool = False   # residual sum + next norm as one CUDA kernel each way (residual_rms_norm)
+    fuse_loss: bool = False   # with targets: no logits, forward returns (None, loss) (linear_cross_entropy)
     dt_min: float = 0.001
     dt_max: float = 0.1
     norm_eps: float = 1e-6
@@ -228,8 +236,11 @@ class MambaBlock(nn.Module):
         return y
 
     def forward(self, x, cache=None):
-        residual = x
-        x, z = self.in_proj(self.norm(x)).chunk(2, dim=-1)
+        return x + self.mix(self.norm(x), cache)
+
+    def mix(self, x, cache=None):
+        """The block between its norm and the residual sum."""
+        x, z = self.in_proj(x).chunk(2, dim=-1)
         kc = self.conv.kernel_size[0]
         if cache is not None and cache.get("h") is not None and x.shape[1] == 1:
             # one-token recurrent step against the cached conv window and state
@@ -251,9 +262,9 @@ class MambaBlock(nn.Module):
             if cache is not None:
                 cache["h"], cache["h_owned"] = h_last, False
         if self.fuse_gate and y.is_cuda and self.scan_impl != "torch":
-            return residual + self.out_proj(gated_output(y, z, self.D_skip, impl=self.scan_impl))
+            return self.out_proj(gated_output(y, z, self.D_skip, impl=self.scan_impl))
         y = y + self.D_skip
-        return residual + self.out_proj(y * F.silu(z))
+        return self.out_proj(y * F.silu(z))
 
 
 class TinyMamba(nn.Module):
@@ -283,19 +294,43 @@ class TinyMamba(nn.Module):
         elif isinstance(m, nn.Embedding):
             nn.init.normal_(m.weight, mean=0.0, std=0.02)
 
-    def forward(self, idx, targets=None, cache=None):
+    def hidden(self, idx, cache=None):
+        """The head's input: the last block's residual stream after ln_f, (B, T, d_model)."""
         if cache is not None and "blocks" not in cache:
             cache["blocks"] = [{} for _ in self.blocks]
         per_block = cache["blocks"] if cache is not None else [None] * len(self.blocks)
         x = self.tok(idx)
+        if self.cfg.fuse_norm and len(self.blocks):
+            norms = [b.norm for b in self.blocks] + [self.ln_f]
+            u = norms[0](x)
+            for block, bc, norm in zip(self.blocks, per_block, norms[1:]):
+                x, u = residual_rms_norm(x, block.mix(u, bc), norm.weight, eps=norm.eps,
+                                         impl=self.cfg.scan_impl)
+            return u
         for block, bc in zip(self.blocks, per_block):
             x = block(x, bc)
-        logits = self.head(self.ln_f(x))
+        return self.ln_f(x)
+
+    def forward(self, idx, targets=None, cache=None):
+        x = self.hidden(idx, cache)
+        if targets is not None and self.cfg.fuse_loss:
+            return None, linear_cross_entropy(x, self.head.weight, targets, ignore_index=-100,
+                                              impl=self.cfg.scan_impl)
+        logits = self.head(x)
         loss = None
         if targets is not None:
             loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1),
                                    ignore_index=-100)
         return logits, loss
+
+    def distill_loss(self, idx, teacher_index, teacher_logits, temperature: float = 1.0,
+                     reduction: str = "mean"):
+        """KL divergence of the model's next-token distribution from a teacher's top k logits.
+
+        teacher_index, teacher_logits (B, T, k): see `linear_distillation`.
+        """
+        return linear_distillation(self.hidden(idx), self.head.weight, teacher_index, teacher_logits,
+                                   temperature, reduction, impl=self.cfg.scan_impl)
 
     def count_params(self) -> int:
         """Unique parameters (the tied head counts once)."""

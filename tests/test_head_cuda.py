@@ -333,7 +333,7 @@ def test_norm_head_and_both_losses_together(dtype):
     # bf16: the norm's output, each loss' dz, each loss' gradient, their sum and the norm's
     # gradient are rounded: six roundings of 2^-8; float32 as above
     tol = 6 * u(dtype) if dtype == BF16 else 2e-5
-    assert abs(float(got[0]) - float(want[0])) <= tol * float(want[0])
+    assert abs(float(got[0].detach()) - float(want[0].detach())) <= tol * float(want[0].detach())
     for name, a, b in zip(("dx", "dy", "dnorm", "dw"), got[1], want[1]):
         check_norm(name, a, b, tol)
 

@@ -184,14 +184,14 @@ def test_deterministic_streams_and_graphs():
     t, dh, du = norm_inputs(700, 640, F32, True, True, True, seed=6)
     d = on_device(t)
     dh, du = dh.to(DEV), du.to(DEV)
-    a = run(d, dh, du)
+    a = {n: v.detach() for n, v in run(d, dh, du).items()}
+    d = on_device(t)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         b = run(d, dh, du)
         side.synchronize()
     assert all(torch.equal(a[n], b[n]) for n in a)
-    a = {n: v.detach() for n, v in a.items()}
     del b
     d = on_device(t)                    # leaves that no eager graph has met
     graph = torch.cuda.CUDAGraph()
