@@ -245,7 +245,7 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * of z / temperature in units of log 2 as its largest term and the rest;
  * logq2 (rows, k; k = 1 for the cross entropy), log2 of q at the indices;
  * prob (rows, k)
- * = p; count (1) = the rows that count. dx (rows, dim) and dw (vocab, dim)
+ * = p; count (2) = the rows that count, and for float32 the largest |w|. dx (rows, dim) and dw (vocab, dim)
  * are contiguous; either may be NULL and is then not computed.
  *
  * x, w, dx, dw need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.

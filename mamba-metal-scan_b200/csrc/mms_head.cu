@@ -91,7 +91,7 @@ int piece_size(int vocab, size_t bytes_per_row)
 struct Layout {
     bool stage_x, stage_w;
     int planes, piece, last;        // vocabulary entries of a piece, of the last one
-    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and maxima)
+    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and r x's maximum)
     size_t total;
 };
 
@@ -198,6 +198,20 @@ __device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, 
     }
 }
 
+// *top = the larger of it and the CTA's maximum of v >= 0 (256 threads). One
+// atomic a CTA: a few thousand on one address would take longer than the reads.
+__device__ __forceinline__ void block_top(float v, unsigned *top) {
+    __shared__ float sh[8];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v = fmaxf(v, sh[i]);
+    if (v > 0.f) atomicMax(top, __float_as_uint(v));        // non-negative floats compare as their bits
+}
+
 // How a staged matrix is scaled: not at all (bf16), each row to its own
 // maximum, or all of it to the maximum that `top` holds.
 enum StageKind { ST_COPY, ST_ROWS, ST_WHOLE };
@@ -276,29 +290,27 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
                 *reinterpret_cast<uint4 *>(out + a.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
-    if (KIND == ST_ROWS && a.top) {                         // non-negative floats compare as their bits
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(a.top, __float_as_uint(top));
-    }
+    if (KIND == ST_ROWS && a.top) block_top(top, a.top);
 }
 
 // The largest finite magnitude of a float32 matrix, as bits (top starts at 0).
+// A warp reads two rows at a time.
 __global__ void __launch_bounds__(256)
 top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, unsigned *top)
 {
     float m = 0.f;
-    for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
+    for (long long r = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * 2; r < rows; r += gridDim.x * 16) {
+        const float *p = src + (size_t)r * lds, *q = r + 1 < rows ? p + lds : p;
 #pragma unroll 2
         for (int c = threadIdx.x % 32 * 8; c < cols; c += 256) {
-            float v[8];
-            load8(src + (size_t)r * lds, c, cols, v);
+            float v[8], w[8];
+            load8(p, c, cols, v);
+            load8(q, c, cols, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(finite_abs(v[i]), finite_abs(w[i])));
         }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if (threadIdx.x % 32 == 0 && m > 0.f) atomicMax(top, __float_as_uint(m));
+    }
+    block_top(m, top);
 }
 
 int grid_of(long long rows, int per_block) { return (int)std::min<long long>((rows + per_block - 1) / per_block, 148 * 16); }
@@ -573,13 +585,16 @@ before_kernel(const int *__restrict__ col, int k, int rows, int blocks, uint16_t
 
 // One row a lane, 32 threads a row over the tiles. Parts 1..ntiles, and part
 // 0 (the pieces before) unless `first`. Writes part 0, or in the last piece
-// lse2 and, from the target's logit in logq2, the cross entropy's row loss.
+// lse2 and, from the target's logit in logq2, the cross entropy's row loss;
+// with `total` (up to 32 rows) total_kernel's work too.
 __global__ void __launch_bounds__(1024)
 lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__restrict__ lse2,
            const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
-           const float *__restrict__ rest, float *__restrict__ loss)
+           const float *__restrict__ rest, float *__restrict__ loss, int reduction,
+           float *__restrict__ total, float *__restrict__ count)
 {
     __shared__ float2 sh[32][33];
+    __shared__ float row_loss[32];
     const int m = blockIdx.x * 32 + threadIdx.x;
     float2 v = make_float2(-INFINITY, 0.f);
     if (m < rows)
@@ -594,19 +609,31 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
     for (int o = 16; o; o >>= 1)
         v = join(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
     const int r = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x || r >= rows) return;
-    if (!last) {
-        part[r] = v;
-        return;
+    if (threadIdx.x == 0 && r < rows) {
+        if (!last) {
+            part[r] = v;
+        } else {
+            v.y = log2f(v.y);
+            lse2[r] = v;
+        }
+        if (last && target) {
+            const int64_t t = target[r];
+            float l = 0.f;
+            if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - v.y;
+            logq2[r] = l;
+            loss[r] = row_loss[threadIdx.y] = -LN2 * l;
+        }
     }
-    v.y = log2f(v.y);
-    lse2[r] = v;
-    if (!target) return;
-    const int64_t t = target[r];
-    float l = 0.f;
-    if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - v.y;
-    logq2[r] = l;
-    loss[r] = -LN2 * l;
+    if (!total) return;                                     // one CTA has all rows
+    __syncthreads();
+    if (threadIdx.y) return;
+    const bool in = threadIdx.x < rows;
+    const float s = warp_sum(in ? row_loss[threadIdx.x] : 0.f);
+    const float n = warp_sum(in && target[threadIdx.x] != ignore ? 1.f : 0.f);
+    if (threadIdx.x == 0) {
+        *count = n;
+        if (reduction != MMS_REDUCE_NONE) *total = reduction == MMS_REDUCE_MEAN ? s / n : s;
+    }
 }
 
 // Distillation's row loss, a warp a row: the teacher's softmax over its
@@ -749,13 +776,20 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
 uint16_t *u16(void *base, size_t off) { return reinterpret_cast<uint16_t *>(static_cast<char *>(base) + off); }
 float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast<char *>(base) + off); }
 
-// muls: w's scale, r x's scale, and the bits of the two maxima they come from.
-cudaError_t top_of_w(const HeadArgs &a, const Layout &l, cudaStream_t s)
+// Where w's largest magnitude is: the forward keeps it for the backward
+// (count[1]), but for few rows, whose forward does not need it.
+unsigned *w_top(const HeadArgs &a, const Layout &l)
 {
-    unsigned *top = reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 2);
-    const cudaError_t e = cudaMemsetAsync(top, 0, 2 * sizeof(unsigned), s);
+    if (a.count) return reinterpret_cast<unsigned *>(a.count + 1);
+    if (a.rows <= FEW_FWD) return reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3);
+    return reinterpret_cast<unsigned *>(const_cast<float *>(a.c_count) + 1);
+}
+cudaError_t top_of_w(const HeadArgs &a, unsigned *top, cudaStream_t s)
+{
+    const cudaError_t e = cudaMemsetAsync(top, 0, sizeof(unsigned), s);
     if (e == cudaSuccess)
-        top_kernel<<<grid_of(a.vocab, 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw, a.vocab, a.dim, top);
+        top_kernel<<<std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw,
+                                                                           a.vocab, a.dim, top);
     return e;
 }
 
@@ -766,8 +800,7 @@ Factor w_factor(const HeadArgs &a, const Layout &l, int v0, int n, cudaStream_t 
     const long long ld = padded(a.dim);
     float *muls = fl(a.workspace, l.muls);
     StageArgs st{static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4), a.ldw,
-                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, muls,
-                 reinterpret_cast<unsigned *>(muls + 2)};
+                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, muls, w_top(a, l)};
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
     else stage<float, ST_WHOLE>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
@@ -780,7 +813,7 @@ Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, cudaStream_
     const long long ld = padded(a.dim);
     StageArgs st{a.x, a.ldx, u16(a.workspace, l.xs), ld, ld * a.rows, a.rows, a.dim, rs,
                  fl(a.workspace, l.row_mul),
-                 rs ? reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3) : nullptr};
+                 rs ? reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 2) : nullptr};
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
     else stage<float, ST_ROWS>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
@@ -802,6 +835,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     float2 *part = reinterpret_cast<float2 *>(fl(a.workspace, l.part));
     float *rowloss = a.reduction == MMS_REDUCE_NONE ? a.loss : fl(a.workspace, l.rowloss);
     float *rest = fl(a.workspace, l.rest);
+    float *total = a.kd || a.rows > 32 ? nullptr : a.loss;
     cudaError_t e;
     const int64_t *target = a.kd ? nullptr : a.index;
     Lists lists{};
@@ -832,9 +866,9 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         else launch_few<float>(f, blocks, false, stream);
         lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows,
                                                   reinterpret_cast<float2 *>(a.lse2), target,
-                                                  a.ignore_index, a.vocab, a.logq2, rest, rowloss);
+                                                  a.ignore_index, a.vocab, a.logq2, rest, rowloss, a.reduction, total, a.count);
     }
-    if (!l.few && l.planes > 1 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
+    if (l.planes > 1 && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
     const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, stream);
     for (int v0 = l.few ? a.vocab : 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
@@ -856,13 +890,14 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
             part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
-            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rest, rowloss);
+            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rest, rowloss, a.reduction, total, a.count);
     }
     if (a.kd)
         kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau,
                                                           reinterpret_cast<const float2 *>(a.lse2),
                                                           a.logq2, rest, a.prob, rowloss, a.rows);
-    total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, a.kd ? a.prob : nullptr, a.k,
+    if (!total)
+        total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, a.kd ? a.prob : nullptr, a.k,
                                          a.ignore_index, a.rows, a.reduction, a.loss, a.count);
     return cudaGetLastError();
 }
@@ -882,12 +917,13 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     cudaError_t e;
     const bool f32 = l.planes > 1;
     float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
-    if (f32 && (e = top_of_w(a, l, stream)) != cudaSuccess) return e;
+    if (f32 && (e = cudaMemsetAsync(muls + 2, 0, sizeof(float), stream)) != cudaSuccess) return e;
+    if (f32 && l.few && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
     const Factor x = x_factor(a, l, rs, stream);
     Factor xr = x;                                      // the factor of dw: x, or r x
     if (f32) {
         StageArgs st{a.x, a.ldx, u16(a.workspace, l.xr), x.ld, x.plane, a.rows, a.dim, rs, muls + 1,
-                     reinterpret_cast<unsigned *>(muls + 3)};
+                     reinterpret_cast<unsigned *>(muls + 2)};
         stage<float, ST_WHOLE>(st, stream);
         xr.p = st.out;
     }

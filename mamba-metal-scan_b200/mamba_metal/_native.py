@@ -110,7 +110,13 @@ def _ptr(t: torch.Tensor) -> int:
     return t.data_ptr()
 
 
+# the current stream's handle without building a Stream object, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -270,67 +276,81 @@ def _head_workspace(x, w, k: int, backward: bool):
     return torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
 
 
+def _kept(m: int, k: int, kd: bool, base: int):
+    """Addresses of lse2, logq2, prob, count in the one buffer that the forward keeps, and its
+    length in floats."""
+    at = [0, 2 * m, 2 * m + m * k, 2 * m + m * k * (2 if kd else 1)]
+    return [base + 4 * o for o in at], at[3] + 2
+
+
 def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
-    """(loss, lse2, logq2, count) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides."""
+    """(loss, kept) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides. kept: lse2, logq2
+    and count in one float32 buffer."""
     m, d = x.shape
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    lse2, logq2, count = (torch.empty(n, device=x.device) for n in ((m, 2), m, 1))
+    kept = torch.empty(_kept(m, 1, False, 0)[1], device=x.device)
+    (lse2, logq2, _, count), _ = _kept(m, 1, False, kept.data_ptr())
     ws = _head_workspace(x, w, 0, False)
-    rc = load().mms_linear_ce_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
-                                  ignore_index, red, _ptr(loss), _ptr(lse2), _ptr(logq2),
-                                  _ptr(count), _ptr(ws), ws.numel(), m, w.shape[0], d, _dtype(x),
+    rc = load().mms_linear_ce_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                  target.data_ptr(), ignore_index, red, loss.data_ptr(), lse2, logq2,
+                                  count, ws.data_ptr(), ws.numel(), m, w.shape[0], d, _dtype(x),
                                   _stream(x.device))
     _check(rc, "mms_linear_ce_fwd")
-    return loss, lse2, logq2, count
+    return loss, kept
 
 
 def _head_grads(x, w, need_x: bool, need_w: bool):
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
     dw = torch.empty(w.shape, device=w.device, dtype=w.dtype) if need_w else None
-    return dx, dw, 0 if dx is None else _ptr(dx), 0 if dw is None else _ptr(dw)
+    return dx, dw, 0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr()
 
 
-def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, lse2, logq2, count,
+def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, kept,
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
+    m, d = x.shape
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
+    (lse2, logq2, _, count), _ = _kept(m, 1, False, kept.data_ptr())
     ws = _head_workspace(x, w, 0, True)
-    rc = load().mms_linear_ce_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(target),
-                                  ignore_index, REDUCTIONS[reduction], _ptr(dloss), _ptr(lse2),
-                                  _ptr(logq2), _ptr(count), pdx, pdw, _ptr(ws), ws.numel(),
-                                  x.shape[0], w.shape[0], x.shape[1], _dtype(x), _stream(x.device))
+    rc = load().mms_linear_ce_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                  target.data_ptr(), ignore_index, REDUCTIONS[reduction],
+                                  dloss.data_ptr(), lse2, logq2, count, pdx, pdw, ws.data_ptr(),
+                                  ws.numel(), m, w.shape[0], d, _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_ce_bwd")
     return dx, dw
 
 
 def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
-    """(loss, lse2, logq2, prob, count) of mms_linear_kd_fwd."""
+    """(loss, kept) of mms_linear_kd_fwd. kept: lse2, logq2, prob and count in one float32 buffer."""
     m, d = x.shape
     k = index.shape[1]
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    lse2, count = torch.empty(m, 2, device=x.device), torch.empty(1, device=x.device)
-    logq2, prob = torch.empty(m, k, device=x.device), torch.empty(m, k, device=x.device)
+    kept = torch.empty(_kept(m, k, True, 0)[1], device=x.device)
+    (lse2, logq2, prob, count), _ = _kept(m, k, True, kept.data_ptr())
     ws = _head_workspace(x, w, k, False)
-    rc = load().mms_linear_kd_fwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
-                                  _ptr(logits), k, temperature, red, _ptr(loss), _ptr(lse2),
-                                  _ptr(logq2), _ptr(prob), _ptr(count), _ptr(ws), ws.numel(), m,
-                                  w.shape[0], d, _dtype(x), _stream(x.device))
+    rc = load().mms_linear_kd_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                  index.data_ptr(), logits.data_ptr(), k, temperature, red,
+                                  loss.data_ptr(), lse2, logq2, prob, count, ws.data_ptr(),
+                                  ws.numel(), m, w.shape[0], d, _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_kd_fwd")
-    return loss, lse2, logq2, prob, count
+    return loss, kept
 
 
-def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, lse2, logq2, prob, count,
+def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, kept,
                   need_x: bool = True, need_w: bool = True):
     """(dx, dw) of mms_linear_kd_bwd; None for one that is not needed."""
+    m, d = x.shape
+    k = index.shape[1]
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    ws = _head_workspace(x, w, index.shape[1], True)
-    rc = load().mms_linear_kd_bwd(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(index),
-                                  index.shape[1], temperature, REDUCTIONS[reduction], _ptr(dloss),
-                                  _ptr(lse2), _ptr(logq2), _ptr(prob), _ptr(count), pdx, pdw,
-                                  _ptr(ws), ws.numel(), x.shape[0], w.shape[0], x.shape[1],
-                                  _dtype(x), _stream(x.device))
+    (lse2, logq2, prob, count), _ = _kept(m, k, True, kept.data_ptr())
+    ws = _head_workspace(x, w, k, True)
+    rc = load().mms_linear_kd_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                  index.data_ptr(), k, temperature, REDUCTIONS[reduction],
+                                  dloss.data_ptr(), lse2, logq2, prob, count, pdx, pdw,
+                                  ws.data_ptr(), ws.numel(), m, w.shape[0], d, _dtype(x),
+                                  _stream(x.device))
     _check(rc, "mms_linear_kd_bwd")
     return dx, dw
 

@@ -113,18 +113,18 @@ class LinearCrossEntropyCUDA(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
         with _native.on_device(x.device):
-            loss, lse2, logq2, count = _native.linear_ce_fwd(x, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(x, weight, target, lse2, logq2, count)
+            loss, kept = _native.linear_ce_fwd(x, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(x, weight, target, kept)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, weight, target, lse2, logq2, count = ctx.saved_tensors
+        x, weight, target, kept = ctx.saved_tensors
         with _native.on_device(x.device):
             dx, dw = _native.linear_ce_bwd(x, weight, target, ctx.ignore_index, ctx.reduction,
-                                           dloss.float().contiguous(), lse2, logq2, count,
+                                           dloss.float().contiguous(), kept,
                                            *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None
 
@@ -135,19 +135,18 @@ class LinearDistillationCUDA(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, index, logits, temperature, reduction):
         with _native.on_device(x.device):
-            loss, lse2, logq2, prob, count = _native.linear_kd_fwd(x, weight, index, logits,
-                                                                    temperature, reduction)
-        ctx.save_for_backward(x, weight, index, lse2, logq2, prob, count)
+            loss, kept = _native.linear_kd_fwd(x, weight, index, logits, temperature, reduction)
+        ctx.save_for_backward(x, weight, index, kept)
         ctx.temperature, ctx.reduction = temperature, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, weight, index, lse2, logq2, prob, count = ctx.saved_tensors
+        x, weight, index, kept = ctx.saved_tensors
         with _native.on_device(x.device):
             dx, dw = _native.linear_kd_bwd(x, weight, index, ctx.temperature, ctx.reduction,
-                                           dloss.float().contiguous(), lse2, logq2, prob, count,
+                                           dloss.float().contiguous(), kept,
                                            *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None, None
 
