@@ -22,7 +22,7 @@
 //            by lse_kernel. The logits at the indices are the product's own
 //            values, so that its errors cancel against lse2's; the
 //            distillation's lists are sorted for that (order_kernel,
-//            before_kernel). Then a loss kernel; one block adds the rows up. Up to FEW_FWD rows (few_kernel) w is read once, as it
+//            before_kernel). Then a loss kernel; one block adds the rows up. Up to few_rows() rows (few_kernel) w is read once, as it
 //            is, by the CUDA cores: nothing is staged. The backward then takes
 //            dz from the same sums (few_grad_kernel), and so do pick_kernel's
 //            dot products for the distillation.
@@ -67,7 +67,9 @@ namespace {
 constexpr float LN2 = 0.6931471805599453f;
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // bound on one staged or dz piece
 constexpr int FEW_ROWS = 256;
-constexpr int FEW_FWD = 8;
+// Rows that the CUDA cores take: at 50176 x 1024 they need (us, forward) 34, 49, 45, 68 for 1, 2,
+// 4, 8 rows of float32, where staging alone is 100; in bf16 20, 20, 36, 58, the tensor cores 31.
+int few_rows(bool bf16) { return bf16 ? 2 : 8; }
 constexpr int FEW_BLOCKS = 148 * 4;
 constexpr float DZ_UNIT = 16384.f;                  // float32: the scale of dz's planes
 
@@ -124,7 +126,7 @@ size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
 FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw)
 {
     FwdLayout l;
-    l.few = rows <= FEW_FWD;
+    l.few = rows <= few_rows(bf16);
     l.planes = bf16 || l.few ? 1 : 2;
     l.stage_x = !l.few && (!bf16 || ldx % 8);
     l.stage_w = !l.few && (!bf16 || ldw % 8);
@@ -146,7 +148,7 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
 {
     BwdLayout l;
     l.planes = bf16 ? 1 : 2;
-    l.few = rows <= FEW_FWD;
+    l.few = rows <= few_rows(bf16);
     l.gplanes = bf16 && rows > FEW_ROWS ? 1 : 2;
     l.stage_x = true;
     l.stage_w = !bf16 || ldw % 8;
@@ -210,6 +212,22 @@ __device__ __forceinline__ void block_top(float v, unsigned *top) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) v = fmaxf(v, sh[i]);
     if (v > 0.f) atomicMax(top, __float_as_uint(v));        // non-negative floats compare as their bits
+}
+
+// The same in pairs; VEC: every piece of 8 is whole and aligned.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, float2 (&v)[4]) {
+    if (!VEC) {
+        load8(p, c, cols, reinterpret_cast<float (&)[8]>(v));
+    } else if (sizeof(T) == 4) {
+        const float4 a = ld4(reinterpret_cast<const float *>(p + c)), b = ld4(reinterpret_cast<const float *>(p + c) + 4);
+        v[0] = lo(a); v[1] = hi(a); v[2] = lo(b); v[3] = hi(b);
+    } else {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p + c));
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    }
 }
 
 // How a staged matrix is scaled: not at all (bf16), each row to its own
@@ -352,15 +370,15 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
         s = __int_as_float(0x7fc00000);
     } else {
         const T *xr = x + e / k * ldx, *wr = w + v * ldw;
-#pragma unroll 2
+        float2 acc = f2(0.f, 0.f);
         for (int i = lane * 8; i < dim; i += 256) {
-            float p[8], q[8];
-            load8(xr, i, dim, p);
-            load8(wr, i, dim, q);
+            float2 p[4], q[4];
+            load8<false>(xr, i, dim, p);
+            load8<false>(wr, i, dim, q);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s = fmaf(p[j], q[j], s);
+            for (int j = 0; j < 4; ++j) acc = fma2(p[j], q[j], acc);
         }
-        s = warp_sum(s);
+        s = warp_sum(acc.x + acc.y);
     }
     if (lane) return;
     const float p = s * c;
@@ -375,37 +393,41 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
 }
 
-// Up to FEW_FWD rows: a warp takes 4 rows of w at a time, its lanes 8 columns
+// Up to few_rows() rows: a warp takes 4 rows of w at a time, its lanes 8 columns
 // each, against R rows of x (L1 holds them). Bound by reading w once. These
 // are the 4 R dot products, in every lane; pick_kernel adds in the same order.
-template <typename T, int R>
+template <typename T, int R, bool VEC>
 __device__ __forceinline__ void few_dots(const T *__restrict__ x, long long ldx, const T *__restrict__ w,
                                          long long ldw, int rows, int vocab, int dim, int v, float (&s)[R][4]) {
-    const T *wr[4];
+    const T *wr[4], *xr[R];
+    float2 acc[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) xr[r] = x + (size_t)min(r, rows - 1) * ldx;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         wr[i] = w + (size_t)min(v + i, vocab - 1) * ldw;
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r][i] = 0.f;
+        for (int r = 0; r < R; ++r) acc[r][i] = f2(0.f, 0.f);
     }
+#pragma unroll(sizeof(T) == 2 ? 2 : 1)
     for (int k = threadIdx.x % 32 * 8; k < dim; k += 256) {
-        float q[4][8];
+        float2 q[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load8(wr[i], k, dim, q[i]);
+        for (int i = 0; i < 4; ++i) load8<VEC>(wr[i], k, dim, q[i]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float p[8];
-            load8(x + (size_t)min(r, rows - 1) * ldx, k, dim, p);
+            float2 p[4];
+            load8<VEC>(xr[r], k, dim, p);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[r][i] = fmaf(p[j], q[i][j], s[r][i]);
+                for (int j = 0; j < 4; ++j) acc[r][i] = fma2(p[j], q[i][j], acc[r][i]);
         }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][i] = warp_sum(s[r][i]);
+        for (int i = 0; i < 4; ++i) s[r][i] = warp_sum(acc[r][i].x + acc[r][i].y);
 }
 
 struct FewArgs {
@@ -426,7 +448,7 @@ struct FewArgs {
 };
 
 // The log-sum-exp over a share of w's rows per CTA.
-template <typename T, int R>
+template <typename T, int R, bool VEC>
 __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 {
     __shared__ float2 sh[8][R];
@@ -441,7 +463,7 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
     }
     for (int v = (blockIdx.x * 8 + warp) * 4; v < a.vocab; v += gridDim.x * 32) {
         float s[R][4];
-        few_dots(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w), a.ldw, a.rows, a.vocab, a.dim, v, s);
+        few_dots<T, R, VEC>(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w), a.ldw, a.rows, a.vocab, a.dim, v, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float m = run[r].x;
@@ -474,7 +496,7 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 }
 
 // dz of a piece of the vocabulary, two planes.
-template <typename T, int R>
+template <typename T, int R, bool VEC>
 __global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
 {
     const int lane = threadIdx.x % 32, row = lane / 4, i = lane % 4;
@@ -483,7 +505,7 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
     const float rs = in ? a.rs[row] : 0.f, by = rs != 0.f && a.unit != 0.f ? a.unit : rs;
     for (int v = (blockIdx.x * 8 + threadIdx.x / 32) * 4; v < a.n; v += gridDim.x * 32) {
         float s[R][4];
-        few_dots(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w) + (size_t)a.v0 * a.ldw, a.ldw,
+        few_dots<T, R, VEC>(static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w) + (size_t)a.v0 * a.ldw, a.ldw,
                  a.rows, a.n, a.dim, v, s);
         float z = 0.f;                                      // lane 4 r + i takes s[r][i]
 #pragma unroll
@@ -507,20 +529,28 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
     }
 }
 
-template <typename T, int R>
+template <typename T, int R, bool VEC>
 void launch_few_rows(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
 {
-    if (backward) few_grad_kernel<T, R><<<blocks, 256, 0, s>>>(a);
-    else few_kernel<T, R><<<blocks, 256, 0, s>>>(a);
+    if (backward) few_grad_kernel<T, R, VEC><<<blocks, 256, 0, s>>>(a);
+    else few_kernel<T, R, VEC><<<blocks, 256, 0, s>>>(a);
+}
+
+template <typename T, bool VEC>
+void launch_few_vec(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
+{
+    if (a.rows == 1) launch_few_rows<T, 1, VEC>(a, blocks, backward, s);
+    else if (a.rows == 2) launch_few_rows<T, 2, VEC>(a, blocks, backward, s);
+    else if (a.rows <= 4) launch_few_rows<T, 4, VEC>(a, blocks, backward, s);
+    else launch_few_rows<T, 8, VEC>(a, blocks, backward, s);
 }
 
 template <typename T>
 void launch_few(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
 {
-    if (a.rows == 1) launch_few_rows<T, 1>(a, blocks, backward, s);
-    else if (a.rows == 2) launch_few_rows<T, 2>(a, blocks, backward, s);
-    else if (a.rows <= 4) launch_few_rows<T, 4>(a, blocks, backward, s);
-    else launch_few_rows<T, 8>(a, blocks, backward, s);
+    constexpr int PER16 = 16 / (int)sizeof(T);              // bases are 16-byte aligned
+    if (a.dim % 8 == 0 && a.ldx % PER16 == 0 && a.ldw % PER16 == 0) launch_few_vec<T, true>(a, blocks, backward, s);
+    else launch_few_vec<T, false>(a, blocks, backward, s);
 }
 
 FewArgs few_args(const HeadArgs &a, float c)
@@ -781,7 +811,7 @@ float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast
 unsigned *w_top(const HeadArgs &a, const Layout &l)
 {
     if (a.count) return reinterpret_cast<unsigned *>(a.count + 1);
-    if (a.rows <= FEW_FWD) return reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3);
+    if (a.rows <= few_rows(a.bf16)) return reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3);
     return reinterpret_cast<unsigned *>(const_cast<float *>(a.c_count) + 1);
 }
 cudaError_t top_of_w(const HeadArgs &a, unsigned *top, cudaStream_t s)

@@ -401,6 +401,9 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             item_of(q, t, tile, split, k_begin, k_end);
             tile_of(q, tile, mi, ni);
             const int m0 = mi * TM + rank * 128, n0 = ni * q.bn + rank * bhalf;
+            // the second CTA may have no rows: its part of a then stays as it is, and so does its product
+            const bool some = m0 < a.m;
+            const uint32_t a_bytes = HALF + (mi * TM + 128 < a.m ? HALF : 0);
             for (int k_first = k_begin; ok && k_first < k_end; k_first += q.part)
             for (int c = 0; ok && c < passes; ++c) {
                 int pa, pb;
@@ -413,10 +416,11 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     if (it == skip) continue;
                     const uint32_t bar = leader_addr(full + 8 * st);
-                    if (rank == 0) mbar_expect(full + 8 * st, 2 * (HALF + b_bytes));
+                    if (rank == 0) mbar_expect(full + 8 * st, a_bytes + 2 * b_bytes);
                     const uint32_t sa = tiles + st * 2 * HALF, sb = sa + HALF;
                     const int k0 = kb * BK;
-                    if (AT) {
+                    if (!some) {
+                    } else if (AT) {
                         tma3_pair(sa, &map_a, m0, k0, pa, bar);
                         tma3_pair(sa + 8192, &map_a, m0 + 64, k0, pa, bar);
                     } else {
@@ -488,7 +492,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const int m0 = mi * TM + rank * 128 + quad * 32, m = m0 + lane;
             Epilogue<KIND> ep;
             ep.begin(a, m, ni * q.bn + c0);
-            float2 sum[PARTS ? 4 : 1][16];
+            float2 sum[4][16];                               // unused without PARTS
             for (int k_first = k_begin; k_first < k_end; k_first += q.part, ++use) {
                 const int buf = use & 1;
                 // every lane polls; the warp leaves together
@@ -499,17 +503,18 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     break;
                 }
                 umma_fence_after();
+                const uint32_t from = lane_base + buf * 256 + c0;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float v[32];
                     if (32 * c < cols) {
-                        tmem_load32(lane_base + buf * 256 + c0 + 32 * c, v);
+                        tmem_load32(from + 32 * c, v);
                         tmem_wait();
                         if (PARTS) {
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 sum[c][i] = k_first > k_begin ? add2(sum[c][i], f2(v[2 * i], v[2 * i + 1]))
-                                                    : f2(v[2 * i], v[2 * i + 1]);
+                                                              : f2(v[2 * i], v[2 * i + 1]);
                         }
                     }
                     if (c == 3) {                       // read: the next multiplies may overwrite it
@@ -517,7 +522,8 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(leader_addr(tempty + 8 * buf));
                     }
-                    if (!PARTS && 32 * c < cols) ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c, v, turn);
+                    if (!PARTS && 32 * c < cols)
+                        ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c, v, turn);
                 }
             }
             if (!ok) break;
@@ -536,7 +542,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                     for (int j = 0; j < 3; ++j)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) sum[j][i] = sum[PARTS ? j + 1 : 0][i];
+                        for (int i = 0; i < 16; ++i) sum[j][i] = sum[j + 1][i];
                 }
             }
             ep.end(a, m, ni * 2 + side);
@@ -570,7 +576,7 @@ template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
     // one round of tiles is short anyway: finer parts
-    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? 2 : PART / BK;
+    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? 4 : PART / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -619,7 +625,7 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
     const int steps = q.whole ? q.steps : q.kb;
-    const bool parts = (steps * BK > PART || (steps > 2 && q.items <= N_SM / 2)) && (kind == MM_LSE || a.b.planes > 1);
+    const bool parts = (steps * BK > PART || (steps > 4 && q.items <= N_SM / 2)) && (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);
