@@ -241,16 +241,15 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * are float32, sums are float32. float32 products run on the tensor cores as
  * two scaled fp16 parts a factor (22 bits; see csrc/mms_head.cu).
  *
- * The forward writes what the backward needs: lse2 (rows, 2), the log-sum-exp
- * of z / temperature in units of log 2 as its largest term and the rest;
- * logq2 (rows, k; k = 1 for the cross entropy), log2 of q at the indices;
- * prob (rows, k)
- * = p; count (2) = the rows that count, and for float32 the largest |w|. dx (rows, dim) and dw (vocab, dim)
- * are contiguous; either may be NULL and is then not computed.
+ * The forward writes to `kept` (mms_head_kept_size() bytes) what the backward
+ * of the same inputs reads; it is not changed there. dx (rows, dim) and dw
+ * (vocab, dim) are contiguous; either may be NULL and is then not computed.
+ * Rows that are left out cost next to nothing above 512 rows: the products
+ * skip them.
  *
- * x, w, dx, dw need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.
- * The workspace (256-byte aligned) has mms_head_workspace_size() bytes, with
- * k = 0 for the cross entropy; the two directions' sizes differ.
+ * x, w, dx, dw, kept need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.
+ * The workspace (256-byte aligned) has mms_head_workspace_size() bytes; both
+ * sizes with k = 0 for the cross entropy; the two directions' sizes differ.
  * No counterpart in the reference, which computes the logits and calls
  * PyTorch's cross entropy (mamba_metal/model.py:293-297).
  */
@@ -260,28 +259,26 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
 #define MMS_REDUCE_MEAN 1
 #define MMS_REDUCE_SUM 2
 #define MMS_HEAD_MAX_K 1024
+size_t mms_head_kept_size(int rows, int k);
 size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, long long ldx,
                                long long ldw, int backward);
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction, float *loss,
-                      float *lse2, float *logq2, float *count, void *workspace,
-                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
-                      void *stream);
+                      void *kept, void *workspace, size_t workspace_bytes, int rows, int vocab,
+                      int dim, int dtype, void *stream);
 int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction,
-                      const float *dloss, const float *lse2, const float *logq2,
-                      const float *count, void *dx, void *dw, void *workspace,
+                      const float *dloss, const void *kept, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
                       void *stream);
 int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, const float *logits, int k, float temperature,
-                      int reduction, float *loss, float *lse2, float *logq2, float *prob,
-                      float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
-                      int dim, int dtype, void *stream);
+                      int reduction, float *loss, void *kept, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
+                      void *stream);
 int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, int k, float temperature, int reduction,
-                      const float *dloss, const float *lse2, const float *logq2,
-                      const float *prob, const float *count, void *dx, void *dw, void *workspace,
+                      const float *dloss, const void *kept, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype,
                       void *stream);
 

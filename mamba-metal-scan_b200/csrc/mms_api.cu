@@ -102,41 +102,29 @@ int check_head(const void *x, long long ldx, const void *w, long long ldw, int r
 }
 
 mms::HeadArgs head_args(const void *x, long long ldx, const void *w, long long ldw,
-                        const int64_t *index, int k, int reduction, void *workspace, int rows,
-                        int vocab, int dim, int dtype)
+                        const int64_t *index, int k, int reduction, void *kept, void *workspace,
+                        int rows, int vocab, int dim, int dtype)
 {
     mms::HeadArgs a{};
     a.x = x; a.w = w; a.ldx = ldx; a.ldw = ldw;
     a.rows = rows; a.vocab = vocab; a.dim = dim; a.bf16 = dtype == MMS_BF16;
-    a.index = index; a.k = k; a.tau = 1.f; a.reduction = reduction; a.workspace = workspace;
+    a.index = index; a.k = k; a.tau = 1.f; a.reduction = reduction;
+    a.kept = kept; a.workspace = workspace;
     return a;
 }
 
-int head_fwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
+int head_run(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
 {
-    if (!a.index || !a.loss || !a.lse2 || !a.logq2 || !a.count) return MMS_ERR_INVALID_ARG;
-    if (!aligned(a.index, 8) || !aligned(a.logits, 4) || !aligned(a.loss, 4) ||
-        !aligned(a.lse2, 8) || !aligned(a.logq2, 4) || !aligned(a.prob, 4) || !aligned(a.count, 4))
+    if (!a.index || !a.kept || !(a.backward ? a.dloss : a.loss)) return MMS_ERR_INVALID_ARG;
+    if (!aligned(a.index, 8) || !aligned(a.logits, 4) || !aligned(a.loss, 4) || !aligned(a.dloss, 4) ||
+        !aligned(a.kept, 16) || !aligned(a.dx, 16) || !aligned(a.dw, 16))
         return MMS_ERR_MISALIGNED;
     if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.kd ? a.k : 0,
-                                                                    a.bf16, a.ldx, a.ldw, false))
+                                                                    a.bf16, a.ldx, a.ldw, a.backward))
         return MMS_ERR_WORKSPACE;
     if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
-    return status_of(mms::launch_head_fwd(a, static_cast<cudaStream_t>(stream)));
-}
-
-int head_bwd(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
-{
-    if (!a.index || !a.dloss || !a.c_lse2 || !a.c_logq2 || !a.c_count) return MMS_ERR_INVALID_ARG;
-    if (!aligned(a.index, 8) || !aligned(a.dloss, 4) || !aligned(a.c_lse2, 8) ||
-        !aligned(a.c_logq2, 4) || !aligned(a.c_prob, 4) || !aligned(a.c_count, 4) ||
-        !aligned(a.dx, 16) || !aligned(a.dw, 16))
-        return MMS_ERR_MISALIGNED;
-    if (!a.workspace || workspace_bytes < mms::head_workspace_bytes(a.rows, a.vocab, a.dim, a.kd ? a.k : 0,
-                                                                    a.bf16, a.ldx, a.ldw, true))
-        return MMS_ERR_WORKSPACE;
-    if (!aligned(a.workspace, 256)) return MMS_ERR_MISALIGNED;
-    return status_of(mms::launch_head_bwd(a, static_cast<cudaStream_t>(stream)));
+    return status_of(a.backward ? mms::launch_head_bwd(a, static_cast<cudaStream_t>(stream))
+                                : mms::launch_head_fwd(a, static_cast<cudaStream_t>(stream)));
 }
 
 int check_norm(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
@@ -323,63 +311,65 @@ size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, l
     return mms::head_workspace_bytes(rows, vocab, dim, k, dtype == MMS_BF16, ldx, ldw, backward != 0);
 }
 
+size_t mms_head_kept_size(int rows, int k)
+{
+    if (rows < 1 || rows > (1 << 24) || k < 0 || k > MMS_HEAD_MAX_K) return 0;
+    return mms::head_kept_bytes(rows, k ? k : 1, k != 0);
+}
+
 int mms_linear_ce_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction, float *loss,
-                      float *lse2, float *logq2, float *count, void *workspace,
-                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
+                      void *kept, void *workspace, size_t workspace_bytes, int rows, int vocab,
+                      int dim, int dtype, void *stream)
 {
     const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, 1, 1.f, dtype, reduction);
     if (rc) return rc;
-    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, kept, workspace, rows, vocab, dim, dtype);
     a.ignore_index = ignore_index;
-    a.loss = loss; a.lse2 = lse2; a.logq2 = logq2; a.count = count;
-    return head_fwd(a, workspace_bytes, stream);
+    a.loss = loss;
+    return head_run(a, workspace_bytes, stream);
 }
 
 int mms_linear_ce_bwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *target, int64_t ignore_index, int reduction,
-                      const float *dloss, const float *lse2, const float *logq2,
-                      const float *count, void *dx, void *dw, void *workspace,
+                      const float *dloss, const void *kept, void *dx, void *dw, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
 {
     const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, 1, 1.f, dtype, reduction);
     if (rc) return rc;
-    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, workspace, rows, vocab, dim, dtype);
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, target, 1, reduction, const_cast<void *>(kept), workspace, rows,
+                                vocab, dim, dtype);
     a.ignore_index = ignore_index;
-    a.dloss = dloss; a.c_lse2 = lse2; a.c_logq2 = logq2; a.c_count = count;
-    a.dx = dx; a.dw = dw;
-    return head_bwd(a, workspace_bytes, stream);
+    a.backward = true; a.dloss = dloss; a.dx = dx; a.dw = dw;
+    return head_run(a, workspace_bytes, stream);
 }
 
 int mms_linear_kd_fwd(const void *x, long long ldx, const void *w, long long ldw,
                       const int64_t *index, const float *logits, int k, float temperature,
-                      int reduction, float *loss, float *lse2, float *logq2, float *prob,
-                      float *count, void *workspace, size_t workspace_bytes, int rows, int vocab,
-                      int dim, int dtype, void *stream)
-{
-    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, k, temperature, dtype, reduction);
-    if (rc) return rc;
-    if (!logits || !prob) return MMS_ERR_INVALID_ARG;
-    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
-    a.kd = true; a.tau = temperature; a.logits = logits;
-    a.loss = loss; a.lse2 = lse2; a.logq2 = logq2; a.prob = prob; a.count = count;
-    return head_fwd(a, workspace_bytes, stream);
-}
-
-int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
-                      const int64_t *index, int k, float temperature, int reduction,
-                      const float *dloss, const float *lse2, const float *logq2,
-                      const float *prob, const float *count, void *dx, void *dw, void *workspace,
+                      int reduction, float *loss, void *kept, void *workspace,
                       size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
 {
     const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, k, temperature, dtype, reduction);
     if (rc) return rc;
-    if (!prob) return MMS_ERR_INVALID_ARG;
-    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, workspace, rows, vocab, dim, dtype);
+    if (!logits) return MMS_ERR_INVALID_ARG;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, kept, workspace, rows, vocab, dim, dtype);
+    a.kd = true; a.tau = temperature; a.logits = logits;
+    a.loss = loss;
+    return head_run(a, workspace_bytes, stream);
+}
+
+int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw,
+                      const int64_t *index, int k, float temperature, int reduction,
+                      const float *dloss, const void *kept, void *dx, void *dw, void *workspace,
+                      size_t workspace_bytes, int rows, int vocab, int dim, int dtype, void *stream)
+{
+    const int rc = check_head(x, ldx, w, ldw, rows, vocab, dim, k, temperature, dtype, reduction);
+    if (rc) return rc;
+    mms::HeadArgs a = head_args(x, ldx, w, ldw, index, k, reduction, const_cast<void *>(kept), workspace, rows,
+                                vocab, dim, dtype);
     a.kd = true; a.tau = temperature;
-    a.dloss = dloss; a.c_lse2 = lse2; a.c_logq2 = logq2; a.c_prob = prob; a.c_count = count;
-    a.dx = dx; a.dw = dw;
-    return head_bwd(a, workspace_bytes, stream);
+    a.backward = true; a.dloss = dloss; a.dx = dx; a.dw = dw;
+    return head_run(a, workspace_bytes, stream);
 }
 
 size_t mms_norm_workspace_size(int rows, int dim)

@@ -18,6 +18,11 @@
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
 // workspace; the two products with dz follow piece by piece (6 more).
 //
+// Rows that do not count (an ignored target, an empty list) take no part: with
+// more than MAP_ROWS rows a map lists those that do (map_kernel), x is staged
+// in that order, everything between works on the listed rows, and the products
+// read their number from the device. The host never learns it.
+//
 // Forward:   products (MM_LSE) -> one (max, sum) per row and half tile, joined
 //            by lse_kernel. The logits at the indices are the product's own
 //            values, so that its errors cancel against lse2's; the
@@ -67,6 +72,7 @@ namespace {
 constexpr float LN2 = 0.6931471805599453f;
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // bound on one staged or dz piece
 constexpr int FEW_ROWS = 256;
+constexpr int MAP_ROWS = 512;                       // two tiles of rows: with fewer there is little to leave out
 // Rows that the CUDA cores take: at 50176 x 1024 they need (us, forward) 34, 49, 45, 68 for 1, 2,
 // 4, 8 rows of float32, where staging alone is 100; in bf16 20, 20, 36, 58, the tensor cores 31.
 int few_rows(bool bf16) { return bf16 ? 2 : 8; }
@@ -97,9 +103,26 @@ struct Layout {
     size_t total;
 };
 
+// What the forward keeps for the backward.
+struct Kept {
+    float2 *lse2;       // (rows)
+    float *logq2;       // (rows, k)
+    float *prob;        // (rows, k), distillation
+    float *count;       // (2): the rows that count; float32: the largest |w|
+    int *map, *live;    // more than MAP_ROWS rows: those that count, and their number
+};
+
+// Row i of the listed rows, and how many there are.
+struct RowMap {
+    const int *map, *live;
+    __device__ __forceinline__ int n(int rows) const { return live ? *live : rows; }
+    __device__ __forceinline__ int row(int i) const { return map ? map[i] : i; }
+};
+
 struct FwdLayout : Layout {
     bool few;
     size_t col, pos, before;        // the distillation's sorted lists
+    size_t flags;                   // the distillation's rows that count
     size_t part, rowloss, rest;
 };
 
@@ -128,7 +151,7 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long l
     FwdLayout l;
     l.few = rows <= few_rows(bf16);
     l.planes = bf16 || l.few ? 1 : 2;
-    l.stage_x = !l.few && (!bf16 || ldx % 8);
+    l.stage_x = !l.few && (!bf16 || ldx % 8 || rows > MAP_ROWS);
     l.stage_w = !l.few && (!bf16 || ldw % 8);
     size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * sizeof(float2) / 32 + 1);
     const int parts = l.few ? FEW_BLOCKS : std::max(mm_lse_parts(rows, l.piece, dim, l.planes, l.planes),
@@ -137,6 +160,7 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long l
     l.rowloss = o; o += up256((size_t)rows * sizeof(float));
     l.rest = o; o += up256((size_t)rows * std::max(k, 1) * sizeof(float));
     const size_t lists = l.few ? 0 : (size_t)rows * k, blocks = lists ? (size_t)(vocab - 1) / LIST_BLOCK + 1 : 0;
+    l.flags = o; o += k && rows > MAP_ROWS ? up256(rows) : 0;
     l.col = o; o += up256(lists * sizeof(int));
     l.pos = o; o += up256(lists * sizeof(uint16_t));
     l.before = o; o += up256(blocks * rows * sizeof(uint16_t));
@@ -159,8 +183,8 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
     l.dxacc = o; o += l.piece < vocab ? up256((size_t)rows * dim * sizeof(float)) : 0;
     l.rs = o; o += up256((size_t)rows * sizeof(float));
     // partial sums; the last, smaller piece splits as far as this room goes
-    l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.gplanes, l.planes),
-                             mm_split_bytes(l.piece, dim, rows, l.gplanes, l.planes));
+    l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.gplanes, l.planes, rows > MAP_ROWS),
+                             mm_split_bytes(l.piece, dim, rows, l.gplanes, l.planes, false));
     l.split = o; o += up256(l.split_bytes);
     l.total = o;
     return l;
@@ -241,6 +265,7 @@ struct StageArgs {
     long long ld, plane;
     int rows, cols;
     const float *rs;            // ST_COPY, ST_ROWS: rows with 0 there become 0; ST_WHOLE: factors of the rows
+    RowMap rows_map;            // row i of `out` comes from there; rows beyond them are 0
     float *mul;                 // ST_ROWS: 2^-e of each row; ST_WHOLE: of all
     unsigned *top;              // ST_WHOLE: the maximum's bits; ST_ROWS: the maximum of |rs| row maximum goes here
 };
@@ -252,12 +277,14 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
     const int lane = threadIdx.x % LP;
     float top = 0.f;
     constexpr int RW = 32 / LP;                             // rows a warp has at once
-    for (int r0 = (blockIdx.x * 8 + threadIdx.x / 32) * RW; r0 < a.rows; r0 += gridDim.x * 8 * RW) {
+    // a last tile's padding is 0: nothing behind it is read
+    const int live = a.rows_map.n(a.rows), rows = min(a.rows, (max(live, 1) + 255) / 256 * 256);
+    for (int r0 = (blockIdx.x * 8 + threadIdx.x / 32) * RW; r0 < rows; r0 += gridDim.x * 8 * RW) {
         const int r = r0 + threadIdx.x % 32 / LP;           // lanes beyond the rows stay for the shuffles
-        const bool in = r < a.rows;
-        const T *src = static_cast<const T *>(a.src) + (size_t)r * a.lds;
+        const bool in = r < rows;
+        const T *src = static_cast<const T *>(a.src) + (size_t)(r < live ? a.rows_map.row(r) : 0) * a.lds;
         uint16_t *out = a.out + (size_t)r * a.ld;
-        const float rs = !in ? 0.f : a.rs ? a.rs[r] : 1.f;
+        const float rs = r >= live ? 0.f : a.rs ? a.rs[r] : 1.f;
         const int cols = rs == 0.f ? 0 : a.cols;            // nothing of a left-out row is read
         Pow2 by{1.f, 1.f};
         if (KIND == ST_ROWS) {
@@ -564,15 +591,16 @@ FewArgs few_args(const HeadArgs &a, float c)
 // The distillation's lists in ascending order, a warp a row: an entry's place
 // is the number of entries before it. Indices outside the vocabulary go last.
 __global__ void __launch_bounds__(256)
-order_kernel(const int64_t *__restrict__ index, int k, int rows, int vocab, int *__restrict__ col,
+order_kernel(const int64_t *__restrict__ index, int k, int rows, RowMap rm, int vocab, int *__restrict__ col,
              uint16_t *__restrict__ pos, float *__restrict__ logq2, float *__restrict__ rest)
 {
     extern __shared__ int sh_index[];
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (m >= rows) return;
+    if (m >= rm.n(rows)) return;
     int *v = sh_index + threadIdx.x / 32 * k;
+    const int64_t *from = index + (size_t)rm.row(m) * k;
     for (int j = lane; j < k; j += 32) {
-        const int64_t t = index[(size_t)m * k + j];
+        const int64_t t = from[j];
         v[j] = t < 0 || t >= vocab ? INT_MAX : (int)t;
         // no product will come for these
         if (v[j] == INT_MAX) {
@@ -594,10 +622,10 @@ order_kernel(const int64_t *__restrict__ index, int k, int rows, int vocab, int 
 // before[b * rows + m]: entries of row m below column LIST_BLOCK * b. A thread
 // a row (32 a CTA, so that the stores are whole sectors) and 1/8 of the blocks.
 __global__ void __launch_bounds__(256)
-before_kernel(const int *__restrict__ col, int k, int rows, int blocks, uint16_t *__restrict__ before)
+before_kernel(const int *__restrict__ col, int k, int rows, RowMap rm, int blocks, uint16_t *__restrict__ before)
 {
     const int m = blockIdx.x * 32 + threadIdx.x % 32;
-    if (m >= rows) return;
+    if (m >= rm.n(rows)) return;
     const int each = (blocks + 7) / 8, b0 = threadIdx.x / 32 * each, b1 = min(blocks, b0 + each);
     const int *c = col + (size_t)m * k;
     int lo = 0, hi = k;                                     // the first entry not below b0's column
@@ -618,16 +646,16 @@ before_kernel(const int *__restrict__ col, int k, int rows, int blocks, uint16_t
 // lse2 and, from the target's logit in logq2, the cross entropy's row loss;
 // with `total` (up to 32 rows) total_kernel's work too.
 __global__ void __launch_bounds__(1024)
-lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__restrict__ lse2,
+lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm, float2 *__restrict__ lse2,
            const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
            const float *__restrict__ rest, float *__restrict__ loss, int reduction,
            float *__restrict__ total, float *__restrict__ count)
 {
     __shared__ float2 sh[32][33];
     __shared__ float row_loss[32];
-    const int m = blockIdx.x * 32 + threadIdx.x;
+    const int m = blockIdx.x * 32 + threadIdx.x, live = rm.n(rows);
     float2 v = make_float2(-INFINITY, 0.f);
-    if (m < rows)
+    if (m < live)
 #pragma unroll 4
         for (int t = threadIdx.y + (first ? 1 : 0); t <= ntiles; t += 32)
             v = join(v, part[(size_t)t * rows + m]);
@@ -639,7 +667,7 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
     for (int o = 16; o; o >>= 1)
         v = join(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
     const int r = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && r < rows) {
+    if (threadIdx.x == 0 && r < live) {
         if (!last) {
             part[r] = v;
         } else {
@@ -647,11 +675,11 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
             lse2[r] = v;
         }
         if (last && target) {
-            const int64_t t = target[r];
+            const int64_t t = target[rm.row(r)];
             float l = 0.f;
             if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - v.y;
             logq2[r] = l;
-            loss[r] = row_loss[threadIdx.y] = -LN2 * l;
+            loss[reduction == MMS_REDUCE_NONE ? rm.row(r) : r] = row_loss[threadIdx.y] = -LN2 * l;
         }
     }
     if (!total) return;                                     // one CTA has all rows
@@ -671,21 +699,24 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, float2 *__
 __global__ void __launch_bounds__(256)
 kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, float tau,
           const float2 *__restrict__ lse2, float *__restrict__ logq2,
-          const float *__restrict__ rest, float *__restrict__ prob, float *__restrict__ loss, int rows)
+          const float *__restrict__ rest, float *__restrict__ prob, float *__restrict__ loss, int rows, RowMap rm,
+          int reduction)
 {
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (m >= rows) return;
+    if (m >= rm.n(rows)) return;
     const size_t o = (size_t)m * k;
+    index += (size_t)rm.row(m) * k;
+    logits += (size_t)rm.row(m) * k;
     const float inv = 1.f / tau;
     const float2 l2 = lse2[m];
     float top = -INFINITY;
     for (int j = lane; j < k; j += 32)
-        if (index[o + j] >= 0) top = fmaxf(top, logits[o + j]);
+        if (index[j] >= 0) top = fmaxf(top, logits[j]);
     top = warp_max(top);
     float sum = 0.f;
     for (int j = lane; j < k; j += 32)
-        if (index[o + j] >= 0 && !(top == -INFINITY && logits[o + j] == -INFINITY))
-            sum += expf((logits[o + j] - top) * inv);
+        if (index[j] >= 0 && !(top == -INFINITY && logits[j] == -INFINITY))
+            sum += expf((logits[j] - top) * inv);
     sum = warp_sum(sum);
     const float log_sum = logf(sum), over = 1.f / sum;
     const bool some = sum != 0.f;                       // NaN counts as some
@@ -694,15 +725,15 @@ kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, i
         float p = 0.f;
         const float lq = ((logq2[o + j] - l2.x) + rest[o + j]) - l2.y;
         logq2[o + j] = lq;
-        if (some && index[o + j] >= 0) {
-            const float t = (logits[o + j] - top) * inv;
+        if (some && index[j] >= 0) {
+            const float t = (logits[j] - top) * inv;
             p = expf(t) * over;
             if (p != 0.f) acc += p * ((t - log_sum) - LN2 * lq);
         }
         prob[o + j] = p;
     }
     acc = warp_sum(acc);
-    if (lane == 0) loss[m] = some ? tau * tau * acc : 0.f;
+    if (lane == 0) loss[reduction == MMS_REDUCE_NONE ? rm.row(m) : m] = some ? tau * tau * acc : 0.f;
 }
 
 // Whether row m counts.
@@ -717,14 +748,15 @@ __device__ __forceinline__ bool row_counts(const int64_t *index, const float *pr
 // count, and loss = the rows' sum (over count for a mean), in a fixed order.
 __global__ void __launch_bounds__(1024)
 total_kernel(const float *__restrict__ rowloss, const int64_t *__restrict__ index,
-             const float *__restrict__ prob, int k, int64_t ignore, int rows, int reduction,
+             const float *__restrict__ prob, int k, int64_t ignore, int rows, RowMap rm, int reduction,
              float *__restrict__ loss, float *__restrict__ count)
 {
     __shared__ float sh[2][32];
     float s = 0.f, n = 0.f;
-    for (int m = threadIdx.x; m < rows; m += 1024) {
-        s += rowloss[m];
-        n += row_counts(index, prob, k, ignore, m) ? 1.f : 0.f;
+    const int live = rm.n(rows);
+    for (int m = threadIdx.x; m < live; m += 1024) {
+        if (reduction != MMS_REDUCE_NONE) s += rowloss[m];
+        n += rm.live || row_counts(index, prob, k, ignore, m) ? 1.f : 0.f;
     }
     s = warp_sum(s);
     n = warp_sum(n);
@@ -748,14 +780,16 @@ total_kernel(const float *__restrict__ rowloss, const int64_t *__restrict__ inde
 __global__ void rows_kernel(const float *__restrict__ dloss, const float *__restrict__ count,
                             const int64_t *__restrict__ index, const float *__restrict__ prob,
                             const float *__restrict__ logq2, int k, int64_t ignore, int reduction,
-                            float tau, float *__restrict__ rs, float *whole, int rows)
+                            float tau, float *__restrict__ rs, float *whole, float *zero, int rows, RowMap rm)
 {
     const int m = blockIdx.x * blockDim.x + threadIdx.x;
+    if (m == 0 && zero) *zero = 0.f;
     if (m >= rows) return;
-    float r = dloss[reduction == MMS_REDUCE_NONE ? m : 0] * tau;
+    const bool live = m < rm.n(rows);
+    float r = dloss[reduction != MMS_REDUCE_NONE ? 0 : live ? rm.row(m) : m] * tau;
     if (reduction == MMS_REDUCE_MEAN) r /= *count;
     if (m == 0 && whole) *whole = r;
-    if (!row_counts(index, prob, k, ignore, m)) r = 0.f;
+    if (!live || (!rm.live && !row_counts(index, prob, k, ignore, m))) r = 0.f;
     if (r != 0.f)
         for (int j = 0; j < k; ++j) {
             const float z = logq2[(size_t)m * k + j];
@@ -764,18 +798,61 @@ __global__ void rows_kernel(const float *__restrict__ dloss, const float *__rest
     rs[m] = r;
 }
 
+// flags[m]: whether the teacher's list has an entry with index >= 0 and a logit above -inf.
+__global__ void __launch_bounds__(256)
+flags_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, int rows,
+             uint8_t *__restrict__ flags)
+{
+    const int m = blockIdx.x * 8 + threadIdx.x / 32;
+    if (m >= rows) return;
+    bool some = false;
+    for (int j = threadIdx.x % 32; j < k; j += 32)
+        some |= index[(size_t)m * k + j] >= 0 && logits[(size_t)m * k + j] != -INFINITY;
+    some = __any_sync(~0u, some);
+    if (threadIdx.x % 32 == 0) flags[m] = some;
+}
+
+// The rows that count, in order, and their number: one CTA, 1024 rows at a time.
+__global__ void __launch_bounds__(1024)
+map_kernel(const int64_t *__restrict__ target, int64_t ignore, const uint8_t *__restrict__ flags, int rows,
+           int *__restrict__ map, int *__restrict__ live)
+{
+    __shared__ int sh[32];
+    int base = 0;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int m0 = 0; m0 < rows; m0 += 1024) {
+        const int m = m0 + threadIdx.x;
+        const bool in = m < rows && (flags ? flags[m] != 0 : target[m] != ignore);
+        const unsigned vote = __ballot_sync(~0u, in);
+        if (lane == 0) sh[warp] = __popc(vote);
+        __syncthreads();
+        int at = sh[lane];                                  // inclusive sums of the 32 warps' counts
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(~0u, at, o);
+            if (lane >= o) at += t;
+        }
+        const int all = __shfl_sync(~0u, at, 31);
+        const int before = warp ? __shfl_sync(~0u, at, warp - 1) : 0;
+        if (in) map[base + before + __popc(vote & ((1u << lane) - 1))] = m;
+        base += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *live = base;
+}
+
 // dz at the sparse entries that lie in this piece of the vocabulary; `unit` in
 // place of r if it is not 0.
 __global__ void __launch_bounds__(256)
 sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
-              const float *__restrict__ logq2, const float *__restrict__ rs, float unit, int k, long long n, int v0, int v1,
+              const float *__restrict__ logq2, const float *__restrict__ rs, float unit, int k, int rows, RowMap rm, int v0, int v1,
               uint16_t *__restrict__ g, long long ldg, long long gplane, int planes, bool fp16)
 {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= n) return;
-    const int64_t v = index[e];
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x, m = e / k;
+    if (m >= rm.n(rows)) return;
+    const int64_t *list = index + (size_t)rm.row((int)m) * k;
+    const int64_t v = list[e - m * k];
     if (v < v0 || v >= v1) return;
-    const long long m = e / k;
     const float r = rs[m];
     if (r == 0.f) return;                               // dz is 0 there already
     uint16_t *o = g + m * ldg + (v - v0);
@@ -783,10 +860,9 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
     if (prob) {                                         // an index may occur twice: the first one writes
         p = 0.f;
         for (int j = 0; j < k; ++j) {
-            const long long f = m * k + j;
-            if (index[f] != v) continue;
-            if (f < e) return;
-            p += prob[f];
+            if (list[j] != v) continue;
+            if (m * k + j < e) return;
+            p += prob[m * k + j];
         }
     }
     d = (unit != 0.f ? unit : r) * (d + (1.f - p));
@@ -804,15 +880,34 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
 }
 
 uint16_t *u16(void *base, size_t off) { return reinterpret_cast<uint16_t *>(static_cast<char *>(base) + off); }
+size_t kept_layout(int rows, int k, bool kd, char *base, Kept &o)
+{
+    size_t at = 0;
+    const auto take = [&](size_t bytes) { char *p = base + at; at += (bytes + 15) / 16 * 16; return p; };
+    o.lse2 = reinterpret_cast<float2 *>(take((size_t)rows * sizeof(float2)));
+    o.logq2 = reinterpret_cast<float *>(take((size_t)rows * k * sizeof(float)));
+    o.prob = kd ? reinterpret_cast<float *>(take((size_t)rows * k * sizeof(float))) : nullptr;
+    o.count = reinterpret_cast<float *>(take(2 * sizeof(float)));
+    const bool mapped = rows > MAP_ROWS;
+    o.live = mapped ? reinterpret_cast<int *>(take(sizeof(int))) : nullptr;
+    o.map = mapped ? reinterpret_cast<int *>(take((size_t)rows * sizeof(int))) : nullptr;
+    return at;
+}
+Kept kept_of(const HeadArgs &a)
+{
+    Kept o;
+    kept_layout(a.rows, a.k, a.kd, static_cast<char *>(a.kept), o);
+    return o;
+}
+
 float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast<char *>(base) + off); }
 
 // Where w's largest magnitude is: the forward keeps it for the backward
 // (count[1]), but for few rows, whose forward does not need it.
 unsigned *w_top(const HeadArgs &a, const Layout &l)
 {
-    if (a.count) return reinterpret_cast<unsigned *>(a.count + 1);
-    if (a.rows <= few_rows(a.bf16)) return reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 3);
-    return reinterpret_cast<unsigned *>(const_cast<float *>(a.c_count) + 1);
+    return reinterpret_cast<unsigned *>(a.backward && a.rows <= few_rows(a.bf16) ? fl(a.workspace, l.muls) + 3
+                                                                                 : kept_of(a).count + 1);
 }
 cudaError_t top_of_w(const HeadArgs &a, unsigned *top, cudaStream_t s)
 {
@@ -830,18 +925,18 @@ Factor w_factor(const HeadArgs &a, const Layout &l, int v0, int n, cudaStream_t 
     const long long ld = padded(a.dim);
     float *muls = fl(a.workspace, l.muls);
     StageArgs st{static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4), a.ldw,
-                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, muls, w_top(a, l)};
+                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, RowMap{}, muls, w_top(a, l)};
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
     else stage<float, ST_WHOLE>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
 }
 
 // x as a factor of z: staged (rows with rs = 0 as zeros), or x itself.
-Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, cudaStream_t s)
+Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, RowMap rm, cudaStream_t s)
 {
     if (!l.stage_x) return Factor{static_cast<const uint16_t *>(a.x), a.ldx, 0, 1, false};
     const long long ld = padded(a.dim);
-    StageArgs st{a.x, a.ldx, u16(a.workspace, l.xs), ld, ld * a.rows, a.rows, a.dim, rs,
+    StageArgs st{a.x, a.ldx, u16(a.workspace, l.xs), ld, ld * a.rows, a.rows, a.dim, rs, rm,
                  fl(a.workspace, l.row_mul),
                  rs ? reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 2) : nullptr};
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
@@ -850,6 +945,12 @@ Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, cudaStream_
 }
 
 }  // namespace
+
+size_t head_kept_bytes(int rows, int k, bool kd)
+{
+    Kept o;
+    return kept_layout(rows, k, kd, nullptr, o);
+}
 
 size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw,
                             bool backward)
@@ -861,45 +962,54 @@ size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long
 cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
 {
     const FwdLayout l = fwd_layout(a.rows, a.vocab, a.dim, a.kd ? a.k : 0, a.bf16, a.ldx, a.ldw);
+    const Kept o = kept_of(a);
+    const RowMap rm{o.map, o.live};
     const float c = MMS_LOG2E / a.tau;
+    const bool none = a.reduction == MMS_REDUCE_NONE;
     float2 *part = reinterpret_cast<float2 *>(fl(a.workspace, l.part));
-    float *rowloss = a.reduction == MMS_REDUCE_NONE ? a.loss : fl(a.workspace, l.rowloss);
-    float *rest = fl(a.workspace, l.rest);
+    float *rowloss = none ? a.loss : fl(a.workspace, l.rowloss), *rest = fl(a.workspace, l.rest);
     float *total = a.kd || a.rows > 32 ? nullptr : a.loss;
-    cudaError_t e;
     const int64_t *target = a.kd ? nullptr : a.index;
+    cudaError_t e;
+    if (rm.live) {
+        uint8_t *flags = a.kd ? static_cast<uint8_t *>(a.workspace) + l.flags : nullptr;
+        if (a.kd) flags_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.rows, flags);
+        map_kernel<<<1, 1024, 0, stream>>>(a.index, a.ignore_index, flags, a.rows, o.map, o.live);
+        // the rows that are left out
+        if (none && (e = cudaMemsetAsync(a.loss, 0, (size_t)a.rows * sizeof(float), stream)) != cudaSuccess) return e;
+    }
     Lists lists{};
     if (a.kd && l.few) {
         const int n = a.rows * a.k;
         if (a.bf16)
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w), a.ldw,
-                a.index, a.k, c, a.logq2, rest, n, a.vocab, a.dim);
+                a.index, a.k, c, o.logq2, rest, n, a.vocab, a.dim);
         else
             pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
                 static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index, a.k, c,
-                a.logq2, rest, n, a.vocab, a.dim);
+                o.logq2, rest, n, a.vocab, a.dim);
     } else if (a.kd) {
         int *col = reinterpret_cast<int *>(fl(a.workspace, l.col));
         uint16_t *pos = u16(a.workspace, l.pos), *before = u16(a.workspace, l.before);
-        order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, a.vocab, col,
-                                                                                pos, a.logq2, rest);
-        before_kernel<<<ceil_div(a.rows, 32), 256, 0, stream>>>(col, a.k, a.rows, (a.vocab - 1) / LIST_BLOCK + 1,
+        order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, rm, a.vocab,
+                                                                                col, pos, o.logq2, rest);
+        before_kernel<<<ceil_div(a.rows, 32), 256, 0, stream>>>(col, a.k, a.rows, rm, (a.vocab - 1) / LIST_BLOCK + 1,
                                                                before);
         lists = Lists{col, pos, before, a.k, a.rows};
     }
     if (l.few) {
         const int blocks = std::min(ceil_div(a.vocab, 32), FEW_BLOCKS);
         FewArgs f = few_args(a, c);
-        f.target = target; f.at = a.logq2; f.rest = rest; f.part = part + a.rows;
+        f.target = target; f.at = o.logq2; f.rest = rest; f.part = part + a.rows;
         if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, false, stream);
         else launch_few<float>(f, blocks, false, stream);
-        lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows,
-                                                  reinterpret_cast<float2 *>(a.lse2), target,
-                                                  a.ignore_index, a.vocab, a.logq2, rest, rowloss, a.reduction, total, a.count);
+        lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows, rm, o.lse2, target,
+                                                  a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction,
+                                                  total, o.count);
     }
     if (l.planes > 1 && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
-    const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, stream);
+    const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, rm, stream);
     for (int v0 = l.few ? a.vocab : 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
         MmArgs mm{};
@@ -907,6 +1017,8 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.b = w_factor(a, l, v0, nv, stream);
         mm.fp16 = !a.bf16;
         mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
+        mm.live = rm.live;
+        mm.row_of = rm.map;
         if (l.planes > 1) {
             mm.row_mul = fl(a.workspace, l.row_mul);
             mm.mul = fl(a.workspace, l.muls);
@@ -915,44 +1027,47 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.target = target;
         mm.lists = lists;
         mm.first_col = v0;
-        mm.at = a.logq2;
+        mm.at = o.logq2;
         mm.rest = rest;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
-            part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows,
-            reinterpret_cast<float2 *>(a.lse2), target, a.ignore_index, a.vocab, a.logq2, rest, rowloss, a.reduction, total, a.count);
+            part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows, rm,
+            o.lse2, target, a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction, total, o.count);
     }
     if (a.kd)
-        kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau,
-                                                          reinterpret_cast<const float2 *>(a.lse2),
-                                                          a.logq2, rest, a.prob, rowloss, a.rows);
+        kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau, o.lse2, o.logq2, rest,
+                                                          o.prob, rowloss, a.rows, rm, a.reduction);
     if (!total)
-        total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, a.kd ? a.prob : nullptr, a.k,
-                                         a.ignore_index, a.rows, a.reduction, a.loss, a.count);
+        total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, o.prob, a.k, a.ignore_index, a.rows, rm, a.reduction,
+                                             a.loss, o.count);
     return cudaGetLastError();
 }
 
 cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
 {
     const BwdLayout l = bwd_layout(a.rows, a.vocab, a.dim, a.bf16, a.ldw);
+    const Kept o = kept_of(a);
+    const RowMap rm{o.map, o.live};
     const float c = MMS_LOG2E / a.tau;
-    const float *prob = a.kd ? a.c_prob : nullptr;
+    const bool f32 = l.planes > 1;
     // bf16, all rows alike: dz without r, which comes in with the products' factors
     const bool uniform = a.bf16 && a.reduction != MMS_REDUCE_NONE;
     float *rs = fl(a.workspace, l.rs), *acc = fl(a.workspace, l.dxacc);
-    rows_kernel<<<ceil_div(a.rows, 256), 256, 0, stream>>>(a.dloss, a.c_count, a.index, prob,
-                                                           a.c_logq2, a.k, a.ignore_index,
-                                                           a.reduction, a.tau, rs,
-                                                           uniform ? fl(a.workspace, l.muls) + 1 : nullptr, a.rows);
-    cudaError_t e;
-    const bool f32 = l.planes > 1;
     float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
-    if (f32 && (e = cudaMemsetAsync(muls + 2, 0, sizeof(float), stream)) != cudaSuccess) return e;
+    rows_kernel<<<ceil_div(a.rows, 256), 256, 0, stream>>>(a.dloss, o.count, a.index, o.prob, o.logq2, a.k,
+                                                           a.ignore_index, a.reduction, a.tau, rs,
+                                                           uniform ? muls + 1 : nullptr, f32 ? muls + 2 : nullptr,
+                                                           a.rows, rm);
+    cudaError_t e;
     if (f32 && l.few && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
-    const Factor x = x_factor(a, l, rs, stream);
+    // the rows that are left out
+    if (rm.live && a.dx &&
+        (e = cudaMemsetAsync(a.dx, 0, (size_t)a.rows * a.dim * (a.bf16 ? 2 : 4), stream)) != cudaSuccess)
+        return e;
+    const Factor x = x_factor(a, l, rs, rm, stream);
     Factor xr = x;                                      // the factor of dw: x, or r x
     if (f32) {
-        StageArgs st{a.x, a.ldx, u16(a.workspace, l.xr), x.ld, x.plane, a.rows, a.dim, rs, muls + 1,
+        StageArgs st{a.x, a.ldx, u16(a.workspace, l.xr), x.ld, x.plane, a.rows, a.dim, rs, rm, muls + 1,
                      reinterpret_cast<unsigned *>(muls + 2)};
         stage<float, ST_WHOLE>(st, stream);
         xr.p = st.out;
@@ -969,15 +1084,16 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         mm.b = w_factor(a, l, v0, nv, stream);
         mm.fp16 = f32;
         mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
+        mm.live = rm.live;
         if (f32) {
             mm.row_mul = row_mul;
             mm.mul = muls;
         }
-        mm.lse2 = reinterpret_cast<const float2 *>(a.c_lse2); mm.rs = rs; mm.g_unit = unit;
+        mm.lse2 = o.lse2; mm.rs = rs; mm.g_unit = unit;
         mm.g = g; mm.ldg = l.ldg; mm.gplane = gplane; mm.gplanes = l.gplanes;
         if (l.few) {
             FewArgs f = few_args(a, c);
-            f.lse2 = mm.lse2; f.rs = rs; f.unit = unit; f.g = g; f.ldg = l.ldg; f.gplane = gplane;
+            f.lse2 = o.lse2; f.rs = rs; f.unit = unit; f.g = g; f.ldg = l.ldg; f.gplane = gplane;
             f.v0 = v0; f.n = nv;
             const int blocks = std::min(ceil_div(nv, 32), FEW_BLOCKS);
             if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, true, stream);
@@ -985,12 +1101,13 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         } else if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) {
             return e;
         }
-        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, prob, a.c_logq2, rs, unit, a.k, n, v0,
+        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, o.prob, o.logq2, rs, unit, a.k, a.rows, rm, v0,
                                                             v0 + nv, g, l.ldg, gplane, l.gplanes, f32);
         MmArgs out{};
         out.fp16 = f32;
         out.c = f32 ? 1.f / DZ_UNIT : 1.f;
         out.n = a.dim;
+        out.live = rm.live;
         out.split = fl(a.workspace, l.split);
         out.split_bytes = l.split_bytes;
         out.a = Factor{g, l.ldg, gplane, l.gplanes, false};
@@ -1003,7 +1120,9 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             out.acc = first ? nullptr : acc;
             out.out = last ? a.dx : acc;
             out.out_bf16 = last && a.bf16;
+            out.row_of = last ? rm.map : nullptr;
             if ((e = launch_mm(MM_OUT, out, stream)) != cudaSuccess) return e;
+            out.row_of = nullptr;
         }
         if (a.dw) {
             out.a.t = true;

@@ -49,10 +49,16 @@ struct MmArgs {
     Factor a, b;
     bool fp16;                  // the planes are fp16, else bf16
     int m, n, k;
+    // How many of a's rows there are, or (a transposed) of the summed elements:
+    // *live <= m (k); null: all. The rest is not read but for the padding that
+    // fills a last step (64 elements) or tile (256 rows; MM_GRAD writes those
+    // rows, as zeros where rs is 0).
+    const int *live;
+    const int *row_of;          // row m's place in target and (not beside `acc` or split) in out; null: m
     float c;
     const float *row_mul, *mul;
     float2 *part;               // MM_LSE
-    // MM_LSE: the products at given columns. One a row: where target[m] - first_col
+    // MM_LSE: the products at given columns. One a row: where target[row_of[m]] - first_col
     // is a column, at[m] + rest[m] = s, rest the rounding of at. Or `lists` of them
     // (see Lists) at m * k + pos.
     const int64_t *target;
@@ -65,7 +71,7 @@ struct MmArgs {
     uint16_t *g;                // MM_GRAD
     long long ldg, gplane;      // MM_GRAD
     int gplanes;                // MM_GRAD
-    const float *acc;           // MM_OUT: added, laid out as out; may be null
+    const float *acc;           // MM_OUT: added, row stride n; may be null
     void *out;                  // MM_OUT, row stride n
     bool out_bf16;              // MM_OUT
     float *split;               // MM_OUT: room for partial sums,
@@ -74,7 +80,8 @@ struct MmArgs {
 
 // Planes: 1 x 1, 2 x 1 or 2 x 2; the product of the second planes is left out.
 int mm_lse_parts(int m, int n, int k, int planes_a, int planes_b);
-size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b);
+// live: for a product whose `live` rows are fewer than m
+size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b, bool live);
 // Factors: 16-byte aligned, ld and plane multiples of 8. `g`: 16-byte aligned,
 // ldg and gplane multiples of 8, its rows are written up to the next multiple
 // of 8 columns. `out` 16-byte aligned.
@@ -97,12 +104,15 @@ struct HeadArgs {
     bool kd;
     float tau;
     int reduction;
-    float *loss, *lse2, *logq2, *prob, *count;     // forward outputs
-    const float *dloss, *c_lse2, *c_logq2, *c_prob, *c_count;   // backward inputs
+    float *loss;
+    void *kept;                 // written by the forward, read by the backward (KeptLayout)
+    const float *dloss;
     void *dx, *dw;
     void *workspace;
+    bool backward;
 };
 
+size_t head_kept_bytes(int rows, int k, bool kd);
 // k: entries of the distillation's lists, 0 for the cross entropy
 size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long long ldx, long long ldw,
                             bool backward);

@@ -116,28 +116,6 @@ Tiles plan(MmKind kind, int m, int n, int k, int passes, size_t split_bytes)
     return best;
 }
 
-// Item t: its tile, and its steps of the sum; `split` its number among the
-// items of split tiles, or -1.
-__device__ __forceinline__ void item_of(const Tiles &q, int t, int &tile, int &split, int &begin, int &end) {
-    if (t < q.whole) {
-        tile = t;
-        split = -1;
-        begin = 0;
-        end = q.steps;
-    } else {
-        split = t - q.whole;
-        tile = q.whole + split / q.splits;
-        begin = split % q.splits * q.kb;
-        end = min(q.steps, begin + q.kb);
-    }
-}
-
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t limit) {
-    for (uint32_t i = 0; i < limit; ++i)
-        if (mbar_try(bar, parity)) return true;
-    return false;
-}
-
 // Tile number t as (row tile, column tile).
 __device__ __forceinline__ void tile_of(const Tiles &q, int t, int &mi, int &ni) {
     const bool rows_fast = q.mt <= q.nt;
@@ -147,6 +125,78 @@ __device__ __forceinline__ void tile_of(const Tiles &q, int t, int &mi, int &ni)
     const int f = base + r % w, s = r / w;
     mi = rows_fast ? f : s;
     ni = rows_fast ? s : f;
+}
+
+// The rows and steps that are live (MmArgs::live): rows of results, rows that
+// tiles cover (at least one tile, so that there is something to write), steps.
+struct Live {
+    int rows, tile_rows, steps;
+};
+template <bool AT>
+__device__ __forceinline__ Live live_of(const MmArgs &a, const Tiles &q) {
+    const int n = a.live ? *a.live : INT_MAX;
+    if (AT) return Live{a.m, a.m, min(q.steps, max(1, (min(n, a.k) + BK - 1) / BK))};
+    return Live{min(a.m, n), min(a.m, max(1, n)), q.steps};
+}
+
+// The plan for the live rows: their tiles alone, dense over the pairs; those
+// beyond whole rounds split into up to LIVE_ITEMS items.
+constexpr int LIVE_ITEMS = 4 * N_SM / 2;
+template <int KIND, bool AT>
+__device__ __forceinline__ Tiles live_plan(const MmArgs &a, Tiles q, const Live &l) {
+    if (AT || !a.live) return q;
+    constexpr int PAIRS = N_SM / 2;
+    q.mt = (l.tile_rows + TM - 1) / TM;
+    const int tiles = q.mt * q.nt, rest = tiles % PAIRS;
+    q.whole = q.items = tiles;
+    q.splits = 1;
+    if (KIND == MM_OUT && rest && (size_t)LIVE_ITEMS * TM * q.bn * 4 <= a.split_bytes) {
+        // rounds of items times their steps, 8 steps more for partial sums
+        int least = q.steps, best = 1;
+        for (int i = 2; i <= 9; ++i) {
+            const int s = i == 9 ? PAIRS / rest : i;
+            if (s < 2 || rest * s > LIVE_ITEMS || s * 4 > q.steps) continue;
+            const int cost = (rest * s + PAIRS - 1) / PAIRS * ((q.steps + s - 1) / s) + 8;
+            if (cost < least) {
+                least = cost;
+                best = s;
+            }
+        }
+        q.kb = (q.steps + best - 1) / best;
+        q.splits = (q.steps + q.kb - 1) / q.kb;
+        if (q.splits > 1) {
+            q.whole = tiles - rest;
+            q.items = q.whole + rest * q.splits;
+        }
+    }
+    return q;
+}
+
+// Item t: its tile, and its steps of the sum; `split` its number among the
+// items of split tiles, or -1.
+// False if there is nothing to do: no live rows in the tile, or no live steps in the item.
+__device__ __forceinline__ bool item_of(const Tiles &q, const Live &l, int t, int &mi, int &ni, int &split,
+                                        int &begin, int &end) {
+    int tile;
+    if (t < q.whole) {
+        tile = t;
+        split = -1;
+        begin = 0;
+        end = l.steps;
+    } else {
+        split = t - q.whole;
+        tile = q.whole + split / q.splits;
+        begin = split % q.splits * q.kb;
+        end = min(l.steps, begin + q.kb);
+    }
+    tile_of(q, tile, mi, ni);
+    return mi * TM < l.tile_rows && begin < end;
+}
+
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t limit) {
+    for (uint32_t i = 0; i < limit; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return false;
 }
 
 // The planes of pass c of (planes_a, planes_b): the last pass is (0, 0), before
@@ -185,13 +235,16 @@ struct Epilogue {
     int at, nth;                // MM_LSE: the next column whose product is asked for, its number in the list
     float2 lse2;                // MM_GRAD
     float rs;
+    int rows;                   // rows of results
     __device__ __forceinline__ void next(const MmArgs &a, int m) {
         const int c = nth < a.lists.k ? a.lists.col[(size_t)m * a.lists.k + nth] : INT_MAX;
         at = c == INT_MAX ? c : c - a.first_col;
     }
     // m: this lane's row, n: the first column that this warp will see
-    __device__ __forceinline__ void begin(const MmArgs &a, int m, int n) {
-        const bool in = m < a.m;
+    __device__ __forceinline__ void begin(const MmArgs &a, const Live &l, int m, int n) {
+        // dz's padding rows up to the tile's end are written too
+        rows = KIND == MM_GRAD ? min(a.m, (l.tile_rows + TM - 1) / TM * TM) : l.rows;
+        const bool in = m < rows;
         f = a.c;
         if (a.row_mul) f *= in ? a.row_mul[m] : 0.f;
         if (a.mul) f *= *a.mul;
@@ -201,7 +254,7 @@ struct Epilogue {
             at = INT_MAX;
             nth = 0;
             if (a.target && in) {
-                const long long t = a.target[m] - a.first_col;
+                const long long t = a.target[a.row_of ? a.row_of[m] : m] - a.first_col;
                 if (t >= 0 && t < a.n) at = (int)t;
             }
             if (a.lists.col && in && n < a.n) {
@@ -214,6 +267,9 @@ struct Epilogue {
             rs = in ? a.rs[m] : 0.f;
             if (rs != 0.f && a.g_unit != 0.f) rs = a.g_unit;
         }
+    }
+    __device__ static __forceinline__ size_t out_row(const int *row_of, int m0, int r) {
+        return row_of ? row_of[r] : m0 + r;
     }
     // m0: the row of lane 0; rows and columns beyond the product are left out.
     __device__ __forceinline__ void chunk(const MmArgs &a, const Tiles &q, int split, int m0, int n, int tile_col,
@@ -250,7 +306,7 @@ struct Epilogue {
             s = t;
             return;
         }
-        if (n >= a.n || m0 >= a.m) return;                     // the whole warp
+        if (n >= a.n || m0 >= rows) return;                    // the whole warp
         const int lane = threadIdx.x % 32;
         __syncwarp();
 #pragma unroll
@@ -258,13 +314,13 @@ struct Epilogue {
             turn[lane * 33 + i] = KIND != MM_GRAD ? v[i] * f
                                   : rs == 0.f ? 0.f : rs * ex2(fmaf(v[i], f, -lse2.x) - lse2.y);
         __syncwarp();
-        const int rows = min(32, a.m - m0), cols = min(32, a.n - n);
+        const int left = min(32, rows - m0), cols = min(32, a.n - n);
         if (KIND == MM_GRAD) {
             const int g8 = lane % 4 * 8;                       // 8 columns, 8 rows at a time
             if (g8 >= cols) return;
 #pragma unroll
             for (int r = lane / 4; r < 32; r += 8) {
-                if (r >= rows) break;
+                if (r >= left) break;
                 uint16_t *g = a.g + (size_t)(m0 + r) * a.ldg + n + g8;
                 uint32_t hi[4], lo[4];
 #pragma unroll
@@ -292,15 +348,15 @@ struct Epilogue {
             }
             return;
         }
-        const size_t o = (size_t)m0 * a.n + n;
-        const float *acc = a.acc ? a.acc + o : nullptr;
+        const float *acc = a.acc ? a.acc + (size_t)m0 * a.n + n : nullptr;
+        const int *row_of = a.row_of ? a.row_of + m0 : nullptr;
         if (a.out_bf16) {
-            __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + o;
+            __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + n;
             if (cols == 32 && a.n % 8 == 0) {
                 const int c = lane % 4 * 8;
 #pragma unroll
                 for (int r = lane / 4; r < 32; r += 8) {
-                    if (r >= rows) break;
+                    if (r >= left) break;
                     const size_t e = (size_t)r * a.n + c;
                     uint32_t w[4];
 #pragma unroll
@@ -312,22 +368,22 @@ struct Epilogue {
                         }
                         w[j] = half_bits(false, x) | (uint32_t)half_bits(false, y) << 16;
                     }
-                    *reinterpret_cast<uint4 *>(p + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4 *>(p + out_row(row_of, m0, r) * a.n + c) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             } else if (lane < cols) {
 #pragma unroll 4
-                for (int r = 0; r < rows; ++r) {
+                for (int r = 0; r < left; ++r) {
                     const size_t e = (size_t)r * a.n + lane;
-                    p[e] = __float2bfloat16_rn(turn[r * 33 + lane] + (acc ? acc[e] : 0.f));
+                    p[out_row(row_of, m0, r) * a.n + lane] = __float2bfloat16_rn(turn[r * 33 + lane] + (acc ? acc[e] : 0.f));
                 }
             }
         } else {
-            float *p = static_cast<float *>(a.out) + o;
+            float *p = static_cast<float *>(a.out) + n;
             if (cols == 32 && a.n % 4 == 0) {
                 const int c = lane % 8 * 4;
 #pragma unroll
                 for (int r = lane / 8; r < 32; r += 4) {
-                    if (r >= rows) break;
+                    if (r >= left) break;
                     const size_t e = (size_t)r * a.n + c;
                     const float *t = turn + r * 33 + c;
                     float4 w = make_float4(t[0], t[1], t[2], t[3]);
@@ -335,26 +391,26 @@ struct Epilogue {
                         const float4 q4 = *reinterpret_cast<const float4 *>(acc + e);
                         w = make_float4(w.x + q4.x, w.y + q4.y, w.z + q4.z, w.w + q4.w);
                     }
-                    st4(p + e, w);
+                    st4(p + out_row(row_of, m0, r) * a.n + c, w);
                 }
             } else if (lane < cols) {
 #pragma unroll 4
-                for (int r = 0; r < rows; ++r) {
+                for (int r = 0; r < left; ++r) {
                     const size_t e = (size_t)r * a.n + lane;
-                    p[e] = turn[r * 33 + lane] + (acc ? acc[e] : 0.f);
+                    p[out_row(row_of, m0, r) * a.n + lane] = turn[r * 33 + lane] + (acc ? acc[e] : 0.f);
                 }
             }
         }
     }
     __device__ __forceinline__ void end(const MmArgs &a, int m, int i) {
-        if (KIND == MM_LSE && m < a.m) a.part[(size_t)i * a.m + m] = make_float2(mx, s);
+        if (KIND == MM_LSE && m < rows) a.part[(size_t)i * a.m + m] = make_float2(mx, s);
     }
 };
 
 template <int KIND, bool AT, bool BT, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-          const MmArgs a, const Tiles q, uint32_t limit, int skip)
+          const MmArgs a, const Tiles planned, uint32_t limit, int skip)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * STAGES + 5];
@@ -387,8 +443,10 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const uint32_t tmem = tmem_slot;
     const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     const int passes = a.a.planes + a.b.planes - 1;
-    const int bhalf = q.bn / 2;
+    const int bhalf = planned.bn / 2;
     const int bblocks = BT ? (bhalf + 63) / 64 : 0;
+    const Live live = live_of<AT>(a, planned);
+    const Tiles q = live_plan<KIND, AT>(a, planned, live);
 
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
@@ -397,13 +455,12 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         int it = 0;
         bool ok = true;
         for (int t = pair; ok && t < q.items; t += pairs) {
-            int tile, split, k_begin, k_end, mi, ni;
-            item_of(q, t, tile, split, k_begin, k_end);
-            tile_of(q, tile, mi, ni);
+            int split, k_begin, k_end, mi, ni;
+            if (!item_of(q, live, t, mi, ni, split, k_begin, k_end)) continue;
             const int m0 = mi * TM + rank * 128, n0 = ni * q.bn + rank * bhalf;
             // the second CTA may have no rows: its part of a then stays as it is, and so does its product
-            const bool some = m0 < a.m;
-            const uint32_t a_bytes = HALF + (mi * TM + 128 < a.m ? HALF : 0);
+            const bool some = m0 < live.tile_rows;
+            const uint32_t a_bytes = HALF + (mi * TM + 128 < live.tile_rows ? HALF : 0);
             for (int k_first = k_begin; ok && k_first < k_end; k_first += q.part)
             for (int c = 0; ok && c < passes; ++c) {
                 int pa, pb;
@@ -442,8 +499,8 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         int it = 0, use = 0;
         bool ok = true;
         for (int t = pair; ok && t < q.items; t += pairs) {
-        int tile, split, k_begin, k_end;
-        item_of(q, t, tile, split, k_begin, k_end);
+        int split, k_begin, k_end, mi, ni;
+        if (!item_of(q, live, t, mi, ni, split, k_begin, k_end)) continue;
         for (int k_first = k_begin; k_first < k_end; k_first += q.part, ++use) {
             const int buf = use & 1;
             if (!wait_bar(tempty + 8 * buf, ((use >> 1) & 1) ^ 1, limit)) {
@@ -486,12 +543,11 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         int use = 0;
         bool ok = true;
         for (int t = pair; ok && t < q.items; t += pairs) {
-            int tile, split, k_begin, k_end, mi, ni;
-            item_of(q, t, tile, split, k_begin, k_end);
-            tile_of(q, tile, mi, ni);
+            int split, k_begin, k_end, mi, ni;
+            if (!item_of(q, live, t, mi, ni, split, k_begin, k_end)) continue;
             const int m0 = mi * TM + rank * 128 + quad * 32, m = m0 + lane;
             Epilogue<KIND> ep;
-            ep.begin(a, m, ni * q.bn + c0);
+            ep.begin(a, live, m, ni * q.bn + c0);
             float2 sum[4][16];                               // unused without PARTS
             for (int k_first = k_begin; k_first < k_end; k_first += q.part, ++use) {
                 const int buf = use & 1;
@@ -584,27 +640,38 @@ cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
     constexpr auto kernel = mm_kernel<KIND, AT, BT, PARTS>;
     const cudaError_t e = smem_opt_in<kernel>(SMEM);
     if (e != cudaSuccess) return e;
-    const int pairs = std::min(N_SM / 2, q.items);
+    const int pairs = a.live && !AT ? N_SM / 2 : std::min(N_SM / 2, q.items);
     kernel<<<2 * pairs, THREADS, SMEM, stream>>>(ma, mb, a, q, tma_wait_limit(), tma_skip_item());
     return cudaGetLastError();
 }
 
 // out = acc + the partial sums of the split tiles, in order; a CTA per 8 rows of a tile.
-template <typename T>
-__global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Tiles q)
+template <typename T, bool AT>
+__global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Tiles planned)
 {
     int mi, ni;
+    const Live live = live_of<AT>(a, planned);
+    const Tiles q = live_plan<MM_OUT, AT>(a, planned, live);
+    if (q.whole + (int)blockIdx.y >= q.mt * q.nt) return;
     tile_of(q, q.whole + blockIdx.y, mi, ni);
+    const int splits = min(q.splits, (live.steps + q.kb - 1) / q.kb);
     const float *p = a.split + (size_t)blockIdx.y * q.splits * TM * q.bn;
     for (int i = threadIdx.x; i < 8 * q.bn; i += 256) {
         const int r = blockIdx.x * 8 + i / q.bn, c = i % q.bn, m = mi * TM + r, n = ni * q.bn + c;
-        if (m >= a.m || n >= a.n) continue;
-        const size_t o = (size_t)m * a.n + n;
-        float s = a.acc ? a.acc[o] : 0.f;
+        if (m >= live.rows || n >= a.n) continue;
+        float s = a.acc ? a.acc[(size_t)m * a.n + n] : 0.f;
 #pragma unroll 4
-        for (int k = 0; k < q.splits; ++k) s += p[((size_t)k * TM + r) * q.bn + c];
-        static_cast<T *>(a.out)[o] = from_f<T>(s);
+        for (int k = 0; k < splits; ++k) s += p[((size_t)k * TM + r) * q.bn + c];
+        static_cast<T *>(a.out)[(size_t)(a.row_of ? a.row_of[m] : m) * a.n + n] = from_f<T>(s);
     }
+}
+
+template <bool AT>
+void split_sum(const MmArgs &a, const Tiles &q, int rest, cudaStream_t stream)
+{
+    const dim3 grid(TM / 8, rest);
+    if (a.out_bf16) split_sum_kernel<__nv_bfloat16, AT><<<grid, 256, 0, stream>>>(a, q);
+    else split_sum_kernel<float, AT><<<grid, 256, 0, stream>>>(a, q);
 }
 
 }  // namespace
@@ -614,8 +681,9 @@ int mm_lse_parts(int m, int n, int k, int planes_a, int planes_b)
     return 2 * plan(MM_LSE, m, n, k, passes_of(planes_a, planes_b), 0).nt;
 }
 
-size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b)
+size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b, bool live)
 {
+    if (live) return (size_t)LIVE_ITEMS * TM * MM_COLS * 4;
     const Tiles q = plan(MM_OUT, m, n, k, passes_of(planes_a, planes_b), ~(size_t)0);
     return (size_t)(q.items - q.whole) * TM * q.bn * 4;
 }
@@ -636,11 +704,11 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
                                         : launch<MM_OUT, true, true, false>(a, q, stream)
                                 : parts ? launch<MM_OUT, false, true, true>(a, q, stream)
                                         : launch<MM_OUT, false, true, false>(a, q, stream);
-    const int rest = q.mt * q.nt - q.whole;
+    // the live rows' tiles are not known here: as many CTAs as they may need
+    const int rest = a.live && !a.a.t ? N_SM / 2 - 1 : q.mt * q.nt - q.whole;
     if (e != cudaSuccess || !rest) return e;
-    const dim3 grid(TM / 8, rest);
-    if (a.out_bf16) split_sum_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a, q);
-    else split_sum_kernel<float><<<grid, 256, 0, stream>>>(a, q);
+    if (a.a.t) split_sum<true>(a, q, rest, stream);
+    else split_sum<false>(a, q, rest, stream);
     return cudaGetLastError();
 }
 

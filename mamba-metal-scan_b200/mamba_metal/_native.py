@@ -51,12 +51,13 @@ SIGNATURES = {
                      + [_P], _I),
     "mms_fwd_bf16": ([_P] * 7 + [_I] * 5 + [_P], _I),
     "mms_bwd_bf16": ([_P] * 13 + [ctypes.c_size_t] + [_I] * 5 + [_P], _I),
+    "mms_head_kept_size": ([_I] * 2, _Z),
     "mms_head_workspace_size": ([_I] * 5 + [_L] * 2 + [_I], _Z),
-    "mms_linear_ce_fwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 5 + [_Z] + [_I] * 4 + [_P], _I),
-    "mms_linear_ce_bwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 7 + [_Z] + [_I] * 4 + [_P], _I),
-    "mms_linear_kd_fwd": ([_P, _L, _P, _L, _P, _P, _I, _F, _I] + [_P] * 6 + [_Z] + [_I] * 4
+    "mms_linear_ce_fwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 3 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_linear_ce_bwd": ([_P, _L, _P, _L, _P, _L, _I] + [_P] * 5 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_linear_kd_fwd": ([_P, _L, _P, _L, _P, _P, _I, _F, _I] + [_P] * 3 + [_Z] + [_I] * 4
                           + [_P], _I),
-    "mms_linear_kd_bwd": ([_P, _L, _P, _L, _P, _I, _F, _I] + [_P] * 8 + [_Z] + [_I] * 4 + [_P], _I),
+    "mms_linear_kd_bwd": ([_P, _L, _P, _L, _P, _I, _F, _I] + [_P] * 5 + [_Z] + [_I] * 4 + [_P], _I),
     "mms_norm_workspace_size": ([_I] * 2, _Z),
     "mms_norm_fwd": ([_P] * 3 + [_L] + [_P] * 3 + [_F] + [_P] * 3 + [_I] * 3 + [_P], _I),
     "mms_norm_bwd": ([_P] * 3 + [_L] + [_P] * 13 + [_Z] + [_I] * 3 + [_P], _I),
@@ -276,26 +277,22 @@ def _head_workspace(x, w, k: int, backward: bool):
     return torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
 
 
-def _kept(m: int, k: int, kd: bool, base: int):
-    """Addresses of lse2, logq2, prob, count in the one buffer that the forward keeps, and its
-    length in floats."""
-    at = [0, 2 * m, 2 * m + m * k, 2 * m + m * k * (2 if kd else 1)]
-    return [base + 4 * o for o in at], at[3] + 2
+def _kept(m: int, k: int, device):
+    return torch.empty(int(load().mms_head_kept_size(m, k)), dtype=torch.uint8, device=device)
 
 
 def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
-    """(loss, kept) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides. kept: lse2, logq2
-    and count in one float32 buffer."""
+    """(loss, kept) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides. kept: what the
+    backward needs."""
     m, d = x.shape
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    kept = torch.empty(_kept(m, 1, False, 0)[1], device=x.device)
-    (lse2, logq2, _, count), _ = _kept(m, 1, False, kept.data_ptr())
+    kept = _kept(m, 0, x.device)
     ws = _head_workspace(x, w, 0, False)
     rc = load().mms_linear_ce_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
-                                  target.data_ptr(), ignore_index, red, loss.data_ptr(), lse2, logq2,
-                                  count, ws.data_ptr(), ws.numel(), m, w.shape[0], d, _dtype(x),
-                                  _stream(x.device))
+                                  target.data_ptr(), ignore_index, red, loss.data_ptr(),
+                                  kept.data_ptr(), ws.data_ptr(), ws.numel(), m, w.shape[0], d,
+                                  _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_ce_fwd")
     return loss, kept
 
@@ -311,29 +308,27 @@ def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, kept,
     """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
     m, d = x.shape
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    (lse2, logq2, _, count), _ = _kept(m, 1, False, kept.data_ptr())
     ws = _head_workspace(x, w, 0, True)
     rc = load().mms_linear_ce_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   target.data_ptr(), ignore_index, REDUCTIONS[reduction],
-                                  dloss.data_ptr(), lse2, logq2, count, pdx, pdw, ws.data_ptr(),
+                                  dloss.data_ptr(), kept.data_ptr(), pdx, pdw, ws.data_ptr(),
                                   ws.numel(), m, w.shape[0], d, _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_ce_bwd")
     return dx, dw
 
 
 def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
-    """(loss, kept) of mms_linear_kd_fwd. kept: lse2, logq2, prob and count in one float32 buffer."""
+    """(loss, kept) of mms_linear_kd_fwd. kept: what the backward needs."""
     m, d = x.shape
     k = index.shape[1]
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    kept = torch.empty(_kept(m, k, True, 0)[1], device=x.device)
-    (lse2, logq2, prob, count), _ = _kept(m, k, True, kept.data_ptr())
+    kept = _kept(m, k, x.device)
     ws = _head_workspace(x, w, k, False)
     rc = load().mms_linear_kd_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   index.data_ptr(), logits.data_ptr(), k, temperature, red,
-                                  loss.data_ptr(), lse2, logq2, prob, count, ws.data_ptr(),
-                                  ws.numel(), m, w.shape[0], d, _dtype(x), _stream(x.device))
+                                  loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), ws.numel(),
+                                  m, w.shape[0], d, _dtype(x), _stream(x.device))
     _check(rc, "mms_linear_kd_fwd")
     return loss, kept
 
@@ -344,11 +339,10 @@ def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, kept,
     m, d = x.shape
     k = index.shape[1]
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    (lse2, logq2, prob, count), _ = _kept(m, k, True, kept.data_ptr())
     ws = _head_workspace(x, w, k, True)
     rc = load().mms_linear_kd_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   index.data_ptr(), k, temperature, REDUCTIONS[reduction],
-                                  dloss.data_ptr(), lse2, logq2, prob, count, pdx, pdw,
+                                  dloss.data_ptr(), kept.data_ptr(), pdx, pdw,
                                   ws.data_ptr(), ws.numel(), m, w.shape[0], d, _dtype(x),
                                   _stream(x.device))
     _check(rc, "mms_linear_kd_bwd")

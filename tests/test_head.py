@@ -119,35 +119,38 @@ def test_c_entries_check_before_any_launch():
     bad, mis, ws_err = (_native.MMS_ERR_INVALID_ARG, _native.MMS_ERR_MISALIGNED, _native.MMS_ERR_WORKSPACE)
     ok = _p(0x10000)
 
-    def ce_fwd(x=ok, ldx=16, w=ok, ldw=16, t=ok, red=1, out=ok, ws=_p(0x20000), nb=1 << 40, m=4, v=8,
-               d=16, ty=0):
-        return lib.mms_linear_ce_fwd(x, ldx, w, ldw, t, -100, red, out, out, out, out, ws, nb, m, v, d,
-                                     ty, None)
+    def ce_fwd(x=ok, ldx=16, w=ok, ldw=16, t=ok, red=1, loss=ok, kept=ok, ws=_p(0x20000), nb=1 << 40,
+               m=4, v=8, d=16, ty=0):
+        return lib.mms_linear_ce_fwd(x, ldx, w, ldw, t, -100, red, loss, kept, ws, nb, m, v, d, ty, None)
 
     assert ce_fwd(m=0) == bad and ce_fwd(v=0) == bad and ce_fwd(d=0) == bad
     assert ce_fwd(ldx=15) == bad and ce_fwd(ldw=15) == bad and ce_fwd(ty=2) == bad
     assert ce_fwd(red=3) == bad and ce_fwd(red=-1) == bad and ce_fwd(m=(1 << 24) + 1) == bad
-    assert ce_fwd(x=None) == bad and ce_fwd(t=None) == bad and ce_fwd(out=None) == bad
-    assert ce_fwd(x=_p(0x10008)) == mis and ce_fwd(t=_p(0x10004)) == mis
+    assert ce_fwd(x=None) == bad and ce_fwd(t=None) == bad
+    assert ce_fwd(loss=None) == bad and ce_fwd(kept=None) == bad
+    assert ce_fwd(x=_p(0x10008)) == mis and ce_fwd(t=_p(0x10004)) == mis and ce_fwd(kept=_p(0x10008)) == mis
     need = lib.mms_head_workspace_size(4, 8, 16, 0, 0, 16, 16, 0)
     assert need > 0 and ce_fwd(nb=need - 1) == ws_err and ce_fwd(ws=None) == ws_err
     assert ce_fwd(ws=_p(0x20010)) == mis
     assert lib.mms_head_workspace_size(0, 8, 16, 0, 0, 16, 16, 0) == 0
+    assert lib.mms_head_workspace_size(4, 8, 16, 1025, 0, 16, 16, 0) == 0
+    assert lib.mms_head_kept_size(4, 0) > 0 and lib.mms_head_kept_size(4, 9) > lib.mms_head_kept_size(4, 1)
+    assert lib.mms_head_kept_size(0, 0) == 0 and lib.mms_head_kept_size(4, 1025) == 0
 
     def kd_fwd(k=2, tau=1.0, logits=ok, nb=0):
-        return lib.mms_linear_kd_fwd(ok, 16, ok, 16, ok, logits, k, tau, 1, ok, ok, ok, ok, ok,
-                                     _p(0x20000), nb, 4, 8, 16, 1, None)
+        return lib.mms_linear_kd_fwd(ok, 16, ok, 16, ok, logits, k, tau, 1, ok, ok, _p(0x20000), nb, 4, 8, 16,
+                                     1, None)
 
     assert kd_fwd() == ws_err and kd_fwd(k=0) == bad and kd_fwd(k=1025) == bad
     assert kd_fwd(tau=0.0) == bad and kd_fwd(tau=float("nan")) == bad and kd_fwd(logits=None) == bad
 
-    def bwd(dl=ok, dx=ok, nb=0):
-        return lib.mms_linear_ce_bwd(ok, 16, ok, 16, ok, -100, 1, dl, ok, ok, ok, dx, ok, _p(0x20000), nb,
-                                     4, 8, 16, 1, None)
+    def bwd(dl=ok, kept=ok, dx=ok, nb=0):
+        return lib.mms_linear_ce_bwd(ok, 16, ok, 16, ok, -100, 1, dl, kept, dx, ok, _p(0x20000), nb, 4, 8, 16, 1,
+                                     None)
 
-    assert bwd() == ws_err and bwd(dl=None) == bad and bwd(dx=_p(0x10008)) == mis
-    assert lib.mms_linear_kd_bwd(ok, 16, ok, 16, ok, 2, 1.0, 1, ok, ok, ok, None, ok, ok, ok, _p(0x20000),
-                                 0, 4, 8, 16, 1, None) == bad
+    assert bwd() == ws_err and bwd(dl=None) == bad and bwd(kept=None) == bad and bwd(dx=_p(0x10008)) == mis
+    assert lib.mms_linear_kd_bwd(ok, 16, ok, 16, ok, 2, 1.0, 1, None, ok, ok, ok, _p(0x20000), 0, 4, 8, 16, 1,
+                                 None) == bad
 
     def norm(x=ok, gate=None, ldg=16, m=4, d=16, ty=0, stat=ok, eps=1e-6):
         return lib.mms_norm_fwd(x, ok, gate, ldg, ok, None, None, eps, ok, ok, stat, m, d, ty, None)

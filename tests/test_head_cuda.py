@@ -129,11 +129,49 @@ def test_left_out_rows_may_hold_anything(dtype):
     assert (loss[::4] == 0).all() and (grads[0][::4] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,kept", [(513, 0.5), (700, 0.02), (1100, 0.9), (1100, 0.47), (2000, 0.0005)])
+def test_many_rows_of_which_some_count(rows, kept, dtype):
+    """Above 512 rows the products run over the listed rows alone: their numbers fall between
+    tiles and steps, what is left out holds NaN, and every reduction puts results in place."""
+    vocab, dim = 300, 72
+    x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=rows)
+    out = torch.rand(rows, generator=gen) >= kept
+    out[rows // 2] = False
+    target[out] = -100
+    x[out] = float("nan")
+    for reduction in ("none", "mean", "sum"):
+        dloss = torch.randn(rows, generator=gen) if reduction == "none" else torch.tensor(1.7)
+        loss, grads = run_ce(x, w, target, reduction, dloss)
+        compare(x, w, sparse(1, target=target, ignore=-100), 1.0, reduction, dloss, loss, grads)
+        assert (grads[0].cpu()[out] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_lists_of_which_some_are_empty(dtype):
+    rows, vocab, dim, k = 900, 700, 72, 9
+    x, w, _, gen = head_inputs(rows, vocab, dim, dtype, seed=3)
+    index = torch.randint(-2, vocab, (rows, k), generator=gen)
+    logits = 2 * torch.randn(rows, k, generator=gen)
+    index[::3] = -1
+    logits[1::3] = float("-inf")
+    index[7], logits[7] = 5, 0.25                        # one index nine times
+    x[::3] = float("inf")
+    parts = sparse(k, index=index, logits=logits, tau=1.5)
+    for reduction in ("none", "mean"):
+        dloss = torch.randn(rows, generator=gen) if reduction == "none" else torch.tensor(1.0)
+        xd, wd = leaves(x, w)
+        loss = linear_distillation(xd, wd, index.to(DEV), logits.to(DEV), 1.5, reduction=reduction)
+        grads = torch.autograd.grad(loss, [xd, wd], dloss.to(DEV).reshape(loss.shape))
+        compare(x, w, parts, 1.5, reduction, dloss, loss, grads)
+
+
+@pytest.mark.parametrize("rows", [9, 700])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_every_row_left_out(reduction):
-    x, w, target, _ = head_inputs(9, 50, 24, F32)
+def test_every_row_left_out(reduction, rows):
+    x, w, target, _ = head_inputs(rows, 50, 24, F32)
     target[:] = -100
-    loss, grads = run_ce(x, w, target, reduction, torch.ones(9) if reduction == "none" else torch.tensor(1.0))
+    loss, grads = run_ce(x, w, target, reduction, torch.ones(rows) if reduction == "none" else torch.tensor(1.0))
     if reduction == "mean":
         assert torch.isnan(loss)                                       # 0 / 0, as PyTorch's
     else:
