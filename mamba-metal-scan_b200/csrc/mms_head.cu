@@ -208,16 +208,35 @@ __device__ __forceinline__ float finite_abs(float v) {
     return v <= 3.4028234e38f ? v : 0.f;
 }
 
-// 8 elements of a row from column c on; 0 beyond `cols`.
+// 8 elements of a row from column c on; 0 beyond `cols`. Where the row is not
+// 16-byte aligned: bf16 from the two aligned pieces around them if both lie
+// within the row (which any 8 but the first and the last do), else one by one.
 template <typename T>
 __device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, float (&v)[8]) {
-    if (c + 8 <= cols && reinterpret_cast<uintptr_t>(p + c) % 16 == 0) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(p + c) % 16);     // bytes past an aligned place
+    if (c + 8 <= cols && off == 0) {
         uint4 q[sizeof(T) / 2];
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = __ldg(reinterpret_cast<const uint4 *>(p + c) + i);
         const T *e = reinterpret_cast<const T *>(q);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
+    } else if (sizeof(T) == 2 && c >= off / 2 && c - off / 2 + 16 <= cols) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(p + c - off / 2);
+        const uint4 a = __ldg(q), b = __ldg(q + 1);
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (off & 4)
+#pragma unroll
+            for (int i = 0; i < 7; ++i) w[i] = w[i + 1];
+        if (off & 8)
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = w[i + 2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = __funnelshift_r(w[i], w[i + 1], off % 4 * 8);
+            v[2 * i] = __uint_as_float(t << 16);
+            v[2 * i + 1] = __uint_as_float(t & 0xffff0000u);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(p[c + i]) : 0.f;

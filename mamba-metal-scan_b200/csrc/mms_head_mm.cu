@@ -151,12 +151,13 @@ __device__ __forceinline__ Tiles live_plan(const MmArgs &a, Tiles q, const Live 
     q.whole = q.items = tiles;
     q.splits = 1;
     if (KIND == MM_OUT && rest && (size_t)LIVE_ITEMS * TM * q.bn * 4 <= a.split_bytes) {
-        // rounds of items times their steps, 8 steps more for partial sums
+        // rounds of items times their steps; partial sums cost 8 steps for the launch and a third
+        // of one (256 KB written and read) for each item
         int least = q.steps, best = 1;
         for (int i = 2; i <= 9; ++i) {
             const int s = i == 9 ? PAIRS / rest : i;
             if (s < 2 || rest * s > LIVE_ITEMS || s * 4 > q.steps) continue;
-            const int cost = (rest * s + PAIRS - 1) / PAIRS * ((q.steps + s - 1) / s) + 8;
+            const int cost = (rest * s + PAIRS - 1) / PAIRS * ((q.steps + s - 1) / s) + 8 + rest * s / 3;
             if (cost < least) {
                 least = cost;
                 best = s;
@@ -645,7 +646,8 @@ cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
     return cudaGetLastError();
 }
 
-// out = acc + the partial sums of the split tiles, in order; a CTA per 8 rows of a tile.
+// out = acc + the partial sums of the split tiles, in order; a CTA per 4 rows of a tile,
+// a thread per 4 columns.
 template <typename T, bool AT>
 __global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Tiles planned)
 {
@@ -656,20 +658,25 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Ti
     tile_of(q, q.whole + blockIdx.y, mi, ni);
     const int splits = min(q.splits, (live.steps + q.kb - 1) / q.kb);
     const float *p = a.split + (size_t)blockIdx.y * q.splits * TM * q.bn;
-    for (int i = threadIdx.x; i < 8 * q.bn; i += 256) {
-        const int r = blockIdx.x * 8 + i / q.bn, c = i % q.bn, m = mi * TM + r, n = ni * q.bn + c;
-        if (m >= live.rows || n >= a.n) continue;
-        float s = a.acc ? a.acc[(size_t)m * a.n + n] : 0.f;
-#pragma unroll 4
-        for (int k = 0; k < splits; ++k) s += p[((size_t)k * TM + r) * q.bn + c];
-        static_cast<T *>(a.out)[(size_t)(a.row_of ? a.row_of[m] : m) * a.n + n] = from_f<T>(s);
+    const int i = threadIdx.x * 4, r = blockIdx.x * 4 + i / q.bn, c = i % q.bn, m = mi * TM + r, n = ni * q.bn + c;
+    if (i >= 4 * q.bn || m >= live.rows || n >= a.n) return;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) {
+        const float4 t = ld4(p + ((size_t)k * TM + r) * q.bn + c);
+        s = make_float4(s.x + t.x, s.y + t.y, s.z + t.z, s.w + t.w);
     }
+    const float *acc = a.acc ? a.acc + (size_t)m * a.n + n : nullptr;
+    T *out = static_cast<T *>(a.out) + (size_t)(a.row_of ? a.row_of[m] : m) * a.n + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (n + j < a.n) out[j] = from_f<T>(comp(s, j) + (acc ? acc[j] : 0.f));
 }
 
 template <bool AT>
 void split_sum(const MmArgs &a, const Tiles &q, int rest, cudaStream_t stream)
 {
-    const dim3 grid(TM / 8, rest);
+    const dim3 grid(TM / 4, rest);
     if (a.out_bf16) split_sum_kernel<__nv_bfloat16, AT><<<grid, 256, 0, stream>>>(a, q);
     else split_sum_kernel<float, AT><<<grid, 256, 0, stream>>>(a, q);
 }
@@ -692,7 +699,7 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
-    const int steps = q.whole ? q.steps : q.kb;
+    const int steps = q.whole || a.live ? q.steps : q.kb;       // live rows split as the device finds it
     const bool parts = (steps * BK > PART || (steps > 4 && q.items <= N_SM / 2)) && (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
@@ -705,7 +712,7 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
                                 : parts ? launch<MM_OUT, false, true, true>(a, q, stream)
                                         : launch<MM_OUT, false, true, false>(a, q, stream);
     // the live rows' tiles are not known here: as many CTAs as they may need
-    const int rest = a.live && !a.a.t ? N_SM / 2 - 1 : q.mt * q.nt - q.whole;
+    const int rest = a.live && !a.a.t ? std::min(N_SM / 2 - 1, q.mt * q.nt) : q.mt * q.nt - q.whole;
     if (e != cudaSuccess || !rest) return e;
     if (a.a.t) split_sum<true>(a, q, rest, stream);
     else split_sum<false>(a, q, rest, stream);
