@@ -30,8 +30,14 @@
 // beside the multiplies; of 256, 25 % of the log-sum-exp at 8192 x 131072 x
 // 2048 (4.15 ms against 3.31); of 128, 80 %.
 //
-// The epilogue turns a warp's 32 rows x 32 columns through shared memory, so
-// that its stores (and the reads of `acc`) cover whole sectors of a row.
+// The epilogue turns a warp's 32 rows x 32 columns through shared memory, in
+// 16-byte pieces (16-bit results already rounded and packed), so that its
+// stores and the reads of `acc` cover whole sectors of a row. Its arithmetic
+// is on packed pairs with independent sums. At 8192 x 32768 x 64 (bf16), where
+// it is all there is, a tile of the log-sum-exp takes 6.2 k clocks and of dz
+// 8.0 k (7.0 and 10 k with scalar sums and turns; the exponentials alone
+// 2.0 k); under a product of 2048 elements, 16.4 k, it is hidden. Loading the
+// next 32 columns of tensor memory ahead measured the same, and spilled.
 //
 // Tiles that do not fill a last round of the 74 pairs are split along the
 // summed dimension; their partial sums go to a workspace that a second kernel
@@ -45,6 +51,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mms_common.cuh"
 #include "mms_head.h"
@@ -207,13 +214,6 @@ __device__ __forceinline__ void planes_of(int passes, int c, int &pa, int &pb) {
     pb = passes > 2 && c == 1;
 }
 
-__device__ __forceinline__ uint16_t half_bits(bool fp16, float v) {
-    return fp16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
-}
-__device__ __forceinline__ float half_value(bool fp16, uint16_t b) {
-    return fp16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
-}
-
 // v[i] without an indexed register file: halves of the candidates by each bit of i.
 __device__ __forceinline__ float pick32(const float (&v)[32], int i) {
     float t[16];
@@ -275,133 +275,174 @@ struct Epilogue {
     // m0: the row of lane 0; rows and columns beyond the product are left out.
     __device__ __forceinline__ void chunk(const MmArgs &a, const Tiles &q, int split, int m0, int n, int tile_col,
                                           float (&v)[32], float *turn) {
+        if (n >= a.n || (KIND != MM_LSE && m0 >= rows)) return;        // the whole warp
         if (KIND == MM_LSE) {
-            if (n >= a.n) return;
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (n + i >= a.n) v[i] = -INFINITY;
-                top = fmaxf(top, v[i]);
-            }
-            top *= f;                                          // f > 0
-            while (at < n + 32) {
-                const int m = m0 + threadIdx.x % 32;
-                if (at >= n) {
-                    const size_t to = a.target ? m : (size_t)m * a.lists.k + a.lists.pos[(size_t)m * a.lists.k + nth];
-                    const float z = pick32(v, at - n), p = z * f;
-                    a.at[to] = p;
-                    a.rest[to] = rounding_of(z, f, p);
-                }
-                if (a.target) {
-                    at = INT_MAX;
-                } else {
-                    ++nth;
-                    next(a, m);
-                }
-            }
-            const float now = fmaxf(mx, top), ref = now == -INFINITY ? 0.f : now;
-            float t = s * ex2(mx - ref);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) t += ex2(fmaf(v[i], f, -ref));
-            mx = now;
-            s = t;
+            lse(a, m0, n, v);
             return;
         }
-        if (n >= a.n || m0 >= rows) return;                    // the whole warp
-        const int lane = threadIdx.x % 32;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            turn[lane * 33 + i] = KIND != MM_GRAD ? v[i] * f
-                                  : rs == 0.f ? 0.f : rs * ex2(fmaf(v[i], f, -lse2.x) - lse2.y);
-        __syncwarp();
-        const int left = min(32, rows - m0), cols = min(32, a.n - n);
+        const int lane = threadIdx.x % 32, left = min(32, rows - m0), cols = min(32, a.n - n);
+        const float2 fp = f2(f, f);
         if (KIND == MM_GRAD) {
-            const int g8 = lane % 4 * 8;                       // 8 columns, 8 rows at a time
-            if (g8 >= cols) return;
+            const float2 x = f2(-lse2.x, -lse2.x), y = f2(-lse2.y, -lse2.y), r = f2(rs, rs);
 #pragma unroll
-            for (int r = lane / 4; r < 32; r += 8) {
-                if (r >= left) break;
-                uint16_t *g = a.g + (size_t)(m0 + r) * a.ldg + n + g8;
-                uint32_t hi[4], lo[4];
+            for (int i = 0; i < 32; i += 2) {
+                const float2 e = ex2x2(add2(fma2(f2(v[i], v[i + 1]), fp, x), y)), g = mul2(r, e);
+                v[i] = g.x;
+                v[i + 1] = g.y;
+            }
+            if (__any_sync(~0u, rs == 0.f))
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = turn[r * 33 + g8 + 2 * j], y = turn[r * 33 + g8 + 2 * j + 1];
-                    const uint16_t p = half_bits(a.fp16, x), o = half_bits(a.fp16, y);
-                    hi[j] = p | (uint32_t)o << 16;
-                    if (a.gplanes > 1)
-                        lo[j] = half_bits(a.fp16, x - half_value(a.fp16, p)) |
-                                (uint32_t)half_bits(a.fp16, y - half_value(a.fp16, o)) << 16;
-                }
-                *reinterpret_cast<uint4 *>(g) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (a.gplanes > 1)
-                    *reinterpret_cast<uint4 *>(g + a.gplane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int i = 0; i < 32; ++i) v[i] = rs == 0.f ? 0.f : v[i];
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack(a.fp16, v[2 * i], v[2 * i + 1]);
+            uint16_t *g = a.g + (size_t)m0 * a.ldg + n;
+            turn16(w, turn, left, (cols + 7) / 8, g, a.ldg, nullptr, 0);
+            if (a.gplanes > 1) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = pack_rest(a.fp16, v[2 * i], v[2 * i + 1], w[i]);
+                turn16(w, turn, left, (cols + 7) / 8, g + a.gplane, a.ldg, nullptr, 0);
             }
             return;
         }
-        if (split >= 0) {                                      // 4 rows of 32 columns at a time
-            float *p = a.split + (size_t)split * TM * q.bn + tile_col;
-            const int c = lane % 8 * 4, tile_row = m0 % TM;
 #pragma unroll
-            for (int r = lane / 8; r < 32; r += 4) {
-                const float *t = turn + r * 33 + c;
-                st4(p + (size_t)(tile_row + r) * q.bn + c, make_float4(t[0], t[1], t[2], t[3]));
-            }
-            return;
+        for (int i = 0; i < 32; i += 2) {
+            const float2 p = mul2(f2(v[i], v[i + 1]), fp);
+            v[i] = p.x;
+            v[i + 1] = p.y;
         }
-        const float *acc = a.acc ? a.acc + (size_t)m0 * a.n + n : nullptr;
         const int *row_of = a.row_of ? a.row_of + m0 : nullptr;
-        if (a.out_bf16) {
-            __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + n;
-            if (cols == 32 && a.n % 8 == 0) {
-                const int c = lane % 4 * 8;
+        if (split < 0 && a.out_bf16 && !a.acc && cols == 32 && a.n % 8 == 0) {
+            uint32_t w[16];
 #pragma unroll
-                for (int r = lane / 4; r < 32; r += 8) {
-                    if (r >= left) break;
-                    const size_t e = (size_t)r * a.n + c;
-                    uint32_t w[4];
+            for (int i = 0; i < 16; ++i) w[i] = pack(false, v[2 * i], v[2 * i + 1]);
+            turn16(w, turn, left, 4, static_cast<uint16_t *>(a.out) + n, a.n, row_of, m0);
+            return;
+        }
+        __syncwarp();
+        const float *acc = a.acc ? a.acc + (size_t)m0 * a.n + n : nullptr;
+        if (split < 0 && (cols < 32 || a.n % (a.out_bf16 ? 8 : 4))) {
+            // ragged columns, or rows that do not start at whole pieces: a row at a time
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float x = turn[r * 33 + c + 2 * j], y = turn[r * 33 + c + 2 * j + 1];
-                        if (acc) {
-                            x += acc[e + 2 * j];
-                            y += acc[e + 2 * j + 1];
-                        }
-                        w[j] = half_bits(false, x) | (uint32_t)half_bits(false, y) << 16;
-                    }
-                    *reinterpret_cast<uint4 *>(p + out_row(row_of, m0, r) * a.n + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else if (lane < cols) {
+            for (int i = 0; i < 32; ++i) turn[lane * 33 + i] = v[i];
+            __syncwarp();
+            if (lane >= cols) return;
+            const auto store = [&](auto *out) {
+                using O = typename std::remove_pointer<decltype(out)>::type;
+                if (row_of || acc || left < 32) {
 #pragma unroll 4
-                for (int r = 0; r < left; ++r) {
-                    const size_t e = (size_t)r * a.n + lane;
-                    p[out_row(row_of, m0, r) * a.n + lane] = __float2bfloat16_rn(turn[r * 33 + lane] + (acc ? acc[e] : 0.f));
+                    for (int r = 0; r < left; ++r)
+                        out[out_row(row_of, m0, r) * a.n + n + lane] =
+                            from_f<O>(turn[r * 33 + lane] + (acc ? acc[(size_t)r * a.n + lane] : 0.f));
+                } else {
+                    O *p = out + (size_t)m0 * a.n + n + lane;
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) p[(size_t)r * a.n] = from_f<O>(turn[r * 33 + lane]);
                 }
+            };
+            if (a.out_bf16) store(static_cast<__nv_bfloat16 *>(a.out));
+            else store(static_cast<float *>(a.out));
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            st4(turn + lane * 32 + ((j ^ (lane & 7)) << 2), make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+        __syncwarp();
+        const int c = lane % 8 * 4;                            // 4 columns, 4 rows at a time
+        if (split >= 0) {
+            float *p = a.split + ((size_t)split * TM + m0 % TM) * q.bn + tile_col + c;
+#pragma unroll
+            for (int r = lane / 8; r < 32; r += 4) st4(p + (size_t)r * q.bn, turned(turn, r, lane % 8));
+            return;
+        }
+#pragma unroll
+        for (int r = lane / 8; r < 32; r += 4) {
+            if (r >= left) break;
+            float4 w = turned(turn, r, lane % 8);
+            if (acc) {
+                // not through the read-only path: out may be the same array
+                const float4 t = *reinterpret_cast<const float4 *>(acc + (size_t)r * a.n + c);
+                w = make_float4(w.x + t.x, w.y + t.y, w.z + t.z, w.w + t.w);
             }
-        } else {
-            float *p = static_cast<float *>(a.out) + n;
-            if (cols == 32 && a.n % 4 == 0) {
-                const int c = lane % 8 * 4;
+            const size_t o = out_row(row_of, m0, r) * a.n + n + c;
+            if (a.out_bf16)
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + o) =
+                    make_uint2(pack(false, w.x, w.y), pack(false, w.z, w.w));
+            else
+                st4(static_cast<float *>(a.out) + o, w);
+        }
+    }
+    __device__ static __forceinline__ float4 turned(const float *turn, int r, int piece) {
+        return *reinterpret_cast<const float4 *>(turn + r * 32 + ((piece ^ (r & 7)) << 2));
+    }
+    __device__ static __forceinline__ uint32_t pack(bool fp16, float x, float y) {
+        if (fp16) {
+            const __half2 h = __floats2half2_rn(x, y);
+            return *reinterpret_cast<const uint32_t *>(&h);
+        }
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    // what the 16-bit parts in p left of x and y
+    __device__ static __forceinline__ uint32_t pack_rest(bool fp16, float x, float y, uint32_t p) {
+        float2 h;
+        if (fp16) h = __half22float2(*reinterpret_cast<const __half2 *>(&p));
+        else h = f2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+        return pack(fp16, x - h.x, y - h.y);
+    }
+    // This lane's row of 32 16-bit values to rows of `out` (at its column n) with stride ld, 4 lanes a
+    // row: `pieces` of 8 columns, `left` rows. In shared memory piece j of row r lies at j ^ (r / 2 % 4).
+    __device__ static __forceinline__ void turn16(const uint32_t (&w)[16], float *turn, int left, int pieces,
+                                                  uint16_t *out, long long ld, const int *row_of, int m0) {
+        const int lane = threadIdx.x % 32;
+        uint4 *t = reinterpret_cast<uint4 *>(turn);
+        __syncwarp();
 #pragma unroll
-                for (int r = lane / 8; r < 32; r += 4) {
-                    if (r >= left) break;
-                    const size_t e = (size_t)r * a.n + c;
-                    const float *t = turn + r * 33 + c;
-                    float4 w = make_float4(t[0], t[1], t[2], t[3]);
-                    if (acc) {
-                        const float4 q4 = *reinterpret_cast<const float4 *>(acc + e);
-                        w = make_float4(w.x + q4.x, w.y + q4.y, w.z + q4.z, w.w + q4.w);
-                    }
-                    st4(p + out_row(row_of, m0, r) * a.n + c, w);
-                }
-            } else if (lane < cols) {
-#pragma unroll 4
-                for (int r = 0; r < left; ++r) {
-                    const size_t e = (size_t)r * a.n + lane;
-                    p[out_row(row_of, m0, r) * a.n + lane] = turn[r * 33 + lane] + (acc ? acc[e] : 0.f);
-                }
+        for (int j = 0; j < 4; ++j)
+            t[lane * 4 + (j ^ (lane >> 1 & 3))] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        __syncwarp();
+        const int j = lane % 4;
+        if (j >= pieces) return;
+#pragma unroll
+        for (int r = lane / 4; r < 32; r += 8)
+            if (r < left)
+                *reinterpret_cast<uint4 *>(out + out_row(row_of, m0, r) * ld + 8 * j) = t[r * 4 + (j ^ (r >> 1 & 3))];
+    }
+    __device__ __forceinline__ void lse(const MmArgs &a, int m0, int n, float (&v)[32]) {
+        if (n + 32 > a.n)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (n + i >= a.n) v[i] = -INFINITY;
+        float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 4; i < 32; ++i) top[i % 4] = fmaxf(top[i % 4], v[i]);
+        while (at < n + 32) {
+            const int m = m0 + threadIdx.x % 32;
+            if (at >= n) {
+                const size_t to = a.target ? m : (size_t)m * a.lists.k + a.lists.pos[(size_t)m * a.lists.k + nth];
+                const float z = pick32(v, at - n), p = z * f;
+                a.at[to] = p;
+                a.rest[to] = rounding_of(z, f, p);
+            }
+            if (a.target) {
+                at = INT_MAX;
+            } else {
+                ++nth;
+                next(a, m);
             }
         }
+        const float now = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f);   // f > 0
+        const float ref = now == -INFINITY ? 0.f : now;
+        const float2 fp = f2(f, f), rp = f2(-ref, -ref);
+        float2 t[4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 e = ex2x2(fma2(f2(v[2 * i], v[2 * i + 1]), fp, rp));
+            t[i % 4] = i < 4 ? e : add2(t[i % 4], e);
+        }
+        const float2 u = add2(add2(t[0], t[1]), add2(t[2], t[3]));
+        s = fmaf(s, ex2(mx - ref), u.x + u.y);
+        mx = now;
     }
     __device__ __forceinline__ void end(const MmArgs &a, int m, int i) {
         if (KIND == MM_LSE && m < rows) a.part[(size_t)i * a.m + m] = make_float2(mx, s);
@@ -539,6 +580,12 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
         const int quad = warp % 4, side = warp / 4;
         const uint32_t lane_base = tmem + ((uint32_t)quad << 21);
+        // this warp has read its share of a buffer: the next multiplies may overwrite it
+        const auto release = [&](uint32_t bar) {
+            umma_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_addr(bar));
+        };
         const int c0 = side * q.half, cols = side ? q.bn - q.half : q.half;
         float *turn = reinterpret_cast<float *>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * 2 * HALF) + warp * TURN;
         int use = 0;
@@ -561,26 +608,31 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
                 umma_fence_after();
                 const uint32_t from = lane_base + buf * 256 + c0;
+                if (PARTS) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    if (32 * c < cols) {
+                    for (int c = 0; c < 4; ++c) {
+                        if (32 * c >= cols) continue;
+                        float v[32];
                         tmem_load32(from + 32 * c, v);
-                        tmem_wait();
-                        if (PARTS) {
+                        tmem_wait(v);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                sum[c][i] = k_first > k_begin ? add2(sum[c][i], f2(v[2 * i], v[2 * i + 1]))
-                                                              : f2(v[2 * i], v[2 * i + 1]);
+                        for (int i = 0; i < 16; ++i)
+                            sum[c][i] = k_first > k_begin ? add2(sum[c][i], f2(v[2 * i], v[2 * i + 1]))
+                                                          : f2(v[2 * i], v[2 * i + 1]);
+                    }
+                    release(tempty + 8 * buf);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        if (32 * c < cols) {
+                            tmem_load32(from + 32 * c, v);
+                            tmem_wait(v);
                         }
+                        if (c == 3) release(tempty + 8 * buf);
+                        if (32 * c < cols)
+                            ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c, v, turn);
                     }
-                    if (c == 3) {                       // read: the next multiplies may overwrite it
-                        umma_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(leader_addr(tempty + 8 * buf));
-                    }
-                    if (!PARTS && 32 * c < cols)
-                        ep.chunk(a, q, split, m0, ni * q.bn + c0 + 32 * c, c0 + 32 * c, v, turn);
                 }
             }
             if (!ok) break;
@@ -632,8 +684,9 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
 template <int KIND, bool AT, bool BT, bool PARTS>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
-    // one round of tiles is short anyway: finer parts
-    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? 4 : PART / BK;
+    // one round of tiles is short anyway: finer parts, as far as the multiplies hide them (a part costs the
+    // epilogue some 1900 clocks, a step 512 a pass)
+    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? (a.b.planes > 1 ? 2 : 4) : PART / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -700,7 +753,8 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
     const int steps = q.whole || a.live ? q.steps : q.kb;       // live rows split as the device finds it
-    const bool parts = (steps * BK > PART || (steps > 4 && q.items <= N_SM / 2)) && (kind == MM_LSE || a.b.planes > 1);
+    const bool parts = (steps * BK > PART || (steps > (a.b.planes > 1 ? 2 : 4) && q.items <= N_SM / 2)) &&
+                       (kind == MM_LSE || a.b.planes > 1);
     if (kind == MM_LSE)
         return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
                      : launch<MM_LSE, false, false, false>(a, q, stream);
