@@ -806,7 +806,7 @@ __global__ void rows_kernel(const float *__restrict__ dloss, const float *__rest
     if (m >= rows) return;
     const bool live = m < rm.n(rows);
     float r = dloss[reduction != MMS_REDUCE_NONE ? 0 : live ? rm.row(m) : m] * tau;
-    if (reduction == MMS_REDUCE_MEAN) r /= *count;
+    if (reduction == MMS_REDUCE_MEAN) r = *count == 0.f ? 0.f : r / *count;     // no row counts: gradients of 0
     if (m == 0 && whole) *whole = r;
     if (!live || (!rm.live && !row_counts(index, prob, k, ignore, m))) r = 0.f;
     if (r != 0.f)

@@ -166,10 +166,11 @@ def test_many_lists_of_which_some_are_empty(dtype):
         compare(x, w, parts, 1.5, reduction, dloss, loss, grads)
 
 
-@pytest.mark.parametrize("rows", [9, 700])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 9, 700])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_every_row_left_out(reduction, rows):
-    x, w, target, _ = head_inputs(rows, 50, 24, F32)
+def test_every_row_left_out(reduction, rows, dtype):
+    x, w, target, _ = head_inputs(rows, 50, 24, dtype)
     target[:] = -100
     loss, grads = run_ce(x, w, target, reduction, torch.ones(rows) if reduction == "none" else torch.tensor(1.0))
     if reduction == "mean":
