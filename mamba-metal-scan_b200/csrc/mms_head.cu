@@ -34,8 +34,8 @@
 // Backward:  rows_kernel: r; x staged with the left-out rows as zeros (so that
 //            nothing in them, NaN included, reaches dw); per piece: product
 //            MM_GRAD, sparse_kernel sets dz at the indices (from logq2, in
-//            fp32, as expm1(log q) + 1 - p: no cancellation when a target's
-//            probability is near 1), then MM_OUT twice.
+//            fp32; as expm1(log q) + 1 - p where p is near 1, so that nothing
+//            cancels), then MM_OUT twice.
 //
 // bf16: dz is stored in bf16, one plane: without r where it is the same for
 // all rows (mean, sum: q - p is often close to -1, which bf16 holds better
@@ -875,7 +875,7 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
     const float r = rs[m];
     if (r == 0.f) return;                               // dz is 0 there already
     uint16_t *o = g + m * ldg + (v - v0);
-    float p = 1.f, d = expm1f(LN2 * logq2[e]);
+    float p = 1.f;
     if (prob) {                                         // an index may occur twice: the first one writes
         p = 0.f;
         for (int j = 0; j < k; ++j) {
@@ -884,7 +884,9 @@ sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
             p += prob[m * k + j];
         }
     }
-    d = (unit != 0.f ? unit : r) * (d + (1.f - p));
+    // q - p without rounding at 1 where both are small, nor losing 1 - q where p is near 1
+    const float lq = LN2 * logq2[e];
+    float d = (unit != 0.f ? unit : r) * (p > 0.5f ? expm1f(lq) + (1.f - p) : expf(lq) - p);
     for (int q = 0; q < planes; ++q, o += gplane) {
         if (fp16) {
             const __half t = __float2half_rn(d);

@@ -75,10 +75,12 @@ def solve(x, w, index, p, own, counts, tau, reduction, dloss):
     q = torch.exp(z - lse[:, None])
     mass = p.sum(1, keepdim=True)
     dz = (q * mass).scatter_add(1, index, -p) * r[:, None]
-    # dz: q to within the errors of z and lse; p to 32 roundings; then stored with dtype's
-    # roundoff (float32: two parts, 2^-22)
-    ed = r.abs()[:, None] * (q * (2 * (ez + e_lse)[:, None] + 16 * U32)
-                             + torch.zeros_like(q).scatter_add(1, index, (64 + p.shape[1]) * U32 * (p + log_q.abs().clamp(max=1))))
+    # dz: q to within the errors of z and lse; p to its exponential (arguments up to 40, a few
+    # roundings) and its sum over lists (k / 32 a lane, five levels); q - p itself rounds at its
+    # own size, or at 1 where p is above 1/2; then dz is stored with dtype's roundoff (float32:
+    # two parts, 2^-22)
+    ep = (64 + p.shape[1] / 32) * U32 * p + 4 * U32 * (p > 0.5)
+    ed = r.abs()[:, None] * (q * (2 * (ez + e_lse)[:, None] + 16 * U32) + torch.zeros_like(q).scatter_add(1, index, ep))
     ed = ed + dz.abs() * (u(dtype) if dtype != torch.float32 else 4 * U32)
     if dtype == torch.float32:
         ed = ed + 2 * FOOT * r.abs()[:, None]

@@ -74,7 +74,7 @@ def test_cross_entropy_at_odd_sizes(rows, vocab, dim, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,vocab,dim,k,tau", [(1, 1, 1, 1, 1.0), (1, 70, 24, 1, 2.0), (5, 300, 65, 7, 0.5),
                                                   (130, 1000, 72, 33, 2.0), (257, 513, 640, 64, 4.0),
-                                                  (40, 2000, 128, 1024, 1.0)])
+                                                  (40, 2000, 128, 1024, 1.0), (600, 5000, 64, 500, 2.0)])
 def test_distillation_at_odd_sizes(rows, vocab, dim, k, tau, dtype):
     x, w, _, gen = head_inputs(rows, vocab, dim, dtype, seed=rows + vocab + dim)
     index = torch.randint(0, vocab, (rows, k), generator=gen)          # with repeats
@@ -114,6 +114,22 @@ def test_pieces_of_the_vocabulary(dtype, monkeypatch):
     tol = 2.0 ** -7 if dtype == BF16 else 2e-5
     check_norm("dx", grads[0], dx.cpu(), tol)
     check_norm("dw", grads[1], dw.cpu(), tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_small_probabilities_of_long_lists(dtype):
+    """Teacher probabilities near 1e-3 against student ones near 1e-5: dz is their difference to
+    float32's roundoff of its own size (8 roundings: 5e-7), not of 1."""
+    rows, vocab, dim, k = 400, 20000, 64, 1024
+    x, w, _, gen = head_inputs(rows, vocab, dim, dtype, seed=21)
+    index = torch.stack([torch.randperm(vocab, generator=gen)[:k] for _ in range(rows)])
+    logits = 0.5 * torch.randn(rows, k, generator=gen)
+    xd, wd = leaves(x, w)
+    grads = torch.autograd.grad(linear_distillation(xd, wd, index.to(DEV), logits.to(DEV), 2.0), [xd, wd])
+    want = solve(x, w, *sparse(k, index=index, logits=logits, tau=2.0), 2.0, "mean", torch.tensor(1.0))
+    for name, got in zip(("dx", "dw"), grads):
+        check(name, got, want[name], want["e_" + name])
+        check_norm(name, got, want[name], 2.0 ** -7 if dtype == BF16 else 3e-6)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
