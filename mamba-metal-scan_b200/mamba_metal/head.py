@@ -68,25 +68,31 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     d = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, d)
-    if t.shape[0] == 1 or d == 1 or t.stride(1) != 1 or t.stride(0) < d:
-        t = t.contiguous()
-        if t.stride() != (d, 1):                # sizes of one: strides are free, the kernels' are not
-            t = t.as_strided(t.shape, (d, 1))
+    if t.stride() != (d, 1):                    # not plainly contiguous
+        if t.shape[0] == 1 or d == 1 or t.stride(1) != 1 or t.stride(0) < d:
+            t = t.contiguous()
+            if t.stride() != (d, 1):            # sizes of one: strides are free, the kernels' are not
+                t = t.as_strided(t.shape, (d, 1))
     return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
 
 
-def _check_head(what, x, weight, others, reduction):
-    tensors = (x, weight, *others)
-    if not x.is_cuda or any(t.device != x.device for t in tensors):
+_INDEX_TYPES = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
+
+
+def _check_head(what, x, weight, index, other=None):
+    device, dtype = x.device, x.dtype
+    if not x.is_cuda or weight.device != device or index.device != device \
+            or (other is not None and other.device != device):
         raise RuntimeError(f"{what} runs the CUDA kernels and needs every input on the same CUDA "
-                           "device; saw " + ", ".join(str(t.device) for t in tensors))
-    if x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
-        raise RuntimeError(f"{what} takes float32 or bfloat16, x and weight alike; got {x.dtype}, "
+                           "device; saw " + ", ".join(str(t.device) for t in (x, weight, index, other)
+                                                      if t is not None))
+    if dtype not in (torch.float32, torch.bfloat16) or weight.dtype != dtype:
+        raise RuntimeError(f"{what} takes float32 or bfloat16, x and weight alike; got {dtype}, "
                            f"{weight.dtype}")
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError(f"bad shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    if others[0].dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
-        raise RuntimeError(f"{what} takes integer indices; got {others[0].dtype}")
+    if index.dtype not in _INDEX_TYPES:
+        raise RuntimeError(f"{what} takes integer indices; got {index.dtype}")
 
 
 def _check_reduction(reduction):
@@ -97,6 +103,12 @@ def _check_reduction(reduction):
 def _flat(t, *shape):
     """t.reshape(shape), without a view where the shape is that already."""
     return t if t.dim() == len(shape) else t.reshape(shape)
+
+
+def _as(t, dtype):
+    """t contiguous and of this type; t itself where it is that already."""
+    t = t if t.dtype == dtype else t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _no_rows(x, shape, reduction):
@@ -124,7 +136,7 @@ class LinearCrossEntropyCUDA(torch.autograd.Function):
         x, weight, target, kept = ctx.saved_tensors
         with _native.on_device(x.device):
             dx, dw = _native.linear_ce_bwd(x, weight, target, ctx.ignore_index, ctx.reduction,
-                                           dloss.float().contiguous(), kept,
+                                           _as(dloss, torch.float32), kept,
                                            *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None
 
@@ -146,7 +158,7 @@ class LinearDistillationCUDA(torch.autograd.Function):
         x, weight, index, kept = ctx.saved_tensors
         with _native.on_device(x.device):
             dx, dw = _native.linear_kd_bwd(x, weight, index, ctx.temperature, ctx.reduction,
-                                           dloss.float().contiguous(), kept,
+                                           _as(dloss, torch.float32), kept,
                                            *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None, None
 
@@ -174,13 +186,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     _check_reduction(reduction)
     if not _dispatch(impl, x):
         return linear_cross_entropy_ref(x, weight, target, ignore_index, reduction)
-    _check_head("linear_cross_entropy", x, weight, (target,), reduction)
+    _check_head("linear_cross_entropy", x, weight, target)
     if target.shape != x.shape[:-1]:
         raise ValueError(f"target {tuple(target.shape)} does not match x {tuple(x.shape)}")
     if target.numel() == 0:
         return _no_rows(x, target.shape, reduction)
     x2, w2 = _rows(x), _rows(weight)
-    t = _flat(target, -1).long().contiguous()
+    t = _as(_flat(target, -1), torch.int64)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         loss = LinearCrossEntropyCUDA.apply(x2, w2, t, int(ignore_index), reduction)
     else:
@@ -219,15 +231,15 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: to
     if not _dispatch(impl, x):
         return linear_distillation_ref(x, weight, teacher_index, teacher_logits.detach(),
                                        temperature, reduction)
-    _check_head("linear_distillation", x, weight, (teacher_index, teacher_logits), reduction)
+    _check_head("linear_distillation", x, weight, teacher_index, teacher_logits)
     if not teacher_logits.is_floating_point():
         raise RuntimeError(f"teacher_logits must be floating point; got {teacher_logits.dtype}")
     lead = x.shape[:-1]
     if teacher_index.numel() == 0:
         return _no_rows(x, lead, reduction)
     x2, w2 = _rows(x), _rows(weight)
-    index = _flat(teacher_index, -1, k).long().contiguous()
-    logits = _flat(teacher_logits.detach(), -1, k).float().contiguous()
+    index = _as(_flat(teacher_index, -1, k), torch.int64)
+    logits = _as(_flat(teacher_logits.detach(), -1, k), torch.float32)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         loss = LinearDistillationCUDA.apply(x2, w2, index, logits, temperature, reduction)
     else:
