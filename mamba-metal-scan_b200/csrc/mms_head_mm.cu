@@ -24,8 +24,12 @@
 // so the concurrent tiles share one side's panels in L2 and the long side is
 // read from HBM once.
 //
-// float32 factors are two fp16 planes each (see mms_head.cu); a product then
-// runs over the pairs of planes but the two second ones, smallest terms first.
+// float32 factors are two fp16 planes each (see mms_head.cu) and a product the
+// sum of three of their products (not the second by the second). A stage then
+// holds both planes of both factors (3 stages of 64 KB) and each is copied
+// once for its three uses: 64 KB for 12 multiplies where one pair of planes
+// after the other takes 96 KB. At 8192 x 32768 x 640 that is 3.1 ms for the
+// four products against 3.6: the copies no longer bound them.
 //
 // The tensor core adds each 16 summed elements to its fp32 sum with truncation,
 // not rounding, so a long sum drifts towards zero by about n 2^-25 of itself
@@ -34,7 +38,9 @@
 // goes to its own tensor memory buffer and the epilogue warps add the parts up
 // in registers, rounding to nearest (`PARTS`). Parts of 512 cost nothing
 // beside the multiplies; of 256, 25 % of the log-sum-exp at 8192 x 131072 x
-// 2048 (4.15 ms against 3.31); of 128, 80 %.
+// 2048 (4.15 ms against 3.31); of 128, 80 %. With two planes by two each
+// element is added three times, so parts are of 256 (3.17 ms for the four
+// products; of 384 3.06 ms but errors up to 1.5e-6, of 192 3.37 ms).
 //
 // The epilogue turns a warp's 32 rows x 32 columns through shared memory, in
 // 16-byte pieces (16-bit results already rounded and packed), so that its
@@ -70,12 +76,15 @@ namespace mms {
 
 namespace {
 
-constexpr int TM = 256, BK = 64, STAGES = 6, THREADS = 384;
+constexpr int TM = 256, BK = 64, THREADS = 384;
 constexpr int HALF = 16384;                                  // bytes of one CTA's a (or b) per stage
 constexpr int GROUP = 16;
-constexpr int PART = 512;                                    // summed elements (of each pair of planes) per part
+constexpr int PART = 512;                                    // summed elements per part
+constexpr int PART_BOTH = 256;                               // the same for two planes by two
 constexpr int TURN = 32 * 33;                                // floats of a warp's tile to turn
-constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * HALF + 8 * TURN * 4;
+// Stages: two planes by two stand side by side in one stage, and are read once for all three passes.
+constexpr int STAGE_BYTES = 6 * 2 * HALF;                    // of all stages
+constexpr size_t SMEM = 1024 + (size_t)STAGE_BYTES + 8 * TURN * 4;
 
 __device__ unsigned int g_mm_timeout;
 
@@ -93,7 +102,9 @@ int passes_of(int planes_a, int planes_b) { return planes_a + planes_b - 1; }
 // Columns per tile and splits of the tiles beyond whole rounds: the cheapest
 // by a model of a pair's clocks. A step of 64 summed elements is the larger of
 // the multiplies (2 clocks a column, at full rate) and the copies of 16 KB +
-// 64 bytes a column into each CTA; an item ends with an epilogue that nothing
+// 64 bytes a column into each CTA; two planes by two need fewer copies, but
+// narrow tiles pay there for the parts (d = 640: dx 0.88 ms at 128 columns,
+// 0.71 at 224), so the same model serves; an item ends with an epilogue that nothing
 // overlaps on the last one. Splits pay a write and a read of their partial
 // sums and one more launch.
 Tiles plan(MmKind kind, int m, int n, int k, int passes, size_t split_bytes)
@@ -455,11 +466,12 @@ struct Epilogue {
     }
 };
 
-template <int KIND, bool AT, bool BT, bool PARTS>
+template <int KIND, bool AT, bool BT, bool PARTS, bool BOTH>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const MmArgs a, const Tiles planned, uint32_t limit, int skip)
 {
+    constexpr int STAGES = BOTH ? 3 : 6, PLANES = BOTH ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * STAGES + 5];
     __shared__ uint32_t tmem_slot;
@@ -490,7 +502,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     umma_fence_after();
     const uint32_t tmem = tmem_slot;
     const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    const int passes = a.a.planes + a.b.planes - 1;
+    const int passes = BOTH ? 1 : a.a.planes + a.b.planes - 1;      // over the stages
     const int bhalf = planned.bn / 2;
     const int bblocks = BT ? (bhalf + 63) / 64 : 0;
     const Live live = live_of<AT>(a, planned);
@@ -521,21 +533,26 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     if (it == skip) continue;
                     const uint32_t bar = leader_addr(full + 8 * st);
-                    if (rank == 0) mbar_expect(full + 8 * st, a_bytes + 2 * b_bytes);
-                    const uint32_t sa = tiles + st * 2 * HALF, sb = sa + HALF;
+                    if (rank == 0) mbar_expect(full + 8 * st, PLANES * (a_bytes + 2 * b_bytes));
+                    const uint32_t sa = tiles + st * PLANES * 2 * HALF, sb = sa + PLANES * HALF;
                     const int k0 = kb * BK;
-                    if (!some) {
-                    } else if (AT) {
-                        tma3_pair(sa, &map_a, m0, k0, pa, bar);
-                        tma3_pair(sa + 8192, &map_a, m0 + 64, k0, pa, bar);
-                    } else {
-                        tma3_pair(sa, &map_a, k0, m0, pa, bar);
-                    }
-                    if (BT) {
-                        for (int b = 0; b < bblocks; ++b)
-                            tma3_pair(sb + b * 8192, &map_b, n0 + 64 * b, k0, pb, bar);
-                    } else {
-                        tma3_pair(sb, &map_b, k0, n0, pb, bar);
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        const uint32_t da = sa + p * HALF, db = sb + p * HALF;
+                        if (BOTH) pa = pb = p;
+                        if (!some) {
+                        } else if (AT) {
+                            tma3_pair(da, &map_a, m0, k0, pa, bar);
+                            tma3_pair(da + 8192, &map_a, m0 + 64, k0, pa, bar);
+                        } else {
+                            tma3_pair(da, &map_a, k0, m0, pa, bar);
+                        }
+                        if (BT) {
+                            for (int b = 0; b < bblocks; ++b)
+                                tma3_pair(db + b * 8192, &map_b, n0 + 64 * b, k0, pb, bar);
+                        } else {
+                            tma3_pair(db, &map_b, k0, n0, pb, bar);
+                        }
                     }
                     issued = it + 1;
                 }
@@ -564,13 +581,17 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     break;
                 }
                 umma_fence_after();
-                const uint32_t sa = tiles + st * 2 * HALF, sb = sa + HALF;
-                const uint64_t da = AT ? umma_desc(sa, 8192, 1024) : umma_desc(sa, 16, 1024);
-                const uint64_t db = BT ? umma_desc(sb, 8192, 1024) : umma_desc(sb, 16, 1024);
+                const uint32_t sa = tiles + st * PLANES * 2 * HALF, sb = sa + PLANES * HALF;
 #pragma unroll
-                for (int k = 0; k < BK / 16; ++k)       // 16 elements on: 32 bytes along a row, or 16 rows
-                    umma_pair(tmem + buf * 256, da + (AT ? 2048 / 16 : 32 / 16) * k,
-                              db + (BT ? 2048 / 16 : 32 / 16) * k, idesc, i > 0 || k > 0);
+                for (int c = 0; c < (BOTH ? 3 : 1); ++c) {      // (1, 0), (0, 1), (0, 0): the small products first
+                    const uint32_t pa = sa + (BOTH && c == 0 ? HALF : 0), pb = sb + (BOTH && c == 1 ? HALF : 0);
+                    const uint64_t da = AT ? umma_desc(pa, 8192, 1024) : umma_desc(pa, 16, 1024);
+                    const uint64_t db = BT ? umma_desc(pb, 8192, 1024) : umma_desc(pb, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)   // 16 elements on: 32 bytes along a row, or 16 rows
+                        umma_pair(tmem + buf * 256, da + (AT ? 2048 / 16 : 32 / 16) * k,
+                                  db + (BT ? 2048 / 16 : 32 / 16) * k, idesc, i > 0 || c > 0 || k > 0);
+                }
                 umma_commit_pair(empty + 8 * st);
             }
             if (!ok) break;
@@ -593,7 +614,7 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive_cluster(leader_addr(bar));
         };
         const int c0 = side * q.half, cols = side ? q.bn - q.half : q.half;
-        float *turn = reinterpret_cast<float *>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * 2 * HALF) + warp * TURN;
+        float *turn = reinterpret_cast<float *>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGE_BYTES) + warp * TURN;
         int use = 0;
         bool ok = true;
         for (int t = pair; ok && t < q.items; t += pairs) {
@@ -687,22 +708,32 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap *map, const Factor
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool AT, bool BT, bool PARTS>
+template <int KIND, bool AT, bool BT, bool PARTS, bool BOTH>
 cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
     // one round of tiles is short anyway: finer parts, as far as the multiplies hide them (a part costs the
     // epilogue some 1900 clocks, a step 512 a pass)
-    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? (a.b.planes > 1 ? 2 : 4) : PART / BK;
+    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? (BOTH ? 2 : 4) : (BOTH ? PART_BOTH : PART) / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
         return cudaErrorInvalidValue;
-    constexpr auto kernel = mm_kernel<KIND, AT, BT, PARTS>;
+    constexpr auto kernel = mm_kernel<KIND, AT, BT, PARTS, BOTH>;
     const cudaError_t e = smem_opt_in<kernel>(SMEM);
     if (e != cudaSuccess) return e;
     const int pairs = a.live && !AT ? N_SM / 2 : std::min(N_SM / 2, q.items);
     kernel<<<2 * pairs, THREADS, SMEM, stream>>>(ma, mb, a, q, tma_wait_limit(), tma_skip_item());
     return cudaGetLastError();
+}
+
+template <int KIND, bool AT, bool BT>
+cudaError_t launch_as(const MmArgs &a, const Tiles &q, bool parts, bool both, cudaStream_t stream)
+{
+    if (both)
+        return parts ? launch<KIND, AT, BT, true, true>(a, q, stream) : launch<KIND, AT, BT, false, true>(a, q, stream);
+    if constexpr (KIND == MM_LSE)
+        if (parts) return launch<KIND, AT, BT, true, false>(a, q, stream);
+    return launch<KIND, AT, BT, false, false>(a, q, stream);
 }
 
 // out = acc + the partial sums of the split tiles, in order; a CTA per 4 rows of a tile,
@@ -759,18 +790,13 @@ cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
     // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
     const int steps = q.whole || a.live ? q.steps : q.kb;       // live rows split as the device finds it
-    const bool parts = (steps * BK > PART || (steps > (a.b.planes > 1 ? 2 : 4) && q.items <= N_SM / 2)) &&
-                       (kind == MM_LSE || a.b.planes > 1);
-    if (kind == MM_LSE)
-        return parts ? launch<MM_LSE, false, false, true>(a, q, stream)
-                     : launch<MM_LSE, false, false, false>(a, q, stream);
-    if (kind == MM_GRAD)
-        return parts ? launch<MM_GRAD, false, false, true>(a, q, stream)
-                     : launch<MM_GRAD, false, false, false>(a, q, stream);
-    const cudaError_t e = a.a.t ? parts ? launch<MM_OUT, true, true, true>(a, q, stream)
-                                        : launch<MM_OUT, true, true, false>(a, q, stream)
-                                : parts ? launch<MM_OUT, false, true, true>(a, q, stream)
-                                        : launch<MM_OUT, false, true, false>(a, q, stream);
+    const bool both = a.a.planes == 2 && a.b.planes == 2;
+    const bool parts = (kind == MM_LSE || both) && (steps * BK > (both ? PART_BOTH : PART) ||
+                                                    (q.items <= N_SM / 2 && steps > (both ? 2 : 4)));
+    if (kind == MM_LSE) return launch_as<MM_LSE, false, false>(a, q, parts, both, stream);
+    if (kind == MM_GRAD) return launch_as<MM_GRAD, false, false>(a, q, parts, both, stream);
+    const cudaError_t e = a.a.t ? launch_as<MM_OUT, true, true>(a, q, parts, both, stream)
+                                : launch_as<MM_OUT, false, true>(a, q, parts, both, stream);
     // the live rows' tiles are not known here: as many CTAs as they may need
     const int rest = a.live && !a.a.t ? std::min(N_SM / 2 - 1, q.mt * q.nt) : q.mt * q.nt - q.whole;
     if (e != cudaSuccess || !rest) return e;
