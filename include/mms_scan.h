@@ -290,8 +290,8 @@ int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw
  *     u = weight * h / rms(h)             rms(v) = sqrt(mean(v^2) + eps)
  * x, y, h, u (rows, dim) contiguous, gate (rows, dim) with row stride ldg >=
  * dim, weight, post, scale (dim), all of storage type dtype; u comes from h
- * before its rounding. The forward also writes stat (rows, 2) float32: 1/rms(a)
- * (0 without post) and 1/rms(h). The backward gives the gradients of every
+ * before its rounding. The forward also writes stat (rows, 2) float32, which the
+ * backward reads: 1/rms(a) (0 without post) and 1/rms(h); NULL: not wanted. The backward gives the gradients of every
  * input from dh and du; dgate (rows, dim) is contiguous; dweight, dpost,
  * dscale are sums over the rows in a fixed order, through a workspace of
  * mms_norm_workspace_size() bytes (256-byte aligned). dy may be dx's pointer

@@ -383,7 +383,7 @@ int mms_norm_fwd(const void *x, const void *y, const void *gate, long long ldg, 
 {
     const int rc = check_norm(x, y, gate, ldg, weight, post, scale, rows, dim, dtype);
     if (rc) return rc;
-    if (!h || !u || !stat || !(eps >= 0.f)) return MMS_ERR_INVALID_ARG;
+    if (!h || !u || !(eps >= 0.f)) return MMS_ERR_INVALID_ARG;
     const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
     if (!aligned(h, e) || !aligned(u, e) || !aligned(stat, 4)) return MMS_ERR_MISALIGNED;
     mms::NormArgs a{};

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_fwd_kernel(const NormArgs a)
 #pragma unroll
         for (int i = 0; i < E; ++i) h[i] *= r2 * w[i];
         C::store(static_cast<T *>(a.u) + o, a.dim, h);
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && a.stat) {
             a.stat[2 * r] = r1;
             a.stat[2 * r + 1] = r2;
         }
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormArgs a)
             static_cast<T *>(a.h)[r * a.dim + i] = from_f<T>(v);
             static_cast<T *>(a.u)[r * a.dim + i] = from_f<T>(v * r2 * to_f(row.w[i]));
         }
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && a.stat) {
             a.stat[2 * r] = r1;
             a.stat[2 * r + 1] = r2;
         }

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -271,28 +272,46 @@ def _dtype(t) -> int:
     return 1 if t.dtype == torch.bfloat16 else 0
 
 
-def _head_workspace(x, w, k: int, backward: bool):
-    nb = int(load().mms_head_workspace_size(x.shape[0], w.shape[0], x.shape[1], k, _dtype(x),
-                                            x.stride(0), w.stride(0), int(backward)))
-    return torch.empty(max(nb, 1), dtype=torch.uint8, device=x.device)
+@functools.lru_cache(maxsize=256)
+def _head_sizes(m: int, v: int, d: int, k: int, dtype: int, ldx: int, ldw: int, backward: bool):
+    """(workspace, kept) bytes, the workspace rounded up to 256."""
+    lib = load()
+    ws = int(lib.mms_head_workspace_size(m, v, d, k, dtype, ldx, ldw, int(backward)))
+    return (ws + 255) // 256 * 256, int(lib.mms_head_kept_size(m, k))
 
 
-def _kept(m: int, k: int, device):
-    return torch.empty(int(load().mms_head_kept_size(m, k)), dtype=torch.uint8, device=device)
+def _head_buffers(x, w, k: int, keep: bool):
+    """(workspace address, its bytes, kept address, kept tensor, all that must live until the call).
+    Without `keep` what the backward would need goes behind the workspace, in one allocation."""
+    nb, kept_nb = _head_sizes(x.shape[0], w.shape[0], x.shape[1], k, _dtype(x), x.stride(0),
+                              w.stride(0), False)
+    if not keep:
+        ws = torch.empty(nb + kept_nb, dtype=torch.uint8, device=x.device)
+        base = ws.data_ptr()
+        return base, nb, base + nb, None, ws
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    kept = torch.empty(kept_nb, dtype=torch.uint8, device=x.device)
+    return ws.data_ptr(), nb, kept.data_ptr(), kept, ws
 
 
-def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str):
+def _head_workspace(x, w, k: int):
+    """The backward's."""
+    nb, _ = _head_sizes(x.shape[0], w.shape[0], x.shape[1], k, _dtype(x), x.stride(0), w.stride(0),
+                        True)
+    return torch.empty(nb, dtype=torch.uint8, device=x.device)
+
+
+def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str, keep: bool = True):
     """(loss, kept) of mms_linear_ce_fwd; x (M, D), w (V, D) with row strides. kept: what the
-    backward needs."""
+    backward needs (None without `keep`)."""
     m, d = x.shape
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    kept = _kept(m, 0, x.device)
-    ws = _head_workspace(x, w, 0, False)
+    ws, nb, kept_at, kept, _live = _head_buffers(x, w, 0, keep)
     rc = load().mms_linear_ce_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   target.data_ptr(), ignore_index, red, loss.data_ptr(),
-                                  kept.data_ptr(), ws.data_ptr(), ws.numel(), m, w.shape[0], d,
-                                  _dtype(x), _stream(x.device))
+                                  kept_at, ws, nb, m, w.shape[0], d, _dtype(x),
+                                  _stream(x.device))
     if rc:
         _check(rc, "mms_linear_ce_fwd")
     return loss, kept
@@ -309,7 +328,7 @@ def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, kept,
     """(dx, dw) of mms_linear_ce_bwd; None for one that is not needed."""
     m, d = x.shape
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    ws = _head_workspace(x, w, 0, True)
+    ws = _head_workspace(x, w, 0)
     rc = load().mms_linear_ce_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   target.data_ptr(), ignore_index, REDUCTIONS[reduction],
                                   dloss.data_ptr(), kept.data_ptr(), pdx, pdw, ws.data_ptr(),
@@ -319,18 +338,17 @@ def linear_ce_bwd(x, w, target, ignore_index: int, reduction: str, dloss, kept,
     return dx, dw
 
 
-def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str):
-    """(loss, kept) of mms_linear_kd_fwd. kept: what the backward needs."""
+def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str, keep: bool = True):
+    """(loss, kept) of mms_linear_kd_fwd. kept: what the backward needs (None without `keep`)."""
     m, d = x.shape
     k = index.shape[1]
     red = REDUCTIONS[reduction]
     loss = torch.empty((m,) if red == 0 else (), device=x.device)
-    kept = _kept(m, k, x.device)
-    ws = _head_workspace(x, w, k, False)
+    ws, nb, kept_at, kept, _live = _head_buffers(x, w, k, keep)
     rc = load().mms_linear_kd_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   index.data_ptr(), logits.data_ptr(), k, temperature, red,
-                                  loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), ws.numel(),
-                                  m, w.shape[0], d, _dtype(x), _stream(x.device))
+                                  loss.data_ptr(), kept_at, ws, nb, m, w.shape[0], d, _dtype(x),
+                                  _stream(x.device))
     if rc:
         _check(rc, "mms_linear_kd_fwd")
     return loss, kept
@@ -342,7 +360,7 @@ def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, kept,
     m, d = x.shape
     k = index.shape[1]
     dx, dw, pdx, pdw = _head_grads(x, w, need_x, need_w)
-    ws = _head_workspace(x, w, k, True)
+    ws = _head_workspace(x, w, k)
     rc = load().mms_linear_kd_bwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   index.data_ptr(), k, temperature, REDUCTIONS[reduction],
                                   dloss.data_ptr(), kept.data_ptr(), pdx, pdw,
@@ -357,14 +375,15 @@ def _opt(t) -> int:
     return 0 if t is None else _ptr(t)
 
 
-def norm_fwd(x, y, gate, weight, post, scale, eps: float):
-    """(h, u, stat) of mms_norm_fwd; x, y (M, D) contiguous, gate (M, D) with a row stride."""
+def norm_fwd(x, y, gate, weight, post, scale, eps: float, keep: bool = True):
+    """(h, u, stat) of mms_norm_fwd; x, y (M, D) contiguous, gate (M, D) with a row stride.
+    stat: what the backward needs (None without `keep`)."""
     m, d = x.shape
     h, u = torch.empty_like(x), torch.empty_like(x)
-    stat = torch.empty(m, 2, device=x.device)
+    stat = torch.empty(m, 2, device=x.device) if keep else None
     rc = load().mms_norm_fwd(_ptr(x), _ptr(y), _opt(gate), d if gate is None else gate.stride(0),
                              _ptr(weight), _opt(post), _opt(scale), eps, _ptr(h), _ptr(u),
-                             _ptr(stat), m, d, _dtype(x), _stream(x.device))
+                             _opt(stat), m, d, _dtype(x), _stream(x.device))
     if rc:
         _check(rc, "mms_norm_fwd")
     return h, u, stat

@@ -197,7 +197,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         loss = LinearCrossEntropyCUDA.apply(x2, w2, t, int(ignore_index), reduction)
     else:
         with _native.on_device(x.device):
-            loss = _native.linear_ce_fwd(x2, w2, t, int(ignore_index), reduction)[0]
+            loss, _ = _native.linear_ce_fwd(x2, w2, t, int(ignore_index), reduction, keep=False)
     return _flat(loss, *target.shape) if reduction == "none" else loss
 
 
@@ -244,5 +244,5 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: to
         loss = LinearDistillationCUDA.apply(x2, w2, index, logits, temperature, reduction)
     else:
         with _native.on_device(x.device):
-            loss = _native.linear_kd_fwd(x2, w2, index, logits, temperature, reduction)[0]
+            loss, _ = _native.linear_kd_fwd(x2, w2, index, logits, temperature, reduction, keep=False)
     return _flat(loss, *lead) if reduction == "none" else loss

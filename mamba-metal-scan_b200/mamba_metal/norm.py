@@ -114,5 +114,5 @@ def residual_rms_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
     else:
         x, y, weight, post_weight, gate, scale = args
         with _native.on_device(device):
-            h, u, _ = _native.norm_fwd(x, y, gate, weight, post_weight, scale, eps)
+            h, u, _ = _native.norm_fwd(x, y, gate, weight, post_weight, scale, eps, keep=False)
     return (h, u) if flat else (h.view(shape), u.view(shape))

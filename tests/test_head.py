@@ -156,7 +156,7 @@ def test_c_entries_check_before_any_launch():
         return lib.mms_norm_fwd(x, ok, gate, ldg, ok, None, None, eps, ok, ok, stat, m, d, ty, None)
 
     assert norm(m=0) == bad and norm(d=0) == bad and norm(ty=5) == bad and norm(x=None) == bad
-    assert norm(gate=ok, ldg=15) == bad and norm(stat=None) == bad and norm(eps=-1.0) == bad
+    assert norm(gate=ok, ldg=15) == bad and norm(eps=-1.0) == bad
     assert norm(eps=float("nan")) == bad
     assert norm(x=_p(0x10002)) == mis and norm(x=_p(0x10001), ty=1) == mis
 
