@@ -237,8 +237,7 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  *
  * reduction: MMS_REDUCE_NONE (loss, dloss: rows floats), MMS_REDUCE_MEAN (over
  * the rows that count; NaN if there is none) or MMS_REDUCE_SUM (one float).
- * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, lse, picked, prob, count
- * are float32, sums are float32. float32 products run on the tensor cores as
+ * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, dloss and the sums are float32. float32 products run on the tensor cores as
  * two scaled fp16 parts a factor (22 bits; see csrc/mms_head.cu).
  *
  * The forward writes to `kept` (mms_head_kept_size() bytes) what the backward
@@ -247,7 +246,8 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * Rows that are left out cost next to nothing above 512 rows: the products
  * skip them.
  *
- * x, w, dx, dw, kept need 16-byte alignment, ldx, ldw >= dim; k <= MMS_HEAD_MAX_K.
+ * x, w, dx, dw, kept need 16-byte alignment, ldx, ldw >= dim; k, rows, vocab and
+ * dim have the limits below.
  * The workspace (256-byte aligned) has mms_head_workspace_size() bytes; both
  * sizes with k = 0 for the cross entropy; the two directions' sizes differ.
  * No counterpart in the reference, which computes the logits and calls
@@ -259,6 +259,9 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
 #define MMS_REDUCE_MEAN 1
 #define MMS_REDUCE_SUM 2
 #define MMS_HEAD_MAX_K 1024
+#define MMS_HEAD_MAX_ROWS (1 << 24)
+#define MMS_HEAD_MAX_VOCAB (1 << 30)
+#define MMS_HEAD_MAX_DIM (1 << 20)
 size_t mms_head_kept_size(int rows, int k);
 size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, long long ldx,
                                long long ldw, int backward);
@@ -291,14 +294,15 @@ int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw
  * x, y, h, u (rows, dim) contiguous, gate (rows, dim) with row stride ldg >=
  * dim, weight, post, scale (dim), all of storage type dtype; u comes from h
  * before its rounding. The forward also writes stat (rows, 2) float32, which the
- * backward reads: 1/rms(a) (0 without post) and 1/rms(h); NULL: not wanted. The backward gives the gradients of every
- * input from dh and du; dgate (rows, dim) is contiguous; dweight, dpost,
+ * backward reads: 1/rms(a) (0 without post) and 1/rms(h); NULL: not wanted. The
+ * backward gives the gradients of every input from dh and du; dgate (rows, dim) is contiguous; dweight, dpost,
  * dscale are sums over the rows in a fixed order, through a workspace of
  * mms_norm_workspace_size() bytes (256-byte aligned). dy may be dx's pointer
  * where gate, post and scale are NULL (their values are the same).
- * Arrays need their element's alignment.
+ * Arrays need their element's alignment; rows, dim <= MMS_NORM_MAX.
  * No counterpart in the reference (PyTorch ops there, mamba_metal/model.py:85-95).
  */
+#define MMS_NORM_MAX (1 << 30)
 size_t mms_norm_workspace_size(int rows, int dim);
 int mms_norm_fwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
                  const void *post, const void *scale, float eps, void *h, void *u, float *stat,

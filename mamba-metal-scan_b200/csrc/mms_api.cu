@@ -89,11 +89,18 @@ bool proj_ok(float dt_min, float dt_max)
            dt_max > dt_min;
 }
 
+// Beyond these the kernels' 32-bit tile and column numbers could run over.
+bool head_sizes_ok(int rows, int vocab, int dim)
+{
+    return rows >= 1 && vocab >= 1 && dim >= 1 && rows <= MMS_HEAD_MAX_ROWS && vocab <= MMS_HEAD_MAX_VOCAB &&
+           dim <= MMS_HEAD_MAX_DIM;
+}
+
 // Sizes, types and pointers of the head's losses; the workspace's size comes last.
 int check_head(const void *x, long long ldx, const void *w, long long ldw, int rows, int vocab,
                int dim, int k, float tau, int dtype, int reduction)
 {
-    if (rows < 1 || vocab < 1 || dim < 1 || rows > (1 << 24) || k < 1 || k > MMS_HEAD_MAX_K ||
+    if (!head_sizes_ok(rows, vocab, dim) || k < 1 || k > MMS_HEAD_MAX_K ||
         ldx < dim || ldw < dim || (dtype != MMS_F32 && dtype != MMS_BF16) ||
         reduction < MMS_REDUCE_NONE || reduction > MMS_REDUCE_SUM || !(tau > 0.f) || tau > 3.0e38f ||
         !x || !w)
@@ -130,7 +137,7 @@ int head_run(const mms::HeadArgs &a, size_t workspace_bytes, void *stream)
 int check_norm(const void *x, const void *y, const void *gate, long long ldg, const void *weight,
                const void *post, const void *scale, int rows, int dim, int dtype)
 {
-    if (rows < 1 || dim < 1 || (gate && ldg < dim) || (dtype != MMS_F32 && dtype != MMS_BF16) ||
+    if (rows < 1 || dim < 1 || rows > MMS_NORM_MAX || dim > MMS_NORM_MAX || (gate && ldg < dim) || (dtype != MMS_F32 && dtype != MMS_BF16) ||
         !x || !y || !weight)
         return MMS_ERR_INVALID_ARG;
     const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
@@ -305,7 +312,7 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg, const
 size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, long long ldx,
                                long long ldw, int backward)
 {
-    if (rows < 1 || vocab < 1 || dim < 1 || k < 0 || k > MMS_HEAD_MAX_K || rows > (1 << 24) || ldx < dim || ldw < dim ||
+    if (!head_sizes_ok(rows, vocab, dim) || k < 0 || k > MMS_HEAD_MAX_K || ldx < dim || ldw < dim ||
         (dtype != MMS_F32 && dtype != MMS_BF16))
         return 0;
     return mms::head_workspace_bytes(rows, vocab, dim, k, dtype == MMS_BF16, ldx, ldw, backward != 0);
@@ -313,7 +320,7 @@ size_t mms_head_workspace_size(int rows, int vocab, int dim, int k, int dtype, l
 
 size_t mms_head_kept_size(int rows, int k)
 {
-    if (rows < 1 || rows > (1 << 24) || k < 0 || k > MMS_HEAD_MAX_K) return 0;
+    if (rows < 1 || rows > MMS_HEAD_MAX_ROWS || k < 0 || k > MMS_HEAD_MAX_K) return 0;
     return mms::head_kept_bytes(rows, k ? k : 1, k != 0);
 }
 
@@ -374,7 +381,7 @@ int mms_linear_kd_bwd(const void *x, long long ldx, const void *w, long long ldw
 
 size_t mms_norm_workspace_size(int rows, int dim)
 {
-    return rows < 1 || dim < 1 ? 0 : mms::norm_workspace_bytes(rows, dim);
+    return rows < 1 || dim < 1 || rows > MMS_NORM_MAX || dim > MMS_NORM_MAX ? 0 : mms::norm_workspace_bytes(rows, dim);
 }
 
 int mms_norm_fwd(const void *x, const void *y, const void *gate, long long ldg, const void *weight,

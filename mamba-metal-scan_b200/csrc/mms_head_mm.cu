@@ -271,6 +271,8 @@ struct Epilogue {
             s = 0.f;
             at = INT_MAX;
             nth = 0;
+            // as 0 it would make NaN of the -inf behind the last column; the products it stands for are below 2^-60
+            f = fmaxf(f, 1.17549435e-38f);
             if (a.target && in) {
                 const long long t = a.target[a.row_of ? a.row_of[m] : m] - a.first_col;
                 if (t >= 0 && t < a.n) at = (int)t;

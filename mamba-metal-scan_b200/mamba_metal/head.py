@@ -24,6 +24,8 @@ from mamba_metal import _native
 from mamba_metal.scan import _IMPLS
 
 MAX_K = 1024          # entries a row of linear_distillation's teacher lists (MMS_HEAD_MAX_K)
+# the kernels' largest sizes (MMS_HEAD_MAX_ROWS, _VOCAB, _DIM)
+MAX_ROWS, MAX_VOCAB, MAX_DIM = 1 << 24, 1 << 30, 1 << 20
 
 
 def _reduce(rows, counts, reduction: str):
@@ -91,6 +93,10 @@ def _check_head(what, x, weight, index, other=None):
                            f"{weight.dtype}")
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError(f"bad shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    d = x.shape[-1]
+    if x.numel() > MAX_ROWS * d or weight.shape[0] > MAX_VOCAB or d > MAX_DIM:
+        raise ValueError(f"{what} takes up to {MAX_ROWS} rows, {MAX_VOCAB} entries of the vocabulary "
+                         f"and {MAX_DIM} columns; got x {tuple(x.shape)}, weight {tuple(weight.shape)}")
     if index.dtype not in _INDEX_TYPES:
         raise RuntimeError(f"{what} takes integer indices; got {index.dtype}")
 

@@ -21,6 +21,8 @@ from torch.autograd.function import once_differentiable
 from mamba_metal import _native
 from mamba_metal.scan import _IMPLS
 
+MAX_SIZE = 1 << 30    # rows, and columns, of the kernels (MMS_NORM_MAX)
+
 
 def residual_rms_norm_ref(x, y, weight, post_weight=None, gate=None, scale=None, eps: float = 1e-6):
     """residual_rms_norm in PyTorch ops: float32 arithmetic (float64 for float64), results in x's type."""
@@ -101,6 +103,8 @@ def residual_rms_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor,
     if dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != dtype for t in tensors):
         raise RuntimeError("residual_rms_norm takes float32 or bfloat16, all tensors alike; got "
                            + ", ".join(str(t.dtype) for t in tensors))
+    if x.shape[-1] > MAX_SIZE or x.numel() > MAX_SIZE * x.shape[-1]:
+        raise ValueError(f"residual_rms_norm takes up to {MAX_SIZE} rows and columns; got {tuple(x.shape)}")
     if x.numel() == 0:
         return residual_rms_norm_ref(x, y, weight, post_weight, gate, scale, eps)
     d = shape[-1]

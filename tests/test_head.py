@@ -126,6 +126,7 @@ def test_c_entries_check_before_any_launch():
     assert ce_fwd(m=0) == bad and ce_fwd(v=0) == bad and ce_fwd(d=0) == bad
     assert ce_fwd(ldx=15) == bad and ce_fwd(ldw=15) == bad and ce_fwd(ty=2) == bad
     assert ce_fwd(red=3) == bad and ce_fwd(red=-1) == bad and ce_fwd(m=(1 << 24) + 1) == bad
+    assert ce_fwd(v=(1 << 30) + 1) == bad and ce_fwd(d=(1 << 20) + 1, ldx=1 << 21, ldw=1 << 21) == bad
     assert ce_fwd(x=None) == bad and ce_fwd(t=None) == bad
     assert ce_fwd(loss=None) == bad and ce_fwd(kept=None) == bad
     assert ce_fwd(x=_p(0x10008)) == mis and ce_fwd(t=_p(0x10004)) == mis and ce_fwd(kept=_p(0x10008)) == mis
@@ -157,7 +158,7 @@ def test_c_entries_check_before_any_launch():
 
     assert norm(m=0) == bad and norm(d=0) == bad and norm(ty=5) == bad and norm(x=None) == bad
     assert norm(gate=ok, ldg=15) == bad and norm(eps=-1.0) == bad
-    assert norm(eps=float("nan")) == bad
+    assert norm(eps=float("nan")) == bad and norm(m=(1 << 30) + 1) == bad and norm(d=(1 << 30) + 1) == bad
     assert norm(x=_p(0x10002)) == mis and norm(x=_p(0x10001), ty=1) == mis
 
     def norm_bwd(dx=ok, dy=_p(0x30000), post=None, nb=0):

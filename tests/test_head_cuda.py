@@ -231,6 +231,64 @@ def test_indices_outside_the_vocabulary_are_loud_and_stay_in_bounds():
     assert torch.isnan(loss[2]) and torch.isfinite(loss[torch.arange(10) != 2]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [2, 40, 600])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_target_outside_the_vocabulary_makes_its_gradients_nan(reduction, rows, dtype):
+    x, w, target, _ = head_inputs(rows, 60, 24, dtype)
+    target[1] = 60
+    loss, grads = run_ce(x, w, target, reduction, torch.ones(rows) if reduction == "none" else torch.tensor(1.0))
+    bad = torch.arange(rows) == 1
+    assert torch.equal(torch.isnan(loss.cpu()), bad) if reduction == "none" else torch.isnan(loss)
+    assert torch.isnan(grads[0][1]).all() and torch.isnan(grads[1]).all()
+    assert torch.isfinite(grads[0].cpu()[~bad]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 12, 600])
+def test_tiny_values(rows, dtype):
+    """Logits around 1e-45: q is 1 / vocab to its last bit and the loss log(vocab)."""
+    x, w, target, _ = head_inputs(rows, 100, 40, dtype, seed=3)
+    x, w = (x.float() * 1e-30).to(dtype), (w.float() * 1e-15).to(dtype)
+    loss, grads = run_ce(x, w, target, "none", torch.ones(rows))
+    # 100 exponentials and their sum to 2^-20 of them, log and the last rounding of 4.6 to 2^-21 each
+    assert ((loss.cpu().double() - torch.tensor(100.0).double().log()).abs() <= 3 * 2.0 ** -20).all()
+    dz = torch.full((rows, 100), 0.01, dtype=torch.float64)
+    dz[torch.arange(rows), target] -= 1
+    dx = dz @ w.double()
+    # dz to 2^-19 (bf16: two planes or one, 2^-9), sums of 100 terms to 2^-19, the result to its type
+    step = 2.0 ** -18 if dtype == F32 else 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -18
+    assert ((grads[0].cpu().double() - dx).abs() <= step * (dz.abs() @ w.double().abs())).all()
+
+
+def test_calls_on_several_streams_at_once():
+    """Workspaces of calls that run at the same time are their own."""
+    jobs = []
+    for i, (rows, vocab, dim, dtype) in enumerate([(700, 5000, 256, BF16), (260, 3001, 136, F32),
+                                                   (1, 4096, 64, F32)]):
+        x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=30 + i)
+        index = torch.randint(0, vocab, (rows, 5), generator=gen).to(DEV)
+        logits = torch.randn(rows, 5, generator=gen).to(DEV)
+        jobs.append((x, w, target.to(DEV), index, logits, torch.cuda.Stream()))
+
+    def both(xd, wd, target, index, logits):
+        a = linear_cross_entropy(xd, wd, target)
+        b = linear_distillation(xd, wd, index, logits, 2.0)
+        return [a.detach(), b.detach(), *torch.autograd.grad(a, [xd, wd]), *torch.autograd.grad(b, [xd, wd])]
+
+    want = [both(*leaves(x, w), *rest) for x, w, *rest, _ in jobs]
+    ready = [leaves(x, w) for x, w, *_ in jobs]
+    torch.cuda.synchronize()
+    got = [[] for _ in jobs]
+    for _ in range(3):
+        for (_, _, *rest, stream), (xd, wd), g in zip(jobs, ready, got):
+            with torch.cuda.stream(stream):
+                g.append(both(xd, wd, *rest))
+    torch.cuda.synchronize()
+    for one, g in zip(want, got):
+        assert all(torch.equal(a, b) for run in g for a, b in zip(one, run))
+
+
 def test_infinite_and_nan_logits_reach_the_loss():
     """A row that counts and holds inf or NaN has a NaN loss, as PyTorch's."""
     x, w, target, _ = head_inputs(6, 300, 24, F32)
@@ -408,6 +466,10 @@ def test_gpu_refusals():
         linear_cross_entropy(xd, wd, t[:3])
     with pytest.raises(ValueError, match="shapes"):
         linear_cross_entropy(xd, wd[:, :5], t)
+    with pytest.raises(ValueError, match="up to"):      # views: refused before anything is copied
+        linear_cross_entropy(xd[:1].expand((1 << 24) + 1, 8), wd, t[:1].expand((1 << 24) + 1))
+    with pytest.raises(ValueError, match="up to"):
+        linear_cross_entropy(xd[:, :1], wd[:1, :1].expand((1 << 30) + 1, 1), t)
     assert linear_cross_entropy(xd[:0], wd, t[:0], reduction="none").shape == (0,)
     assert torch.isnan(linear_cross_entropy(xd[:0], wd, t[:0]))
     loss = linear_cross_entropy(xd.requires_grad_(True), wd, t)

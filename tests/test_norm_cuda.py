@@ -203,6 +203,26 @@ def test_deterministic_streams_and_graphs():
     assert all(torch.equal(a[n], c[n]) for n in a)
 
 
+def test_two_streams_at_once():
+    """Workspaces and statistics of calls that run at the same time are their own."""
+    jobs = []
+    for i in range(3):
+        t, dh, du = norm_inputs(900 + i, 1024, BF16, True, True, True, seed=20 + i)
+        dh, du = dh.to(DEV), du.to(DEV)
+        want = {n: v.detach() for n, v in run(on_device(t), dh, du).items()}
+        jobs.append((t, dh, du, want, torch.cuda.Stream()))
+    ready = [on_device(t) for t, *_ in jobs]
+    torch.cuda.synchronize()
+    got = [[] for _ in jobs]
+    for _ in range(4):
+        for (_, dh, du, _, stream), d, g in zip(jobs, ready, got):
+            with torch.cuda.stream(stream):
+                g.append({n: v.detach() for n, v in run(d, dh, du).items()})
+    torch.cuda.synchronize()
+    for (_, _, _, want, _), g in zip(jobs, got):
+        assert all(torch.equal(want[n], one[n]) for one in g for n in want)
+
+
 def test_gpu_refusals_and_empty_rows():
     x, w = torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV)
     with pytest.raises(RuntimeError, match="alike"):
@@ -213,4 +233,7 @@ def test_gpu_refusals_and_empty_rows():
         residual_rms_norm(x, x, w.cpu())
     h, uu = residual_rms_norm(x[:0], x[:0], w)
     assert h.shape == (0, 8) and uu.shape == (0, 8)
+    with pytest.raises(ValueError, match="up to"):      # a view: refused before anything is copied
+        long = x[:1, :1].expand((1 << 30) + 1, 1)
+        residual_rms_norm(long, long, w[:1])
     assert _native.device_status() == _native.MMS_OK
