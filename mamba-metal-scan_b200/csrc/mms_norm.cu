@@ -3,8 +3,8 @@
 //     r1 = 1 / sqrt(mean(a^2) + eps),    r2 = 1 / sqrt(mean(h^2) + eps)
 // and with n = h r2, t = weight du, the gradients
 //     dh' = dh + r2 (t - n mean(t n))            dx = dh'
-//     dscale = sum over rows of dh' b,           db = scale dh'
-//     dpost = sum over rows of db a r1,          s = post db
+//     dscale = post sum over rows of dh' a r1,   db = scale dh'
+//     dpost = scale sum over rows of dh' a r1,   s = post db
 //     da = r1 (s - a r1 mean(s a r1))
 //     dy = da silu(gate),                        dgate = da y silu'(gate)
 //     dweight = sum over rows of du n
@@ -18,12 +18,15 @@
 // rows stay in its registers; the CTAs' partial sums meet in the workspace in
 // a fixed order. The backward's five reads a row come a row ahead, by
 // cp.async into shared memory where each thread finds its own pieces again (no
-// barrier), and its arithmetic is on packed pairs. Measured: 16384 x 4096 bf16
-// with all options forward 118 us (5.7 TB/s), backward 234 us (4.6 TB/s; it
-// issues 72 instructions a value and is bound by them; 307 us with loads at
-// the top of the row and scalar arithmetic); 8192 x 640 float32 sum and norm
-// 12 and 18 us, partly from L2. Rows too long for that (above 512 x 16 elements) are read
-// again for each sum.
+// barrier), and its arithmetic is on packed pairs. It is close to issue bound,
+// so nothing is computed twice: post and scale act as one product (in registers
+// for all rows), their gradients come from one sum over the rows, sum of dh' a r1,
+// and silu(gate) and its slope wait in shared memory for da. Measured:
+// 16384 x 4096 bf16 with all options forward 118 us (5.7 TB/s), backward 194 us
+// (5.5 TB/s; 233 us with both sums and the sigmoids twice, 307 us with loads at
+// the top of the row and scalar arithmetic too); 8192 x 640 float32 sum and norm
+// 12 and 18 us, partly from L2. Rows too long for that (above 512 x 16 elements)
+// are read again for each sum.
 #include <algorithm>
 
 #include "mms_common.cuh"
@@ -166,6 +169,11 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_fwd_kernel(const NormArgs a)
     }
 }
 
+// silu'(z) = sig (1 + z (1 - sig)) = sig + z sig - (z sig) sig
+__device__ __forceinline__ float2 silu_slope(float2 zs, float2 sig) {
+    return fma2(zs, fma2(sig, f2(-1.f, -1.f), f2(1.f, 1.f)), sig);
+}
+
 template <int P>
 __device__ __forceinline__ float (&flat(float2 (&v)[P]))[2 * P] {
     return reinterpret_cast<float (&)[2 * P]>(v);
@@ -176,12 +184,12 @@ enum { IN_DU, IN_X, IN_Y, IN_DH, IN_GATE };
 // Rows in shared memory, this one and the next, where ROW_THREADS leave room for
 // them (5 x 512 x 16 bytes a row and piece); 0: loads at the top of the row.
 template <typename T, int E, bool VEC>
-constexpr int fetch_rows() {
+__host__ __device__ constexpr int fetch_rows() {
     return !VEC || E * sizeof(T) > 32 ? 0 : 2;
 }
 
 template <typename T, int E, bool VEC, int F>
-constexpr int fetch_bytes(int threads) {
+__host__ __device__ constexpr int fetch_bytes(int threads) {
     return fetch_rows<T, E, VEC>() * (F & GATE ? 5 : 4) * threads * E * (int)sizeof(T);
 }
 
@@ -234,8 +242,21 @@ struct RowReader {
     }
 };
 
-// Sums over this CTA's rows go to part[(which * gridDim + block) * dim + column],
-// which = 0 dweight, 1 dscale, 2 dpost.
+// With a gate and rows in shared memory: silu(gate) and y silu'(gate) of a row stay there from the
+// pass that computes a to the one that uses them (each thread its own).
+template <typename T, int E, bool VEC, int F>
+__host__ __device__ constexpr bool keeps_gate() {
+    return F & GATE && fetch_rows<T, E, VEC>() > 0;
+}
+
+template <typename T, int E, bool VEC, int F>
+constexpr int bwd_smem(int threads) {
+    return fetch_bytes<T, E, VEC, F>(threads) + (keeps_gate<T, E, VEC, F>() ? threads * E * 8 : 0);
+}
+
+// Sums over this CTA's rows go to part[(which * gridDim + block) * dim + column]: which = 0 those of
+// du n; 1 those of dh' v (v = a r1, or a without post), whose products with post and scale are dscale
+// and dpost.
 template <typename T, int E, bool VEC, int F>
 __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
 {
@@ -245,14 +266,27 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
     BlockSum sum{sh, 0};
     const float inv = 1.f / a.dim;
     constexpr int P = E / 2;                                 // packed pairs: half the instructions
-    float2 sw[P], ss[P], sp[P];
+    constexpr bool KEEP = keeps_gate<T, E, VEC, F>();
+    float2 sw[P], sv[P], ps[P];                              // ps = post scale
 #pragma unroll
-    for (int i = 0; i < P; ++i) sw[i] = ss[i] = sp[i] = f2(0.f, 0.f);
+    for (int i = 0; i < P; ++i) {
+        sw[i] = sv[i] = f2(0.f, 0.f);
+        ps[i] = f2(1.f, 1.f);
+    }
+    if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, flat(ps));
+    if (F & SCALE) {
+        float2 w[P];
+        C::load(static_cast<const T *>(a.scale), a.dim, flat(w));
+#pragma unroll
+        for (int i = 0; i < P; ++i) ps[i] = F & POST ? mul2(ps[i], w[i]) : w[i];
+    }
     RowReader<T, E, VEC, F> in{a, rows_smem, 0, 0};
+    float4 *kept = KEEP ? reinterpret_cast<float4 *>(rows_smem) +
+                              (size_t)fetch_bytes<T, E, VEC, F>(blockDim.x) / 16 + threadIdx.x : nullptr;
     for (in.begin(blockIdx.x); in.r < (size_t)a.rows; in.next()) {
         in.ready();
         const size_t o = in.r * a.dim;
-        float2 h[P], t[P], v[P], w[P], d[P];
+        float2 h[P], t[P], v[P], d[P];
         const float r1 = F & POST ? a.c_stat[2 * in.r] : 1.f, r2 = a.c_stat[2 * in.r + 1];
         const float2 r1p = f2(r1, r1), r2p = f2(r2, r2);
         // v = a r1 (the normed a, or a itself), h = n
@@ -260,25 +294,28 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
         if (F & GATE) {
             in.get(IN_GATE, flat(d));
 #pragma unroll
-            for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(d[i], f2(sigmoid_fast(d[i].x), sigmoid_fast(d[i].y))));
+            for (int i = 0; i < P; ++i) {
+                const float2 sig = f2(sigmoid_fast(d[i].x), sigmoid_fast(d[i].y)), zs = mul2(d[i], sig);
+                if (KEEP) {
+                    const float2 g = mul2(v[i], silu_slope(zs, sig));
+                    kept[i * blockDim.x] = make_float4(zs.x, zs.y, g.x, g.y);
+                }
+                v[i] = mul2(v[i], zs);
+            }
         }
         in.get(IN_X, flat(h));
-        if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, flat(w));
-        if (F & SCALE) C::load(static_cast<const T *>(a.scale), a.dim, flat(d));
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             if (F & POST) v[i] = mul2(v[i], r1p);
-            float2 b = v[i];
-            if (F & POST) b = mul2(b, w[i]);
-            h[i] = mul2(F & SCALE ? fma2(b, d[i], h[i]) : add2(h[i], b), r2p);
+            h[i] = mul2(F & (POST | SCALE) ? fma2(v[i], ps[i], h[i]) : add2(h[i], v[i]), r2p);
         }
         in.get(IN_DU, flat(t));
         float2 s = f2(0.f, 0.f);
-        C::load(static_cast<const T *>(a.weight), a.dim, flat(w));
+        C::load(static_cast<const T *>(a.weight), a.dim, flat(d));
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             sw[i] = fma2(t[i], h[i], sw[i]);
-            t[i] = mul2(t[i], w[i]);
+            t[i] = mul2(t[i], d[i]);
             s = fma2(t[i], h[i], s);
         }
         const float mean = sum(s.x + s.y) * inv;
@@ -288,44 +325,42 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
         for (int i = 0; i < P; ++i) d[i] = fma2(r2p, fma2(h[i], meanp, t[i]), d[i]);        // dh'
         C::store(static_cast<T *>(a.dx) + o, a.dim, flat(d));
         if (F == 0) continue;                                // dy has dx's values
-        if (F & POST) C::load(static_cast<const T *>(a.post), a.dim, flat(w));
-        if (F & SCALE) C::load(static_cast<const T *>(a.scale), a.dim, flat(h));
         s = f2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            t[i] = d[i];
-            if (F & SCALE) {
-                ss[i] = fma2(d[i], F & POST ? mul2(v[i], w[i]) : v[i], ss[i]);
-                t[i] = mul2(t[i], h[i]);                     // db
+            if (F & (POST | SCALE)) {
+                sv[i] = fma2(d[i], v[i], sv[i]);
+                d[i] = mul2(d[i], ps[i]);
             }
-            if (F & POST) {
-                sp[i] = fma2(t[i], v[i], sp[i]);
-                t[i] = mul2(t[i], w[i]);
-                s = fma2(t[i], v[i], s);
-            }
+            if (F & POST) s = fma2(d[i], v[i], s);
         }
         if (F & POST) {
             const float mean1 = sum(s.x + s.y) * inv;
             const float2 mean1p = f2(-mean1, -mean1);
 #pragma unroll
-            for (int i = 0; i < P; ++i) t[i] = mul2(r1p, fma2(v[i], mean1p, t[i]));
+            for (int i = 0; i < P; ++i) d[i] = mul2(r1p, fma2(v[i], mean1p, d[i]));
         }
         if (F & GATE) {
-            in.get(IN_GATE, flat(w));
-            in.get(IN_Y, flat(v));
-            const float2 one = f2(1.f, 1.f);
+            if (KEEP) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const float2 sig = f2(sigmoid_fast(w[i].x), sigmoid_fast(w[i].y));
-                const float2 zs = mul2(w[i], sig);
-                // silu' = sig (1 + z (1 - sig)) = sig + z sig - (z sig) sig
-                const float2 slope = fma2(zs, fma2(sig, f2(-1.f, -1.f), one), sig);
-                d[i] = mul2(mul2(t[i], v[i]), slope);
-                t[i] = mul2(t[i], zs);
+                for (int i = 0; i < P; ++i) {
+                    const float4 k = kept[i * blockDim.x];
+                    t[i] = mul2(d[i], f2(k.z, k.w));
+                    d[i] = mul2(d[i], f2(k.x, k.y));
+                }
+            } else {
+                in.get(IN_GATE, flat(h));
+                in.get(IN_Y, flat(v));
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float2 sig = f2(sigmoid_fast(h[i].x), sigmoid_fast(h[i].y)), zs = mul2(h[i], sig);
+                    t[i] = mul2(d[i], mul2(v[i], silu_slope(zs, sig)));
+                    d[i] = mul2(d[i], zs);
+                }
             }
-            C::store(static_cast<T *>(a.dgate) + o, a.dim, flat(d));
+            C::store(static_cast<T *>(a.dgate) + o, a.dim, flat(t));
         }
-        C::store(static_cast<T *>(a.dy) + o, a.dim, flat(t));
+        C::store(static_cast<T *>(a.dy) + o, a.dim, flat(d));
     }
     const size_t plane = (size_t)gridDim.x * a.dim;
     float *part = static_cast<float *>(a.workspace) + (size_t)blockIdx.x * a.dim;
@@ -334,8 +369,7 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
         const int c = C::at(i / C::VW) + i % C::VW;
         if (c >= a.dim) continue;
         part[c] = flat(sw)[i];
-        if (F & SCALE) part[plane + c] = flat(ss)[i];
-        if (F & POST) part[2 * plane + c] = flat(sp)[i];
+        if (F & (POST | SCALE)) part[plane + c] = flat(sv)[i];
     }
 }
 
@@ -409,11 +443,11 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a)
     const float inv = 1.f / a.dim;
     const size_t plane = (size_t)gridDim.x * a.dim;
     float *pw = static_cast<float *>(a.workspace) + (size_t)blockIdx.x * a.dim;
-    float *ps = pw + plane, *pp = ps + plane;
+    float *pv = pw + plane;
+    const bool any = a.post || a.scale;
     for (int i = threadIdx.x; i < a.dim; i += blockDim.x) {
         pw[i] = 0.f;
-        if (a.scale) ps[i] = 0.f;
-        if (a.post) pp[i] = 0.f;
+        if (any) pv[i] = 0.f;
     }
     for (size_t r = blockIdx.x; r < (size_t)a.rows; r += gridDim.x) {
         const Row<T> row = row_of<T>(a, r);
@@ -436,16 +470,13 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a)
         }
         for (int i = threadIdx.x; i < a.dim; i += blockDim.x) {
             const size_t o = r * a.dim + i;
-            const float av = row.a_at(i), b = row.b_at(i, r1), h = row.h_at(i, r1);
+            const float av = row.a_at(i), h = row.h_at(i, r1);
             const float d = dh_at(i, h);
             pw[i] += to_f(du[i]) * h * r2;
             float v = d;
-            if (a.scale) {
-                ps[i] += d * b;
-                v *= to_f(row.scale[i]);
-            }
+            if (any) pv[i] += d * (a.post ? av * r1 : av);
+            if (a.scale) v *= to_f(row.scale[i]);
             if (a.post) {
-                pp[i] += v * av * r1;
                 v = r1 * (v * to_f(row.post[i]) - av * r1 * mean1);
             }
             if (a.gate) {
@@ -465,8 +496,6 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormArgs a, int
 {
     __shared__ float sh[32][33];
     const int which = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x;
-    T *out = static_cast<T *>(which == 0 ? a.dweight : which == 1 ? a.dscale : a.dpost);
-    if (!out) return;
     const float *p = static_cast<const float *>(a.workspace) + (size_t)which * blocks * a.dim;
     float s = 0.f;
     if (col < a.dim)
@@ -478,7 +507,11 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormArgs a, int
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     const int c = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && c < a.dim) out[c] = from_f<T>(s);
+    if (threadIdx.x || c >= a.dim) return;
+    const T *post = static_cast<const T *>(a.post), *scale = static_cast<const T *>(a.scale);
+    if (which == 0) static_cast<T *>(a.dweight)[c] = from_f<T>(s);
+    if (which == 1 && scale) static_cast<T *>(a.dscale)[c] = from_f<T>(post ? s * to_f(post[c]) : s);
+    if (which == 1 && post) static_cast<T *>(a.dpost)[c] = from_f<T>(scale ? s * to_f(scale[c]) : s);
 }
 
 bool rows_aligned(const NormArgs &a)
@@ -521,8 +554,8 @@ template <typename T, int E, bool VEC, int F>
 cudaError_t run(const NormArgs &a, int threads, bool backward, int *blocks, cudaStream_t stream)
 {
     if (backward) {
-        const int smem = fetch_bytes<T, E, VEC, F>(threads);
-        const cudaError_t e = smem_opt_in<norm_bwd_kernel<T, E, VEC, F>>(fetch_bytes<T, E, VEC, F>(ROW_THREADS));
+        const int smem = bwd_smem<T, E, VEC, F>(threads);
+        const cudaError_t e = smem_opt_in<norm_bwd_kernel<T, E, VEC, F>>(bwd_smem<T, E, VEC, F>(ROW_THREADS));
         if (e != cudaSuccess) return e;
         *blocks = std::min({a.rows, resident<norm_bwd_kernel<T, E, VEC, F>>(threads, smem), MAX_ROW_BLOCKS});
         norm_bwd_kernel<T, E, VEC, F><<<*blocks, threads, smem, stream>>>(a);
@@ -574,7 +607,7 @@ cudaError_t run_type(const NormArgs &a, bool backward, int *blocks, cudaStream_t
 
 size_t norm_workspace_bytes(int rows, int dim)
 {
-    return (size_t)3 * std::min(rows, MAX_ROW_BLOCKS) * dim * sizeof(float);
+    return (size_t)2 * std::min(rows, MAX_ROW_BLOCKS) * dim * sizeof(float);
 }
 
 cudaError_t launch_norm_fwd(const NormArgs &a, cudaStream_t stream)
@@ -589,7 +622,7 @@ cudaError_t launch_norm_bwd(const NormArgs &a, cudaStream_t stream)
     const cudaError_t e = a.bf16 ? run_type<__nv_bfloat16>(a, true, &blocks, stream)
                                  : run_type<float>(a, true, &blocks, stream);
     if (e != cudaSuccess) return e;
-    const dim3 grid((a.dim + 31) / 32, a.post || a.scale ? 3 : 1);
+    const dim3 grid((a.dim + 31) / 32, a.post || a.scale ? 2 : 1);
     if (a.bf16) norm_reduce_kernel<__nv_bfloat16><<<grid, dim3(32, 32), 0, stream>>>(a, blocks);
     else norm_reduce_kernel<float><<<grid, dim3(32, 32), 0, stream>>>(a, blocks);
     return cudaGetLastError();
