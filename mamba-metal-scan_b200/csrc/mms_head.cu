@@ -496,11 +496,12 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
 struct Part {
     float x;
     double y;
+    // the same with the larger maximum m
+    __device__ __forceinline__ Part at(float m) const { return Part{m, y * ex2(x - (m == -INFINITY ? 0.f : m))}; }
 };
 __device__ __forceinline__ Part join(Part a, Part b) {
     const float m = fmaxf(a.x, b.x);
-    if (m == -INFINITY) return Part{m, a.y + b.y};
-    return Part{m, a.y * ex2(a.x - m) + b.y * ex2(b.x - m)};
+    return Part{m, a.at(m).y + b.at(m).y};
 }
 
 // Up to few_rows() rows: a warp takes 4 rows of w at a time, its lanes 8 columns
@@ -702,14 +703,15 @@ order_kernel(const int64_t *__restrict__ index, int k, int rows, RowMap rm, int 
     }
 }
 
-// before[b * rows + m]: entries of row m below column LIST_BLOCK * b. A thread
-// a row (32 a CTA, so that the stores are whole sectors) and 1/8 of the blocks.
+// before[b * rows + m]: entries of row m below column LIST_BLOCK * b. A thread a row
+// (32 a CTA, so that the stores are whole sectors) and its CTA's blocks' eighth.
 __global__ void __launch_bounds__(256)
 before_kernel(const int *__restrict__ col, int k, int rows, RowMap rm, int blocks, uint16_t *__restrict__ before)
 {
     const int m = blockIdx.x * 32 + threadIdx.x % 32;
     if (m >= rm.n(rows)) return;
-    const int each = (blocks + 7) / 8, b0 = threadIdx.x / 32 * each, b1 = min(blocks, b0 + each);
+    const int each = (blocks + 8 * gridDim.y - 1) / (8 * gridDim.y);
+    const int b0 = min(blocks, (int)(blockIdx.y * 8 + threadIdx.x / 32) * each), b1 = min(blocks, b0 + each);
     const int *c = col + (size_t)m * k;
     int lo = 0, hi = k;                                     // the first entry not below b0's column
     while (lo < hi) {
@@ -723,6 +725,8 @@ before_kernel(const int *__restrict__ col, int k, int rows, RowMap rm, int block
         before[(size_t)b * rows + m] = (uint16_t)lo;
     }
 }
+
+constexpr int AT_ONCE = 8;
 
 // One row a lane, 32 threads a row over the tiles. Parts 1..ntiles, and part
 // 0 (the pieces before) unless `first`. Writes part 0, or in the last piece
@@ -739,18 +743,35 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm,
     const int m = blockIdx.x * 32 + threadIdx.x, live = rm.n(rows);
     Part v{-INFINITY, 0.};
     if (m < live)
-#pragma unroll 4
-        for (int t = threadIdx.y + (first ? 1 : 0); t <= ntiles; t += 32) {
-            const float2 p = part[(size_t)t * rows + m];
-            v = join(v, Part{p.x, p.y});
+        for (int t0 = threadIdx.y + (first ? 1 : 0); t0 <= ntiles; t0 += 32 * AT_ONCE) {
+            // all loads, then the maximum, then independent terms: no chain of joins
+            float2 p[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i)
+                p[i] = t0 + 32 * i <= ntiles ? part[(size_t)(t0 + 32 * i) * rows + m] : make_float2(-INFINITY, 0.f);
+            float top = v.x;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, p[i].x);
+            v = v.at(top);
+            // a float32 sum and what it lost: converting each term to double bounds the kernel (888 parts of
+            // 16 rows 11.1 us, this way 7.7)
+            const float ref = top == -INFINITY ? 0.f : top;
+            float s = 0.f, lost = 0.f;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float y = __fmul_rn(p[i].y, ex2(p[i].x - ref)), n = s + y, d = n - s;
+                lost += (s - (n - d)) + (y - d);
+                s = n;
+            }
+            v.y += (double)s + lost;
         }
     sh[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
     // transposed: a warp joins the 32 values of one row
     v = sh[threadIdx.x][threadIdx.y];
+    v = v.at(warp_max(v.x));
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-        v = join(v, Part{__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)});
+    for (int o = 16; o; o >>= 1) v.y += __shfl_xor_sync(~0u, v.y, o);
     const int r = blockIdx.x * 32 + threadIdx.y;
     if (threadIdx.x == 0 && r < live) {
         if (!last) {
@@ -824,8 +845,12 @@ kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, i
 __device__ __forceinline__ bool row_counts(const int64_t *index, const float *prob, int k,
                                            int64_t ignore, size_t m) {
     if (!prob) return index[m] != ignore;
-    for (int j = 0; j < k; ++j)
-        if (!(prob[m * k + j] == 0.f)) return true;     // NaN counts
+    for (int j0 = 0; j0 < k; j0 += 8) {                 // 8 loads at once
+        bool some = false;
+#pragma unroll
+        for (int j = j0; j < j0 + 8; ++j) some |= j < k && !(prob[m * k + j] == 0.f);   // NaN counts
+        if (some) return true;
+    }
     return false;
 }
 
@@ -1063,8 +1088,10 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         uint16_t *pos = u16(a.workspace, l.pos), *before = u16(a.workspace, l.before);
         order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, rm, a.vocab,
                                                                                 col, pos, o.logq2, rest);
-        before_kernel<<<ceil_div(a.rows, 32), 256, 0, stream>>>(col, a.k, a.rows, rm, (a.vocab - 1) / LIST_BLOCK + 1,
-                                                               before);
+        // few rows: more CTAs a row, down to 4 blocks a thread
+        const int blocks = (a.vocab - 1) / LIST_BLOCK + 1, ctas = ceil_div(a.rows, 32);
+        const dim3 grid(ctas, std::max(1, std::min(2 * 148 / ctas, blocks / 32)));
+        before_kernel<<<grid, 256, 0, stream>>>(col, a.k, a.rows, rm, blocks, before);
         lists = Lists{col, pos, before, a.k, a.rows};
     }
     if (l.few) {
