@@ -27,10 +27,11 @@
 //            by lse_kernel. The logits at the indices are the product's own
 //            values, so that its errors cancel against lse2's; the
 //            distillation's lists are sorted for that (order_kernel,
-//            before_kernel). Then a loss kernel; one block adds the rows up. Up to few_rows() rows (few_kernel) w is read once, as it
-//            is, by the CUDA cores: nothing is staged. The backward then takes
-//            dz from the same sums (few_grad_kernel), and so do pick_kernel's
-//            dot products for the distillation.
+//            before_kernel). Then a loss kernel; one block adds the rows up.
+//            Up to few_rows() rows (few_kernel) w is read once, as it is, by
+//            the CUDA cores: nothing is staged. The backward then takes dz from
+//            the same sums (few_grad_kernel), and the distillation's logits
+//            come from dot products in the same order (pick_kernel).
 // Backward:  x staged, and r with it, left-out rows as zeros (so that nothing
 //            in them, NaN included, reaches dw); per piece: product
 //            MM_GRAD, sparse_kernel sets dz at the indices (from logq2, in
