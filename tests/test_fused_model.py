@@ -81,3 +81,38 @@ def test_distillation_through_the_model(device):
 def test_a_model_without_blocks():
     _, fused, idx = models("cpu", n_layers=0)
     assert fused(idx, idx)[1].ndim == 0
+
+
+@pytest.mark.gpu
+def test_a_captured_training_step():
+    """Both losses' steps in one graph, replayed on other tokens: the eager step's values."""
+    _, fused, idx = models("cuda")
+    g = torch.Generator().manual_seed(7)
+    index = torch.randint(-1, VOCAB, (3, 40, 6), generator=g).cuda()
+    logits = torch.randn(3, 40, 6, generator=g).cuda()
+    other = torch.randint(0, VOCAB, (3, 41), generator=g).cuda()
+    tokens = idx.clone()
+    tokens_in, targets = tokens[:, :-1], tokens[:, 1:]
+
+    def step():
+        loss = fused(tokens_in, targets)[1] + fused.distill_loss(tokens_in, index, logits, 2.0)
+        return loss.detach(), grads_of(fused, loss)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        tokens.copy_(other)
+        want, want_grads = step()
+        tokens.copy_(idx)
+    torch.cuda.current_stream().wait_stream(side)
+    fused.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = step()
+    tokens.copy_(other)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert abs(loss.item() - want.item()) <= 1e-5 * want.item()
+    same_grads(grads, want_grads)
