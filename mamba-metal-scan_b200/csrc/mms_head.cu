@@ -64,6 +64,7 @@
 
 #include "mms_common.cuh"
 #include "mms_head.h"
+#include "mms_kernels.h"
 #include "mms_scan.h"
 
 namespace mms {
@@ -336,6 +337,7 @@ __device__ __forceinline__ float row_factor(const RowFactors &f, RowMap rm, int 
 template <typename T, int KIND, int LP>
 __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
 {
+    chained();
     const int lane = threadIdx.x % LP;
     float top = 0.f;
     Pow2 whole{1.f, 1.f};
@@ -417,6 +419,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
 __global__ void __launch_bounds__(256)
 top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, float *top)
 {
+    chained();
     float m = 0.f;
     for (long long r = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * 2; r < rows; r += gridDim.x * 16) {
         const float *p = src + (size_t)r * lds, *q = r + 1 < rows ? p + lds : p;
@@ -441,9 +444,9 @@ template <typename T, int KIND>
 void stage(const StageArgs &a, cudaStream_t s)
 {
     const int grid = stage_grid(a.rows, a.cols);
-    if (a.cols <= 64) stage_kernel<T, KIND, 8><<<grid, 256, 0, s>>>(a);
-    else if (a.cols <= 128) stage_kernel<T, KIND, 16><<<grid, 256, 0, s>>>(a);
-    else stage_kernel<T, KIND, 32><<<grid, 256, 0, s>>>(a);
+    if (a.cols <= 64) launch_chained(stage_kernel<T, KIND, 8>, grid, 256, 0, s, a);
+    else if (a.cols <= 128) launch_chained(stage_kernel<T, KIND, 16>, grid, 256, 0, s, a);
+    else launch_chained(stage_kernel<T, KIND, 32>, grid, 256, 0, s, a);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -465,6 +468,7 @@ pick_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, lon
             const int64_t *__restrict__ index, int k, float c, float *__restrict__ logq2,
             float *__restrict__ rest, long long n, int vocab, int dim)
 {
+    chained();
     const long long e = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (e >= n) return;
@@ -563,6 +567,7 @@ struct FewArgs {
 template <typename T, int R, bool VEC>
 __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 {
+    chained();
     __shared__ Part sh[8][R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const float c = a.c;
@@ -611,6 +616,7 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
 template <typename T, int R, bool VEC>
 __global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
 {
+    chained();
     const int lane = threadIdx.x % 32, row = lane / 4, i = lane % 4;
     const bool in = row < a.rows;
     const float2 l = in ? a.lse2[row] : make_float2(0.f, 0.f);
@@ -644,8 +650,8 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const FewArgs a)
 template <typename T, int R, bool VEC>
 void launch_few_rows(const FewArgs &a, int blocks, bool backward, cudaStream_t s)
 {
-    if (backward) few_grad_kernel<T, R, VEC><<<blocks, 256, 0, s>>>(a);
-    else few_kernel<T, R, VEC><<<blocks, 256, 0, s>>>(a);
+    if (backward) launch_chained(few_grad_kernel<T, R, VEC>, blocks, 256, 0, s, a);
+    else launch_chained(few_kernel<T, R, VEC>, blocks, 256, 0, s, a);
 }
 
 template <typename T, bool VEC>
@@ -679,6 +685,7 @@ __global__ void __launch_bounds__(256)
 order_kernel(const int64_t *__restrict__ index, int k, int rows, RowMap rm, int vocab, int *__restrict__ col,
              uint16_t *__restrict__ pos, float *__restrict__ logq2, float *__restrict__ rest)
 {
+    chained();
     extern __shared__ int sh_index[];
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (m >= rm.n(rows)) return;
@@ -707,8 +714,9 @@ order_kernel(const int64_t *__restrict__ index, int k, int rows, RowMap rm, int 
 // before[b * rows + m]: entries of row m below column LIST_BLOCK * b. A thread a row
 // (32 a CTA, so that the stores are whole sectors) and its CTA's blocks' eighth.
 __global__ void __launch_bounds__(256)
-before_kernel(const int *__restrict__ col, int k, int rows, RowMap rm, int blocks, uint16_t *__restrict__ before)
+before_kernel(const int *col, int k, int rows, RowMap rm, int blocks, uint16_t *__restrict__ before)
 {
+    chained();
     const int m = blockIdx.x * 32 + threadIdx.x % 32;
     if (m >= rm.n(rows)) return;
     const int each = (blocks + 8 * gridDim.y - 1) / (8 * gridDim.y);
@@ -736,9 +744,10 @@ constexpr int AT_ONCE = 8;
 __global__ void __launch_bounds__(1024)
 lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm, float2 *__restrict__ lse2,
            const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
-           const float *__restrict__ rest, float *__restrict__ loss, int reduction,
+           const float *rest, float *__restrict__ loss, int reduction,
            float *__restrict__ total, float *__restrict__ count)
 {
+    chained();
     __shared__ Part sh[32][33];
     __shared__ float row_loss[32];
     const int m = blockIdx.x * 32 + threadIdx.x, live = rm.n(rows);
@@ -804,10 +813,11 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm,
 // entries, kept as prob, against the student's log-probabilities.
 __global__ void __launch_bounds__(256)
 kd_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, float tau,
-          const float2 *__restrict__ lse2, float *__restrict__ logq2,
-          const float *__restrict__ rest, float *__restrict__ prob, float *__restrict__ loss, int rows, RowMap rm,
+          const float2 *lse2, float *__restrict__ logq2,
+          const float *rest, float *__restrict__ prob, float *__restrict__ loss, int rows, RowMap rm,
           int reduction)
 {
+    chained();
     const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (m >= rm.n(rows)) return;
     const size_t o = (size_t)m * k;
@@ -857,10 +867,11 @@ __device__ __forceinline__ bool row_counts(const int64_t *index, const float *pr
 
 // count, and loss = the rows' sum (over count for a mean), in a fixed order.
 __global__ void __launch_bounds__(1024)
-total_kernel(const float *__restrict__ rowloss, const int64_t *__restrict__ index,
-             const float *__restrict__ prob, int k, int64_t ignore, int rows, RowMap rm, int reduction,
+total_kernel(const float *rowloss, const int64_t *__restrict__ index,
+             const float *prob, int k, int64_t ignore, int rows, RowMap rm, int reduction,
              float *__restrict__ loss, float *__restrict__ count)
 {
+    chained();
     __shared__ float sh[2][32];
     float s = 0.f, n = 0.f;
     const int live = rm.n(rows);
@@ -889,6 +900,7 @@ __global__ void __launch_bounds__(256)
 flags_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits, int k, int rows,
              uint8_t *__restrict__ flags)
 {
+    chained();
     const int m = blockIdx.x * 8 + threadIdx.x / 32;
     if (m >= rows) return;
     bool some = false;
@@ -900,9 +912,10 @@ flags_kernel(const int64_t *__restrict__ index, const float *__restrict__ logits
 
 // The rows that count, in order, and their number: one CTA, 1024 rows at a time.
 __global__ void __launch_bounds__(1024)
-map_kernel(const int64_t *__restrict__ target, int64_t ignore, const uint8_t *__restrict__ flags, int rows,
+map_kernel(const int64_t *__restrict__ target, int64_t ignore, const uint8_t *flags, int rows,
            int *__restrict__ map, int *__restrict__ live)
 {
+    chained();
     __shared__ int sh[32];
     int base = 0;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -930,10 +943,11 @@ map_kernel(const int64_t *__restrict__ target, int64_t ignore, const uint8_t *__
 // dz at the sparse entries that lie in this piece of the vocabulary; `unit` in
 // place of r if it is not 0.
 __global__ void __launch_bounds__(256)
-sparse_kernel(const int64_t *__restrict__ index, const float *__restrict__ prob,
-              const float *__restrict__ logq2, const float *__restrict__ rs, float unit, int k, int rows, RowMap rm, int v0, int v1,
+sparse_kernel(const int64_t *__restrict__ index, const float *prob,
+              const float *logq2, const float *rs, float unit, int k, int rows, RowMap rm, int v0, int v1,
               uint16_t *__restrict__ g, long long ldg, long long gplane, int planes, bool fp16)
 {
+    chained();
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x, m = e / k;
     if (m >= rm.n(rows)) return;
     const int64_t *list = index + (size_t)rm.row((int)m) * k;
@@ -998,7 +1012,7 @@ float *w_top(const HeadArgs &a, const Layout &l)
 }
 void top_of_w(const HeadArgs &a, float *top, cudaStream_t s)
 {
-    top_kernel<<<std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s>>>(static_cast<const float *>(a.w), a.ldw,
+    launch_chained(top_kernel, std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s, static_cast<const float *>(a.w), a.ldw,
                                                                        a.vocab, a.dim, top);
 }
 
@@ -1056,6 +1070,7 @@ size_t head_workspace_bytes(int rows, int vocab, int dim, int k, bool bf16, long
 
 cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
 {
+    chain_begin();
     const FwdLayout l = fwd_layout(a.rows, a.vocab, a.dim, a.kd ? a.k : 0, a.bf16, a.ldx, a.ldw);
     const Kept o = kept_of(a);
     const RowMap rm{o.map, o.live};
@@ -1068,8 +1083,8 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     cudaError_t e;
     if (rm.live) {
         uint8_t *flags = a.kd ? static_cast<uint8_t *>(a.workspace) + l.flags : nullptr;
-        if (a.kd) flags_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.rows, flags);
-        map_kernel<<<1, 1024, 0, stream>>>(a.index, a.ignore_index, flags, a.rows, o.map, o.live);
+        if (a.kd) launch_chained(flags_kernel, ceil_div(a.rows, 8), 256, 0, stream, a.index, a.logits, a.k, a.rows, flags);
+        launch_chained(map_kernel, 1, 1024, 0, stream, a.index, a.ignore_index, flags, a.rows, o.map, o.live);
         // the rows that are left out
         if (none && (e = cudaMemsetAsync(a.loss, 0, (size_t)a.rows * sizeof(float), stream)) != cudaSuccess) return e;
     }
@@ -1077,22 +1092,22 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
     if (a.kd && l.few) {
         const int n = a.rows * a.k;
         if (a.bf16)
-            pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
+            launch_chained(pick_kernel<__nv_bfloat16>, ceil_div(n, 8), 256, 0, stream,
                 static_cast<const __nv_bfloat16 *>(a.x), a.ldx, static_cast<const __nv_bfloat16 *>(a.w), a.ldw,
                 a.index, a.k, c, o.logq2, rest, n, a.vocab, a.dim);
         else
-            pick_kernel<<<ceil_div(n, 8), 256, 0, stream>>>(
+            launch_chained(pick_kernel<float>, ceil_div(n, 8), 256, 0, stream,
                 static_cast<const float *>(a.x), a.ldx, static_cast<const float *>(a.w), a.ldw, a.index, a.k, c,
                 o.logq2, rest, n, a.vocab, a.dim);
     } else if (a.kd) {
         int *col = reinterpret_cast<int *>(fl(a.workspace, l.col));
         uint16_t *pos = u16(a.workspace, l.pos), *before = u16(a.workspace, l.before);
-        order_kernel<<<ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream>>>(a.index, a.k, a.rows, rm, a.vocab,
+        launch_chained(order_kernel, ceil_div(a.rows, 8), 256, 8 * a.k * sizeof(int), stream, a.index, a.k, a.rows, rm, a.vocab,
                                                                                 col, pos, o.logq2, rest);
         // few rows: more CTAs a row, down to 4 blocks a thread
         const int blocks = (a.vocab - 1) / LIST_BLOCK + 1, ctas = ceil_div(a.rows, 32);
         const dim3 grid(ctas, std::max(1, std::min(2 * 148 / ctas, blocks / 32)));
-        before_kernel<<<grid, 256, 0, stream>>>(col, a.k, a.rows, rm, blocks, before);
+        launch_chained(before_kernel, grid, 256, 0, stream, col, a.k, a.rows, rm, blocks, before);
         lists = Lists{col, pos, before, a.k, a.rows};
     }
     if (l.few) {
@@ -1101,7 +1116,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         f.target = target; f.at = o.logq2; f.rest = rest; f.part = part + a.rows;
         if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, false, stream);
         else launch_few<float>(f, blocks, false, stream);
-        lse_kernel<<<1, dim3(32, 32), 0, stream>>>(part, blocks, true, true, a.rows, rm, o.lse2, target,
+        launch_chained(lse_kernel, 1, dim3(32, 32), 0, stream, part, blocks, true, true, a.rows, rm, o.lse2, target,
                                                   a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction,
                                                   total, o.count);
     }
@@ -1127,21 +1142,22 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.at = o.logq2;
         mm.rest = rest;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
-        lse_kernel<<<ceil_div(a.rows, 32), dim3(32, 32), 0, stream>>>(
+        launch_chained(lse_kernel, ceil_div(a.rows, 32), dim3(32, 32), 0, stream,
             part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows, rm,
             o.lse2, target, a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction, total, o.count);
     }
     if (a.kd)
-        kd_kernel<<<ceil_div(a.rows, 8), 256, 0, stream>>>(a.index, a.logits, a.k, a.tau, o.lse2, o.logq2, rest,
+        launch_chained(kd_kernel, ceil_div(a.rows, 8), 256, 0, stream, a.index, a.logits, a.k, a.tau, o.lse2, o.logq2, rest,
                                                           o.prob, rowloss, a.rows, rm, a.reduction);
     if (!total)
-        total_kernel<<<1, 1024, 0, stream>>>(rowloss, a.index, o.prob, a.k, a.ignore_index, a.rows, rm, a.reduction,
+        launch_chained(total_kernel, 1, 1024, 0, stream, rowloss, a.index, o.prob, a.k, a.ignore_index, a.rows, rm, a.reduction,
                                              a.loss, o.count);
     return cudaGetLastError();
 }
 
 cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
 {
+    chain_begin();
     const BwdLayout l = bwd_layout(a.rows, a.vocab, a.dim, a.bf16, a.ldw);
     const Kept o = kept_of(a);
     const RowMap rm{o.map, o.live};
@@ -1201,7 +1217,7 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         } else if ((e = launch_mm(MM_GRAD, mm, stream)) != cudaSuccess) {
             return e;
         }
-        sparse_kernel<<<ceil_div(n, 256), 256, 0, stream>>>(a.index, o.prob, o.logq2, rs, unit, a.k, a.rows, rm, v0,
+        launch_chained(sparse_kernel, ceil_div(n, 256), 256, 0, stream, a.index, o.prob, o.logq2, rs, unit, a.k, a.rows, rm, v0,
                                                             v0 + nv, g, l.ldg, gplane, l.gplanes, f32);
         MmArgs out{};
         out.fp16 = f32;

@@ -473,6 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const MmArgs a, const Tiles planned, uint32_t limit, int skip)
 {
+    chain_next();
     constexpr int STAGES = BOTH ? 3 : 6, PLANES = BOTH ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * STAGES + 5];
@@ -502,6 +503,8 @@ mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     __syncthreads();
     cluster_sync();
     umma_fence_after();
+    chain_wait();
+    asm volatile("fence.proxy.async.global;\n" ::: "memory");      // the copies read what kernels before have stored
     const uint32_t tmem = tmem_slot;
     const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     const int passes = BOTH ? 1 : a.a.planes + a.b.planes - 1;      // over the stages
@@ -724,7 +727,7 @@ cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
     const cudaError_t e = smem_opt_in<kernel>(SMEM);
     if (e != cudaSuccess) return e;
     const int pairs = a.live && !AT ? N_SM / 2 : std::min(N_SM / 2, q.items);
-    kernel<<<2 * pairs, THREADS, SMEM, stream>>>(ma, mb, a, q, tma_wait_limit(), tma_skip_item());
+    launch_chained(kernel, 2 * pairs, THREADS, SMEM, stream, ma, mb, a, q, tma_wait_limit(), tma_skip_item());
     return cudaGetLastError();
 }
 
@@ -743,6 +746,7 @@ cudaError_t launch_as(const MmArgs &a, const Tiles &q, bool parts, bool both, cu
 template <typename T, bool AT>
 __global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Tiles planned)
 {
+    chained();
     int mi, ni;
     const Live live = live_of<AT>(a, planned);
     const Tiles q = live_plan<MM_OUT, AT>(a, planned, live);
@@ -755,7 +759,7 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const MmArgs a, const Ti
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int k = 0; k < splits; ++k) {
-        const float4 t = ld4(p + ((size_t)k * TM + r) * q.bn + c);
+        const float4 t = *reinterpret_cast<const float4 *>(p + ((size_t)k * TM + r) * q.bn + c);
         s = make_float4(s.x + t.x, s.y + t.y, s.z + t.z, s.w + t.w);
     }
     const float *acc = a.acc ? a.acc + (size_t)m * a.n + n : nullptr;
@@ -769,8 +773,8 @@ template <bool AT>
 void split_sum(const MmArgs &a, const Tiles &q, int rest, cudaStream_t stream)
 {
     const dim3 grid(TM / 4, rest);
-    if (a.out_bf16) split_sum_kernel<__nv_bfloat16, AT><<<grid, 256, 0, stream>>>(a, q);
-    else split_sum_kernel<float, AT><<<grid, 256, 0, stream>>>(a, q);
+    if (a.out_bf16) launch_chained(split_sum_kernel<__nv_bfloat16, AT>, grid, 256, 0, stream, a, q);
+    else launch_chained(split_sum_kernel<float, AT>, grid, 256, 0, stream, a, q);
 }
 
 }  // namespace

@@ -69,6 +69,36 @@ inline cudaError_t smem_opt_in(size_t bytes)
     return e;
 }
 
+// A call's kernels, each of which begins with chained(): all but the first may be
+// set up while the one before still runs. The first waits for the stream as any
+// launch does, so what the call was given is complete for all of them; what they
+// hand one another they must not read through the read-only path (__ldg, const
+// __restrict__), which need not respect chained().
+inline bool &chain_open()
+{
+    static thread_local bool open = false;
+    return open;
+}
+inline void chain_begin() { chain_open() = false; }
+
+template <typename... P, typename... A>
+inline cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                  A &&...args)
+{
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    c.attrs = &early;
+    c.numAttrs = chain_open() ? 1 : 0;
+    chain_open() = true;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
 // Lanes per channel: ceil(N/4) rounded up to a power of two (N in [4, 64]).
 inline int groups_for(int N)
 {

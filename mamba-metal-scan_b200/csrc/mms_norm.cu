@@ -119,6 +119,7 @@ enum { POST = 1, GATE = 2, SCALE = 4 };
 template <typename T, int E, bool VEC, int F>
 __global__ void __launch_bounds__(ROW_THREADS) norm_fwd_kernel(const NormArgs a)
 {
+    chained();
     using C = Cols<T, E, VEC>;
     __shared__ float sh[2][32];
     BlockSum sum{sh, 0};
@@ -260,6 +261,7 @@ constexpr int bwd_smem(int threads) {
 template <typename T, int E, bool VEC, int F>
 __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_kernel(const NormArgs a)
 {
+    chained();
     using C = Cols<T, E, VEC>;
     extern __shared__ uint4 rows_smem[];
     __shared__ float sh[2][32];
@@ -404,6 +406,7 @@ __device__ __forceinline__ Row<T> row_of(const NormArgs &a, size_t r) {
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormArgs a)
 {
+    chained();
     __shared__ float sh[2][32];
     BlockSum sum{sh, 0};
     const float inv = 1.f / a.dim;
@@ -438,6 +441,7 @@ __global__ void __launch_bounds__(1024) norm_fwd_long_kernel(const NormArgs a)
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a)
 {
+    chained();
     __shared__ float sh[2][32];
     BlockSum sum{sh, 0};
     const float inv = 1.f / a.dim;
@@ -494,6 +498,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormArgs a)
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormArgs a, int blocks)
 {
+    chained();
     __shared__ float sh[32][33];
     const int which = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x;
     const float *p = static_cast<const float *>(a.workspace) + (size_t)which * blocks * a.dim;
@@ -558,10 +563,10 @@ cudaError_t run(const NormArgs &a, int threads, bool backward, int *blocks, cuda
         const cudaError_t e = smem_opt_in<norm_bwd_kernel<T, E, VEC, F>>(bwd_smem<T, E, VEC, F>(ROW_THREADS));
         if (e != cudaSuccess) return e;
         *blocks = std::min({a.rows, resident<norm_bwd_kernel<T, E, VEC, F>>(threads, smem), MAX_ROW_BLOCKS});
-        norm_bwd_kernel<T, E, VEC, F><<<*blocks, threads, smem, stream>>>(a);
+        launch_chained(norm_bwd_kernel<T, E, VEC, F>, *blocks, threads, smem, stream, a);
     } else {
         const int grid = std::min(a.rows, resident<norm_fwd_kernel<T, E, VEC, F>>(threads, 0));
-        norm_fwd_kernel<T, E, VEC, F><<<grid, threads, 0, stream>>>(a);
+        launch_chained(norm_fwd_kernel<T, E, VEC, F>, grid, threads, 0, stream, a);
     }
     return cudaGetLastError();
 }
@@ -598,8 +603,8 @@ cudaError_t run_type(const NormArgs &a, bool backward, int *blocks, cudaStream_t
         if (q.e == 16) return run_flags<T, 16, false>(a, q.threads, backward, blocks, s);
     }
     *blocks = std::min(a.rows, N_SM * 2);
-    if (backward) norm_bwd_long_kernel<T><<<*blocks, 1024, 0, s>>>(a);
-    else norm_fwd_long_kernel<T><<<*blocks, 1024, 0, s>>>(a);
+    if (backward) launch_chained(norm_bwd_long_kernel<T>, *blocks, 1024, 0, s, a);
+    else launch_chained(norm_fwd_long_kernel<T>, *blocks, 1024, 0, s, a);
     return cudaGetLastError();
 }
 
@@ -612,19 +617,21 @@ size_t norm_workspace_bytes(int rows, int dim)
 
 cudaError_t launch_norm_fwd(const NormArgs &a, cudaStream_t stream)
 {
+    chain_begin();
     int blocks;
     return a.bf16 ? run_type<__nv_bfloat16>(a, false, &blocks, stream) : run_type<float>(a, false, &blocks, stream);
 }
 
 cudaError_t launch_norm_bwd(const NormArgs &a, cudaStream_t stream)
 {
+    chain_begin();
     int blocks = 0;
     const cudaError_t e = a.bf16 ? run_type<__nv_bfloat16>(a, true, &blocks, stream)
                                  : run_type<float>(a, true, &blocks, stream);
     if (e != cudaSuccess) return e;
     const dim3 grid((a.dim + 31) / 32, a.post || a.scale ? 2 : 1);
-    if (a.bf16) norm_reduce_kernel<__nv_bfloat16><<<grid, dim3(32, 32), 0, stream>>>(a, blocks);
-    else norm_reduce_kernel<float><<<grid, dim3(32, 32), 0, stream>>>(a, blocks);
+    if (a.bf16) launch_chained(norm_reduce_kernel<__nv_bfloat16>, grid, dim3(32, 32), 0, stream, a, blocks);
+    else launch_chained(norm_reduce_kernel<float>, grid, dim3(32, 32), 0, stream, a, blocks);
     return cudaGetLastError();
 }
 
