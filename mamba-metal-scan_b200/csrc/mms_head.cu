@@ -608,7 +608,8 @@ __global__ void __launch_bounds__(256) few_kernel(const FewArgs a)
         Part t = sh[0][threadIdx.x];
 #pragma unroll
         for (int i = 1; i < 8; ++i) t = join(t, sh[i][threadIdx.x]);
-        a.part[(size_t)blockIdx.x * a.rows + threadIdx.x] = make_float2(t.x, (float)t.y);
+        // without the top's own 1, beside which float32 would lose the rest (less_one in lse_kernel)
+        a.part[(size_t)blockIdx.x * a.rows + threadIdx.x] = make_float2(t.x, (float)(t.y - 1.));
     }
 }
 
@@ -740,9 +741,10 @@ constexpr int AT_ONCE = 8;
 // One row a lane, 32 threads a row over the tiles. Parts 1..ntiles, and part
 // 0 (the pieces before) unless `first`. Writes part 0, or in the last piece
 // lse2 and, from the target's logit in logq2, the cross entropy's row loss;
-// with `total` (up to 32 rows) total_kernel's work too.
+// with `total` (up to 32 rows) total_kernel's work too. less_one: the parts' sums are less the 1 of
+// their maximum.
 __global__ void __launch_bounds__(1024)
-lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm, float2 *__restrict__ lse2,
+lse_kernel(float2 *part, bool less_one, int ntiles, bool first, bool last, int rows, RowMap rm, float2 *__restrict__ lse2,
            const int64_t *__restrict__ target, int64_t ignore, int vocab, float *__restrict__ logq2,
            const float *rest, float *__restrict__ loss, int reduction,
            float *__restrict__ total, float *__restrict__ count)
@@ -769,8 +771,8 @@ lse_kernel(float2 *part, int ntiles, bool first, bool last, int rows, RowMap rm,
             float s = 0.f, lost = 0.f;
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
-                const float y = __fmul_rn(p[i].y, ex2(p[i].x - ref)), n = s + y, d = n - s;
-                lost += (s - (n - d)) + (y - d);
+                const float e = ex2(p[i].x - ref), z = __fmul_rn(p[i].y, e), y = less_one ? e : z, n = s + y, d = n - s;
+                lost += (s - (n - d)) + (y - d) + (less_one ? z : 0.f);
                 s = n;
             }
             v.y += (double)s + lost;
@@ -1116,7 +1118,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         f.target = target; f.at = o.logq2; f.rest = rest; f.part = part + a.rows;
         if (a.bf16) launch_few<__nv_bfloat16>(f, blocks, false, stream);
         else launch_few<float>(f, blocks, false, stream);
-        launch_chained(lse_kernel, 1, dim3(32, 32), 0, stream, part, blocks, true, true, a.rows, rm, o.lse2, target,
+        launch_chained(lse_kernel, 1, dim3(32, 32), 0, stream, part, true, blocks, true, true, a.rows, rm, o.lse2, target,
                                                   a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction,
                                                   total, o.count);
     }
@@ -1143,7 +1145,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.rest = rest;
         if ((e = launch_mm(MM_LSE, mm, stream)) != cudaSuccess) return e;
         launch_chained(lse_kernel, ceil_div(a.rows, 32), dim3(32, 32), 0, stream,
-            part, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows, rm,
+            part, false, mm_lse_parts(a.rows, nv, a.dim, l.planes, l.planes), v0 == 0, v0 + nv == a.vocab, a.rows, rm,
             o.lse2, target, a.ignore_index, a.vocab, o.logq2, rest, rowloss, a.reduction, total, o.count);
     }
     if (a.kd)
