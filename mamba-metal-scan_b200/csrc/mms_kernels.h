@@ -73,8 +73,9 @@ inline cudaError_t smem_opt_in(size_t bytes)
 // set up while the one before still runs. The first waits for the stream as any
 // launch does, so what the call was given is complete for all of them; what they
 // hand one another they must not read through the read-only path (__ldg, const
-// __restrict__), which need not respect chained(). Between small kernels this saves the drain and
-// the start: seven kernels of a distillation of 130 rows 75 -> 62 us.
+// __restrict__), which need not respect chained(). Between small kernels this
+// saves the drain and the start: seven kernels of a distillation of 130 rows
+// 75 -> 62 us.
 inline bool &chain_open()
 {
     static thread_local bool open = false;

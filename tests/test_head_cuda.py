@@ -414,6 +414,35 @@ def test_another_stream_and_a_captured_graph():
         assert torch.equal(loss, want_loss) and all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_calls_with_left_out_rows(dtype):
+    """Above 512 rows a row map and cleared results stand between the kernels of a call."""
+    rows, vocab, dim = 700, 3000, 72
+    x, w, target, gen = head_inputs(rows, vocab, dim, dtype, seed=5)
+    target[::3] = -100
+    index, logits = torch.randint(-1, vocab, (rows, 3), generator=gen), torch.randn(rows, 3, generator=gen)
+    index[::4] = -1
+    t, index, logits = target.to(DEV), index.to(DEV), logits.to(DEV)
+
+    def calls(xd, wd):
+        a = linear_cross_entropy(xd, wd, t, reduction="none")
+        b = linear_distillation(xd, wd, index, logits, 2.0, reduction="none")
+        return [a.detach(), b.detach(), *torch.autograd.grad(a.sum(), [xd, wd]),
+                *torch.autograd.grad(b.sum(), [xd, wd])]
+
+    want = calls(*leaves(x, w))
+    xd, wd = leaves(x, w)               # leaves that no eager graph has met
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls(xd, wd)
+    for _ in range(3):
+        for one in got:
+            one.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 def test_the_refs_agree_with_the_kernels():
     x, w, target, gen = head_inputs(50, 400, 64, F32, seed=9)
     index, logits = torch.randint(-1, 400, (50, 5), generator=gen), torch.randn(50, 5, generator=gen)
