@@ -237,8 +237,10 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  *
  * reduction: MMS_REDUCE_NONE (loss, dloss: rows floats), MMS_REDUCE_MEAN (over
  * the rows that count; NaN if there is none) or MMS_REDUCE_SUM (one float).
- * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, dloss and the sums are float32. float32 products run on the tensor cores as
- * two scaled fp16 parts a factor (22 bits; see csrc/mms_head.cu).
+ * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, dloss and the sums are
+ * float32. float32 products run on the tensor cores as two scaled fp16 parts a
+ * factor (22 bits; see csrc/mms_head.cu). The backward of bf16 holds r (q - p)
+ * to 2^-11 of each value (up to 256 rows 2^-17) beside the rounding of dx and dw.
  *
  * The forward writes to `kept` (mms_head_kept_size() bytes) what the backward
  * of the same inputs reads; it is not changed there. dx (rows, dim) and dw

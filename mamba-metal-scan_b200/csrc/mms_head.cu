@@ -38,12 +38,19 @@
 //            fp32; as expm1(log q) + 1 - p where p is near 1, so that nothing
 //            cancels), then MM_OUT twice.
 //
-// bf16: dz is stored in bf16, one plane: without r where it is the same for
-// all rows (mean, sum: q - p is often close to -1, which bf16 holds better
-// than -1 / rows), as r (q - p) where it is not. The rounding (2^-8 a value at
-// most) averages out over a sum of many; with up to FEW_ROWS rows one value
-// can dominate a whole gradient, so a second plane holds the rest there (one
-// more pass of two products that such sizes do not feel).
+// bf16 backward: dz needs more bits than bf16's 8 beside the result's own
+// rounding. Above FEW_ROWS rows it is one plane of scaled fp16 (2^-11 of a value
+// at most; in bf16, 2^-8, gradients were 14 to 37 % further from float64 than
+// their own rounding, now 1 %), and x and w follow it into fp16, scaled by powers of two, which
+// holds a bf16 value exactly down to 2^-31 of the largest: r = M E with E a
+// power of two and M in [1, 2),
+//   dz = 2^14 M (q - p),  dx = E dz w,  dw = dz^T (E x)
+// so that dz is all that is rounded; below 2^-28 it loses bits to fp16's range
+// (2^-39 absolute). The price is w's copy and maximum: 8192 x 131072 x 2048
+// 15.4 -> 15.6 ms, 1000 x 50021 x 1001 with unaligned rows 464 -> 482 us. Up to FEW_ROWS rows, where w's bytes are what counts, w is taken as it
+// is and dz is two planes of bf16 (2^-17; a pass of the tensor cores more that
+// such sizes do not feel): without r where it is the same for all rows (mean,
+// sum), as r (q - p) where it is not.
 //
 // float32: factors are split into two fp16 planes, 22 bits, after a scaling by
 // a power of two that brings the largest element into [2^14, 2^15); the
@@ -80,7 +87,7 @@ constexpr int MAP_ROWS = 512;                       // two tiles of rows: with f
 int few_rows(bool bf16) { return bf16 ? 2 : 8; }
 constexpr int FEW_BLOCKS = 148 * 4;
 constexpr int STAGE_GRID = 148 * 16;                // CTAs of a staging pass, at most
-constexpr float DZ_UNIT = 16384.f;                  // float32: the scale of dz's planes
+constexpr float DZ_UNIT = 16384.f;                  // the scale of dz's planes in fp16
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -98,11 +105,12 @@ int piece_size(int vocab, size_t bytes_per_row)
     return (int)std::min<long long>(v, vocab);
 }
 
-// Both directions: planes of x and w, and whether they are staged.
+// Both directions: planes of x and w, and whether they are staged, and then as scaled fp16.
 struct Layout {
-    bool stage_x, stage_w;
+    bool stage_x, stage_w, scaled;
     int planes, piece, last;        // vocabulary entries of a piece, of the last one
-    size_t xs, ws, row_mul, muls;   // staged x, w; float32: their scales (muls: w's, r x's, and for few rows w's maximum)
+    size_t xs, ws, row_mul, muls;   // staged x, w; scaled: their scales (muls: w's, r x's, and w's maximum where
+                                    // the forward did not keep it)
     size_t total;
 };
 
@@ -133,7 +141,7 @@ struct BwdLayout : Layout {
     bool few;
     int gplanes;
     long long ldg;
-    size_t xr, g, dxacc, rs, tops, split, split_bytes;
+    size_t xr, g, dxacc, rs, pow, tops, split, split_bytes;
 };
 
 size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
@@ -143,7 +151,7 @@ size_t common_layout(Layout &l, int rows, int vocab, int dim, size_t per_entry)
     l.last = vocab - (vocab - 1) / l.piece * l.piece;
     size_t o = 0;
     l.muls = o; o += 256;
-    l.row_mul = o; o += l.planes > 1 ? up256((size_t)rows * sizeof(float)) : 0;
+    l.row_mul = o; o += l.scaled ? up256((size_t)rows * sizeof(float)) : 0;
     l.xs = o; o += l.stage_x ? up256(row * rows) : 0;
     l.ws = o; o += l.stage_w ? up256(row * l.piece) : 0;
     return o;
@@ -154,6 +162,7 @@ FwdLayout fwd_layout(int rows, int vocab, int dim, int k, bool bf16, long long l
     FwdLayout l;
     l.few = rows <= few_rows(bf16);
     l.planes = bf16 || l.few ? 1 : 2;
+    l.scaled = l.planes > 1;
     l.stage_x = !l.few && (!bf16 || ldx % 8 || rows > MAP_ROWS);
     l.stage_w = !l.few && (!bf16 || ldw % 8);
     size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * sizeof(float2) / 32 + 1);
@@ -176,16 +185,18 @@ BwdLayout bwd_layout(int rows, int vocab, int dim, bool bf16, long long ldw)
     BwdLayout l;
     l.planes = bf16 ? 1 : 2;
     l.few = rows <= few_rows(bf16);
-    l.gplanes = bf16 && rows > FEW_ROWS ? 1 : 2;
+    l.scaled = !bf16 || rows > FEW_ROWS;
+    l.gplanes = bf16 && l.scaled ? 1 : 2;
     l.stage_x = true;
-    l.stage_w = !bf16 || ldw % 8;
+    l.stage_w = l.scaled || ldw % 8;
     size_t o = common_layout(l, rows, vocab, dim, (size_t)rows * 2 * l.gplanes);
     l.ldg = (l.piece + 7) / 8 * 8;
-    l.xr = o; o += l.planes > 1 ? up256((size_t)padded(dim) * 2 * l.planes * rows) : 0;
+    l.xr = o; o += l.scaled ? up256((size_t)padded(dim) * 2 * l.planes * rows) : 0;
     l.g = o; o += up256((size_t)rows * l.ldg * 2 * l.gplanes);
     l.dxacc = o; o += l.piece < vocab ? up256((size_t)rows * dim * sizeof(float)) : 0;
     l.rs = o; o += up256((size_t)rows * sizeof(float));
-    l.tops = o; o += l.planes > 1 ? up256(STAGE_GRID * sizeof(float)) : 0;
+    l.pow = o; o += bf16 && l.scaled ? up256((size_t)rows * sizeof(float)) : 0;
+    l.tops = o; o += l.scaled ? up256(STAGE_GRID * sizeof(float)) : 0;
     // partial sums; the last, smaller piece splits as far as this room goes
     l.split_bytes = std::max(mm_split_bytes(rows, dim, l.piece, l.gplanes, l.planes, rows > MAP_ROWS),
                              mm_split_bytes(l.piece, dim, rows, l.gplanes, l.planes, false));
@@ -288,6 +299,8 @@ struct RowFactors {
     float tau;
     float *rs;                  // written: r of each row; NaN where an index that counts lies outside the
                                 // vocabulary (logq2 is NaN there)
+    float *pow;                 // written, if not null: E of each row, and DZ_UNIT M to rs; r = M E with E a
+                                // power of two
     float *whole;               // written, may be null: the factor of all rows that count, where it is the same
 };
 
@@ -302,7 +315,7 @@ struct StageArgs {
     const float *rs;            // ST_WHOLE: factors of the rows, or null
     float *mul;                 // ST_ROWS: 2^-e of each row; ST_WHOLE: of all
     float *top;                 // ST_WHOLE: maxima whose largest sets the scale, `tops` of them
-    int tops;                   // ST_ROWS: the CTAs' maxima of |r| times the row's go to `top` (if not null),
+    int tops;                   // ST_ROWS: the CTAs' maxima of |r| (or E) times the row's go to `top` (if not null),
                                 //          and with `zero` a zero there
     float *zero;
 };
@@ -331,6 +344,12 @@ __device__ __forceinline__ float row_factor(const RowFactors &f, RowMap rm, int 
     return !some ? 0.f : bad && r != 0.f ? __int_as_float(0x7fc00000) : r;
 }
 
+// r's E: its exponent alone, 1 where r is 0 or not finite (M = r then).
+__device__ __forceinline__ float pow2_of(float r) {
+    const uint32_t e = __float_as_uint(r) >> 23 & 255;
+    return r == 0.f || e == 255 ? 1.f : __uint_as_float(max(e, 1u) << 23);
+}
+
 // LP lanes a row, 8 columns a lane and step. Bound by memory: 32768 x 640 of
 // float32 weights in 26 us (84 MB in, 84 out: 6.4 TB/s); 50021 x 1001 bf16,
 // whose rows are not aligned, in 42 us (4.8 TB/s).
@@ -349,6 +368,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
     }
     if (KIND == ST_ROWS && a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0.f;
     constexpr int RW = 32 / LP;                             // rows a warp has at once
+    constexpr bool REST = KIND != ST_COPY && sizeof(T) == 4;    // a second plane: bf16 needs none in fp16
     // a last tile's padding is 0: nothing behind it is read
     const int live = a.rows_map.n(a.rows), rows = min(a.rows, (max(live, 1) + 255) / 256 * 256);
     for (int r0 = (blockIdx.x * 8 + threadIdx.x / 32) * RW; r0 < rows; r0 += gridDim.x * 8 * RW) {
@@ -359,7 +379,10 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
         float rs = r >= live ? 0.f : a.rs ? a.rs[r] : 1.f;
         if (KIND != ST_WHOLE && a.from.dloss) {
             rs = row_factor<LP>(a.from, a.rows_map, r, live, lane);
-            if (in && lane == 0) a.from.rs[r] = rs;
+            const float pow = a.from.pow ? pow2_of(rs) : 1.f;
+            if (in && lane == 0) a.from.rs[r] = a.from.pow ? rs / pow * DZ_UNIT : rs;
+            if (a.from.pow && rs != 0.f) rs = pow;
+            if (in && lane == 0 && a.from.pow) a.from.pow[r] = rs;
         }
         const int cols = rs == 0.f ? 0 : a.cols;            // nothing of a left-out row is read
         Pow2 by{1.f, 1.f};
@@ -396,14 +419,14 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
                         x = by(KIND == ST_WHOLE ? rs * x : x);
                         const __half q = __float2half_rn(x);
                         h[j] = __half_as_ushort(q);
-                        l[j] = __half_as_ushort(__float2half_rn(x - __half2float(q)));
+                        if (REST) l[j] = __half_as_ushort(__float2half_rn(x - __half2float(q)));
                     }
                 }
                 hi[i] = h[0] | (uint32_t)h[1] << 16;
-                if (KIND != ST_COPY) lo[i] = l[0] | (uint32_t)l[1] << 16;
+                if (REST) lo[i] = l[0] | (uint32_t)l[1] << 16;
             }
             *reinterpret_cast<uint4 *>(out + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (KIND != ST_COPY)
+            if (REST)
                 *reinterpret_cast<uint4 *>(out + a.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
@@ -413,23 +436,42 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageArgs a)
     }
 }
 
-// The largest finite magnitude of a float32 matrix (*top starts at 0). A warp
-// reads two rows at a time; one atomic a CTA, a few thousand on one address
-// would take longer than the reads. 32768 x 640: 18 us (4.6 TB/s).
+// The largest finite magnitude of a matrix (*top starts at 0), whose last row
+// has `last` columns; VEC: every row begins at 16 bytes. A warp reads a row, 4
+// pieces a lane at a time; one atomic a CTA, a few thousand on one address
+// would take longer than the reads. 131072 x 2048 bf16: 95 us (5.6 TB/s).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-top_kernel(const float *__restrict__ src, long long lds, int rows, int cols, float *top)
+top_kernel(const T *__restrict__ src, long long lds, int rows, int cols, int last, float *top)
 {
     chained();
+    constexpr int PIECE = VEC ? 16 / (int)sizeof(T) : 8;
+    const int lane = threadIdx.x % 32;
     float m = 0.f;
-    for (long long r = ((long long)blockIdx.x * 8 + threadIdx.x / 32) * 2; r < rows; r += gridDim.x * 16) {
-        const float *p = src + (size_t)r * lds, *q = r + 1 < rows ? p + lds : p;
-#pragma unroll 2
-        for (int c = threadIdx.x % 32 * 8; c < cols; c += 256) {
-            float v[8], w[8];
-            load8(p, c, cols, v);
-            load8(q, c, cols, w);
+    for (long long r = (long long)blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
+        const T *p = src + (size_t)r * lds;
+        const int n = r + 1 < rows ? cols : last;
+        if (VEC) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(p);
+            for (int c = lane; c < n / PIECE; c += 128) {
+                uint4 t[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(finite_abs(v[i]), finite_abs(w[i])));
+                for (int k = 0; k < 4; ++k) t[k] = c + 32 * k < n / PIECE ? __ldg(q + c + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < PIECE; ++i) m = fmaxf(m, finite_abs(to_f(reinterpret_cast<const T *>(t + k)[i])));
+            }
+            const int c = n / PIECE * PIECE + lane;
+            if (c < n) m = fmaxf(m, finite_abs(to_f(p[c])));
+        } else {
+#pragma unroll 2
+            for (int c = lane * PIECE; c < n; c += 32 * PIECE) {
+                float v[8];
+                load8(p, c, n, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i]));
+            }
         }
     }
     m = block_max(m);                                       // non-negative floats compare as their bits
@@ -1006,16 +1048,45 @@ Kept kept_of(const HeadArgs &a)
 
 float *fl(void *base, size_t off) { return reinterpret_cast<float *>(static_cast<char *>(base) + off); }
 
-// Where w's largest magnitude is: the forward keeps it for the backward
-// (count[1]), but for few rows, whose forward does not need it.
+// Where w's largest magnitude is: the float32 forward keeps it for the backward
+// (count[1]), but for few rows, where it does not need it, as the bf16 one never does.
+bool finds_top(const HeadArgs &a, const Layout &l)
+{
+    return l.scaled && (!a.backward || a.bf16 || a.rows <= few_rows(a.bf16));
+}
 float *w_top(const HeadArgs &a, const Layout &l)
 {
-    return a.backward && a.rows <= few_rows(a.bf16) ? fl(a.workspace, l.muls) + 3 : kept_of(a).count + 1;
+    return a.backward && finds_top(a, l) ? fl(a.workspace, l.muls) + 3 : kept_of(a).count + 1;
+}
+template <typename T>
+void top_of(const HeadArgs &a, float *top, cudaStream_t s)
+{
+    int rows = a.vocab, cols = a.dim, last = a.dim;
+    long long ld = a.ldw;
+    if (ld == cols && ld * sizeof(T) % 16) {                // rows without gaps: aligned ones of another length
+        const long long n = (long long)rows * cols;
+        ld = cols = 2048;
+        rows = ceil_div(n, cols);
+        last = (int)(n - (rows - 1) * ld);
+    }
+    const auto run = [&](auto kernel) {
+        launch_chained(kernel, std::min(ceil_div(rows, 8), 148 * 8), 256, 0, s, static_cast<const T *>(a.w), ld, rows, cols,
+                       last, top);
+    };
+    if (ld * sizeof(T) % 16 == 0) run(top_kernel<T, true>);
+    else run(top_kernel<T, false>);
 }
 void top_of_w(const HeadArgs &a, float *top, cudaStream_t s)
 {
-    launch_chained(top_kernel, std::min(ceil_div(a.vocab, 16), 148 * 8), 256, 0, s, static_cast<const float *>(a.w), a.ldw,
-                                                                       a.vocab, a.dim, top);
+    if (a.bf16) top_of<__nv_bfloat16>(a, top, s);
+    else top_of<float>(a, top, s);
+}
+
+template <int KIND>
+void stage_scaled(const HeadArgs &a, const StageArgs &st, cudaStream_t s)
+{
+    if (a.bf16) stage<__nv_bfloat16, KIND>(st, s);
+    else stage<float, KIND>(st, s);
 }
 
 // Rows [v0, v0 + n) of w as a factor: staged, or w itself.
@@ -1030,14 +1101,14 @@ Factor w_factor(const HeadArgs &a, const Layout &l, int v0, int n, cudaStream_t 
     st.rows = n; st.cols = a.dim;
     st.mul = fl(a.workspace, l.muls);
     st.top = w_top(a, l); st.tops = 1;
-    if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
-    else stage<float, ST_WHOLE>(st, s);
+    if (l.scaled) stage_scaled<ST_WHOLE>(a, st, s);
+    else stage<__nv_bfloat16, ST_COPY>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
 }
 
 // x as a factor of z: staged, or x itself. Backward: with the rows' factors
-// (`from`), and for float32 the maxima of r x. In float32 the place of w's
-// maximum is zeroed for top_of_w.
+// (`from`), and if scaled the maxima of r x. The place of w's maximum is zeroed
+// for top_of_w.
 Factor x_factor(const HeadArgs &a, const Layout &l, const RowFactors &from, float *tops, RowMap rm, cudaStream_t s)
 {
     if (!l.stage_x) return Factor{static_cast<const uint16_t *>(a.x), a.ldx, 0, 1, false};
@@ -1049,9 +1120,9 @@ Factor x_factor(const HeadArgs &a, const Layout &l, const RowFactors &from, floa
     st.from = from;
     st.mul = fl(a.workspace, l.row_mul);
     st.top = tops;
-    st.zero = !a.backward || a.rows <= few_rows(a.bf16) ? w_top(a, l) : nullptr;
-    if (a.bf16) stage<__nv_bfloat16, ST_COPY>(st, s);
-    else stage<float, ST_ROWS>(st, s);
+    st.zero = finds_top(a, l) ? w_top(a, l) : nullptr;
+    if (l.scaled) stage_scaled<ST_ROWS>(a, st, s);
+    else stage<__nv_bfloat16, ST_COPY>(st, s);
     return Factor{st.out, ld, st.plane, l.planes, false};
 }
 
@@ -1123,7 +1194,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
                                                   total, o.count);
     }
     const Factor x = l.few ? Factor{} : x_factor(a, l, RowFactors{}, nullptr, rm, stream);
-    if (l.planes > 1) top_of_w(a, w_top(a, l), stream);
+    if (finds_top(a, l)) top_of_w(a, w_top(a, l), stream);
     for (int v0 = l.few ? a.vocab : 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
         MmArgs mm{};
@@ -1133,7 +1204,7 @@ cudaError_t launch_head_fwd(const HeadArgs &a, cudaStream_t stream)
         mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
         mm.live = rm.live;
         mm.row_of = rm.map;
-        if (l.planes > 1) {
+        if (l.scaled) {
             mm.row_mul = fl(a.workspace, l.row_mul);
             mm.mul = fl(a.workspace, l.muls);
         }
@@ -1164,10 +1235,11 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
     const Kept o = kept_of(a);
     const RowMap rm{o.map, o.live};
     const float c = MMS_LOG2E / a.tau;
-    const bool f32 = l.planes > 1;
-    // bf16, all rows alike: dz without r, which comes in with the products' factors
-    const bool uniform = a.bf16 && a.reduction != MMS_REDUCE_NONE;
+    // unscaled, all rows alike: dz without r, which comes in with the products' factors
+    const bool uniform = !l.scaled && a.reduction != MMS_REDUCE_NONE;
     float *rs = fl(a.workspace, l.rs), *acc = fl(a.workspace, l.dxacc);
+    float *pow = a.bf16 && l.scaled ? fl(a.workspace, l.pow) : nullptr;
+    const float *row_by = pow ? pow : rs;               // what dz is without: E or r
     float *muls = fl(a.workspace, l.muls), *row_mul = fl(a.workspace, l.row_mul);
     cudaError_t e;
     // the rows that are left out
@@ -1175,24 +1247,24 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         (e = cudaMemsetAsync(a.dx, 0, (size_t)a.rows * a.dim * (a.bf16 ? 2 : 4), stream)) != cudaSuccess)
         return e;
     const RowFactors from{a.dloss, o.count, o.prob, o.logq2, a.index, a.ignore_index, a.k, a.reduction, a.tau, rs,
-                          uniform ? muls + 1 : nullptr};
-    const Factor x = x_factor(a, l, from, f32 ? fl(a.workspace, l.tops) : nullptr, rm, stream);
-    if (f32 && l.few) top_of_w(a, w_top(a, l), stream);
-    Factor xr = x;                                      // the factor of dw: x, or r x
-    if (f32) {
+                          pow, uniform ? muls + 1 : nullptr};
+    const Factor x = x_factor(a, l, from, l.scaled ? fl(a.workspace, l.tops) : nullptr, rm, stream);
+    if (finds_top(a, l)) top_of_w(a, w_top(a, l), stream);
+    Factor xr = x;                                      // the factor of dw: x, r x or E x
+    if (l.scaled) {
         StageArgs st{};
         st.src = a.x; st.lds = a.ldx;
         st.out = u16(a.workspace, l.xr); st.ld = x.ld; st.plane = x.plane;
         st.rows = a.rows; st.cols = a.dim; st.rows_map = rm;
-        st.rs = rs;
+        st.rs = row_by;
         st.mul = muls + 1;
         st.top = fl(a.workspace, l.tops); st.tops = stage_grid(a.rows, a.dim);
-        stage<float, ST_WHOLE>(st, stream);
+        stage_scaled<ST_WHOLE>(a, st, stream);
         xr.p = st.out;
     }
     xr.t = true;
     const long long n = (long long)a.rows * a.k, gplane = (long long)a.rows * l.ldg;
-    const float unit = f32 ? DZ_UNIT : uniform ? 1.f : 0.f;
+    const float unit = !a.bf16 ? DZ_UNIT : uniform ? 1.f : 0.f;
     uint16_t *g = u16(a.workspace, l.g);
     for (int v0 = 0; v0 < a.vocab; v0 += l.piece) {
         const int nv = std::min(l.piece, a.vocab - v0);
@@ -1200,10 +1272,10 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
         MmArgs mm{};
         mm.a = x;
         mm.b = w_factor(a, l, v0, nv, stream);
-        mm.fp16 = f32;
+        mm.fp16 = l.scaled;
         mm.m = a.rows; mm.n = nv; mm.k = a.dim; mm.c = c;
         mm.live = rm.live;
-        if (f32) {
+        if (l.scaled) {
             mm.row_mul = row_mul;
             mm.mul = muls;
         }
@@ -1220,10 +1292,10 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             return e;
         }
         launch_chained(sparse_kernel, ceil_div(n, 256), 256, 0, stream, a.index, o.prob, o.logq2, rs, unit, a.k, a.rows, rm, v0,
-                                                            v0 + nv, g, l.ldg, gplane, l.gplanes, f32);
+                                                            v0 + nv, g, l.ldg, gplane, l.gplanes, l.scaled);
         MmArgs out{};
-        out.fp16 = f32;
-        out.c = f32 ? 1.f / DZ_UNIT : 1.f;
+        out.fp16 = l.scaled;
+        out.c = l.scaled ? 1.f / DZ_UNIT : 1.f;
         out.n = a.dim;
         out.live = rm.live;
         out.split = fl(a.workspace, l.split);
@@ -1233,8 +1305,8 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             out.b = mm.b;
             out.b.t = true;
             out.m = a.rows; out.k = nv;
-            out.row_mul = f32 || uniform ? rs : nullptr;
-            out.mul = f32 ? muls : nullptr;
+            out.row_mul = l.scaled || uniform ? row_by : nullptr;
+            out.mul = l.scaled ? muls : nullptr;
             out.acc = first ? nullptr : acc;
             out.out = last ? a.dx : acc;
             out.out_bf16 = last && a.bf16;
@@ -1247,7 +1319,7 @@ cudaError_t launch_head_bwd(const HeadArgs &a, cudaStream_t stream)
             out.b = xr;
             out.m = nv; out.k = a.rows;
             out.row_mul = nullptr;
-            out.mul = f32 || uniform ? muls + 1 : nullptr;
+            out.mul = l.scaled || uniform ? muls + 1 : nullptr;
             out.acc = nullptr;
             out.out = static_cast<char *>(a.dw) + (size_t)v0 * a.dim * (a.bf16 ? 2 : 4);
             out.out_bf16 = a.bf16;
