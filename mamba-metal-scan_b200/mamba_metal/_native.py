@@ -306,7 +306,7 @@ def linear_ce_fwd(x, w, target, ignore_index: int, reduction: str, keep: bool = 
     backward needs (None without `keep`)."""
     m, d = x.shape
     red = REDUCTIONS[reduction]
-    loss = torch.empty((m,) if red == 0 else (), device=x.device)
+    loss = torch.empty((m,) if red == 0 else (), device=x.device, dtype=torch.float32)
     ws, nb, kept_at, kept, _live = _head_buffers(x, w, 0, keep)
     rc = load().mms_linear_ce_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   target.data_ptr(), ignore_index, red, loss.data_ptr(),
@@ -343,7 +343,7 @@ def linear_kd_fwd(x, w, index, logits, temperature: float, reduction: str, keep:
     m, d = x.shape
     k = index.shape[1]
     red = REDUCTIONS[reduction]
-    loss = torch.empty((m,) if red == 0 else (), device=x.device)
+    loss = torch.empty((m,) if red == 0 else (), device=x.device, dtype=torch.float32)
     ws, nb, kept_at, kept, _live = _head_buffers(x, w, k, keep)
     rc = load().mms_linear_kd_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                   index.data_ptr(), logits.data_ptr(), k, temperature, red,
@@ -380,7 +380,7 @@ def norm_fwd(x, y, gate, weight, post, scale, eps: float, keep: bool = True):
     stat: what the backward needs (None without `keep`)."""
     m, d = x.shape
     h, u = torch.empty_like(x), torch.empty_like(x)
-    stat = torch.empty(m, 2, device=x.device) if keep else None
+    stat = torch.empty(m, 2, device=x.device, dtype=torch.float32) if keep else None
     rc = load().mms_norm_fwd(_ptr(x), _ptr(y), _opt(gate), d if gate is None else gate.stride(0),
                              _ptr(weight), _opt(post), _opt(scale), eps, _ptr(h), _ptr(u),
                              _opt(stat), m, d, _dtype(x), _stream(x.device))
@@ -418,7 +418,7 @@ def pipe_rate(kind: str, device=None, iters: int = 4096, ctas_per_sm: int = 4) -
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     n_sm = torch.cuda.get_device_properties(device).multi_processor_count
     blocks = n_sm * ctas_per_sm
-    sink = torch.empty(256, device=device)
+    sink = torch.empty(256, device=device, dtype=torch.float32)
     cycles = torch.empty(blocks, dtype=torch.int64, device=device)
     sm = torch.empty(blocks, dtype=torch.int32, device=device)
     k = PROBE_KINDS[kind]
