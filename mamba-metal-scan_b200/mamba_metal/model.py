@@ -55,11 +55,11 @@ class MambaConfig:
     scan_impl: str = "auto"   # 'auto' | 'cuda' | 'metal' | 'torch'
     fuse_proj: bool = True    # CUDA scan computes dt and softplus(A) itself (selective_scan_proj)
     fuse_gate: bool = True    # (y + D_skip) * silu(z) as one CUDA kernel each way (gated_output)
-    fuse_norm: bool = False   # residual sum + next norm as one CUDA kernel each way (residual_rms_norm)
-    fuse_loss: bool = False   # with targets: no logits, forward returns (None, loss) (linear_cross_entropy)
     dt_min: float = 0.001
     dt_max: float = 0.1
     norm_eps: float = 1e-6
+    fuse_norm: bool = False   # residual sum + next norm as one CUDA kernel each way (residual_rms_norm)
+    fuse_loss: bool = False   # with targets: no logits, forward returns (None, loss) (linear_cross_entropy)
 
 
 def transformer_block_params(d_model: int, d_ff: int) -> int:
