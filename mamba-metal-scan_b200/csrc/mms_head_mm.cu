@@ -32,15 +32,20 @@
 // four products against 3.6: the copies no longer bound them.
 //
 // The tensor core adds each 16 summed elements to its fp32 sum with truncation,
-// not rounding, so a long sum drifts towards zero by about n 2^-25 of itself
-// over n additions (measured: 1.1e-5 at 8192 elements). Where the result
-// stays float32 the sum is therefore cut into parts of PART elements: each
+// not rounding, so a long sum drifts towards zero: each addition loses up to
+// 2^-23 of the sum so far (measured: 1.1e-5 of a result at 8192 elements, 1.1e-3
+// at 262144). The sum is therefore cut into parts: each
 // goes to its own tensor memory buffer and the epilogue warps add the parts up
-// in registers, rounding to nearest (`PARTS`). Parts of 512 cost nothing
-// beside the multiplies; of 256, 25 % of the log-sum-exp at 8192 x 131072 x
-// 2048 (4.15 ms against 3.31); of 128, 80 %. With two planes by two each
+// in registers, rounding to nearest (`PARTS`). Where the result stays float32,
+// parts of 512 cost nothing beside the multiplies; of 256, 25 % of the
+// log-sum-exp at 8192 x 131072 x 2048 (4.15 ms against 3.31); of 128, 80 %. With
+// two planes by two each
 // element is added three times, so parts are of 256 (3.17 ms for the four
-// products; of 384 3.06 ms but errors up to 1.5e-6, of 192 3.37 ms).
+// products; of 384 3.06 ms but errors up to 1.5e-6, of 192 3.37 ms). Where 16
+// bits are kept of the result, sums of more than 2048 elements are cut into parts
+// of as many (a drift of 2^-16 at most, and so the backward's q of 2^-16 of its
+// logit; 8192 x 131072 x 2048, forward and backward, 15.4 -> 15.6 ms; with parts
+// of 512 for dz alone 16.4, everywhere 17.2).
 //
 // The epilogue turns a warp's 32 rows x 32 columns through shared memory, in
 // 16-byte pieces (16-bit results already rounded and packed), so that its
@@ -81,6 +86,7 @@ constexpr int HALF = 16384;                                  // bytes of one CTA
 constexpr int GROUP = 16;
 constexpr int PART = 512;                                    // summed elements per part
 constexpr int PART_BOTH = 256;                               // the same for two planes by two
+constexpr int PART_LONG = 2048;                              // the same where 16 bits are kept of the result
 constexpr int TURN = 32 * 33;                                // floats of a warp's tile to turn
 // Stages: two planes by two stand side by side in one stage, and are read once for all three passes.
 constexpr int STAGE_BYTES = 6 * 2 * HALF;                    // of all stages
@@ -718,7 +724,9 @@ cudaError_t launch(const MmArgs &a, Tiles q, cudaStream_t stream)
 {
     // one round of tiles is short anyway: finer parts, as far as the multiplies hide them (a part costs the
     // epilogue some 1900 clocks, a step 512 a pass)
-    q.part = !PARTS ? q.steps : q.items <= N_SM / 2 ? (BOTH ? 2 : 4) : (BOTH ? PART_BOTH : PART) / BK;
+    q.part = !PARTS ? q.steps
+             : KIND != MM_LSE && !BOTH ? PART_LONG / BK
+             : q.items <= N_SM / 2 ? (BOTH ? 2 : 4) : (BOTH ? PART_BOTH : PART) / BK;
     const auto fn = tma_encoder();
     CUtensorMap ma, mb;
     if (!fn || !tma_context() || !encode(fn, &ma, a.a, a.m, a.k, 128) || !encode(fn, &mb, a.b, a.n, a.k, q.bn / 2))
@@ -736,9 +744,7 @@ cudaError_t launch_as(const MmArgs &a, const Tiles &q, bool parts, bool both, cu
 {
     if (both)
         return parts ? launch<KIND, AT, BT, true, true>(a, q, stream) : launch<KIND, AT, BT, false, true>(a, q, stream);
-    if constexpr (KIND == MM_LSE)
-        if (parts) return launch<KIND, AT, BT, true, false>(a, q, stream);
-    return launch<KIND, AT, BT, false, false>(a, q, stream);
+    return parts ? launch<KIND, AT, BT, true, false>(a, q, stream) : launch<KIND, AT, BT, false, false>(a, q, stream);
 }
 
 // out = acc + the partial sums of the split tiles, in order; a CTA per 4 rows of a tile,
@@ -794,11 +800,11 @@ size_t mm_split_bytes(int m, int n, int k, int planes_a, int planes_b, bool live
 cudaError_t launch_mm(MmKind kind, const MmArgs &a, cudaStream_t stream)
 {
     const Tiles q = plan(kind, a.m, a.n, a.k, passes_of(a.a.planes, a.b.planes), a.split_bytes);
-    // float32 results in parts; what is rounded to bf16 anyway (2^-9) in one sum
     const int steps = q.whole || a.live ? q.steps : q.kb;       // live rows split as the device finds it
     const bool both = a.a.planes == 2 && a.b.planes == 2;
-    const bool parts = (kind == MM_LSE || both) && (steps * BK > (both ? PART_BOTH : PART) ||
-                                                    (q.items <= N_SM / 2 && steps > (both ? 2 : 4)));
+    const bool parts = kind != MM_LSE && !both ? steps > PART_LONG / BK
+                                               : steps * BK > (both ? PART_BOTH : PART) ||
+                                                     (q.items <= N_SM / 2 && steps > (both ? 2 : 4));
     if (kind == MM_LSE) return launch_as<MM_LSE, false, false>(a, q, parts, both, stream);
     if (kind == MM_GRAD) return launch_as<MM_GRAD, false, false>(a, q, parts, both, stream);
     const cudaError_t e = a.a.t ? launch_as<MM_OUT, true, true>(a, q, parts, both, stream)
