@@ -16,7 +16,7 @@
 // where the difference of a likely entry's logit to lse2 is small and exact.
 // z is computed once forward (2 rows vocab dim flops) and again backward, in
 // pieces of the vocabulary small enough that dz's piece stays in a bounded
-// workspace; the two products with dz follow piece by piece (6 more).
+// workspace (piece_size); the two products with dz follow piece by piece (6 more).
 //
 // Rows that do not count (an ignored target, an empty list) take no part: with
 // more than MAP_ROWS rows a map lists those that do (map_kernel), x is staged
@@ -79,7 +79,9 @@ namespace mms {
 namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
-constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // bound on one staged or dz piece
+constexpr size_t PIECE_BYTES = (size_t)512 << 20;   // a staged or dz piece; or up to this much more
+constexpr size_t PIECE_MOST = (size_t)2 << 30;      // for PIECE_ENTRIES of the vocabulary
+constexpr int PIECE_ENTRIES = 4096;
 constexpr int FEW_ROWS = 256;
 constexpr int MAP_ROWS = 512;                       // two tiles of rows: with fewer there is little to leave out
 // Rows that the CUDA cores take: at 50176 x 1024 they need (us, forward) 34, 49, 45, 68 for 1, 2,
@@ -95,12 +97,16 @@ long long padded(int dim) { return (dim + 7) / 8 * 8; }     // rows of 16-byte m
 
 // Pieces of the vocabulary (each a multiple of MM_COLS rows of w but the
 // last): as few equal ones as keep `bytes_per_row` (per vocabulary entry)
-// times the piece below PIECE_BYTES, at least 4096 entries each so that a
-// piece's products stay long.
+// times the piece below PIECE_BYTES, or below PIECE_MOST for pieces of
+// PIECE_ENTRIES, so that their products stay long and the float32 sums of dx are
+// not read and written too often (7 % of the time with 4096 entries a piece); of MM_COLS
+// where even those are more (dz above 4 M rows).
 int piece_size(int vocab, size_t bytes_per_row)
 {
-    const long long most = std::max<long long>(4096, (long long)(PIECE_BYTES / bytes_per_row));
-    const int pieces = ceil_div(vocab, most);
+    const size_t long_ones = std::min<size_t>(PIECE_ENTRIES, PIECE_MOST / bytes_per_row);
+    const int most = (int)std::min<size_t>(vocab, std::max({(size_t)MM_COLS, long_ones, PIECE_BYTES / bytes_per_row}));
+    // whole tiles: equal pieces rounded up would pass the bound
+    const int whole = most >= vocab ? vocab : most / MM_COLS * MM_COLS, pieces = ceil_div(vocab, whole);
     const long long v = ceil_div(ceil_div(vocab, pieces), MM_COLS) * (long long)MM_COLS;
     return (int)std::min<long long>(v, vocab);
 }
