@@ -239,7 +239,9 @@ int mms_bwd_bf16(const uint16_t *x, const uint16_t *dt, const float *aneg,
  * the rows that count; NaN if there is none) or MMS_REDUCE_SUM (one float).
  * dtype: MMS_F32 or MMS_BF16 (x, w, dx, dw); loss, dloss and the sums are
  * float32. float32 products run on the tensor cores as two scaled fp16 parts a
- * factor (22 bits; see csrc/mms_head.cu). The backward of bf16 holds r (q - p)
+ * factor: 22 bits of elements down to 2^-16 of the largest, an absolute 2^-39 of the
+ * largest below that; x and dz are scaled row by row, w as a whole (see
+ * csrc/mms_head.cu). The backward of bf16 holds r (q - p)
  * to 2^-11 of each value (up to 256 rows 2^-17) beside the rounding of dx and dw.
  *
  * The forward writes to `kept` (mms_head_kept_size() bytes) what the backward

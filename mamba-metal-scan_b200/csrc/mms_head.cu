@@ -55,10 +55,13 @@
 // float32: factors are split into two fp16 planes, 22 bits, after a scaling by
 // a power of two that brings the largest element into [2^14, 2^15); the
 // product of the second planes (below 2^-22 of a term) is left out. Elements
-// below 2^-29 of the largest lose bits to fp16's range: 2^-39 of the largest is
-// the absolute bound. Three passes of the tensor cores; three bf16 planes would
-// keep float32's range but need six. The scalings follow the output's rows
-// where they can, so that rows do not disturb one another:
+// below 2^-16 of the largest lose bits to fp16's range, one for each power of
+// two (2^-20: 19 bits left, 2^-28: 11): 2^-39 of the largest is the absolute
+// bound. So a vocabulary row of w far above the rest, by 2^16 and more, costs
+// the others bits that float32 sums would keep. Three passes of the tensor
+// cores; three bf16 planes would keep float32's range but need six. The scalings
+// follow the output's rows where they can, so that rows do not disturb one
+// another:
 //   z  = x w^T    x scaled row by row, w as a whole
 //   dz = 2^14 (q - p) without r, in [-2^14, 2^14]
 //   dx = r dz w   r in the epilogue
