@@ -170,7 +170,8 @@ const char *mms_status_string(int status)
     case MMS_ERR_INVALID_ARG: return "invalid argument (size out of range or NULL pointer)";
     case MMS_ERR_UNSUPPORTED_N: return "unsupported d_state: N must be a multiple of 4 in [4, 64]";
     case MMS_ERR_WORKSPACE: return "workspace missing or smaller than the entry point's size function says";
-    case MMS_ERR_MISALIGNED: return "misaligned pointer (B, C, Aneg, ckpt, dB, dC, dAneg need 16 bytes)";
+    case MMS_ERR_MISALIGNED: return "misaligned pointer (the scan's B, C, Aneg, ckpt, dB, dC, dAneg and the head's x, w, kept, dx, "
+                                   "dw need 16 bytes, workspaces 256, everything else its element's size)";
     case MMS_ERR_CUDA: return "CUDA call failed (mms_last_cuda_error() names the CUDA error)";
     case MMS_ERR_TIMEOUT: return "a kernel timed out waiting for its staged copies (results invalid)";
     case MMS_ERR_UNSUPPORTED_BF16:

@@ -1,4 +1,5 @@
-"""What the head's losses ask for beside their inputs: bounded in the vocabulary, linear in the rows."""
+"""What the head's losses ask for beside their inputs: bounded in the vocabulary, linear in the rows;
+and what they say of an array that is not aligned."""
 from __future__ import annotations
 
 import pytest
@@ -6,6 +7,11 @@ import pytest
 from mamba_metal import _native
 
 MB = 1 << 20
+
+
+def test_the_misaligned_status_names_the_heads_arrays():
+    text = _native.status_string(_native.MMS_ERR_MISALIGNED)
+    assert all(word in text for word in ("x, w, kept, dx, dw", "Aneg", "workspace"))
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
