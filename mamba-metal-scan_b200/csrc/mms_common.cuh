@@ -9,9 +9,6 @@
 
 namespace mms {
 
-// 2^x on the MUFU pipe (ex2.approx.ftz.f32). The scan feeds it -dt*Aneg*log2(e),
-// which is <= 0, so the result lies in [0, 1]; flushing denormal results to
-// zero only affects states that have already decayed below 1e-38.
 // In every kernel that launch_chained() starts, before it reads or writes memory: the
 // next one may be set up now (chain_next), and all kernels ahead are complete (chain_wait).
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
@@ -21,6 +18,9 @@ __device__ __forceinline__ void chained() {
     chain_wait();
 }
 
+// 2^x on the MUFU pipe (ex2.approx.ftz.f32). The scan feeds it -dt*Aneg*log2(e),
+// which is <= 0, so the result lies in [0, 1]; flushing denormal results to
+// zero only affects states that have already decayed below 1e-38.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -54,7 +54,7 @@ struct MmArgs {
     // fills a last step (64 elements) or tile (256 rows; MM_GRAD writes those
     // rows, as zeros where rs is 0).
     const int *live;
-    const int *row_of;          // row m's place in target and (not beside `acc` or split) in out; null: m
+    const int *row_of;          // row m's place in target and in out (not in `acc`, nor in partial sums); null: m
     float c;
     const float *row_mul, *mul;
     float2 *part;               // MM_LSE
