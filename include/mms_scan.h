@@ -58,7 +58,10 @@ extern "C" {
 #define MMS_ERR_UNSUPPORTED_BF16 8 /* the bf16 entry points need D % 8 == 0, and K == 8
                                       for the backward                                   */
 
-/* Version of the ABI in this header (major * 100 + minor). */
+/* Version of the ABI in this header (major * 100 + minor). The losses of the
+ * head and the residual norm (mms_head_*, mms_linear_*, mms_norm_*) came after
+ * the first libraries of 105 and did not raise it: a caller that may meet one
+ * of those looks them up by name. */
 #define MMS_ABI_VERSION 105
 int mms_abi_version(void);
 
