@@ -58,6 +58,10 @@ class MambaConfig:
     dt_min: float = 0.001
     dt_max: float = 0.1
     norm_eps: float = 1e-6
+    # The two below call the operators with the modules' parameters, not the modules: with fuse_norm
+    # the blocks', their norms' and ln_f's forward (the first norm's aside), with fuse_loss and in
+    # distill_loss the head's does not run, nor do hooks and wrappers on them (sharding or
+    # checkpointing by module).
     fuse_norm: bool = False   # residual sum + next norm as one CUDA kernel each way (residual_rms_norm)
     fuse_loss: bool = False   # with targets: no logits, forward returns (None, loss) (linear_cross_entropy)
 
