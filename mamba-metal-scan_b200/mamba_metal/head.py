@@ -37,30 +37,41 @@ def _reduce(rows, counts, reduction: str):
     return rows.sum() / counts.sum() if reduction == "mean" else rows.sum()
 
 
+def _logits(x, weight, counts):
+    """x W^T, float32 at least, with zeros for the rows that do not count, whatever x holds there."""
+    z = F.linear(torch.where(counts[..., None], x, torch.zeros((), dtype=x.dtype, device=x.device)), weight)
+    return z.float() if x.dtype in (torch.bfloat16, torch.float16) else z
+
+
+def _loud(values, bad):
+    """values, NaN with NaN gradients where bad."""
+    return values * torch.where(bad, float("nan"), 1.0).to(values.dtype)
+
+
 def linear_cross_entropy_ref(x, weight, target, ignore_index: int = -100, reduction: str = "mean"):
     """linear_cross_entropy in PyTorch ops, with the logits (any device and float type)."""
-    logits = F.linear(x, weight).float() if x.dtype in (torch.bfloat16, torch.float16) \
-        else F.linear(x, weight)
-    loss = F.cross_entropy(logits.reshape(-1, weight.shape[0]), target.reshape(-1).long(),
-                           ignore_index=ignore_index, reduction=reduction)
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    vocab, target = weight.shape[0], target.long()
+    counts = target != ignore_index
+    rows = F.cross_entropy(_logits(x, weight, counts).reshape(-1, vocab), target.clamp(0, vocab - 1).reshape(-1),
+                           reduction="none").reshape(target.shape)
+    rows = torch.where(counts, _loud(rows, counts & ((target < 0) | (target >= vocab))), torch.zeros_like(rows))
+    return _reduce(rows, counts, reduction)
 
 
 def linear_distillation_ref(x, weight, teacher_index, teacher_logits, temperature: float = 1.0,
                             reduction: str = "mean"):
     """linear_distillation in PyTorch ops, with the logits (any device and float type)."""
-    logits = F.linear(x, weight)
-    if x.dtype in (torch.bfloat16, torch.float16):
-        logits = logits.float()
-    index = teacher_index.long()
+    index, vocab = teacher_index.long(), weight.shape[0]
     valid = index >= 0
-    t = (teacher_logits.to(logits.dtype) / temperature).masked_fill(~valid, float("-inf"))
+    dtype = x.dtype if x.dtype == torch.float64 else torch.float32
+    t = (teacher_logits.to(dtype) / temperature).masked_fill(~valid, float("-inf"))
     some = ~(t == float("-inf")).all(-1)
+    logits = _logits(x, weight, some)
     # a row without entries gets a finite stand-in, then probability 0 everywhere
     log_p = torch.log_softmax(t.masked_fill(~some[..., None], 0.0), -1)
     p = torch.where(some[..., None] & valid, log_p.exp(), torch.zeros_like(log_p))
-    log_q = torch.log_softmax(logits / temperature, -1).gather(-1, index.clamp(min=0))
-    terms = torch.where(p == 0, torch.zeros_like(p), p * (log_p - log_q))
+    log_q = torch.log_softmax(logits / temperature, -1).gather(-1, index.clamp(0, vocab - 1))
+    terms = torch.where(p == 0, torch.zeros_like(p), p * (log_p - _loud(log_q, (p != 0) & (index >= vocab))))
     rows = torch.where(some, temperature ** 2 * terms.sum(-1), torch.zeros_like(terms[..., 0]))
     return _reduce(rows, some, reduction)
 
@@ -187,7 +198,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     x (..., D), weight (V, D), target (...) integers. Rows whose target is
     ignore_index have loss and gradient 0, whatever x holds there, and do not
-    count in the mean (which is NaN if no row counts). A target outside
+    count in the mean (which is NaN if no row counts, with gradients 0). A target outside
     [0, V) that is not ignore_index gives a NaN loss and NaN gradients.
     reduction 'mean', 'sum' or 'none' (target's shape); the loss is float32.
     Differentiable once, with respect to x and weight.
