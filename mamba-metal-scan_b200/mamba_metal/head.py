@@ -50,12 +50,11 @@ def _loud(values, bad):
 
 def linear_cross_entropy_ref(x, weight, target, ignore_index: int = -100, reduction: str = "mean"):
     """linear_cross_entropy in PyTorch ops, with the logits (any device and float type)."""
-    vocab, target = weight.shape[0], target.long()
-    counts = target != ignore_index
-    rows = F.cross_entropy(_logits(x, weight, counts).reshape(-1, vocab), target.clamp(0, vocab - 1).reshape(-1),
-                           reduction="none").reshape(target.shape)
-    rows = torch.where(counts, _loud(rows, counts & ((target < 0) | (target >= vocab))), torch.zeros_like(rows))
-    return _reduce(rows, counts, reduction)
+    vocab, index = weight.shape[0], target.reshape(-1).long()
+    counts = index != ignore_index
+    rows = F.cross_entropy(_logits(x.reshape(-1, x.shape[-1]), weight, counts), index.clamp(0, vocab - 1), reduction="none")
+    rows = torch.where(counts, _loud(rows, counts & ((index < 0) | (index >= vocab))), torch.zeros_like(rows))
+    return _reduce(rows.reshape(target.shape), counts, reduction)
 
 
 def linear_distillation_ref(x, weight, teacher_index, teacher_logits, temperature: float = 1.0,

@@ -76,3 +76,8 @@ def test_indices_outside_the_vocabulary(bad, device):
         assert torch.isnan(dx[2]).all() and torch.isfinite(dx[rest]).all() and torch.isnan(dw).all()
     logits[2, 1] = float("-inf")                        # probability 0: counts for nothing
     assert all(torch.isfinite(t).all() for t in run(cases[1], x, w))
+
+
+def test_flat_targets_beside_a_batch():
+    x, w, target, *_ = problem("cpu", (2, 3))
+    assert torch.equal(linear_cross_entropy(x, w, target.reshape(-1)), linear_cross_entropy(x, w, target))
