@@ -130,11 +130,12 @@ def _as(t, dtype):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _no_rows(x, shape, reduction):
-    """The loss of no rows (0 / 0 for a mean), part of x's graph."""
+def _no_rows(x, weight, shape, reduction):
+    """The loss of no rows (0 / 0 for a mean), part of x's and weight's graph."""
+    nothing = weight[:0].float().sum()
     if reduction == "none":
-        return x.float().sum(-1).reshape(shape)
-    s = x.float().sum()
+        return x.float().sum(-1).reshape(shape) + nothing
+    s = x.float().sum() + nothing
     return s / 0.0 if reduction == "mean" else s
 
 
@@ -209,7 +210,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if target.shape != x.shape[:-1]:
         raise ValueError(f"target {tuple(target.shape)} does not match x {tuple(x.shape)}")
     if target.numel() == 0:
-        return _no_rows(x, target.shape, reduction)
+        return _no_rows(x, weight, target.shape, reduction)
     x2, w2 = _rows(x), _rows(weight)
     t = _as(_flat(target, -1), torch.int64)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
@@ -255,7 +256,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: to
         raise RuntimeError(f"teacher_logits must be floating point; got {teacher_logits.dtype}")
     lead = x.shape[:-1]
     if teacher_index.numel() == 0:
-        return _no_rows(x, lead, reduction)
+        return _no_rows(x, weight, lead, reduction)
     x2, w2 = _rows(x), _rows(weight)
     index = _as(_flat(teacher_index, -1, k), torch.int64)
     logits = _as(_flat(teacher_logits.detach(), -1, k), torch.float32)
