@@ -41,16 +41,18 @@
 // bf16 backward: dz needs more bits than bf16's 8 beside the result's own
 // rounding. Above FEW_ROWS rows it is one plane of scaled fp16 (2^-11 of a value
 // at most; in bf16, 2^-8, gradients were 14 to 37 % further from float64 than
-// their own rounding, now 1 %), and x and w follow it into fp16, scaled by powers of two, which
-// holds a bf16 value exactly down to 2^-31 of the largest: r = M E with E a
-// power of two and M in [1, 2),
+// their own rounding, now 1 %), and x and w follow it into fp16, scaled by
+// powers of two, which holds a bf16 value exactly down to 2^-31 of the largest:
+// r = M E with E a power of two and M in [1, 2),
 //   dz = 2^14 M (q - p),  dx = E dz w,  dw = dz^T (E x)
 // so that dz is all that is rounded; below 2^-28 it loses bits to fp16's range
-// (2^-39 absolute). The price is w's copy and maximum: 8192 x 131072 x 2048
-// 15.4 -> 15.6 ms, 1000 x 50021 x 1001 with unaligned rows 464 -> 482 us. Up to FEW_ROWS rows, where w's bytes are what counts, w is taken as it
-// is and dz is two planes of bf16 (2^-17; a pass of the tensor cores more that
-// such sizes do not feel): without r where it is the same for all rows (mean,
-// sum), as r (q - p) where it is not.
+// (2^-39 absolute). The price is w's copy and maximum (against one plane of
+// bf16: 512 x 65536 x 2048 507 -> 650 us, 2048 rows 1.80 -> 1.95 ms, 8192 x 131072
+// x 2048 15.4 -> 15.6; unaligned rows, copied anyway, 1000 x 50021 x 1001 504 ->
+// 540). Up to FEW_ROWS rows, where w's bytes are what counts, w is taken as it is
+// and dz is two planes of bf16 (2^-17; one more pass of two products): without r
+// where it is the same for all rows (mean, sum), as r (q - p) where it is not. At
+// 257 rows of 65536 x 2048 that takes 613 us, fp16 618; at 512 rows 730 and 650.
 //
 // float32: factors are split into two fp16 planes, 22 bits, after a scaling by
 // a power of two that brings the largest element into [2^14, 2^15); the
