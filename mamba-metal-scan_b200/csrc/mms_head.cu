@@ -48,7 +48,7 @@
 // so that dz is all that is rounded; below 2^-28 it loses bits to fp16's range
 // (2^-39 absolute). The price is w's copy and maximum (against one plane of
 // bf16: 512 x 65536 x 2048 507 -> 650 us, 2048 rows 1.80 -> 1.95 ms, 8192 x 131072
-// x 2048 15.4 -> 15.6; unaligned rows, copied anyway, 1000 x 50021 x 1001 504 ->
+// x 2048 15.5 -> 16.0; unaligned rows, copied anyway, 1000 x 50021 x 1001 504 ->
 // 540). Up to FEW_ROWS rows, where w's bytes are what counts, w is taken as it is
 // and dz is two planes of bf16 (2^-17; one more pass of two products): without r
 // where it is the same for all rows (mean, sum), as r (q - p) where it is not. At
