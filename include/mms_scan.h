@@ -321,6 +321,93 @@ int mms_norm_bwd(const void *x, const void *y, const void *gate, long long ldg, 
                  int dtype, void *stream);
 
 /*
+ * Short depthwise causal convolution, with SiLU (silu != 0) or without:
+ *     pre[b,t,d] = bias[d] + sum_k w[d,k] x[b, t-K+1+k, d]   (x = 0 before t = 0)
+ *     y = pre * sigmoid(pre), or pre
+ * x has element (b, t, d) at x[b*ldb + t*ldt + d]; y, dy, dx (Bt, T, D), w, dw
+ * (D, K), bias, dbias (D; NULL: none) are contiguous, all of storage type dtype
+ * (MMS_F32 or MMS_BF16), arithmetic and sums in float32, sums in a
+ * fixed order. 1 <= K <= MMS_CONV_MAX_K. The backward's workspace has
+ * mms_conv_workspace_size() bytes (256-byte aligned). Arrays need their
+ * element's alignment; 4 of them (and strides and D a multiple of 4) for full speed.
+ * Sizes above MMS_SERVE_MAX and MMS_SERVE_MAX_DIM are refused here and below.
+ * No counterpart in the reference (a transposed nn.Conv1d and F.silu there,
+ * mamba_metal/model.py:175-177, 214-219).
+ */
+#define MMS_CONV_MAX_K 8
+#define MMS_SERVE_MAX (1 << 30)      /* Bt * T, rows, count, places, and vocab of mms_sample */
+#define MMS_SERVE_MAX_DIM (1 << 24)  /* D */
+size_t mms_conv_workspace_size(int Bt, int T, int D, int K);
+int mms_conv_fwd(const void *x, long long ldb, long long ldt, const void *w, const void *bias,
+                 void *y, int Bt, int T, int D, int K, int silu, int dtype, void *stream);
+int mms_conv_bwd(const void *x, long long ldb, long long ldt, const void *w, const void *bias,
+                 const void *dy, void *dx, void *dw, void *dbias, void *workspace,
+                 size_t workspace_bytes, int Bt, int T, int D, int K, int silu, int dtype,
+                 void *stream);
+
+/*
+ * Packed sequences: `count` sequences behind one another in `rows` rows, sequence
+ * s in rows starts[s] .. starts[s+1]-1 (count + 1 ascending numbers within [0,
+ * rows]; NULL: count == rows, row s alone). What a sequence goes on from lies in
+ * place slots[s] of a cache of `places`, what it leaves goes to place
+ * out_slots[s]; slots NULL: place s; out_slots NULL: slots; a place outside
+ * the cache (-1, say): from nothing, and nowhere. A place that one sequence writes
+ * is neither read nor written by another of the same call (several may read
+ * one). Places that no sequence writes stay as they are; rows of no sequence get
+ * zeros in y. The lists hold 32-bit numbers, or 64-bit ones where `wide` has
+ * MMS_WIDE_STARTS, MMS_WIDE_SLOTS, MMS_WIDE_OUT_SLOTS. They are read on the device:
+ * a list that is not as described gives wrong rows, but no access outside the arrays.
+ *
+ * mms_conv_packed: the convolution above; the cache is `window` (places, D, K-1), the
+ * last K-1 inputs, oldest first (zeros before the first), in x's type. x (rows, D)
+ * with row stride ldx, y (rows, D) contiguous.
+ *
+ * mms_scan_packed: the selective scan, state (places, D, N) float32; x, dt, z
+ * (rows, D) and y (contiguous) of type dtype, B and C (rows, N) of type bc_dtype (with dtype
+ * MMS_F32: MMS_F32), each with its row stride; aneg (D, N), d_skip (D)
+ * float32. y = (scan + d_skip) * silu(z), each where it is given. raw != 0: dt
+ * holds logits and aneg the raw A, as in mms_fwd_proj. aneg, state and the
+ * workspace 16-byte aligned; without starts B and C 4 elements aligned, strides
+ * too. Workspace: mms_scan_packed_workspace_size() bytes (0 without starts).
+ *
+ * No counterpart in the reference, whose cache goes on by single tokens of one
+ * batch (mamba_metal/model.py:203-241).
+ */
+#define MMS_WIDE_STARTS 1
+#define MMS_WIDE_SLOTS 2
+#define MMS_WIDE_OUT_SLOTS 4
+int mms_conv_packed(const void *x, long long ldx, const void *w, const void *bias, void *window,
+                    int places, const void *starts, const void *slots, const void *out_slots,
+                    int wide, void *y, int rows, int count, int D, int K, int silu, int dtype,
+                    void *stream);
+size_t mms_scan_packed_workspace_size(int rows, int count, int D, int N);
+int mms_scan_packed(const void *x, long long ldx, const void *dt, long long lddt, const float *aneg,
+                    const void *B, long long ldB, const void *C, long long ldC, const void *z,
+                    long long ldz, const float *d_skip, int raw, float dt_min, float dt_max,
+                    float *state, int places, const void *starts, const void *slots,
+                    const void *out_slots, int wide, void *y, void *workspace,
+                    size_t workspace_bytes, int rows, int count, int D, int N, int dtype,
+                    int bc_dtype, void *stream);
+
+/*
+ * One token from each row of logits (rows, vocab), row stride ld, type dtype:
+ *     w_i = exp((z_i - max z) / temperature), of the top_k largest z (0 or less: all)
+ *     of those the shortest run, largest first, whose weight is >= top_p of theirs
+ *     of those the ones with w_i >= min_p
+ *     token: the first i in index order whose weights up to it pass uniform[row] * their sum
+ * Equal logits rank by lowest index. Settings come from device arrays of one value a row
+ * or, where those are NULL, from the value behind them; top_k from 64-bit
+ * numbers if top_k_wide. temperature <= 0: the largest logit. A row with a
+ * NaN, or without a logit above -inf, gives -1. logprob (NULL: not wanted): the log of
+ * w_token over their sum, NaN beside -1. Weights and sums are float64.
+ * No counterpart in the reference.
+ */
+int mms_sample(const void *logits, long long ld, const float *uniform, const float *temperature,
+               float temperature1, const void *top_k, int top_k_wide, long long top_k1,
+               const float *top_p, float top_p1, const float *min_p, float min_p1, int64_t *token,
+               float *logprob, int rows, int vocab, int dtype, void *stream);
+
+/*
  * Device-side status of the kernels launched so far, for failure detection.
  * The backward's TMA staging waits on completion barriers with a bounded
  * poll; a wait that runs out records a flag instead of hanging the GPU (the

@@ -12,6 +12,7 @@
 #include "mms_head.h"
 #include "mms_kernels.h"
 #include "mms_scan.h"
+#include "mms_serve.h"
 
 namespace {
 
@@ -147,6 +148,37 @@ int check_norm(const void *x, const void *y, const void *gate, long long ldg, co
 
 std::atomic<uint32_t> g_wait_limit{0};
 std::atomic<int> g_skip_item{-1};
+
+int check_dtype(int dtype) { return dtype == MMS_F32 || dtype == MMS_BF16 ? MMS_OK : MMS_ERR_INVALID_ARG; }
+
+int check_conv_sizes(int Bt, int T, int D, int K)
+{
+    return Bt < 1 || T < 1 || D < 1 || K < 1 || K > MMS_CONV_MAX_K || (long long)Bt * T > MMS_SERVE_MAX ||
+                   D > MMS_SERVE_MAX_DIM
+               ? MMS_ERR_INVALID_ARG
+               : MMS_OK;
+}
+
+int check_packed(int rows, int count, int places, int D, const void *starts, const void *slots,
+                 const void *out_slots, int wide)
+{
+    if (rows < 1 || count < 1 || places < 1 || D < 1 || rows > MMS_SERVE_MAX || count > MMS_SERVE_MAX ||
+        places > MMS_SERVE_MAX || D > MMS_SERVE_MAX_DIM || (!starts && rows != count))
+        return MMS_ERR_INVALID_ARG;
+    if (!aligned(starts, wide & MMS_WIDE_STARTS ? 8 : 4) || !aligned(slots, wide & MMS_WIDE_SLOTS ? 8 : 4) ||
+        !aligned(out_slots, wide & MMS_WIDE_OUT_SLOTS ? 8 : 4))
+        return MMS_ERR_MISALIGNED;
+    return MMS_OK;
+}
+
+mms::Sequences sequences(int rows, int count, int places, const void *starts, const void *slots,
+                         const void *out_slots, int wide)
+{
+    return {{starts, (wide & MMS_WIDE_STARTS) != 0},
+            {slots, (wide & MMS_WIDE_SLOTS) != 0},
+            {out_slots, (wide & MMS_WIDE_OUT_SLOTS) != 0},
+            count, rows, places};
+}
 
 }  // namespace
 
@@ -426,6 +458,129 @@ int mms_norm_bwd(const void *x, const void *y, const void *gate, long long ldg, 
     a.workspace = workspace;
     a.rows = rows; a.dim = dim; a.bf16 = dtype == MMS_BF16;
     return status_of(mms::launch_norm_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t mms_conv_workspace_size(int Bt, int T, int D, int K)
+{
+    return check_conv_sizes(Bt, T, D, K) ? 0 : mms::conv_workspace_bytes(Bt, T, D, K);
+}
+
+int mms_conv_fwd(const void *x, long long ldb, long long ldt, const void *w, const void *bias,
+                 void *y, int Bt, int T, int D, int K, int silu, int dtype, void *stream)
+{
+    int rc = check_conv_sizes(Bt, T, D, K);
+    if (rc || (rc = check_dtype(dtype))) return rc;
+    if (!x || !w || !y || ldb < 0 || ldt < 0) return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    if (!aligned(x, e) || !aligned(w, e) || !aligned(bias, e) || !aligned(y, e)) return MMS_ERR_MISALIGNED;
+    mms::ConvArgs a{};
+    a.x = x; a.ldb = ldb; a.ldt = ldt; a.w = w; a.bias = bias; a.y = y;
+    a.Bt = Bt; a.T = T; a.D = D; a.K = K; a.silu = silu != 0; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_conv_fwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int mms_conv_bwd(const void *x, long long ldb, long long ldt, const void *w, const void *bias,
+                 const void *dy, void *dx, void *dw, void *dbias, void *workspace,
+                 size_t workspace_bytes, int Bt, int T, int D, int K, int silu, int dtype,
+                 void *stream)
+{
+    int rc = check_conv_sizes(Bt, T, D, K);
+    if (rc || (rc = check_dtype(dtype))) return rc;
+    if (!x || !w || !dy || !dx || !dw || ldb < 0 || ldt < 0) return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    if (!aligned(x, e) || !aligned(w, e) || !aligned(bias, e) || !aligned(dy, e) || !aligned(dx, e) ||
+        !aligned(dw, e) || !aligned(dbias, e))
+        return MMS_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < mms::conv_workspace_bytes(Bt, T, D, K)) return MMS_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return MMS_ERR_MISALIGNED;
+    mms::ConvArgs a{};
+    a.x = x; a.ldb = ldb; a.ldt = ldt; a.w = w; a.bias = bias; a.dy = dy;
+    a.dx = dx; a.dw = dw; a.dbias = dbias; a.part = static_cast<float *>(workspace);
+    a.Bt = Bt; a.T = T; a.D = D; a.K = K; a.silu = silu != 0; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_conv_bwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int mms_conv_packed(const void *x, long long ldx, const void *w, const void *bias, void *window,
+                    int places, const void *starts, const void *slots, const void *out_slots,
+                    int wide, void *y, int rows, int count, int D, int K, int silu, int dtype,
+                    void *stream)
+{
+    int rc = check_packed(rows, count, places, D, starts, slots, out_slots, wide);
+    if (rc || (rc = check_dtype(dtype))) return rc;
+    if (K < 1 || K > MMS_CONV_MAX_K || !x || !w || (!window && K > 1) || !y || ldx < 0) return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4;
+    if (!aligned(x, e) || !aligned(w, e) || !aligned(bias, e) || !aligned(window, e) || !aligned(y, e))
+        return MMS_ERR_MISALIGNED;
+    mms::ConvPackedArgs a{};
+    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.window = window; a.y = y;
+    a.seq = sequences(rows, count, places, starts, slots, out_slots, wide);
+    a.D = D; a.K = K; a.silu = silu != 0; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_conv_packed(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t mms_scan_packed_workspace_size(int rows, int count, int D, int N)
+{
+    if (rows < 1 || count < 1 || D < 1 || N < 4 || N > 64 || N % 4 || rows > MMS_SERVE_MAX || D > MMS_SERVE_MAX_DIM) return 0;
+    return mms::scan_packed_workspace_bytes(rows, count, D, N);
+}
+
+int mms_scan_packed(const void *x, long long ldx, const void *dt, long long lddt, const float *aneg,
+                    const void *B, long long ldB, const void *C, long long ldC, const void *z,
+                    long long ldz, const float *d_skip, int raw, float dt_min, float dt_max,
+                    float *state, int places, const void *starts, const void *slots,
+                    const void *out_slots, int wide, void *y, void *workspace,
+                    size_t workspace_bytes, int rows, int count, int D, int N, int dtype,
+                    int bc_dtype, void *stream)
+{
+    if (N < 4 || N > 64 || N % 4 != 0) return MMS_ERR_UNSUPPORTED_N;
+    int rc = check_packed(rows, count, places, D, starts, slots, out_slots, wide);
+    if (rc || (rc = check_dtype(dtype)) || (rc = check_dtype(bc_dtype))) return rc;
+    if (dtype == MMS_F32 && bc_dtype != MMS_F32) return MMS_ERR_INVALID_ARG;
+    if (!x || !dt || !aneg || !B || !C || !state || !y || ldx < 0 || lddt < 0 || ldB < 0 || ldC < 0 || ldz < 0)
+        return MMS_ERR_INVALID_ARG;
+    if (raw && !proj_ok(dt_min, dt_max)) return MMS_ERR_INVALID_ARG;
+    const uintptr_t e = dtype == MMS_BF16 ? 2 : 4, be = bc_dtype == MMS_BF16 ? 2 : 4;
+    const uintptr_t group = starts ? 1 : 4;                // single tokens read B and C four at a time
+    if (!aligned(x, e) || !aligned(dt, e) || !aligned(z, e) || !aligned(y, e) || !aligned(aneg, 16) ||
+        !aligned(state, 16) || !aligned(d_skip, 4) || !aligned(B, group * be) || !aligned(C, group * be) ||
+        ldB % (long long)group || ldC % (long long)group)
+        return MMS_ERR_MISALIGNED;
+    if (starts) {
+        const size_t need = mms::scan_packed_workspace_bytes(rows, count, D, N);
+        if (need && (!workspace || workspace_bytes < need)) return MMS_ERR_WORKSPACE;
+        if (!aligned(workspace, 16)) return MMS_ERR_MISALIGNED;
+    }
+    mms::ScanPackedArgs a{};
+    a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z;
+    a.ldx = ldx; a.lddt = lddt; a.ldB = ldB; a.ldC = ldC; a.ldz = ldz;
+    a.aneg = aneg; a.d_skip = d_skip; a.state = state; a.y = y; a.workspace = workspace;
+    a.seq = sequences(rows, count, places, starts, slots, out_slots, wide);
+    a.D = D; a.N = N; a.bf16 = dtype == MMS_BF16; a.bc_bf16 = bc_dtype == MMS_BF16;
+    a.proj = raw ? mms::Proj{1, dt_min, dt_max - dt_min, 1.f / (dt_max - dt_min)} : mms::Proj{0, 0.f, 0.f, 0.f};
+    return status_of(mms::launch_scan_packed(a, static_cast<cudaStream_t>(stream)));
+}
+
+int mms_sample(const void *logits, long long ld, const float *uniform, const float *temperature,
+               float temperature1, const void *top_k, int top_k_wide, long long top_k1,
+               const float *top_p, float top_p1, const float *min_p, float min_p1, int64_t *token,
+               float *logprob, int rows, int vocab, int dtype, void *stream)
+{
+    const int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (rows < 1 || vocab < 1 || rows > MMS_HEAD_MAX_ROWS || vocab > MMS_SERVE_MAX || !logits || !uniform || !token || ld < 0)
+        return MMS_ERR_INVALID_ARG;
+    if (!aligned(logits, dtype == MMS_BF16 ? 2 : 4) || !aligned(uniform, 4) || !aligned(temperature, 4) ||
+        !aligned(top_k, top_k_wide ? 8 : 4) || !aligned(top_p, 4) || !aligned(min_p, 4) || !aligned(token, 8) ||
+        !aligned(logprob, 4))
+        return MMS_ERR_MISALIGNED;
+    mms::SampleArgs a{};
+    a.logits = logits; a.ld = ld; a.uniform = uniform;
+    a.temperature = temperature; a.temperature1 = temperature1;
+    a.top_k = mms::Ints{top_k, top_k_wide != 0}; a.top_k1 = top_k1;
+    a.top_p = top_p; a.top_p1 = top_p1; a.min_p = min_p; a.min_p1 = min_p1;
+    a.token = token; a.logprob = logprob;
+    a.rows = rows; a.vocab = vocab; a.bf16 = dtype == MMS_BF16;
+    return status_of(mms::launch_sample(a, static_cast<cudaStream_t>(stream)));
 }
 
 int mms_device_status(void)

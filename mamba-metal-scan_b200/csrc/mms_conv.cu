@@ -1,0 +1,475 @@
+// Short depthwise causal convolution with SiLU for sm_100a, forward, backward
+// and over packed sequences with their last inputs kept in a cache.
+//
+//     pre[t, d] = bias[d] + sum_k w[d, k] x[t - K + 1 + k, d]      y = pre * sigmoid(pre), or pre
+//     ds = dy * act'(pre),   dx[t] = sum_k w[k] ds[t + K - 1 - k],
+//     dw[k] = sum_t ds[t] x[t - K + 1 + k],   dbias = sum_t ds[t]
+//
+// All of it is bound by HBM: a few FMAs an element beside x and y (forward, 2
+// elements moved), x, dy and dx (backward, 3). The reference transposes to
+// channels first, calls a convolution and a SiLU and transposes back (reference
+// mamba_metal/model.py:175-177, 214-219); here rows stay as they are in memory,
+// channels innermost: a thread owns VEC neighbouring channels, a warp 32 * VEC,
+// so that every access is a whole line, and x may be a view with strides (a half
+// of in_proj's output).
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "mms_common.cuh"
+#include "mms_serve.h"
+
+namespace mms {
+
+namespace {
+
+constexpr int WARPS = 4;                // per CTA, each with rows of its own and the same channels
+constexpr int THREADS = 32 * WARPS;
+constexpr int FWD_ROWS = 8;             // rows of a warp's tile, all loaded before the first is used
+constexpr int BWD_STEP = 4;             // rows the backward loads at once
+
+template <typename E, int VEC>
+struct alignas(sizeof(E) * VEC) Pack {
+    E v[VEC];
+};
+
+template <typename E, int VEC>
+__device__ __forceinline__ Pack<E, VEC> load(const E *p) {
+    return *reinterpret_cast<const Pack<E, VEC> *>(p);
+}
+template <typename E, int VEC>
+__device__ __forceinline__ void store(E *p, const float (&v)[VEC]) {
+    Pack<E, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_f<E>(v[i]);
+    *reinterpret_cast<Pack<E, VEC> *>(p) = o;
+}
+template <typename E, int VEC>
+__device__ __forceinline__ Pack<E, VEC> nothing() {
+    Pack<E, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_f<E>(0.f);
+    return o;
+}
+
+// sigmoid(v) = 1 / (1 + e^-v) on MUFU's ex2 and reciprocal
+__device__ __forceinline__ float act(float v, bool silu) { return silu ? v * sigmoid_fast(v) : v; }
+
+// A channel group's taps. KT: taps the code is unrolled for; with fewer of them
+// (K < KT) the first KT - K stand for none and are skipped, not multiplied by zero:
+// an infinite input there must not turn into a NaN.
+template <typename E, int KT, int VEC>
+struct Taps {
+    float w[KT][VEC], bias[VEC];
+    __device__ __forceinline__ void read(const E *wp, const E *bp, int d, int K) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            bias[i] = bp ? to_f(bp[d + i]) : 0.f;
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+                w[k][i] = k >= KT - K ? to_f(wp[(long long)(d + i) * K + k - (KT - K)]) : 0.f;
+        }
+    }
+    // the sum over rows x[0 .. KT - 1]
+    template <typename Row>
+    __device__ __forceinline__ void sum(float (&acc)[VEC], int K, Row row) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = bias[i];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+            if (k >= KT - K) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[k][i], row(k, i), acc[i]);
+            }
+    }
+};
+
+// K as the code knows it: KT itself where the kernel is for exactly KT taps.
+template <int KT, bool EXACT>
+__device__ __forceinline__ int taps_of(int K) { return EXACT ? KT : K; }
+
+// ---------------------------------------------------------------- forward
+
+template <typename E, int KT, bool EXACT, int VEC>
+__global__ void __launch_bounds__(THREADS)
+conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
+                const E *__restrict__ bias, E *__restrict__ y, int T, int D, int K_in, bool silu, int nd, int nt)
+{
+    const int K = taps_of<KT, EXACT>(K_in);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int blk = blockIdx.x;                            // (b, tile, channel block), the last fastest
+    const int d = (blk % nd) * 32 * VEC + lane * VEC;
+    const int tile = blk / nd % nt, b = blk / nd / nt;
+    const int t0 = (tile * WARPS + warp) * FWD_ROWS;
+    if (d >= D || t0 >= T) return;
+    const E *xb = x + b * ldb + d;
+    Pack<E, VEC> xs[FWD_ROWS + KT - 1];
+#pragma unroll
+    for (int j = 0; j < FWD_ROWS + KT - 1; ++j) {
+        const int t = t0 - (KT - 1) + j;
+        xs[j] = t >= 0 && t < T ? load<E, VEC>(xb + t * ldt) : nothing<E, VEC>();
+    }
+    Taps<E, KT, VEC> taps;
+    taps.read(w, bias, d, K);
+    E *yb = y + ((long long)b * T + t0) * D + d;
+#pragma unroll
+    for (int r = 0; r < FWD_ROWS; ++r) {
+        float acc[VEC];
+        taps.sum(acc, K, [&](int k, int i) { return to_f(xs[r + k].v[i]); });
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
+        if (t0 + r < T) store<E, VEC>(yb + (long long)r * D, acc);
+    }
+}
+
+// --------------------------------------------------------------- backward
+
+// A warp walks `len` rows of one sequence, ds rolling through registers: after
+// ds[t] the row dx[t - KT + 1] is complete. The KT - 1 rows behind its own are
+// computed as well, for dx alone. dw and dbias stay in registers; the CTA's four
+// warps are joined in shared memory and leave one partial sum a CTA.
+template <typename E, int KT, bool EXACT, int VEC>
+__global__ void __launch_bounds__(THREADS)
+conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
+                const E *__restrict__ bias, const E *__restrict__ dy, E *__restrict__ dx,
+                float *__restrict__ part, int T, int D, int K_in, bool silu, int nd, int ns, int len)
+{
+    const int K = taps_of<KT, EXACT>(K_in);
+    __shared__ float sums[WARPS][KT + 1][VEC][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int blk = blockIdx.x;                            // (b, segment, channel block)
+    const int d = (blk % nd) * 32 * VEC + lane * VEC;
+    const int seg = blk / nd % ns, b = blk / nd / ns;
+    const int t0 = (seg * WARPS + warp) * len, t1 = min(T, t0 + len);
+    float dw[KT][VEC] = {}, db[VEC] = {};
+    if (d < D && t0 < T) {
+        const E *xb = x + b * ldb + d;
+        const E *gb = dy + (long long)b * T * D + d;
+        E *ob = dx + (long long)b * T * D + d;
+        Taps<E, KT, VEC> taps;
+        taps.read(w, bias, d, K);
+        Pack<E, VEC> xs[BWD_STEP + KT - 1];                // rows t - KT + 1 .. t + BWD_STEP - 1
+        float ds[BWD_STEP + KT - 1][VEC];
+#pragma unroll
+        for (int j = 0; j < KT - 1; ++j) {
+            const int t = t0 - (KT - 1) + j;
+            xs[j] = t >= 0 ? load<E, VEC>(xb + t * ldt) : nothing<E, VEC>();
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ds[j][i] = 0.f;
+        }
+        for (int t = t0; t < t1 + KT - 1; t += BWD_STEP) {
+            Pack<E, VEC> g[BWD_STEP];
+#pragma unroll
+            for (int u = 0; u < BWD_STEP; ++u) {
+                const bool in = t + u < T && t + u < t1 + KT - 1;
+                xs[KT - 1 + u] = in ? load<E, VEC>(xb + (t + u) * ldt) : nothing<E, VEC>();
+                g[u] = in ? load<E, VEC>(gb + (long long)(t + u) * D) : nothing<E, VEC>();
+            }
+#pragma unroll
+            for (int u = 0; u < BWD_STEP; ++u) {
+                float pre[VEC];
+                if (silu) taps.sum(pre, K, [&](int k, int i) { return to_f(xs[u + k].v[i]); });
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    float s = to_f(g[u].v[i]);
+                    if (silu) {
+                        const float sg = sigmoid_fast(pre[i]);
+                        s *= sg * fmaf(pre[i], 1.f - sg, 1.f);
+                    }
+                    ds[KT - 1 + u][i] = t + u < T ? s : 0.f;
+                }
+                if (t + u < t1) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        db[i] += ds[KT - 1 + u][i];
+#pragma unroll
+                        for (int k = 0; k < KT; ++k)
+                            dw[k][i] = fmaf(ds[KT - 1 + u][i], to_f(xs[u + k].v[i]), dw[k][i]);
+                    }
+                }
+                const int to = t + u - (KT - 1);
+                if (to >= t0 && to < t1) {
+                    float o[VEC] = {};
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+                        if (k >= KT - K) {
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) o[i] = fmaf(taps.w[k][i], ds[KT - 1 + u - k][i], o[i]);
+                        }
+                    store<E, VEC>(ob + (long long)to * D, o);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < KT - 1; ++j) {
+                xs[j] = xs[j + BWD_STEP];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) ds[j][i] = ds[j + BWD_STEP][i];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k) sums[warp][k][i][lane] = dw[k][i];
+        sums[warp][KT][i][lane] = db[i];
+    }
+    __syncthreads();
+    // part[(b, segment)][K + 1][D]
+    float *pb = part + (long long)(blk / nd) * (K + 1) * D + (blk % nd) * 32 * VEC;
+    const int left = D - (blk % nd) * 32 * VEC;
+    for (int o = threadIdx.x; o < (KT + 1) * VEC * 32; o += THREADS) {
+        const int c = o % (VEC * 32), k = o / (VEC * 32);
+        if (c >= left || k < KT - K) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) s += sums[q][k][c % VEC][c / VEC];
+        pb[(long long)(k - (KT - K)) * D + c] = s;
+    }
+}
+
+// dw (D, K) and dbias (D) from the partial sums, in a fixed order: row q of 8 takes
+// every eighth partial sum, then the rows are joined.
+template <typename E>
+__global__ void __launch_bounds__(256)
+conv_reduce_kernel(const float *__restrict__ part, E *__restrict__ dw, E *__restrict__ dbias, int parts, int D, int K)
+{
+    __shared__ float rows[8][32];
+    const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+    const int d = blockIdx.x * 32 + c, k = blockIdx.y;
+    float s = 0.f;
+    if (d < D)
+        for (int p = q; p < parts; p += 8) s += part[((long long)p * (K + 1) + k) * D + d];
+    rows[q][c] = s;
+    __syncthreads();
+    if (q == 0 && d < D) {
+        for (int r = 1; r < 8; ++r) s += rows[r][c];
+        if (k < K) dw[(long long)d * K + k] = from_f<E>(s);
+        else if (dbias) dbias[d] = from_f<E>(s);
+    }
+}
+
+// ----------------------------------------------------------------- packed
+
+// Packed sequences in one launch of two kinds of warps that write different rows,
+// so that none waits for another though the cache is updated in place:
+//   heads  (sequence, channel block): the outputs that still see the old window,
+//          rows 0 .. min(length, K - 1) - 1, and then the new window;
+//   tails  (8 rows, channel block): the rows at place K - 1 and later of their
+//          sequence, which depend on x alone; rows of no sequence get zeros.
+template <typename E, int KT, bool EXACT, int VEC>
+__global__ void __launch_bounds__(THREADS)
+conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__ w, const E *__restrict__ bias,
+                   E *__restrict__ window, E *__restrict__ y, Sequences seq, int D, int K_in, bool silu, int nd,
+                   long long heads, long long units)
+{
+    const int K = taps_of<KT, EXACT>(K_in);
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const int d = (int)(unit % nd) * 32 * VEC + lane * VEC;
+    if (unit < heads) {
+        if (d >= D) return;
+        const int s = (int)(unit / nd);
+        const int first = seq.start(s), end = seq.starts.p ? max(first, seq.start(s + 1)) : s + 1;
+        const int len = end - first;
+        const long long from = seq.from(s), to = seq.to(s);
+        const int K1 = K - 1;
+        // rows[0 .. KT - 2] the old window, then the first inputs
+        float rows[2 * (KT - 1) + 1][VEC];
+#pragma unroll
+        for (int j = 0; j < KT - 1; ++j) {
+            const int jw = j - (KT - K);                   // its place in the window
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                rows[j][i] = from >= 0 && jw >= 0 ? to_f(window[(from * D + d + i) * K1 + jw]) : 0.f;
+            const bool in = j < len && j < K1;
+            const Pack<E, VEC> v = in ? load<E, VEC>(x + (first + j) * ldx + d) : nothing<E, VEC>();
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) rows[KT - 1 + j][i] = to_f(v.v[i]);
+        }
+        if (to >= 0) {
+            // the last K - 1 of the window and the inputs behind it
+#pragma unroll
+            for (int j = 0; j < KT - 1; ++j) {
+                if (j >= K1) continue;
+                const int p = len - K1 + j;                // its row; below 0: in the old window
+                if (p >= 0) {
+                    const Pack<E, VEC> v = load<E, VEC>(x + (first + p) * ldx + d);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = v.v[i];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < KT - 1; ++q)       // (a constant index into the registers)
+                        if (q - (KT - K) == p + K1) {
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = from_f<E>(rows[q][i]);
+                        }
+                }
+            }
+        }
+        Taps<E, KT, VEC> taps;
+        taps.read(w, bias, d, K);
+#pragma unroll
+        for (int r = 0; r < KT - 1; ++r) {
+            if (r >= K1 || r >= len) continue;
+            float acc[VEC];
+            taps.sum(acc, K, [&](int k, int i) { return rows[r + k][i]; });
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
+            store<E, VEC>(y + (long long)(first + r) * D + d, acc);
+        }
+        return;
+    }
+    const int r0 = (int)((unit - heads) / nd) * FWD_ROWS;
+    Pack<E, VEC> xs[FWD_ROWS + KT - 1];
+#pragma unroll
+    for (int j = 0; j < FWD_ROWS + KT - 1; ++j) {
+        const int t = r0 - (KT - 1) + j;
+        xs[j] = d < D && t >= 0 && t < seq.rows ? load<E, VEC>(x + t * ldx + d) : nothing<E, VEC>();
+    }
+    // lane r finds row r0 + r: 0 a head's, 1 a tail's, 2 nobody's
+    int kind = 0;
+    if (lane < FWD_ROWS && r0 + lane < seq.rows) {
+        if (!seq.starts.p) kind = K == 1 ? 1 : 0;
+        else {
+            const int s = Sequences::last_at_most(seq.count + 1, r0 + lane, [&](int i) { return seq.start(i); });
+            kind = s < 0 || s >= seq.count ? 2 : r0 + lane - seq.start(s) >= K - 1 ? 1 : 0;
+        }
+    }
+    Taps<E, KT, VEC> taps;
+    if (d < D) taps.read(w, bias, d, K);
+#pragma unroll
+    for (int r = 0; r < FWD_ROWS; ++r) {
+        const int what = __shfl_sync(0xffffffffu, kind, r);
+        if (what == 0 || d >= D) continue;
+        float acc[VEC] = {};
+        if (what == 1) {
+            taps.sum(acc, K, [&](int k, int i) { return to_f(xs[r + k].v[i]); });
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
+        }
+        store<E, VEC>(y + (long long)(r0 + r) * D + d, acc);
+    }
+}
+
+// ------------------------------------------------------------------ launch
+
+// 4 channels a thread where every row starts at a whole group of 4: 16 (float32) or
+// 8 (bf16) bytes an access; one channel otherwise.
+template <typename E>
+bool groups_of_4(int D, std::initializer_list<const void *> arrays, std::initializer_list<long long> strides)
+{
+    bool ok = D % 4 == 0;
+    for (const void *p : arrays) ok = ok && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(E)) == 0;
+    for (long long s : strides) ok = ok && s % 4 == 0;
+    return ok;
+}
+
+// Rows a warp of the backward walks: as many as leave 8 CTAs an SM, so that the halo
+// of K - 1 rows and the partial sums stay small beside them; at least 16, at most 128.
+int bwd_rows(int Bt, int T, int D)
+{
+    const long long base = (long long)Bt * ((D + 127) / 128);
+    const long long want = std::max<long long>(1, 8LL * N_SM / base);
+    const long long len = (T + want * WARPS - 1) / (want * WARPS);
+    return (int)std::min<long long>(128, std::max<long long>(16, (len + BWD_STEP - 1) / BWD_STEP * BWD_STEP));
+}
+
+int bwd_segments(int T, int len) { return (T + WARPS * len - 1) / (WARPS * len); }
+
+// The kernels for 2, 3 and 4 taps are unrolled for exactly those; 1 and 5 to 8 taps
+// run one that is unrolled for 8.
+template <typename F>
+cudaError_t by_taps(int K, F f)
+{
+    switch (K) {
+    case 2: return f(std::integral_constant<int, 2>{}, std::true_type{});
+    case 3: return f(std::integral_constant<int, 3>{}, std::true_type{});
+    case 4: return f(std::integral_constant<int, 4>{}, std::true_type{});
+    default: return f(std::integral_constant<int, 8>{}, std::false_type{});
+    }
+}
+
+template <typename E, int VEC>
+cudaError_t fwd_of(const ConvArgs &a, cudaStream_t stream)
+{
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), nt = (a.T + WARPS * FWD_ROWS - 1) / (WARPS * FWD_ROWS);
+    const long long blocks = (long long)a.Bt * nt * nd;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return by_taps(a.K, [&](auto kt, auto exact) {
+        conv_fwd_kernel<E, decltype(kt)::value, decltype(exact)::value, VEC><<<(unsigned)blocks, THREADS, 0, stream>>>(
+            (const E *)a.x, a.ldb, a.ldt, (const E *)a.w, (const E *)a.bias, (E *)a.y, a.T, a.D, a.K, a.silu, nd, nt);
+        return cudaGetLastError();
+    });
+}
+
+template <typename E, int VEC>
+cudaError_t bwd_of(const ConvArgs &a, cudaStream_t stream)
+{
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), len = bwd_rows(a.Bt, a.T, a.D), ns = bwd_segments(a.T, len);
+    const long long blocks = (long long)a.Bt * ns * nd;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const cudaError_t e = by_taps(a.K, [&](auto kt, auto exact) {
+        conv_bwd_kernel<E, decltype(kt)::value, decltype(exact)::value, VEC><<<(unsigned)blocks, THREADS, 0, stream>>>(
+            (const E *)a.x, a.ldb, a.ldt, (const E *)a.w, (const E *)a.bias, (const E *)a.dy, (E *)a.dx, a.part, a.T,
+            a.D, a.K, a.silu, nd, ns, len);
+        return cudaGetLastError();
+    });
+    if (e != cudaSuccess) return e;
+    conv_reduce_kernel<E><<<dim3((a.D + 31) / 32, a.K + 1), 256, 0, stream>>>(a.part, (E *)a.dw, (E *)a.dbias,
+                                                                             a.Bt * ns, a.D, a.K);
+    return cudaGetLastError();
+}
+
+template <typename E, int VEC>
+cudaError_t packed_of(const ConvPackedArgs &a, cudaStream_t stream)
+{
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC);
+    // single tokens have no tails unless there is no window
+    const long long heads = a.K > 1 || a.seq.starts.p ? (long long)a.seq.count * nd : 0;
+    const long long tails = a.seq.starts.p || a.K == 1 ? (long long)((a.seq.rows + FWD_ROWS - 1) / FWD_ROWS) * nd : 0;
+    const long long blocks = (heads + tails + WARPS - 1) / WARPS;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (blocks == 0) return cudaSuccess;
+    return by_taps(a.K, [&](auto kt, auto exact) {
+        conv_packed_kernel<E, decltype(kt)::value, decltype(exact)::value, VEC>
+            <<<(unsigned)blocks, THREADS, 0, stream>>>((const E *)a.x, a.ldx, (const E *)a.w, (const E *)a.bias,
+                                                       (E *)a.window, (E *)a.y, a.seq, a.D, a.K, a.silu, nd, heads,
+                                                       heads + tails);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace
+
+size_t conv_workspace_bytes(int Bt, int T, int D, int K)
+{
+    return (size_t)Bt * bwd_segments(T, bwd_rows(Bt, T, D)) * (K + 1) * D * sizeof(float);
+}
+
+cudaError_t launch_conv_fwd(const ConvArgs &a, cudaStream_t stream)
+{
+    if (a.bf16)
+        return groups_of_4<__nv_bfloat16>(a.D, {a.x, a.y}, {a.ldb, a.ldt}) ? fwd_of<__nv_bfloat16, 4>(a, stream)
+                                                                           : fwd_of<__nv_bfloat16, 1>(a, stream);
+    return groups_of_4<float>(a.D, {a.x, a.y}, {a.ldb, a.ldt}) ? fwd_of<float, 4>(a, stream) : fwd_of<float, 1>(a, stream);
+}
+
+cudaError_t launch_conv_bwd(const ConvArgs &a, cudaStream_t stream)
+{
+    if (a.bf16)
+        return groups_of_4<__nv_bfloat16>(a.D, {a.x, a.dy, a.dx}, {a.ldb, a.ldt})
+                   ? bwd_of<__nv_bfloat16, 4>(a, stream) : bwd_of<__nv_bfloat16, 1>(a, stream);
+    return groups_of_4<float>(a.D, {a.x, a.dy, a.dx}, {a.ldb, a.ldt}) ? bwd_of<float, 4>(a, stream)
+                                                                      : bwd_of<float, 1>(a, stream);
+}
+
+cudaError_t launch_conv_packed(const ConvPackedArgs &a, cudaStream_t stream)
+{
+    if (a.bf16)
+        return groups_of_4<__nv_bfloat16>(a.D, {a.x, a.y}, {a.ldx}) ? packed_of<__nv_bfloat16, 4>(a, stream)
+                                                                    : packed_of<__nv_bfloat16, 1>(a, stream);
+    return groups_of_4<float>(a.D, {a.x, a.y}, {a.ldx}) ? packed_of<float, 4>(a, stream) : packed_of<float, 1>(a, stream);
+}
+
+}  // namespace mms

@@ -62,6 +62,14 @@ SIGNATURES = {
     "mms_norm_workspace_size": ([_I] * 2, _Z),
     "mms_norm_fwd": ([_P] * 3 + [_L] + [_P] * 3 + [_F] + [_P] * 3 + [_I] * 3 + [_P], _I),
     "mms_norm_bwd": ([_P] * 3 + [_L] + [_P] * 13 + [_Z] + [_I] * 3 + [_P], _I),
+    "mms_conv_workspace_size": ([_I] * 4, _Z),
+    "mms_conv_fwd": ([_P, _L, _L] + [_P] * 3 + [_I] * 6 + [_P], _I),
+    "mms_conv_bwd": ([_P, _L, _L] + [_P] * 7 + [_Z] + [_I] * 6 + [_P], _I),
+    "mms_conv_packed": ([_P, _L] + [_P] * 3 + [_I] + [_P] * 3 + [_I, _P] + [_I] * 6 + [_P], _I),
+    "mms_scan_packed_workspace_size": ([_I] * 4, _Z),
+    "mms_scan_packed": ([_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _L, _P, _I, _F, _F, _P, _I] + [_P] * 3
+                        + [_I, _P, _P, _Z] + [_I] * 6 + [_P], _I),
+    "mms_sample": ([_P, _L, _P, _P, _F, _P, _I, _L, _P, _F, _P, _F, _P, _P] + [_I] * 3 + [_P], _I),
     "mms_debug_set_wait": ([ctypes.c_uint, _I], _I),
     "mms_probe_pipe": ([_I] * 3 + [_P] * 4, _I),
     "mms_probe_ops_per_cta": ([_I] * 2, ctypes.c_longlong),
@@ -408,6 +416,98 @@ def norm_bwd(x, y, gate, weight, post, scale, stat, dh, du):
     if rc:
         _check(rc, "mms_norm_bwd")
     return dx, dy, dgate, dweight, dpost, dscale
+
+
+SERVE_MAX, SERVE_MAX_DIM = 1 << 30, 1 << 24    # MMS_SERVE_MAX, MMS_SERVE_MAX_DIM
+
+
+def conv_fwd(x, w, bias, silu: bool):
+    """y of mms_conv_fwd; x (B, T, D) with strides, w (D, K)."""
+    bt, t_len, d = x.shape
+    y = torch.empty((bt, t_len, d), device=x.device, dtype=x.dtype)
+    rc = load().mms_conv_fwd(x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _opt(bias), y.data_ptr(),
+                             bt, t_len, d, w.shape[1], silu, _dtype(x), _stream(x.device))
+    if rc:
+        _check(rc, "mms_conv_fwd")
+    return y
+
+
+@functools.lru_cache(maxsize=256)
+def _conv_workspace(bt: int, t_len: int, d: int, k: int) -> int:
+    return int(load().mms_conv_workspace_size(bt, t_len, d, k))
+
+
+def conv_bwd(x, w, bias, dy, silu: bool):
+    """(dx, dw, dbias) of mms_conv_bwd; dbias None without a bias."""
+    bt, t_len, d = x.shape
+    k = w.shape[1]
+    dx, dw = torch.empty((bt, t_len, d), device=x.device, dtype=x.dtype), torch.empty_like(w)
+    db = None if bias is None else torch.empty_like(bias)
+    nb = _conv_workspace(bt, t_len, d, k)
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    rc = load().mms_conv_bwd(x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _opt(bias), dy.data_ptr(),
+                             dx.data_ptr(), dw.data_ptr(), _opt(db), ws.data_ptr(), nb, bt, t_len, d, k, silu,
+                             _dtype(x), _stream(x.device))
+    if rc:
+        _check(rc, "mms_conv_bwd")
+    return dx, dw, db
+
+
+def _wide(starts, slots, out_slots) -> int:
+    """Which of the lists hold 64-bit numbers (MMS_WIDE_*)."""
+    return sum(bit for bit, t in ((1, starts), (2, slots), (4, out_slots))
+               if t is not None and t.dtype == torch.int64)
+
+
+def conv_packed(rows, w, bias, window, starts, slots, out_slots, count: int, silu: bool):
+    """y of mms_conv_packed, window updated; rows = (x (L, D), its row stride)."""
+    x, ldx = rows
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    rc = load().mms_conv_packed(x.data_ptr(), ldx, w.data_ptr(), _opt(bias), window.data_ptr(), window.shape[0],
+                                _opt(starts), _opt(slots), _opt(out_slots), _wide(starts, slots, out_slots),
+                                y.data_ptr(), x.shape[0], count, x.shape[1], w.shape[1], silu, _dtype(x),
+                                _stream(x.device))
+    if rc:
+        _check(rc, "mms_conv_packed")
+    return y
+
+
+@functools.lru_cache(maxsize=256)
+def _scan_packed_workspace(rows: int, count: int, d: int, n: int) -> int:
+    return int(load().mms_scan_packed_workspace_size(rows, count, d, n))
+
+
+def scan_packed(x, dt, aneg, b_in, c_in, z, d_skip, dt_range, state, starts, slots, out_slots, count: int):
+    """y of mms_scan_packed, state updated; x, dt, b_in, c_in, z as (tensor, row stride)."""
+    (x, ldx), (dt, lddt), (b_in, ldb), (c_in, ldc) = x, dt, b_in, c_in
+    z, ldz = (None, 0) if z is None else z
+    n_rows, d = x.shape
+    n = aneg.shape[1]
+    y = torch.empty((n_rows, d), device=x.device, dtype=x.dtype)
+    nb = 0 if starts is None else _scan_packed_workspace(n_rows, count, d, n)
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+    lo, hi = (0.0, 0.0) if dt_range is None else dt_range
+    rc = load().mms_scan_packed(x.data_ptr(), ldx, dt.data_ptr(), lddt, aneg.data_ptr(), b_in.data_ptr(), ldb,
+                                c_in.data_ptr(), ldc, _opt(z), ldz, _opt(d_skip), dt_range is not None, lo, hi,
+                                state.data_ptr(), state.shape[0], _opt(starts), _opt(slots), _opt(out_slots),
+                                _wide(starts, slots, out_slots), y.data_ptr(), _opt(ws), nb, n_rows, count, d, n,
+                                _dtype(x), _dtype(b_in), _stream(x.device))
+    if rc:
+        _check(rc, "mms_scan_packed")
+    return y
+
+
+def sample(z, ld: int, uniform, t, t1, k, k1, p, p1, m, m1, with_logprob: bool):
+    """(token, logprob) of mms_sample; of each setting a tensor of one value a row, or None and a number."""
+    rows, vocab = z.shape
+    token = torch.empty(rows, dtype=torch.int64, device=z.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=z.device) if with_logprob else None
+    rc = load().mms_sample(z.data_ptr(), ld, uniform.data_ptr(), _opt(t), t1, _opt(k),
+                           k is not None and k.dtype == torch.int64, k1, _opt(p), p1, _opt(m), m1,
+                           token.data_ptr(), _opt(logprob), rows, vocab, _dtype(z), _stream(z.device))
+    if rc:
+        _check(rc, "mms_sample")
+    return token, logprob
 
 
 def pipe_rate(kind: str, device=None, iters: int = 4096, ctas_per_sm: int = 4) -> float:
