@@ -25,12 +25,20 @@ namespace {
 
 constexpr int WARPS = 4;                // per CTA, each with rows of its own and the same channels
 constexpr int THREADS = 32 * WARPS;
-constexpr int FWD_ROWS = 8;             // rows of a warp's tile, all loaded before the first is used
 constexpr int BWD_STEP = 4;             // rows the backward loads at once
+
+// VEC neighbouring channels of a row as they are stored, and as NP pairs of floats (one
+// channel alone: the second of its pair is 0).
+template <int VEC>
+constexpr int NP = (VEC + 1) / 2;
 
 template <typename E, int VEC>
 struct alignas(sizeof(E) * VEC) Pack {
     E v[VEC];
+    __device__ __forceinline__ float2 pair(int p) const {
+        if constexpr (VEC == 1) return f2(to_f(v[0]), 0.f);
+        else return f2(to_f(v[2 * p]), to_f(v[2 * p + 1]));
+    }
 };
 
 template <typename E, int VEC>
@@ -38,11 +46,17 @@ __device__ __forceinline__ Pack<E, VEC> load(const E *p) {
     return *reinterpret_cast<const Pack<E, VEC> *>(p);
 }
 template <typename E, int VEC>
-__device__ __forceinline__ void store(E *p, const float (&v)[VEC]) {
-    Pack<E, VEC> o;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o.v[i] = from_f<E>(v[i]);
-    *reinterpret_cast<Pack<E, VEC> *>(p) = o;
+__device__ __forceinline__ void store(E *p, const float2 (&v)[NP<VEC>]) {
+    if constexpr (VEC == 1) {
+        *p = from_f<E>(v[0].x);
+    } else if constexpr (sizeof(E) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    } else {
+        Pack<__nv_bfloat162, 2> o;
+        o.v[0] = __float22bfloat162_rn(v[0]);
+        o.v[1] = __float22bfloat162_rn(v[1]);
+        *reinterpret_cast<Pack<__nv_bfloat162, 2> *>(p) = o;
+    }
 }
 template <typename E, int VEC>
 __device__ __forceinline__ Pack<E, VEC> nothing() {
@@ -53,33 +67,43 @@ __device__ __forceinline__ Pack<E, VEC> nothing() {
 }
 
 // sigmoid(v) = 1 / (1 + e^-v) on MUFU's ex2 and reciprocal
-__device__ __forceinline__ float act(float v, bool silu) { return silu ? v * sigmoid_fast(v) : v; }
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+    const float2 d = add2(ex2x2(mul2(v, f2(-MMS_LOG2E, -MMS_LOG2E))), f2(1.f, 1.f));
+    float2 r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+    return r;
+}
+__device__ __forceinline__ float2 act(float2 v, bool silu) { return silu ? mul2(v, sigmoid2(v)) : v; }
 
 // A channel group's taps. KT: taps the code is unrolled for; with fewer of them
 // (K < KT) the first KT - K stand for none and are skipped, not multiplied by zero:
 // an infinite input there must not turn into a NaN.
 template <typename E, int KT, int VEC>
 struct Taps {
-    float w[KT][VEC], bias[VEC];
+    float2 w[KT][NP<VEC>], bias[NP<VEC>];
     __device__ __forceinline__ void read(const E *wp, const E *bp, int d, int K) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            bias[i] = bp ? to_f(bp[d + i]) : 0.f;
+        for (int p = 0; p < NP<VEC>; ++p) {
+            const int c0 = d + 2 * p, c1 = VEC == 1 ? c0 : c0 + 1;
+            bias[p] = bp ? f2(to_f(bp[c0]), to_f(bp[c1])) : f2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < KT; ++k)
-                w[k][i] = k >= KT - K ? to_f(wp[(long long)(d + i) * K + k - (KT - K)]) : 0.f;
+            for (int k = 0; k < KT; ++k) {
+                const int kk = k - (KT - K);
+                w[k][p] = kk >= 0 ? f2(to_f(wp[(long long)c0 * K + kk]), to_f(wp[(long long)c1 * K + kk])) : f2(0.f, 0.f);
+            }
         }
     }
     // the sum over rows x[0 .. KT - 1]
     template <typename Row>
-    __device__ __forceinline__ void sum(float (&acc)[VEC], int K, Row row) const {
+    __device__ __forceinline__ void sum(float2 (&acc)[NP<VEC>], int K, Row row) const {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = bias[i];
+        for (int p = 0; p < NP<VEC>; ++p) acc[p] = bias[p];
 #pragma unroll
         for (int k = 0; k < KT; ++k)
             if (k >= KT - K) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[k][i], row(k, i), acc[i]);
+                for (int p = 0; p < NP<VEC>; ++p) acc[p] = fma2(w[k][p], row(k, p), acc[p]);
             }
     }
 };
@@ -88,6 +112,10 @@ struct Taps {
 template <int KT, bool EXACT>
 __device__ __forceinline__ int taps_of(int K) { return EXACT ? KT : K; }
 
+// Rows of a warp's tile, all loaded before the first is used: 8 of 16 bytes a lane, 16 of 8.
+template <typename E>
+constexpr int FWD_ROWS = sizeof(E) == 4 ? 8 : 16;
+
 // ---------------------------------------------------------------- forward
 
 template <typename E, int KT, bool EXACT, int VEC>
@@ -95,17 +123,18 @@ __global__ void __launch_bounds__(THREADS)
 conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
                 const E *__restrict__ bias, E *__restrict__ y, int T, int D, int K_in, bool silu, int nd, int nt)
 {
+    constexpr int ROWS = FWD_ROWS<E>;
     const int K = taps_of<KT, EXACT>(K_in);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int blk = blockIdx.x;                            // (b, tile, channel block), the last fastest
     const int d = (blk % nd) * 32 * VEC + lane * VEC;
     const int tile = blk / nd % nt, b = blk / nd / nt;
-    const int t0 = (tile * WARPS + warp) * FWD_ROWS;
+    const int t0 = (tile * WARPS + warp) * ROWS;
     if (d >= D || t0 >= T) return;
     const E *xb = x + b * ldb + d;
-    Pack<E, VEC> xs[FWD_ROWS + KT - 1];
+    Pack<E, VEC> xs[ROWS + KT - 1];
 #pragma unroll
-    for (int j = 0; j < FWD_ROWS + KT - 1; ++j) {
+    for (int j = 0; j < ROWS + KT - 1; ++j) {
         const int t = t0 - (KT - 1) + j;
         xs[j] = t >= 0 && t < T ? load<E, VEC>(xb + t * ldt) : nothing<E, VEC>();
     }
@@ -113,12 +142,13 @@ conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
     taps.read(w, bias, d, K);
     E *yb = y + ((long long)b * T + t0) * D + d;
 #pragma unroll
-    for (int r = 0; r < FWD_ROWS; ++r) {
-        float acc[VEC];
-        taps.sum(acc, K, [&](int k, int i) { return to_f(xs[r + k].v[i]); });
+    for (int r = 0; r < ROWS; ++r) {
+        float2 acc[NP<VEC>];
+        taps.sum(acc, K, [&](int k, int p) { return xs[r + k].pair(p); });
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
-        if (t0 + r < T) store<E, VEC>(yb + (long long)r * D, acc);
+        for (int p = 0; p < NP<VEC>; ++p) acc[p] = act(acc[p], silu);
+        if (t0 + r < T) store<E, VEC>(yb, acc);
+        yb += D;
     }
 }
 
@@ -129,101 +159,122 @@ conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
 // computed as well, for dx alone. dw and dbias stay in registers; the CTA's four
 // warps are joined in shared memory and leave one partial sum a CTA.
 template <typename E, int KT, bool EXACT, int VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, KT <= 4 ? 4 : 2)
 conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
                 const E *__restrict__ bias, const E *__restrict__ dy, E *__restrict__ dx,
                 float *__restrict__ part, int T, int D, int K_in, bool silu, int nd, int ns, int len)
 {
+    constexpr int P = NP<VEC>;
     const int K = taps_of<KT, EXACT>(K_in);
-    __shared__ float sums[WARPS][KT + 1][VEC][32];
+    __shared__ float2 sums[WARPS][KT + 1][P][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int blk = blockIdx.x;                            // (b, segment, channel block)
     const int d = (blk % nd) * 32 * VEC + lane * VEC;
     const int seg = blk / nd % ns, b = blk / nd / ns;
     const int t0 = (seg * WARPS + warp) * len, t1 = min(T, t0 + len);
-    float dw[KT][VEC] = {}, db[VEC] = {};
+    float2 dw[KT][P], db[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        db[p] = f2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < KT; ++k) dw[k][p] = f2(0.f, 0.f);
+    }
     if (d < D && t0 < T) {
-        const E *xb = x + b * ldb + d;
-        const E *gb = dy + (long long)b * T * D + d;
-        E *ob = dx + (long long)b * T * D + d;
+        const E *xp = x + b * ldb + d + t0 * ldt;          // row t
+        const E *gp = dy + ((long long)b * T + t0) * D + d;
+        E *op = dx + ((long long)b * T + t0 - (KT - 1)) * D + d;  // row t - KT + 1
         Taps<E, KT, VEC> taps;
         taps.read(w, bias, d, K);
         Pack<E, VEC> xs[BWD_STEP + KT - 1];                // rows t - KT + 1 .. t + BWD_STEP - 1
-        float ds[BWD_STEP + KT - 1][VEC];
+        float2 ds[BWD_STEP + KT - 1][P];
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
-            const int t = t0 - (KT - 1) + j;
-            xs[j] = t >= 0 ? load<E, VEC>(xb + t * ldt) : nothing<E, VEC>();
+            const int back = KT - 1 - j;
+            xs[j] = t0 >= back ? load<E, VEC>(xp - back * ldt) : nothing<E, VEC>();
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ds[j][i] = 0.f;
+            for (int p = 0; p < P; ++p) ds[j][p] = f2(0.f, 0.f);
         }
-        for (int t = t0; t < t1 + KT - 1; t += BWD_STEP) {
+        // inner: all rows of the step are the warp's own, and so are those whose dx they complete
+        auto step = [&](int t, auto inner) {
+            constexpr bool INNER = decltype(inner)::value;
             Pack<E, VEC> g[BWD_STEP];
 #pragma unroll
             for (int u = 0; u < BWD_STEP; ++u) {
-                const bool in = t + u < T && t + u < t1 + KT - 1;
-                xs[KT - 1 + u] = in ? load<E, VEC>(xb + (t + u) * ldt) : nothing<E, VEC>();
-                g[u] = in ? load<E, VEC>(gb + (long long)(t + u) * D) : nothing<E, VEC>();
+                const bool in = INNER || (t + u < T && t + u < t1 + KT - 1);
+                xs[KT - 1 + u] = in ? load<E, VEC>(xp) : nothing<E, VEC>();
+                g[u] = in ? load<E, VEC>(gp) : nothing<E, VEC>();
+                xp += ldt, gp += D;
             }
 #pragma unroll
             for (int u = 0; u < BWD_STEP; ++u) {
-                float pre[VEC];
-                if (silu) taps.sum(pre, K, [&](int k, int i) { return to_f(xs[u + k].v[i]); });
+                float2 pre[P];
+                if (silu) taps.sum(pre, K, [&](int k, int p) { return xs[u + k].pair(p); });
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    float s = to_f(g[u].v[i]);
-                    if (silu) {
-                        const float sg = sigmoid_fast(pre[i]);
-                        s *= sg * fmaf(pre[i], 1.f - sg, 1.f);
+                for (int p = 0; p < P; ++p) {
+                    float2 s = g[u].pair(p);
+                    if (silu) {                            // dy sg (1 + pre (1 - sg))
+                        const float2 sg = sigmoid2(pre[p]);
+                        const float2 rest = fma2(sg, f2(-1.f, -1.f), f2(1.f, 1.f));
+                        s = mul2(s, mul2(sg, fma2(pre[p], rest, f2(1.f, 1.f))));
                     }
-                    ds[KT - 1 + u][i] = t + u < T ? s : 0.f;
+                    ds[KT - 1 + u][p] = INNER || t + u < T ? s : f2(0.f, 0.f);
                 }
-                if (t + u < t1) {
+                if (INNER || t + u < t1) {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        db[i] += ds[KT - 1 + u][i];
+                    for (int p = 0; p < P; ++p) {
+                        db[p] = add2(db[p], ds[KT - 1 + u][p]);
 #pragma unroll
-                        for (int k = 0; k < KT; ++k)
-                            dw[k][i] = fmaf(ds[KT - 1 + u][i], to_f(xs[u + k].v[i]), dw[k][i]);
+                        for (int k = 0; k < KT; ++k) dw[k][p] = fma2(ds[KT - 1 + u][p], xs[u + k].pair(p), dw[k][p]);
                     }
                 }
                 const int to = t + u - (KT - 1);
-                if (to >= t0 && to < t1) {
-                    float o[VEC] = {};
+                if (INNER || (to >= t0 && to < t1)) {
+                    float2 o[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) o[p] = f2(0.f, 0.f);
 #pragma unroll
                     for (int k = 0; k < KT; ++k)
                         if (k >= KT - K) {
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) o[i] = fmaf(taps.w[k][i], ds[KT - 1 + u - k][i], o[i]);
+                            for (int p = 0; p < P; ++p) o[p] = fma2(taps.w[k][p], ds[KT - 1 + u - k][p], o[p]);
                         }
-                    store<E, VEC>(ob + (long long)to * D, o);
+                    store<E, VEC>(op, o);
                 }
+                op += D;
             }
 #pragma unroll
             for (int j = 0; j < KT - 1; ++j) {
                 xs[j] = xs[j + BWD_STEP];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ds[j][i] = ds[j + BWD_STEP][i];
+                for (int p = 0; p < P; ++p) ds[j][p] = ds[j + BWD_STEP][p];
             }
+        };
+        for (int t = t0; t < t1 + KT - 1; t += BWD_STEP) {
+            if (t - (KT - 1) >= t0 && t + BWD_STEP <= t1) step(t, std::true_type{});
+            else step(t, std::false_type{});
         }
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+    for (int p = 0; p < P; ++p) {
 #pragma unroll
-        for (int k = 0; k < KT; ++k) sums[warp][k][i][lane] = dw[k][i];
-        sums[warp][KT][i][lane] = db[i];
+        for (int k = 0; k < KT; ++k) sums[warp][k][p][lane] = dw[k][p];
+        sums[warp][KT][p][lane] = db[p];
     }
     __syncthreads();
     // part[(b, segment)][K + 1][D]
     float *pb = part + (long long)(blk / nd) * (K + 1) * D + (blk % nd) * 32 * VEC;
     const int left = D - (blk % nd) * 32 * VEC;
-    for (int o = threadIdx.x; o < (KT + 1) * VEC * 32; o += THREADS) {
-        const int c = o % (VEC * 32), k = o / (VEC * 32);
-        if (c >= left || k < KT - K) continue;
-        float s = 0.f;
+    for (int o = threadIdx.x; o < (KT + 1) * P * 32; o += THREADS) {
+        const int c = o % (P * 32), k = o / (P * 32);
+        const int at = VEC == 1 ? c : 2 * c;               // its first channel in the CTA
+        if (at >= left || k < KT - K) continue;
+        const int p = c % P, l = c / P;
+        float2 s = sums[0][k][p][l];
 #pragma unroll
-        for (int q = 0; q < WARPS; ++q) s += sums[q][k][c % VEC][c / VEC];
-        pb[(long long)(k - (KT - K)) * D + c] = s;
+        for (int q = 1; q < WARPS; ++q) s = add2(s, sums[q][k][p][l]);
+        float *to = pb + (long long)(k - (KT - K)) * D + at;
+        to[0] = s.x;
+        if (VEC > 1) to[1] = s.y;
     }
 }
 
@@ -254,7 +305,7 @@ conv_reduce_kernel(const float *__restrict__ part, E *__restrict__ dw, E *__rest
 // so that none waits for another though the cache is updated in place:
 //   heads  (sequence, channel block): the outputs that still see the old window,
 //          rows 0 .. min(length, K - 1) - 1, and then the new window;
-//   tails  (8 rows, channel block): the rows at place K - 1 and later of their
+//   tails  (8 or 16 rows, channel block): the rows at place K - 1 and later of their
 //          sequence, which depend on x alone; rows of no sequence get zeros.
 template <typename E, int KT, bool EXACT, int VEC>
 __global__ void __launch_bounds__(THREADS)
@@ -271,39 +322,41 @@ conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__
         if (d >= D) return;
         const int s = (int)(unit / nd);
         const int first = seq.start(s), end = seq.starts.p ? max(first, seq.start(s + 1)) : s + 1;
-        const int len = end - first;
+        const int len = end - first, K1 = K - 1;
         const long long from = seq.from(s), to = seq.to(s);
-        const int K1 = K - 1;
-        // rows[0 .. KT - 2] the old window, then the first inputs
-        float rows[2 * (KT - 1) + 1][VEC];
+        // rows[0 .. KT - 2] the old window (as pairs, the same rounding as x's), then the first inputs
+        E old[KT > 1 ? KT - 1 : 1][VEC];
+        float2 rows[2 * (KT - 1) + 1][NP<VEC>];
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
             const int jw = j - (KT - K);                   // its place in the window
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                rows[j][i] = from >= 0 && jw >= 0 ? to_f(window[(from * D + d + i) * K1 + jw]) : 0.f;
+                old[j][i] = from >= 0 && jw >= 0 ? window[(from * D + d + i) * K1 + jw] : from_f<E>(0.f);
             const bool in = j < len && j < K1;
             const Pack<E, VEC> v = in ? load<E, VEC>(x + (first + j) * ldx + d) : nothing<E, VEC>();
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) rows[KT - 1 + j][i] = to_f(v.v[i]);
+            for (int p = 0; p < NP<VEC>; ++p) {
+                rows[j][p] = VEC == 1 ? f2(to_f(old[j][0]), 0.f) : f2(to_f(old[j][2 * p]), to_f(old[j][(2 * p + 1) % VEC]));
+                rows[KT - 1 + j][p] = v.pair(p);
+            }
         }
         if (to >= 0) {
             // the last K - 1 of the window and the inputs behind it
 #pragma unroll
             for (int j = 0; j < KT - 1; ++j) {
-                if (j >= K1) continue;
                 const int p = len - K1 + j;                // its row; below 0: in the old window
-                if (p >= 0) {
-                    const Pack<E, VEC> v = load<E, VEC>(x + (first + p) * ldx + d);
+                Pack<E, VEC> v = nothing<E, VEC>();
+                if (p >= 0 && j < K1) v = load<E, VEC>(x + (first + p) * ldx + d);
+#pragma unroll
+                for (int q = 0; q < KT - 1; ++q)           // (constant indices: registers)
+                    if (p < 0 && q - (KT - K) == p + K1) {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) v.v[i] = old[q][i];
+                    }
+                if (j < K1) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = v.v[i];
-                } else {
-#pragma unroll
-                    for (int q = 0; q < KT - 1; ++q)       // (a constant index into the registers)
-                        if (q - (KT - K) == p + K1) {
-#pragma unroll
-                            for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = from_f<E>(rows[q][i]);
-                        }
                 }
             }
         }
@@ -312,43 +365,55 @@ conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__
 #pragma unroll
         for (int r = 0; r < KT - 1; ++r) {
             if (r >= K1 || r >= len) continue;
-            float acc[VEC];
-            taps.sum(acc, K, [&](int k, int i) { return rows[r + k][i]; });
+            float2 acc[NP<VEC>];
+            taps.sum(acc, K, [&](int k, int p) { return rows[r + k][p]; });
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
+            for (int p = 0; p < NP<VEC>; ++p) acc[p] = act(acc[p], silu);
             store<E, VEC>(y + (long long)(first + r) * D + d, acc);
         }
         return;
     }
-    const int r0 = (int)((unit - heads) / nd) * FWD_ROWS;
-    Pack<E, VEC> xs[FWD_ROWS + KT - 1];
+    constexpr int ROWS = FWD_ROWS<E>;
+    const int r0 = (int)((unit - heads) / nd) * ROWS;
+    Pack<E, VEC> xs[ROWS + KT - 1];
 #pragma unroll
-    for (int j = 0; j < FWD_ROWS + KT - 1; ++j) {
+    for (int j = 0; j < ROWS + KT - 1; ++j) {
         const int t = r0 - (KT - 1) + j;
         xs[j] = d < D && t >= 0 && t < seq.rows ? load<E, VEC>(x + t * ldx + d) : nothing<E, VEC>();
     }
-    // lane r finds row r0 + r: 0 a head's, 1 a tail's, 2 nobody's
-    int kind = 0;
-    if (lane < FWD_ROWS && r0 + lane < seq.rows) {
-        if (!seq.starts.p) kind = K == 1 ? 1 : 0;
-        else {
-            const int s = Sequences::last_at_most(seq.count + 1, r0 + lane, [&](int i) { return seq.start(i); });
-            kind = s < 0 || s >= seq.count ? 2 : r0 + lane - seq.start(s) >= K - 1 ? 1 : 0;
-        }
-    }
     Taps<E, KT, VEC> taps;
     if (d < D) taps.read(w, bias, d, K);
-#pragma unroll
-    for (int r = 0; r < FWD_ROWS; ++r) {
-        const int what = __shfl_sync(0xffffffffu, kind, r);
-        if (what == 0 || d >= D) continue;
-        float acc[VEC] = {};
-        if (what == 1) {
-            taps.sum(acc, K, [&](int k, int i) { return to_f(xs[r + k].v[i]); });
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] = act(acc[i], silu);
+    // what row r0 + r is: bit r of `tails`, of `nobody`, or of neither (a head's)
+    unsigned tails = 0, nobody = 0;
+    const int rows = min(ROWS, seq.rows - r0);
+    if (!seq.starts.p) {
+        tails = K == 1 ? ~0u : 0u;
+    } else {
+        auto start = [&](int i) { return seq.start(i); };
+        const int n = seq.count + 1;
+        int s = Sequences::last_at_most(n, r0, start);
+        int first = s < 0 ? 0 : seq.start(s), next = s + 1 < n ? seq.start(s + 1) : seq.rows;
+        for (int r = 0; r < rows; ++r) {
+            if (r0 + r >= next) {                          // a sequence ends inside the tile
+                s = Sequences::last_at_most(n, r0 + r, start);
+                first = s < 0 ? 0 : seq.start(s), next = s + 1 < n ? seq.start(s + 1) : seq.rows;
+            }
+            if (s < 0 || s >= seq.count) nobody |= 1u << r;
+            else if (r0 + r - first >= K - 1) tails |= 1u << r;
         }
-        store<E, VEC>(y + (long long)(r0 + r) * D + d, acc);
+    }
+    if (d >= D) return;
+    E *yp = y + (long long)r0 * D + d;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (r < rows && ((tails | nobody) >> r & 1)) {
+            float2 acc[NP<VEC>];
+            taps.sum(acc, K, [&](int k, int p) { return xs[r + k].pair(p); });
+#pragma unroll
+            for (int p = 0; p < NP<VEC>; ++p) acc[p] = nobody >> r & 1 ? f2(0.f, 0.f) : act(acc[p], silu);
+            store<E, VEC>(yp, acc);
+        }
+        yp += D;
     }
 }
 
@@ -393,7 +458,7 @@ cudaError_t by_taps(int K, F f)
 template <typename E, int VEC>
 cudaError_t fwd_of(const ConvArgs &a, cudaStream_t stream)
 {
-    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), nt = (a.T + WARPS * FWD_ROWS - 1) / (WARPS * FWD_ROWS);
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), nt = (a.T + WARPS * FWD_ROWS<E> - 1) / (WARPS * FWD_ROWS<E>);
     const long long blocks = (long long)a.Bt * nt * nd;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     return by_taps(a.K, [&](auto kt, auto exact) {
@@ -427,7 +492,7 @@ cudaError_t packed_of(const ConvPackedArgs &a, cudaStream_t stream)
     const int nd = (a.D + 32 * VEC - 1) / (32 * VEC);
     // single tokens have no tails unless there is no window
     const long long heads = a.K > 1 || a.seq.starts.p ? (long long)a.seq.count * nd : 0;
-    const long long tails = a.seq.starts.p || a.K == 1 ? (long long)((a.seq.rows + FWD_ROWS - 1) / FWD_ROWS) * nd : 0;
+    const long long tails = a.seq.starts.p || a.K == 1 ? (long long)((a.seq.rows + FWD_ROWS<E> - 1) / FWD_ROWS<E>) * nd : 0;
     const long long blocks = (heads + tails + WARPS - 1) / WARPS;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (blocks == 0) return cudaSuccess;

@@ -12,12 +12,14 @@
 // scan does; G = 1, 2 or 4 lanes share a channel of up to 16, 32 or 64 states. A
 // sequence is cut into segments of `seg` rows, so that one long prompt fills the GPU
 // as well as many short ones, whatever the lengths, which the host does not know:
-//   first   the first segment of every sequence, in full; of those between it and the
-//           last only the end state from nothing and the sum of dt (the decay of a
-//           state over the segment is exp(-Aneg sum dt));
+//   first   the first segment of a sequence in full; of those between it and the last
+//           only the end state from nothing and the sum of dt (the decay of a state
+//           over the segment is exp(-Aneg sum dt));
 //   rest    all later segments, each from the chain of the end states before it.
 // A sequence of one segment is done in the first launch, with one exponential a state
-// and step; only the segments between the first and the last take two.
+// and step; only the segments between the first and the last take two. Of a sequence of
+// more than FEW segments the first is taken like those between: the launch would
+// otherwise end with its CTAs alone, which have half as much again to do.
 //
 // Unit u of a launch is segment i of sequence s with u = s + start_s / seg + i: as
 // a sequence of n rows has at most (start_s + n) / seg - start_s / seg + 1
@@ -37,7 +39,15 @@ namespace mms {
 namespace {
 
 constexpr int THREADS = 128;
-constexpr int TT = 8;                   // rows of a tile: loaded ahead, B and C through shared memory
+constexpr int TT = 8;                   // rows of a tile of B and C
+constexpr int SUB = 4;                  // rows of x, dt and z in registers
+constexpr int FEW = 3;                  // segments of a sequence whose first is done in full at once
+#ifndef MMS_PACKED_POLY
+#define MMS_PACKED_POLY 1
+#endif
+#ifndef MMS_PACKED_MINB
+#define MMS_PACKED_MINB 4
+#endif
 
 template <typename E, typename BE>
 struct Args {
@@ -51,6 +61,7 @@ struct Args {
     int D, N;
     Proj pj;
     float *ends, *sums;                 // end states (row, D, N) and sums of dt (row, D) of segments
+    float *entry;                       // (row, D, N) what long sequences go on from
     int seg, nd;                        // rows of a segment, channel blocks
     int units;                          // units of segments; the blocks behind them clear rows of no sequence
 };
@@ -64,7 +75,9 @@ struct Split {
 // ------------------------------------------------------------- segments
 
 // The rows [t0, t1) from state h; FULL: with outputs, else h from what it is and the
-// sum of dt.
+// sum of dt. Rows come through registers SUB at a time, the next ones requested as
+// soon as these are converted; B and C as float32 through shared memory, TT rows at a time.
+// POLY of a thread's pairs of exponentials are taken from MUFU to the FMA pipe.
 template <bool FULL, typename E, typename BE, typename S>
 __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S::NP], float2 (&h)[S::NS / 2],
                                       const float2 (&nan2)[S::NS / 2], int t0, int t1, int d, int g, bool act)
@@ -72,15 +85,28 @@ __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S
     constexpr int NS = S::NS, NP = S::NP;
     constexpr int ARR = FULL ? 2 : 1;                      // B, and C where it is wanted
     constexpr int PER = (TT * ARR * NP + THREADS - 1) / THREADS;
+    constexpr int POLY = MMS_PACKED_POLY * NS / 16;
     const int tid = threadIdx.x;
     const bool gate = FULL && a.z != nullptr;
     const float skip = FULL && a.d_skip && act ? a.d_skip[d] : 0.f;
-    E xr[TT], dr[TT], zr[TT];
-    auto row_in = [&](int j, int t) {
-        const bool in = act && t < t1;
-        xr[j] = in ? a.x[t * a.ldx + d] : from_f<E>(0.f);
-        dr[j] = in ? a.dt[t * a.lddt + d] : from_f<E>(0.f);
-        if (FULL) zr[j] = in && gate ? a.z[t * a.ldz + d] : from_f<E>(0.f);
+    const int ds = act ? d : 0;                            // a channel that is there
+    const E *xp = a.x + t0 * a.ldx + ds, *dp = a.dt + t0 * a.lddt + ds;
+    const E *zp = gate ? a.z + t0 * a.ldz + ds : a.x;
+    const long long ldz = gate ? a.ldz : 0;
+    E *yp = a.y + (long long)t0 * a.D + ds;
+    E xr[SUB], dr[SUB], zr[SUB];
+    auto rows_in = [&](int left) {                         // the next SUB rows, of which `left` are there
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            if (j < left) {
+                xr[j] = *xp, dr[j] = *dp;
+                if (gate) zr[j] = *zp;
+            } else {
+                xr[j] = dr[j] = from_f<E>(0.f);
+            }
+            xp += a.ldx, dp += a.lddt;
+            if (FULL) zp += ldz;
+        }
     };
     float next[PER];
     auto bc_in = [&](int t) {                              // this thread's share of a tile of B and C
@@ -101,8 +127,7 @@ __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S
         }
     };
     bc_in(t0);
-#pragma unroll
-    for (int j = 0; j < TT; ++j) row_in(j, t0 + j);
+    rows_in(t1 - t0);
     bc_out(0);
     __syncthreads();
     float total = 0.f;
@@ -111,38 +136,50 @@ __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S
         const bool more = t + TT < t1;
         if (more) bc_in(t + TT);
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            const float xv = to_f(xr[j]);
-            float dtv = to_f(dr[j]);
-            float zv = 0.f;
-            if (FULL) zv = to_f(zr[j]);
-            row_in(j, t + TT + j);                         // a tile ahead, into the registers just read
-            if (a.pj.on) dtv = fmaf(a.pj.range, sigmoid_fast(dtv), a.pj.lo);
-            if (t + j >= t1) dtv = 0.f;                    // decay 1, nothing added
-            if (!FULL) total += dtv;
-            const float2 dt2 = f2(dtv, dtv), bx2 = f2(dtv * xv, dtv * xv);
-            const float4 *bp = reinterpret_cast<const float4 *>(&bc[buf][j][0][g * NS]);
-            const float4 *cp = reinterpret_cast<const float4 *>(&bc[buf][j][1][g * NS]);
-            float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        for (int sub = 0; sub < TT; sub += SUB) {
+            const int left = t1 - t - sub;                 // rows from here on
+            if (sub > 0 && left <= 0) break;
+            float xf[SUB], df[SUB], gf[SUB];
 #pragma unroll
-            for (int q = 0; q < NS / 4; ++q) {
-                const float4 Bv = bp[q];
-                h[2 * q] = fma2(ex2x2(mul2(dt2, nan2[2 * q])), h[2 * q], mul2(bx2, lo(Bv)));
-                h[2 * q + 1] = fma2(ex2x2(mul2(dt2, nan2[2 * q + 1])), h[2 * q + 1], mul2(bx2, hi(Bv)));
-                if (FULL) {
-                    const float4 Cv = cp[q];
-                    acc[0] = fma2(lo(Cv), h[2 * q], acc[0]);
-                    acc[1] = fma2(hi(Cv), h[2 * q + 1], acc[1]);
-                }
+            for (int j = 0; j < SUB; ++j) xf[j] = to_f(xr[j]), df[j] = to_f(dr[j]), gf[j] = 1.f;
+            if (a.pj.on) {
+#pragma unroll
+                for (int j = 0; j < SUB; ++j) df[j] = j < left ? fmaf(a.pj.range, sigmoid_fast(df[j]), a.pj.lo) : 0.f;
             }
-            if (FULL) {
-                acc[0] = add2(acc[0], acc[1]);
-                float yv = acc[0].x + acc[0].y;
+            if (gate) {
 #pragma unroll
-                for (int o = S::G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
-                yv += skip;
-                if (gate) yv *= zv * sigmoid_fast(zv);
-                if (act && g == 0 && t + j < t1) a.y[(long long)(t + j) * a.D + d] = from_f<E>(yv);
+                for (int j = 0; j < SUB; ++j) gf[j] = to_f(zr[j]) * sigmoid_fast(to_f(zr[j]));
+            }
+            rows_in(left - SUB);
+            // rows behind the last have dt = 0: decay 1, nothing added
+#pragma unroll
+            for (int j = 0; j < SUB; ++j) {
+                const float2 dt2 = f2(df[j], df[j]), bx2 = f2(df[j] * xf[j], df[j] * xf[j]);
+                if (!FULL) total += df[j];
+                const float4 *bp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][0][g * NS]);
+                const float4 *cp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][1][g * NS]);
+                float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+                for (int q = 0; q < NS / 4; ++q) {
+                    const float4 Bv = bp[q];
+                    const float2 e0 = mul2(dt2, nan2[2 * q]), e1 = mul2(dt2, nan2[2 * q + 1]);
+                    h[2 * q] = fma2(2 * q < POLY ? ex2_poly2(e0) : ex2x2(e0), h[2 * q], mul2(bx2, lo(Bv)));
+                    h[2 * q + 1] = fma2(2 * q + 1 < POLY ? ex2_poly2(e1) : ex2x2(e1), h[2 * q + 1], mul2(bx2, hi(Bv)));
+                    if (FULL) {
+                        const float4 Cv = cp[q];
+                        acc[0] = fma2(lo(Cv), h[2 * q], acc[0]);
+                        acc[1] = fma2(hi(Cv), h[2 * q + 1], acc[1]);
+                    }
+                }
+                if (FULL) {
+                    acc[0] = add2(acc[0], acc[1]);
+                    float yv = acc[0].x + acc[0].y;
+#pragma unroll
+                    for (int o = S::G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
+                    yv = (yv + skip) * gf[j];
+                    if (act && g == 0 && j < left) *yp = from_f<E>(yv);
+                    yp += a.D;
+                }
             }
         }
         if (more) {
@@ -191,7 +228,7 @@ __device__ __forceinline__ void read_rates(float2 (&nan2)[S::NS / 2], const floa
 }
 
 template <typename E, typename BE, typename S, bool REST>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, MMS_PACKED_MINB)
 scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
 {
     __shared__ __align__(16) float bc[2][TT][2][S::NP];
@@ -210,8 +247,9 @@ scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
     const int first = a.seq.start(s), end = max(first, a.seq.start(s + 1));
     const int i = unit - (s + first / a.seg);
     const int segs = max(1, (end - first + a.seg - 1) / a.seg);
-    // the first launch: first segments, and the end states of those before the last
-    if (i < 0 || i >= segs || (REST ? i == 0 : i > 0 && i == segs - 1)) return;
+    if (i < 0 || i >= segs) return;
+    const bool split = segs > FEW;                         // its first segment is left for the second launch, too
+    if (REST ? i == 0 && !split : i > 0 && i == segs - 1) return;
 
     const int d = (blockIdx.x % a.nd) * S::DPB + tid / S::G;
     const bool act = d < a.D;
@@ -221,13 +259,19 @@ scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
     read_rates<S>(nan2, a.aneg + at, a.N, g, act, a.pj.on);
     const long long row = first / a.seg;                   // of the sequence's first end state
     const size_t DN = (size_t)a.D * a.N;
-    if (!REST && i == 0) {
+    // a sequence of more than FEW segments has more than FEW * seg rows: the next one's is another
+    float *entry = a.entry + (size_t)(first / (FEW * a.seg)) * DN + at;
+    if (i == 0) {
         const long long from = a.seq.from(s);
-        read_state<S>(h, a.state + (from >= 0 ? from : 0) * DN + at, a.N, g, act && from >= 0);
+        if (REST) read_state<S>(h, entry, a.N, g, act);
+        else read_state<S>(h, a.state + (from >= 0 ? from : 0) * DN + at, a.N, g, act && from >= 0);
+        // (its last segment may write the place that it was read from)
+        if (!REST && split) write_state<S>(h, entry, a.N, g, act);
     } else if (REST) {
         // the states at the ends of the segments before: of the first as it is, of the others
         // what was left of the one before and their own
         read_state<S>(h, a.ends + row * DN + at, a.N, g, act);
+#pragma unroll 2
         for (int j = 1; j < i; ++j) {
             float2 v[S::NS / 2];
             read_state<S>(v, a.ends + (row + j) * DN + at, a.N, g, act);
@@ -239,7 +283,7 @@ scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
 #pragma unroll
         for (int q = 0; q < S::NS / 2; ++q) h[q] = f2(0.f, 0.f);
     }
-    if (REST || i == 0) {
+    if (REST || (i == 0 && !split)) {
         walk<true, E, BE, S>(a, bc, h, nan2, t0, t1, d, g, act);
     } else {
         const float total = walk<false, E, BE, S>(a, bc, h, nan2, t0, t1, d, g, act);
@@ -337,6 +381,9 @@ int segment_rows(int rows, int D, int N)
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
 }
 
+// Sequences of more than FEW segments are told apart by start / (FEW * seg).
+int entries_of(int rows, int seg) { return rows > FEW * seg ? rows / (FEW * seg) + 1 : 0; }
+
 template <typename E, typename BE>
 Args<E, BE> args_of(const ScanPackedArgs &p)
 {
@@ -357,7 +404,8 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
     a.seg = segment_rows(rows, p.D, p.N);
     a.nd = (p.D + S::DPB - 1) / S::DPB;
     a.ends = static_cast<float *>(p.workspace);
-    a.sums = a.ends + (size_t)(rows / a.seg) * p.D * p.N;
+    a.entry = a.ends + (size_t)(rows / a.seg) * p.D * p.N;
+    a.sums = a.entry + (size_t)entries_of(rows, a.seg) * p.D * p.N;
     const long long units = (long long)p.seq.count + rows / a.seg;
     const long long clear = 2 * N_SM;
     if (units * a.nd + clear > 0x7fffffffLL) return cudaErrorInvalidValue;
@@ -404,12 +452,13 @@ cudaError_t packed_of(const ScanPackedArgs &p, cudaStream_t stream)
 
 }  // namespace
 
-// Segments before the last of their sequence: at most one for every `seg` rows.
+// Segments before the last of their sequence, at most one for every `seg` rows, and entries.
 size_t scan_packed_workspace_bytes(int rows, int count, int D, int N)
 {
     (void)count;
-    const size_t n = rows / segment_rows(rows, D, N);
-    return n * D * (N + 1) * sizeof(float);
+    const int seg = segment_rows(rows, D, N);
+    const size_t ends = rows / seg, entries = entries_of(rows, seg);
+    return (ends * (N + 1) + entries * N) * D * sizeof(float);
 }
 
 cudaError_t launch_scan_packed(const ScanPackedArgs &p, cudaStream_t stream)

@@ -11,18 +11,23 @@
 // given by its last entry: (tau, ti) keeps z > tau, and z == tau up to index ti.
 //
 // A sum next to a border decides a token, and sums of 131072 weights in float32 are
-// off by more than the distance between neighbours: weights and sums are doubles, in a
-// fixed order (a lane, a warp, then the warps in order), so a call's result is the
-// same every time. No order of atomics reaches it: what they collect is counted in
-// whole numbers, or sorted.
+// off by more than the distance between neighbours. Weights are computed in float64
+// and held as whole numbers of 2^-45 of the largest (fewer bits above 2^17 entries, so that
+// no sum passes 2^62): their sums are exact in any order, so bins may be filled by atomics
+// and a call's result is the same every time.
 //
 // A row is read by a cluster of C CTAs; warp q of all of theirs has the q-th piece of the
-// row in every pass, so that sums in index order are sums over warps. The k-th largest
-// entry and the end of the mass p are found by bins over the range of the logits: counts or
-// fixed-point weights of 2048 equal bins, then the bin in question is made the range,
-// until it holds one value or few enough entries to sort. Whole-number bins only choose
-// where to look: the weights before the bin are summed again as doubles, and a bin
-// that was chosen wrongly by the rounding of the fixed-point weights is left for its neighbour.
+// row in every pass, so that sums in index order are sums over warps.
+//   k up to 256 C: every warp has the j-th largest of its 32 lanes' maxima, j = k / warps
+//     rounded up; the smallest of these has k entries above it or equal, and not many
+//     more. Those are listed and sorted, and all else happens on the list.
+//   else: the end of the run of k entries, and of the mass p, is found by bins over the
+//     range of the logits, counts or weights of 2048 equal bins; then the bin in question
+//     becomes the range, until it holds one value or few enough entries to sort.
+// The row is read from HBM once; the later passes, one to five, find it in L2.
+
+#include <float.h>
+
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -35,10 +40,14 @@ namespace mms {
 
 namespace {
 
+using u64 = unsigned long long;
 constexpr int THREADS = 512, NW = THREADS / 32;
 constexpr int BINS = 2048;
 constexpr int CAP = 2048;               // entries that are sorted rather than divided further
+constexpr int PER = BINS / THREADS;     // bins, and list entries, of a thread
+static_assert(CAP == BINS, "one scan serves both");
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr int EVERY = 0x7fffffff;       // ti: all entries equal to tau
 
 // Larger keys for larger floats; -0 and 0 are one value.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -49,80 +58,17 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// What the CTAs of a row tell one another.
-struct Part {
-    double mass, bin_mass;              // weight of the bins before the one in question, and of it
-    float lo, hi;                       // smallest and largest value of the bin
-    float before, after;                // smallest value of the bins before, largest of those after
-    int bin_count;
-    float top;                          // largest value, and its lowest index
-    int top_at;
-    float least;                        // smallest value above -inf
-    int nan;
-};
-
 struct Shared {
-    unsigned long long bins[BINS];      // counts, or fixed-point weights
-    unsigned long long list[CAP];       // (key, index), to be sorted so that the largest value comes first
-    unsigned long long warp_bins[NW];
-    double warp_mass[NW];               // of the CTA's warps
-    double all_mass[8 * NW];            // of all the row's warps
-    int warp_count[NW], all_count[8 * NW];
-    Part part, warp_part[NW];
-    int listed;
-    float tau;
-    int ti;
-    int bin;
-    int token;
-    double weight;
-};
-
-// The row as one CTA sees it.
-template <typename E, int C>
-struct Row {
-    static constexpr int VEC = 16 / (int)sizeof(E);
-    const E *p;
-    int vocab, off;                     // entries before p back to a 16-byte boundary
-    int from, to;                       // this warp's piece, counted from that boundary
-    float top;
-    double rate;                        // 1 / T
-    float tau;
-    int ti;
-
-    __device__ __forceinline__ double weight(float v) const {
-        if (isinf(top)) return v == top ? 1.0 : 0.0;
-        return exp(((double)v - (double)top) * rate);
-    }
-    __device__ __forceinline__ bool kept(float v, int i) const { return v > tau || (v == tau && i <= ti); }
-
-    // f(value, index) over the piece, 32 * VEC entries at a time; lane l has VEC neighbours
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const {
-        const int lane = threadIdx.x & 31;
-        constexpr int UN = 2;
-        for (int at = from; at < to; at += 32 * VEC * UN) {
-            E v[UN][VEC];
-#pragma unroll
-            for (int q = 0; q < UN; ++q) read(v[q], at + (q * 32 + lane) * VEC);
-#pragma unroll
-            for (int q = 0; q < UN; ++q)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int i = at + (q * 32 + lane) * VEC + j - off;
-                    if (i >= 0 && i < vocab && i + off < to) f(to_f(v[q][j]), i);
-                }
-        }
-    }
-    // entries at .. at + VEC - 1 of the piece; those outside the row are left as they are
-    __device__ __forceinline__ void read(E (&v)[VEC], int at) const {
-        if (at >= off && at + VEC <= vocab + off) {
-            *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(p - off + at));
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (at + j >= off && at + j < vocab + off) v[j] = p[at + j - off];
-        }
-    }
+    u64 bins[BINS];                     // counts or weights
+    u64 list[CAP];
+    double powers[16];                  // 2^(j / 16)
+    u64 warp_sum[NW];                   // of the CTA's warps
+    u64 all_sum[8 * NW];                // of all the row's warps
+    float warp_max[NW], warp_pivot[NW], warp_lo[NW], warp_hi[NW];
+    u64 before;                         // what lies before the bin in question
+    u64 scan[NW];
+    float top, pivot, lo, hi;
+    int listed, bin, least, tau_key, ti;
 };
 
 template <int C>
@@ -141,87 +87,186 @@ __device__ __forceinline__ int rank_of() {
     else return 0;
 }
 
-__device__ __forceinline__ double warp_sum(double v) {
+// max that hands a NaN on
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <typename F>
+__device__ __forceinline__ float warp_fold(float v, F f) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
-
-// Every warp's value (lane-wise `v`) to sh.all_mass of all CTAs, in the row's order.
-template <int C>
-__device__ double row_sums(Shared &sh, double v)
-{
-    const int warp = threadIdx.x >> 5;
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) sh.warp_mass[warp] = v;
-    row_sync<C>();
-    for (int i = threadIdx.x; i < C * NW; i += THREADS) sh.all_mass[i] = of_rank<C>(sh.warp_mass, i / NW)[i % NW];
-    row_sync<C>();
-    double total = 0.0;
-    for (int i = 0; i < C * NW; ++i) total += sh.all_mass[i];
-    return total;
-}
-template <int C>
-__device__ int row_counts(Shared &sh, int v)
-{
-    const int warp = threadIdx.x >> 5;
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) sh.warp_count[warp] = v;
-    row_sync<C>();
-    for (int i = threadIdx.x; i < C * NW; i += THREADS) sh.all_count[i] = of_rank<C>(sh.warp_count, i / NW)[i % NW];
-    row_sync<C>();
-    int total = 0;
-    for (int i = 0; i < C * NW; ++i) total += sh.all_count[i];
-    return total;
-}
-
-__device__ __forceinline__ void join(Part &a, const Part &b)
-{
-    a.mass += b.mass, a.bin_mass += b.bin_mass, a.bin_count += b.bin_count;
-    a.lo = fminf(a.lo, b.lo), a.hi = fmaxf(a.hi, b.hi);
-    a.before = fminf(a.before, b.before), a.after = fmaxf(a.after, b.after);
-    if (b.top > a.top || (b.top == a.top && b.top_at < a.top_at)) a.top = b.top, a.top_at = b.top_at;
-    a.least = fminf(a.least, b.least);
-    a.nan |= b.nan;
-}
-__device__ __forceinline__ Part no_part()
-{
-    return Part{0.0, 0.0, -NEG_INF, NEG_INF, -NEG_INF, NEG_INF, 0, NEG_INF, 0x7fffffff, -NEG_INF, 0};
-}
-
-// Parts of all lanes joined in the row's order; every thread gets the whole.
-template <int C>
-__device__ Part row_part(Shared &sh, Part v)
-{
-    const int warp = threadIdx.x >> 5;
+__device__ __forceinline__ u64 warp_scan(u64 v) {          // inclusive
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Part b;
-        b.mass = __shfl_xor_sync(0xffffffffu, v.mass, o), b.bin_mass = __shfl_xor_sync(0xffffffffu, v.bin_mass, o);
-        b.lo = __shfl_xor_sync(0xffffffffu, v.lo, o), b.hi = __shfl_xor_sync(0xffffffffu, v.hi, o);
-        b.before = __shfl_xor_sync(0xffffffffu, v.before, o), b.after = __shfl_xor_sync(0xffffffffu, v.after, o);
-        b.bin_count = __shfl_xor_sync(0xffffffffu, v.bin_count, o);
-        b.top = __shfl_xor_sync(0xffffffffu, v.top, o), b.top_at = __shfl_xor_sync(0xffffffffu, v.top_at, o);
-        b.least = __shfl_xor_sync(0xffffffffu, v.least, o), b.nan = __shfl_xor_sync(0xffffffffu, v.nan, o);
-        join(v, b);
+    for (int o = 1; o < 32; o *= 2) {
+        const u64 b = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += b;
     }
-    if ((threadIdx.x & 31) == 0) sh.warp_part[warp] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        v = sh.warp_part[0];
-        for (int i = 1; i < NW; ++i) join(v, sh.warp_part[i]);
-        sh.part = v;
-    }
-    row_sync<C>();
-    v = *of_rank<C>(&sh.part, 0);
-    for (int r = 1; r < C; ++r) join(v, *of_rank<C>(&sh.part, r));
-    row_sync<C>();
     return v;
 }
+// What the threads before this one hold together (sh.scan; every thread gets the whole in `all`).
+__device__ __forceinline__ u64 block_before(Shared &sh, u64 v, u64 &all) {
+    const int warp = threadIdx.x >> 5;
+    const u64 upto = warp_scan(v);
+    __syncthreads();                                       // sh.scan of a call before
+    if ((threadIdx.x & 31) == 31) sh.scan[warp] = upto;
+    __syncthreads();
+    u64 r = upto - v;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        if (w < warp) r += sh.scan[w];
+        all += sh.scan[w];
+    }
+    return r;
+}
 
-// The list sorted ascending, padded with ones to a power of two.
-__device__ void sort_list(unsigned long long *list, int n)
+// 16 bytes of a row.
+template <typename E>
+struct Words {
+    static constexpr int VEC = 16 / (int)sizeof(E);
+    uint4 q;
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(E) == 4) return __uint_as_float(word(j));
+        else return __uint_as_float(j & 1 ? word(j >> 1) & 0xffff0000u : word(j >> 1) << 16);
+    }
+};
+
+// The row as one CTA sees it. Places count from the 16-byte boundary at or before its start.
+template <typename E, int C>
+struct Row {
+    static constexpr int VEC = Words<E>::VEC, STEP = 32 * VEC;
+    const E *p;                         // that boundary
+    int off, end;                       // first place, and the one behind the last
+    int piece;                          // places of a warp's piece, whole steps
+    float top;
+    double rate;                        // 1 / T
+    int bits;                           // weights are whole numbers of 2^-bits
+    const double *powers;
+    float tau;
+    int ti;
+
+    __device__ __forceinline__ int from(int w) const { return (int)min((long long)w * piece, (long long)end); }
+
+    // (v - top) / T
+    __device__ __forceinline__ double exponent(float v) const { return ((double)v - (double)top) * rate; }
+    // 2^bits e^exponent, rounded. e^x = 2^(k / 16) e^r, |r| <= log(2) / 32, the first factor from a
+    // table, the second to r^6: what is left out is r^7 / 5040 < 5e-16 (table-driven exponentials
+    // after Tang, 1989).
+    __device__ __forceinline__ u64 weight(float v) const {
+        if (isinf(top)) return v == top ? 1ull << bits : 0ull;
+        const double x = exponent(v);
+        if (!(x > -45.0)) return 0;                        // below 2^-64
+        constexpr double ROUND = 6755399441055744.0;       // 1.5 * 2^52: the sum's last bit is worth 1
+        const double m = fma(x, 16.0 * 1.4426950408889634, ROUND);
+        const int k = __double2loint(m);
+        const double r = fma(m - ROUND, -0.69314718055994531 / 16.0, x);
+        double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+        e = fma(e, r, 1.0 / 24.0);
+        e = fma(e, r, 1.0 / 6.0);
+        e = fma(e, r, 0.5);
+        e = fma(e, r, 1.0);
+        e = fma(e, r, 1.0);
+        e *= powers[k & 15];
+        e = __hiloint2double(__double2hiint(e) + (((k >> 4) + bits) << 20), __double2loint(e));
+        return (u64)__double_as_longlong(e + 4503599627370496.0) & ((1ull << 52) - 1);
+    }
+    __device__ __forceinline__ bool kept(float v, int i) const { return v > tau || (v == tau && i <= ti); }
+
+    // 16 bytes at a place; entries outside the row are -inf
+    __device__ __forceinline__ Words<E> read(int at) const {
+        Words<E> v;
+        if (at >= off && at + VEC <= end) {
+            v.q = __ldg(reinterpret_cast<const uint4 *>(p + at));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(E) == 4) {
+                    w[i] = at + i >= off && at + i < end ? __float_as_uint(to_f(p[at + i])) : 0xff800000u;
+                } else {
+                    uint32_t h[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int a = at + 2 * i + j;
+                        h[j] = a >= off && a < end ? __float_as_uint(to_f(p[a])) >> 16 : 0xff80u;
+                    }
+                    w[i] = h[0] | h[1] << 16;
+                }
+            }
+            v.q = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return v;
+    }
+    // f(words, place of the first) over the warp's share [a, b) of the row, a multiple of STEP;
+    // several loads at a time. Entries of a step are all within [a, b) or outside the row.
+    template <typename F>
+    __device__ __forceinline__ void words(int a, int b, F f) const {
+        const int lane = threadIdx.x & 31;
+        constexpr int UN = 4;
+        int at = a;
+        for (; at + (UN - 1) * STEP < b; at += UN * STEP) {
+            Words<E> v[UN];
+#pragma unroll
+            for (int q = 0; q < UN; ++q) v[q] = read(at + q * STEP + lane * VEC);
+#pragma unroll
+            for (int q = 0; q < UN; ++q) f(v[q], at + q * STEP + lane * VEC);
+        }
+        for (; at < b; at += STEP) f(read(at + lane * VEC), at + lane * VEC);
+    }
+    // f(value, index) for entries above -inf
+    template <typename F>
+    __device__ __forceinline__ void each(int a, int b, F f) const {
+        words(a, b, [&](const Words<E> &v, int at) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float x = v.at(j);
+                if (x > NEG_INF) f(x, at + j - off);
+            }
+        });
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int w = rank_of<C>() * NW + (threadIdx.x >> 5);
+        each(from(w), from(w + 1), f);
+    }
+};
+
+// Every warp's value to sh.all_sum of all CTAs, in the row's order.
+template <int C>
+__device__ __forceinline__ void row_sums(Shared &sh, u64 v)
+{
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = v;
+    row_sync<C>();
+    if (threadIdx.x < C * NW) sh.all_sum[threadIdx.x] = of_rank<C>(sh.warp_sum, threadIdx.x / NW)[threadIdx.x % NW];
+    row_sync<C>();
+}
+// A float of every warp joined over the row (`mine` and `all` in shared memory).
+template <int C, typename F>
+__device__ __forceinline__ float row_fold(float (&mine)[NW], float v, F f)
+{
+    v = warp_fold(v, f);
+    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = v;
+    row_sync<C>();
+    // lane l of every warp joins the warps l, l + 32, ... of the row
+    const int lane = threadIdx.x & 31;
+    v = of_rank<C>(mine, (lane % (C * NW)) / NW)[lane % NW];
+    for (int i = lane + 32; i < C * NW; i += 32) v = f(v, of_rank<C>(mine, i / NW)[i % NW]);
+    return warp_fold(v, f);
+}
+
+// The first n entries of sh.list sorted ascending (behind them: ones, up to a power of two).
+__device__ void sort_list(u64 *list, int n)
 {
     int m = 2;
     while (m < n) m *= 2;
@@ -231,44 +276,72 @@ __device__ void sort_list(unsigned long long *list, int n)
             __syncthreads();
             for (int i = threadIdx.x; i < m / 2; i += THREADS) {
                 const int a = 2 * i - (i & (gap - 1)), b = a + gap;
-                const unsigned long long x = list[a], y = list[b];
+                const u64 x = list[a], y = list[b];
                 if ((x > y) == ((a & size) == 0)) list[a] = y, list[b] = x;
             }
         }
     __syncthreads();
+}
+// List entries that sort by rank (z descending, index ascending), and by index.
+__device__ __forceinline__ u64 ranked(float v, int i) { return (u64)(~key_of(v)) << 32 | (unsigned)i; }
+__device__ __forceinline__ float ranked_value(u64 e) { return of_key(~(uint32_t)(e >> 32)); }
+
+// The first index of 0 .. n - 1 at which the sums of value(i) reach `target` (n - 1 if none does).
+template <typename F>
+__device__ int reached(Shared &sh, int n, u64 target, F value)
+{
+    u64 v[PER], sum = 0, all;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int i = threadIdx.x * PER + q;
+        v[q] = i < n ? value(i) : 0;
+        sum += v[q];
+    }
+    if (threadIdx.x == 0) sh.least = n - 1;
+    u64 upto = block_before(sh, sum, all);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const u64 lo = upto;
+        upto += v[q];
+        if (lo < target && upto >= target) atomicMin(&sh.least, threadIdx.x * PER + q);
+    }
+    __syncthreads();
+    return sh.least;
+}
+
+// ceil(share * sum) as the sum that has to be reached
+__device__ __forceinline__ u64 share_of(float share, u64 sum) {
+    return max(1ull, (u64)ceil((double)share * (double)sum));
+}
+// sums above this one pass u * sum; below `sum`, as u is below 1
+__device__ __forceinline__ u64 border_of(float u, u64 sum) {
+    u = u > 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
+    return min((u64)((double)u * (double)sum), sum - 1);
 }
 
 // The index of the n-th (from 1) kept entry equal to `value`.
 template <typename E, int C>
 __device__ int nth_equal(Shared &sh, const Row<E, C> &row, float value, int n)
 {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = rank_of<C>();
-    int mine = 0;
-    row.each([&](float v, int i) { mine += v == value && row.kept(v, i); });
-    row_counts<C>(sh, mine);
-    int w = 0, left = n;
-    while (w < C * NW - 1 && left > sh.all_count[w]) left -= sh.all_count[w++];
-    if (w == rank * NW + warp) {
-        constexpr int VEC = Row<E, C>::VEC;
-        for (int at = row.from; at < row.to; at += 32 * VEC) {
-            E v[VEC];
-            row.read(v, at + lane * VEC);
+    const int lane = threadIdx.x & 31, mine = rank_of<C>() * NW + (threadIdx.x >> 5);
+    u64 count = 0;
+    row.each([&](float v, int i) { count += v == value && row.kept(v, i); });
+    row_sums<C>(sh, count);
+    int w = 0;
+    u64 left = n;
+    while (w < C * NW - 1 && left > sh.all_sum[w]) left -= sh.all_sum[w++];
+    if (w == mine) {
+        for (int at = row.from(w); at < row.from(w + 1); at += row.STEP) {
+            const Words<E> v = row.read(at + lane * row.VEC);
             unsigned hits = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int i = at + lane * VEC + j - row.off;
-                if (i >= 0 && i < row.vocab && i + row.off < row.to && to_f(v[j]) == value && row.kept(value, i)) hits |= 1u << j;
-            }
-            int upto = __popc(hits);
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int b = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += b;
-            }
-            const int before = upto - __popc(hits), all = __shfl_sync(0xffffffffu, upto, 31);
+            for (int j = 0; j < Row<E, C>::VEC; ++j)
+                if (v.at(j) == value && row.kept(value, at + lane * row.VEC + j - row.off)) hits |= 1u << j;
+            const u64 upto = warp_scan(__popc(hits)), before = upto - __popc(hits);
+            const u64 all = __shfl_sync(0xffffffffu, upto, 31);
             if (left > before && left <= upto) {
-                for (int k = left - before; k > 1; --k) hits &= hits - 1;
-                const int i = at + lane * VEC + __ffs(hits) - 1 - row.off;
+                for (u64 k = left - before; k > 1; --k) hits &= hits - 1;
+                const int i = at + lane * row.VEC + __ffs(hits) - 1 - row.off;
                 for (int r = 0; r < C; ++r) of_rank<C>(&sh, r)->ti = i;
             }
             if (left <= all) break;
@@ -279,245 +352,303 @@ __device__ int nth_equal(Shared &sh, const Row<E, C> &row, float value, int n)
     return sh.ti;
 }
 
-// Cuts what is kept to the shortest run of the ranking that reaches `target`: so many
-// entries (MASS false), or so much weight. Where all of it does not, nothing changes.
-// Every round ends in a smaller [a, b]; MOST bounds them all the same.
+// Cuts what is kept to the shortest run of the ranking that reaches `target` entries
+// (MASS false) or the share `share` of the weight kept before. [a, b]: the range that the end
+// of the run lies in, smaller in every round; MOST bounds the rounds all the same.
 template <bool MASS, typename E, int C>
-__device__ void cut(Shared &sh, Row<E, C> &row, double target, float least)
+__device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a)
 {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = rank_of<C>();
-    float a = fmaxf(least, row.tau), b = row.top;          // the last entry of the run lies in [a, b]
-    double above = 0.0;                                    // what lies above b
-    // fixed point of the bins' weights: sums of all entries stay below 2^63
-    const double unit = MASS ? exp2((double)min(45, 62 - (32 - __clz(row.vocab)))) : 1.0;
+    const int tid = threadIdx.x, rank = rank_of<C>();
+    float b = row.top;
+    u64 above = 0;                                         // what lies above b
     constexpr int MOST = 100;
     for (int round = 0; round < MOST; ++round) {
         const double scale = BINS / ((double)b - (double)a);
         auto bin_of = [&](float v) { return a == b ? 0 : min(BINS - 1, (int)(((double)b - (double)v) * scale)); };
-        // where no sum reaches the target by the rounding of the weights: the bin of the smallest value
-        const int last = a == b ? 0 : BINS - 1;
         for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
-        if (tid == 0) sh.listed = 0, sh.bin = last;
+        if (tid == 0) sh.listed = 0;
         __syncthreads();
+        u64 beside = 0;                                    // kept below the range, in the first round
         row.each([&](float v, int i) {
-            if (v <= b && v >= a && row.kept(v, i))
-                atomicAdd(&sh.bins[bin_of(v)], MASS ? (unsigned long long)(row.weight(v) * unit) : 1ull);
+            if (v > b || !row.kept(v, i)) return;
+            const u64 w = MASS ? row.weight(v) : 1ull;
+            if (w == 0) return;
+            if (v >= a) atomicAdd(&sh.bins[bin_of(v)], w);
+            else if (round == 0) beside += w;
         });
-        row_sync<C>();
+        if (MASS && round == 0) row_sums<C>(sh, beside);
+        else row_sync<C>();
         // each thread's bins of the whole row, then where the sum reaches the target
-        constexpr int PER = BINS / THREADS;
-        unsigned long long mine[PER], sum = 0;
+        u64 mine[PER], sum = 0, all;
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             mine[q] = 0;
             for (int r = 0; r < C; ++r) mine[q] += of_rank<C>(sh.bins, r)[tid * PER + q];
             sum += mine[q];
         }
-        unsigned long long upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
+        u64 upto = block_before(sh, sum, all);
+        if (MASS && round == 0) {
+            u64 kept = all;
+            for (int w = 0; w < C * NW; ++w) kept += sh.all_sum[w];
+            target = share_of(share, kept);
         }
-        if (lane == 31) sh.warp_bins[warp] = upto;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) upto += sh.warp_bins[w];
-        upto -= sum;
-        const double want = fmax(0.0, (target - above) * unit);
+        if (above + all < target) {                        // the whole range is kept, and more is not there
+            row_sync<C>();
+            break;
+        }
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
-            const double lo = (double)upto;
+            const u64 lo = above + upto;
             upto += mine[q];
-            if (lo < want && (double)upto >= want) atomicMin(&sh.bin, tid * PER + q);
+            if (lo < target && above + upto >= target) sh.bin = tid * PER + q, sh.before = lo;
         }
-        row_sync<C>();                                     // the bins are read, the bin is known
+        row_sync<C>();                                     // bins read, the bin known
         const int bin = sh.bin;
-        // the bins before it and it itself, as doubles; its entries to the list
-        Part p = no_part();
+        const u64 before = sh.before;
+        float lo = -NEG_INF, hi = NEG_INF;
         row.each([&](float v, int i) {
-            if (v > b || v < a || !row.kept(v, i)) return;
-            const int k = bin_of(v);
-            const double w = MASS ? (k <= bin ? row.weight(v) : 0.0) : 1.0;
-            if (k < bin) {
-                p.mass += w;
-                p.before = fminf(p.before, v);
-            } else if (k > bin) {
-                p.after = fmaxf(p.after, v);
-            } else {
-                p.bin_mass += w;
-                p.lo = fminf(p.lo, v), p.hi = fmaxf(p.hi, v);
-                ++p.bin_count;
-                const int at = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
-                if (at < CAP) of_rank<C>(&sh, 0)->list[at] = (unsigned long long)(~key_of(v)) << 32 | (unsigned)i;
-            }
+            if (v > b || v < a || !row.kept(v, i) || bin_of(v) != bin) return;
+            lo = fminf(lo, v), hi = fmaxf(hi, v);
+            const int at = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
+            if (at < CAP) of_rank<C>(&sh, 0)->list[at] = ranked(v, i);
         });
-        p = row_part<C>(sh, p);
-        const double ahead = above + p.mass;
-        if (p.before <= b && ahead >= target) {            // rounding: it is in a bin before
-            a = p.before;
-            continue;
-        }
-        if (p.bin_count == 0 || ahead + p.bin_mass < target) {
-            if (p.after < a) break;                        // all of it does not reach the target
-            above = ahead + p.bin_mass;                    // rounding: it is in a bin behind
-            b = p.after;
-            continue;
-        }
-        if (p.lo == p.hi) {
-            const double each = MASS ? row.weight(p.lo) : 1.0;
-            const int n = (int)fmin((double)p.bin_count, fmax(1.0, ceil((target - ahead) / each)));
-            if (n < p.bin_count) {
-                const int ti = nth_equal(sh, row, p.lo, n);
-                row.ti = ti;
-            } else if (p.lo != row.tau) {
-                row.ti = 0x7fffffff;
+        lo = row_fold<C>(sh.warp_lo, lo, [](float x, float y) { return fminf(x, y); });
+        hi = row_fold<C>(sh.warp_hi, hi, [](float x, float y) { return fmaxf(x, y); });
+        const int n = of_rank<C>(&sh, 0)->listed;
+        if (lo == hi) {
+            const u64 each = MASS ? row.weight(lo) : 1ull;
+            const u64 need = (target - before + each - 1) / each;
+            if (need < (u64)n) {
+                row.ti = nth_equal(sh, row, lo, (int)need);
+            } else {
+                if (lo != row.tau) row.ti = EVERY;
+                row_sync<C>();
             }
-            row.tau = p.lo;
+            row.tau = lo;
             return;
         }
-        if (p.bin_count <= CAP) {
+        if (n <= CAP) {
             if (rank == 0) {
-                sort_list(sh.list, p.bin_count);
-                if (tid == 0) {
-                    double sum = ahead;
-                    int i = 0;
-                    for (; i < p.bin_count - 1; ++i) {
-                        sum += MASS ? row.weight(of_key(~(uint32_t)(sh.list[i] >> 32))) : 1.0;
-                        if (sum >= target) break;
-                    }
-                    sh.tau = of_key(~(uint32_t)(sh.list[i] >> 32));
-                    sh.ti = (int)(uint32_t)sh.list[i];
-                }
+                sort_list(sh.list, n);
+                const int i = reached(sh, n, target - before,
+                                      [&](int q) { return MASS ? row.weight(ranked_value(sh.list[q])) : 1ull; });
+                if (tid == 0) sh.tau_key = (int)key_of(ranked_value(sh.list[i])), sh.ti = (int)(uint32_t)sh.list[i];
             }
             row_sync<C>();
-            row.tau = of_rank<C>(&sh, 0)->tau;
+            row.tau = of_key((uint32_t)of_rank<C>(&sh, 0)->tau_key);
             row.ti = of_rank<C>(&sh, 0)->ti;
             row_sync<C>();
             return;
         }
-        a = p.lo, b = p.hi, above = ahead;
+        a = lo, b = hi, above = before;
+        row_sync<C>();
     }
-    if (a != row.tau) row.ti = 0x7fffffff;
-    row.tau = a;
+    // MASS: entries below the range weigh nothing and may stay
+    if (!MASS) {
+        if (a != row.tau) row.ti = EVERY;
+        row.tau = a;
+    }
+}
+
+// The rest of a row whose candidates are all in sh.list: n entries, of which the k first in rank count.
+template <typename E, int C>
+__device__ void finish_list(Shared &sh, const Row<E, C> &row, const SampleArgs &s, int at, int n, int k, float top_p,
+                            u64 least)
+{
+    const int tid = threadIdx.x;
+    sort_list(sh.list, n);
+    n = min(n, k);
+    // the cuts are prefixes of the sorted list
+    u64 sum = 0, all;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int i = tid + q * THREADS;
+        if (i < n) {
+            const u64 w = row.weight(ranked_value(sh.list[i]));
+            sh.bins[i] = w;
+            sum += w;
+        }
+    }
+    block_before(sh, sum, all);                            // (two barriers: sh.bins is written)
+    if (top_p < 1.f) n = reached(sh, n, share_of(top_p, all), [&](int i) { return sh.bins[i]; }) + 1;
+    __syncthreads();
+    // by index: (index, key), the ones too light last
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int i = tid + q * THREADS;
+        if (i < n) {
+            const u64 e = sh.list[i];
+            sh.list[i] = sh.bins[i] >= least ? (e & 0xffffffffull) << 32 | (uint32_t)~(uint32_t)(e >> 32) : ~0ull;
+        }
+    }
+    sort_list(sh.list, n);
+    auto weight_at = [&](int i) { return sh.list[i] == ~0ull ? 0ull : row.weight(of_key((uint32_t)sh.list[i])); };
+    sum = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int i = tid + q * THREADS;
+        if (i < n) {
+            const u64 w = weight_at(i);
+            sh.bins[i] = w;
+            sum += w;
+        }
+    }
+    block_before(sh, sum, all);
+    const int i = reached(sh, n, border_of(s.uniform[at], all) + 1, [&](int q) { return sh.bins[q]; });
+    if (tid == 0) {
+        const u64 e = sh.list[i];
+        s.token[at] = (int64_t)(e >> 32);
+        if (s.logprob)
+            s.logprob[at] = isinf(row.top) ? (float)-log(ldexp((double)all, -row.bits))
+                                           : (float)(row.exponent(of_key((uint32_t)e)) - log(ldexp((double)all, -row.bits)));
+    }
 }
 
 template <typename E, int C>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_kernel(const __grid_constant__ SampleArgs s)
 {
     __shared__ Shared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = rank_of<C>(), at = blockIdx.x / C;
-    constexpr int VEC = Row<E, C>::VEC;
     Row<E, C> row;
-    row.p = reinterpret_cast<const E *>(s.logits) + at * s.ld;
-    row.vocab = s.vocab;
-    row.off = (int)((reinterpret_cast<uintptr_t>(row.p) & 15) / sizeof(E));
-    const int piece = ((s.vocab + row.off + C * NW - 1) / (C * NW) + 32 * VEC - 1) / (32 * VEC) * (32 * VEC);
-    row.from = (int)min((long long)(rank * NW + warp) * piece, (long long)s.vocab + row.off);
-    row.to = (int)min((long long)row.from + piece, (long long)s.vocab + row.off);
-    row.tau = NEG_INF, row.ti = -1, row.top = 0.f;
+    constexpr int VEC = Row<E, C>::VEC, STEP = Row<E, C>::STEP;
+    const E *start = reinterpret_cast<const E *>(s.logits) + at * s.ld;
+    row.off = (int)((reinterpret_cast<uintptr_t>(start) & 15) / sizeof(E));
+    row.p = start - row.off;
+    row.end = s.vocab + row.off;
+    row.piece = ((row.end + C * NW - 1) / (C * NW) + STEP - 1) / STEP * STEP;
+    row.powers = sh.powers;
+    row.bits = min(45, 62 - (32 - __clz(s.vocab)));
+    row.tau = NEG_INF, row.ti = EVERY;
+    const int w = rank * NW + warp;
+    if (tid < 16) sh.powers[tid] = exp2(tid / 16.0);
+    if (tid == 0) sh.listed = 0, sh.least = EVERY;
 
-    Part p = no_part();
-    row.each([&](float v, int i) {
-        p.nan |= v != v;
-        if (v > p.top) p.top = v, p.top_at = i;
-        if (v > NEG_INF) p.least = fminf(p.least, v);
+    // the largest value (NaN if there is one)
+    float most = NEG_INF;
+    row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) most = max_nan(most, v.at(j));
     });
-    p = row_part<C>(sh, p);
-    row.top = p.top;
-    if (isinf(p.top)) row.tau = p.top, row.ti = 0x7fffffff;        // nothing beside it has weight
     const float t = s.temperature ? s.temperature[at] : s.temperature1;
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
     const float min_p = fminf(s.min_p ? s.min_p[at] : s.min_p1, 1.f);
+    // k entries at least are as large as the smallest of all warps' j-th largest of their lanes' maxima
+    const int j = (int)min((k + C * NW - 1) / (C * NW), 1000ll);
+    const bool listed = k > 1 && k < s.vocab && j <= 16;
+    if (listed) {
+        uint32_t mine = most == most ? key_of(most) : 0, best = 0;
+        for (int q = 0; q < j; ++q) {
+            best = __reduce_max_sync(0xffffffffu, mine);
+            const unsigned has = __ballot_sync(0xffffffffu, mine == best);
+            if (lane == __ffs(has) - 1) mine = 0;
+        }
+        if (lane == 0) sh.warp_pivot[warp] = best ? of_key(best) : NEG_INF;
+    }
+    row.top = row_fold<C>(sh.warp_max, most, [](float x, float y) { return max_nan(x, y); });
     row.rate = 1.0 / (double)t;
     // nothing to draw from, or nothing to draw
-    const bool none = p.nan || !(p.top > NEG_INF) || t != t || top_p != top_p;
+    const bool none = !(row.top > NEG_INF) || t != t || top_p != top_p;
     if (none || t <= 0.f || k == 1 || top_p <= 0.f) {
+        int first = EVERY;
+        if (!none)
+            row.each([&](float v, int i) {
+                if (v == row.top) first = min(first, i);
+            });
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0) atomicMin(&of_rank<C>(&sh, 0)->least, first);
+        row_sync<C>();
         if (rank == 0 && tid == 0) {
-            s.token[at] = none ? -1 : p.top_at;
+            s.token[at] = none ? -1 : sh.least;
             if (s.logprob) s.logprob[at] = none ? __int_as_float(0x7fc00000) : 0.f;
         }
-        if constexpr (C > 1) cg::this_cluster().sync();    // no CTA leaves while another reads its memory
         return;
     }
-    if (k > 0 && k < s.vocab) cut<false>(sh, row, (double)k, p.least);
-    if (top_p < 1.f) {
-        double mass = 0.0;
+    const u64 least = min_p > 0.f ? (u64)ceil(ldexp((double)min_p, row.bits)) : 0;
+    if (listed) {
+        float pivot = of_rank<C>(sh.warp_pivot, (lane % (C * NW)) / NW)[lane % NW];
+        for (int i = lane + 32; i < C * NW; i += 32) pivot = fminf(pivot, of_rank<C>(sh.warp_pivot, i / NW)[i % NW]);
+        pivot = warp_fold(pivot, [](float x, float y) { return fminf(x, y); });
         row.each([&](float v, int i) {
-            if (row.kept(v, i)) mass += row.weight(v);
+            if (v < pivot) return;
+            const int to = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
+            if (to < CAP) of_rank<C>(&sh, 0)->list[to] = ranked(v, i);
         });
-        const double all = row_sums<C>(sh, mass);
-        cut<true>(sh, row, (double)top_p * all, p.least);
+        row_sync<C>();
+        const int n = of_rank<C>(&sh, 0)->listed;
+        row_sync<C>();
+        if (n <= CAP) {
+            if (rank == 0) finish_list(sh, row, s, at, n, (int)k, top_p, least);
+            return;
+        }
     }
-    double mass = 0.0;
-    auto weight = [&](float v, int i) {
-        const double w = row.kept(v, i) ? row.weight(v) : 0.0;
-        return w >= (double)min_p ? w : 0.0;
+    if (isinf(row.top)) row.tau = row.top;                 // nothing beside it has weight
+    if (k > 0 && k < s.vocab) {
+        float lo = -NEG_INF;
+        row.each([&](float v, int) { lo = fminf(lo, v); });
+        lo = row_fold<C>(sh.warp_lo, lo, [](float x, float y) { return fminf(x, y); });
+        row_sync<C>();
+        cut<false>(sh, row, (u64)k, 0.f, fmaxf(lo, row.tau));
+    }
+    // below top - 33 T no weight is left
+    if (top_p < 1.f) cut<true>(sh, row, 0, top_p, fmaxf(row.tau, fmaxf(-FLT_MAX, (float)((double)row.top - 33.0 * (double)t))));
+    auto weight = [&](float v, int i) -> u64 {
+        if (!row.kept(v, i)) return 0;
+        const u64 x = row.weight(v);
+        return x >= least ? x : 0;
     };
+    u64 mass = 0;
     row.each([&](float v, int i) { mass += weight(v, i); });
-    const double all = row_sums<C>(sh, mass);
-    const float u = s.uniform[at];
-    const double want = (u > 0.f ? fmin((double)u, 1.0) : 0.0) * all;
-    // the warp whose piece passes it (or the last that has any weight), then the entry
-    int w = -1;
-    double upto = 0.0, base = 0.0;
-    for (int i = 0; i < C * NW; ++i) {
-        const double m = sh.all_mass[i];
-        if (m > 0.0 && (w < 0 || upto <= want)) w = i, base = upto;
-        upto += m;
-    }
-    if (w == rank * NW + warp) {
-        int token = -1;
-        double of_token = 0.0;
-        for (int a = row.from; a < row.to; a += 32 * VEC) {
-            E v[VEC];
-            row.read(v, a + lane * VEC);
-            double ws[VEC], sum = 0.0;
+    row_sums<C>(sh, mass);
+    u64 all = 0;
+    for (int i = 0; i < C * NW; ++i) all += sh.all_sum[i];
+    const u64 border = border_of(s.uniform[at], all);
+    // the piece, the part of it, then the entry, that pass the border
+    int hit = 0;
+    u64 base = 0;
+    while (hit < C * NW - 1 && base + sh.all_sum[hit] <= border) base += sh.all_sum[hit++];
+    if (hit / NW == rank) {
+        const int a = row.from(hit), b = row.from(hit + 1);
+        const int part = ((b - a + NW - 1) / NW + STEP - 1) / STEP * STEP;
+        auto part_from = [&](int q) { return min(a + q * part, b); };
+        mass = 0;
+        row.each(part_from(warp), part_from(warp + 1), [&](float v, int i) { mass += weight(v, i); });
+        mass = warp_sum(mass);
+        if (lane == 0) sh.scan[warp] = mass;
+        __syncthreads();
+        int q = 0;
+        while (q < NW - 1 && base + sh.scan[q] <= border) base += sh.scan[q++];
+        if (q == warp) {
+            for (int x = part_from(q); x < part_from(q + 1); x += STEP) {
+                const Words<E> v = row.read(x + lane * VEC);
+                u64 ws[VEC], sum = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int i = a + lane * VEC + j - row.off;
-                ws[j] = i >= 0 && i < row.vocab && i + row.off < row.to ? weight(to_f(v[j]), i) : 0.0;
-                sum += ws[j];
-            }
-            double incl = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double b = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += b;
-            }
-            // the lane's first entry past `want`, else its last with weight
-            double run = base + incl - sum;
-            int hit = -1, last = -1;
-            double hit_w = 0.0, last_w = 0.0;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                run += ws[j];
-                if (ws[j] > 0.0) {
-                    const int i = a + lane * VEC + j - row.off;
-                    if (hit < 0 && run > want) hit = i, hit_w = ws[j];
-                    last = i, last_w = ws[j];
+                for (int i = 0; i < VEC; ++i) {
+                    ws[i] = v.at(i) > NEG_INF ? weight(v.at(i), x + lane * VEC + i - row.off) : 0;
+                    sum += ws[i];
                 }
+                const u64 incl = warp_scan(sum);
+                u64 run = base + incl - sum;
+                if (run <= border && run + sum > border) {
+                    bool done = false;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        run += ws[i];
+                        if (!done && run > border) {
+                            done = true;
+                            s.token[at] = x + lane * VEC + i - row.off;
+                            if (s.logprob)
+                                s.logprob[at] = (float)((isinf(row.top) ? 0.0 : row.exponent(v.at(i))) - log(ldexp((double)all, -row.bits)));
+                        }
+                    }
+                }
+                base += __shfl_sync(0xffffffffu, incl, 31);
+                if (base > border) break;
             }
-            const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
-            if (hits) {
-                const int l = __ffs(hits) - 1;
-                token = __shfl_sync(0xffffffffu, hit, l), of_token = __shfl_sync(0xffffffffu, hit_w, l);
-                break;
-            }
-            if (any) {
-                const int l = 31 - __clz(any);
-                token = __shfl_sync(0xffffffffu, last, l), of_token = __shfl_sync(0xffffffffu, last_w, l);
-            }
-            base += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0) {
-            s.token[at] = token;
-            if (s.logprob) s.logprob[at] = (float)log(of_token / all);
         }
     }
-    if constexpr (C > 1) cg::this_cluster().sync();
 }
 
 template <typename E, int C>

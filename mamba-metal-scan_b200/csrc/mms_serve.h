@@ -58,16 +58,20 @@ struct Sequences {
     }
     __device__ __forceinline__ long long from(int s) const { return place(slots, s); }
     __device__ __forceinline__ long long to(int s) const { return place(out_slots.p ? out_slots : slots, s); }
-    // the last s in [0, n) with key(s) <= v for ascending keys, -1 if there is none
+    // The last s in [0, n) with key(s) <= v for ascending keys, -1 if there is none; by a whole
+    // warp, 32 keys at a time (two loads deep up to 1024 sequences).
     template <typename Key>
     __device__ static __forceinline__ int last_at_most(int n, int v, Key key) {
-        int lo = 0, hi = n;
-        while (lo < hi) {
-            const int mid = lo + (hi - lo) / 2;
-            if (key(mid) <= v) lo = mid + 1;
-            else hi = mid;
+        const int lane = threadIdx.x & 31;
+        int lo = 0;
+        while (n > 32) {
+            const int step = (n + 31) / 32, i = lane * step;
+            const int below = __popc(__ballot_sync(0xffffffffu, i < n && key(lo + i) <= v));
+            if (below == 0) return lo - 1;
+            lo += (below - 1) * step;
+            n = min(step, n - (below - 1) * step);
         }
-        return lo - 1;
+        return lo + __popc(__ballot_sync(0xffffffffu, lane < n && key(lo + lane) <= v)) - 1;
     }
 };
 

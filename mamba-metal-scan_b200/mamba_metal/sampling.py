@@ -47,7 +47,7 @@ def sample_tokens_ref(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_
     t, k = column(temperature, torch.float32).double(), column(top_k, torch.int64)
     p, m = column(top_p, torch.float32).double(), column(min_p, torch.float32).double().clamp(max=1.0)
     u = column(uniform, torch.float32).double()
-    u = torch.where(u > 0, u, torch.zeros_like(u)).clamp(max=1.0)
+    u = torch.where(u > 0, u, torch.zeros_like(u)).clamp(max=1.0 - 2.0 ** -24)
     z, index = torch.sort(logits, dim=1, descending=True, stable=True)
     z = z.double()
     top = z[:, :1]
@@ -84,7 +84,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     with one a row. temperature 0 takes the largest logit. logits of -inf are never drawn; a
     row without any above it, or with a NaN, gives -1. With return_logprob also the log of the
     token's share of the kept weights (float32, NaN beside -1). logits float32 or bfloat16 on
-    the CUDA kernel, rows may be strided; weights and sums are float64. Not differentiable.
+    the CUDA kernel, rows may be strided. Weights are float64, in the kernel rounded to whole
+    numbers of 2^-45 of the largest (2^-(61 - log2 V) above 2^17 entries) and summed exactly.
+    Not differentiable.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1 or uniform.shape != logits.shape[:-1]:
         raise ValueError(f"bad shapes: logits {tuple(logits.shape)}, uniform {tuple(uniform.shape)}")

@@ -1,8 +1,10 @@
 """The sampling kernel against sample_tokens_ref: the same tokens, log-probabilities to float32.
 
-Both hold weights and sums in float64, in different orders; a draw or a cut would have to lie
-within about 1e-15 of a border to differ. The log-probability is a float64 rounded once, and the
-reference's too: two roundings of its value apart at most.
+The kernel's weights are float64 rounded to whole numbers of 2^-45 of the largest, at most 2^-46
+off, and their sums are exact; a draw or a cut would have to lie within the sums' error (V 2^-46 at
+most, 2^-46 sqrt(V) as a rule) of a border to differ. The log-probability is the logarithm of a
+float64 quotient rounded once, and the reference's too: two roundings of its value and the kept
+weights' error, V 2^-46 of a sum of at least 1, apart at most.
 """
 from __future__ import annotations
 
@@ -25,7 +27,7 @@ def check(z, u, t=1.0, k=0, p=1.0, m=0.0):
     lp = lp.cpu()
     assert torch.equal(lp.isnan(), wlp.isnan())
     good = ~wlp.isnan()
-    assert ((lp - wlp).abs()[good] <= 2 * 2.0 ** -24 * wlp[good].abs() + 1e-12).all()
+    assert ((lp - wlp).abs()[good] <= 2 * 2.0 ** -24 * wlp[good].abs() + z.shape[-1] * 2.0 ** -46).all()
     assert torch.equal(sample_tokens(on(z), on(u), on(t), on(k), on(p), on(m)).cpu(), want)
     return token
 
