@@ -520,7 +520,7 @@ int mms_conv_packed(const void *x, long long ldx, const void *w, const void *bia
 
 size_t mms_scan_packed_workspace_size(int rows, int count, int D, int N)
 {
-    if (rows < 1 || count < 1 || D < 1 || N < 4 || N > 64 || N % 4 || rows > MMS_SERVE_MAX || D > MMS_SERVE_MAX_DIM) return 0;
+    if (rows < 1 || count < 1 || count > MMS_SERVE_MAX || D < 1 || N < 4 || N > 64 || N % 4 || rows > MMS_SERVE_MAX || D > MMS_SERVE_MAX_DIM) return 0;
     return mms::scan_packed_workspace_bytes(rows, count, D, N);
 }
 

@@ -25,7 +25,12 @@ namespace {
 
 constexpr int WARPS = 4;                // per CTA, each with rows of its own and the same channels
 constexpr int THREADS = 32 * WARPS;
-constexpr int BWD_STEP = 4;             // rows the backward loads at once
+constexpr int TAIL_ROWS = 32;           // rows of packed sequences a warp walks
+// Rows that a warp loads at once, and computes while the next are on their way.
+template <typename E>
+constexpr int FWD_STEP = sizeof(E) == 4 ? 4 : 8;
+template <typename E>
+constexpr int BWD_STEP = sizeof(E) == 4 ? 2 : 4;
 
 // VEC neighbouring channels of a row as they are stored, and as NP pairs of floats (one
 // channel alone: the second of its pair is 0).
@@ -33,17 +38,36 @@ template <int VEC>
 constexpr int NP = (VEC + 1) / 2;
 
 template <typename E, int VEC>
-struct alignas(sizeof(E) * VEC) Pack {
-    E v[VEC];
+struct Pack {
+    static constexpr int WORDS = VEC == 1 ? 1 : VEC * (int)sizeof(E) / 4;
+    uint32_t w[WORDS];
     __device__ __forceinline__ float2 pair(int p) const {
-        if constexpr (VEC == 1) return f2(to_f(v[0]), 0.f);
-        else return f2(to_f(v[2 * p]), to_f(v[2 * p + 1]));
+        if constexpr (sizeof(E) == 4) return VEC == 1 ? f2(__uint_as_float(w[0]), 0.f)
+                                                      : f2(__uint_as_float(w[2 * p % WORDS]), __uint_as_float(w[(2 * p + 1) % WORDS]));
+        else return f2(__uint_as_float(w[p] << 16), VEC == 1 ? 0.f : __uint_as_float(w[p] & 0xffff0000u));
     }
 };
 
 template <typename E, int VEC>
+__device__ __forceinline__ Pack<E, VEC> nothing() {
+    Pack<E, VEC> o;
+#pragma unroll
+    for (int i = 0; i < o.WORDS; ++i) o.w[i] = 0;
+    return o;
+}
+template <typename E, int VEC>
 __device__ __forceinline__ Pack<E, VEC> load(const E *p) {
-    return *reinterpret_cast<const Pack<E, VEC> *>(p);
+    Pack<E, VEC> o;
+    if constexpr (VEC == 1 && sizeof(E) == 2) o.w[0] = *reinterpret_cast<const uint16_t *>(p);
+    else if constexpr (VEC == 1) o.w[0] = *reinterpret_cast<const uint32_t *>(p);
+    else if constexpr (sizeof(E) == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        o.w[0] = v.x, o.w[1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        o.w[0] = v.x, o.w[1] = v.y, o.w[2] = v.z, o.w[3] = v.w;
+    }
+    return o;
 }
 template <typename E, int VEC>
 __device__ __forceinline__ void store(E *p, const float2 (&v)[NP<VEC>]) {
@@ -52,18 +76,9 @@ __device__ __forceinline__ void store(E *p, const float2 (&v)[NP<VEC>]) {
     } else if constexpr (sizeof(E) == 4) {
         *reinterpret_cast<float4 *>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     } else {
-        Pack<__nv_bfloat162, 2> o;
-        o.v[0] = __float22bfloat162_rn(v[0]);
-        o.v[1] = __float22bfloat162_rn(v[1]);
-        *reinterpret_cast<Pack<__nv_bfloat162, 2> *>(p) = o;
+        const __nv_bfloat162 a = __float22bfloat162_rn(v[0]), b = __float22bfloat162_rn(v[1]);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(reinterpret_cast<const uint32_t &>(a), reinterpret_cast<const uint32_t &>(b));
     }
-}
-template <typename E, int VEC>
-__device__ __forceinline__ Pack<E, VEC> nothing() {
-    Pack<E, VEC> o;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o.v[i] = from_f<E>(0.f);
-    return o;
 }
 
 // sigmoid(v) = 1 / (1 + e^-v) on MUFU's ex2 and reciprocal
@@ -112,44 +127,74 @@ struct Taps {
 template <int KT, bool EXACT>
 __device__ __forceinline__ int taps_of(int K) { return EXACT ? KT : K; }
 
-// Rows of a warp's tile, all loaded before the first is used: 8 of 16 bytes a lane, 16 of 8.
-template <typename E>
-constexpr int FWD_ROWS = sizeof(E) == 4 ? 8 : 16;
-
 // ---------------------------------------------------------------- forward
+
+// The rows [t0, t1) from xp, row t0; `above`: how many rows before t0 there are (zeros above them).
+// out(t, sums) takes each row's sum of taps.
+template <typename E, int KT, int VEC, typename Out>
+__device__ __forceinline__ void walk(const E *xp, long long ldt, int t0, int t1, int above, int K,
+                                     const Taps<E, KT, VEC> &taps, Out out)
+{
+    constexpr int STEP = FWD_STEP<E>;
+    Pack<E, VEC> xs[STEP + KT - 1], next[STEP];            // rows t - KT + 1 .. t + STEP - 1, the STEP behind them
+    auto rows_in = [&](int t) {
+        if (t + STEP <= t1) {
+#pragma unroll
+            for (int u = 0; u < STEP; ++u) {
+                next[u] = load<E, VEC>(xp);
+                xp += ldt;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < STEP; ++u) {
+                next[u] = t + u < t1 ? load<E, VEC>(xp) : nothing<E, VEC>();
+                xp += ldt;
+            }
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < KT - 1; ++j) {
+        const int back = KT - 1 - j;
+        xs[j] = back <= above ? load<E, VEC>(xp - back * ldt) : nothing<E, VEC>();
+    }
+    rows_in(t0);
+    for (int t = t0; t < t1; t += STEP) {
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) xs[KT - 1 + u] = next[u];
+        rows_in(t + STEP);
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            float2 acc[NP<VEC>];
+            taps.sum(acc, K, [&](int k, int p) { return xs[u + k].pair(p); });
+            out(t + u, acc);
+        }
+#pragma unroll
+        for (int j = 0; j < KT - 1; ++j) xs[j] = xs[j + STEP];
+    }
+}
 
 template <typename E, int KT, bool EXACT, int VEC>
 __global__ void __launch_bounds__(THREADS)
 conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
-                const E *__restrict__ bias, E *__restrict__ y, int T, int D, int K_in, bool silu, int nd, int nt)
+                const E *__restrict__ bias, E *__restrict__ y, int T, int D, int K_in, bool silu, int nd, int segs,
+                int len, long long units)
 {
-    constexpr int ROWS = FWD_ROWS<E>;
     const int K = taps_of<KT, EXACT>(K_in);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int blk = blockIdx.x;                            // (b, tile, channel block), the last fastest
-    const int d = (blk % nd) * 32 * VEC + lane * VEC;
-    const int tile = blk / nd % nt, b = blk / nd / nt;
-    const int t0 = (tile * WARPS + warp) * ROWS;
-    if (d >= D || t0 >= T) return;
-    const E *xb = x + b * ldb + d;
-    Pack<E, VEC> xs[ROWS + KT - 1];
-#pragma unroll
-    for (int j = 0; j < ROWS + KT - 1; ++j) {
-        const int t = t0 - (KT - 1) + j;
-        xs[j] = t >= 0 && t < T ? load<E, VEC>(xb + t * ldt) : nothing<E, VEC>();
-    }
+    const long long unit = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);   // (b, segment, channel block)
+    if (unit >= units) return;
+    const int d = (int)(unit % nd) * 32 * VEC + (threadIdx.x & 31) * VEC;
+    const int seg = (int)(unit / nd % segs), b = (int)(unit / nd / segs);
+    const int t0 = seg * len, t1 = min(T, t0 + len);
+    if (d >= D) return;
     Taps<E, KT, VEC> taps;
     taps.read(w, bias, d, K);
-    E *yb = y + ((long long)b * T + t0) * D + d;
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        float2 acc[NP<VEC>];
-        taps.sum(acc, K, [&](int k, int p) { return xs[r + k].pair(p); });
+    E *yp = y + ((long long)b * T + t0) * D + d;
+    walk<E, KT, VEC>(x + b * ldb + t0 * ldt + d, ldt, t0, t1, t0, K, taps, [&](int t, float2 (&acc)[NP<VEC>]) {
 #pragma unroll
         for (int p = 0; p < NP<VEC>; ++p) acc[p] = act(acc[p], silu);
-        if (t0 + r < T) store<E, VEC>(yb, acc);
-        yb += D;
-    }
+        if (t < t1) store<E, VEC>(yp, acc);
+        yp += D;
+    });
 }
 
 // --------------------------------------------------------------- backward
@@ -162,16 +207,16 @@ template <typename E, int KT, bool EXACT, int VEC>
 __global__ void __launch_bounds__(THREADS, KT <= 4 ? 4 : 2)
 conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
                 const E *__restrict__ bias, const E *__restrict__ dy, E *__restrict__ dx,
-                float *__restrict__ part, int T, int D, int K_in, bool silu, int nd, int ns, int len)
+                float *__restrict__ part, int T, int D, int K_in, bool silu, int nd, int segs, int len, long long rows)
 {
-    constexpr int P = NP<VEC>;
+    constexpr int P = NP<VEC>, STEP = BWD_STEP<E>;
     const int K = taps_of<KT, EXACT>(K_in);
     __shared__ float2 sums[WARPS][KT + 1][P][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int blk = blockIdx.x;                            // (b, segment, channel block)
-    const int d = (blk % nd) * 32 * VEC + lane * VEC;
-    const int seg = blk / nd % ns, b = blk / nd / ns;
-    const int t0 = (seg * WARPS + warp) * len, t1 = min(T, t0 + len);
+    const int d = (blockIdx.x % nd) * 32 * VEC + lane * VEC;
+    const long long row = (long long)(blockIdx.x / nd) * WARPS + warp;     // (b, segment)
+    const int seg = (int)(row % segs), b = (int)(row / segs);
+    const int t0 = seg * len, t1 = min(T, t0 + len);
     float2 dw[KT][P], db[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -179,14 +224,32 @@ conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
 #pragma unroll
         for (int k = 0; k < KT; ++k) dw[k][p] = f2(0.f, 0.f);
     }
-    if (d < D && t0 < T) {
+    if (d < D && row < rows) {
         const E *xp = x + b * ldb + d + t0 * ldt;          // row t
         const E *gp = dy + ((long long)b * T + t0) * D + d;
         E *op = dx + ((long long)b * T + t0 - (KT - 1)) * D + d;  // row t - KT + 1
         Taps<E, KT, VEC> taps;
         taps.read(w, bias, d, K);
-        Pack<E, VEC> xs[BWD_STEP + KT - 1];                // rows t - KT + 1 .. t + BWD_STEP - 1
-        float2 ds[BWD_STEP + KT - 1][P];
+        Pack<E, VEC> xs[STEP + KT - 1], xn[STEP], gn[STEP];       // rows t - KT + 1 .. t + STEP - 1, the next
+        float2 ds[STEP + KT - 1][P];
+        const int end = min(T, t1 + KT - 1);               // rows that are read
+        auto rows_in = [&](int t) {
+            if (t + STEP <= end) {
+#pragma unroll
+                for (int u = 0; u < STEP; ++u) {
+                    xn[u] = load<E, VEC>(xp), gn[u] = load<E, VEC>(gp);
+                    xp += ldt, gp += D;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < STEP; ++u) {
+                    const bool in = t + u < end;
+                    xn[u] = in ? load<E, VEC>(xp) : nothing<E, VEC>();
+                    gn[u] = in ? load<E, VEC>(gp) : nothing<E, VEC>();
+                    xp += ldt, gp += D;
+                }
+            }
+        };
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
             const int back = KT - 1 - j;
@@ -194,19 +257,16 @@ conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
 #pragma unroll
             for (int p = 0; p < P; ++p) ds[j][p] = f2(0.f, 0.f);
         }
+        rows_in(t0);
         // inner: all rows of the step are the warp's own, and so are those whose dx they complete
         auto step = [&](int t, auto inner) {
             constexpr bool INNER = decltype(inner)::value;
-            Pack<E, VEC> g[BWD_STEP];
+            Pack<E, VEC> g[STEP];
 #pragma unroll
-            for (int u = 0; u < BWD_STEP; ++u) {
-                const bool in = INNER || (t + u < T && t + u < t1 + KT - 1);
-                xs[KT - 1 + u] = in ? load<E, VEC>(xp) : nothing<E, VEC>();
-                g[u] = in ? load<E, VEC>(gp) : nothing<E, VEC>();
-                xp += ldt, gp += D;
-            }
+            for (int u = 0; u < STEP; ++u) xs[KT - 1 + u] = xn[u], g[u] = gn[u];
+            rows_in(t + STEP);
 #pragma unroll
-            for (int u = 0; u < BWD_STEP; ++u) {
+            for (int u = 0; u < STEP; ++u) {
                 float2 pre[P];
                 if (silu) taps.sum(pre, K, [&](int k, int p) { return xs[u + k].pair(p); });
 #pragma unroll
@@ -244,13 +304,13 @@ conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
             }
 #pragma unroll
             for (int j = 0; j < KT - 1; ++j) {
-                xs[j] = xs[j + BWD_STEP];
+                xs[j] = xs[j + STEP];
 #pragma unroll
-                for (int p = 0; p < P; ++p) ds[j][p] = ds[j + BWD_STEP][p];
+                for (int p = 0; p < P; ++p) ds[j][p] = ds[j + STEP][p];
             }
         };
-        for (int t = t0; t < t1 + KT - 1; t += BWD_STEP) {
-            if (t - (KT - 1) >= t0 && t + BWD_STEP <= t1) step(t, std::true_type{});
+        for (int t = t0; t < t1 + KT - 1; t += STEP) {
+            if (t - (KT - 1) >= t0 && t + STEP <= t1) step(t, std::true_type{});
             else step(t, std::false_type{});
         }
     }
@@ -261,9 +321,9 @@ conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
         sums[warp][KT][p][lane] = db[p];
     }
     __syncthreads();
-    // part[(b, segment)][K + 1][D]
-    float *pb = part + (long long)(blk / nd) * (K + 1) * D + (blk % nd) * 32 * VEC;
-    const int left = D - (blk % nd) * 32 * VEC;
+    // part[CTA's rows][K + 1][D]
+    float *pb = part + (long long)(blockIdx.x / nd) * (K + 1) * D + (blockIdx.x % nd) * 32 * VEC;
+    const int left = D - (blockIdx.x % nd) * 32 * VEC;
     for (int o = threadIdx.x; o < (KT + 1) * P * 32; o += THREADS) {
         const int c = o % (P * 32), k = o / (P * 32);
         const int at = VEC == 1 ? c : 2 * c;               // its first channel in the CTA
@@ -305,7 +365,7 @@ conv_reduce_kernel(const float *__restrict__ part, E *__restrict__ dw, E *__rest
 // so that none waits for another though the cache is updated in place:
 //   heads  (sequence, channel block): the outputs that still see the old window,
 //          rows 0 .. min(length, K - 1) - 1, and then the new window;
-//   tails  (8 or 16 rows, channel block): the rows at place K - 1 and later of their
+//   tails  (32 rows, channel block): the rows at place K - 1 and later of their
 //          sequence, which depend on x alone; rows of no sequence get zeros.
 template <typename E, int KT, bool EXACT, int VEC>
 __global__ void __launch_bounds__(THREADS)
@@ -324,7 +384,7 @@ conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__
         const int first = seq.start(s), end = seq.starts.p ? max(first, seq.start(s + 1)) : s + 1;
         const int len = end - first, K1 = K - 1;
         const long long from = seq.from(s), to = seq.to(s);
-        // rows[0 .. KT - 2] the old window (as pairs, the same rounding as x's), then the first inputs
+        // rows[0 .. KT - 2] the old window (as pairs of floats), then the first inputs
         E old[KT > 1 ? KT - 1 : 1][VEC];
         float2 rows[2 * (KT - 1) + 1][NP<VEC>];
 #pragma unroll
@@ -345,19 +405,19 @@ conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__
             // the last K - 1 of the window and the inputs behind it
 #pragma unroll
             for (int j = 0; j < KT - 1; ++j) {
+                if (j >= K1) continue;
                 const int p = len - K1 + j;                // its row; below 0: in the old window
-                Pack<E, VEC> v = nothing<E, VEC>();
-                if (p >= 0 && j < K1) v = load<E, VEC>(x + (first + p) * ldx + d);
+                E v[VEC];
 #pragma unroll
-                for (int q = 0; q < KT - 1; ++q)           // (constant indices: registers)
-                    if (p < 0 && q - (KT - K) == p + K1) {
+                for (int i = 0; i < VEC; ++i) v[i] = p >= 0 ? x[(first + p) * ldx + d + i] : from_f<E>(0.f);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) v.v[i] = old[q][i];
-                    }
-                if (j < K1) {
+                for (int q = 0; q < KT - 1; ++q) {         // (constant indices: registers)
+                    const bool here = p < 0 && q - (KT - K) == p + K1;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = v.v[i];
+                    for (int i = 0; i < VEC; ++i) v[i] = here ? old[q][i] : v[i];
                 }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) window[(to * D + d + i) * K1 + j] = v[i];
             }
         }
         Taps<E, KT, VEC> taps;
@@ -373,48 +433,34 @@ conv_packed_kernel(const E *__restrict__ x, long long ldx, const E *__restrict__
         }
         return;
     }
-    constexpr int ROWS = FWD_ROWS<E>;
-    const int r0 = (int)((unit - heads) / nd) * ROWS;
-    Pack<E, VEC> xs[ROWS + KT - 1];
-#pragma unroll
-    for (int j = 0; j < ROWS + KT - 1; ++j) {
-        const int t = r0 - (KT - 1) + j;
-        xs[j] = d < D && t >= 0 && t < seq.rows ? load<E, VEC>(x + t * ldx + d) : nothing<E, VEC>();
-    }
+    const int r0 = (int)((unit - heads) / nd) * TAIL_ROWS, r1 = min(seq.rows, r0 + TAIL_ROWS);
+    auto start = [&](int i) { return seq.start(i); };
+    const int n = seq.count + 1;
+    // the sequence of the row that is next, its first row and the one behind its last
+    int s = seq.starts.p ? Sequences::last_at_most(n, r0, start) : 0, first = 0, next = seq.rows;
+    auto bounds = [&]() {
+        first = s < 0 ? 0 : seq.start(s), next = s + 1 < n ? seq.start(s + 1) : seq.rows;
+    };
+    if (seq.starts.p) bounds();
     Taps<E, KT, VEC> taps;
-    if (d < D) taps.read(w, bias, d, K);
-    // what row r0 + r is: bit r of `tails`, of `nobody`, or of neither (a head's)
-    unsigned tails = 0, nobody = 0;
-    const int rows = min(ROWS, seq.rows - r0);
-    if (!seq.starts.p) {
-        tails = K == 1 ? ~0u : 0u;
-    } else {
-        auto start = [&](int i) { return seq.start(i); };
-        const int n = seq.count + 1;
-        int s = Sequences::last_at_most(n, r0, start);
-        int first = s < 0 ? 0 : seq.start(s), next = s + 1 < n ? seq.start(s + 1) : seq.rows;
-        for (int r = 0; r < rows; ++r) {
-            if (r0 + r >= next) {                          // a sequence ends inside the tile
-                s = Sequences::last_at_most(n, r0 + r, start);
-                first = s < 0 ? 0 : seq.start(s), next = s + 1 < n ? seq.start(s + 1) : seq.rows;
-            }
-            if (s < 0 || s >= seq.count) nobody |= 1u << r;
-            else if (r0 + r - first >= K - 1) tails |= 1u << r;
-        }
-    }
-    if (d >= D) return;
+    const bool act_lane = d < D;
+    if (act_lane) taps.read(w, bias, d, K);
     E *yp = y + (long long)r0 * D + d;
+    walk<E, KT, VEC>(x + r0 * ldx + (act_lane ? d : 0), ldx, r0, r1, r0, K, taps, [&](int r, float2 (&acc)[NP<VEC>]) {
+        if (r < r1) {
+            if (r >= next) {                               // (all lanes)
+                s = Sequences::last_at_most(n, r, start);
+                bounds();
+            }
+            const bool nobody = s < 0 || s >= seq.count;
+            if (act_lane && (nobody || !seq.starts.p || r - first >= K - 1)) {
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        if (r < rows && ((tails | nobody) >> r & 1)) {
-            float2 acc[NP<VEC>];
-            taps.sum(acc, K, [&](int k, int p) { return xs[r + k].pair(p); });
-#pragma unroll
-            for (int p = 0; p < NP<VEC>; ++p) acc[p] = nobody >> r & 1 ? f2(0.f, 0.f) : act(acc[p], silu);
-            store<E, VEC>(yp, acc);
+                for (int p = 0; p < NP<VEC>; ++p) acc[p] = nobody ? f2(0.f, 0.f) : act(acc[p], silu);
+                store<E, VEC>(yp, acc);
+            }
         }
         yp += D;
-    }
+    });
 }
 
 // ------------------------------------------------------------------ launch
@@ -430,17 +476,17 @@ bool groups_of_4(int D, std::initializer_list<const void *> arrays, std::initial
     return ok;
 }
 
-// Rows a warp of the backward walks: as many as leave 8 CTAs an SM, so that the halo
-// of K - 1 rows and the partial sums stay small beside them; at least 16, at most 128.
-int bwd_rows(int Bt, int T, int D)
+// Rows a warp walks: as many as leave 8 CTAs an SM, so that the halo of K - 1 rows and the
+// backward's partial sums stay small beside them; at least 16, at most 128.
+int rows_of_warp(int Bt, int T, int D)
 {
-    const long long base = (long long)Bt * ((D + 127) / 128);
-    const long long want = std::max<long long>(1, 8LL * N_SM / base);
-    const long long len = (T + want * WARPS - 1) / (want * WARPS);
-    return (int)std::min<long long>(128, std::max<long long>(16, (len + BWD_STEP - 1) / BWD_STEP * BWD_STEP));
+    const long long nd = (D + 127) / 128;                  // (the same for one channel a thread: the sums' layout)
+    const long long want = std::max<long long>(1, 8LL * N_SM * WARPS / (nd * Bt));
+    const long long len = (T + want - 1) / want;
+    return (int)std::min<long long>(128, std::max<long long>(16, (len + 7) / 8 * 8));
 }
 
-int bwd_segments(int T, int len) { return (T + WARPS * len - 1) / (WARPS * len); }
+int parts_of(int Bt, int T, int len) { return (int)(((long long)Bt * ((T + len - 1) / len) + WARPS - 1) / WARPS); }
 
 // The kernels for 2, 3 and 4 taps are unrolled for exactly those; 1 and 5 to 8 taps
 // run one that is unrolled for 8.
@@ -458,12 +504,13 @@ cudaError_t by_taps(int K, F f)
 template <typename E, int VEC>
 cudaError_t fwd_of(const ConvArgs &a, cudaStream_t stream)
 {
-    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), nt = (a.T + WARPS * FWD_ROWS<E> - 1) / (WARPS * FWD_ROWS<E>);
-    const long long blocks = (long long)a.Bt * nt * nd;
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), len = rows_of_warp(a.Bt, a.T, a.D), segs = (a.T + len - 1) / len;
+    const long long units = (long long)a.Bt * segs * nd, blocks = (units + WARPS - 1) / WARPS;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     return by_taps(a.K, [&](auto kt, auto exact) {
         conv_fwd_kernel<E, decltype(kt)::value, decltype(exact)::value, VEC><<<(unsigned)blocks, THREADS, 0, stream>>>(
-            (const E *)a.x, a.ldb, a.ldt, (const E *)a.w, (const E *)a.bias, (E *)a.y, a.T, a.D, a.K, a.silu, nd, nt);
+            (const E *)a.x, a.ldb, a.ldt, (const E *)a.w, (const E *)a.bias, (E *)a.y, a.T, a.D, a.K, a.silu, nd, segs,
+            len, units);
         return cudaGetLastError();
     });
 }
@@ -471,18 +518,19 @@ cudaError_t fwd_of(const ConvArgs &a, cudaStream_t stream)
 template <typename E, int VEC>
 cudaError_t bwd_of(const ConvArgs &a, cudaStream_t stream)
 {
-    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), len = bwd_rows(a.Bt, a.T, a.D), ns = bwd_segments(a.T, len);
-    const long long blocks = (long long)a.Bt * ns * nd;
+    const int nd = (a.D + 32 * VEC - 1) / (32 * VEC), len = rows_of_warp(a.Bt, a.T, a.D), segs = (a.T + len - 1) / len;
+    const int parts = parts_of(a.Bt, a.T, len);
+    const long long blocks = (long long)parts * nd;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     const cudaError_t e = by_taps(a.K, [&](auto kt, auto exact) {
         conv_bwd_kernel<E, decltype(kt)::value, decltype(exact)::value, VEC><<<(unsigned)blocks, THREADS, 0, stream>>>(
             (const E *)a.x, a.ldb, a.ldt, (const E *)a.w, (const E *)a.bias, (const E *)a.dy, (E *)a.dx, a.part, a.T,
-            a.D, a.K, a.silu, nd, ns, len);
+            a.D, a.K, a.silu, nd, segs, len, (long long)a.Bt * segs);
         return cudaGetLastError();
     });
     if (e != cudaSuccess) return e;
-    conv_reduce_kernel<E><<<dim3((a.D + 31) / 32, a.K + 1), 256, 0, stream>>>(a.part, (E *)a.dw, (E *)a.dbias,
-                                                                             a.Bt * ns, a.D, a.K);
+    conv_reduce_kernel<E><<<dim3((a.D + 31) / 32, a.K + 1), 256, 0, stream>>>(a.part, (E *)a.dw, (E *)a.dbias, parts,
+                                                                             a.D, a.K);
     return cudaGetLastError();
 }
 
@@ -492,7 +540,7 @@ cudaError_t packed_of(const ConvPackedArgs &a, cudaStream_t stream)
     const int nd = (a.D + 32 * VEC - 1) / (32 * VEC);
     // single tokens have no tails unless there is no window
     const long long heads = a.K > 1 || a.seq.starts.p ? (long long)a.seq.count * nd : 0;
-    const long long tails = a.seq.starts.p || a.K == 1 ? (long long)((a.seq.rows + FWD_ROWS<E> - 1) / FWD_ROWS<E>) * nd : 0;
+    const long long tails = a.seq.starts.p || a.K == 1 ? (long long)((a.seq.rows + TAIL_ROWS - 1) / TAIL_ROWS) * nd : 0;
     const long long blocks = (heads + tails + WARPS - 1) / WARPS;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (blocks == 0) return cudaSuccess;
@@ -509,7 +557,7 @@ cudaError_t packed_of(const ConvPackedArgs &a, cudaStream_t stream)
 
 size_t conv_workspace_bytes(int Bt, int T, int D, int K)
 {
-    return (size_t)Bt * bwd_segments(T, bwd_rows(Bt, T, D)) * (K + 1) * D * sizeof(float);
+    return (size_t)parts_of(Bt, T, rows_of_warp(Bt, T, D)) * (K + 1) * D * sizeof(float);
 }
 
 cudaError_t launch_conv_fwd(const ConvArgs &a, cudaStream_t stream)

@@ -12,18 +12,21 @@
 // scan does; G = 1, 2 or 4 lanes share a channel of up to 16, 32 or 64 states. A
 // sequence is cut into segments of `seg` rows, so that one long prompt fills the GPU
 // as well as many short ones, whatever the lengths, which the host does not know:
-//   first   the first segment of a sequence in full; of those between it and the last
-//           only the end state from nothing and the sum of dt (the decay of a state
-//           over the segment is exp(-Aneg sum dt));
-//   rest    all later segments, each from the chain of the end states before it.
-// A sequence of one segment is done in the first launch, with one exponential a state
-// and step; only the segments between the first and the last take two. Of a sequence of
-// more than FEW segments the first is taken like those between: the launch would
-// otherwise end with its CTAs alone, which have half as much again to do.
+//   first   segments whose state is known, the first ones of short sequences, with their
+//           outputs; of the others but a sequence's last the state at the end from nothing
+//           and the sum of dt (a state's decay over the segment is exp(-Aneg sum dt));
+//   rest    all other segments with their outputs, each from the chain of the ends before it.
+// The ends are sums over the rows, v_n = sum_t exp(-Aneg_n sum_{t' > t} dt) dt_t B_tn x_t, from
+// the last row back: a state's rows are left out where the decay is flushed to 0
+// (below 2^-126), which leaves a quarter of the exponentials where dt is around 0.14
+// and Aneg 1 to 16. (Walking forward through all of them: 16384 x 2048 x 16, float32, 343 us.
+// Adding what enters a segment to outputs computed from nothing, with the same
+// exponentials left out: 313 us, 381 instead of 226 for 8192 x 2304 x 16 in bf16; it reads and
+// writes the outputs once more.)
 //
 // Unit u of a launch is segment i of sequence s with u = s + start_s / seg + i: as
 // a sequence of n rows has at most (start_s + n) / seg - start_s / seg + 1
-// segments, no two share a number, and a binary search over the starts finds s.
+// segments, no two share a number, and a search over the starts finds s.
 //
 // Single tokens without a list of starts are bound by the states' bytes, read and
 // written once: 4 states a lane, G lanes a channel, several sequences a thread so that
@@ -40,13 +43,26 @@ namespace {
 
 constexpr int THREADS = 128;
 constexpr int TT = 8;                   // rows of a tile of B and C
-constexpr int SUB = 4;                  // rows of x, dt and z in registers
-constexpr int FEW = 3;                  // segments of a sequence whose first is done in full at once
+#ifndef MMS_SUB
+#define MMS_SUB 4
+#endif
+constexpr int SUB = MMS_SUB;            // rows of x, dt and z in registers
+constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 flushes to 0
+// A sequence's first segment is done in full in the first launch if it has at most FEW
+// segments; of longer ones its end comes first, like the others', so that the launch does not
+// end with its CTAs alone.
+#ifndef MMS_PACKED_FEW
+#define MMS_PACKED_FEW 3
+#endif
+constexpr int FEW = MMS_PACKED_FEW;
 #ifndef MMS_PACKED_POLY
 #define MMS_PACKED_POLY 1
 #endif
 #ifndef MMS_PACKED_MINB
 #define MMS_PACKED_MINB 4
+#endif
+#ifndef MMS_PACKED_FILL
+#define MMS_PACKED_FILL 4
 #endif
 
 template <typename E, typename BE>
@@ -61,7 +77,7 @@ struct Args {
     int D, N;
     Proj pj;
     float *ends, *sums;                 // end states (row, D, N) and sums of dt (row, D) of segments
-    float *entry;                       // (row, D, N) what long sequences go on from
+    float *entry;                       // (row, D, N) what sequences of more than FEW segments go on from
     int seg, nd;                        // rows of a segment, channel blocks
     int units;                          // units of segments; the blocks behind them clear rows of no sequence
 };
@@ -72,28 +88,67 @@ struct Split {
     static constexpr int NS = NS_, G = G_, NP = NS_ * G_, DPB = THREADS / G_;
 };
 
+// What a CTA of a segment's launch is to do.
+struct Unit {
+    int s, i, segs, t0, t1;             // sequence, segment of how many, rows
+    int row;                            // of the sequence in the workspace
+};
+template <typename E, typename BE>
+__device__ __forceinline__ bool find_unit(const Args<E, BE> &a, int unit, Unit &u)
+{
+    u.s = Sequences::last_at_most(a.seq.count, unit, [&](int i) { return i + a.seq.start(i) / a.seg; });
+    if (u.s < 0) return false;
+    const int first = a.seq.start(u.s), end = max(first, a.seq.start(u.s + 1));
+    u.row = first / a.seg;
+    u.i = unit - (u.s + u.row);
+    u.segs = max(1, (end - first + a.seg - 1) / a.seg);
+    u.t0 = first + u.i * a.seg, u.t1 = min(end, u.t0 + a.seg);
+    return u.i >= 0 && u.i < u.segs;
+}
+
+// A tile of TT rows of B and C as float32 in shared memory: this thread's share of it.
+template <int NP, int ARR>
+struct Share {
+    static constexpr int PER = (TT * ARR * NP + THREADS - 1) / THREADS;
+    float v[PER];
+    template <typename BE>
+    __device__ __forceinline__ void read(const BE *B, long long ldB, const BE *C, long long ldC, int N, int t, int t1) {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int o = threadIdx.x + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
+            v[q] = 0.f;
+            if (j < TT && n < N && t + j < t1) v[q] = arr ? to_f(C[(t + j) * ldC + n]) : to_f(B[(t + j) * ldB + n]);
+        }
+    }
+    __device__ __forceinline__ void write(float (*bc)[ARR][NP]) const {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int o = threadIdx.x + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
+            if (j < TT) bc[j][arr][n] = v[q];
+        }
+    }
+};
+
 // ------------------------------------------------------------- segments
 
-// The rows [t0, t1) from state h; FULL: with outputs, else h from what it is and the
-// sum of dt. Rows come through registers SUB at a time, the next ones requested as
-// soon as these are converted; B and C as float32 through shared memory, TT rows at a time.
-// POLY of a thread's pairs of exponentials are taken from MUFU to the FMA pipe.
-template <bool FULL, typename E, typename BE, typename S>
-__device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S::NP], float2 (&h)[S::NS / 2],
+// The rows [t0, t1) from state h, with their outputs. Rows come through registers
+// SUB at a time, the next ones requested as soon as these are converted; B and C through
+// shared memory, TT rows at a time. POLY of a thread's 8 pairs of exponentials are taken
+// from MUFU to the FMA pipe (16384 x 2048 x 16: 0 pairs 360 us, 1 343, 2 366, in the form with two
+// walks).
+template <typename E, typename BE, typename S>
+__device__ __forceinline__ void walk(const Args<E, BE> &a, float (*bc)[TT][2][S::NP], float2 (&h)[S::NS / 2],
                                       const float2 (&nan2)[S::NS / 2], int t0, int t1, int d, int g, bool act)
 {
-    constexpr int NS = S::NS, NP = S::NP;
-    constexpr int ARR = FULL ? 2 : 1;                      // B, and C where it is wanted
-    constexpr int PER = (TT * ARR * NP + THREADS - 1) / THREADS;
+    constexpr int NS = S::NS;
     constexpr int POLY = MMS_PACKED_POLY * NS / 16;
-    const int tid = threadIdx.x;
-    const bool gate = FULL && a.z != nullptr;
-    const float skip = FULL && a.d_skip && act ? a.d_skip[d] : 0.f;
+    const bool gate = a.z != nullptr;
+    const float skip = a.d_skip && act ? a.d_skip[d] : 0.f;
     const int ds = act ? d : 0;                            // a channel that is there
     const E *xp = a.x + t0 * a.ldx + ds, *dp = a.dt + t0 * a.lddt + ds;
     const E *zp = gate ? a.z + t0 * a.ldz + ds : a.x;
     const long long ldz = gate ? a.ldz : 0;
-    E *yp = a.y + (long long)t0 * a.D + ds;
+    long long yo = (long long)t0 * a.D + ds;
     E xr[SUB], dr[SUB], zr[SUB];
     auto rows_in = [&](int left) {                         // the next SUB rows, of which `left` are there
 #pragma unroll
@@ -104,37 +159,18 @@ __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S
             } else {
                 xr[j] = dr[j] = from_f<E>(0.f);
             }
-            xp += a.ldx, dp += a.lddt;
-            if (FULL) zp += ldz;
+            xp += a.ldx, dp += a.lddt, zp += ldz;
         }
     };
-    float next[PER];
-    auto bc_in = [&](int t) {                              // this thread's share of a tile of B and C
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int o = tid + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
-            float v = 0.f;
-            if (j < TT && n < a.N && t + j < t1)
-                v = arr ? to_f(a.C[(t + j) * a.ldC + n]) : to_f(a.B[(t + j) * a.ldB + n]);
-            next[q] = v;
-        }
-    };
-    auto bc_out = [&](int buf) {
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int o = tid + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
-            if (j < TT) bc[buf][j][arr][n] = next[q];
-        }
-    };
-    bc_in(t0);
+    Share<S::NP, 2> next;
+    next.read(a.B, a.ldB, a.C, a.ldC, a.N, t0, t1);
     rows_in(t1 - t0);
-    bc_out(0);
+    next.write(bc[0]);
     __syncthreads();
-    float total = 0.f;
     int buf = 0;
     for (int t = t0; t < t1; t += TT, buf ^= 1) {
         const bool more = t + TT < t1;
-        if (more) bc_in(t + TT);
+        if (more) next.read(a.B, a.ldB, a.C, a.ldC, a.N, t + TT, t1);
 #pragma unroll
         for (int sub = 0; sub < TT; sub += SUB) {
             const int left = t1 - t - sub;                 // rows from here on
@@ -155,38 +191,118 @@ __device__ __forceinline__ float walk(const Args<E, BE> &a, float (*bc)[TT][2][S
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
                 const float2 dt2 = f2(df[j], df[j]), bx2 = f2(df[j] * xf[j], df[j] * xf[j]);
-                if (!FULL) total += df[j];
                 const float4 *bp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][0][g * NS]);
                 const float4 *cp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][1][g * NS]);
                 float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
                 for (int q = 0; q < NS / 4; ++q) {
-                    const float4 Bv = bp[q];
+                    const float4 Bv = bp[q], Cv = cp[q];
                     const float2 e0 = mul2(dt2, nan2[2 * q]), e1 = mul2(dt2, nan2[2 * q + 1]);
                     h[2 * q] = fma2(2 * q < POLY ? ex2_poly2(e0) : ex2x2(e0), h[2 * q], mul2(bx2, lo(Bv)));
                     h[2 * q + 1] = fma2(2 * q + 1 < POLY ? ex2_poly2(e1) : ex2x2(e1), h[2 * q + 1], mul2(bx2, hi(Bv)));
-                    if (FULL) {
-                        const float4 Cv = cp[q];
-                        acc[0] = fma2(lo(Cv), h[2 * q], acc[0]);
-                        acc[1] = fma2(hi(Cv), h[2 * q + 1], acc[1]);
-                    }
+                    acc[0] = fma2(lo(Cv), h[2 * q], acc[0]);
+                    acc[1] = fma2(hi(Cv), h[2 * q + 1], acc[1]);
                 }
-                if (FULL) {
-                    acc[0] = add2(acc[0], acc[1]);
-                    float yv = acc[0].x + acc[0].y;
+                acc[0] = add2(acc[0], acc[1]);
+                float yv = acc[0].x + acc[0].y;
 #pragma unroll
-                    for (int o = S::G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
-                    yv = (yv + skip) * gf[j];
-                    if (act && g == 0 && j < left) *yp = from_f<E>(yv);
-                    yp += a.D;
-                }
+                for (int o = S::G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
+                yv = (yv + skip) * gf[j];
+                if (act && g == 0 && j < left) a.y[yo] = from_f<E>(yv);
+                yo += a.D;
             }
         }
         if (more) {
-            bc_out(buf ^ 1);                               // the tile before was read before the last barrier
+            next.write(bc[buf ^ 1]);                       // the tile before was read before the last barrier
             __syncthreads();
         }
     }
+}
+
+// What the rows [t0, t1) leave of nothing, v, and the sum of their dt, from the last row back.
+// An x or B that is not finite stays in the state for good, whatever its decay: a product
+// with 0 keeps it, also where its row is left out.
+template <typename E, typename BE, typename S>
+__device__ __forceinline__ float leave(const Args<E, BE> &a, float (*bc)[TT][1][S::NP], float (&lost)[S::NP],
+                                       float2 (&v)[S::NS / 2], const float2 (&nan2)[S::NS / 2], int t0, int t1, int d,
+                                       int g, bool act)
+{
+    constexpr int NPAIR = S::NS / 2;
+    const int tid = threadIdx.x, ds = act ? d : 0;
+    const E *xp = a.x + (t1 - 1) * a.ldx + ds, *dp = a.dt + (t1 - 1) * a.lddt + ds;
+    E xr[TT], dr[TT];                                      // rows t - 1, t - 2, ..
+    auto rows_in = [&](int left) {
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+            if (j < left) {
+                xr[j] = *xp, dr[j] = *dp;
+            } else {
+                xr[j] = dr[j] = from_f<E>(0.f);
+            }
+            xp -= a.ldx, dp -= a.lddt;
+        }
+    };
+    if (tid < S::NP) lost[tid] = 0.f;
+    // (rows of B in front of t0 are other segments', or not there: read() takes rows from t0 on)
+    Share<S::NP, 1> next;
+    float bad_b = 0.f;
+    auto b_in = [&](int t) {                               // rows t - 1 down to t - TT
+#pragma unroll
+        for (int q = 0; q < next.PER; ++q) {
+            const int o = tid + q * THREADS, n = o % S::NP, j = o / S::NP;
+            next.v[q] = 0.f;
+            if (j < TT && n < a.N && t - 1 - j >= t0) next.v[q] = to_f(a.B[(t - 1 - j) * a.ldB + n]);
+            bad_b = fmaf(next.v[q], 0.f, bad_b);
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < NPAIR; ++q) v[q] = f2(0.f, 0.f);
+    b_in(t1);
+    rows_in(t1 - t0);
+    next.write(bc[0]);
+    __syncthreads();
+    float total = 0.f, bad_x = 0.f;
+    int buf = 0;
+    for (int t = t1; t > t0; t -= TT, buf ^= 1) {
+        const int left = t - t0;
+        float sum[TT], bx[TT], least = INFINITY, most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+            float dtv = to_f(dr[j]);
+            if (a.pj.on) dtv = j < left ? fmaf(a.pj.range, sigmoid_fast(dtv), a.pj.lo) : 0.f;
+            sum[j] = total;                                // of the rows behind
+            least = fminf(least, total), most = fmaxf(most, total);
+            total += dtv;
+            bx[j] = dtv * to_f(xr[j]);
+            bad_x = fmaf(bx[j], 0.f, bad_x);
+        }
+        const bool more = left > TT;
+        if (more) {
+            b_in(t - TT);
+            rows_in(left - TT);
+        }
+#pragma unroll
+        for (int q = 0; q < NPAIR; ++q) {
+            // the pair's largest decay in the tile
+            const float top = fmaxf(fmaxf(nan2[q].x * least, nan2[q].x * most), fmaxf(nan2[q].y * least, nan2[q].y * most));
+            if (!__any_sync(0xffffffffu, act && !(top < GONE))) continue;
+#pragma unroll
+            for (int j = 0; j < TT; ++j) {
+                const float2 e = ex2x2(mul2(f2(sum[j], sum[j]), nan2[q]));
+                const float2 Bv = *reinterpret_cast<const float2 *>(&bc[buf][j][0][g * S::NS + 2 * q]);
+                v[q] = fma2(mul2(e, f2(bx[j], bx[j])), Bv, v[q]);
+            }
+        }
+        if (more) {
+            next.write(bc[buf ^ 1]);                       // the tile before was read before the last barrier
+            __syncthreads();
+        }
+    }
+    if (bad_b != bad_b) lost[tid % S::NP] = bad_b;         // (whichever of those that found one)
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NPAIR; ++q)
+        v[q] = add2(v[q], f2(bad_x + lost[g * S::NS + 2 * q], bad_x + lost[g * S::NS + 2 * q + 1]));
     return total;
 }
 
@@ -229,12 +345,14 @@ __device__ __forceinline__ void read_rates(float2 (&nan2)[S::NS / 2], const floa
 
 template <typename E, typename BE, typename S, bool REST>
 __global__ void __launch_bounds__(THREADS, MMS_PACKED_MINB)
-scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
+scan_segments_kernel(const __grid_constant__ Args<E, BE> a)
 {
-    __shared__ __align__(16) float bc[2][TT][2][S::NP];
+    __shared__ __align__(16) float bc[2 * TT * 2 * S::NP];
+    __shared__ float lost[S::NP];
+    constexpr int NPAIR = S::NS / 2;
     const int tid = threadIdx.x, g = tid % S::G;
     const int unit = blockIdx.x / a.nd;
-    if (unit >= a.units) {                                 // rows of no sequence: zeros
+    if (!REST && unit >= a.units) {                        // rows of no sequence: zeros
         const int behind = a.seq.start(a.seq.count), before = a.seq.start(0);
         const long long lead = (long long)before * a.D, all = lead + (long long)(a.seq.rows - behind) * a.D;
         const long long step = (long long)(gridDim.x - a.units * a.nd) * THREADS;
@@ -242,59 +360,53 @@ scan_packed_kernel(const __grid_constant__ Args<E, BE> a)
             a.y[i < lead ? i : (long long)behind * a.D + (i - lead)] = from_f<E>(0.f);
         return;
     }
-    const int s = Sequences::last_at_most(a.seq.count, unit, [&](int i) { return i + a.seq.start(i) / a.seg; });
-    if (s < 0) return;
-    const int first = a.seq.start(s), end = max(first, a.seq.start(s + 1));
-    const int i = unit - (s + first / a.seg);
-    const int segs = max(1, (end - first + a.seg - 1) / a.seg);
-    if (i < 0 || i >= segs) return;
-    const bool split = segs > FEW;                         // its first segment is left for the second launch, too
-    if (REST ? i == 0 && !split : i > 0 && i == segs - 1) return;
+    Unit u;
+    if (!find_unit(a, unit, u)) return;
+    const bool late = u.i > 0 || u.segs > FEW;             // its outputs come in the second launch
+    if (REST ? !late : u.i > 0 && u.i == u.segs - 1) return;
 
     const int d = (blockIdx.x % a.nd) * S::DPB + tid / S::G;
     const bool act = d < a.D;
-    const size_t at = (size_t)(act ? d : 0) * a.N;
-    const int t0 = first + i * a.seg, t1 = min(end, t0 + a.seg);
-    float2 nan2[S::NS / 2], h[S::NS / 2];
+    const size_t at = (size_t)(act ? d : 0) * a.N, DN = (size_t)a.D * a.N;
+    float2 nan2[NPAIR], h[NPAIR];
     read_rates<S>(nan2, a.aneg + at, a.N, g, act, a.pj.on);
-    const long long row = first / a.seg;                   // of the sequence's first end state
-    const size_t DN = (size_t)a.D * a.N;
     // a sequence of more than FEW segments has more than FEW * seg rows: the next one's is another
-    float *entry = a.entry + (size_t)(first / (FEW * a.seg)) * DN + at;
-    if (i == 0) {
-        const long long from = a.seq.from(s);
-        if (REST) read_state<S>(h, entry, a.N, g, act);
-        else read_state<S>(h, a.state + (from >= 0 ? from : 0) * DN + at, a.N, g, act && from >= 0);
-        // (its last segment may write the place that it was read from)
-        if (!REST && split) write_state<S>(h, entry, a.N, g, act);
-    } else if (REST) {
-        // the states at the ends of the segments before: of the first as it is, of the others
-        // what was left of the one before and their own
-        read_state<S>(h, a.ends + row * DN + at, a.N, g, act);
+    float *entry = a.entry + (size_t)(u.row / FEW) * DN + at;
+    if (REST && u.i > 0) {
+        // the first segment's end, then of each one between what was left of it and its own
+        read_state<S>(h, a.ends + u.row * DN + at, a.N, g, act);
 #pragma unroll 2
-        for (int j = 1; j < i; ++j) {
-            float2 v[S::NS / 2];
-            read_state<S>(v, a.ends + (row + j) * DN + at, a.N, g, act);
-            const float dtv = act ? a.sums[(row + j) * a.D + d] : 0.f;
+        for (int j = 1; j < u.i; ++j) {
+            float2 v[NPAIR];
+            read_state<S>(v, a.ends + (u.row + j) * DN + at, a.N, g, act);
+            const float dtv = act ? a.sums[(size_t)(u.row + j) * a.D + d] : 0.f;
 #pragma unroll
-            for (int q = 0; q < S::NS / 2; ++q) h[q] = fma2(ex2x2(mul2(f2(dtv, dtv), nan2[q])), h[q], v[q]);
+            for (int q = 0; q < NPAIR; ++q) h[q] = fma2(ex2x2(mul2(f2(dtv, dtv), nan2[q])), h[q], v[q]);
         }
     } else {
-#pragma unroll
-        for (int q = 0; q < S::NS / 2; ++q) h[q] = f2(0.f, 0.f);
+        const long long from = REST || u.i > 0 ? -1 : a.seq.from(u.s);
+        const float *src = REST ? entry : a.state + (from >= 0 ? from : 0) * DN + at;
+        read_state<S>(h, src, a.N, g, act && (REST || from >= 0));
+        // (its last segment may write the place that it was read from)
+        if (!REST && u.i == 0 && late) write_state<S>(h, entry, a.N, g, act);
     }
-    if (REST || (i == 0 && !split)) {
-        walk<true, E, BE, S>(a, bc, h, nan2, t0, t1, d, g, act);
+    if (REST || !late) {
+        walk<E, BE, S>(a, reinterpret_cast<float(*)[TT][2][S::NP]>(bc), h, nan2, u.t0, u.t1, d, g, act);
+        if (u.i == u.segs - 1) {
+            const long long to = a.seq.to(u.s);
+            if (to >= 0) write_state<S>(h, a.state + to * DN + at, a.N, g, act);
+            return;
+        }
+        if (REST) return;
     } else {
-        const float total = walk<false, E, BE, S>(a, bc, h, nan2, t0, t1, d, g, act);
-        if (act && g == 0) a.sums[(row + i) * a.D + d] = total;
+        float2 v[NPAIR];
+        const float total = leave<E, BE, S>(a, reinterpret_cast<float(*)[TT][1][S::NP]>(bc), lost, v, nan2, u.t0, u.t1,
+                                            d, g, act);
+        if (act && g == 0) a.sums[(size_t)(u.row + u.i) * a.D + d] = total;
+#pragma unroll
+        for (int q = 0; q < NPAIR; ++q) h[q] = fma2(ex2x2(mul2(f2(total, total), nan2[q])), h[q], v[q]);
     }
-    if (i == segs - 1) {
-        const long long to = a.seq.to(s);
-        if (to >= 0) write_state<S>(h, a.state + to * DN + at, a.N, g, act);
-    } else if (!REST) {
-        write_state<S>(h, a.ends + (row + i) * DN + at, a.N, g, act);
-    }
+    write_state<S>(h, a.ends + (u.row + u.i) * DN + at, a.N, g, act);
 }
 
 // --------------------------------------------------------- single tokens
@@ -376,13 +488,30 @@ int lanes_of(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 int segment_rows(int rows, int D, int N)
 {
     const long long nd = (D + THREADS / lanes_of(N) - 1) / (THREADS / lanes_of(N));
-    const long long want = std::max<long long>(1, 4LL * N_SM / nd);
+    const long long want = std::max<long long>(1, (long long)MMS_PACKED_FILL * N_SM / nd);
     const long long seg = std::max<long long>(64, (rows + want - 1) / want);
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
 }
 
-// Sequences of more than FEW segments are told apart by start / (FEW * seg).
-int entries_of(int rows, int seg) { return rows > FEW * seg ? rows / (FEW * seg) + 1 : 0; }
+// A call's units and its workspace (bytes from the start, regions of whole 256 bytes):
+// segments before the last of their sequence, of which there is at most one for every `seg`
+// rows; entries of sequences of more than FEW segments, told apart by start / (FEW * seg).
+struct Plan {
+    int seg;
+    long long nd, units;
+    bool more;                          // a sequence can have a second segment
+    size_t sums = 0, entry = 0, total = 0;
+    Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, D, N)) {
+        nd = ((long long)D * lanes_of(N) + THREADS - 1) / THREADS;
+        units = (long long)count + rows / seg;
+        more = rows > seg;
+        const size_t ends = rows / seg, d = D;
+        auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+        sums = up(ends * d * N * 4);
+        entry = sums + up(ends * d * 4);
+        total = !more ? 0 : entry + (ends >= FEW ? up((ends / FEW + 1) * d * N * 4) : 0);
+    }
+};
 
 template <typename E, typename BE>
 Args<E, BE> args_of(const ScanPackedArgs &p)
@@ -400,20 +529,16 @@ template <typename E, typename BE, typename S>
 cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
 {
     Args<E, BE> a = args_of<E, BE>(p);
-    const int rows = p.seq.rows;
-    a.seg = segment_rows(rows, p.D, p.N);
-    a.nd = (p.D + S::DPB - 1) / S::DPB;
-    a.ends = static_cast<float *>(p.workspace);
-    a.entry = a.ends + (size_t)(rows / a.seg) * p.D * p.N;
-    a.sums = a.entry + (size_t)entries_of(rows, a.seg) * p.D * p.N;
-    const long long units = (long long)p.seq.count + rows / a.seg;
-    const long long clear = 2 * N_SM;
-    if (units * a.nd + clear > 0x7fffffffLL) return cudaErrorInvalidValue;
-    a.units = (int)units;
-    scan_packed_kernel<E, BE, S, false><<<(unsigned)(units * a.nd + clear), THREADS, 0, stream>>>(a);
+    const Plan plan(p.seq.rows, p.seq.count, p.D, p.N);
+    char *ws = static_cast<char *>(p.workspace);
+    a.seg = plan.seg, a.nd = (int)plan.nd, a.units = (int)plan.units;
+    a.ends = (float *)ws, a.sums = (float *)(ws + plan.sums), a.entry = (float *)(ws + plan.entry);
+    const long long clear = 2 * N_SM, blocks = plan.units * plan.nd;
+    if (blocks + clear > 0x7fffffffLL) return cudaErrorInvalidValue;
+    scan_segments_kernel<E, BE, S, false><<<(unsigned)(blocks + clear), THREADS, 0, stream>>>(a);
     cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || rows <= a.seg) return e;       // no sequence can have a second segment
-    scan_packed_kernel<E, BE, S, true><<<(unsigned)(units * a.nd), THREADS, 0, stream>>>(a);
+    if (e != cudaSuccess || !plan.more) return e;
+    scan_segments_kernel<E, BE, S, true><<<(unsigned)blocks, THREADS, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -452,14 +577,7 @@ cudaError_t packed_of(const ScanPackedArgs &p, cudaStream_t stream)
 
 }  // namespace
 
-// Segments before the last of their sequence, at most one for every `seg` rows, and entries.
-size_t scan_packed_workspace_bytes(int rows, int count, int D, int N)
-{
-    (void)count;
-    const int seg = segment_rows(rows, D, N);
-    const size_t ends = rows / seg, entries = entries_of(rows, seg);
-    return (ends * (N + 1) + entries * N) * D * sizeof(float);
-}
+size_t scan_packed_workspace_bytes(int rows, int count, int D, int N) { return Plan(rows, count, D, N).total; }
 
 cudaError_t launch_scan_packed(const ScanPackedArgs &p, cudaStream_t stream)
 {

@@ -158,6 +158,26 @@ def test_infinite_steps_forget_and_nan_stays_with_its_sequence():
     assert torch.equal(y[4:], z[4:]) and not torch.equal(y[:4], z[:4])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_what_enters_a_segment_far_from_its_start(dtype):
+    """NaN and infinite states reach every later row; negative steps bring decayed states back."""
+    rows = 400
+    t = make(rows, 8, 16, dtype, seed=12)
+    t["dt"] = torch.full_like(t["dt"], 4.0)                # nothing is left of a state after a few rows
+    t["x"][3, 2], t["x"][5, 4] = float("nan"), float("inf")
+    y, state = run(t, [0, rows], [0], [0])
+    assert torch.isnan(y[3:, 2]).all() and torch.isnan(state[0, 2]).all() and not torch.isfinite(y[5:, 4]).any()
+    keep = [c for c in range(8) if c not in (2, 4)]
+    assert torch.isfinite(y[:, keep]).all() and torch.isfinite(state[:, keep]).all()
+    for slow in (False, True):
+        t = make(rows, 8, 16, dtype, seed=13)
+        t["dt"] = torch.full((rows, 8), 1.0).to(dtype)
+        t["dt"][65:130:2] = -1.0 if not slow else 0.0
+        t["dt"][130:190] = -0.5 if not slow else 0.0
+        t["aneg"] = t["aneg"] * (0.1 if not slow else -0.002)      # slow: states that grow
+        check(t, [0, rows], [0], [0])
+
+
 def test_lists_that_break_the_rules_stay_inside_the_arrays():
     t = make(300, 40, 16, F32, places=5)
     guard = torch.full((7, 40, 16), 7.0, device=DEV)
