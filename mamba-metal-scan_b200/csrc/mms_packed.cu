@@ -8,8 +8,8 @@
 // mamba_metal/model.py:203-221, 228-241).
 //
 // Prompts are bound by the exponentials, one a state and step (MUFU, 16 an SM and
-// clock). A thread holds up to 16 states of one channel in registers, as the forward
-// scan does; G = 1, 2 or 4 lanes share a channel of up to 16, 32 or 64 states. A
+// clock). A thread holds up to 8 states of two neighbouring channels in registers; G = 1, 2, 4
+// or 8 lanes share the two, for up to 8, 16, 32 or 64 states. A
 // sequence is cut into segments of `seg` rows, so that one long prompt fills the GPU
 // as well as many short ones, whatever the lengths, which the host does not know:
 //   first   segments whose state is known, the first ones of short sequences, with their
@@ -36,28 +36,23 @@
 
 #include "mms_common.cuh"
 #include "mms_serve.h"
+#include "mms_stage.cuh"
 
 namespace mms {
 
 namespace {
 
 constexpr int THREADS = 128;
-constexpr int TT = 8;                   // rows of a tile of B and C
-#ifndef MMS_SUB
-#define MMS_SUB 4
-#endif
-constexpr int SUB = MMS_SUB;            // rows of x, dt and z in registers
+constexpr int TT = 8;                   // rows of a tile in shared memory
+constexpr int STAGES = 3;               // tiles of x, dt and z
 constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 flushes to 0
 // A sequence's first segment is done in full in the first launch if it has at most FEW
 // segments; of longer ones its end comes first, like the others', so that the launch does not
 // end with its CTAs alone.
 #ifndef MMS_PACKED_FEW
-#define MMS_PACKED_FEW 3
+#define MMS_PACKED_FEW 1
 #endif
 constexpr int FEW = MMS_PACKED_FEW;
-#ifndef MMS_PACKED_POLY
-#define MMS_PACKED_POLY 1
-#endif
 #ifndef MMS_PACKED_MINB
 #define MMS_PACKED_MINB 4
 #endif
@@ -82,11 +77,19 @@ struct Args {
     int units;                          // units of segments; the blocks behind them clear rows of no sequence
 };
 
-// NS states of a channel on each of G lanes.
+// A thread holds NS states of 2 neighbouring channels; G lanes share the two. Lane g has the pairs
+// g, G + g, 2G + g, .. of states: where the rates rise with the state, as they do at
+// first, a warp's lanes then come to decays of 0 together.
 template <int NS_, int G_>
 struct Split {
-    static constexpr int NS = NS_, G = G_, NP = NS_ * G_, DPB = THREADS / G_;
+    static constexpr int NS = NS_, G = G_, NP = NS_ * G_, NPAIR = NS_ / 2, DPB = 2 * THREADS / G_;
+    // the first state of lane g's pair q, and where state n lies in a row of B or C: lane by lane
+    __device__ static __forceinline__ int state(int g, int q) { return 2 * (q * G + g); }
+    __device__ static __forceinline__ int place(int n) { return n / 2 % G * NS + n / 2 / G * 2 + n % 2; }
 };
+// The states of a thread: [channel][pair of states].
+template <typename S>
+using States = float2[2][S::NPAIR];
 
 // What a CTA of a segment's launch is to do.
 struct Unit {
@@ -107,249 +110,296 @@ __device__ __forceinline__ bool find_unit(const Args<E, BE> &a, int unit, Unit &
 }
 
 // A tile of TT rows of B and C as float32 in shared memory: this thread's share of it.
-template <int NP, int ARR>
+template <typename S, int ARR>
 struct Share {
-    static constexpr int PER = (TT * ARR * NP + THREADS - 1) / THREADS;
+    static constexpr int NP = S::NP, PER = (TT * ARR * NP + THREADS - 1) / THREADS;
     float v[PER];
     template <typename BE>
-    __device__ __forceinline__ void read(const BE *B, long long ldB, const BE *C, long long ldC, int N, int t, int t1) {
+    __device__ __forceinline__ void read(const BE *B, long long ldB, const BE *C, long long ldC, int N, int t, int t0, int t1) {
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const int o = threadIdx.x + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
             v[q] = 0.f;
-            if (j < TT && n < N && t + j < t1) v[q] = arr ? to_f(C[(t + j) * ldC + n]) : to_f(B[(t + j) * ldB + n]);
+            if (j < TT && n < N && t + j >= t0 && t + j < t1)
+                v[q] = arr ? to_f(C[(t + j) * ldC + n]) : to_f(B[(t + j) * ldB + n]);
         }
     }
     __device__ __forceinline__ void write(float (*bc)[ARR][NP]) const {
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const int o = threadIdx.x + q * THREADS, n = o % NP, arr = o / NP % ARR, j = o / (NP * ARR);
-            if (j < TT) bc[j][arr][n] = v[q];
+            if (j < TT) bc[j][arr][S::place(n)] = v[q];
         }
     }
 };
 
-// ------------------------------------------------------------- segments
-
-// The rows [t0, t1) from state h, with their outputs. Rows come through registers
-// SUB at a time, the next ones requested as soon as these are converted; B and C through
-// shared memory, TT rows at a time. POLY of a thread's 8 pairs of exponentials are taken
-// from MUFU to the FMA pipe (16384 x 2048 x 16: 0 pairs 360 us, 1 343, 2 366, in the form with two
-// walks).
-template <typename E, typename BE, typename S>
-__device__ __forceinline__ void walk(const Args<E, BE> &a, float (*bc)[TT][2][S::NP], float2 (&h)[S::NS / 2],
-                                      const float2 (&nan2)[S::NS / 2], int t0, int t1, int d, int g, bool act)
+// Rows t .. t + TT - 1 of ARR of x, dt and z, channels d0 .. d0 + DPB - 1, to a tile [row][array][channel];
+// zeros for rows outside [t0, t1) and channels behind the last. VEC: 16 bytes at a time (D, the
+// strides and the bases whole 16 bytes); else one element, bf16 ones through registers.
+template <bool VEC, int ARR, int DPB, typename E, typename BE>
+__device__ __forceinline__ void stage(const Args<E, BE> &a, E *tile, int d0, int t, int t0, int t1)
 {
-    constexpr int NS = S::NS;
-    constexpr int POLY = MMS_PACKED_POLY * NS / 16;
-    const bool gate = a.z != nullptr;
-    const float skip = a.d_skip && act ? a.d_skip[d] : 0.f;
-    const int ds = act ? d : 0;                            // a channel that is there
-    const E *xp = a.x + t0 * a.ldx + ds, *dp = a.dt + t0 * a.lddt + ds;
-    const E *zp = gate ? a.z + t0 * a.ldz + ds : a.x;
-    const long long ldz = gate ? a.ldz : 0;
-    long long yo = (long long)t0 * a.D + ds;
-    E xr[SUB], dr[SUB], zr[SUB];
-    auto rows_in = [&](int left) {                         // the next SUB rows, of which `left` are there
+    constexpr int EPV = VEC ? 16 / (int)sizeof(E) : 1, CH = DPB / EPV, ALL = TT * ARR * CH;
 #pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            if (j < left) {
-                xr[j] = *xp, dr[j] = *dp;
-                if (gate) zr[j] = *zp;
-            } else {
-                xr[j] = dr[j] = from_f<E>(0.f);
-            }
-            xp += a.ldx, dp += a.lddt, zp += ldz;
-        }
-    };
-    Share<S::NP, 2> next;
-    next.read(a.B, a.ldB, a.C, a.ldC, a.N, t0, t1);
-    rows_in(t1 - t0);
-    next.write(bc[0]);
-    __syncthreads();
-    int buf = 0;
-    for (int t = t0; t < t1; t += TT, buf ^= 1) {
-        const bool more = t + TT < t1;
-        if (more) next.read(a.B, a.ldB, a.C, a.ldC, a.N, t + TT, t1);
-#pragma unroll
-        for (int sub = 0; sub < TT; sub += SUB) {
-            const int left = t1 - t - sub;                 // rows from here on
-            if (sub > 0 && left <= 0) break;
-            float xf[SUB], df[SUB], gf[SUB];
-#pragma unroll
-            for (int j = 0; j < SUB; ++j) xf[j] = to_f(xr[j]), df[j] = to_f(dr[j]), gf[j] = 1.f;
-            if (a.pj.on) {
-#pragma unroll
-                for (int j = 0; j < SUB; ++j) df[j] = j < left ? fmaf(a.pj.range, sigmoid_fast(df[j]), a.pj.lo) : 0.f;
-            }
-            if (gate) {
-#pragma unroll
-                for (int j = 0; j < SUB; ++j) gf[j] = to_f(zr[j]) * sigmoid_fast(to_f(zr[j]));
-            }
-            rows_in(left - SUB);
-            // rows behind the last have dt = 0: decay 1, nothing added
-#pragma unroll
-            for (int j = 0; j < SUB; ++j) {
-                const float2 dt2 = f2(df[j], df[j]), bx2 = f2(df[j] * xf[j], df[j] * xf[j]);
-                const float4 *bp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][0][g * NS]);
-                const float4 *cp = reinterpret_cast<const float4 *>(&bc[buf][sub + j][1][g * NS]);
-                float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-                for (int q = 0; q < NS / 4; ++q) {
-                    const float4 Bv = bp[q], Cv = cp[q];
-                    const float2 e0 = mul2(dt2, nan2[2 * q]), e1 = mul2(dt2, nan2[2 * q + 1]);
-                    h[2 * q] = fma2(2 * q < POLY ? ex2_poly2(e0) : ex2x2(e0), h[2 * q], mul2(bx2, lo(Bv)));
-                    h[2 * q + 1] = fma2(2 * q + 1 < POLY ? ex2_poly2(e1) : ex2x2(e1), h[2 * q + 1], mul2(bx2, hi(Bv)));
-                    acc[0] = fma2(lo(Cv), h[2 * q], acc[0]);
-                    acc[1] = fma2(hi(Cv), h[2 * q + 1], acc[1]);
-                }
-                acc[0] = add2(acc[0], acc[1]);
-                float yv = acc[0].x + acc[0].y;
-#pragma unroll
-                for (int o = S::G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
-                yv = (yv + skip) * gf[j];
-                if (act && g == 0 && j < left) a.y[yo] = from_f<E>(yv);
-                yo += a.D;
-            }
-        }
-        if (more) {
-            next.write(bc[buf ^ 1]);                       // the tile before was read before the last barrier
-            __syncthreads();
-        }
+    for (int k0 = 0; k0 < ALL; k0 += THREADS) {
+        const int k = k0 + threadIdx.x;
+        if (ALL % THREADS && k >= ALL) break;
+        const int q = k % CH, arr = k / CH % ARR, r = k / (CH * ARR), d = d0 + EPV * q;
+        const bool in = t + r >= t0 && t + r < t1 && d < a.D;
+        const E *src = arr == 0 ? a.x + (t + r) * a.ldx : arr == 1 ? a.dt + (t + r) * a.lddt : a.z + (t + r) * a.ldz;
+        E *to = tile + (r * ARR + arr) * DPB + EPV * q;
+        if constexpr (VEC) cp16(to, in ? src + d : a.x, in);
+        else if constexpr (sizeof(E) == 4) cp4(to, in ? src + d : a.x, in);
+        else *to = in ? src[d] : from_f<E>(0.f);
+    }
+    cp_commit();
+}
+
+// Both channels' values of a tile's row.
+template <typename E>
+__device__ __forceinline__ float2 both(const E *p)
+{
+    if constexpr (sizeof(E) == 4) {
+        return *reinterpret_cast<const float2 *>(p);
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
+        return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     }
 }
 
-// What the rows [t0, t1) leave of nothing, v, and the sum of their dt, from the last row back.
+// ------------------------------------------------------------- segments
+
+// The rows [t0, t1) from states h, with their outputs. Every value of B and C that a lane takes
+// from shared memory serves its two channels: read for one channel each, 8 of them 16
+// bytes at a time a row, they take as long as the row's 16 exponentials
+// (shared memory returns 128 bytes a clock, 16 for the lanes of a quarter warp that all
+// read the same). All exponentials are MUFU's: with one, two or three of a thread's 8 pairs on the FMA pipe the
+// second launch took 184, 198 and 215 us, without 183 (16384 x 2048 x 16, float32).
+template <bool VEC, bool GATE, typename E, typename BE, typename S>
+__device__ __forceinline__ void walk(const Args<E, BE> &a, float (*bc)[TT][2][S::NP], E *tiles, States<S> &h,
+                                     const States<S> &nan2, int t0, int t1, int d0)
+{
+    constexpr int G = S::G, DPB = S::DPB, ARR = GATE ? 3 : 2, TILE = TT * ARR * DPB;
+    const int tid = threadIdx.x, g = tid % G, c = 2 * (tid / G);
+    // the channels whose outputs this lane writes: both, or one of them (lanes 0 and 1 of G)
+    const int own = G == 1 ? 0 : g & 1;
+    const int d = d0 + c + own;
+    const bool out0 = g < 2 && d < a.D, out1 = G == 1 && d + 1 < a.D;
+    const float skip0 = a.d_skip && out0 ? a.d_skip[d] : 0.f, skip1 = a.d_skip && out1 ? a.d_skip[d + 1] : 0.f;
+    Share<S, 2> next;
+    next.read(a.B, a.ldB, a.C, a.ldC, a.N, t0, t0, t1);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) stage<VEC, ARR, DPB>(a, tiles + s * TILE, d0, t0 + s * TT, t0, t1);
+    next.write(bc[0]);
+    E *yp = a.y + (long long)t0 * a.D + (out0 ? d : 0);
+    int buf = 0, at = 0;                                   // of B and C, of the tile
+    for (int t = t0; t < t1; t += TT, buf ^= 1) {
+        cp_wait<STAGES - 2>();
+        __syncthreads();                                   // the tile is there, the one before it read
+        const int ahead = at == 0 ? STAGES - 1 : at - 1;
+        stage<VEC, ARR, DPB>(a, tiles + ahead * TILE, d0, t + (STAGES - 1) * TT, t0, t1);
+        const bool more = t + TT < t1;
+        if (more) next.read(a.B, a.ldB, a.C, a.ldC, a.N, t + TT, t0, t1);
+        const E *row = tiles + at * TILE + c;
+        const int left = t1 - t;
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+            const float2 xv = both(row + j * ARR * DPB);
+            float2 dtv = both(row + (j * ARR + 1) * DPB);
+            if (a.pj.on)                                   // (rows behind the last have dt = 0)
+                dtv = j < left ? f2(fmaf(a.pj.range, sigmoid_fast(dtv.x), a.pj.lo), fmaf(a.pj.range, sigmoid_fast(dtv.y), a.pj.lo))
+                               : f2(0.f, 0.f);
+            const float2 bx = mul2(dtv, xv);
+            const float4 *bp = reinterpret_cast<const float4 *>(&bc[buf][j][0][g * S::NS]);
+            const float4 *cp = reinterpret_cast<const float4 *>(&bc[buf][j][1][g * S::NS]);
+            float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+            for (int q = 0; q < S::NPAIR / 2; ++q) {
+                const float4 Bv = bp[q], Cv = cp[q];
+#pragma unroll
+                for (int ch = 0; ch < 2; ++ch) {
+                    const float dt1 = ch ? dtv.y : dtv.x, bx1 = ch ? bx.y : bx.x;
+                    const float2 e0 = mul2(f2(dt1, dt1), nan2[ch][2 * q]), e1 = mul2(f2(dt1, dt1), nan2[ch][2 * q + 1]);
+                    h[ch][2 * q] = fma2(ex2x2(e0), h[ch][2 * q], mul2(f2(bx1, bx1), lo(Bv)));
+                    h[ch][2 * q + 1] = fma2(ex2x2(e1), h[ch][2 * q + 1], mul2(f2(bx1, bx1), hi(Bv)));
+                    acc[ch] = fma2(lo(Cv), h[ch][2 * q], acc[ch]);
+                    acc[ch] = fma2(hi(Cv), h[ch][2 * q + 1], acc[ch]);
+                }
+            }
+            float y0 = acc[0].x + acc[0].y, y1 = acc[1].x + acc[1].y;
+            if (G > 1) {                                   // lanes of even g go on with the first channel
+                const float mine = own ? y1 : y0, other = own ? y0 : y1;
+                y0 = mine + __shfl_xor_sync(0xffffffffu, other, 1);
+#pragma unroll
+                for (int o = 2; o < G; o *= 2) y0 += __shfl_xor_sync(0xffffffffu, y0, o);
+            }
+            y0 += skip0, y1 += skip1;
+            if (GATE) {
+                const float z0 = to_f(row[(j * ARR + 2) * DPB + own]);
+                y0 *= z0 * sigmoid_fast(z0);
+                if (G == 1) {
+                    const float z1 = to_f(row[(j * ARR + 2) * DPB + 1]);
+                    y1 *= z1 * sigmoid_fast(z1);
+                }
+            }
+            if (out0 && j < left) *yp = from_f<E>(y0);
+            if (out1 && j < left) yp[1] = from_f<E>(y1);
+            yp += a.D;
+        }
+        if (more) next.write(bc[buf ^ 1]);
+        at = at + 1 < STAGES ? at + 1 : 0;
+    }
+    cp_wait<0>();
+    __syncthreads();
+}
+
+// What the rows [t0, t1) leave of nothing, v, and the sums of their dt, from the last row back.
 // An x or B that is not finite stays in the state for good, whatever its decay: a product
 // with 0 keeps it, also where its row is left out.
-template <typename E, typename BE, typename S>
-__device__ __forceinline__ float leave(const Args<E, BE> &a, float (*bc)[TT][1][S::NP], float (&lost)[S::NP],
-                                       float2 (&v)[S::NS / 2], const float2 (&nan2)[S::NS / 2], int t0, int t1, int d,
-                                       int g, bool act)
+template <bool VEC, typename E, typename BE, typename S>
+__device__ __forceinline__ float2 leave(const Args<E, BE> &a, float (*bc)[TT][1][S::NP], float (&lost)[S::NP], E *tiles,
+                                        States<S> &v, const States<S> &nan2, int t0, int t1, int d0, int channels)
 {
-    constexpr int NPAIR = S::NS / 2;
-    const int tid = threadIdx.x, ds = act ? d : 0;
-    const E *xp = a.x + (t1 - 1) * a.ldx + ds, *dp = a.dt + (t1 - 1) * a.lddt + ds;
-    E xr[TT], dr[TT];                                      // rows t - 1, t - 2, ..
-    auto rows_in = [&](int left) {
-#pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            if (j < left) {
-                xr[j] = *xp, dr[j] = *dp;
-            } else {
-                xr[j] = dr[j] = from_f<E>(0.f);
-            }
-            xp -= a.ldx, dp -= a.lddt;
-        }
-    };
+    constexpr int G = S::G, DPB = S::DPB, TILE = TT * 2 * DPB;
+    const int tid = threadIdx.x, g = tid % G, c = 2 * (tid / G);
     if (tid < S::NP) lost[tid] = 0.f;
-    // (rows of B in front of t0 are other segments', or not there: read() takes rows from t0 on)
-    Share<S::NP, 1> next;
+    Share<S, 1> next;
     float bad_b = 0.f;
-    auto b_in = [&](int t) {                               // rows t - 1 down to t - TT
+    auto b_in = [&](int t) { next.read(a.B, a.ldB, a.B, a.ldB, a.N, t, t0, t1); };   // rows t .. t + TT - 1
+    auto b_out = [&](int buf) {
 #pragma unroll
-        for (int q = 0; q < next.PER; ++q) {
-            const int o = tid + q * THREADS, n = o % S::NP, j = o / S::NP;
-            next.v[q] = 0.f;
-            if (j < TT && n < a.N && t - 1 - j >= t0) next.v[q] = to_f(a.B[(t - 1 - j) * a.ldB + n]);
-            bad_b = fmaf(next.v[q], 0.f, bad_b);
-        }
+        for (int q = 0; q < next.PER; ++q) bad_b = fmaf(next.v[q], 0.f, bad_b);
+        next.write(bc[buf]);
     };
 #pragma unroll
-    for (int q = 0; q < NPAIR; ++q) v[q] = f2(0.f, 0.f);
-    b_in(t1);
-    rows_in(t1 - t0);
-    next.write(bc[0]);
-    __syncthreads();
-    float total = 0.f, bad_x = 0.f;
-    int buf = 0;
-    for (int t = t1; t > t0; t -= TT, buf ^= 1) {
-        const int left = t - t0;
-        float sum[TT], bx[TT], least = INFINITY, most = -INFINITY;
+    for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            float dtv = to_f(dr[j]);
-            if (a.pj.on) dtv = j < left ? fmaf(a.pj.range, sigmoid_fast(dtv), a.pj.lo) : 0.f;
+        for (int q = 0; q < S::NPAIR; ++q) v[ch][q] = f2(0.f, 0.f);
+    b_in(t1 - TT);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) stage<VEC, 2, DPB>(a, tiles + s * TILE, d0, t1 - (s + 1) * TT, t0, t1);
+    b_out(0);
+    float2 total = f2(0.f, 0.f), bad_x = f2(0.f, 0.f);
+    int buf = 0, at = 0;
+    for (int t = t1 - TT; t > t0 - TT; t -= TT, buf ^= 1) {        // rows t .. t + TT - 1
+        cp_wait<STAGES - 2>();
+        __syncthreads();
+        const int ahead = at == 0 ? STAGES - 1 : at - 1;
+        stage<VEC, 2, DPB>(a, tiles + ahead * TILE, d0, t - (STAGES - 1) * TT, t0, t1);
+        const bool more = t > t0;
+        if (more) b_in(t - TT);
+        const E *row = tiles + at * TILE + c;
+        float2 sum[TT], bx[TT], least = total, most = total;
+#pragma unroll
+        for (int j = TT - 1; j >= 0; --j) {
+            float2 dtv = both(row + (2 * j + 1) * DPB);
+            if (a.pj.on)
+                dtv = t + j >= t0 ? f2(fmaf(a.pj.range, sigmoid_fast(dtv.x), a.pj.lo), fmaf(a.pj.range, sigmoid_fast(dtv.y), a.pj.lo))
+                                  : f2(0.f, 0.f);
             sum[j] = total;                                // of the rows behind
-            least = fminf(least, total), most = fmaxf(most, total);
-            total += dtv;
-            bx[j] = dtv * to_f(xr[j]);
-            bad_x = fmaf(bx[j], 0.f, bad_x);
-        }
-        const bool more = left > TT;
-        if (more) {
-            b_in(t - TT);
-            rows_in(left - TT);
+            least = f2(fminf(least.x, total.x), fminf(least.y, total.y));
+            most = f2(fmaxf(most.x, total.x), fmaxf(most.y, total.y));
+            total = add2(total, dtv);
+            bx[j] = mul2(dtv, both(row + 2 * j * DPB));
+            bad_x = fma2(bx[j], f2(0.f, 0.f), bad_x);
         }
 #pragma unroll
-        for (int q = 0; q < NPAIR; ++q) {
-            // the pair's largest decay in the tile
-            const float top = fmaxf(fmaxf(nan2[q].x * least, nan2[q].x * most), fmaxf(nan2[q].y * least, nan2[q].y * most));
-            if (!__any_sync(0xffffffffu, act && !(top < GONE))) continue;
+        for (int q = 0; q < S::NPAIR; ++q) {
+            // the largest decay of the two channels' pairs in the tile
+            float top = __int_as_float(0xff800000);
 #pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                const float2 e = ex2x2(mul2(f2(sum[j], sum[j]), nan2[q]));
+            for (int ch = 0; ch < 2; ++ch) {
+                const float lo1 = ch ? least.y : least.x, hi1 = ch ? most.y : most.x;
+                const float2 r = nan2[ch][q];
+                if (ch < channels) top = fmaxf(fmaxf(top, fmaxf(r.x * lo1, r.x * hi1)), fmaxf(r.y * lo1, r.y * hi1));
+            }
+            if (!__any_sync(0xffffffffu, S::state(g, q) < a.N && !(top < GONE))) continue;
+#pragma unroll
+            for (int j = TT - 1; j >= 0; --j) {
                 const float2 Bv = *reinterpret_cast<const float2 *>(&bc[buf][j][0][g * S::NS + 2 * q]);
-                v[q] = fma2(mul2(e, f2(bx[j], bx[j])), Bv, v[q]);
+#pragma unroll
+                for (int ch = 0; ch < 2; ++ch) {
+                    const float s1 = ch ? sum[j].y : sum[j].x, b1 = ch ? bx[j].y : bx[j].x;
+                    const float2 e = ex2x2(mul2(f2(s1, s1), nan2[ch][q]));
+                    v[ch][q] = fma2(mul2(e, f2(b1, b1)), Bv, v[ch][q]);
+                }
             }
         }
-        if (more) {
-            next.write(bc[buf ^ 1]);                       // the tile before was read before the last barrier
-            __syncthreads();
-        }
+        if (more) b_out(buf ^ 1);
+        at = at + 1 < STAGES ? at + 1 : 0;
     }
-    if (bad_b != bad_b) lost[tid % S::NP] = bad_b;         // (whichever of those that found one)
+    cp_wait<0>();
+    if (bad_b != bad_b) lost[S::place(tid % S::NP)] = bad_b;         // (whichever of those that found one)
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < NPAIR; ++q)
-        v[q] = add2(v[q], f2(bad_x + lost[g * S::NS + 2 * q], bad_x + lost[g * S::NS + 2 * q + 1]));
+    for (int q = 0; q < S::NPAIR; ++q) {
+        const float2 bad = *reinterpret_cast<const float2 *>(&lost[g * S::NS + 2 * q]);
+        v[0][q] = add2(v[0][q], add2(bad, f2(bad_x.x, bad_x.x)));
+        v[1][q] = add2(v[1][q], add2(bad, f2(bad_x.y, bad_x.y)));
+    }
     return total;
 }
 
+// This lane's states of channels d and d + 1 from p, channel d's; zeros where a channel or state is not there.
 template <typename S>
-__device__ __forceinline__ void read_state(float2 (&h)[S::NS / 2], const float *p, int N, int g, bool act)
+__device__ __forceinline__ void read_states(States<S> &h, const float *p, int N, int g, int channels)
 {
 #pragma unroll
-    for (int q = 0; q < S::NS / 4; ++q) {
-        const int n = g * S::NS + 4 * q;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (act && n < N) v = *reinterpret_cast<const float4 *>(p + n);
-        h[2 * q] = lo(v);
-        h[2 * q + 1] = hi(v);
-    }
+    for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+        for (int q = 0; q < S::NPAIR; ++q) {
+            const int n = S::state(g, q);
+            h[ch][q] = ch < channels && n < N ? *reinterpret_cast<const float2 *>(p + ch * N + n) : f2(0.f, 0.f);
+        }
 }
 
 template <typename S>
-__device__ __forceinline__ void write_state(const float2 (&h)[S::NS / 2], float *p, int N, int g, bool act)
+__device__ __forceinline__ void write_states(const States<S> &h, float *p, int N, int g, int channels)
 {
 #pragma unroll
-    for (int q = 0; q < S::NS / 4; ++q) {
-        const int n = g * S::NS + 4 * q;
-        if (act && n < N) st4(p + n, make_float4(h[2 * q].x, h[2 * q].y, h[2 * q + 1].x, h[2 * q + 1].y));
-    }
+    for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+        for (int q = 0; q < S::NPAIR; ++q) {
+            const int n = S::state(g, q);
+            if (ch < channels && n < N) *reinterpret_cast<float2 *>(p + ch * N + n) = h[ch][q];
+        }
 }
 
-// -Aneg * log2(e) of the lane's states, 0 behind the last
+// -Aneg * log2(e) of the lane's states, 0 where there is none
 template <typename S>
-__device__ __forceinline__ void read_rates(float2 (&nan2)[S::NS / 2], const float *aneg, int N, int g, bool act, bool raw)
+__device__ __forceinline__ void read_rates(States<S> &nan2, const float *aneg, int N, int g, int channels, bool raw)
 {
-    read_state<S>(nan2, aneg, N, g, act);
+    read_states<S>(nan2, aneg, N, g, channels);
 #pragma unroll
-    for (int q = 0; q < S::NS / 2; ++q) {
-        float2 v = nan2[q];
-        if (raw) v = f2(softplus(v.x), softplus(v.y));
-        const bool in = act && g * S::NS + 2 * q < N;
-        nan2[q] = in ? f2(-v.x * MMS_LOG2E, -v.y * MMS_LOG2E) : f2(0.f, 0.f);
+    for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+        for (int q = 0; q < S::NPAIR; ++q) {
+            float2 v = nan2[ch][q];
+            if (raw) v = f2(softplus(v.x), softplus(v.y));
+            nan2[ch][q] = ch < channels && S::state(g, q) < N ? f2(-v.x * MMS_LOG2E, -v.y * MMS_LOG2E) : f2(0.f, 0.f);
+        }
+}
+
+// h moved over a segment whose dt have these sums, and what the segment leaves of nothing
+template <typename S>
+__device__ __forceinline__ void carry(States<S> &h, const States<S> &nan2, float2 sums, const States<S> &v)
+{
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        const float s = ch ? sums.y : sums.x;
+#pragma unroll
+        for (int q = 0; q < S::NPAIR; ++q) h[ch][q] = fma2(ex2x2(mul2(f2(s, s), nan2[ch][q])), h[ch][q], v[ch][q]);
     }
 }
 
-template <typename E, typename BE, typename S, bool REST>
+template <typename E, typename BE, typename S, bool REST, bool VEC>
 __global__ void __launch_bounds__(THREADS, MMS_PACKED_MINB)
 scan_segments_kernel(const __grid_constant__ Args<E, BE> a)
 {
     __shared__ __align__(16) float bc[2 * TT * 2 * S::NP];
-    __shared__ float lost[S::NP];
-    constexpr int NPAIR = S::NS / 2;
+    __shared__ __align__(8) float lost[S::NP];
+    extern __shared__ __align__(16) unsigned char rows[];
+    E *tiles = reinterpret_cast<E *>(rows);
     const int tid = threadIdx.x, g = tid % S::G;
     const int unit = blockIdx.x / a.nd;
     if (!REST && unit >= a.units) {                        // rows of no sequence: zeros
@@ -365,48 +415,58 @@ scan_segments_kernel(const __grid_constant__ Args<E, BE> a)
     const bool late = u.i > 0 || u.segs > FEW;             // its outputs come in the second launch
     if (REST ? !late : u.i > 0 && u.i == u.segs - 1) return;
 
-    const int d = (blockIdx.x % a.nd) * S::DPB + tid / S::G;
-    const bool act = d < a.D;
-    const size_t at = (size_t)(act ? d : 0) * a.N, DN = (size_t)a.D * a.N;
-    float2 nan2[NPAIR], h[NPAIR];
-    read_rates<S>(nan2, a.aneg + at, a.N, g, act, a.pj.on);
+    const int d0 = (blockIdx.x % a.nd) * S::DPB, d = d0 + 2 * (tid / S::G);
+    const int channels = min(2, max(0, a.D - d));          // of the lane's that are there
+    const size_t at = channels ? (size_t)d * a.N : 0, DN = (size_t)a.D * a.N;
+    States<S> nan2, h;
+    read_rates<S>(nan2, a.aneg + at, a.N, g, channels, a.pj.on);
     // a sequence of more than FEW segments has more than FEW * seg rows: the next one's is another
     float *entry = a.entry + (size_t)(u.row / FEW) * DN + at;
     if (REST && u.i > 0) {
         // the first segment's end, then of each one between what was left of it and its own
-        read_state<S>(h, a.ends + u.row * DN + at, a.N, g, act);
-#pragma unroll 2
-        for (int j = 1; j < u.i; ++j) {
-            float2 v[NPAIR];
-            read_state<S>(v, a.ends + (u.row + j) * DN + at, a.N, g, act);
-            const float dtv = act ? a.sums[(size_t)(u.row + j) * a.D + d] : 0.f;
+        read_states<S>(h, a.ends + u.row * DN + at, a.N, g, channels);
+        constexpr int AHEAD = 3;                           // ends that are read at a time
+        for (int j = 1; j < u.i; j += AHEAD) {
+            States<S> v[AHEAD];
+            float2 sums[AHEAD];
 #pragma unroll
-            for (int q = 0; q < NPAIR; ++q) h[q] = fma2(ex2x2(mul2(f2(dtv, dtv), nan2[q])), h[q], v[q]);
+            for (int k = 0; k < AHEAD; ++k) {
+                const int c = j + k < u.i ? channels : 0;
+                read_states<S>(v[k], a.ends + (u.row + j + k) * DN + at, a.N, g, c);
+                const float *s = a.sums + (size_t)(u.row + j + k) * a.D + d;
+                sums[k] = f2(c > 0 ? s[0] : 0.f, c > 1 ? s[1] : 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (j + k < u.i) carry<S>(h, nan2, sums[k], v[k]);
         }
     } else {
         const long long from = REST || u.i > 0 ? -1 : a.seq.from(u.s);
         const float *src = REST ? entry : a.state + (from >= 0 ? from : 0) * DN + at;
-        read_state<S>(h, src, a.N, g, act && (REST || from >= 0));
+        read_states<S>(h, src, a.N, g, REST || from >= 0 ? channels : 0);
         // (its last segment may write the place that it was read from)
-        if (!REST && u.i == 0 && late) write_state<S>(h, entry, a.N, g, act);
+        if (!REST && u.i == 0 && late) write_states<S>(h, entry, a.N, g, channels);
     }
     if (REST || !late) {
-        walk<E, BE, S>(a, reinterpret_cast<float(*)[TT][2][S::NP]>(bc), h, nan2, u.t0, u.t1, d, g, act);
+        auto tile = reinterpret_cast<float(*)[TT][2][S::NP]>(bc);
+        if (a.z) walk<VEC, true, E, BE, S>(a, tile, tiles, h, nan2, u.t0, u.t1, d0);
+        else walk<VEC, false, E, BE, S>(a, tile, tiles, h, nan2, u.t0, u.t1, d0);
         if (u.i == u.segs - 1) {
             const long long to = a.seq.to(u.s);
-            if (to >= 0) write_state<S>(h, a.state + to * DN + at, a.N, g, act);
+            if (to >= 0) write_states<S>(h, a.state + to * DN + at, a.N, g, channels);
             return;
         }
         if (REST) return;
     } else {
-        float2 v[NPAIR];
-        const float total = leave<E, BE, S>(a, reinterpret_cast<float(*)[TT][1][S::NP]>(bc), lost, v, nan2, u.t0, u.t1,
-                                            d, g, act);
-        if (act && g == 0) a.sums[(size_t)(u.row + u.i) * a.D + d] = total;
-#pragma unroll
-        for (int q = 0; q < NPAIR; ++q) h[q] = fma2(ex2x2(mul2(f2(total, total), nan2[q])), h[q], v[q]);
+        States<S> v;
+        const float2 total = leave<VEC, E, BE, S>(a, reinterpret_cast<float(*)[TT][1][S::NP]>(bc), lost, tiles, v, nan2,
+                                                  u.t0, u.t1, d0, channels);
+        float *s = a.sums + (size_t)(u.row + u.i) * a.D + d;
+        if (g == 0 && channels > 0) s[0] = total.x;
+        if (g == 0 && channels > 1) s[1] = total.y;
+        carry<S>(h, nan2, total, v);
     }
-    write_state<S>(h, a.ends + (u.row + u.i) * DN + at, a.N, g, act);
+    write_states<S>(h, a.ends + (u.row + u.i) * DN + at, a.N, g, channels);
 }
 
 // --------------------------------------------------------- single tokens
@@ -481,13 +541,20 @@ scan_token_kernel(const __grid_constant__ Args<E, BE> a)
 
 // ----------------------------------------------------------------- launch
 
-int lanes_of(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+// Lanes that share two channels in the segments' launches.
+int lanes_of(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }
+
+long long channel_blocks(int D, int N)
+{
+    const int dpb = 2 * THREADS / lanes_of(N);
+    return (D + dpb - 1) / dpb;
+}
 
 // Rows of a segment: as few as give every SM 4 CTAs (16 warps, what the registers hold)
 // when the rows belong to one sequence, at least 64, a whole number of tiles.
 int segment_rows(int rows, int D, int N)
 {
-    const long long nd = (D + THREADS / lanes_of(N) - 1) / (THREADS / lanes_of(N));
+    const long long nd = channel_blocks(D, N);
     const long long want = std::max<long long>(1, (long long)MMS_PACKED_FILL * N_SM / nd);
     const long long seg = std::max<long long>(64, (rows + want - 1) / want);
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
@@ -502,7 +569,7 @@ struct Plan {
     bool more;                          // a sequence can have a second segment
     size_t sums = 0, entry = 0, total = 0;
     Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, D, N)) {
-        nd = ((long long)D * lanes_of(N) + THREADS - 1) / THREADS;
+        nd = channel_blocks(D, N);
         units = (long long)count + rows / seg;
         more = rows > seg;
         const size_t ends = rows / seg, d = D;
@@ -525,6 +592,9 @@ Args<E, BE> args_of(const ScanPackedArgs &p)
     return a;
 }
 
+// the tiles of the widest CTA (256 channels, N up to 8, float32 with a gate)
+constexpr size_t MAX_TILES = (size_t)STAGES * TT * 3 * 2 * THREADS * sizeof(float);
+
 template <typename E, typename BE, typename S>
 cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
 {
@@ -535,11 +605,25 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
     a.ends = (float *)ws, a.sums = (float *)(ws + plan.sums), a.entry = (float *)(ws + plan.entry);
     const long long clear = 2 * N_SM, blocks = plan.units * plan.nd;
     if (blocks + clear > 0x7fffffffLL) return cudaErrorInvalidValue;
-    scan_segments_kernel<E, BE, S, false><<<(unsigned)(blocks + clear), THREADS, 0, stream>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || !plan.more) return e;
-    scan_segments_kernel<E, BE, S, true><<<(unsigned)blocks, THREADS, 0, stream>>>(a);
-    return cudaGetLastError();
+    auto launch = [&](auto vec) {
+        constexpr bool VEC = decltype(vec)::value;
+        const size_t smem = (size_t)STAGES * TT * (a.z ? 3 : 2) * S::DPB * sizeof(E);
+        cudaError_t e = smem_opt_in<scan_segments_kernel<E, BE, S, false, VEC>>(MAX_TILES);
+        if (e == cudaSuccess) e = smem_opt_in<scan_segments_kernel<E, BE, S, true, VEC>>(MAX_TILES);
+        if (e != cudaSuccess) return e;
+        scan_segments_kernel<E, BE, S, false, VEC><<<(unsigned)(blocks + clear), THREADS, smem, stream>>>(a);
+        e = cudaGetLastError();
+        if (e != cudaSuccess || !plan.more) return e;
+        scan_segments_kernel<E, BE, S, true, VEC><<<(unsigned)blocks, THREADS, smem, stream>>>(a);
+        return cudaGetLastError();
+    };
+    // whole 16 bytes of rows
+    auto whole = [&](const void *p, long long ld) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (long long)sizeof(E) % 16 == 0;
+    };
+    if (p.D * sizeof(E) % 16 == 0 && whole(p.x, p.ldx) && whole(p.dt, p.lddt) && (!p.z || whole(p.z, p.ldz)))
+        return launch(std::true_type{});
+    return launch(std::false_type{});
 }
 
 template <typename E, typename BE, int G>
@@ -570,9 +654,9 @@ cudaError_t packed_of(const ScanPackedArgs &p, cudaStream_t stream)
     }
     if (p.N <= 4) return segments_of<E, BE, Split<4, 1>>(p, stream);
     if (p.N <= 8) return segments_of<E, BE, Split<8, 1>>(p, stream);
-    if (p.N <= 16) return segments_of<E, BE, Split<16, 1>>(p, stream);
-    if (p.N <= 32) return segments_of<E, BE, Split<16, 2>>(p, stream);
-    return segments_of<E, BE, Split<16, 4>>(p, stream);
+    if (p.N <= 16) return segments_of<E, BE, Split<8, 2>>(p, stream);
+    if (p.N <= 32) return segments_of<E, BE, Split<8, 4>>(p, stream);
+    return segments_of<E, BE, Split<8, 8>>(p, stream);
 }
 
 }  // namespace
