@@ -632,10 +632,13 @@ cudaError_t tokens_of(const ScanPackedArgs &p, cudaStream_t stream)
     Args<E, BE> a = args_of<E, BE>(p);
     a.nd = (p.D * G + TOKEN_THREADS - 1) / TOKEN_THREADS;
     // 4 sequences a thread once that still leaves 8 CTAs an SM, else one: the shorter chain of loads
-    const bool many = (long long)a.nd * p.seq.count >= 4LL * 8 * N_SM;
-    const long long blocks = (long long)a.nd * (many ? (p.seq.count + 3) / 4 : p.seq.count);
+#ifndef MMS_TOKEN_SEQ
+#define MMS_TOKEN_SEQ 1
+#endif
+    const bool many = MMS_TOKEN_SEQ > 1 && (long long)a.nd * p.seq.count >= (long long)MMS_TOKEN_SEQ * 8 * N_SM;
+    const long long blocks = (long long)a.nd * (many ? (p.seq.count + MMS_TOKEN_SEQ - 1) / MMS_TOKEN_SEQ : p.seq.count);
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (many) scan_token_kernel<E, BE, G, 4><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a);
+    if (many) scan_token_kernel<E, BE, G, MMS_TOKEN_SEQ><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a);
     else scan_token_kernel<E, BE, G, 1><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a);
     return cudaGetLastError();
 }

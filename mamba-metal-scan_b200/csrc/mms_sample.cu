@@ -21,10 +21,13 @@
 //   k up to 256 C: every warp has the j-th largest of its 32 lanes' maxima, j = k / warps
 //     rounded up; the smallest of these has k entries above it or equal, and not many
 //     more. Those are listed and sorted, and all else happens on the list.
-//   else: the end of the run of k entries, and of the mass p, is found by bins over the
-//     range of the logits, counts or weights of 2048 equal bins; then the bin in question
-//     becomes the range, until it holds one value or few enough entries to sort.
-// The row is read from HBM once; the later passes, one to five, find it in L2.
+//   else: the end of the run of k entries, or of the mass p, is found by bins over the
+//     range of the logits, counts and weights of 2048 equal bins. If the entries down to the bin in
+//     question fit the list, all else happens there; otherwise that bin becomes the range,
+//     until it holds one value or few enough entries to sort, and another pass draws.
+// The row is read from HBM once; the later passes, one to five, find it in L2. What bounds a
+// pass over all weights is their arithmetic (12 operations in float64 and some 30 others an
+// entry), not the bytes.
 
 #include <float.h>
 
@@ -59,7 +62,8 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 }
 
 struct Shared {
-    u64 bins[BINS];                     // counts or weights
+    u64 bins[BINS];                     // weights
+    unsigned counts[BINS];
     u64 list[CAP];
     double powers[16];                  // 2^(j / 16)
     u64 warp_sum[NW];                   // of the CTA's warps
@@ -67,8 +71,9 @@ struct Shared {
     float warp_max[NW], warp_pivot[NW], warp_lo[NW], warp_hi[NW];
     u64 before;                         // what lies before the bin in question
     u64 scan[NW];
-    float top, pivot, lo, hi;
+    float queue[NW][64];                // a warp's entries that wait for a whole warp of them
     int listed, bin, least, tau_key, ti;
+    unsigned entries;                   // of the range, down to the bin in question
 };
 
 template <int C>
@@ -87,6 +92,11 @@ __device__ __forceinline__ int rank_of() {
     else return 0;
 }
 
+// the next smaller float
+__device__ __forceinline__ float below(float v) {
+    const int b = __float_as_int(v);
+    return v == 0.f ? -1e-45f : __int_as_float(v > 0.f ? b - 1 : b + 1);
+}
 // max that hands a NaN on
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -139,6 +149,17 @@ struct Words {
         if constexpr (sizeof(E) == 4) return __uint_as_float(word(j));
         else return __uint_as_float(j & 1 ? word(j >> 1) & 0xffff0000u : word(j >> 1) << 16);
     }
+    // the largest, or a NaN if there is one
+    __device__ __forceinline__ float most() const {
+        if constexpr (sizeof(E) == 4) {
+            return max_nan(max_nan(at(0), at(1)), max_nan(at(2), at(3)));
+        } else {
+            auto two = [](uint32_t w) { return reinterpret_cast<const __nv_bfloat162 &>(w); };
+            const __nv_bfloat162 a = __hmax2_nan(two(q.x), two(q.y)), b = __hmax2_nan(two(q.z), two(q.w));
+            const __nv_bfloat162 m = __hmax2_nan(a, b);
+            return max_nan(__low2float(m), __high2float(m));
+        }
+    }
 };
 
 // The row as one CTA sees it. Places count from the 16-byte boundary at or before its start.
@@ -148,8 +169,8 @@ struct Row {
     const E *p;                         // that boundary
     int off, end;                       // first place, and the one behind the last
     int piece;                          // places of a warp's piece, whole steps
-    float top;
-    double rate;                        // 1 / T
+    float top, floor;                   // the largest; no weight is left here and below
+    double limit, rate;                 // the largest as a finite number; 1 / T
     int bits;                           // weights are whole numbers of 2^-bits
     const double *powers;
     float tau;
@@ -158,18 +179,17 @@ struct Row {
     __device__ __forceinline__ int from(int w) const { return (int)min((long long)w * piece, (long long)end); }
 
     // (v - top) / T
-    __device__ __forceinline__ double exponent(float v) const { return ((double)v - (double)top) * rate; }
+    __device__ __forceinline__ double exponent(float v) const { return ((double)fminf(v, FLT_MAX) - limit) * rate; }
     // 2^bits e^exponent, rounded. e^x = 2^(k / 16) e^r, |r| <= log(2) / 32, the first factor from a
     // table, the second to r^6: what is left out is r^7 / 5040 < 5e-16 (table-driven exponentials
-    // after Tang, 1989).
+    // after Tang, 1989). At `floor` and below, where x is -34 or less, it is 0.
     __device__ __forceinline__ u64 weight(float v) const {
-        if (isinf(top)) return v == top ? 1ull << bits : 0ull;
-        const double x = exponent(v);
-        if (!(x > -45.0)) return 0;                        // below 2^-64
         constexpr double ROUND = 6755399441055744.0;       // 1.5 * 2^52: the sum's last bit is worth 1
-        const double m = fma(x, 16.0 * 1.4426950408889634, ROUND);
+        constexpr double STEP16 = 0.69314718055994531 / 16.0;
+        const double x = ((double)fmaxf(fminf(v, FLT_MAX), floor) - limit) * rate;
+        const double m = fma(x, 1.0 / STEP16, ROUND);
         const int k = __double2loint(m);
-        const double r = fma(m - ROUND, -0.69314718055994531 / 16.0, x);
+        const double r = fma(m - ROUND, -STEP16, x);
         double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
         e = fma(e, r, 1.0 / 24.0);
         e = fma(e, r, 1.0 / 6.0);
@@ -178,7 +198,8 @@ struct Row {
         e = fma(e, r, 1.0);
         e *= powers[k & 15];
         e = __hiloint2double(__double2hiint(e) + (((k >> 4) + bits) << 20), __double2loint(e));
-        return (u64)__double_as_longlong(e + 4503599627370496.0) & ((1ull << 52) - 1);
+        const u64 w = (u64)__double_as_longlong(e + 4503599627370496.0) & ((1ull << 52) - 1);
+        return v > floor ? w : 0;
     }
     __device__ __forceinline__ bool kept(float v, int i) const { return v > tau || (v == tau && i <= ti); }
 
@@ -353,37 +374,64 @@ __device__ int nth_equal(Shared &sh, const Row<E, C> &row, float value, int n)
 }
 
 // Cuts what is kept to the shortest run of the ranking that reaches `target` entries
-// (MASS false) or the share `share` of the weight kept before. [a, b]: the range that the end
-// of the run lies in, smaller in every round; MOST bounds the rounds all the same.
+// (MASS false) or the share `share` of the weight kept before; then `target` is the weight
+// that it has to reach. [a, b]: the range that the end of the run lies in, smaller in every
+// round; MOST bounds the rounds all the same. Returns the entries that it put into the list, if
+// all that is kept is there, else 0.
 template <bool MASS, typename E, int C>
-__device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a)
+__device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
 {
     const int tid = threadIdx.x, rank = rank_of<C>();
-    float b = row.top;
+    float a = fmaxf(row.tau, fmaxf(row.floor, -FLT_MAX)), b = row.top;   // (at the floor and below nothing weighs anything)
     u64 above = 0;                                         // what lies above b
+    const bool all_in = row.tau == NEG_INF;
+    // an entry this light is not in the run: all that are make up less than half of 1 - share
+    const u64 light = MASS ? (u64)(0.5 * (1.0 - (double)share) / row.end * (double)(1ull << row.bits)) : 0;
     constexpr int MOST = 100;
     for (int round = 0; round < MOST; ++round) {
-        const double scale = BINS / ((double)b - (double)a);
-        auto bin_of = [&](float v) { return a == b ? 0 : min(BINS - 1, (int)(((double)b - (double)v) * scale)); };
-        for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+        // bins of equal width from b down; halves, so that no difference overflows
+        const float width = 0.5f * b - 0.5f * a, scale = BINS / width;
+        const bool fine = width >= 1e-34f;                 // (scale is finite)
+        const double scale2 = BINS / ((double)b - (double)a);
+        auto bin_of = [&](float v) {
+            const float f = fine ? (0.5f * b - 0.5f * v) * scale : (float)(((double)b - (double)v) * scale2);
+            return a == b ? 0 : min(BINS - 1, (int)f);
+        };
+        for (int i = tid; i < BINS; i += THREADS) {
+            sh.counts[i] = 0;
+            if (MASS) sh.bins[i] = 0;
+        }
         if (tid == 0) sh.listed = 0;
         __syncthreads();
-        u64 beside = 0;                                    // kept below the range, in the first round
+        u64 beside = 0;                                    // kept and not in a bin, in the first round
         row.each([&](float v, int i) {
-            if (v > b || !row.kept(v, i)) return;
-            const u64 w = MASS ? row.weight(v) : 1ull;
-            if (w == 0) return;
-            if (v >= a) atomicAdd(&sh.bins[bin_of(v)], w);
-            else if (round == 0) beside += w;
+            if (!(v >= a && v <= b) || !(all_in || row.kept(v, i))) return;
+            if constexpr (MASS) {
+                const u64 w = row.weight(v);
+                if (w <= light) {
+                    beside += w;
+                } else {
+                    const int k = bin_of(v);
+                    atomicAdd(&sh.bins[k], w);
+                    atomicAdd(&sh.counts[k], 1u);
+                }
+            } else {
+                atomicAdd(&sh.counts[bin_of(v)], 1u);
+            }
         });
         if (MASS && round == 0) row_sums<C>(sh, beside);
         else row_sync<C>();
         // each thread's bins of the whole row, then where the sum reaches the target
         u64 mine[PER], sum = 0, all;
+        unsigned counts[PER];
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
-            mine[q] = 0;
-            for (int r = 0; r < C; ++r) mine[q] += of_rank<C>(sh.bins, r)[tid * PER + q];
+            counts[q] = 0, mine[q] = 0;
+            for (int r = 0; r < C; ++r) {
+                counts[q] += of_rank<C>(sh.counts, r)[tid * PER + q];
+                if (MASS) mine[q] += of_rank<C>(sh.bins, r)[tid * PER + q];
+            }
+            if (!MASS) mine[q] = counts[q];
             sum += mine[q];
         }
         u64 upto = block_before(sh, sum, all);
@@ -392,22 +440,29 @@ __device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a
             for (int w = 0; w < C * NW; ++w) kept += sh.all_sum[w];
             target = share_of(share, kept);
         }
-        if (above + all < target) {                        // the whole range is kept, and more is not there
+        if (above + all < target) {                        // all of the range is kept, and more is not there
             row_sync<C>();
             break;
         }
+        u64 dummy;
+        unsigned entries = (unsigned)block_before(sh, (u64)counts[0] + counts[1] + counts[2] + counts[3], dummy);
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const u64 lo = above + upto;
             upto += mine[q];
-            if (lo < target && above + upto >= target) sh.bin = tid * PER + q, sh.before = lo;
+            entries += counts[q];
+            if (lo < target && above + upto >= target) sh.bin = tid * PER + q, sh.before = lo, sh.entries = entries;
         }
         row_sync<C>();                                     // bins read, the bin known
         const int bin = sh.bin;
         const u64 before = sh.before;
+        const bool whole = round == 0 && sh.entries <= CAP;          // all that is kept fits the list
         float lo = -NEG_INF, hi = NEG_INF;
         row.each([&](float v, int i) {
-            if (v > b || v < a || !row.kept(v, i) || bin_of(v) != bin) return;
+            if (!(v >= a && v <= b) || !(all_in || row.kept(v, i))) return;
+            const int k = bin_of(v);
+            if (whole ? k > bin : k != bin) return;
+            if (MASS && row.weight(v) <= light) return;    // (not in the bins either)
             lo = fminf(lo, v), hi = fmaxf(hi, v);
             const int at = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
             if (at < CAP) of_rank<C>(&sh, 0)->list[at] = ranked(v, i);
@@ -415,6 +470,10 @@ __device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a
         lo = row_fold<C>(sh.warp_lo, lo, [](float x, float y) { return fminf(x, y); });
         hi = row_fold<C>(sh.warp_hi, hi, [](float x, float y) { return fmaxf(x, y); });
         const int n = of_rank<C>(&sh, 0)->listed;
+        if (whole) {
+            row_sync<C>();
+            return min(n, CAP);
+        }
         if (lo == hi) {
             const u64 each = MASS ? row.weight(lo) : 1ull;
             const u64 need = (target - before + each - 1) / each;
@@ -425,7 +484,7 @@ __device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a
                 row_sync<C>();
             }
             row.tau = lo;
-            return;
+            return 0;
         }
         if (n <= CAP) {
             if (rank == 0) {
@@ -438,22 +497,19 @@ __device__ void cut(Shared &sh, Row<E, C> &row, u64 target, float share, float a
             row.tau = of_key((uint32_t)of_rank<C>(&sh, 0)->tau_key);
             row.ti = of_rank<C>(&sh, 0)->ti;
             row_sync<C>();
-            return;
+            return 0;
         }
         a = lo, b = hi, above = before;
         row_sync<C>();
     }
-    // MASS: entries below the range weigh nothing and may stay
-    if (!MASS) {
-        if (a != row.tau) row.ti = EVERY;
-        row.tau = a;
-    }
+    return 0;                                              // nothing to cut: what is below the range weighs nothing
 }
 
-// The rest of a row whose candidates are all in sh.list: n entries, of which the k first in rank count.
+// The rest of a row whose candidates are all in sh.list: n entries, of which the k first in rank count,
+// and of those the ones that reach `target`, or (0) the share top_p of their weight.
 template <typename E, int C>
 __device__ void finish_list(Shared &sh, const Row<E, C> &row, const SampleArgs &s, int at, int n, int k, float top_p,
-                            u64 least)
+                            u64 target, u64 least)
 {
     const int tid = threadIdx.x;
     sort_list(sh.list, n);
@@ -470,7 +526,7 @@ __device__ void finish_list(Shared &sh, const Row<E, C> &row, const SampleArgs &
         }
     }
     block_before(sh, sum, all);                            // (two barriers: sh.bins is written)
-    if (top_p < 1.f) n = reached(sh, n, share_of(top_p, all), [&](int i) { return sh.bins[i]; }) + 1;
+    if (top_p < 1.f) n = reached(sh, n, target ? target : share_of(top_p, all), [&](int i) { return sh.bins[i]; }) + 1;
     __syncthreads();
     // by index: (index, key), the ones too light last
 #pragma unroll
@@ -499,13 +555,12 @@ __device__ void finish_list(Shared &sh, const Row<E, C> &row, const SampleArgs &
         const u64 e = sh.list[i];
         s.token[at] = (int64_t)(e >> 32);
         if (s.logprob)
-            s.logprob[at] = isinf(row.top) ? (float)-log(ldexp((double)all, -row.bits))
-                                           : (float)(row.exponent(of_key((uint32_t)e)) - log(ldexp((double)all, -row.bits)));
+            s.logprob[at] = (float)(row.exponent(of_key((uint32_t)e)) - log(ldexp((double)all, -row.bits)));
     }
 }
 
 template <typename E, int C>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, C > 2 ? 1 : 2)
 sample_kernel(const __grid_constant__ SampleArgs s)
 {
     __shared__ Shared sh;
@@ -527,10 +582,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
 
     // the largest value (NaN if there is one)
     float most = NEG_INF;
-    row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) most = max_nan(most, v.at(j));
-    });
+    row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) { most = max_nan(most, v.most()); });
     const float t = s.temperature ? s.temperature[at] : s.temperature1;
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
@@ -549,6 +601,9 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     }
     row.top = row_fold<C>(sh.warp_max, most, [](float x, float y) { return max_nan(x, y); });
     row.rate = 1.0 / (double)t;
+    row.limit = (double)fminf(row.top, FLT_MAX);
+    row.floor = isinf(row.top) ? below(FLT_MAX)
+                               : fminf(below(row.top), __double2float_rd(row.limit - 34.0 * (double)t));
     // nothing to draw from, or nothing to draw
     const bool none = !(row.top > NEG_INF) || t != t || top_p != top_p;
     if (none || t <= 0.f || k == 1 || top_p <= 0.f) {
@@ -580,27 +635,56 @@ sample_kernel(const __grid_constant__ SampleArgs s)
         const int n = of_rank<C>(&sh, 0)->listed;
         row_sync<C>();
         if (n <= CAP) {
-            if (rank == 0) finish_list(sh, row, s, at, n, (int)k, top_p, least);
+            if (rank == 0) finish_list(sh, row, s, at, n, (int)k, top_p, 0, least);
             return;
         }
     }
     if (isinf(row.top)) row.tau = row.top;                 // nothing beside it has weight
-    if (k > 0 && k < s.vocab) {
-        float lo = -NEG_INF;
-        row.each([&](float v, int) { lo = fminf(lo, v); });
-        lo = row_fold<C>(sh.warp_lo, lo, [](float x, float y) { return fminf(x, y); });
-        row_sync<C>();
-        cut<false>(sh, row, (u64)k, 0.f, fmaxf(lo, row.tau));
+    u64 target = (u64)k;
+    int in_list = k > 0 && k < s.vocab ? cut<false>(sh, row, target, 0.f) : 0;
+    const bool few = in_list > 0;
+    if (!few && top_p < 1.f) in_list = cut<true>(sh, row, target, top_p);
+    if (in_list > 0) {
+        if (rank == 0) finish_list(sh, row, s, at, in_list, few ? (int)k : in_list, top_p, few ? 0 : target, least);
+        return;
     }
-    // below top - 33 T no weight is left
-    if (top_p < 1.f) cut<true>(sh, row, 0, top_p, fmaxf(row.tau, fmaxf(-FLT_MAX, (float)((double)row.top - 33.0 * (double)t))));
     auto weight = [&](float v, int i) -> u64 {
         if (!row.kept(v, i)) return 0;
         const u64 x = row.weight(v);
         return x >= least ? x : 0;
     };
     u64 mass = 0;
-    row.each([&](float v, int i) { mass += weight(v, i); });
+    if (row.tau == NEG_INF) {
+        row.each([&](float v, int i) { mass += weight(v, i); });
+    } else {
+        // few of the entries are kept: their weights are computed 32 at a time
+        float *queue = sh.queue[warp];
+        int waiting = 0;
+        auto heavy = [&](float v) {
+            const u64 x = row.weight(v);
+            return x >= least ? x : 0;
+        };
+        row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int place) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float x = v.at(i);
+                const bool in = row.kept(x, place + i - row.off);
+                const unsigned who = __ballot_sync(0xffffffffu, in);
+                if (in) queue[waiting + __popc(who & ((1u << lane) - 1))] = x;
+                waiting += __popc(who);
+                if (waiting >= 32) {
+                    __syncwarp();
+                    mass += heavy(queue[lane]);
+                    const float rest = queue[32 + lane];
+                    __syncwarp();
+                    queue[lane] = rest;
+                    waiting -= 32;
+                }
+            }
+        });
+        __syncwarp();
+        if (lane < waiting) mass += heavy(queue[lane]);
+    }
     row_sums<C>(sh, mass);
     u64 all = 0;
     for (int i = 0; i < C * NW; ++i) all += sh.all_sum[i];
@@ -640,7 +724,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
                             done = true;
                             s.token[at] = x + lane * VEC + i - row.off;
                             if (s.logprob)
-                                s.logprob[at] = (float)((isinf(row.top) ? 0.0 : row.exponent(v.at(i))) - log(ldexp((double)all, -row.bits)));
+                                s.logprob[at] = (float)(row.exponent(v.at(i)) - log(ldexp((double)all, -row.bits)));
                         }
                     }
                 }
@@ -666,15 +750,15 @@ cudaError_t sample_of(const SampleArgs &a, cudaStream_t stream)
     return cudaLaunchKernelEx(&c, sample_kernel<E, C>, a);
 }
 
-// CTAs a row: as many (up to 8, a portable cluster) as still fit the GPU at 2 an SM, none of
-// fewer than 2048 entries.
+// CTAs a row: as many (up to 8, a portable cluster) as the GPU holds, 2 an SM or, of larger
+// clusters, whose joins need more registers, one; none of fewer than 2048 entries.
 template <typename E>
 cudaError_t sample_by_rows(const SampleArgs &a, cudaStream_t stream)
 {
-    const long long most = std::min<long long>(2LL * N_SM / a.rows, a.vocab / 2048);
+    const long long most = std::min<long long>(N_SM / a.rows, a.vocab / 2048);
     if (most >= 8) return sample_of<E, 8>(a, stream);
     if (most >= 4) return sample_of<E, 4>(a, stream);
-    if (most >= 2) return sample_of<E, 2>(a, stream);
+    if (2LL * N_SM / a.rows >= 2 && a.vocab >= 4096) return sample_of<E, 2>(a, stream);
     return sample_of<E, 1>(a, stream);
 }
 

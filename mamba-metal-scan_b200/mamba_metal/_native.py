@@ -380,7 +380,7 @@ def linear_kd_bwd(x, w, index, temperature: float, reduction: str, dloss, kept,
 
 
 def _opt(t) -> int:
-    return 0 if t is None else _ptr(t)
+    return 0 if t is None else t.data_ptr()
 
 
 def norm_fwd(x, y, gate, weight, post, scale, eps: float, keep: bool = True):
@@ -455,18 +455,19 @@ def conv_bwd(x, w, bias, dy, silu: bool):
 
 def _wide(starts, slots, out_slots) -> int:
     """Which of the lists hold 64-bit numbers (MMS_WIDE_*)."""
-    return sum(bit for bit, t in ((1, starts), (2, slots), (4, out_slots))
-               if t is not None and t.dtype == torch.int64)
+    wide = torch.int64
+    return ((starts is not None and starts.dtype == wide) + 2 * (slots is not None and slots.dtype == wide)
+            + 4 * (out_slots is not None and out_slots.dtype == wide))
 
 
 def conv_packed(rows, w, bias, window, starts, slots, out_slots, count: int, silu: bool):
     """y of mms_conv_packed, window updated; rows = (x (L, D), its row stride)."""
     x, ldx = rows
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    n_rows, d = x.shape
+    y = torch.empty((n_rows, d), device=x.device, dtype=x.dtype)
     rc = load().mms_conv_packed(x.data_ptr(), ldx, w.data_ptr(), _opt(bias), window.data_ptr(), window.shape[0],
                                 _opt(starts), _opt(slots), _opt(out_slots), _wide(starts, slots, out_slots),
-                                y.data_ptr(), x.shape[0], count, x.shape[1], w.shape[1], silu, _dtype(x),
-                                _stream(x.device))
+                                y.data_ptr(), n_rows, count, d, w.shape[1], silu, _dtype(x), _stream(x.device))
     if rc:
         _check(rc, "mms_conv_packed")
     return y
@@ -480,18 +481,19 @@ def _scan_packed_workspace(rows: int, count: int, d: int, n: int) -> int:
 def scan_packed(x, dt, aneg, b_in, c_in, z, d_skip, dt_range, state, starts, slots, out_slots, count: int):
     """y of mms_scan_packed, state updated; x, dt, b_in, c_in, z as (tensor, row stride)."""
     (x, ldx), (dt, lddt), (b_in, ldb), (c_in, ldc) = x, dt, b_in, c_in
-    z, ldz = (None, 0) if z is None else z
+    z, ldz = (0, 0) if z is None else (z[0].data_ptr(), z[1])
     n_rows, d = x.shape
     n = aneg.shape[1]
-    y = torch.empty((n_rows, d), device=x.device, dtype=x.dtype)
+    device = x.device
+    y = torch.empty((n_rows, d), device=device, dtype=x.dtype)
     nb = 0 if starts is None else _scan_packed_workspace(n_rows, count, d, n)
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
     lo, hi = (0.0, 0.0) if dt_range is None else dt_range
     rc = load().mms_scan_packed(x.data_ptr(), ldx, dt.data_ptr(), lddt, aneg.data_ptr(), b_in.data_ptr(), ldb,
-                                c_in.data_ptr(), ldc, _opt(z), ldz, _opt(d_skip), dt_range is not None, lo, hi,
+                                c_in.data_ptr(), ldc, z, ldz, _opt(d_skip), dt_range is not None, lo, hi,
                                 state.data_ptr(), state.shape[0], _opt(starts), _opt(slots), _opt(out_slots),
                                 _wide(starts, slots, out_slots), y.data_ptr(), _opt(ws), nb, n_rows, count, d, n,
-                                _dtype(x), _dtype(b_in), _stream(x.device))
+                                _dtype(x), _dtype(b_in), _stream(device))
     if rc:
         _check(rc, "mms_scan_packed")
     return y

@@ -18,7 +18,8 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from mamba_metal import _native
-from mamba_metal.packed import (_FLOATS, _nothing_packed, check_lists, dispatch, int_list, places_of, rows_of)
+from mamba_metal.packed import (_FLOATS, _nothing_packed, check_lists, dispatch, int_list, places_of, rows_of,
+                                same_device)
 
 MAX_TAPS = 8          # the kernels' (MMS_CONV_MAX_K)
 
@@ -66,18 +67,18 @@ class CausalConvCUDA(torch.autograd.Function):
             return (*_native.conv_bwd(x, weight, bias, dy.contiguous(), ctx.silu), None)
 
 
-def _check_kernel(what, x, weight, bias, more=()):
-    tensors = [t for t in (x, weight, bias, *more) if t is not None]
-    if any(t.device != x.device for t in tensors):
-        raise RuntimeError(f"{what} needs every tensor on the same CUDA device; saw "
-                           + ", ".join(str(t.device) for t in tensors))
-    if x.dtype not in _FLOATS or any(t.dtype != x.dtype for t in tensors):
+def _check_kernel(what, x, weight, bias, window=None):
+    same_device(what, x, (weight, bias, window))
+    dtype = x.dtype
+    if dtype not in _FLOATS or weight.dtype != dtype or (bias is not None and bias.dtype != dtype) \
+            or (window is not None and window.dtype != dtype):
         raise RuntimeError(f"{what} takes float32 or bfloat16, all tensors alike; got "
-                           + ", ".join(str(t.dtype) for t in tensors))
+                           + ", ".join(str(t.dtype) for t in (x, weight, bias, window) if t is not None))
     if weight.shape[1] > MAX_TAPS:
         raise ValueError(f"{what} takes up to {MAX_TAPS} taps on CUDA; got {weight.shape[1]} "
                          "(impl='torch' takes any number)")
-    if x.numel() > _native.SERVE_MAX * max(1, x.shape[-1]) or x.shape[-1] > _native.SERVE_MAX_DIM:
+    d = x.shape[-1]
+    if x.numel() > _native.SERVE_MAX * max(1, d) or d > _native.SERVE_MAX_DIM:
         raise ValueError(f"{what} takes up to {_native.SERVE_MAX} rows and {_native.SERVE_MAX_DIM} channels; "
                          f"got {tuple(x.shape)}")
 
@@ -147,10 +148,10 @@ def causal_conv_packed(x: torch.Tensor, weight: torch.Tensor, bias, window: torc
         raise ValueError(f"bias must be ({x.shape[1]},); got {tuple(bias.shape)}")
     if window.dim() != 3 or window.shape[1:] != (x.shape[1], k - 1):
         raise ValueError(f"window must be (places, {x.shape[1]}, {k - 1}); got {tuple(window.shape)}")
-    count = check_lists(x.shape[0], window.shape[0], starts, slots, out_slots, x.device)
+    count = check_lists(x.shape[0], window.shape[0], starts, slots, out_slots, x)
     if not dispatch(impl, x):
         return causal_conv_packed_ref(x, weight, bias, window, starts, slots, out_slots, silu)
-    _check_kernel("causal_conv_packed", x, weight, bias, (window,))
+    _check_kernel("causal_conv_packed", x, weight, bias, window)
     if not window.is_contiguous():
         raise ValueError(f"window must be contiguous (it is updated in place); got strides {window.stride()}")
     if window.shape[0] > _native.SERVE_MAX or count > _native.SERVE_MAX:

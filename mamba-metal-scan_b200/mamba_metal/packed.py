@@ -34,6 +34,8 @@ _FLOATS = (torch.float32, torch.bfloat16)
 
 def dispatch(impl: str, x) -> bool:
     """Whether the kernels run."""
+    if impl == "auto":
+        return x.is_cuda
     if impl not in _IMPLS:
         raise ValueError(f"unknown scan_impl {impl!r}; want 'auto', 'cuda', 'metal' or 'torch'")
     if impl in ("cuda", "metal") and not x.is_cuda:
@@ -41,7 +43,7 @@ def dispatch(impl: str, x) -> bool:
     return impl != "torch" and x.is_cuda
 
 
-def check_lists(rows: int, places: int, starts, slots, out_slots, device) -> int:
+def check_lists(rows: int, places: int, starts, slots, out_slots, x) -> int:
     """The number of sequences, from the lists' shapes; the host does not look inside."""
     if starts is not None:
         if starts.dim() != 1 or starts.shape[0] < 1:
@@ -49,17 +51,28 @@ def check_lists(rows: int, places: int, starts, slots, out_slots, device) -> int
         count = starts.shape[0] - 1
     else:
         count = rows
-    for name, t in (("slots", slots), ("out_slots", out_slots)):
-        if t is not None and t.shape != (count,):
-            raise ValueError(f"{name} must be ({count},), one place a sequence; got {tuple(t.shape)}")
     if slots is None and places < count:
         raise ValueError(f"without slots the cache needs a place for each of {count} sequences; it has {places}")
     for name, t in (("starts", starts), ("slots", slots), ("out_slots", out_slots)):
-        if t is not None and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool):
-            raise RuntimeError(f"{name} must hold integers; got {t.dtype}")
-        if t is not None and t.device != device:
-            raise RuntimeError(f"{name} must be on {device}; got {t.device}")
+        if t is None:
+            continue
+        if name != "starts" and t.shape != (count,):
+            raise ValueError(f"{name} must be ({count},), one place a sequence; got {tuple(t.shape)}")
+        dtype = t.dtype
+        if dtype != torch.int64 and dtype != torch.int32 and (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool):
+            raise RuntimeError(f"{name} must hold integers; got {dtype}")
+        if t.get_device() != x.get_device():
+            raise RuntimeError(f"{name} must be on {x.device}; got {t.device}")
     return count
+
+
+def same_device(what, x, tensors):
+    """RuntimeError unless every tensor (None: no tensor) is on x's device."""
+    index = x.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"{what} needs every tensor on the same CUDA device; saw "
+                               + ", ".join(str(t.device) for t in (x, *tensors) if t is not None))
 
 
 def int_list(t):
@@ -74,11 +87,11 @@ def int_list(t):
 def rows_of(t, group: int = 1):
     """(tensor, row stride) of a 2-D t with unit column stride: t itself where it has one; with
     `group`, also bases and strides of whole groups of so many elements."""
-    d = t.shape[1]
-    ld = t.stride(0)
-    if t.shape[0] == 1:
+    ld, step = t.stride()
+    rows, d = t.shape
+    if rows == 1:
         ld = d
-    if (t.stride(1) != 1 and d > 1) or (group > 1 and (ld % group or t.data_ptr() % (group * t.element_size()))):
+    if (step != 1 and d > 1) or (group > 1 and (ld % group or t.data_ptr() % (group * t.element_size()))):
         t, ld = t.clone(memory_format=torch.contiguous_format), d
     return t, ld
 
@@ -143,49 +156,52 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     (`selective_scan` trains). On CUDA tensors 'auto', 'cuda', 'metal' run the kernels
     (csrc/mms_packed.cu); elsewhere, or with 'torch', PyTorch ops.
     """
-    if x.dim() != 2 or dt.shape != x.shape or aneg.dim() != 2 or aneg.shape[0] != x.shape[1]:
-        raise ValueError(f"bad shapes: x {tuple(x.shape)}, dt {tuple(dt.shape)}, Aneg {tuple(aneg.shape)}")
-    rows, d = x.shape
+    shape = x.shape
+    if len(shape) != 2 or dt.shape != shape or aneg.dim() != 2 or aneg.shape[0] != shape[1]:
+        raise ValueError(f"bad shapes: x {tuple(shape)}, dt {tuple(dt.shape)}, Aneg {tuple(aneg.shape)}")
+    rows, d = shape
     n = aneg.shape[1]
     if b_in.shape != (rows, n) or c_in.shape != (rows, n):
         raise ValueError(f"B {tuple(b_in.shape)} / C {tuple(c_in.shape)} must be ({rows}, {n})")
     if state.dim() != 3 or state.shape[1:] != (d, n):
         raise ValueError(f"state must be (places, {d}, {n}); got {tuple(state.shape)}")
-    if (z is not None and z.shape != x.shape) or (d_skip is not None and d_skip.shape != (d,)):
-        raise ValueError(f"z must be {tuple(x.shape)} and d_skip ({d},)")
+    if (z is not None and z.shape != shape) or (d_skip is not None and d_skip.shape != (d,)):
+        raise ValueError(f"z must be {tuple(shape)} and d_skip ({d},)")
     if dt_range is not None and not float(dt_range[1]) > float(dt_range[0]):
         raise ValueError(f"need dt_min < dt_max; got {dt_range}")
-    count = check_lists(rows, state.shape[0], starts, slots, out_slots, x.device)
+    places = state.shape[0]
+    count = check_lists(rows, places, starts, slots, out_slots, x)
     if not dispatch(impl, x):
         return selective_scan_packed_ref(x, dt, aneg, b_in, c_in, state, starts, slots, out_slots, z, d_skip, dt_range)
-    dtype, device = x.dtype, x.device
-    if any(t is not None and t.device != device for t in (dt, aneg, b_in, c_in, state, z, d_skip)):
-        raise RuntimeError(f"selective_scan_packed needs every tensor on {device}")
+    same_device("selective_scan_packed", x, (dt, aneg, b_in, c_in, state, z, d_skip))
+    dtype, f32 = x.dtype, torch.float32
     if dtype not in _FLOATS or dt.dtype != dtype or (z is not None and z.dtype != dtype):
         raise RuntimeError(f"selective_scan_packed takes float32 or bfloat16 x, dt and z alike; got {dtype}, {dt.dtype}"
                            + ("" if z is None else f", {z.dtype}"))
-    if not all(t.is_floating_point() for t in (aneg, b_in, c_in)):
-        raise RuntimeError("Aneg, B and C must be floating point")
+    if b_in.dtype != c_in.dtype or (b_in.dtype != dtype and b_in.dtype != f32):
+        if not (b_in.is_floating_point() and c_in.is_floating_point()):
+            raise RuntimeError(f"B and C must be floating point; got {b_in.dtype}, {c_in.dtype}")
+        b_in, c_in = b_in.float(), c_in.float()
+    if aneg.dtype != f32 or (d_skip is not None and d_skip.dtype != f32):
+        if not aneg.is_floating_point() or (d_skip is not None and not d_skip.is_floating_point()):
+            raise RuntimeError("Aneg and d_skip must be floating point")
+        aneg, d_skip = aneg.float(), None if d_skip is None else d_skip.float()
     if n % 4 != 0 or n <= 0 or n > 64:
         raise ValueError(f"d_state must be a positive multiple of 4 no larger than 64 for the CUDA scan; got {n} "
                          "(scan_impl='torch' takes any size)")
-    if state.dtype != torch.float32 or not state.is_contiguous() or state.data_ptr() % 16:
+    if state.dtype != f32 or not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be float32, contiguous and 16-byte aligned (it is updated in place); got "
                          f"{state.dtype}, strides {state.stride()}")
-    if rows > _native.SERVE_MAX or state.shape[0] > _native.SERVE_MAX or count > _native.SERVE_MAX \
-            or d > _native.SERVE_MAX_DIM:
-        raise ValueError(f"selective_scan_packed takes up to {_native.SERVE_MAX} rows, sequences and places and "
+    most = _native.SERVE_MAX
+    if rows > most or places > most or count > most or d > _native.SERVE_MAX_DIM:
+        raise ValueError(f"selective_scan_packed takes up to {most} rows, sequences and places and "
                          f"{_native.SERVE_MAX_DIM} channels")
-    if d == 0 or count == 0 or state.shape[0] == 0 or rows == 0:
+    if d == 0 or count == 0 or places == 0 or rows == 0:
         return _nothing_packed(x, state, count, slots, out_slots)
-    with _native.on_device(device):
+    with _native.on_device(x.device):
         group = 4 if starts is None else 1
-        if b_in.dtype != c_in.dtype or b_in.dtype not in (dtype, torch.float32):
-            b_in, c_in = b_in.float(), c_in.float()
-        aneg = aneg if aneg.dtype == torch.float32 else aneg.float()
-        if d_skip is not None:
-            d_skip = d_skip if d_skip.dtype == torch.float32 else d_skip.float()
-            d_skip = d_skip if d_skip.is_contiguous() else d_skip.contiguous()
+        if d_skip is not None and not d_skip.is_contiguous():
+            d_skip = d_skip.contiguous()
         return _native.scan_packed(rows_of(x), rows_of(dt), _aligned(aneg, 16), rows_of(b_in, group),
                                    rows_of(c_in, group), None if z is None else rows_of(z), d_skip, dt_range,
                                    state, int_list(starts), int_list(slots), int_list(out_slots), count)
