@@ -400,7 +400,7 @@ int mms_scan_packed(const void *x, long long ldx, const void *dt, long long lddt
  * numbers if top_k_wide. temperature <= 0: the largest logit. A row with a
  * NaN, or without a logit above -inf, gives -1. logprob (NULL: not wanted): the log of
  * w_token over their sum, NaN beside -1. Weights are float64 rounded to whole numbers of
- * 2^-45 of the largest (2^-(61 - log2 vocab) above 2^17 entries), their sums exact.
+ * 2^-44 of the largest (2^-(62 - log2 vocab) above 2^18 entries), their sums exact.
  * uniform is taken into [0, 1 - 2^-24].
  * No counterpart in the reference.
  */

@@ -12,7 +12,7 @@
 //
 // A sum next to a border decides a token, and sums of 131072 weights in float32 are
 // off by more than the distance between neighbours. Weights are computed in float64
-// and held as whole numbers of 2^-45 of the largest (fewer bits above 2^17 entries, so that
+// and held as whole numbers of 2^-44 of the largest (fewer bits above 2^18 entries, so that
 // no sum passes 2^62): their sums are exact in any order, so bins may be filled by atomics
 // and a call's result is the same every time.
 //
@@ -50,6 +50,8 @@ constexpr int CAP = 2048;               // entries that are sorted rather than d
 constexpr int PER = BINS / THREADS;     // bins, and list entries, of a thread
 static_assert(CAP == BINS, "one scan serves both");
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr int BITS = 44;                // of weights, fewer above 2^18 entries
+constexpr int LIMBS_MAX = 1 << 17;      // entries whose weights' 15-bit parts add up in 32 bits
 constexpr int EVERY = 0x7fffffff;       // ti: all entries equal to tau
 
 // Larger keys for larger floats; -0 and 0 are one value.
@@ -62,9 +64,15 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 }
 
 struct Shared {
-    u64 bins[BINS];                     // weights
+    union {
+        unsigned limbs[2][BINS];        // weights of bins, 15 bits of each weight in one sum, ..
+        u64 bins[BINS];                 // .. or whole
+    };
     unsigned counts[BINS];
-    u64 list[CAP];
+    union {
+        unsigned limb2[BINS];           // the uppermost 15 bits
+        u64 list[CAP];
+    };
     double powers[16];                  // 2^(j / 16)
     u64 warp_sum[NW];                   // of the CTA's warps
     u64 all_sum[8 * NW];                // of all the row's warps
@@ -201,6 +209,30 @@ struct Row {
         const u64 w = (u64)__double_as_longlong(e + 4503599627370496.0) & ((1ull << 52) - 1);
         return v > floor ? w : 0;
     }
+    // w to a bin. Shared memory adds 32 bits at a time: three sums of 15 bits of each weight hold it (of
+    // rows above LIMBS_MAX, 64 bits in a loop), and most weights have the lowest 15 alone.
+    __device__ __forceinline__ void add(Shared &sh, int bin, u64 w) const {
+        atomicAdd(&sh.counts[bin], 1u);
+        if (end - off > LIMBS_MAX) {
+            atomicAdd(&sh.bins[bin], w);
+        } else {
+            atomicAdd(&sh.limbs[0][bin], (unsigned)w & 0x7fffu);
+            const unsigned up = (unsigned)(w >> 15);
+            if (up) {
+                atomicAdd(&sh.limbs[1][bin], up & 0x7fffu);
+                if (up >> 15) atomicAdd(&sh.limb2[bin], up >> 15);
+            }
+        }
+    }
+    template <int C1>
+    __device__ __forceinline__ u64 sum_of(Shared &sh, int bin) const {
+        u64 s = 0;
+        for (int r = 0; r < C1; ++r) {
+            Shared *o = of_rank<C1>(&sh, r);
+            s += end - off > LIMBS_MAX ? o->bins[bin] : o->limbs[0][bin] + ((u64)o->limbs[1][bin] << 15) + ((u64)o->limb2[bin] << 30);
+        }
+        return s;
+    }
     __device__ __forceinline__ bool kept(float v, int i) const { return v > tau || (v == tau && i <= ti); }
 
     // 16 bytes at a place; entries outside the row are -inf
@@ -229,25 +261,35 @@ struct Row {
         return v;
     }
     // f(words, place of the first) over the warp's share [a, b) of the row, a multiple of STEP;
-    // several loads at a time. Entries of a step are all within [a, b) or outside the row.
-    template <typename F>
+    // UN loads at a time (one where f is long: its code is there UN + 1 times, and a pass whose code
+    // does not fit the instruction caches waits for it). Entries of a step are all within [a, b) or
+    // outside the row.
+    template <int UN, typename F>
     __device__ __forceinline__ void words(int a, int b, F f) const {
         const int lane = threadIdx.x & 31;
-        constexpr int UN = 4;
         int at = a;
-        for (; at + (UN - 1) * STEP < b; at += UN * STEP) {
-            Words<E> v[UN];
+        if constexpr (UN > 1) {
+            for (; at + (UN - 1) * STEP < b; at += UN * STEP) {
+                Words<E> v[UN];
 #pragma unroll
-            for (int q = 0; q < UN; ++q) v[q] = read(at + q * STEP + lane * VEC);
+                for (int q = 0; q < UN; ++q) v[q] = read(at + q * STEP + lane * VEC);
 #pragma unroll
-            for (int q = 0; q < UN; ++q) f(v[q], at + q * STEP + lane * VEC);
+                for (int q = 0; q < UN; ++q) f(v[q], at + q * STEP + lane * VEC);
+            }
         }
-        for (; at < b; at += STEP) f(read(at + lane * VEC), at + lane * VEC);
+        if (at >= b) return;
+        Words<E> next = read(at + lane * VEC);
+#pragma unroll 1
+        for (; at < b; at += STEP) {
+            const Words<E> v = next;
+            if (at + STEP < b) next = read(at + STEP + lane * VEC);
+            f(v, at + lane * VEC);
+        }
     }
     // f(value, index) for entries above -inf
     template <typename F>
     __device__ __forceinline__ void each(int a, int b, F f) const {
-        words(a, b, [&](const Words<E> &v, int at) {
+        words<1>(a, b, [&](const Words<E> &v, int at) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const float x = v.at(j);
@@ -399,7 +441,7 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
         };
         for (int i = tid; i < BINS; i += THREADS) {
             sh.counts[i] = 0;
-            if (MASS) sh.bins[i] = 0;
+            if (MASS) sh.bins[i] = 0, sh.limb2[i] = 0;
         }
         if (tid == 0) sh.listed = 0;
         __syncthreads();
@@ -412,8 +454,7 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
                     beside += w;
                 } else {
                     const int k = bin_of(v);
-                    atomicAdd(&sh.bins[k], w);
-                    atomicAdd(&sh.counts[k], 1u);
+                    row.add(sh, k, w);
                 }
             } else {
                 atomicAdd(&sh.counts[bin_of(v)], 1u);
@@ -427,11 +468,8 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             counts[q] = 0, mine[q] = 0;
-            for (int r = 0; r < C; ++r) {
-                counts[q] += of_rank<C>(sh.counts, r)[tid * PER + q];
-                if (MASS) mine[q] += of_rank<C>(sh.bins, r)[tid * PER + q];
-            }
-            if (!MASS) mine[q] = counts[q];
+            for (int r = 0; r < C; ++r) counts[q] += of_rank<C>(sh.counts, r)[tid * PER + q];
+            mine[q] = MASS ? row.template sum_of<C>(sh, tid * PER + q) : counts[q];
             sum += mine[q];
         }
         u64 upto = block_before(sh, sum, all);
@@ -574,7 +612,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     row.end = s.vocab + row.off;
     row.piece = ((row.end + C * NW - 1) / (C * NW) + STEP - 1) / STEP * STEP;
     row.powers = sh.powers;
-    row.bits = min(45, 62 - (32 - __clz(s.vocab)));
+    row.bits = min(BITS, 62 - (32 - __clz(s.vocab - 1)));
     row.tau = NEG_INF, row.ti = EVERY;
     const int w = rank * NW + warp;
     if (tid < 16) sh.powers[tid] = exp2(tid / 16.0);
@@ -582,7 +620,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
 
     // the largest value (NaN if there is one)
     float most = NEG_INF;
-    row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) { most = max_nan(most, v.most()); });
+    row.template words<4>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) { most = max_nan(most, v.most()); });
     const float t = s.temperature ? s.temperature[at] : s.temperature1;
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
@@ -664,7 +702,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
             const u64 x = row.weight(v);
             return x >= least ? x : 0;
         };
-        row.words(row.from(w), row.from(w + 1), [&](const Words<E> &v, int place) {
+        row.template words<1>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int place) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float x = v.at(i);

@@ -85,7 +85,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     row without any above it, or with a NaN, gives -1. With return_logprob also the log of the
     token's share of the kept weights (float32, NaN beside -1). logits float32 or bfloat16 on
     the CUDA kernel, rows may be strided. Weights are float64, in the kernel rounded to whole
-    numbers of 2^-45 of the largest (2^-(61 - log2 V) above 2^17 entries) and summed exactly.
+    numbers of 2^-44 of the largest (2^-(62 - log2 V) above 2^18 entries) and summed exactly.
     Not differentiable.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1 or uniform.shape != logits.shape[:-1]:

@@ -1,10 +1,10 @@
 """The sampling kernel against sample_tokens_ref: the same tokens, log-probabilities to float32.
 
-The kernel's weights are float64 rounded to whole numbers of 2^-45 of the largest, at most 2^-46
-off, and their sums are exact; a draw or a cut would have to lie within the sums' error (V 2^-46 at
-most, 2^-46 sqrt(V) as a rule) of a border to differ. The log-probability is the logarithm of a
+The kernel's weights are float64 rounded to whole numbers of 2^-44 of the largest, at most 2^-45
+off, and their sums are exact; a draw or a cut would have to lie within the sums' error (V 2^-45 at
+most, 2^-45 sqrt(V) as a rule) of a border to differ. The log-probability is the logarithm of a
 float64 quotient rounded once, and the reference's too: two roundings of its value and the kept
-weights' error, V 2^-46 of a sum of at least 1, apart at most.
+weights' error, V 2^-45 of a sum of at least 1, apart at most.
 """
 from __future__ import annotations
 
@@ -27,7 +27,7 @@ def check(z, u, t=1.0, k=0, p=1.0, m=0.0):
     lp = lp.cpu()
     assert torch.equal(lp.isnan(), wlp.isnan())
     good = ~wlp.isnan()
-    assert ((lp - wlp).abs()[good] <= 2 * 2.0 ** -24 * wlp[good].abs() + z.shape[-1] * 2.0 ** -46).all()
+    assert ((lp - wlp).abs()[good] <= 2 * 2.0 ** -24 * wlp[good].abs() + z.shape[-1] * 2.0 ** -45).all()
     assert torch.equal(sample_tokens(on(z), on(u), on(t), on(k), on(p), on(m)).cpu(), want)
     return token
 
@@ -38,6 +38,7 @@ def logits(rows, vocab, dtype, seed, spread=2.0):
     return z.to(dtype), torch.rand(rows, generator=g), g
 
 
+WIDE = [(1, 300000), (2, 131072), (3, 131073)]
 SIZES = [(1, 1), (3, 2), (2, 31), (5, 33), (1, 511), (4, 4097), (1, 32768), (40, 5003), (80, 20001), (150, 9001), (300, 1000), (2, 131072)]
 
 
@@ -49,6 +50,16 @@ def test_each_cut_matches(rows, vocab, dtype):
                dict(k=vocab + 5), dict(p=0.5), dict(p=0.9), dict(p=0.999), dict(p=0.0), dict(p=1e-9), dict(m=0.05), dict(m=1.0),
                dict(k=50, p=0.9, m=0.01, t=1.3), dict(p=0.95, t=5.0), dict(t=100.0, p=0.7), dict(t=0.05, p=0.99)):
         check(z, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", WIDE)
+def test_flat_and_wide_rows_do_not_overflow(rows, vocab, dtype):
+    """All weights the largest there is, at and above the sizes where sums need more bits."""
+    flat, u, g = logits(rows, vocab, dtype, vocab)
+    for z in (torch.zeros_like(flat), flat, torch.where(flat > 4, 0.0, -3.0).to(dtype)):
+        for kw in (dict(), dict(p=0.5), dict(p=0.999), dict(k=vocab // 2, p=0.7), dict(k=70000)):
+            check(z, u, **kw)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
