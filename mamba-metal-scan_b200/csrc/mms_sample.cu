@@ -25,6 +25,10 @@
 //     range of the logits, counts and weights of 2048 equal bins. If the entries down to the bin in
 //     question fit the list, all else happens there; otherwise that bin becomes the range,
 //     until it holds one value or few enough entries to sort, and another pass draws.
+//   bf16, where k is not small: a row has few different values, so one pass counts each of 5633 of them
+//     (magnitudes 2^-16 to 64 and 0; the others are listed one by one), and every cut and sum
+//     follows from the counts; one more pass, with the weights from a table, draws. Only where a cut
+//     falls among the values that are not counted, or too many are not, the bins above find it.
 // The row is read from HBM once; the later passes, one to five, find it in L2. What bounds a
 // pass over all weights is their arithmetic (12 operations in float64 and some 30 others an
 // entry), not the bytes.
@@ -63,15 +67,48 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// The values of bf16 rows that are counted, in descending order: 2^6 (1 - 2^-8) .. 2^-16, 0, -2^-16 ..
+// Between and around them lie the others, in four gaps: above, between the counted ones and 0 on
+// either side, below.
+constexpr int CORE_LOW = 0x3780, CORE = 0x4280 - CORE_LOW;           // bits of 2^-16; magnitudes
+constexpr int ZERO = CORE + 2, VALUES = 2 * CORE + 5;                // gap, CORE, gap, 0, gap, CORE, gap
+constexpr int PER_VALUE = (VALUES + THREADS - 1) / THREADS;
+// the place of a value (bf16 bits) in that order; `gap`: whether it is one of a gap
+__device__ __forceinline__ int value_place(uint32_t b, bool &gap) {
+    const uint32_t mag = b & 0x7fffu, off = mag - CORE_LOW;
+    const bool minus = b >> 15;
+    gap = off >= (uint32_t)CORE && mag != 0;
+    if (!gap) return mag == 0 ? ZERO : minus ? ZERO + 2 + (int)off : CORE - (int)off;
+    return mag >= CORE_LOW ? (minus ? VALUES - 1 : 0) : minus ? ZERO + 1 : ZERO - 1;
+}
+__device__ __forceinline__ bool is_gap(int place) {
+    return place == 0 || place == ZERO - 1 || place == ZERO + 1 || place == VALUES - 1;
+}
+__device__ __forceinline__ float value_at(int place) {               // of one that is no gap
+    if (place == ZERO) return 0.f;
+    const uint32_t b = place < ZERO ? (uint32_t)(CORE_LOW + CORE - place) : 0x8000u + CORE_LOW + (place - ZERO - 2);
+    return __uint_as_float(b << 16);
+}
+
 struct Shared {
     union {
-        unsigned limbs[2][BINS];        // weights of bins, 15 bits of each weight in one sum, ..
-        u64 bins[BINS];                 // .. or whole
-    };
-    unsigned counts[BINS];
-    union {
-        unsigned limb2[BINS];           // the uppermost 15 bits
-        u64 list[CAP];
+        struct {
+            union {
+                unsigned limbs[2][BINS];    // weights of bins, 15 bits of each weight in one sum, ..
+                u64 bins[BINS];             // .. or whole
+            };
+            unsigned counts[BINS];
+            union {
+                unsigned limb2[BINS];       // the uppermost 15 bits
+                u64 list[CAP];
+            };
+            float queue[NW][64];            // a warp's entries that wait for a whole warp of them
+        };
+        struct {
+            u64 table[VALUES];              // a value's weight; a gap's whole
+            unsigned found[VALUES];         // its count
+            float others[CAP];
+        };
     };
     double powers[16];                  // 2^(j / 16)
     u64 warp_sum[NW];                   // of the CTA's warps
@@ -79,8 +116,7 @@ struct Shared {
     float warp_max[NW], warp_pivot[NW], warp_lo[NW], warp_hi[NW];
     u64 before;                         // what lies before the bin in question
     u64 scan[NW];
-    float queue[NW][64];                // a warp's entries that wait for a whole warp of them
-    int listed, bin, least, tau_key, ti;
+    int listed, bin, least, tau_key, ti, others_count;
     unsigned entries;                   // of the range, down to the bin in question
 };
 
@@ -543,6 +579,100 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
     return 0;                                              // nothing to cut: what is below the range weighs nothing
 }
 
+// Where the sums of value(place) over the counted values reach `target`: the place (sh.bin), the sum
+// before it (sh.before); false if they do not. All CTAs of the row hold the same.
+template <typename F>
+__device__ bool value_reached(Shared &sh, u64 target, F value)
+{
+    u64 v[PER_VALUE], sum = 0, all;
+#pragma unroll
+    for (int q = 0; q < PER_VALUE; ++q) {
+        const int i = threadIdx.x * PER_VALUE + q;
+        v[q] = i < VALUES ? value(i) : 0;
+        sum += v[q];
+    }
+    u64 upto = block_before(sh, sum, all);
+#pragma unroll
+    for (int q = 0; q < PER_VALUE; ++q) {
+        const u64 lo = upto;
+        upto += v[q];
+        if (lo < target && upto >= target) sh.bin = threadIdx.x * PER_VALUE + q, sh.before = lo;
+    }
+    __syncthreads();
+    return all >= target;
+}
+
+// The cuts of a row whose values were counted (sh.found of this CTA's part, sh.others): sets what the row
+// keeps and sh.table. False where a cut falls into a gap.
+template <typename E, int C>
+__device__ bool cut_counted(Shared &sh, Row<E, C> &row, long long k, float top_p)
+{
+    const int tid = threadIdx.x;
+    for (int i = tid; i < VALUES; i += THREADS) sh.table[i] = is_gap(i) ? 0 : row.weight(value_at(i));
+    __syncthreads();
+    for (int i = tid; i < sh.others_count; i += THREADS) {
+        bool gap;
+        const int place = value_place(__float_as_uint(sh.others[i]) >> 16, gap);
+        atomicAdd(&sh.table[place], row.weight(sh.others[i]));
+        atomicAdd(&sh.found[place], 1u);
+    }
+    row_sync<C>();
+    // the whole row's, into registers, then back
+    unsigned n[PER_VALUE];
+    u64 gap[PER_VALUE];
+#pragma unroll
+    for (int q = 0; q < PER_VALUE; ++q) {
+        const int i = tid * PER_VALUE + q;
+        n[q] = 0, gap[q] = 0;
+        if (i >= VALUES) continue;
+        for (int r = 0; r < C; ++r) {
+            n[q] += of_rank<C>(sh.found, r)[i];
+            if (C > 1 && is_gap(i)) gap[q] += of_rank<C>(sh.table, r)[i];
+        }
+    }
+    row_sync<C>();
+#pragma unroll
+    for (int q = 0; q < PER_VALUE; ++q) {
+        const int i = tid * PER_VALUE + q;
+        if (i >= VALUES) continue;
+        sh.found[i] = n[q];
+        if (C > 1 && is_gap(i)) sh.table[i] = gap[q];
+    }
+    __syncthreads();
+    int last = VALUES - 1;                                 // the last place that is kept, and how many of it
+    unsigned of_last = sh.found[last];
+    auto kept_of = [&](int i) -> u64 { return i < last ? sh.found[i] : i == last ? of_last : 0; };
+    // the run ends in place sh.bin with `need` of its entries
+    auto end_at = [&](u64 need) {
+        if (is_gap(sh.bin) && need < kept_of(sh.bin)) return false;
+        of_last = (unsigned)min(need, kept_of(sh.bin));
+        last = sh.bin;
+        return true;
+    };
+    if (k > 0 && k < row.end - row.off && value_reached(sh, (u64)k, [&](int i) { return (u64)sh.found[i]; }))
+        if (!end_at((u64)k - sh.before)) return false;
+    if (top_p < 1.f) {
+        auto weight = [&](int i) -> u64 { return is_gap(i) ? (kept_of(i) ? sh.table[i] : 0) : kept_of(i) * sh.table[i]; };
+        u64 mine = 0, all;
+        for (int i = tid; i < VALUES; i += THREADS) mine += weight(i);
+        block_before(sh, mine, all);
+        const u64 target = share_of(top_p, all);
+        if (value_reached(sh, target, weight)) {
+            if (is_gap(sh.bin)) return false;
+            const u64 each = sh.table[sh.bin];
+            end_at((target - sh.before + each - 1) / each);
+        }
+    }
+    if (is_gap(last)) return last == VALUES - 1;           // nothing was cut, or a gap's smallest is wanted
+    row.tau = value_at(last), row.ti = EVERY;
+    if (of_last < sh.found[last]) {
+        Row<E, C> whole = row;
+        whole.tau = NEG_INF;
+        row.ti = nth_equal(sh, whole, row.tau, (int)of_last);
+    }
+    return true;
+}
+
 // The rest of a row whose candidates are all in sh.list: n entries, of which the k first in rank count,
 // and of those the ones that reach `target`, or (0) the share top_p of their weight.
 template <typename E, int C>
@@ -601,7 +731,8 @@ template <typename E, int C>
 __global__ void __launch_bounds__(THREADS, C > 2 ? 1 : 2)
 sample_kernel(const __grid_constant__ SampleArgs s)
 {
-    __shared__ Shared sh;
+    extern __shared__ __align__(16) unsigned char memory[];
+    Shared &sh = *reinterpret_cast<Shared *>(memory);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = rank_of<C>(), at = blockIdx.x / C;
     Row<E, C> row;
@@ -616,11 +747,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     row.tau = NEG_INF, row.ti = EVERY;
     const int w = rank * NW + warp;
     if (tid < 16) sh.powers[tid] = exp2(tid / 16.0);
-    if (tid == 0) sh.listed = 0, sh.least = EVERY;
-
-    // the largest value (NaN if there is one)
-    float most = NEG_INF;
-    row.template words<4>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) { most = max_nan(most, v.most()); });
+    if (tid == 0) sh.listed = 0, sh.least = EVERY, sh.others_count = 0;
     const float t = s.temperature ? s.temperature[at] : s.temperature1;
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
@@ -628,6 +755,31 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     // k entries at least are as large as the smallest of all warps' j-th largest of their lanes' maxima
     const int j = (int)min((k + C * NW - 1) / (C * NW), 1000ll);
     const bool listed = k > 1 && k < s.vocab && j <= 16;
+    bool counted = sizeof(E) == 2 && !listed && k != 1 && t > 0.f && top_p > 0.f;
+    if (counted)
+        for (int i = tid; i < VALUES; i += THREADS) sh.found[i] = 0;
+    __syncthreads();
+    // the largest value (NaN if there is one)
+    float most = NEG_INF;
+    if (counted) {
+        row.template words<1>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) {
+            most = max_nan(most, v.most());
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const uint32_t b = __float_as_uint(v.at(i)) >> 16;
+                bool gap;
+                const int place = value_place(b, gap);
+                if (!gap) {
+                    atomicAdd(&sh.found[place], 1u);
+                } else if (b != 0xff80u) {
+                    const int to = atomicAdd(&sh.others_count, 1);
+                    if (to < CAP) sh.others[to] = v.at(i);
+                }
+            }
+        });
+    } else {
+        row.template words<4>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) { most = max_nan(most, v.most()); });
+    }
     if (listed) {
         uint32_t mine = most == most ? key_of(most) : 0, best = 0;
         for (int q = 0; q < j; ++q) {
@@ -677,22 +829,33 @@ sample_kernel(const __grid_constant__ SampleArgs s)
             return;
         }
     }
-    if (isinf(row.top)) row.tau = row.top;                 // nothing beside it has weight
-    u64 target = (u64)k;
-    int in_list = k > 0 && k < s.vocab ? cut<false>(sh, row, target, 0.f) : 0;
-    const bool few = in_list > 0;
-    if (!few && top_p < 1.f) in_list = cut<true>(sh, row, target, top_p);
-    if (in_list > 0) {
-        if (rank == 0) finish_list(sh, row, s, at, in_list, few ? (int)k : in_list, top_p, few ? 0 : target, least);
-        return;
+    if (counted) {
+        for (int r = 0; r < C; ++r) counted = counted && *of_rank<C>(&sh.others_count, r) <= CAP;
+        counted = counted && !isinf(row.top) && cut_counted(sh, row, k, top_p);
+    }
+    if (!counted) {
+        row_sync<C>();                                     // what was counted gives way to bins
+        row.tau = isinf(row.top) ? row.top : NEG_INF;      // (nothing beside it has weight)
+        u64 target = (u64)k;
+        int in_list = k > 0 && k < s.vocab ? cut<false>(sh, row, target, 0.f) : 0;
+        const bool few = in_list > 0;
+        if (!few && top_p < 1.f) in_list = cut<true>(sh, row, target, top_p);
+        if (in_list > 0) {
+            if (rank == 0) finish_list(sh, row, s, at, in_list, few ? (int)k : in_list, top_p, few ? 0 : target, least);
+            return;
+        }
     }
     auto weight = [&](float v, int i) -> u64 {
         if (!row.kept(v, i)) return 0;
-        const u64 x = row.weight(v);
+        u64 x;
+        bool gap = true;
+        const int place = counted ? value_place(__float_as_uint(v) >> 16, gap) : 0;
+        if (!gap) x = sh.table[place];
+        else x = row.weight(v);
         return x >= least ? x : 0;
     };
     u64 mass = 0;
-    if (row.tau == NEG_INF) {
+    if (counted || row.tau == NEG_INF) {
         row.each([&](float v, int i) { mass += weight(v, i); });
     } else {
         // few of the entries are kept: their weights are computed 32 at a time
@@ -776,12 +939,15 @@ sample_kernel(const __grid_constant__ SampleArgs s)
 template <typename E, int C>
 cudaError_t sample_of(const SampleArgs &a, cudaStream_t stream)
 {
+    const cudaError_t e = smem_opt_in<sample_kernel<E, C>>(sizeof(Shared));
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c{};
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = C, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     c.gridDim = dim3((unsigned)((long long)a.rows * C));
     c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = sizeof(Shared);
     c.stream = stream;
     c.attrs = &cluster;
     c.numAttrs = C > 1 ? 1 : 0;
