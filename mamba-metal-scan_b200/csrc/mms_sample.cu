@@ -18,7 +18,7 @@
 //
 // A row is read by a cluster of C CTAs; warp q of all of theirs has the q-th piece of the
 // row in every pass, so that sums in index order are sums over warps.
-//   k up to 256 C: every warp has the j-th largest of its 32 lanes' maxima, j = k / warps
+//   k up to about 256 C: every warp has the j-th largest of its 32 lanes' maxima, j = k / warps
 //     rounded up; the smallest of these has k entries above it or equal, and not many
 //     more. Those are listed and sorted, and all else happens on the list.
 //   else: the end of the run of k entries, or of the mass p, is found by bins over the
@@ -73,16 +73,23 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 constexpr int CORE_LOW = 0x3780, CORE = 0x4280 - CORE_LOW;           // bits of 2^-16; magnitudes
 constexpr int ZERO = CORE + 2, VALUES = 2 * CORE + 5;                // gap, CORE, gap, 0, gap, CORE, gap
 constexpr int PER_VALUE = (VALUES + THREADS - 1) / THREADS;
-// the place of a value (bf16 bits) in that order; `gap`: whether it is one of a gap
-__device__ __forceinline__ int value_place(uint32_t b, bool &gap) {
-    const uint32_t mag = b & 0x7fffu, off = mag - CORE_LOW;
-    const bool minus = b >> 15;
-    gap = off >= (uint32_t)CORE && mag != 0;
-    if (!gap) return mag == 0 ? ZERO : minus ? ZERO + 2 + (int)off : CORE - (int)off;
-    return mag >= CORE_LOW ? (minus ? VALUES - 1 : 0) : minus ? ZERO + 1 : ZERO - 1;
+// Where a counted value (bf16 bits) lies in the tables: positive ones by magnitude, then negative
+// ones, then 0; -1 for the others.
+__device__ __forceinline__ int value_slot(uint32_t b) {
+    const uint32_t off = (b & 0x7fffu) - CORE_LOW;
+    return off < (uint32_t)CORE ? (int)(off + (b >> 15) * CORE) : (b & 0x7fffu) == 0 ? 2 * CORE : -1;
+}
+// A gap's slot behind them.
+__device__ __forceinline__ int gap_slot(uint32_t b) {
+    return 2 * CORE + 1 + ((b & 0x7fffu) < CORE_LOW ? 1 + (b >> 15) : 3 * (b >> 15));
 }
 __device__ __forceinline__ bool is_gap(int place) {
     return place == 0 || place == ZERO - 1 || place == ZERO + 1 || place == VALUES - 1;
+}
+// the slot of a place in the descending order
+__device__ __forceinline__ int slot_at(int place) {
+    if (is_gap(place)) return 2 * CORE + 1 + (place == 0 ? 0 : place == ZERO - 1 ? 1 : place == ZERO + 1 ? 2 : 3);
+    return place == ZERO ? 2 * CORE : place < ZERO ? CORE - place : CORE + (place - ZERO - 2);
 }
 __device__ __forceinline__ float value_at(int place) {               // of one that is no gap
     if (place == ZERO) return 0.f;
@@ -105,7 +112,7 @@ struct Shared {
             float queue[NW][64];            // a warp's entries that wait for a whole warp of them
         };
         struct {
-            u64 table[VALUES];              // a value's weight; a gap's whole
+            u64 table[VALUES];              // a value's weight; a gap's whole (by slot)
             unsigned found[VALUES];         // its count
             float others[CAP];
         };
@@ -260,14 +267,8 @@ struct Row {
             }
         }
     }
-    template <int C1>
-    __device__ __forceinline__ u64 sum_of(Shared &sh, int bin) const {
-        u64 s = 0;
-        for (int r = 0; r < C1; ++r) {
-            Shared *o = of_rank<C1>(&sh, r);
-            s += end - off > LIMBS_MAX ? o->bins[bin] : o->limbs[0][bin] + ((u64)o->limbs[1][bin] << 15) + ((u64)o->limb2[bin] << 30);
-        }
-        return s;
+    __device__ __forceinline__ u64 weight_of(const Shared &o, int bin) const {
+        return end - off > LIMBS_MAX ? o.bins[bin] : o.limbs[0][bin] + ((u64)o.limbs[1][bin] << 15) + ((u64)o.limb2[bin] << 30);
     }
     __device__ __forceinline__ bool kept(float v, int i) const { return v > tau || (v == tau && i <= ti); }
 
@@ -385,6 +386,31 @@ __device__ void sort_list(u64 *list, int n)
 __device__ __forceinline__ u64 ranked(float v, int i) { return (u64)(~key_of(v)) << 32 | (unsigned)i; }
 __device__ __forceinline__ float ranked_value(u64 e) { return of_key(~(uint32_t)(e >> 32)); }
 
+// An entry to the CTA's list (counted, but not kept, above CAP).
+__device__ __forceinline__ void to_list(Shared &sh, float v, int i) {
+    const int at = atomicAdd(&sh.listed, 1);
+    if (at < CAP) sh.list[at] = ranked(v, i);
+}
+// All CTAs' lists to the first one's, if it holds them; how many entries that are (all CTAs get it).
+template <int C>
+__device__ int join_lists(Shared &sh) {
+    row_sync<C>();
+    if constexpr (C == 1) return sh.listed;
+    int n[C], all = 0;
+#pragma unroll
+    for (int r = 0; r < C; ++r) all += n[r] = *of_rank<C>(&sh.listed, r);
+    if (rank_of<C>() == 0 && all <= CAP) {
+        int to = n[0];
+#pragma unroll
+        for (int r = 1; r < C; ++r) {
+            for (int i = threadIdx.x; i < n[r]; i += THREADS) sh.list[to + i] = of_rank<C>(sh.list, r)[i];
+            to += n[r];
+        }
+    }
+    row_sync<C>();
+    return all;
+}
+
 // The first index of 0 .. n - 1 at which the sums of value(i) reach `target` (n - 1 if none does).
 template <typename F>
 __device__ int reached(Shared &sh, int n, u64 target, F value)
@@ -498,14 +524,29 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
         });
         if (MASS && round == 0) row_sums<C>(sh, beside);
         else row_sync<C>();
-        // each thread's bins of the whole row, then where the sum reaches the target
         u64 mine[PER], sum = 0, all;
         unsigned counts[PER];
+        if constexpr (C > 1) {                             // the whole row's bins to every CTA
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                counts[q] = 0, mine[q] = 0;
+                for (int r = 0; r < C; ++r) counts[q] += of_rank<C>(sh.counts, r)[tid + q * THREADS];
+                if (MASS)
+                    for (int r = 0; r < C; ++r) mine[q] += row.weight_of(*of_rank<C>(&sh, r), tid + q * THREADS);
+            }
+            row_sync<C>();
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                sh.counts[tid + q * THREADS] = counts[q];
+                if (MASS) sh.bins[tid + q * THREADS] = mine[q];
+            }
+            __syncthreads();
+        }
+        // each thread's bins, then where the sum reaches the target
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
-            counts[q] = 0, mine[q] = 0;
-            for (int r = 0; r < C; ++r) counts[q] += of_rank<C>(sh.counts, r)[tid * PER + q];
-            mine[q] = MASS ? row.template sum_of<C>(sh, tid * PER + q) : counts[q];
+            counts[q] = sh.counts[tid * PER + q];
+            mine[q] = !MASS ? counts[q] : C > 1 ? sh.bins[tid * PER + q] : row.weight_of(sh, tid * PER + q);
             sum += mine[q];
         }
         u64 upto = block_before(sh, sum, all);
@@ -538,16 +579,12 @@ __device__ int cut(Shared &sh, Row<E, C> &row, u64 &target, float share)
             if (whole ? k > bin : k != bin) return;
             if (MASS && row.weight(v) <= light) return;    // (not in the bins either)
             lo = fminf(lo, v), hi = fmaxf(hi, v);
-            const int at = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
-            if (at < CAP) of_rank<C>(&sh, 0)->list[at] = ranked(v, i);
+            to_list(sh, v, i);
         });
         lo = row_fold<C>(sh.warp_lo, lo, [](float x, float y) { return fminf(x, y); });
         hi = row_fold<C>(sh.warp_hi, hi, [](float x, float y) { return fmaxf(x, y); });
-        const int n = of_rank<C>(&sh, 0)->listed;
-        if (whole) {
-            row_sync<C>();
-            return min(n, CAP);
-        }
+        const int n = join_lists<C>(sh);
+        if (whole) return min(n, CAP);
         if (lo == hi) {
             const u64 each = MASS ? row.weight(lo) : 1ull;
             const u64 need = (target - before + each - 1) / each;
@@ -602,46 +639,45 @@ __device__ bool value_reached(Shared &sh, u64 target, F value)
     return all >= target;
 }
 
-// The cuts of a row whose values were counted (sh.found of this CTA's part, sh.others): sets what the row
-// keeps and sh.table. False where a cut falls into a gap.
+// Weights by value (sh.table) and, where there are `cuts`, what the row keeps, from the counts of its values
+// (sh.found of this CTA's part, sh.others). False where a cut falls into a gap.
 template <typename E, int C>
-__device__ bool cut_counted(Shared &sh, Row<E, C> &row, long long k, float top_p)
+__device__ bool cut_counted(Shared &sh, Row<E, C> &row, bool cuts, long long k, float top_p, u64 least)
 {
     const int tid = threadIdx.x;
-    for (int i = tid; i < VALUES; i += THREADS) sh.table[i] = is_gap(i) ? 0 : row.weight(value_at(i));
+    for (int i = tid; i < VALUES; i += THREADS) sh.table[slot_at(i)] = is_gap(i) ? 0 : row.weight(value_at(i));
     __syncthreads();
-    for (int i = tid; i < sh.others_count; i += THREADS) {
-        bool gap;
-        const int place = value_place(__float_as_uint(sh.others[i]) >> 16, gap);
-        atomicAdd(&sh.table[place], row.weight(sh.others[i]));
-        atomicAdd(&sh.found[place], 1u);
-    }
-    row_sync<C>();
-    // the whole row's, into registers, then back
-    unsigned n[PER_VALUE];
-    u64 gap[PER_VALUE];
+    if (cuts) {
+        for (int i = tid; i < sh.others_count; i += THREADS) {
+            const int slot = gap_slot(__float_as_uint(sh.others[i]) >> 16);
+            atomicAdd(&sh.table[slot], row.weight(sh.others[i]));
+            atomicAdd(&sh.found[slot], 1u);
+        }
+        row_sync<C>();
+        if constexpr (C > 1) {
+            // the whole row's, into registers, then back
+            unsigned n[PER_VALUE];
+            u64 gap = 0;
 #pragma unroll
-    for (int q = 0; q < PER_VALUE; ++q) {
-        const int i = tid * PER_VALUE + q;
-        n[q] = 0, gap[q] = 0;
-        if (i >= VALUES) continue;
-        for (int r = 0; r < C; ++r) {
-            n[q] += of_rank<C>(sh.found, r)[i];
-            if (C > 1 && is_gap(i)) gap[q] += of_rank<C>(sh.table, r)[i];
+            for (int q = 0; q < PER_VALUE; ++q) {
+                const int i = tid + q * THREADS;
+                n[q] = 0;
+                if (i < VALUES)
+                    for (int r = 0; r < C; ++r) n[q] += of_rank<C>(sh.found, r)[i];
+            }
+            if (tid < VALUES - 2 * CORE - 1)
+                for (int r = 0; r < C; ++r) gap += of_rank<C>(sh.table, r)[2 * CORE + 1 + tid];
+            row_sync<C>();
+#pragma unroll
+            for (int q = 0; q < PER_VALUE; ++q)
+                if (tid + q * THREADS < VALUES) sh.found[tid + q * THREADS] = n[q];
+            if (tid < VALUES - 2 * CORE - 1) sh.table[2 * CORE + 1 + tid] = gap;
+            __syncthreads();
         }
     }
-    row_sync<C>();
-#pragma unroll
-    for (int q = 0; q < PER_VALUE; ++q) {
-        const int i = tid * PER_VALUE + q;
-        if (i >= VALUES) continue;
-        sh.found[i] = n[q];
-        if (C > 1 && is_gap(i)) sh.table[i] = gap[q];
-    }
-    __syncthreads();
     int last = VALUES - 1;                                 // the last place that is kept, and how many of it
-    unsigned of_last = sh.found[last];
-    auto kept_of = [&](int i) -> u64 { return i < last ? sh.found[i] : i == last ? of_last : 0; };
+    unsigned of_last = cuts ? sh.found[slot_at(last)] : 1;
+    auto kept_of = [&](int i) -> u64 { return i < last ? sh.found[slot_at(i)] : i == last ? of_last : 0; };
     // the run ends in place sh.bin with `need` of its entries
     auto end_at = [&](u64 need) {
         if (is_gap(sh.bin) && need < kept_of(sh.bin)) return false;
@@ -649,27 +685,40 @@ __device__ bool cut_counted(Shared &sh, Row<E, C> &row, long long k, float top_p
         last = sh.bin;
         return true;
     };
-    if (k > 0 && k < row.end - row.off && value_reached(sh, (u64)k, [&](int i) { return (u64)sh.found[i]; }))
+    if (cuts && k > 0 && k < row.end - row.off && value_reached(sh, (u64)k, [&](int i) { return (u64)sh.found[slot_at(i)]; }))
         if (!end_at((u64)k - sh.before)) return false;
     if (top_p < 1.f) {
-        auto weight = [&](int i) -> u64 { return is_gap(i) ? (kept_of(i) ? sh.table[i] : 0) : kept_of(i) * sh.table[i]; };
+        auto weight = [&](int i) -> u64 {
+            const u64 n = kept_of(i);
+            return n ? (is_gap(i) ? 1 : n) * sh.table[slot_at(i)] : 0;
+        };
         u64 mine = 0, all;
         for (int i = tid; i < VALUES; i += THREADS) mine += weight(i);
         block_before(sh, mine, all);
         const u64 target = share_of(top_p, all);
         if (value_reached(sh, target, weight)) {
             if (is_gap(sh.bin)) return false;
-            const u64 each = sh.table[sh.bin];
+            const u64 each = sh.table[slot_at(sh.bin)];
             end_at((target - sh.before + each - 1) / each);
         }
     }
-    if (is_gap(last)) return last == VALUES - 1;           // nothing was cut, or a gap's smallest is wanted
-    row.tau = value_at(last), row.ti = EVERY;
-    if (of_last < sh.found[last]) {
-        Row<E, C> whole = row;
-        whole.tau = NEG_INF;
-        row.ti = nth_equal(sh, whole, row.tau, (int)of_last);
+    if (is_gap(last) && last != VALUES - 1) return false;  // a gap's smallest is wanted
+    if (last != VALUES - 1) {
+        const unsigned there = sh.found[slot_at(last)];
+        row.tau = value_at(last), row.ti = EVERY;
+        if (of_last < there) {
+            Row<E, C> whole = row;
+            whole.tau = NEG_INF;
+            row.ti = nth_equal(sh, whole, row.tau, (int)of_last);
+        }
     }
+    __syncthreads();
+    // the table for the draw: 0 for what is not kept (of the last value, beyond ti, the draw sees to it)
+    for (int i = tid; i < VALUES; i += THREADS) {
+        const int slot = slot_at(i);
+        if (i > last || (!is_gap(i) && sh.table[slot] < least)) sh.table[slot] = 0;
+    }
+    __syncthreads();
     return true;
 }
 
@@ -752,26 +801,27 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
     const float min_p = fminf(s.min_p ? s.min_p[at] : s.min_p1, 1.f);
-    // k entries at least are as large as the smallest of all warps' j-th largest of their lanes' maxima
-    const int j = (int)min((k + C * NW - 1) / (C * NW), 1000ll);
+    // k entries at least are as large as the smallest of the warps' j-th largest of their lanes'
+    // maxima, of those warps whose pieces are whole
+    const int pieces = max(1, row.end / row.piece);
+    const int j = (int)min((k + pieces - 1) / pieces, 1000ll);
     const bool listed = k > 1 && k < s.vocab && j <= 16;
+    const bool cuts = (k > 0 && k < s.vocab) || top_p < 1.f;
     bool counted = sizeof(E) == 2 && !listed && k != 1 && t > 0.f && top_p > 0.f;
-    if (counted)
+    if (counted && cuts)
         for (int i = tid; i < VALUES; i += THREADS) sh.found[i] = 0;
     __syncthreads();
     // the largest value (NaN if there is one)
     float most = NEG_INF;
-    if (counted) {
+    if (counted && cuts) {
         row.template words<1>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) {
             most = max_nan(most, v.most());
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const uint32_t b = __float_as_uint(v.at(i)) >> 16;
-                bool gap;
-                const int place = value_place(b, gap);
-                if (!gap) {
-                    atomicAdd(&sh.found[place], 1u);
-                } else if (b != 0xff80u) {
+                const int slot = value_slot(b);
+                if (slot >= 0) atomicAdd(&sh.found[slot], 1u);
+                if (slot < 0 && b != 0xff80u) {
                     const int to = atomicAdd(&sh.others_count, 1);
                     if (to < CAP) sh.others[to] = v.at(i);
                 }
@@ -787,7 +837,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
             const unsigned has = __ballot_sync(0xffffffffu, mine == best);
             if (lane == __ffs(has) - 1) mine = 0;
         }
-        if (lane == 0) sh.warp_pivot[warp] = best ? of_key(best) : NEG_INF;
+        if (lane == 0) sh.warp_pivot[warp] = w >= pieces ? -NEG_INF : best ? of_key(best) : NEG_INF;
     }
     row.top = row_fold<C>(sh.warp_max, most, [](float x, float y) { return max_nan(x, y); });
     row.rate = 1.0 / (double)t;
@@ -817,13 +867,9 @@ sample_kernel(const __grid_constant__ SampleArgs s)
         for (int i = lane + 32; i < C * NW; i += 32) pivot = fminf(pivot, of_rank<C>(sh.warp_pivot, i / NW)[i % NW]);
         pivot = warp_fold(pivot, [](float x, float y) { return fminf(x, y); });
         row.each([&](float v, int i) {
-            if (v < pivot) return;
-            const int to = atomicAdd(&of_rank<C>(&sh, 0)->listed, 1);
-            if (to < CAP) of_rank<C>(&sh, 0)->list[to] = ranked(v, i);
+            if (v >= pivot) to_list(sh, v, i);
         });
-        row_sync<C>();
-        const int n = of_rank<C>(&sh, 0)->listed;
-        row_sync<C>();
+        const int n = join_lists<C>(sh);
         if (n <= CAP) {
             if (rank == 0) finish_list(sh, row, s, at, n, (int)k, top_p, 0, least);
             return;
@@ -831,7 +877,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     }
     if (counted) {
         for (int r = 0; r < C; ++r) counted = counted && *of_rank<C>(&sh.others_count, r) <= CAP;
-        counted = counted && !isinf(row.top) && cut_counted(sh, row, k, top_p);
+        counted = counted && !isinf(row.top) && cut_counted(sh, row, cuts, k, top_p, least);
     }
     if (!counted) {
         row_sync<C>();                                     // what was counted gives way to bins
@@ -846,16 +892,28 @@ sample_kernel(const __grid_constant__ SampleArgs s)
         }
     }
     auto weight = [&](float v, int i) -> u64 {
+        if (counted) {
+            const int slot = value_slot(__float_as_uint(v) >> 16);
+            if (slot >= 0) return v == row.tau && i > row.ti ? 0 : sh.table[slot];
+        }
         if (!row.kept(v, i)) return 0;
-        u64 x;
-        bool gap = true;
-        const int place = counted ? value_place(__float_as_uint(v) >> 16, gap) : 0;
-        if (!gap) x = sh.table[place];
-        else x = row.weight(v);
+        const u64 x = row.weight(v);
         return x >= least ? x : 0;
     };
     u64 mass = 0;
-    if (counted || row.tau == NEG_INF) {
+    if (counted) {
+        const bool part = row.ti != EVERY;                 // of the entries equal to tau
+        row.template words<1>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int place) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float x = v.at(i);
+                const int slot = value_slot(__float_as_uint(x) >> 16);
+                if (slot >= 0) mass += sh.table[slot];
+                if (slot < 0 && x > NEG_INF) mass += weight(x, place + i - row.off);
+                if (part && x == row.tau && place + i - row.off > row.ti) mass -= sh.table[slot];
+            }
+        });
+    } else if (row.tau == NEG_INF) {
         row.each([&](float v, int i) { mass += weight(v, i); });
     } else {
         // few of the entries are kept: their weights are computed 32 at a time
