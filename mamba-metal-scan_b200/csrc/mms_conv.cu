@@ -26,11 +26,13 @@ namespace {
 constexpr int WARPS = 4;                // per CTA, each with rows of its own and the same channels
 constexpr int THREADS = 32 * WARPS;
 constexpr int TAIL_ROWS = 32;           // rows of packed sequences a warp walks
-// Rows that a warp loads at once, and computes while the next are on their way.
+// Rows that a warp loads at once, and computes while the next are on their way: 64 bytes a lane and
+// array. (Backward with half of them at 4 CTAs an SM: 201 us of 4 x 4096 x 8192 in bf16, so 174;
+// a quarter, 228; a forward that loads a tile and then computes it, 177, so 91.)
 template <typename E>
 constexpr int FWD_STEP = sizeof(E) == 4 ? 4 : 8;
 template <typename E>
-constexpr int BWD_STEP = sizeof(E) == 4 ? 2 : 4;
+constexpr int BWD_STEP = sizeof(E) == 4 ? 4 : 8;
 
 // VEC neighbouring channels of a row as they are stored, and as NP pairs of floats (one
 // channel alone: the second of its pair is 0).
@@ -204,7 +206,7 @@ conv_fwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *
 // computed as well, for dx alone. dw and dbias stay in registers; the CTA's four
 // warps are joined in shared memory and leave one partial sum a CTA.
 template <typename E, int KT, bool EXACT, int VEC>
-__global__ void __launch_bounds__(THREADS, KT <= 4 ? 4 : 2)
+__global__ void __launch_bounds__(THREADS, KT <= 4 ? 3 : 2)
 conv_bwd_kernel(const E *__restrict__ x, long long ldb, long long ldt, const E *__restrict__ w,
                 const E *__restrict__ bias, const E *__restrict__ dy, E *__restrict__ dx,
                 float *__restrict__ part, int T, int D, int K_in, bool silu, int nd, int segs, int len, long long rows)

@@ -29,8 +29,7 @@
 // segments, no two share a number, and a search over the starts finds s.
 //
 // Single tokens without a list of starts are bound by the states' bytes, read and
-// written once: 4 states a lane, G lanes a channel, several sequences a thread so that
-// their loads are in flight together and Aneg is read once.
+// written once: 4 states a lane, G lanes a channel.
 #include <algorithm>
 #include <type_traits>
 
@@ -48,17 +47,9 @@ constexpr int STAGES = 3;               // tiles of x, dt and z
 constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 flushes to 0
 // A sequence's first segment is done in full in the first launch if it has at most FEW
 // segments; of longer ones its end comes first, like the others', so that the launch does not
-// end with its CTAs alone.
-#ifndef MMS_PACKED_FEW
-#define MMS_PACKED_FEW 1
-#endif
-constexpr int FEW = MMS_PACKED_FEW;
-#ifndef MMS_PACKED_MINB
-#define MMS_PACKED_MINB 4
-#endif
-#ifndef MMS_PACKED_FILL
-#define MMS_PACKED_FILL 4
-#endif
+// end with its CTAs alone (3 for 1: 229 for 215 us, 16 prompts of 8192 x 2304 x 16 in bf16).
+constexpr int FEW = 1;
+constexpr int CTAS = 4;                 // an SM: what the registers hold
 
 template <typename E, typename BE>
 struct Args {
@@ -393,7 +384,7 @@ __device__ __forceinline__ void carry(States<S> &h, const States<S> &nan2, float
 }
 
 template <typename E, typename BE, typename S, bool REST, bool VEC>
-__global__ void __launch_bounds__(THREADS, MMS_PACKED_MINB)
+__global__ void __launch_bounds__(THREADS, CTAS)
 scan_segments_kernel(const __grid_constant__ Args<E, BE> a)
 {
     __shared__ __align__(16) float bc[2 * TT * 2 * S::NP];
@@ -485,57 +476,51 @@ __device__ __forceinline__ float4 four(const BE *p)
 
 constexpr int TOKEN_THREADS = 256;
 
-// Lane g of a channel's G holds states 4g .. 4g + 3 of SEQ sequences.
-template <typename E, typename BE, int G, int SEQ>
+// Lane g of a channel's G holds states 4g .. 4g + 3. A CTA takes `per` sequences one after another,
+// the next one's state and the places of the one after it on their way meanwhile.
+template <typename E, typename BE, int G>
 __global__ void __launch_bounds__(TOKEN_THREADS)
-scan_token_kernel(const __grid_constant__ Args<E, BE> a)
+scan_token_kernel(const __grid_constant__ Args<E, BE> a, int per)
 {
-    const int tid = blockIdx.x % a.nd * TOKEN_THREADS + threadIdx.x;
-    const int d = tid / G, g = threadIdx.x % G, n = 4 * g;
-    const int s0 = blockIdx.x / a.nd * SEQ;
+    const int block = blockIdx.x % a.nd;
+    const int d = (block * TOKEN_THREADS + (int)threadIdx.x) / G, g = threadIdx.x % G, n = 4 * g;
+    const int s0 = blockIdx.x / a.nd * per, s1 = min(a.seq.count, s0 + per);
     const bool chan = d < a.D, act = chan && n < a.N;
-    const size_t DN = (size_t)a.D * a.N, at = (size_t)d * a.N + n;
-    float4 hv[SEQ], Bv[SEQ], Cv[SEQ];
-    float xv[SEQ], dtv[SEQ], zv[SEQ];
-    long long to[SEQ];
-#pragma unroll
-    for (int q = 0; q < SEQ; ++q) {
-        const int s = s0 + q;
-        const bool in = s < a.seq.count;
-        const long long from = in ? a.seq.from(s) : -1;
-        to[q] = in ? a.seq.to(s) : -1;
-        hv[q] = Bv[q] = Cv[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-        xv[q] = dtv[q] = zv[q] = 0.f;
-        if (act && from >= 0) hv[q] = *reinterpret_cast<const float4 *>(a.state + from * DN + at);
-        if (act && in) {
-            Bv[q] = four(a.B + s * a.ldB + n);
-            Cv[q] = four(a.C + s * a.ldC + n);
-        }
-        if (chan && in) {
-            xv[q] = to_f(a.x[s * a.ldx + d]);
-            dtv[q] = to_f(a.dt[s * a.lddt + d]);
-            if (a.z) zv[q] = to_f(a.z[s * a.ldz + d]);
-        }
-    }
+    const size_t DN = (size_t)a.D * a.N;
+    float *state = a.state + (act ? (size_t)d * a.N + n : 0);
+    const int ds = chan ? d : 0, ns = act ? n : 0;
     float4 av = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (act) av = ld4(a.aneg + at);
+    if (act) av = ld4(a.aneg + (size_t)d * a.N + n);
+    const float skip = a.d_skip && chan ? a.d_skip[d] : 0.f;
+    auto from_of = [&](int s) { return s < s1 ? (int)a.seq.from(s) : -1; };
+    auto state_of = [&](int from) {
+        return act && from >= 0 ? *reinterpret_cast<const float4 *>(state + from * DN) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    int from = from_of(s0), from_next = from_of(s0 + 1), to = (int)a.seq.to(s0);
+    float4 hv = state_of(from);
     if (a.pj.on) av = make_float4(softplus(av.x), softplus(av.y), softplus(av.z), softplus(av.w));
     const float2 n0 = f2(-av.x * MMS_LOG2E, -av.y * MMS_LOG2E), n1 = f2(-av.z * MMS_LOG2E, -av.w * MMS_LOG2E);
-    const float skip = a.d_skip && chan ? a.d_skip[d] : 0.f;
-#pragma unroll
-    for (int q = 0; q < SEQ; ++q) {
-        if (a.pj.on) dtv[q] = fmaf(a.pj.range, sigmoid_fast(dtv[q]), a.pj.lo);
-        const float2 dt2 = f2(dtv[q], dtv[q]), bx2 = f2(dtv[q] * xv[q], dtv[q] * xv[q]);
-        const float2 h0 = fma2(ex2x2(mul2(dt2, n0)), lo(hv[q]), mul2(bx2, lo(Bv[q])));
-        const float2 h1 = fma2(ex2x2(mul2(dt2, n1)), hi(hv[q]), mul2(bx2, hi(Bv[q])));
-        if (act && to[q] >= 0) st4(a.state + to[q] * DN + at, make_float4(h0.x, h0.y, h1.x, h1.y));
-        const float2 acc = fma2(hi(Cv[q]), h1, mul2(lo(Cv[q]), h0));
-        float yv = acc.x + acc.y;
+    for (int s = s0; s < s1; ++s) {
+        float4 Bv = four(a.B + s * a.ldB + ns), Cv = four(a.C + s * a.ldC + ns);
+        const float xv = to_f(a.x[s * a.ldx + ds]);
+        float dtv = to_f(a.dt[s * a.lddt + ds]), zv = 0.f;
+        if (a.z) zv = to_f(a.z[s * a.ldz + ds]);
+        const float4 h_next = state_of(from_next);
+        const int to_next = s + 1 < s1 ? (int)a.seq.to(s + 1) : -1;
+        from_next = from_of(s + 2);
+        if (a.pj.on) dtv = fmaf(a.pj.range, sigmoid_fast(dtv), a.pj.lo);
+        const float2 dt2 = f2(dtv, dtv), bx2 = f2(dtv * xv, dtv * xv);
+        const float2 h0 = fma2(ex2x2(mul2(dt2, n0)), lo(hv), mul2(bx2, lo(Bv)));
+        const float2 h1 = fma2(ex2x2(mul2(dt2, n1)), hi(hv), mul2(bx2, hi(Bv)));
+        if (act && to >= 0) st4(state + to * DN, make_float4(h0.x, h0.y, h1.x, h1.y));
+        const float2 acc = fma2(hi(Cv), h1, mul2(lo(Cv), h0));
+        float yv = act ? acc.x + acc.y : 0.f;
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o, G);
         yv += skip;
-        if (a.z) yv *= zv[q] * sigmoid_fast(zv[q]);
-        if (chan && g == 0 && s0 + q < a.seq.count) a.y[(long long)(s0 + q) * a.D + d] = from_f<E>(yv);
+        if (a.z) yv *= zv * sigmoid_fast(zv);
+        if (chan && g == 0) a.y[(long long)s * a.D + d] = from_f<E>(yv);
+        hv = h_next, to = to_next;
     }
 }
 
@@ -550,12 +535,12 @@ long long channel_blocks(int D, int N)
     return (D + dpb - 1) / dpb;
 }
 
-// Rows of a segment: as few as give every SM 4 CTAs (16 warps, what the registers hold)
-// when the rows belong to one sequence, at least 64, a whole number of tiles.
+// Rows of a segment: as few as give every SM its CTAs when the rows belong to one sequence, at
+// least 64, a whole number of tiles. (Half of that: 337 for 292 us, 16384 x 2048 x 16.)
 int segment_rows(int rows, int D, int N)
 {
     const long long nd = channel_blocks(D, N);
-    const long long want = std::max<long long>(1, (long long)MMS_PACKED_FILL * N_SM / nd);
+    const long long want = std::max<long long>(1, (long long)CTAS * N_SM / nd);
     const long long seg = std::max<long long>(64, (rows + want - 1) / want);
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
 }
@@ -631,15 +616,11 @@ cudaError_t tokens_of(const ScanPackedArgs &p, cudaStream_t stream)
 {
     Args<E, BE> a = args_of<E, BE>(p);
     a.nd = (p.D * G + TOKEN_THREADS - 1) / TOKEN_THREADS;
-    // 4 sequences a thread once that still leaves 8 CTAs an SM, else one: the shorter chain of loads
-#ifndef MMS_TOKEN_SEQ
-#define MMS_TOKEN_SEQ 1
-#endif
-    const bool many = MMS_TOKEN_SEQ > 1 && (long long)a.nd * p.seq.count >= (long long)MMS_TOKEN_SEQ * 8 * N_SM;
-    const long long blocks = (long long)a.nd * (many ? (p.seq.count + MMS_TOKEN_SEQ - 1) / MMS_TOKEN_SEQ : p.seq.count);
+    // as many sequences a CTA, up to 8, as leave every SM 8 CTAs
+    const int per = (int)std::min<long long>(8, std::max<long long>(1, (long long)a.nd * p.seq.count / (8 * N_SM)));
+    const long long blocks = (long long)a.nd * ((p.seq.count + per - 1) / per);
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (many) scan_token_kernel<E, BE, G, MMS_TOKEN_SEQ><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a);
-    else scan_token_kernel<E, BE, G, 1><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a);
+    scan_token_kernel<E, BE, G><<<(unsigned)blocks, TOKEN_THREADS, 0, stream>>>(a, per);
     return cudaGetLastError();
 }
 
