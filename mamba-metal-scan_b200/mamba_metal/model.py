@@ -9,6 +9,11 @@ residual sum after each block and the next norm as one kernel each way
 (`residual_rms_norm`), `fuse_loss` the head and its cross entropy without the
 logits (`linear_cross_entropy`); `TinyMamba.distill_loss` trains on a
 teacher's top k logits through the same head (`linear_distillation`).
+`fuse_conv` runs the convolution and its SiLU as one kernel each way
+(`causal_conv`). `TinyMamba.serve` takes prompts of unequal lengths and single
+tokens packed behind one another, with the blocks' states in a cache of places
+(`causal_conv_packed`, `selective_scan_packed`), and `TinyMamba.generate` draws from
+its logits (`sample_tokens`).
 
 Block (reference model.py:161-256):
     x -> RMSNorm -> in_proj -> (x, z)
@@ -34,8 +39,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from mamba_metal.conv import causal_conv, causal_conv_packed
 from mamba_metal.head import linear_cross_entropy, linear_distillation
 from mamba_metal.norm import residual_rms_norm
+from mamba_metal.packed import selective_scan_packed
+from mamba_metal.sampling import sample_tokens
 from mamba_metal.scan import (SSM_CHUNK, gated_output, selective_scan, selective_scan_proj,
                               selective_scan_step, selective_scan_step_ref)
 
@@ -64,6 +72,7 @@ class MambaConfig:
     # checkpointing by module).
     fuse_norm: bool = False   # residual sum + next norm as one CUDA kernel each way (residual_rms_norm)
     fuse_loss: bool = False   # with targets: no logits, forward returns (None, loss) (linear_cross_entropy)
+    fuse_conv: bool = False   # convolution + SiLU as one CUDA kernel each way, up to 8 taps (causal_conv)
 
 
 def transformer_block_params(d_model: int, d_ff: int) -> int:
@@ -176,6 +185,7 @@ class MambaBlock(nn.Module):
         self.scan_impl = cfg.scan_impl
         self.fuse_proj = cfg.fuse_proj
         self.fuse_gate = cfg.fuse_gate
+        self.fuse_conv = cfg.fuse_conv
         self.dt_min, self.dt_max = cfg.dt_min, cfg.dt_max
         self.norm = RMSNorm(dm, cfg.norm_eps)
         self.in_proj = nn.Linear(dm, 2 * d_inner, bias=False)
@@ -246,21 +256,33 @@ class MambaBlock(nn.Module):
         """The block between its norm and the residual sum."""
         x, z = self.in_proj(x).chunk(2, dim=-1)
         kc = self.conv.kernel_size[0]
+        fuse_conv = self.fuse_conv and x.is_cuda and self.scan_impl != "torch"
         if cache is not None and cache.get("h") is not None and x.shape[1] == 1:
             # one-token recurrent step against the cached conv window and state
-            window = torch.cat([cache["conv"], x.transpose(1, 2)], dim=2)   # (B, d_inner, kc)
-            x = F.silu(self.conv(window)[:, :, kc - 1:kc]).transpose(1, 2)
-            cache["conv"] = window[:, :, 1:]
+            if fuse_conv and not (torch.is_grad_enabled()
+                                  and any(t.requires_grad for t in (x, self.conv.weight, cache["conv"]))):
+                if not cache.get("conv_owned"):
+                    cache["conv"] = cache["conv"].clone(memory_format=torch.contiguous_format)
+                    cache["conv_owned"] = True
+                x = causal_conv_packed(x[:, 0], self.conv.weight, self.conv.bias, cache["conv"],
+                                       impl=self.scan_impl).unsqueeze(1)
+            else:
+                window = torch.cat([cache["conv"], x.transpose(1, 2)], dim=2)   # (B, d_inner, kc)
+                x = F.silu(self.conv(window)[:, :, kc - 1:kc]).transpose(1, 2)
+                cache["conv"], cache["conv_owned"] = window[:, :, 1:], False
             dt, B_t, C_t, Aneg = self._proj(x)
             y = self._step(x[:, 0], dt[:, 0], Aneg, B_t[:, 0], C_t[:, 0], cache).unsqueeze(1)
         else:
             xc = x.transpose(1, 2)
-            x = F.silu(self.conv(xc)[:, :, :xc.shape[2]]).transpose(1, 2)
+            if fuse_conv:
+                x = causal_conv(x, self.conv.weight, self.conv.bias, impl=self.scan_impl)
+            else:
+                x = F.silu(self.conv(xc)[:, :, :xc.shape[2]]).transpose(1, 2)
             if cache is not None:
                 tail = xc[:, :, -(kc - 1):]
                 if tail.shape[2] < kc - 1:
                     tail = F.pad(tail, (kc - 1 - tail.shape[2], 0))
-                cache["conv"] = tail
+                cache["conv"], cache["conv_owned"] = tail, False
             # the last checkpoint of the scan is h[:, -1]: the cache costs nothing
             y, h_last = self._scan(x, return_state=True)
             if cache is not None:
@@ -269,6 +291,16 @@ class MambaBlock(nn.Module):
             return self.out_proj(gated_output(y, z, self.D_skip, impl=self.scan_impl))
         y = y + self.D_skip
         return self.out_proj(y * F.silu(z))
+
+
+    def serve(self, x, cache, starts=None, slots=None, out_slots=None):
+        """mix on packed rows x (L, d_model) that go on from the states in cache, without gradients."""
+        x, z = self.in_proj(x).chunk(2, dim=-1)
+        lists = dict(starts=starts, slots=slots, out_slots=out_slots, impl=self.scan_impl)
+        x = causal_conv_packed(x, self.conv.weight, self.conv.bias, cache["conv"], **lists)
+        y = selective_scan_packed(x, self.dt_proj(x), self.A, self.B_proj(x), self.C_proj(x), cache["h"], z=z,
+                                  d_skip=self.D_skip, dt_range=(self.dt_min, self.dt_max), **lists)
+        return self.out_proj(y)
 
 
 class TinyMamba(nn.Module):
@@ -335,6 +367,66 @@ class TinyMamba(nn.Module):
         """
         return linear_distillation(self.hidden(idx), self.head.weight, teacher_index, teacher_logits,
                                    temperature, reduction, impl=self.cfg.scan_impl)
+
+    # ------------------------------------------------------------------- serving
+
+    def new_cache(self, places: int):
+        """States of `places` answers for `serve`, all zeros: what a sequence starts from."""
+        w = self.head.weight
+        kc, ds = self.cfg.d_conv, self.cfg.d_state
+        return {"blocks": [{"conv": w.new_zeros(places, self.d_inner, kc - 1),
+                            "h": w.new_zeros(places, self.d_inner, ds, dtype=torch.float32)} for _ in self.blocks]}
+
+    @torch.no_grad()
+    def serve(self, idx, cache, starts=None, slots=None, out_slots=None):
+        """Logits (S, vocab) behind the last token of each of S packed sequences.
+
+        idx (L,): the tokens of prompts, pieces of prompts and single tokens behind one
+        another, each sequence of at least one; cache from `new_cache`, updated in place; starts,
+        slots, out_slots as in `mamba_metal.packed` (without starts: one token a sequence). A
+        sequence whose slot is outside the cache starts anew.
+        """
+        x = self.tok(idx)
+        norms = [b.norm for b in self.blocks] + [self.ln_f]
+        u = norms[0](x)
+        for block, bc, norm in zip(self.blocks, cache["blocks"], norms[1:]):
+            y = block.serve(u, bc, starts, slots, out_slots)
+            if self.cfg.fuse_norm:
+                x, u = residual_rms_norm(x, y, norm.weight, eps=norm.eps, impl=self.cfg.scan_impl)
+            else:
+                x = x + y
+                u = norm(x)
+        if starts is not None:
+            u = u[(starts[1:].long() - 1).clamp(min=0)]
+        return self.head(u)
+
+    @torch.no_grad()
+    def generate(self, prompts, max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 uniform=None, generator=None):
+        """max_new_tokens tokens for each prompt, (S, max_new_tokens), drawn by `sample_tokens`.
+
+        prompts: S 1-D integer tensors of at least one token (of any lengths), or a 2-D tensor.
+        temperature, top_k, top_p, min_p: one number, or a tensor (S,). uniform
+        (max_new_tokens, S): the random numbers; None: torch.rand, with `generator`.
+        """
+        prompts = list(prompts)
+        device = self.head.weight.device
+        lens = [len(p) for p in prompts]
+        if not prompts or min(lens) < 1:
+            raise ValueError(f"generate needs prompts of at least one token; got lengths {lens}")
+        if uniform is None:
+            uniform = torch.rand(max_new_tokens, len(prompts), generator=generator, device=device, dtype=torch.float32)
+        if uniform.shape != (max_new_tokens, len(prompts)):
+            raise ValueError(f"uniform must be ({max_new_tokens}, {len(prompts)}); got {tuple(uniform.shape)}")
+        starts = torch.tensor([0, *lens]).cumsum(0).to(device=device, dtype=torch.int32)
+        cache = self.new_cache(len(prompts))
+        out = torch.empty(len(prompts), max_new_tokens, dtype=torch.int64, device=device)
+        idx = torch.cat([p.to(device) for p in prompts])
+        for i in range(max_new_tokens):
+            logits = self.serve(idx, cache, starts if i == 0 else None)
+            out[:, i] = sample_tokens(logits, uniform[i], temperature, top_k, top_p, min_p, impl=self.cfg.scan_impl)
+            idx = out[:, i].clamp(min=0)             # (-1, where no logit is a number, has no embedding)
+        return out
 
     def count_params(self) -> int:
         """Unique parameters (the tied head counts once)."""
