@@ -120,7 +120,7 @@ def causal_conv_packed_ref(x, weight, bias, window, starts=None, slots=None, out
     k = w.shape[1]
     y, left = torch.zeros_like(x), []
     for first, end, src, dst in places_of(x.shape[0], starts, slots, out_slots, window.shape[0]):
-        old = torch.zeros_like(x[:1]).expand(k - 1, -1) if src is None else window[src].t()
+        old = x.new_zeros(k - 1, x.shape[1]) if src is None else window[src].t()
         rows = torch.cat([old, x[first:end]])
         if end > first:
             y[first:end] = causal_conv_ref(rows[None], w, bias, silu)[0, k - 1:]

@@ -262,7 +262,7 @@ class MambaBlock(nn.Module):
             if fuse_conv and not (torch.is_grad_enabled()
                                   and any(t.requires_grad for t in (x, self.conv.weight, cache["conv"]))):
                 if not cache.get("conv_owned"):
-                    cache["conv"] = cache["conv"].clone(memory_format=torch.contiguous_format)
+                    cache["conv"] = cache["conv"][:, :, :kc - 1].clone(memory_format=torch.contiguous_format)
                     cache["conv_owned"] = True
                 x = causal_conv_packed(x[:, 0], self.conv.weight, self.conv.bias, cache["conv"],
                                        impl=self.scan_impl).unsqueeze(1)

@@ -212,13 +212,12 @@ def _nothing_packed(x, cache, count, slots, out_slots):
     the (empty) sequences still hand their states on; without places a cache cannot be named."""
     if x.shape[0] and cache.shape[0] == 0 and count and x.shape[1]:
         raise ValueError("the cache has no place; give it one, even where every sequence starts from nothing")
-    if count and cache.shape[0] and cache.numel() and out_slots is not None:
-        src = slots if slots is not None else torch.arange(count, device=x.device)
-        src, dst = src.long(), out_slots.long()
-        places = cache.shape[0]
+    if count and cache.numel() and out_slots is not None:
+        src = slots.long() if slots is not None else torch.arange(count, device=x.device)
+        places, lead = cache.shape[0], (-1,) + (1,) * (cache.dim() - 1)
+        old = torch.where(((src >= 0) & (src < places)).view(lead), cache[src.clamp(0, places - 1)],
+                          torch.zeros_like(cache[:1]))
         # every place takes what the sequence that names it goes on from; others keep theirs
-        hit = dst[:, None] == torch.arange(places, device=x.device)
-        who = hit.int().argmax(0)
-        old = cache[src.clamp(0, places - 1)] * ((src >= 0) & (src < places)).view(-1, *([1] * (cache.dim() - 1)))
-        cache.copy_(torch.where(hit.any(0).view(-1, *([1] * (cache.dim() - 1))), old[who], cache))
+        hit = out_slots.long()[:, None] == torch.arange(places, device=x.device)
+        cache.copy_(torch.where(hit.any(0).view(lead), old[hit.int().argmax(0)], cache))
     return torch.zeros_like(x, memory_format=torch.contiguous_format)

@@ -9,6 +9,8 @@ model's head gives the logits (`TinyMamba.generate` uses it); the reference stop
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from mamba_metal import _native
@@ -54,6 +56,7 @@ def sample_tokens_ref(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_
     bad = logits.isnan().any(1) | ~(top[:, 0] > -float("inf")) | t[:, 0].isnan() | p[:, 0].isnan()
     greedy = (t <= 0) | (k == 1) | (p <= 0)
     w = torch.where(top.isinf(), (z == top).double(), torch.exp((z - top) / torch.where(greedy, 1.0, t)))
+    w = torch.where(z == -float("inf"), 0.0, w)              # (at an infinite temperature too)
     place = torch.arange(vocab, device=device)
     w = torch.where((place < torch.where(k > 0, k, vocab)) & ~(greedy & (place > 0)), w, 0.0)
     ahead = torch.cumsum(w, 1) - w
@@ -96,6 +99,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
                          ("min_p", min_p, 0.0)):
         if not isinstance(v, torch.Tensor) and not v >= low:
             raise ValueError(f"{name} must not be negative; got {v}")
+    if not isinstance(top_k, torch.Tensor):
+        top_k = min(operator.index(top_k), logits.shape[-1])
     lead, vocab, device = logits.shape[:-1], logits.shape[-1], logits.device
     if not dispatch(impl, logits):
         for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
