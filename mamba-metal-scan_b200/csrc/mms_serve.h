@@ -1,5 +1,5 @@
 // Internal interface of the causal convolution (mms_conv.cu), the packed scan
-// (mms_packed.cu) and sampling (mms_sample.cu).
+// (mms_packed.cuh) and sampling (mms_sample.cu).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -103,6 +103,7 @@ struct ScanPackedArgs {
 
 size_t scan_packed_workspace_bytes(int rows, int count, int D, int N);
 cudaError_t launch_scan_packed(const ScanPackedArgs &a, cudaStream_t stream);
+cudaError_t launch_scan_packed_bf16(const ScanPackedArgs &a, cudaStream_t stream);   // its part with bf16 set
 
 struct SampleArgs {
     const void *logits;                 // (rows, vocab), row stride ld

@@ -154,7 +154,7 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     `selective_scan_proj`. Rows may be strided views. N is a multiple of 4 up to 64.
     Arithmetic and state are float32. Not differentiable: it is the inference path
     (`selective_scan` trains). On CUDA tensors 'auto', 'cuda', 'metal' run the kernels
-    (csrc/mms_packed.cu); elsewhere, or with 'torch', PyTorch ops.
+    (csrc/mms_packed.cuh); elsewhere, or with 'torch', PyTorch ops.
     """
     shape = x.shape
     if len(shape) != 2 or dt.shape != shape or aneg.dim() != 2 or aneg.shape[0] != shape[1]:
