@@ -49,6 +49,11 @@ constexpr int STAGES = 3;               // tiles of x, dt and z
 constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 flushes to 0
 constexpr int CTAS = 4;                 // an SM: what the registers hold
 constexpr int DIRECT = 2;               // rows that a segment takes straight from memory
+// A segment's state is chained from the ends of those before it, by each segment for itself or, in calls
+// with MANY whole segments and more, for sequences of more than CHAIN of them by a launch between the two.
+// (16384 x 256 x 16, one prompt, 256 segments: 96 us, without that launch 255; 4096 x 1024 x 16, 4
+// prompts, 73 segments: 80 and 92; 512 x 1432 x 16, one prompt, 16 segments: 43 and 39.)
+constexpr int MANY = 32, CHAIN = 4;
 
 template <typename E>
 struct Args {
@@ -65,6 +70,7 @@ struct Args {
     float *ends, *sums;                 // end states (row, D, N) and sums of dt (row, D) of segments
     float *entry;                       // (row, D, N) what sequences of several segments go on from
     int seg, nd;                        // rows of a segment, channel blocks
+    int chain;                          // sequences of more segments are joined by a launch
     int fulls, units;                   // units of whole segments, of all; the blocks behind them clear rows of no sequence
 };
 
@@ -525,21 +531,22 @@ scan_segments_kernel(const __grid_constant__ Args<E> a)
     read_rates<S>(nan2, a.aneg + at, a.N, g, channels, a.pj.on);
     float *entry = a.entry + u.row * DN + at;
     if (REST && u.i > 0) {
+        const bool joined = u.segs > a.chain;
+        read_states<S>(h, a.ends + (u.row + (joined ? u.i - 1 : 0)) * DN + at, a.N, g, channels);
         // the first segment's end, then of each one between what was left of it and its own
-        read_states<S>(h, a.ends + u.row * DN + at, a.N, g, channels);
-        constexpr int AHEAD = 3;                           // ends that are read at a time
-        for (int j = 1; j < u.i; j += AHEAD) {
-            States<S> v[AHEAD];
-            float2 sums[AHEAD];
+        constexpr int AT_ONCE = 3;                         // ends that are read at a time
+        for (int j = 1; j < u.i && !joined; j += AT_ONCE) {
+            States<S> v[AT_ONCE];
+            float2 sums[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
+            for (int k = 0; k < AT_ONCE; ++k) {
                 const int c = j + k < u.i ? channels : 0;
                 read_states<S>(v[k], a.ends + (u.row + j + k) * DN + at, a.N, g, c);
                 const float *s = a.sums + (size_t)(u.row + j + k) * a.D + d;
                 sums[k] = f2(c > 0 ? s[0] : 0.f, c > 1 ? s[1] : 0.f);
             }
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k)
+            for (int k = 0; k < AT_ONCE; ++k)
                 if (j + k < u.i) carry<S>(h, nan2, sums[k], v[k]);
         }
     } else {
@@ -578,6 +585,50 @@ scan_segments_kernel(const __grid_constant__ Args<E> a)
         carry<S>(h, nan2, total, v);
     }
     write_states<S>(h, a.ends + (u.row + u.i) * DN + at, a.N, g, channels);
+}
+
+// The ends of segments, each from nothing but a sequence's first, become states: h moved over a segment, and
+// what it leaves. A thread has four states of a channel; a block a sequence, or the one whose first
+// segment is its unit, whichever are fewer; AHEAD segments are on their way at a time.
+constexpr int JOIN_THREADS = 128, AHEAD = 12;
+template <typename E>
+__global__ void __launch_bounds__(JOIN_THREADS)
+scan_join_kernel(const __grid_constant__ Args<E> a, int blocks, bool by_sequence)
+{
+    Unit u;
+    if (by_sequence) {
+        const int s = blockIdx.x / blocks, start = a.seq.start(s);
+        u.row = start / a.seg, u.segs = (a.seq.start(s + 1) - start + a.seg - 1) / a.seg;
+        if (u.segs <= a.chain) return;
+    } else if (!find_unit(a, blockIdx.x / blocks, u) || u.i > 0 || u.segs <= a.chain) {
+        return;
+    }
+    const int e = (blockIdx.x % blocks * JOIN_THREADS + (int)threadIdx.x) * 4;      // of a place's D * N
+    const size_t DN = (size_t)a.D * a.N;
+    if (e >= (int)DN) return;
+    const int d = e / a.N;
+    float4 r = ld4(a.aneg + e);
+    if (a.pj.on) r = make_float4(softplus(r.x), softplus(r.y), softplus(r.z), softplus(r.w));
+    const float2 n0 = f2(-r.x * MMS_LOG2E, -r.y * MMS_LOG2E), n1 = f2(-r.z * MMS_LOG2E, -r.w * MMS_LOG2E);
+    float *end = a.ends + u.row * DN + e;
+    const float *sums = a.sums + (size_t)u.row * a.D + d;
+    const float4 first = *reinterpret_cast<const float4 *>(end);
+    float2 h0 = lo(first), h1 = hi(first);
+    const int n = u.segs - 1;
+    for (int j = 1; j < n; j += AHEAD) {
+        float4 v[AHEAD];
+        float s[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (j + k < n) v[k] = *reinterpret_cast<const float4 *>(end + (j + k) * DN), s[k] = sums[(size_t)(j + k) * a.D];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (j + k >= n) break;
+            h0 = fma2(ex2x2(mul2(f2(s[k], s[k]), n0)), h0, lo(v[k]));
+            h1 = fma2(ex2x2(mul2(f2(s[k], s[k]), n1)), h1, hi(v[k]));
+            st4(end + (j + k) * DN, make_float4(h0.x, h0.y, h1.x, h1.y));
+        }
+    }
 }
 
 // --------------------------------------------------------- single tokens
@@ -657,12 +708,15 @@ long long channel_blocks(int D, int N)
 }
 
 // Rows of a segment: as few as give every SM its CTAs when the rows belong to one sequence, at
-// least 64, a whole number of tiles. (Half of that: 337 for 292 us, 16384 x 2048 x 16.)
-int segment_rows(int rows, int D, int N)
+// least 32, a whole number of tiles. What is left of each sequence behind its whole segments comes
+// on top; where that is a quarter as many, half as many rows, for a shorter last wave. (16384 x 2048
+// x 16, one prompt: 276 us, with half as many rows 293; 8192 x 2304 x 16, 16 prompts: 202, with all of them 211.)
+int segment_rows(int rows, int count, int D, int N)
 {
     const long long nd = channel_blocks(D, N);
-    const long long want = std::max<long long>(1, (long long)CTAS * N_SM / nd);
-    const long long seg = std::max<long long>(64, (rows + want - 1) / want);
+    long long want = std::max<long long>(1, (long long)CTAS * N_SM / nd);
+    if (4LL * count > want) want *= 2;
+    const long long seg = std::max<long long>(32, (rows + want - 1) / want);
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
 }
 
@@ -674,7 +728,7 @@ struct Plan {
     long long nd, fulls, units;
     bool more;                          // a sequence can have a second segment
     size_t sums = 0, entry = 0, total = 0;
-    Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, D, N)) {
+    Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, count, D, N)) {
         nd = channel_blocks(D, N);
         fulls = rows / seg, units = fulls + count;
         more = rows > seg;
@@ -707,10 +761,12 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
     Args<E> a = args_of<E>(p);
     const Plan plan(p.seq.rows, p.seq.count, p.D, p.N);
     char *ws = static_cast<char *>(p.workspace);
-    a.seg = plan.seg, a.nd = (int)plan.nd, a.fulls = (int)plan.fulls, a.units = (int)plan.units;
+    a.seg = plan.seg, a.nd = (int)plan.nd, a.chain = plan.fulls >= MANY ? CHAIN : 0x7fffffff, a.fulls = (int)plan.fulls, a.units = (int)plan.units;
     a.ends = (float *)ws, a.sums = (float *)(ws + plan.sums), a.entry = (float *)(ws + plan.entry);
     const long long clear = 2 * N_SM, blocks = plan.units * plan.nd;
-    if (blocks + clear > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const long long sequences = std::min<long long>(plan.fulls, p.seq.count);      // that can have several segments
+    const int joins = (int)(((long long)p.D * p.N / 4 + JOIN_THREADS - 1) / JOIN_THREADS);
+    if (blocks + clear > 0x7fffffffLL || sequences * joins > 0x7fffffffLL) return cudaErrorInvalidValue;
     auto launch = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
         const size_t smem = (size_t)STAGES * TT * (a.z ? 3 : 2) * S::DPB * sizeof(E);
@@ -720,6 +776,11 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
         scan_segments_kernel<E, S, false, VEC><<<(unsigned)(blocks + clear), THREADS, smem, stream>>>(a);
         e = cudaGetLastError();
         if (e != cudaSuccess || !plan.more) return e;
+        if (plan.fulls >= MANY) {
+            scan_join_kernel<E><<<(unsigned)(sequences * joins), JOIN_THREADS, 0, stream>>>(a, joins, sequences < plan.fulls);
+            e = cudaGetLastError();
+            if (e != cudaSuccess) return e;
+        }
         scan_segments_kernel<E, S, true, VEC><<<(unsigned)blocks, THREADS, smem, stream>>>(a);
         return cudaGetLastError();
     };
