@@ -240,3 +240,18 @@ def test_refused_on_cuda():
             call(**kw)
     assert call(x=on["x"][:0], dt=on["dt"][:0], b_in=on["b_in"][:0], c_in=on["c_in"][:0], z=on["z"][:0],
                 starts=starts * 0).shape == (0, 8)
+
+
+@pytest.mark.parametrize("dtype,raw", [(F32, False), (F32, True), (BF16, True)])
+@pytest.mark.parametrize("d,n", [(40, 4), (33, 16), (24, 28), (17, 64)])
+@pytest.mark.parametrize("singles", [3, 150])
+def test_a_long_prompt_among_single_tokens(singles, d, n, dtype, raw):
+    """More segments than a segment chains by itself, beside fewer or more sequences than segments; the
+    short ones have 1, 2, 3 and no rows."""
+    lens = [(1, 2, 3, 0)[i % 4] for i in range(singles)] + [1600] + [(2, 1, 300)[i % 3] for i in range(singles)]
+    starts = torch.tensor([5] + lens).cumsum(0)
+    places = len(lens)
+    slots = torch.randperm(places, generator=torch.Generator().manual_seed(1))
+    slots[::7] = -1
+    t = make(int(starts[-1]) + 3, d, n, dtype, places=places, raw=raw, slow=0.01)
+    check(t, starts, slots, None)
