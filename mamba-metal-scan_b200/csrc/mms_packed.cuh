@@ -8,28 +8,32 @@
 // mamba_metal/model.py:203-221, 228-241).
 //
 // Prompts are bound by the exponentials, one a state and step (MUFU, 16 an SM and
-// clock). A thread holds up to 8 states of two neighbouring channels in registers; G = 1, 2, 4
-// or 8 lanes share the two, for up to 8, 16, 32 or 64 states. A
-// sequence is cut into segments of `seg` rows, so that one long prompt fills the GPU
-// as well as many short ones, whatever the lengths, which the host does not know:
-//   first   segments whose state is known, the first ones of short sequences, with their
-//           outputs; of the others but a sequence's last the state at the end from nothing
-//           and the sum of dt (a state's decay over the segment is exp(-Aneg sum dt));
-//   rest    all other segments with their outputs, each from the chain of the ends before it.
+// clock), and by the instructions and shared memory reads around them. A thread holds up to 8
+// states of two neighbouring channels in registers; G = 1, 2, 4 or 8 lanes share the two, for
+// up to 8, 16, 32 or 64 states. A sequence is cut into segments of `seg` rows, so that one long
+// prompt fills the GPU as well as many short ones, whatever the lengths, which the host does not know:
+//   first   sequences of one segment, with their outputs; of others' segments but the last
+//           the state at the end from nothing and the sum of dt (a state's decay over the
+//           segment is exp(-Aneg sum dt));
+//   join    (where there are many segments) the ends one after another become states;
+//   rest    the segments of the other sequences with their outputs, each from the state before it.
 // The ends are sums over the rows, v_n = sum_t exp(-Aneg_n sum_{t' > t} dt) dt_t B_tn x_t, from
 // the last row back: a state's rows are left out where the decay is flushed to 0
-// (below 2^-126), which leaves a quarter of the exponentials where dt is around 0.14
-// and Aneg 1 to 16. (Walking forward through all of them: 16384 x 2048 x 16, float32, 343 us.
-// Adding what enters a segment to outputs computed from nothing, with the same
-// exponentials left out: 313 us, 381 instead of 226 for 8192 x 2304 x 16 in bf16; it reads and
+// (below 2^-126), which leaves two fifths of the exponentials where dt is around 0.14
+// and Aneg 1 to 16. (Walking forward through all of them: 16384 x 2048 x 16, float32, 343 us;
+// adding what enters a segment to outputs computed from nothing, with the same
+// exponentials left out: 313 us, 381 instead of 226 for 8192 x 2304 x 16 in bf16, as it reads and
 // writes the outputs once more.)
 //
-// Unit u of a launch is segment i of sequence s with u = s + start_s / seg + i: as
-// a sequence of n rows has at most (start_s + n) / seg - start_s / seg + 1
-// segments, no two share a number, and a search over the starts finds s.
+// 16384 x 2048 x 16, float32, one prompt: 278 us (100 first, 175 rest: MUFU at 49 and 70 % of its
+// rate, 13 of 16 warps an SM that its registers allow). 8192 x 2304 x 16, bf16, 16 prompts: 205 us;
+// 3001 x 1433 x 64, 63 tokens and 7 prompts: 233 us (rest: MUFU 52 %, shared memory 70 %).
+// Not kept: a launch set up while the one before runs (griddepcontrol, 5 to 10 us slower: CTAs
+// that are to leave at once hold the places of others); more warps of fewer states.
 //
 // Single tokens without a list of starts are bound by the states' bytes, read and
-// written once: 4 states a lane, G lanes a channel.
+// written once: 4 states a lane, G lanes a channel. 256 x 2304 x 16: 22.4 us, 3.4 TB/s (75.5 MB; 5.4
+// warps an issue wait for memory, the ALUs are at 49 %).
 #pragma once
 
 #include <algorithm>
@@ -215,7 +219,7 @@ struct Ready {
 // bytes at a time a row, they take as long as the row's 16 exponentials
 // (shared memory returns 128 bytes a clock, 16 for the lanes of a quarter warp that all
 // read the same). All exponentials are MUFU's: with one, two or three of a thread's 8 pairs on the FMA pipe the
-// second launch took 184, 198 and 215 us, without 183 (16384 x 2048 x 16, float32).
+// second launch took 184, 198 and 215 us, without 183 (16384 x 2048 x 16, float32, at that time).
 template <bool VEC, bool GATE, bool RAW, typename E, typename S>
 __device__ __forceinline__ void walk(const Args<E> &a, float (*bc)[TT][2][S::NP], E *tiles, float *apart,
                                      States<S> &h, const States<S> &nan2, int t0, int t1, int d0)
@@ -397,7 +401,8 @@ __device__ __forceinline__ float2 leave(const Args<E> &a, float (*bc)[TT][1][S::
             R::template make<2>(tile, apart, 1, [&](int r, float v) { return t + r >= t0 ? step_of(a.pj, v) : 0.f; });
             __syncwarp();
         }
-        float2 sum[TT], bx[TT], least = total, most = total;
+        float2 sum[TT], bx[TT], least = f2(0.f, 0.f);
+        const float2 behind = total;                       // of the rows behind the tile
 #pragma unroll
         for (int j = TT - 1; j >= 0; --j) {
             float2 dtv;
@@ -405,23 +410,21 @@ __device__ __forceinline__ float2 leave(const Args<E> &a, float (*bc)[TT][1][S::
             else dtv = both(row + (2 * j + 1) * DPB);
             if (RAW && !DT) dtv = t + j >= t0 ? f2(step_of(a.pj, dtv.x), step_of(a.pj, dtv.y)) : f2(0.f, 0.f);
             sum[j] = total;                                // of the rows behind
-            least = f2(fminf(least.x, total.x), fminf(least.y, total.y));
-            most = f2(fmaxf(most.x, total.x), fmaxf(most.y, total.y));
+            least = f2(fminf(least.x, dtv.x), fminf(least.y, dtv.y));
             total = add2(total, dtv);
             bx[j] = mul2(dtv, both(row + 2 * j * DPB));
             bad_x = fma2(bx[j], f2(0.f, 0.f), bad_x);
         }
 #pragma unroll
         for (int q = 0; q < S::NPAIR; ++q) {
-            // the largest decay of the two channels' pairs in the tile
-            float top = __int_as_float(0xff800000);
+            // With no dt below 0 and a rate that is none either, the tile's largest decay is its last row's.
+            bool gone = fminf(least.x, least.y) >= 0.f;
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
-                const float lo1 = ch ? least.y : least.x, hi1 = ch ? most.y : most.x;
-                const float2 r = nan2[ch][q];
-                if (ch < channels) top = fmaxf(fmaxf(top, fmaxf(r.x * lo1, r.x * hi1)), fmaxf(r.y * lo1, r.y * hi1));
+                const float r = fmaxf(nan2[ch][q].x, nan2[ch][q].y), top = r * (ch ? behind.y : behind.x);
+                if (ch < channels) gone = gone && r <= 0.f && top < GONE;
             }
-            if (!__any_sync(0xffffffffu, S::state(g, q) < a.N && !(top < GONE))) continue;
+            if (!__any_sync(0xffffffffu, S::state(g, q) < a.N && channels && !gone)) continue;
 #pragma unroll
             for (int j = TT - 1; j >= 0; --j) {
                 const float2 Bv = *reinterpret_cast<const float2 *>(&bc[buf][j][0][g * S::NS + 2 * q]);
