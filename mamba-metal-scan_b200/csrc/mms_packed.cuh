@@ -54,9 +54,10 @@ constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 f
 constexpr int CTAS = 4;                 // an SM: what the registers hold
 constexpr int DIRECT = 2;               // rows that a segment takes straight from memory
 // A segment's state is chained from the ends of those before it, by each segment for itself or, in calls
-// with MANY whole segments and more, for sequences of more than CHAIN of them by a launch between the two.
-// (16384 x 256 x 16, one prompt, 256 segments: 96 us, without that launch 255; 4096 x 1024 x 16, 4
-// prompts, 73 segments: 80 and 92; 512 x 1432 x 16, one prompt, 16 segments: 43 and 39.)
+// with MANY more whole segments than sequences, for sequences of more than CHAIN of them by a launch between the
+// two. (16384 x 256 x 16, one prompt, 256 segments: 96 us, without that launch 255; 4096 x 1024 x 16, 4
+// prompts, 73 segments: 76 and 92; 512 x 1432 x 16, one prompt, 16 segments: 43 and 39; 8192 x 2304 x
+// 16, 16 prompts, 32 segments: 224 and 211.)
 constexpr int MANY = 32, CHAIN = 4;
 
 template <typename E>
@@ -711,14 +712,13 @@ long long channel_blocks(int D, int N)
 }
 
 // Rows of a segment: as few as give every SM its CTAs when the rows belong to one sequence, at
-// least 32, a whole number of tiles. What is left of each sequence behind its whole segments comes
-// on top; where that is a quarter as many, half as many rows, for a shorter last wave. (16384 x 2048
-// x 16, one prompt: 276 us, with half as many rows 293; 8192 x 2304 x 16, 16 prompts: 202, with all of them 211.)
-int segment_rows(int rows, int count, int D, int N)
+// least 32, a whole number of tiles. (Half as many: 16384 x 2048 x 16, one prompt, 293 for 276 us; 8192 x
+// 2304 x 16, 16 prompts of four draws, 212 for 205; 16384 x 2048 x 16, 32 prompts, bf16, 414 for 426. At least 64: 2048 x 1432 x
+// 16, one prompt, 78 for 66 us.)
+int segment_rows(int rows, int D, int N)
 {
     const long long nd = channel_blocks(D, N);
-    long long want = std::max<long long>(1, (long long)CTAS * N_SM / nd);
-    if (4LL * count > want) want *= 2;
+    const long long want = std::max<long long>(1, (long long)CTAS * N_SM / nd);
     const long long seg = std::max<long long>(32, (rows + want - 1) / want);
     return (int)std::min<long long>((seg + TT - 1) / TT * TT, 1 << 30);
 }
@@ -731,7 +731,7 @@ struct Plan {
     long long nd, fulls, units;
     bool more;                          // a sequence can have a second segment
     size_t sums = 0, entry = 0, total = 0;
-    Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, count, D, N)) {
+    Plan(int rows, int count, int D, int N) : seg(segment_rows(rows, D, N)) {
         nd = channel_blocks(D, N);
         fulls = rows / seg, units = fulls + count;
         more = rows > seg;
@@ -764,7 +764,8 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
     Args<E> a = args_of<E>(p);
     const Plan plan(p.seq.rows, p.seq.count, p.D, p.N);
     char *ws = static_cast<char *>(p.workspace);
-    a.seg = plan.seg, a.nd = (int)plan.nd, a.chain = plan.fulls >= MANY ? CHAIN : 0x7fffffff, a.fulls = (int)plan.fulls, a.units = (int)plan.units;
+    const bool joined = plan.fulls >= MANY + p.seq.count;
+    a.seg = plan.seg, a.nd = (int)plan.nd, a.chain = joined ? CHAIN : 0x7fffffff, a.fulls = (int)plan.fulls, a.units = (int)plan.units;
     a.ends = (float *)ws, a.sums = (float *)(ws + plan.sums), a.entry = (float *)(ws + plan.entry);
     const long long clear = 2 * N_SM, blocks = plan.units * plan.nd;
     const long long sequences = std::min<long long>(plan.fulls, p.seq.count);      // that can have several segments
@@ -779,7 +780,7 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
         scan_segments_kernel<E, S, false, VEC><<<(unsigned)(blocks + clear), THREADS, smem, stream>>>(a);
         e = cudaGetLastError();
         if (e != cudaSuccess || !plan.more) return e;
-        if (plan.fulls >= MANY) {
+        if (joined) {
             scan_join_kernel<E><<<(unsigned)(sequences * joins), JOIN_THREADS, 0, stream>>>(a, joins, sequences < plan.fulls);
             e = cudaGetLastError();
             if (e != cudaSuccess) return e;

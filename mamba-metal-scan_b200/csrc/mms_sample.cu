@@ -19,8 +19,8 @@
 // A row is read by a cluster of C CTAs; warp q of all of theirs has the q-th piece of the
 // row in every pass, so that sums in index order are sums over warps.
 //   k up to about 256 C: every warp has the j-th largest of its 32 lanes' maxima, j = k / warps
-//     rounded up; the smallest of these has k entries above it or equal, and not many
-//     more. Those are listed and sorted, and all else happens on the list.
+//     rounded up; the m-th largest of these, m = k / j rounded up, has k entries above it or
+//     equal, and not many more. Those are listed and sorted, and all else happens on the list.
 //   else: the end of the run of k entries, or of the mass p, is found by bins over the
 //     range of the logits, counts and weights of 2048 equal bins. If the entries down to the bin in
 //     question fit the list, all else happens there; otherwise that bin becomes the range,
@@ -53,6 +53,7 @@ constexpr int BINS = 2048;
 constexpr int CAP = 2048;               // entries that are sorted rather than divided further
 constexpr int PER = BINS / THREADS;     // bins, and list entries, of a thread
 static_assert(CAP == BINS, "one scan serves both");
+constexpr int RANKED = 128;             // entries that are sorted by counting, at most
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr int BITS = 44;                // of weights, fewer above 2^18 entries
 constexpr int LIMBS_MAX = 1 << 17;      // entries whose weights' 15-bit parts add up in 32 bits
@@ -121,6 +122,7 @@ struct Shared {
     u64 warp_sum[NW];                   // of the CTA's warps
     u64 all_sum[8 * NW];                // of all the row's warps
     float warp_max[NW], warp_pivot[NW], warp_lo[NW], warp_hi[NW];
+    float all_pivot[8 * NW], pivot;
     u64 before;                         // what lies before the bin in question
     u64 scan[NW];
     int listed, bin, least, tau_key, ti, others_count;
@@ -368,6 +370,18 @@ __device__ __forceinline__ float row_fold(float (&mine)[NW], float v, F f)
 // The first n entries of sh.list sorted ascending (behind them: ones, up to a power of two).
 __device__ void sort_list(u64 *list, int n)
 {
+    if (n <= RANKED) {                                     // every entry's place by counting
+        __syncthreads();
+        const int i = threadIdx.x;
+        const u64 mine = i < n ? list[i] : 0;
+        int place = 0;
+        if (i < n)
+            for (int q = 0; q < n; ++q) place += list[q] < mine || (list[q] == mine && q < i);
+        __syncthreads();
+        if (i < n) list[place] = mine;
+        __syncthreads();
+        return;
+    }
     int m = 2;
     while (m < n) m *= 2;
     for (int i = n + threadIdx.x; i < m; i += THREADS) list[i] = ~0ull;
@@ -801,8 +815,8 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
     const float min_p = fminf(s.min_p ? s.min_p[at] : s.min_p1, 1.f);
-    // k entries at least are as large as the smallest of the warps' j-th largest of their lanes'
-    // maxima, of those warps whose pieces are whole
+    // k entries at least are as large as the m-th largest of the warps' j-th largest of their lanes'
+    // maxima, m j >= k; with j from the pieces that are whole there are m warps
     const int pieces = max(1, row.end / row.piece);
     const int j = (int)min((k + pieces - 1) / pieces, 1000ll);
     const bool listed = k > 1 && k < s.vocab && j <= 16;
@@ -837,7 +851,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
             const unsigned has = __ballot_sync(0xffffffffu, mine == best);
             if (lane == __ffs(has) - 1) mine = 0;
         }
-        if (lane == 0) sh.warp_pivot[warp] = w >= pieces ? -NEG_INF : best ? of_key(best) : NEG_INF;
+        if (lane == 0) sh.warp_pivot[warp] = best ? of_key(best) : NEG_INF;
     }
     row.top = row_fold<C>(sh.warp_max, most, [](float x, float y) { return max_nan(x, y); });
     row.rate = 1.0 / (double)t;
@@ -863,9 +877,18 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     }
     const u64 least = min_p > 0.f ? (u64)ceil(ldexp((double)min_p, row.bits)) : 0;
     if (listed) {
-        float pivot = of_rank<C>(sh.warp_pivot, (lane % (C * NW)) / NW)[lane % NW];
-        for (int i = lane + 32; i < C * NW; i += 32) pivot = fminf(pivot, of_rank<C>(sh.warp_pivot, i / NW)[i % NW]);
-        pivot = warp_fold(pivot, [](float x, float y) { return fminf(x, y); });
+        const int m = ((int)k + j - 1) / j;
+        if (tid < C * NW) sh.all_pivot[tid] = of_rank<C>(sh.warp_pivot, tid / NW)[tid % NW];
+        __syncthreads();
+        if (tid < C * NW) {
+            const float mine = sh.all_pivot[tid];
+            int above = 0;
+#pragma unroll 8
+            for (int q = 0; q < C * NW; ++q) above += sh.all_pivot[q] > mine || (sh.all_pivot[q] == mine && q < tid);
+            if (above == m - 1) sh.pivot = mine;
+        }
+        __syncthreads();
+        const float pivot = sh.pivot;
         row.each([&](float v, int i) {
             if (v >= pivot) to_list(sh, v, i);
         });
