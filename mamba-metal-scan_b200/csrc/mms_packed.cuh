@@ -27,7 +27,7 @@
 //
 // 16384 x 2048 x 16, float32, one prompt: 278 us (100 first, 175 rest: MUFU at 49 and 70 % of its
 // rate, 13 of 16 warps an SM that its registers allow). 8192 x 2304 x 16, bf16, 16 prompts: 205 us;
-// 3001 x 1433 x 64, 63 tokens and 7 prompts: 233 us (rest: MUFU 52 %, shared memory 70 %).
+// 3001 x 1433 x 64, 63 tokens and 7 prompts: 227 us (rest: MUFU 52 %, shared memory 70 %).
 // Not kept: a launch set up while the one before runs (griddepcontrol, 5 to 10 us slower: CTAs
 // that are to leave at once hold the places of others); more warps of fewer states.
 //

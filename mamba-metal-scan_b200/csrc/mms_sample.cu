@@ -367,7 +367,7 @@ __device__ __forceinline__ float row_fold(float (&mine)[NW], float v, F f)
     return warp_fold(v, f);
 }
 
-// The first n entries of sh.list sorted ascending (behind them: ones, up to a power of two).
+// The first n entries of sh.list sorted ascending (behind them: ones, up to a power of two, or what was there).
 __device__ void sort_list(u64 *list, int n)
 {
     if (n <= RANKED) {                                     // every entry's place by counting
@@ -382,18 +382,50 @@ __device__ void sort_list(u64 *list, int n)
         __syncthreads();
         return;
     }
-    int m = 2;
+    // A bitonic network of m entries, four of them in a thread's registers: steps of 1 and 2 entries
+    // there, up to 64 between the lanes of a warp, from 128 on (10 of 66 steps for 2048) in shared memory.
+    int m = 256;
     while (m < n) m *= 2;
-    for (int i = n + threadIdx.x; i < m; i += THREADS) list[i] = ~0ull;
-    for (int size = 2; size <= m; size *= 2)
-        for (int gap = size / 2; gap > 0; gap /= 2) {
+    __syncthreads();
+    const int t = threadIdx.x;
+    const bool in = t < m / 4;                             // (whole warps)
+    ulonglong2 *mine = reinterpret_cast<ulonglong2 *>(list) + 2 * t;
+    u64 v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = in && 4 * t + e < n ? list[4 * t + e] : ~0ull;
+    auto keep = [](u64 &x, u64 other, bool low) { x = low == (other < x) ? other : x; };
+    auto order = [](u64 &x, u64 &y, bool up) {
+        const bool swap = (y < x) == up;
+        const u64 a = swap ? y : x, b = swap ? x : y;
+        x = a, y = b;
+    };
+#pragma unroll 1
+    for (int size = 2; size <= m; size *= 2) {
+        const bool up = (4 * t & size) == 0;
+#pragma unroll 1
+        for (int gap = size / 2; gap >= 128; gap /= 2) {
             __syncthreads();
-            for (int i = threadIdx.x; i < m / 2; i += THREADS) {
-                const int a = 2 * i - (i & (gap - 1)), b = a + gap;
-                const u64 x = list[a], y = list[b];
-                if ((x > y) == ((a & size) == 0)) list[a] = y, list[b] = x;
+            if (in) mine[0] = make_ulonglong2(v[0], v[1]), mine[1] = make_ulonglong2(v[2], v[3]);
+            __syncthreads();
+            if (in) {
+                const ulonglong2 *other = reinterpret_cast<const ulonglong2 *>(list) + 2 * (t ^ gap / 4);
+                const ulonglong2 a = other[0], b = other[1];
+                const bool low = ((t & gap / 4) == 0) == up;
+                keep(v[0], a.x, low), keep(v[1], a.y, low), keep(v[2], b.x, low), keep(v[3], b.y, low);
             }
         }
+        if (!in) continue;
+#pragma unroll 1
+        for (int gap = min(size / 2, 64); gap >= 4; gap /= 2) {
+            const bool low = ((t & gap / 4) == 0) == up;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) keep(v[e], __shfl_xor_sync(0xffffffffu, v[e], gap / 4), low);
+        }
+        if (size > 2) order(v[0], v[2], up), order(v[1], v[3], up);
+        order(v[0], v[1], up), order(v[2], v[3], size > 2 && up);
+    }
+    __syncthreads();
+    if (in) mine[0] = make_ulonglong2(v[0], v[1]), mine[1] = make_ulonglong2(v[2], v[3]);
     __syncthreads();
 }
 // List entries that sort by rank (z descending, index ascending), and by index.
