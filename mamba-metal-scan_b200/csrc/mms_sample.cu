@@ -25,10 +25,13 @@
 //     range of the logits, counts and weights of 2048 equal bins. If the entries down to the bin in
 //     question fit the list, all else happens there; otherwise that bin becomes the range,
 //     until it holds one value or few enough entries to sort, and another pass draws.
-//   bf16, where k is not small: a row has few different values, so one pass counts each of 5633 of them
-//     (magnitudes 2^-16 to 64 and 0; the others are listed one by one), and every cut and sum
-//     follows from the counts; one more pass, with the weights from a table, draws. Only where a cut
-//     falls among the values that are not counted, or too many are not, the bins above find it.
+//   bf16, where k is not small or there is a p, and a row has one or two CTAs: there are few different values, so
+//     one pass counts each of 5633 of them (magnitudes 2^-16 to 64 and 0; the others are listed one by one),
+//     and every cut and sum follows from the counts; one more pass, with the weights from a
+//     table, draws. Only where a cut falls among the values that are not counted, or too many are
+//     not, the bins above find it. (p = 0.9: 256 x 131072 by one CTA 141 us, by bins 283; 60 x 20000 by
+//     two 39 and 53. By eight the tables cost more than their part of a row: 1 x 32768 49 and 41. Without a
+//     cut the table loses too: 60 x 131072, 45 us and 34.)
 // The row is read from HBM once; the later passes, one to five, find it in L2. What bounds a
 // pass over all weights is their arithmetic (12 operations in float64 and some 30 others an
 // entry), not the bytes.
@@ -700,44 +703,42 @@ __device__ bool value_reached(Shared &sh, u64 target, F value)
     return all >= target;
 }
 
-// Weights by value (sh.table) and, where there are `cuts`, what the row keeps, from the counts of its values
-// (sh.found of this CTA's part, sh.others). False where a cut falls into a gap.
+// Weights by value (sh.table) and what the row keeps, from the counts of its values (sh.found of
+// this CTA's part, sh.others). False where a cut falls into a gap.
 template <typename E, int C>
-__device__ bool cut_counted(Shared &sh, Row<E, C> &row, bool cuts, long long k, float top_p, u64 least)
+__device__ bool cut_counted(Shared &sh, Row<E, C> &row, long long k, float top_p, u64 least)
 {
     const int tid = threadIdx.x;
     for (int i = tid; i < VALUES; i += THREADS) sh.table[slot_at(i)] = is_gap(i) ? 0 : row.weight(value_at(i));
     __syncthreads();
-    if (cuts) {
-        for (int i = tid; i < sh.others_count; i += THREADS) {
-            const int slot = gap_slot(__float_as_uint(sh.others[i]) >> 16);
-            atomicAdd(&sh.table[slot], row.weight(sh.others[i]));
-            atomicAdd(&sh.found[slot], 1u);
+    for (int i = tid; i < sh.others_count; i += THREADS) {
+        const int slot = gap_slot(__float_as_uint(sh.others[i]) >> 16);
+        atomicAdd(&sh.table[slot], row.weight(sh.others[i]));
+        atomicAdd(&sh.found[slot], 1u);
+    }
+    row_sync<C>();
+    if constexpr (C > 1) {
+        // the whole row's, into registers, then back
+        unsigned n[PER_VALUE];
+        u64 gap = 0;
+#pragma unroll
+        for (int q = 0; q < PER_VALUE; ++q) {
+            const int i = tid + q * THREADS;
+            n[q] = 0;
+            if (i < VALUES)
+                for (int r = 0; r < C; ++r) n[q] += of_rank<C>(sh.found, r)[i];
         }
+        if (tid < VALUES - 2 * CORE - 1)
+            for (int r = 0; r < C; ++r) gap += of_rank<C>(sh.table, r)[2 * CORE + 1 + tid];
         row_sync<C>();
-        if constexpr (C > 1) {
-            // the whole row's, into registers, then back
-            unsigned n[PER_VALUE];
-            u64 gap = 0;
 #pragma unroll
-            for (int q = 0; q < PER_VALUE; ++q) {
-                const int i = tid + q * THREADS;
-                n[q] = 0;
-                if (i < VALUES)
-                    for (int r = 0; r < C; ++r) n[q] += of_rank<C>(sh.found, r)[i];
-            }
-            if (tid < VALUES - 2 * CORE - 1)
-                for (int r = 0; r < C; ++r) gap += of_rank<C>(sh.table, r)[2 * CORE + 1 + tid];
-            row_sync<C>();
-#pragma unroll
-            for (int q = 0; q < PER_VALUE; ++q)
-                if (tid + q * THREADS < VALUES) sh.found[tid + q * THREADS] = n[q];
-            if (tid < VALUES - 2 * CORE - 1) sh.table[2 * CORE + 1 + tid] = gap;
-            __syncthreads();
-        }
+        for (int q = 0; q < PER_VALUE; ++q)
+            if (tid + q * THREADS < VALUES) sh.found[tid + q * THREADS] = n[q];
+        if (tid < VALUES - 2 * CORE - 1) sh.table[2 * CORE + 1 + tid] = gap;
+        __syncthreads();
     }
     int last = VALUES - 1;                                 // the last place that is kept, and how many of it
-    unsigned of_last = cuts ? sh.found[slot_at(last)] : 1;
+    unsigned of_last = sh.found[slot_at(last)];
     auto kept_of = [&](int i) -> u64 { return i < last ? sh.found[slot_at(i)] : i == last ? of_last : 0; };
     // the run ends in place sh.bin with `need` of its entries
     auto end_at = [&](u64 need) {
@@ -746,7 +747,7 @@ __device__ bool cut_counted(Shared &sh, Row<E, C> &row, bool cuts, long long k, 
         last = sh.bin;
         return true;
     };
-    if (cuts && k > 0 && k < row.end - row.off && value_reached(sh, (u64)k, [&](int i) { return (u64)sh.found[slot_at(i)]; }))
+    if (k > 0 && k < row.end - row.off && value_reached(sh, (u64)k, [&](int i) { return (u64)sh.found[slot_at(i)]; }))
         if (!end_at((u64)k - sh.before)) return false;
     if (top_p < 1.f) {
         auto weight = [&](int i) -> u64 {
@@ -867,14 +868,14 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     const int pieces = max(1, row.end / row.piece);
     const int j = (int)min((k + pieces - 1) / pieces, 1000ll);
     const bool listed = k > 1 && k < s.vocab && j <= 16;
-    const bool cuts = (k > 0 && k < s.vocab) || top_p < 1.f;
-    bool counted = sizeof(E) == 2 && !listed && k != 1 && t > 0.f && top_p > 0.f;
-    if (counted && cuts)
+    constexpr bool MAY_COUNT = sizeof(E) == 2 && C <= 2;
+    bool counted = MAY_COUNT && ((k > 0 && k < s.vocab) || top_p < 1.f) && !listed && k != 1 && t > 0.f && top_p > 0.f;
+    if (counted)
         for (int i = tid; i < VALUES; i += THREADS) sh.found[i] = 0;
     __syncthreads();
     // the largest value (NaN if there is one)
     float most = NEG_INF;
-    if (counted && cuts) {
+    if (counted) {
         row.template words<1>(row.from(w), row.from(w + 1), [&](const Words<E> &v, int) {
             most = max_nan(most, v.most());
 #pragma unroll
@@ -945,9 +946,9 @@ sample_kernel(const __grid_constant__ SampleArgs s)
             return;
         }
     }
-    if (counted) {
+    if constexpr (MAY_COUNT) {
         for (int r = 0; r < C; ++r) counted = counted && *of_rank<C>(&sh.others_count, r) <= CAP;
-        counted = counted && !isinf(row.top) && cut_counted(sh, row, cuts, k, top_p, least);
+        counted = counted && !isinf(row.top) && cut_counted(sh, row, k, top_p, least);
     }
     if (!counted) {
         row_sync<C>();                                     // what was counted gives way to bins
