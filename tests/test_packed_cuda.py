@@ -255,3 +255,32 @@ def test_a_long_prompt_among_single_tokens(singles, d, n, dtype, raw):
     slots[::7] = -1
     t = make(int(starts[-1]) + 3, d, n, dtype, places=places, raw=raw, slow=0.01)
     check(t, starts, slots, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sequences_of_whole_segments(dtype):
+    """Lengths at and beside multiples of a segment (32 rows here), few and many of them, and a captured call
+    replayed with other starts."""
+    lens = [32, 64, 31, 33, 128, 1, 160, 0, 1600, 96, 65]
+    starts = torch.tensor([0] + lens).cumsum(0)
+    slots = torch.tensor([3, 1, -1, 0, 10, 9, 2, 4, 5, 6, 7])
+    rows = int(starts[-1])
+    t = make(rows, 64, 16, dtype, places=11, slow=0.02)
+    check(t, starts, slots, None)
+    check(t, torch.tensor([0, 32 * 68, rows]), torch.tensor([3, -1]), torch.tensor([3, 2]))
+    check(t, torch.tensor([0] * 5 + [rows] * 7), slots, None)
+    on = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in t.items()}
+    lists = [starts.to(DEV), slots.to(DEV)]
+    on["state"] = t["state"].clone().to(DEV)
+    call = lambda: selective_scan_packed(starts=lists[0], slots=lists[1], **on)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    other = torch.tensor([0, 700, 700, 701, 760, 1000, 1032, 1064, 1500, 1501, 1502, rows])
+    lists[0].copy_(other)
+    on["state"].copy_(t["state"])
+    graph.replay()
+    got, state = y.clone(), on["state"].clone()
+    want, want_state = run(t, other, slots, None)
+    assert torch.equal(got, want) and torch.equal(state, want_state)
