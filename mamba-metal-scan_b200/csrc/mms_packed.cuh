@@ -42,6 +42,7 @@
 #include "mms_common.cuh"
 #include "mms_serve.h"
 #include "mms_stage.cuh"
+#include "mms_units.h"
 
 namespace mms {
 
@@ -93,27 +94,12 @@ struct Split {
 template <typename S>
 using States = float2[2][S::NPAIR];
 
-// What a CTA of a segment's launch is to do. First the whole segments, unit start / seg + i the i-th of
-// its sequence (another one starts at least as many whole `seg` behind), then what is left of each
-// sequence, so that a launch does not end with long ones. (In the order of the rows:
-// 158 + 151 for 91 + 117 us, 63 single tokens and 7 prompts, 3001 x 1433 x 64, float32.)
-struct Unit {
-    int s, i, segs, t0, t1;             // sequence, segment of how many, rows
-    int row;                            // of the sequence in the workspace
-};
 template <typename E>
 __device__ __forceinline__ bool find_unit(const Args<E> &a, int unit, Unit &u)
 {
-    const bool whole = unit < a.fulls;
-    u.s = whole ? Sequences::last_at_most(a.seq.count, unit, [&](int i) { return a.seq.start(i) / a.seg; }) : unit - a.fulls;
-    if (u.s < 0) return false;
-    const int first = a.seq.start(u.s), end = max(first, a.seq.start(u.s + 1));
-    const int full = (end - first) / a.seg;
-    u.row = first / a.seg;
-    u.i = whole ? unit - u.row : full;
-    u.segs = max(1, (end - first + a.seg - 1) / a.seg);
-    u.t0 = first + u.i * a.seg, u.t1 = whole ? u.t0 + a.seg : end;
-    return u.i < (whole ? full : u.segs);
+    const int s = unit < a.fulls ? Sequences::last_at_most(a.seq.count, unit, [&](int i) { return a.seq.start(i) / a.seg; })
+                                 : unit - a.fulls;
+    return s >= 0 && unit_rows(unit, a.fulls, a.seg, s, a.seq.start(s), a.seq.start(s + 1), u);
 }
 
 // An element of B or C.
