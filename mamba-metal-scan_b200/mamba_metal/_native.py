@@ -481,7 +481,7 @@ def _scan_packed_workspace(rows: int, count: int, d: int, n: int) -> int:
 def scan_packed(x, dt, aneg, b_in, c_in, z, d_skip, dt_range, state, starts, slots, out_slots, count: int):
     """y of mms_scan_packed, state updated; x, dt, b_in, c_in, z as (tensor, row stride)."""
     (x, ldx), (dt, lddt), (b_in, ldb), (c_in, ldc) = x, dt, b_in, c_in
-    z, ldz = (0, 0) if z is None else (z[0].data_ptr(), z[1])
+    z, ldz = (None, 0) if z is None else z               # (the tensor: it may be a copy that nothing else holds)
     n_rows, d = x.shape
     n = aneg.shape[1]
     device = x.device
@@ -490,7 +490,7 @@ def scan_packed(x, dt, aneg, b_in, c_in, z, d_skip, dt_range, state, starts, slo
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
     lo, hi = (0.0, 0.0) if dt_range is None else dt_range
     rc = load().mms_scan_packed(x.data_ptr(), ldx, dt.data_ptr(), lddt, aneg.data_ptr(), b_in.data_ptr(), ldb,
-                                c_in.data_ptr(), ldc, z, ldz, _opt(d_skip), dt_range is not None, lo, hi,
+                                c_in.data_ptr(), ldc, _opt(z), ldz, _opt(d_skip), dt_range is not None, lo, hi,
                                 state.data_ptr(), state.shape[0], _opt(starts), _opt(slots), _opt(out_slots),
                                 _wide(starts, slots, out_slots), y.data_ptr(), _opt(ws), nb, n_rows, count, d, n,
                                 _dtype(x), _dtype(b_in), _stream(device))
