@@ -384,8 +384,11 @@ class TinyMamba(nn.Module):
         idx (L,): the tokens of prompts, pieces of prompts and single tokens behind one
         another, each sequence of at least one; cache from `new_cache`, updated in place; starts,
         slots, out_slots as in `mamba_metal.packed` (without starts: one token a sequence). A
-        sequence whose slot is outside the cache starts anew.
+        sequence whose slot is outside the cache starts anew. An empty one's logits are some
+        other row's.
         """
+        if starts is not None and starts.dim() == 1 and starts.shape[0] > 1 and idx.shape[0] == 0:
+            raise ValueError(f"serve needs a token of each of {starts.shape[0] - 1} sequences; idx is empty")
         x = self.tok(idx)
         norms = [b.norm for b in self.blocks] + [self.ln_f]
         u = norms[0](x)
@@ -397,7 +400,8 @@ class TinyMamba(nn.Module):
                 x = x + y
                 u = norm(x)
         if starts is not None:
-            u = u[(starts[1:].long() - 1).clamp(min=0)]
+            # (a gather outside the rows would be a device assertion, which ends the process's CUDA calls)
+            u = u[(starts[1:].long() - 1).clamp(0, max(0, u.shape[0] - 1))]
         return self.head(u)
 
     @torch.no_grad()

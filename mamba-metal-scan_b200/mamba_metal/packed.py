@@ -97,8 +97,9 @@ def rows_of(t, group: int = 1):
 
 
 def places_of(rows: int, starts, slots, out_slots, places: int):
-    """[(first, end, from, to)] of each sequence, on the host; from and to None for no place."""
-    bounds = range(rows + 1) if starts is None else starts.tolist()
+    """[(first, end, from, to)] of each sequence, on the host; from and to None for no place. Starts that
+    break the rules are brought into the rows as in the kernels."""
+    bounds = range(rows + 1) if starts is None else [min(max(v, 0), rows) for v in starts.tolist()]
     count = len(bounds) - 1
     src = list(range(count)) if slots is None else slots.tolist()
     dst = src if out_slots is None else out_slots.tolist()
@@ -106,7 +107,7 @@ def places_of(rows: int, starts, slots, out_slots, places: int):
     def inside(p):
         return p if 0 <= p < places else None
 
-    return [(bounds[s], bounds[s + 1], inside(src[s]), inside(dst[s])) for s in range(count)]
+    return [(bounds[s], max(bounds[s], bounds[s + 1]), inside(src[s]), inside(dst[s])) for s in range(count)]
 
 
 # --------------------------------------------------------------------- the scan
