@@ -1007,8 +1007,8 @@ sample_kernel(const __grid_constant__ SampleArgs s)
                     mass += heavy(queue[lane]);
                     const float rest = queue[32 + lane];
                     __syncwarp();
-                    queue[lane] = rest;
                     waiting -= 32;
+                    if (lane < waiting) queue[lane] = rest;          // (the places behind are the next entries')
                 }
             }
         });
