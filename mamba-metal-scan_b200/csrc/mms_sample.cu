@@ -904,7 +904,8 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     row.top = row_fold<C>(sh.warp_max, most, [](float x, float y) { return max_nan(x, y); });
     row.rate = 1.0 / (double)t;
     row.limit = (double)fminf(row.top, FLT_MAX);
-    row.floor = isinf(row.top) ? below(FLT_MAX)
+    // (beside +inf not even FLT_MAX, as which an infinite logit is computed, has weight)
+    row.floor = isinf(row.top) ? FLT_MAX
                                : fminf(below(row.top), __double2float_rd(row.limit - 34.0 * (double)t));
     // nothing to draw from, or nothing to draw
     const bool none = !(row.top > NEG_INF) || t != t || top_p != top_p;
