@@ -398,7 +398,7 @@ int mms_scan_packed(const void *x, long long ldx, const void *dt, long long lddt
  * Equal logits rank by lowest index. Settings come from device arrays of one value a row
  * or, where those are NULL, from the value behind them; top_k from 64-bit
  * numbers if top_k_wide. temperature <= 0: the largest logit. A row with a
- * NaN, or without a logit above -inf, gives -1. logprob (NULL: not wanted): the log of
+ * NaN among its logits or settings, or without a logit above -inf, gives -1. logprob (NULL: not wanted): the log of
  * w_token over their sum, NaN beside -1. Weights are float64 rounded to whole numbers of
  * 2^-44 of the largest (2^-(62 - log2 vocab) above 2^18 entries), their sums exact.
  * uniform is taken into [0, 1 - 2^-24].

@@ -862,7 +862,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     const float t = s.temperature ? s.temperature[at] : s.temperature1;
     const long long k = s.top_k.p ? s.top_k.at(at) : s.top_k1;
     const float top_p = s.top_p ? s.top_p[at] : s.top_p1;
-    const float min_p = fminf(s.min_p ? s.min_p[at] : s.min_p1, 1.f);
+    const float share = s.min_p ? s.min_p[at] : s.min_p1, min_p = fminf(share, 1.f);
     // k entries at least are as large as the m-th largest of the warps' j-th largest of their lanes'
     // maxima, m j >= k; with j from the pieces that are whole there are m warps
     const int pieces = max(1, row.end / row.piece);
@@ -908,7 +908,7 @@ sample_kernel(const __grid_constant__ SampleArgs s)
     row.floor = isinf(row.top) ? FLT_MAX
                                : fminf(below(row.top), __double2float_rd(row.limit - 34.0 * (double)t));
     // nothing to draw from, or nothing to draw
-    const bool none = !(row.top > NEG_INF) || t != t || top_p != top_p;
+    const bool none = !(row.top > NEG_INF) || t != t || top_p != top_p || share != share;
     if (none || t <= 0.f || k == 1 || top_p <= 0.f) {
         int first = EVERY;
         if (!none)

@@ -53,7 +53,7 @@ def sample_tokens_ref(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_
     z, index = torch.sort(logits, dim=1, descending=True, stable=True)
     z = z.double()
     top = z[:, :1]
-    bad = logits.isnan().any(1) | ~(top[:, 0] > -float("inf")) | t[:, 0].isnan() | p[:, 0].isnan()
+    bad = logits.isnan().any(1) | ~(top[:, 0] > -float("inf")) | t[:, 0].isnan() | p[:, 0].isnan() | m[:, 0].isnan()
     greedy = (t <= 0) | (k == 1) | (p <= 0)
     w = torch.where(top.isinf(), (z == top).double(), torch.exp((z - top) / torch.where(greedy, 1.0, t)))
     w = torch.where(z == -float("inf"), 0.0, w)              # (at an infinite temperature too)
@@ -85,10 +85,11 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
 
     uniform (...,) in [0, 1); temperature, top_k, top_p, min_p: one number, or a tensor (...,)
     with one a row. temperature 0 takes the largest logit. logits of -inf are never drawn; a
-    row without any above it, or with a NaN, gives -1. With return_logprob also the log of the
-    token's share of the kept weights (float32, NaN beside -1). logits float32 or bfloat16 on
-    the CUDA kernel, rows may be strided. Weights are float64, in the kernel rounded to whole
-    numbers of 2^-44 of the largest (2^-(62 - log2 V) above 2^18 entries) and summed exactly.
+    row without any above it, or with a NaN among its logits or settings, gives -1. With
+    return_logprob also the log of the token's share of the kept weights (float32, NaN beside -1).
+    logits float32 or bfloat16 on the CUDA kernel, rows may be strided. Weights are float64, in the
+    kernel rounded to whole numbers of 2^-44 of the largest (2^-(62 - log2 V) above 2^18 entries)
+    and summed exactly.
     Not differentiable.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1 or uniform.shape != logits.shape[:-1]:

@@ -24,3 +24,19 @@ def test_the_largest_finite_logit_weighs_nothing_beside_an_infinite_one(device, 
     assert token[:2].tolist() == [0, 3] and (lp[:2] == 0).all()
     want, wlp = sample_tokens_ref(z, u, **kw)
     assert torch.equal(token, want) and torch.allclose(lp, wlp, rtol=2.0 ** -22, atol=vocab * 2.0 ** -45)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5, 5000])
+def test_a_setting_that_is_no_number_draws_nothing(device, dtype, vocab):
+    g = torch.Generator().manual_seed(0)
+    z, u = torch.randn(4, vocab, generator=g).to(dtype).to(device), torch.rand(4, generator=g).to(device)
+    for own in ("temperature", "top_p", "min_p"):
+        for kw in (dict(), dict(top_k=3), dict(top_k=1), dict(top_k=vocab // 2)):
+            values = torch.tensor([0.5, float("nan"), 0.2, 0.9], device=device)
+            token, lp = sample_tokens(z, u, return_logprob=True, **{**kw, own: values})
+            want, wlp = sample_tokens_ref(z, u, **{**kw, own: values})
+            assert token[1] == want[1] == -1 and lp[1].isnan() and wlp[1].isnan(), own
+            keep = [0, 2, 3]
+            assert torch.equal(token[keep], want[keep]) and (token[keep] >= 0).all() and torch.isfinite(lp[keep]).all()
