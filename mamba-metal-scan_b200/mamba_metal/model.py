@@ -260,7 +260,7 @@ class MambaBlock(nn.Module):
         if cache is not None and cache.get("h") is not None and x.shape[1] == 1:
             # one-token recurrent step against the cached conv window and state
             if fuse_conv and not (torch.is_grad_enabled()
-                                  and any(t.requires_grad for t in (x, self.conv.weight, cache["conv"]))):
+                                  and any(t.requires_grad for t in (x, *self.conv.parameters(), cache["conv"]))):
                 if not cache.get("conv_owned"):
                     cache["conv"] = cache["conv"][:, :, :kc - 1].clone(memory_format=torch.contiguous_format)
                     cache["conv_owned"] = True
