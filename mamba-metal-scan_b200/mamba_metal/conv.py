@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from mamba_metal import _native
@@ -31,6 +32,11 @@ def _taps(weight, d: int):
     if weight.dim() != 2 or weight.shape[0] != d or weight.shape[1] < 1:
         raise ValueError(f"weight must be ({d}, taps) or ({d}, 1, taps); got {tuple(weight.shape)}")
     return weight
+
+
+def _tangent(t) -> bool:
+    """Whether t carries a forward-mode derivative (a kernel would drop it; the autograd function refuses)."""
+    return unpack_dual(t).tangent is not None
 
 
 def _wide(x):
@@ -89,7 +95,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None
 
     weight (D, K) or nn.Conv1d's (D, 1, K), bias (D,) or None; y (B, T, D) contiguous. Before a
     sequence's first row stand zeros. All float32 or all bfloat16 on the CUDA kernels
-    (float32 arithmetic, K up to 8). Differentiable once, with respect to every tensor.
+    (float32 arithmetic, K up to 8). Differentiable once, with respect to every tensor, in
+    reverse mode; on the kernels a forward-mode tangent is refused.
     """
     if x.dim() != 3:
         raise ValueError(f"x must be (batch, time, channels); got {tuple(x.shape)}")
@@ -106,8 +113,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None
     weight = weight if weight.is_contiguous() else weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                     or (bias is not None and bias.requires_grad))) \
+            or _tangent(x) or _tangent(weight) or (bias is not None and _tangent(bias)):
         return CausalConvCUDA.apply(x, weight, bias, bool(silu))
     with _native.on_device(x.device):
         return _native.conv_fwd(x, weight, bias, silu)

@@ -3,8 +3,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from mamba_metal import MambaConfig, TinyMamba
+from mamba_metal import MambaConfig, TinyMamba, causal_conv
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +28,21 @@ def test_one_parameter_of_the_convolution_trained_through_a_cached_step(name):
         logits.square().sum().backward()
         grads.append(dict(m.named_parameters())[f"blocks.0.{name}"].grad)
     assert grads[1].abs().max() > 0 and torch.allclose(*grads, rtol=1e-5, atol=1e-6)
+
+
+def test_a_forward_mode_tangent_is_refused():
+    """Whichever tensor carries it, with gradients on or off; without one, within a level, nothing changes."""
+    g = torch.Generator().manual_seed(0)
+    t = dict(x=torch.randn(2, 9, 8, generator=g).cuda(), weight=torch.randn(8, 4, generator=g).cuda(),
+             bias=torch.randn(8, generator=g).cuda())
+    want = causal_conv(**t)
+    with forward_ad.dual_level():
+        assert torch.equal(causal_conv(**t), want)
+        for key, v in t.items():
+            dual = {**t, key: forward_ad.make_dual(v, torch.ones_like(v))}
+            with pytest.raises(NotImplementedError):
+                causal_conv(**dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                causal_conv(**dual)
+            # (the PyTorch form has it)
+            assert forward_ad.unpack_dual(causal_conv(**dual, impl="torch")).tangent is not None
