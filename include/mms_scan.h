@@ -369,6 +369,9 @@ int mms_conv_bwd(const void *x, long long ldb, long long ldt, const void *w, con
  * holds logits and aneg the raw A, as in mms_fwd_proj. aneg, state and the
  * workspace 16-byte aligned; without starts B and C 4 elements aligned, strides
  * too. Workspace: mms_scan_packed_workspace_size() bytes (0 without starts).
+ * Any aneg above 2.3e38, an infinite one too, counts as that: a step of 0 decays nothing. What
+ * is not finite in x, B or a state makes what it enters not finite, infinite or NaN by
+ * where the rows lie.
  *
  * No counterpart in the reference, whose cache goes on by single tokens of one
  * batch (mamba_metal/model.py:203-241).

@@ -36,6 +36,8 @@
 // warps an issue wait for memory, the ALUs are at 49 %).
 #pragma once
 
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -100,6 +102,14 @@ __device__ __forceinline__ bool find_unit(const Args<E> &a, int unit, Unit &u)
     const int s = unit < a.fulls ? Sequences::last_at_most(a.seq.count, unit, [&](int i) { return a.seq.start(i) / a.seg; })
                                  : unit - a.fulls;
     return s >= 0 && unit_rows(unit, a.fulls, a.seg, s, a.seq.start(s), a.seq.start(s + 1), u);
+}
+
+// -Aneg log2(e), kept finite: what is infinite there (an Aneg above 2.3e38) would turn a step of 0, as the
+// rows behind a sequence's last have it in a tile, into a NaN of every state.
+__device__ __forceinline__ float rate_of(float aneg)
+{
+    const float v = -aneg * MMS_LOG2E;
+    return isinf(v) ? copysignf(FLT_MAX, v) : v;           // (a NaN stays one)
 }
 
 // An element of B or C.
@@ -463,7 +473,7 @@ __device__ __forceinline__ void write_states(const States<S> &h, float *p, int N
         }
 }
 
-// -Aneg * log2(e) of the lane's states, 0 where there is none
+// The rates of the lane's states, 0 where there is none
 template <typename S>
 __device__ __forceinline__ void read_rates(States<S> &nan2, const float *aneg, int N, int g, int channels, bool raw)
 {
@@ -474,7 +484,7 @@ __device__ __forceinline__ void read_rates(States<S> &nan2, const float *aneg, i
         for (int q = 0; q < S::NPAIR; ++q) {
             float2 v = nan2[ch][q];
             if (raw) v = f2(softplus(v.x), softplus(v.y));
-            nan2[ch][q] = ch < channels && S::state(g, q) < N ? f2(-v.x * MMS_LOG2E, -v.y * MMS_LOG2E) : f2(0.f, 0.f);
+            nan2[ch][q] = ch < channels && S::state(g, q) < N ? f2(rate_of(v.x), rate_of(v.y)) : f2(0.f, 0.f);
         }
 }
 
@@ -599,7 +609,7 @@ scan_join_kernel(const __grid_constant__ Args<E> a, int blocks, bool by_sequence
     const int d = e / a.N;
     float4 r = ld4(a.aneg + e);
     if (a.pj.on) r = make_float4(softplus(r.x), softplus(r.y), softplus(r.z), softplus(r.w));
-    const float2 n0 = f2(-r.x * MMS_LOG2E, -r.y * MMS_LOG2E), n1 = f2(-r.z * MMS_LOG2E, -r.w * MMS_LOG2E);
+    const float2 n0 = f2(rate_of(r.x), rate_of(r.y)), n1 = f2(rate_of(r.z), rate_of(r.w));
     float *end = a.ends + u.row * DN + e;
     const float *sums = a.sums + (size_t)u.row * a.D + d;
     const float4 first = *reinterpret_cast<const float4 *>(end);
@@ -661,7 +671,7 @@ scan_token_kernel(const __grid_constant__ Args<E> a, int per)
     int from = from_of(s0), from_next = from_of(s0 + 1), to = (int)a.seq.to(s0);
     float4 hv = state_of(from);
     if (a.pj.on) av = make_float4(softplus(av.x), softplus(av.y), softplus(av.z), softplus(av.w));
-    const float2 n0 = f2(-av.x * MMS_LOG2E, -av.y * MMS_LOG2E), n1 = f2(-av.z * MMS_LOG2E, -av.w * MMS_LOG2E);
+    const float2 n0 = f2(rate_of(av.x), rate_of(av.y)), n1 = f2(rate_of(av.z), rate_of(av.w));
     for (int s = s0; s < s1; ++s) {
         float4 Bv = four(Bp + s * a.ldB + ns), Cv = four(Cp + s * a.ldC + ns);
         const float xv = to_f(a.x[s * a.ldx + ds]);
