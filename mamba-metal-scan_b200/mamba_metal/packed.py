@@ -219,11 +219,16 @@ def _nothing_packed(x, cache, count, slots, out_slots):
     if x.shape[0] and cache.shape[0] == 0 and count and x.shape[1]:
         raise ValueError("the cache has no place; give it one, even where every sequence starts from nothing")
     if count and cache.numel() and out_slots is not None:
-        src = slots.long() if slots is not None else torch.arange(count, device=x.device)
         places, lead = cache.shape[0], (-1,) + (1,) * (cache.dim() - 1)
-        old = torch.where(((src >= 0) & (src < places)).view(lead), cache[src.clamp(0, places - 1)],
-                          torch.zeros_like(cache[:1]))
+        order = torch.arange(count, device=x.device)
+        src, dst = order if slots is None else slots.long(), out_slots.long()
+        # every place's sequence, -1 for none (one place more takes those that leave nothing)
+        writer = torch.full((places + 1,), -1, dtype=torch.int64, device=x.device)
+        writer.scatter_(0, torch.where((dst >= 0) & (dst < places), dst, places), order)
+        writer = writer[:places]
         # every place takes what the sequence that names it goes on from; others keep theirs
-        hit = out_slots.long()[:, None] == torch.arange(places, device=x.device)
-        cache.copy_(torch.where(hit.any(0).view(lead), old[hit.int().argmax(0)], cache))
+        src = src[writer.clamp(min=0)]
+        old = cache[src.clamp(0, places - 1)]
+        old = torch.where(((src >= 0) & (src < places)).view(lead), old, torch.zeros_like(old))
+        cache.copy_(torch.where((writer >= 0).view(lead), old, cache))
     return torch.zeros_like(x, memory_format=torch.contiguous_format)
