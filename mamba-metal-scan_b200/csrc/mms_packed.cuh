@@ -57,10 +57,12 @@ constexpr float GONE = -126.f;          // log2 of the decays below, which ex2 f
 constexpr int CTAS = 4;                 // an SM: what the registers hold
 constexpr int DIRECT = 2;               // rows that a segment takes straight from memory
 // A segment's state is chained from the ends of those before it, by each segment for itself or, in calls
-// with MANY more whole segments than sequences, for sequences of more than CHAIN of them by a launch between the
-// two. (16384 x 256 x 16, one prompt, 256 segments: 96 us, without that launch 255; 4096 x 1024 x 16, 4
-// prompts, 73 segments: 76 and 92; 512 x 1432 x 16, one prompt, 16 segments: 43 and 39; 8192 x 2304 x
-// 16, 16 prompts, 32 segments: 224 and 211.)
+// with MANY more whole segments than sequences or 2 MANY of them in all, for sequences of more than CHAIN by a
+// launch between the two. (16384 x 256 x 16, one prompt, 256 segments: 96 us, without that launch 255; 4096 x
+// 1024 x 16, 4 prompts, 73 segments: 76 and 92; 512 x 1432 x 16, one prompt, 16 segments: 43 and 39; 8192 x 2304 x
+// 16, 16 prompts, 32 segments: 224 and 211. Beside as many sequences as segments, whose lengths the host
+// does not know: 16384 x 64 x 16, a prompt and 480 single tokens, 77 and 219; 8192 x 256 x 16, 512 sequences of
+// 16 rows, which have nothing to join, 32 and 24.)
 constexpr int MANY = 32, CHAIN = 4;
 
 template <typename E>
@@ -760,7 +762,7 @@ cudaError_t segments_of(const ScanPackedArgs &p, cudaStream_t stream)
     Args<E> a = args_of<E>(p);
     const Plan plan(p.seq.rows, p.seq.count, p.D, p.N);
     char *ws = static_cast<char *>(p.workspace);
-    const bool joined = plan.fulls >= MANY + p.seq.count;
+    const bool joined = plan.fulls >= 2 * MANY || plan.fulls >= MANY + p.seq.count;
     a.seg = plan.seg, a.nd = (int)plan.nd, a.chain = joined ? CHAIN : 0x7fffffff, a.fulls = (int)plan.fulls, a.units = (int)plan.units;
     a.ends = (float *)ws, a.sums = (float *)(ws + plan.sums), a.entry = (float *)(ws + plan.entry);
     const long long clear = 2 * N_SM, blocks = plan.units * plan.nd;
