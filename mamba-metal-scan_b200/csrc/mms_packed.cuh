@@ -106,12 +106,13 @@ __device__ __forceinline__ bool find_unit(const Args<E> &a, int unit, Unit &u)
     return s >= 0 && unit_rows(unit, a.fulls, a.seg, s, a.seq.start(s), a.seq.start(s + 1), u);
 }
 
-// -Aneg log2(e), kept finite: what is infinite there (an Aneg above 2.3e38) would turn a step of 0, as the
-// rows behind a sequence's last have it in a tile, into a NaN of every state.
+// -Aneg log2(e), -FLT_MAX at least: what is -inf there (an Aneg above 2.3e38) would turn a step of 0, as the
+// rows behind a sequence's last have it in a tile, into a NaN of every state. A NaN stays one.
 __device__ __forceinline__ float rate_of(float aneg)
 {
-    const float v = -aneg * MMS_LOG2E;
-    return isinf(v) ? copysignf(FLT_MAX, v) : v;           // (a NaN stays one)
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(-aneg * MMS_LOG2E), "f"(-FLT_MAX));
+    return v;
 }
 
 // An element of B or C.

@@ -120,8 +120,7 @@ def selective_scan_packed_ref(x, dt, aneg, b_in, c_in, state, starts=None, slots
     xf, dtf, bf, cf, af = (t.to(wide) for t in (x, dt, b_in, c_in, aneg))
     if dt_range is not None:
         dtf, af = proj_ref(dtf, af, *dt_range)
-    most = torch.finfo(torch.float32).max
-    af = torch.where(af.isinf(), af.clamp(-most, most), af)
+    af = af.masked_fill(af == float("inf"), torch.finfo(torch.float32).max)
     y = torch.zeros_like(xf)
     left = []
     for first, end, src, dst in places_of(x.shape[0], starts, slots, out_slots, state.shape[0]):
@@ -154,8 +153,8 @@ def selective_scan_packed(x: torch.Tensor, dt: torch.Tensor, aneg: torch.Tensor,
     Aneg (D, N) and d_skip (D,) (used as float32), state (places, D, N) float32, contiguous;
     the lists as in the module docstring. z and d_skip are optional (the block's gate, see
     `gated_output`). dt_range = (dt_min, dt_max): dt holds logits and aneg the raw A, as in
-    `selective_scan_proj`. Rows may be strided views. N is a multiple of 4 up to 64. An infinite Aneg
-    counts as the largest finite one (and any above 2.3e38 as that): a step of 0 decays nothing. An x, B
+    `selective_scan_proj`. Rows may be strided views. N is a multiple of 4 up to 64. Any Aneg
+    above 2.3e38, an infinite one too, counts as that: a step of 0 decays nothing. An x, B
     or state that is not finite makes the states that it enters, and their outputs from there on, not finite,
     but whether infinite or NaN depends on where the sequence's rows lie.
     Arithmetic and state are float32. Not differentiable: it is the inference path
