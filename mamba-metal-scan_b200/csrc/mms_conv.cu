@@ -5,8 +5,10 @@
 //     ds = dy * act'(pre),   dx[t] = sum_k w[k] ds[t + K - 1 - k],
 //     dw[k] = sum_t ds[t] x[t - K + 1 + k],   dbias = sum_t ds[t]
 //
-// All of it is bound by HBM: a few FMAs an element beside x and y (forward, 2
-// elements moved), x, dy and dx (backward, 3). The reference transposes to
+// A few FMAs an element beside x and y (forward, 2 elements moved), x, dy and dx (backward, 3), and with
+// SiLU two MUFU operations. Of 4 x 4096 x 8192 (floor at HBM's rate in brackets): float32 is bound by HBM,
+// forward 172 us (167), backward 266 (250); bf16 not, forward 94 (83): MUFU at 68 %, backward 172 (125):
+// instructions, the FMA pipe at 52 % with the three CTAs an SM that 168 registers leave. The reference transposes to
 // channels first, calls a convolution and a SiLU and transposes back (reference
 // mamba_metal/model.py:175-177, 214-219); here rows stay as they are in memory,
 // channels innermost: a thread owns VEC neighbouring channels, a warp 32 * VEC,
@@ -25,7 +27,10 @@ namespace {
 
 constexpr int WARPS = 4;                // per CTA, each with rows of its own and the same channels
 constexpr int THREADS = 32 * WARPS;
-constexpr int TAIL_ROWS = 32;           // rows of packed sequences a warp walks
+// Rows of packed sequences a warp walks. (With 16, 32 and 64, us: 37 prompts, 8192 x 2304, float32 33.6, 31.4, 31.1,
+// bf16 28.8, 26.3, 26.8, 1319 CTAs of 32 rows where 740 run at a time; 9 prompts, 2048 x 1432, float32 8.2, 10.4, 15.7;
+// 37 prompts, 32768 x 2304, float32 112, 104, 107.)
+constexpr int TAIL_ROWS = 32;
 // Rows that a warp loads at once, and computes while the next are on their way: 64 bytes a lane and
 // array. (Backward with half of them at 4 CTAs an SM: 201 us of 4 x 4096 x 8192 in bf16, so 174;
 // a quarter, 228; a forward that loads a tile and then computes it, 177, so 91.)
@@ -478,8 +483,12 @@ bool groups_of_4(int D, std::initializer_list<const void *> arrays, std::initial
     return ok;
 }
 
-// Rows a warp walks: as many as leave 8 CTAs an SM, so that the halo of K - 1 rows and the
-// backward's partial sums stay small beside them; at least 16, at most 128.
+// Rows a warp walks: as many as make 8 CTAs an SM, so that the halo of K - 1 rows and the
+// backward's partial sums stay small beside them; at least 16, at most 128. Of those 8 the registers let 6 run at a
+// time forward (80 of 4 taps) and 3 backward (168), so that 16 x 512 x 1432, 24 rows a warp, is 1.2 and 2.4
+// waves. (Aiming at 4, 6, 8 and 16, us, forward and backward with its sums: that size in float32 18.7, 17.0, 19.8,
+// 19.4 and 40.2, 34.4, 38.6, 39.8, in bf16 13.9, 13.9, 14.3, 14.3 and 30.5, 30.4, 34.3, 38.1; 4 x 4096 x 8192,
+// bf16, 128 rows up to 8 and 112 at 16: 94 to 91 and 172, at 16 176; 2 x 2048 x 1024, 16 rows for all, 7.7 and 18.1.)
 int rows_of_warp(int Bt, int T, int D)
 {
     const long long nd = (D + 127) / 128;                  // (the same for one channel a thread: the sums' layout)
